@@ -76,6 +76,9 @@ typedef enum tg_aggregator { TG_AGG_MEAN = 0, TG_AGG_MAX = 1 } tg_aggregator;
  *                 transform-first when F_in > F_out, split long rows). */
 typedef enum tg_mode { TG_MODE_EXACT = 0, TG_MODE_FAST = 1 } tg_mode;
 
+/* Element types of the training operators' matrices. */
+typedef enum tg_dtype { TG_F32 = 0, TG_BF16 = 1, TG_F16 = 2 } tg_dtype;
+
 /* OR'ed into a gather entry point's `mode`: every row of the gathered
  * operand is readable up to its leading dimension (the buffer holds
  * rows * ld floats), so rows whose width is not a multiple of 4 can still be
@@ -176,6 +179,90 @@ TG_API tg_status tg_log_softmax_rows_f32(float* X, int64_t rows, int64_t cols, i
 /* X[i][j] += bias[j]  (src/ops.cpp:622-661). */
 TG_API tg_status tg_add_bias_f32(float* X, int64_t rows, int64_t cols, int64_t ld,
                                  const float* bias, void* stream);
+
+/* ── training operators ──────────────────────────────────────────────────── */
+/* Layer norm, typed linear maps and 8-bit saved activations, forward and
+ * backward.  No counterpart in the reference, which runs forward only.
+ * Matrices are fp32, bf16 or fp16 (`dtype`, a tg_dtype), row-major with any
+ * leading dimension and any alignment of their type; sums, statistics and
+ * norms are fp32 and every result is rounded once.  `act` is a tg_activation.
+ *
+ * Saved form.  A rows x cols matrix saved in 8 bits is `codes` (signed
+ * bytes, rows 16-byte aligned: ld_codes % 16 == 0) and `exponents` (one byte
+ * per row and block of 128 columns): value = code * 2^(exponent - 127), with
+ * the least exponent whose 127 * 2^e reaches the block's largest magnitude
+ * (not below 2^-126, for fp16 matrices 2^-24) and codes rounded to nearest
+ * even (at most 63 where 64 * 2^e would overflow the matrix's type), so that
+ * fp32, bf16 and the matrix's own type hold every value.  Exponent 255 marks a block that held an infinity or a NaN: all its
+ * values are NaN. */
+
+/* y = act(x) (y nullable: only save), and x in the saved form. */
+TG_API tg_status tg_save8(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ldx,
+                          int32_t act, float alpha, void* y, int64_t ldy, int8_t* codes,
+                          int64_t ld_codes, uint8_t* exponents, int64_t ld_exponents, void* stream);
+/* y = the values of a saved matrix, of type `dtype`. */
+TG_API tg_status tg_restore8(int64_t rows, int64_t cols, const int8_t* codes, int64_t ld_codes,
+                             const uint8_t* exponents, int64_t ld_exponents, int32_t dtype, void* y,
+                             int64_t ldy, void* stream);
+/* dx = dy * act'(x), x given as it was (x) or in the saved form (codes and
+ * exponents); exactly one of the two. */
+TG_API tg_status tg_activation_grad(int64_t rows, int64_t cols, int32_t dtype, const void* dy,
+                                    int64_t lddy, const void* x, int64_t ldx, const int8_t* codes,
+                                    int64_t ld_codes, const uint8_t* exponents, int64_t ld_exponents,
+                                    int32_t act, float alpha, void* dx, int64_t lddx, void* stream);
+
+/* y = h * gamma + beta with h = (x - mean) * rstd over the columns of each
+ * row, rstd = 1 / sqrt(mean (x - mean)^2 + eps).  gamma and beta are fp32 or
+ * of the rows' type (param_dtype).  stats[2 i], stats[2 i + 1] receive row
+ * i's mean and rstd; codes and exponents (nullable) receive h in the saved
+ * form. */
+TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ldx,
+                               int32_t param_dtype, const void* gamma, const void* beta, float eps,
+                               void* y, int64_t ldy, float* stats, int8_t* codes, int64_t ld_codes,
+                               uint8_t* exponents, int64_t ld_exponents, void* stream);
+/* The backward pass from the forward pass's stats and either x or the saved
+ * h (codes and exponents): dx, and dgamma and dbeta (param_dtype), which are
+ * summed in a fixed order (the same bits every run).  With no rows dgamma and
+ * dbeta are zero. */
+TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, const void* dy,
+                                    int64_t lddy, const void* x, int64_t ldx, const int8_t* codes,
+                                    int64_t ld_codes, const uint8_t* exponents, int64_t ld_exponents,
+                                    const float* stats, int32_t param_dtype, const void* gamma,
+                                    void* dx, int64_t lddx, void* dgamma, void* dbeta, void* stream);
+
+/* Y[r] = act(X[r] . W[t] + bias[t]) for the rows r of each type t, rows
+ * [offsets[t], offsets[t + 1]) of X (rows x K).  W[t] is K x N at
+ * W + t * stride_w (rows ldw apart); bias (nullable) is types x N, fp32.
+ * offsets: types + 1 device integers, non-decreasing from 0 to rows (checked
+ * by tg_typed_check_offsets, not here: a bound outside [0, rows] is clamped,
+ * and rows of no type are not written).  codes and exponents (nullable)
+ * receive the pre-activation in the saved form.  At most 1024 types. */
+TG_API tg_status tg_typed_linear(int64_t rows, int64_t K, int64_t N, int64_t types, int32_t dtype,
+                                 const void* X, int64_t ldx, const void* W, int64_t ldw,
+                                 int64_t stride_w, const int32_t* offsets, const float* bias,
+                                 int32_t act, float alpha, void* Y, int64_t ldy, int8_t* codes,
+                                 int64_t ld_codes, uint8_t* exponents, int64_t ld_exponents,
+                                 void* stream);
+/* dX[r] = dY[r] . W[t]^T. */
+TG_API tg_status tg_typed_linear_grad_input(int64_t rows, int64_t K, int64_t N, int64_t types,
+                                            int32_t dtype, const void* dY, int64_t lddy, const void* W,
+                                            int64_t ldw, int64_t stride_w, const int32_t* offsets,
+                                            void* dX, int64_t lddx, void* stream);
+/* dW[t] = sum over its rows of X[r]^T dY[r] (fp32 or the rows' type:
+ * dw_dtype) and db[t] = sum of dY[r] (fp32, types x N, nullable); zero for a
+ * type without rows.  X is given as it was (X) or in the saved form. */
+TG_API tg_status tg_typed_linear_grad_weight(int64_t rows, int64_t K, int64_t N, int64_t types,
+                                             int32_t dtype, const void* X, int64_t ldx,
+                                             const int8_t* codes, int64_t ld_codes,
+                                             const uint8_t* exponents, int64_t ld_exponents,
+                                             const void* dY, int64_t lddy, const int32_t* offsets,
+                                             int32_t dw_dtype, void* dW, int64_t lddw,
+                                             int64_t stride_dw, float* db, void* stream);
+/* Checks that `offsets` (types + 1 device integers) start at 0, never
+ * decrease and end at rows: TG_ERR_INVALID_ARGUMENT otherwise.  Synchronises
+ * `stream`. */
+TG_API tg_status tg_typed_check_offsets(int64_t rows, int64_t types, const int32_t* offsets,
+                                        void* stream);
 
 /* ── sparse ops ──────────────────────────────────────────────────────────── */
 

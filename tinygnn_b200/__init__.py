@@ -3,7 +3,7 @@
 The compute path is libtinygnn_b200.so (hand-written sm_100a CUDA kernels
 behind the C ABI in include/tinygnn_b200.h).  This package is its Python
 host side: ctypes bindings (``_lib``), torch-tensor front ends of every
-entry point (``ops``), seeded synthetic inputs (``synth``) and the
+entry point (``ops``; training operators: ``training``), seeded synthetic inputs (``synth``) and the
 row-partitioned multi-GPU driver (``dist``).  Importing it without the
 built library raises: there is no CPU fallback.
 """
@@ -13,6 +13,9 @@ from .ops import (CSR, add_bias_, add_self_loops, csr_validate, degree_order, ed
                   edge_softmax, elu_, gat_layer, gcn_layer, gcn_norm, gelu_, leaky_relu_, log_softmax_,
                   matmul, relu_, sage_aggregate, sage_layer, sage_max_aggregate, sigmoid_, softmax_,
                   spmm, tanh_)
+from .training import (Saved8, activation_backward, activation_save8, check_row_offsets, layer_norm,
+                       layer_norm_backward, save8, typed_linear, typed_linear_backward,
+                       typed_linear_grad_input, typed_linear_grad_weight)
 
 __version__ = "0.1.0"
 

@@ -24,6 +24,8 @@ OK, INVALID_ARGUMENT, OUT_OF_RANGE, RUNTIME, CUDA, NCCL, TIMEOUT, DEVICE_CHECK, 
 # activations (tg_activation)
 ACT_NONE, ACT_RELU, ACT_ELU, ACT_LEAKY_RELU, ACT_SIGMOID, ACT_TANH, ACT_GELU = range(7)
 AGG_MEAN, AGG_MAX = 0, 1
+# element types of the training operators (tg_dtype)
+F32, BF16, F16 = range(3)
 MODE_EXACT, MODE_FAST = 0, 1
 
 # name -> (restype, argtypes); the exact list of entry points in the header.
@@ -95,6 +97,18 @@ SIGNATURES = {
     "tg_sage_layer_f32": (i32, [i64, i64, vp, vp, vp, i64, i64, i64, vp, vp, vp, i32, i32, vp, i64, vp, i32, vp]),
     "tg_gat_layer_f32": (i32, [i64, i64, vp, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, f32, i32, i32, vp, i64,
                                vp, i32, vp]),
+    "tg_save8": (i32, [i64, i64, i32, vp, i64, i32, f32, vp, i64, vp, i64, vp, i64, vp]),
+    "tg_restore8": (i32, [i64, i64, vp, i64, vp, i64, i32, vp, i64, vp]),
+    "tg_activation_grad": (i32, [i64, i64, i32, vp, i64, vp, i64, vp, i64, vp, i64, i32, f32, vp, i64, vp]),
+    "tg_layer_norm": (i32, [i64, i64, i32, vp, i64, i32, vp, vp, f32, vp, i64, vp, vp, i64, vp, i64, vp]),
+    "tg_layer_norm_grad": (i32, [i64, i64, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, i32, vp, vp, i64, vp, vp,
+                                 vp]),
+    "tg_typed_linear": (i32, [i64, i64, i64, i64, i32, vp, i64, vp, i64, i64, vp, vp, i32, f32, vp, i64, vp, i64, vp,
+                              i64, vp]),
+    "tg_typed_linear_grad_input": (i32, [i64, i64, i64, i64, i32, vp, i64, vp, i64, i64, vp, vp, i64, vp]),
+    "tg_typed_linear_grad_weight": (i32, [i64, i64, i64, i64, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, i32, vp,
+                                          i64, i64, vp, vp]),
+    "tg_typed_check_offsets": (i32, [i64, i64, vp, vp]),
     "tg_take_device_error": (i32, [vp]),
     "tg_ipc_get_handle": (i32, [vp, vp, P64]),
     "tg_ipc_open_handle": (i32, [vp, C.POINTER(vp)]),

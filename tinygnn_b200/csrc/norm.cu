@@ -1,0 +1,554 @@
+// ============================================================================
+//  norm.cu -- layer norm over the columns of each row, and its backward pass.
+//
+//      mu = mean x,  r = 1 / sqrt(mean (x - mu)^2 + eps),  h = (x - mu) r
+//      y  = h gamma + beta
+//      dx = r (g - mean g - h mean(g h)),  g = gamma dy
+//      dgamma = sum over rows of dy h,  dbeta = sum over rows of dy
+//
+//  The forward pass keeps (mu, r) of each row in fp32 and, if asked, h in 8
+//  bits (values.cuh); the backward pass takes x or that copy.  Both read each
+//  operand once and write each result once: a row stays in the registers of
+//  the TPR threads that share it (4 threads for 32 columns up to 512 threads
+//  for 8192), so the variance is a second pass over registers, not memory.
+//  The bound is HBM.  Rows wider than 8192 columns are walked three times by
+//  one block each (the second and third walk come from L2).
+//
+//  dgamma and dbeta are sums over all rows: each thread adds up its columns
+//  over the rows it walks, a block joins its row groups through shared memory
+//  and writes one partial row, and a second kernel adds the blocks' partial
+//  rows in a fixed order -- no atomics, the same bits every run.
+// ============================================================================
+#include <algorithm>
+
+#include "values.cuh"
+
+namespace tg {
+
+namespace {
+
+struct NormArgs {
+    int64_t rows, cols;
+    float eps;
+    Range8 r8;
+};
+
+// The part of a row that one of TPR threads holds: N slots of V values.
+// Aligned rows: a slot is 16 contiguous bytes.  Others: 4 values, one column
+// per lane, W (= lanes of the row within a warp) columns apart.  Either way a
+// block of 128 columns lies in one slot of 128 / V neighbouring lanes, so its
+// largest magnitude is a shuffle reduction (ROW_IS_BLOCK: the TPR lanes of a
+// row of at most 128 columns, and all their slots).
+template <class T, bool ALIGNED, int TPR, int VPT>
+struct RowPart {
+    static constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
+    static constexpr int N = VPT / V;
+    static constexpr int W = TPR < 32 ? TPR : 32;
+    static constexpr bool ROW_IS_BLOCK = TPR * V < kBlock8;
+    static constexpr int G = ROW_IS_BLOCK ? TPR : kBlock8 / V;
+    static_assert(!ROW_IS_BLOCK || TPR * VPT <= kBlock8, "a row of several slots within a block");
+    static __device__ __forceinline__ int64_t col(int t, int i, int j) {
+        return ALIGNED ? (static_cast<int64_t>(i) * TPR + t) * V + j
+                       : ((static_cast<int64_t>(i) * (TPR / W) + t / W) * V + j) * W + t % W;
+    }
+    template <class P>
+    static __device__ __forceinline__ void load(const P* p, int t, int i, int64_t cols, float (&x)[V]) {
+        // P's slot is a vector load where P's elements are as wide as T's (aligned alike)
+        if (ALIGNED && sizeof(P) == sizeof(T) && col(t, i, 0) + V <= cols) {
+            load_v<P, V>(p + col(t, i, 0), x);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = col(t, i, j) < cols ? to_f32(p[col(t, i, j)]) : 0.0f;
+    }
+    static __device__ __forceinline__ void store(T* p, int t, int i, int64_t cols, const float (&x)[V]) {
+        if (ALIGNED && col(t, i, 0) + V <= cols) {
+            store_v<T, V>(p + col(t, i, 0), x);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (col(t, i, j) < cols) p[col(t, i, j)] = from_f32<T>(x[j]);
+    }
+};
+
+// Sums a and b over the TPR threads of a row; every thread gets them.
+// `red`: 2 floats per warp of the block (TPR > 32 only, where a row is the block).
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
+    a = reduce_sum<float, (TPR < 32 ? TPR : 32)>(a);
+    b = reduce_sum<float, (TPR < 32 ? TPR : 32)>(b);
+    if (TPR <= 32) return;
+    constexpr int NW = TPR > 32 ? TPR / 32 : 1;
+    __syncthreads();  // the previous sum has been read
+    if (threadIdx.x % 32 == 0) {
+        red[threadIdx.x / 32 * 2] = a;
+        red[threadIdx.x / 32 * 2 + 1] = b;
+    }
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        a += red[2 * w];
+        b += red[2 * w + 1];
+    }
+}
+
+template <int TPR>
+constexpr int block_threads() { return TPR < 128 ? 128 : TPR; }
+
+template <class T, class P, bool ALIGNED, int TPR, int VPT>
+__global__ void __launch_bounds__(block_threads<TPR>()) norm_kernel(NormArgs a, const T* x, int64_t ldx, const P* gamma,
+                                                                    const P* beta, T* y, int64_t ldy, float2* stats,
+                                                                    Saved8 s) {
+    using R = RowPart<T, ALIGNED, TPR, VPT>;
+    __shared__ float red[32];
+    constexpr int RPB = block_threads<TPR>() / TPR;
+    const int t = threadIdx.x % TPR;
+    const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPB; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * RPB) {
+        const int64_t row = row0 + threadIdx.x / TPR;
+        const bool live = row < a.rows;
+        const int64_t cols = live ? a.cols : 0;  // every thread takes part in the reductions
+        const T* xr = x + (live ? row * ldx : 0);
+        float v[R::N][R::V];
+        float sum = 0.0f, none = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) {
+            R::load(xr, t, i, cols, v[i]);
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) sum += v[i][j];
+        }
+        row_sum2<TPR>(sum, none, red);
+        const float mean = __fmul_rn(sum, inv_n);
+        float sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R::N; ++i)
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) {
+                v[i][j] = R::col(t, i, j) < cols ? __fsub_rn(v[i][j], mean) : 0.0f;
+                sq = fmaf(v[i][j], v[i][j], sq);
+            }
+        row_sum2<TPR>(sq, none, red);
+        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(sq, inv_n, a.eps)));
+        if (live && t == 0) stats[row] = make_float2(mean, rstd);
+        uint32_t row_max = 0;
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) {
+            map_v(v[i], [rstd](float u) { return __fmul_rn(u, rstd); });
+            if (R::ROW_IS_BLOCK) {
+#pragma unroll
+                for (int j = 0; j < R::V; ++j) row_max = max(row_max, mag_bits(v[i][j]));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) {
+            if (s.codes) {
+                uint32_t m = row_max;
+                if (!R::ROW_IS_BLOCK) {
+#pragma unroll
+                    for (int j = 0; j < R::V; ++j) m = max(m, mag_bits(v[i][j]));
+                }
+                const int byte = exponent8(reduce_max<R::G>(m), a.r8.emin);
+                const float inv = encode8(byte);
+                if (ALIGNED && R::col(t, i, 0) + R::V <= cols) {
+                    Pack<int8_t, R::V> k;
+#pragma unroll
+                    for (int j = 0; j < R::V; ++j) k.v[j] = code8(v[i][j], inv, byte, a.r8.top);
+                    *reinterpret_cast<Pack<int8_t, R::V>*>(s.codes + row * s.ld + R::col(t, i, 0)) = k;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < R::V; ++j)
+                        if (R::col(t, i, j) < cols) s.codes[row * s.ld + R::col(t, i, j)] = code8(v[i][j], inv, byte, a.r8.top);
+                }
+                // the first lane of the group that holds the block writes its exponent
+                if (t % R::G == 0 && (i == 0 || !R::ROW_IS_BLOCK) && R::col(t, i, 0) < cols)
+                    s.exps[row * s.lde + R::col(t, i, 0) / kBlock8] = static_cast<uint8_t>(byte);
+            }
+            float g[R::V], b[R::V];
+            R::load(gamma, t, i, cols, g);
+            R::load(beta, t, i, cols, b);
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) g[j] = fmaf(v[i][j], g[j], b[j]);
+            if (live) R::store(y + row * ldy, t, i, cols, g);
+        }
+    }
+}
+
+// dx, and this block's partial sums of dgamma and dbeta: part[block][2][cols].
+template <class T, class P, bool ALIGNED, int TPR, int VPT, bool SAVED>
+__global__ void __launch_bounds__(block_threads<TPR>()) norm_grad_kernel(NormArgs a, const T* dy, int64_t lddy,
+                                                                         const T* x, int64_t ldx, Saved8 s,
+                                                                         const float2* stats, const P* gamma, T* dx,
+                                                                         int64_t lddx, float* part) {
+    using R = RowPart<T, ALIGNED, TPR, VPT>;
+    constexpr int RPB = block_threads<TPR>() / TPR;
+    __shared__ float red[32];
+    __shared__ float join[RPB > 1 ? RPB * TPR * VPT : 1];
+    const int t = threadIdx.x % TPR;
+    const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
+    float ag[R::N][R::V], ab[R::N][R::V];
+#pragma unroll
+    for (int i = 0; i < R::N; ++i)
+#pragma unroll
+        for (int j = 0; j < R::V; ++j) ag[i][j] = ab[i][j] = 0.0f;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPB; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * RPB) {
+        const int64_t row = row0 + threadIdx.x / TPR;
+        const bool live = row < a.rows;
+        const int64_t cols = live ? a.cols : 0;
+        const int64_t r0 = live ? row : 0;
+        const float2 st = stats[r0];
+        float h[R::N][R::V], g[R::N][R::V];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) {
+            R::load(dy + r0 * lddy, t, i, cols, g[i]);
+            if (SAVED) {
+                const int64_t c = R::col(t, i, 0);
+                const float scale = c < cols ? decode8(s.exps[r0 * s.lde + c / kBlock8]) : 0.0f;
+                if (ALIGNED && c + R::V <= cols) {
+                    const Pack<int8_t, R::V> k = *reinterpret_cast<const Pack<int8_t, R::V>*>(s.codes + r0 * s.ld + c);
+#pragma unroll
+                    for (int j = 0; j < R::V; ++j) h[i][j] = __fmul_rn(static_cast<float>(k.v[j]), scale);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < R::V; ++j)
+                        h[i][j] = R::col(t, i, j) < cols
+                                      ? __fmul_rn(static_cast<float>(s.codes[r0 * s.ld + R::col(t, i, j)]), scale)
+                                      : 0.0f;
+                }
+            } else {
+                R::load(x + r0 * ldx, t, i, cols, h[i]);
+#pragma unroll
+                for (int j = 0; j < R::V; ++j)
+                    h[i][j] = R::col(t, i, j) < cols ? __fmul_rn(__fsub_rn(h[i][j], st.x), st.y) : 0.0f;
+            }
+            float w[R::V];
+            R::load(gamma, t, i, a.cols, w);
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) {
+                ag[i][j] = fmaf(g[i][j], h[i][j], ag[i][j]);
+                ab[i][j] += g[i][j];
+                g[i][j] = __fmul_rn(g[i][j], w[j]);
+                s1 += g[i][j];
+                s2 = fmaf(g[i][j], h[i][j], s2);
+            }
+        }
+        row_sum2<TPR>(s1, s2, red);
+        const float m1 = __fmul_rn(s1, inv_n), m2 = __fmul_rn(s2, inv_n);
+#pragma unroll
+        for (int i = 0; i < R::N; ++i) {
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) g[i][j] = __fmul_rn(st.y, fmaf(-h[i][j], m2, __fsub_rn(g[i][j], m1)));
+            if (live) R::store(dx + row * lddx, t, i, cols, g[i]);
+        }
+    }
+    float* out = part + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+    if constexpr (RPB == 1) {
+#pragma unroll
+        for (int i = 0; i < R::N; ++i)
+#pragma unroll
+            for (int j = 0; j < R::V; ++j)
+                if (R::col(t, i, j) < a.cols) {
+                    out[R::col(t, i, j)] = ag[i][j];
+                    out[a.cols + R::col(t, i, j)] = ab[i][j];
+                }
+    } else {
+        // The block's row groups, joined through shared memory: slot k of
+        // thread t of group q at (q * VPT + k) * TPR + t.
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < R::N; ++i)
+#pragma unroll
+                for (int j = 0; j < R::V; ++j)
+                    join[(threadIdx.x / TPR * VPT + i * R::V + j) * TPR + t] = half ? ab[i][j] : ag[i][j];
+            __syncthreads();
+            for (int q = threadIdx.x; q < TPR * VPT; q += block_threads<TPR>()) {
+                float sum = 0.0f;
+#pragma unroll 4
+                for (int r = 0; r < RPB; ++r) sum += join[r * VPT * TPR + q];
+                const int64_t c = R::col(q % TPR, q / TPR / R::V, q / TPR % R::V);
+                if (c < a.cols) out[half * a.cols + c] = sum;
+            }
+        }
+    }
+}
+
+// Rows wider than the register forms hold: one block walks a row.
+template <class T, class P>
+__global__ void __launch_bounds__(512) norm_wide_kernel(NormArgs a, const T* x, int64_t ldx, const P* gamma,
+                                                        const P* beta, T* y, int64_t ldy, float2* stats, Saved8 s) {
+    __shared__ float red[32];
+    const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* xr = x + row * ldx;
+        float sum = 0.0f, none = 0.0f;
+        for (int64_t c = threadIdx.x; c < a.cols; c += 512) sum += to_f32(xr[c]);
+        row_sum2<512>(sum, none, red);
+        const float mean = __fmul_rn(sum, inv_n);
+        float sq = 0.0f;
+        for (int64_t c = threadIdx.x; c < a.cols; c += 512) {
+            const float d = __fsub_rn(to_f32(xr[c]), mean);
+            sq = fmaf(d, d, sq);
+        }
+        row_sum2<512>(sq, none, red);
+        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(sq, inv_n, a.eps)));
+        if (threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
+        // one warp per block of 128 columns
+        for (int64_t b = warp; b * kBlock8 < a.cols; b += 16) {
+            float h[4];
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t c = b * kBlock8 + j * 32 + lane;
+                h[j] = c < a.cols ? __fmul_rn(__fsub_rn(to_f32(xr[c]), mean), rstd) : 0.0f;
+                m = max(m, mag_bits(h[j]));
+                if (c < a.cols) y[row * ldy + c] = from_f32<T>(fmaf(h[j], to_f32(gamma[c]), to_f32(beta[c])));
+            }
+            if (s.codes) {
+                const int byte = exponent8(reduce_max<32>(m), a.r8.emin);
+                const float inv = encode8(byte);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t c = b * kBlock8 + j * 32 + lane;
+                    if (c < a.cols) s.codes[row * s.ld + c] = code8(h[j], inv, byte, a.r8.top);
+                }
+                if (lane == 0) s.exps[row * s.lde + b] = static_cast<uint8_t>(byte);
+            }
+        }
+    }
+}
+
+template <class T, bool SAVED>
+__device__ __forceinline__ float wide_h(const T* x, int64_t ldx, const Saved8& s, float2 st, int64_t row, int64_t c) {
+    if (SAVED)
+        return __fmul_rn(static_cast<float>(s.codes[row * s.ld + c]), decode8(s.exps[row * s.lde + c / kBlock8]));
+    return __fmul_rn(__fsub_rn(to_f32(x[row * ldx + c]), st.x), st.y);
+}
+
+template <class T, class P, bool SAVED>
+__global__ void __launch_bounds__(512) norm_wide_grad_kernel(NormArgs a, const T* dy, int64_t lddy, const T* x,
+                                                             int64_t ldx, Saved8 s, const float2* stats, const P* gamma,
+                                                             T* dx, int64_t lddx) {
+    __shared__ float red[32];
+    const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float2 st = stats[row];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int64_t c = threadIdx.x; c < a.cols; c += 512) {
+            const float g = __fmul_rn(to_f32(dy[row * lddy + c]), to_f32(gamma[c]));
+            s1 += g;
+            s2 = fmaf(g, wide_h<T, SAVED>(x, ldx, s, st, row, c), s2);
+        }
+        row_sum2<512>(s1, s2, red);
+        const float m1 = __fmul_rn(s1, inv_n), m2 = __fmul_rn(s2, inv_n);
+        for (int64_t c = threadIdx.x; c < a.cols; c += 512) {
+            const float g = __fmul_rn(to_f32(dy[row * lddy + c]), to_f32(gamma[c]));
+            const float h = wide_h<T, SAVED>(x, ldx, s, st, row, c);
+            dx[row * lddx + c] = from_f32<T>(__fmul_rn(st.y, fmaf(-h, m2, __fsub_rn(g, m1))));
+        }
+    }
+}
+
+// Partial sums of dgamma and dbeta for wide rows: a thread per column, the
+// rows split over blockIdx.y.
+template <class T, bool SAVED>
+__global__ void __launch_bounds__(256) norm_wide_sums_kernel(NormArgs a, const T* dy, int64_t lddy, const T* x,
+                                                             int64_t ldx, Saved8 s, const float2* stats, float* part) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= a.cols) return;
+    float sg = 0.0f, sb = 0.0f;
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const float g = to_f32(dy[row * lddy + c]);
+        sg = fmaf(g, wide_h<T, SAVED>(x, ldx, s, stats[row], row, c), sg);
+        sb += g;
+    }
+    float* out = part + static_cast<int64_t>(blockIdx.y) * 2 * a.cols;
+    out[c] = sg;
+    out[a.cols + c] = sb;
+}
+
+// dgamma / dbeta = the sum of `parts` partial rows [2][cols], in their order
+// within each of 8 interleaved chains joined in order.
+template <class P>
+__global__ void __launch_bounds__(256) norm_join_kernel(const float* part, int parts, int64_t cols, P* dgamma, P* dbeta) {
+    __shared__ float sh[8][33];
+    const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // of 2 * cols
+    float sum = 0.0f;
+    if (c < 2 * cols) {
+#pragma unroll 8
+        for (int p = w; p < parts; p += 8) sum += part[static_cast<int64_t>(p) * 2 * cols + c];
+    }
+    sh[w][lane] = sum;
+    __syncthreads();
+    if (w == 0 && c < 2 * cols) {
+        sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sum += sh[q][lane];
+        if (c < cols) dgamma[c] = from_f32<P>(sum);
+        else dbeta[c - cols] = from_f32<P>(sum);
+    }
+}
+
+constexpr int64_t kRegisterCols = 8192;
+
+// Calls f(TPR, VPT) with the row split for `cols` columns.
+template <class F>
+void by_width(int64_t cols, F&& f) {
+    using std::integral_constant;
+    if (cols <= 32) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    else if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (cols <= 1024) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (cols <= 4096) f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
+    else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+}
+
+// gamma and beta are fp32 or of the rows' own type.
+template <class F>
+void by_types(int dtype, int param_dtype, F&& f) {
+    by_dtype(dtype, [&](auto t) {
+        if (param_dtype == TG_F32) f(t, float{});
+        else f(t, t);
+    });
+}
+
+void check_norm(const char* fn, int64_t rows, int64_t cols, int dtype, int param_dtype) {
+    check_rows_cols(fn, rows, cols);
+    check_dtype(fn, "x", dtype);
+    if (param_dtype != TG_F32 && param_dtype != dtype)
+        invalid(std::string(fn) + ": gamma and beta must be float32 or of the rows' type");
+}
+
+void check_stats(const char* fn, const float* stats) {
+    if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) invalid(std::string(fn) + ": stats must be 8-byte aligned");
+}
+
+}  // namespace
+
+}  // namespace tg
+
+extern "C" {
+
+TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ldx,
+                               int32_t param_dtype, const void* gamma, const void* beta, float eps, void* y,
+                               int64_t ldy, float* stats, int8_t* codes, int64_t ld_codes, uint8_t* exponents,
+                               int64_t ld_exponents, void* stream) {
+    return tg::guard([&] {
+        tg::require_device();
+        using namespace tg;
+        const char* fn = "layer_norm";
+        check_norm(fn, rows, cols, dtype, param_dtype);
+        check_ptr(fn, "x", x, rows > 0);
+        check_ptr(fn, "y", y, rows > 0);
+        check_ptr(fn, "stats", stats, rows > 0);
+        check_ptr(fn, "gamma", gamma, true);
+        check_ptr(fn, "beta", beta, true);
+        check_ld(fn, "x", ldx, cols);
+        check_ld(fn, "y", ldy, cols);
+        if (!(eps >= 0.0f)) invalid("layer_norm: eps must not be negative");
+        check_stats(fn, stats);
+        const Saved8 s{codes, ld_codes, exponents, ld_exponents};
+        check_saved8(fn, cols, s, false);
+        const NormArgs a{rows, cols, eps, range8(dtype)};
+        float2* st = reinterpret_cast<float2*>(stats);
+        by_types(dtype, param_dtype, [&](auto t, auto p) {
+            using T = decltype(t);
+            using P = decltype(p);
+            const T* xp = static_cast<const T*>(x);
+            T* yp = static_cast<T*>(y);
+            const P *gp = static_cast<const P*>(gamma), *bp = static_cast<const P*>(beta);
+            if (cols > kRegisterCols) {
+                launch("layer_norm", norm_wide_kernel<T, P>, dim3(static_cast<unsigned>(std::min<int64_t>(rows, num_sms() * 4))),
+                       dim3(512), 0, as_stream(stream), a, xp, ldx, gp, bp, yp, ldy, st, s);
+                return;
+            }
+            const bool al = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(y, ldy, sizeof(T)) &&
+                            rows_aligned16(gamma, 0, 1) && rows_aligned16(beta, 0, 1);
+            by_width(cols, [&](auto tpr, auto vpt) {
+                constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
+                const int64_t blocks = ceil_div(rows, block_threads<TPR>() / TPR);
+                auto kern = al ? norm_kernel<T, P, true, TPR, VPT> : norm_kernel<T, P, false, TPR, VPT>;
+                launch("layer_norm", kern, dim3(static_cast<unsigned>(std::min<int64_t>(blocks, int64_t(1) << 30))),
+                       dim3(block_threads<TPR>()), 0, as_stream(stream), a, xp, ldx, gp, bp, yp, ldy, st, s);
+            });
+        });
+    });
+}
+
+TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, const void* dy, int64_t lddy,
+                                    const void* x, int64_t ldx, const int8_t* codes, int64_t ld_codes,
+                                    const uint8_t* exponents, int64_t ld_exponents, const float* stats,
+                                    int32_t param_dtype, const void* gamma, void* dx, int64_t lddx, void* dgamma,
+                                    void* dbeta, void* stream) {
+    return tg::guard([&] {
+        tg::require_device();
+        using namespace tg;
+        const char* fn = "layer_norm_grad";
+        check_norm(fn, rows, cols, dtype, param_dtype);
+        check_ptr(fn, "dy", dy, rows > 0);
+        check_ptr(fn, "dx", dx, rows > 0);
+        check_ptr(fn, "stats", stats, rows > 0);
+        check_ptr(fn, "gamma", gamma, true);
+        check_ptr(fn, "dgamma", dgamma, true);
+        check_ptr(fn, "dbeta", dbeta, true);
+        check_ld(fn, "dy", lddy, cols);
+        check_ld(fn, "dx", lddx, cols);
+        if ((x != nullptr) == (codes != nullptr) && rows > 0)
+            invalid(std::string(fn) + ": exactly one of x and codes is given");
+        if (x) check_ld(fn, "x", ldx, cols);
+        const Saved8 s{const_cast<int8_t*>(codes), ld_codes, const_cast<uint8_t*>(exponents), ld_exponents};
+        check_saved8(fn, cols, s, codes != nullptr);
+        check_stats(fn, stats);
+        const NormArgs a{rows, cols, 0.0f, range8(dtype)};
+        const float2* st = reinterpret_cast<const float2*>(stats);
+        cudaStream_t str = as_stream(stream);
+        by_types(dtype, param_dtype, [&](auto t, auto p) {
+            using T = decltype(t);
+            using P = decltype(p);
+            const T *dyp = static_cast<const T*>(dy), *xp = static_cast<const T*>(x);
+            T* dxp = static_cast<T*>(dx);
+            const P* gp = static_cast<const P*>(gamma);
+            int64_t parts = 0;
+            const auto join = [&](const float* part) {
+                launch("layer_norm_join", norm_join_kernel<P>, dim3(static_cast<unsigned>(ceil_div(2 * cols, 32))),
+                       dim3(256), 0, str, part, static_cast<int>(parts), cols, static_cast<P*>(dgamma),
+                       static_cast<P*>(dbeta));
+            };
+            if (cols > kRegisterCols) {
+                parts = std::min<int64_t>(std::max<int64_t>(ceil_div(rows, 16), 0), 64);
+                Scratch<float> part(static_cast<size_t>(parts * 2 * cols), str);
+                auto kern = codes ? norm_wide_grad_kernel<T, P, true> : norm_wide_grad_kernel<T, P, false>;
+                launch("layer_norm_grad", kern, dim3(static_cast<unsigned>(std::min<int64_t>(rows, num_sms() * 4))),
+                       dim3(512), 0, str, a, dyp, lddy, xp, ldx, s, st, gp, dxp, lddx);
+                auto sums = codes ? norm_wide_sums_kernel<T, true> : norm_wide_sums_kernel<T, false>;
+                launch("layer_norm_sums", sums,
+                       dim3(static_cast<unsigned>(ceil_div(cols, 256)), static_cast<unsigned>(parts)), dim3(256), 0,
+                       str, a, dyp, lddy, xp, ldx, s, st, part.p);
+                join(part.p);
+                return;
+            }
+            const bool al = rows_aligned16(dy, lddy, sizeof(T)) && (codes || rows_aligned16(x, ldx, sizeof(T))) &&
+                            rows_aligned16(dx, lddx, sizeof(T)) && rows_aligned16(gamma, 0, 1);
+            by_width(cols, [&](auto tpr, auto vpt) {
+                constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
+                constexpr int BT = block_threads<TPR>(), RPB = BT / TPR;
+                auto kern = codes ? (al ? norm_grad_kernel<T, P, true, TPR, VPT, true>
+                                        : norm_grad_kernel<T, P, false, TPR, VPT, true>)
+                                  : (al ? norm_grad_kernel<T, P, true, TPR, VPT, false>
+                                        : norm_grad_kernel<T, P, false, TPR, VPT, false>);
+                parts = std::min<int64_t>(ceil_div(rows, RPB), int64_t(num_sms()) * (BT == 512 ? 2 : 4));
+                Scratch<float> part(static_cast<size_t>(parts * 2 * cols), str);
+                launch("layer_norm_grad", kern, dim3(static_cast<unsigned>(parts)), dim3(BT), 0, str, a, dyp, lddy, xp,
+                       ldx, s, st, gp, dxp, lddx, part.p);
+                join(part.p);
+            });
+        });
+    });
+}
+
+}  // extern "C"
