@@ -194,6 +194,7 @@ bool gemm_tc_supported(int64_t N, int64_t K, const float* A, int64_t lda);
 int gemm_tc_take_error(cudaStream_t s);
 int gather_take_error(cudaStream_t s);
 int peer_take_error(cudaStream_t s);
+int typed_take_error();
 void gemm_tc(int64_t M, int64_t N, int64_t K, const float* A, int64_t lda, const float* B, int64_t ldb, float* C,
              int64_t ldc, const float* bias, int act, float alpha, cudaStream_t s, const PeerOut& peers = PeerOut{},
              bool c_cols_padded = false, const float* row_scale = nullptr);
@@ -383,6 +384,10 @@ TG_API tg_status tg_take_device_error(void* stream) {
         const int code = gemm_tc_take_error(as_stream(stream));
         const int gcode = gather_take_error(as_stream(stream));
         const int pcode = peer_take_error(as_stream(stream));
+        const int tcode = typed_take_error();
+        if (tcode)
+            fail(TG_ERR_TIMEOUT, "a typed product's pipeline wait ran out (code " + std::to_string(tcode) +
+                                     "); its output is invalid");
         if (code)
             fail(TG_ERR_TIMEOUT, "a tensor-core GEMM pipeline wait ran out (stage code " + std::to_string(code) +
                                      "); its output is invalid");

@@ -20,132 +20,6 @@ namespace tg {
 
 namespace {
 
-// ── Products on the FP32 units ───────────────────────────────────────────
-// Tiles of 64 rows and 128 columns, 256 threads of 4 rows x 8 columns, the
-// inner dimension in steps of 16 through shared memory.  Thread (ty, tx)
-// holds columns tx + 16 j: the 128 columns of a row, which share an exponent
-// in the saved form, lie in the 16 lanes of half a warp.
-constexpr int FM = 64, FN = 128, FK = 16;
-
-template <class GetA, class GetB>
-__device__ __forceinline__ void fma_tiles(float (&acc)[4][8], int64_t k0, int64_t k1, GetA&& a, GetB&& b) {
-    __shared__ float As[FK][FM + 4], Bs[FK][FN];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    for (int64_t k = k0; k < k1; k += FK) {
-        for (int i = threadIdx.x; i < FM * FK; i += 256) {
-            const int m = i / FK, kk = i % FK;
-            As[kk][m] = k + kk < k1 ? a(m, k + kk) : 0.0f;
-        }
-        for (int i = threadIdx.x; i < FN * FK; i += 256) {
-            const int kk = i / FN, n = i % FN;
-            Bs[kk][n] = k + kk < k1 ? b(k + kk, n) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < FK; ++kk) {
-            float av[4], bv[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) av[i] = As[kk][ty * 4 + i];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) bv[j] = Bs[kk][tx + 16 * j];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
-        }
-        __syncthreads();
-    }
-}
-
-// C rows [r0, r1) of one type = A . B (+ epilogue).  TRANS: B is W^T.
-template <class T, bool TRANS>
-__global__ void __launch_bounds__(256) typed_rows_kernel(RowsArgs<T> g) {
-    __shared__ int sh_type, sh_begin, sh_end;
-    if (threadIdx.x == 0) {
-        int tile = blockIdx.x;
-        sh_type = -1;
-        for (int t = 0; t < g.types; ++t) {
-            const int b = clamp_row(g.offsets[t], g.M), e = clamp_row(g.offsets[t + 1], g.M);
-            const int n = e > b ? (e - b + FM - 1) / FM : 0;
-            if (tile < n) {
-                sh_type = t;
-                sh_begin = b + tile * FM;
-                sh_end = e;
-                break;
-            }
-            tile -= n;
-        }
-    }
-    __syncthreads();
-    if (sh_type < 0) return;
-    const int64_t r0 = sh_begin, r1 = sh_end, n0 = static_cast<int64_t>(blockIdx.y) * FN;
-    const T* w = g.W + sh_type * g.stride_w;
-    float acc[4][8] = {};
-    fma_tiles(
-        acc, 0, g.K, [&](int m, int64_t k) { return r0 + m < r1 ? to_f32(g.A[(r0 + m) * g.lda + k]) : 0.0f; },
-        [&](int64_t k, int n) {
-            if (n0 + n >= g.N) return 0.0f;
-            return to_f32(TRANS ? w[(n0 + n) * g.ldw + k] : w[k * g.ldw + n0 + n]);
-        });
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t r = r0 + ty * 4 + i;
-        const bool live = r < r1;
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t n = n0 + tx + 16 * j;
-            if (g.bias && n < g.N) acc[i][j] += g.bias[sh_type * g.N + n];
-            if (n < g.N) m = max(m, mag_bits(acc[i][j]));
-        }
-        if (g.saved.codes) {
-            const int byte = exponent8(reduce_max<16>(m), g.r8.emin);
-            const float inv = encode8(byte);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t n = n0 + tx + 16 * j;
-                if (live && n < g.N) g.saved.codes[r * g.saved.ld + n] = code8(acc[i][j], inv, byte, g.r8.top);
-            }
-            if (live && tx == 0) g.saved.exps[r * g.saved.lde + blockIdx.y] = static_cast<uint8_t>(byte);
-        }
-        act_forward(acc[i], g.act, g.alpha);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t n = n0 + tx + 16 * j;
-            if (live && n < g.N) g.C[r * g.ldc + n] = from_f32<T>(acc[i][j]);
-        }
-    }
-}
-
-// dW of one type (blockIdx.z), 64 x 128 of it.
-template <class T, class O, bool SAVED>
-__global__ void __launch_bounds__(256) typed_weight_kernel(WeightArgs<T, O> g) {
-    const int t = blockIdx.z;
-    const int64_t b = clamp_row(g.offsets[t], g.M), e = clamp_row(g.offsets[t + 1], g.M);
-    const int64_t k0 = static_cast<int64_t>(blockIdx.x) * FM, n0 = static_cast<int64_t>(blockIdx.y) * FN;
-    float acc[4][8] = {};
-    fma_tiles(
-        acc, b, e,
-        [&](int m, int64_t r) {
-            const int64_t k = k0 + m;
-            if (k >= g.K) return 0.0f;
-            if (SAVED)
-                return __fmul_rn(static_cast<float>(g.saved.codes[r * g.saved.ld + k]),
-                                 decode8(g.saved.exps[r * g.saved.lde + k / kBlock8]));
-            return to_f32(g.X[r * g.ldx + k]);
-        },
-        [&](int64_t r, int n) { return n0 + n < g.N ? to_f32(g.dY[r * g.lddy + n0 + n]) : 0.0f; });
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t k = k0 + ty * 4 + i, n = n0 + tx + 16 * j;
-            if (k < g.K && n < g.N) g.dW[t * g.stride_dw + k * g.lddw + n] = from_f32<O>(acc[i][j]);
-        }
-}
-
 // db of one type (blockIdx.y), 32 columns of it.
 template <class T, class O>
 __global__ void __launch_bounds__(256) typed_bias_kernel(WeightArgs<T, O> g) {
@@ -211,9 +85,7 @@ TG_API tg_status tg_typed_linear(int64_t rows, int64_t K, int64_t N, int64_t typ
             const RowsArgs<T> g{rows, K, N, static_cast<int>(types), static_cast<const T*>(X), ldx,
                                 static_cast<const T*>(W), ldw, stride_w, offsets, bias, act, alpha,
                                 static_cast<T*>(Y), ldy, s, range8(dtype)};
-            launch("typed_linear", typed_rows_kernel<T, false>,
-                   dim3(static_cast<unsigned>(ceil_div(rows, FM) + types), static_cast<unsigned>(ceil_div(N, FN))),
-                   dim3(256), 0, as_stream(stream), g);
+            typed_rows_tc<T, false>(g, as_stream(stream));
         });
     });
 }
@@ -238,9 +110,7 @@ TG_API tg_status tg_typed_linear_grad_input(int64_t rows, int64_t K, int64_t N, 
             const RowsArgs<T> g{rows, N, K, static_cast<int>(types), static_cast<const T*>(dY), lddy,
                                 static_cast<const T*>(W), ldw, stride_w, offsets, nullptr, TG_ACT_NONE, 0.0f,
                                 static_cast<T*>(dX), lddx, Saved8{}, Range8{}};
-            launch("typed_linear_grad_input", typed_rows_kernel<T, true>,
-                   dim3(static_cast<unsigned>(ceil_div(rows, FM) + types), static_cast<unsigned>(ceil_div(K, FN))),
-                   dim3(256), 0, as_stream(stream), g);
+            typed_rows_tc<T, true>(g, as_stream(stream));
         });
     });
 }
@@ -272,10 +142,7 @@ TG_API tg_status tg_typed_linear_grad_weight(int64_t rows, int64_t K, int64_t N,
             const WeightArgs<T, O> g{rows, K, N, static_cast<int>(types), static_cast<const T*>(X), ldx, s,
                                      static_cast<const T*>(dY), lddy, offsets, static_cast<O*>(dW), lddw, stride_dw,
                                      db};
-            launch("typed_linear_grad_weight", codes ? typed_weight_kernel<T, O, true> : typed_weight_kernel<T, O, false>,
-                   dim3(static_cast<unsigned>(ceil_div(K, FM)), static_cast<unsigned>(ceil_div(N, FN)),
-                        static_cast<unsigned>(types)),
-                   dim3(256), 0, as_stream(stream), g);
+            typed_weight_tc<T, O>(g, as_stream(stream));
             if (db)
                 launch("typed_linear_grad_bias", typed_bias_kernel<T, O>,
                        dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0,

@@ -51,4 +51,11 @@ struct WeightArgs {
     float* db;  // types x N, nullable
 };
 
+// On the tensor cores (typed_tc.cu).
+template <class T, bool TRANS>
+void typed_rows_tc(const RowsArgs<T>& a, cudaStream_t s);
+template <class T, class O>
+void typed_weight_tc(const WeightArgs<T, O>& a, cudaStream_t s);
+int typed_take_error();
+
 }  // namespace tg
