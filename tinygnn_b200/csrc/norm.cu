@@ -44,36 +44,72 @@ struct RowPart {
     static constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
     static constexpr int N = VPT / V;
     static constexpr int W = TPR < 32 ? TPR : 32;
+    static constexpr int J = ALIGNED ? 1 : W;  // columns between a slot's values
     static constexpr bool ROW_IS_BLOCK = TPR * V < kBlock8;
     static constexpr int G = ROW_IS_BLOCK ? TPR : kBlock8 / V;
     static_assert(!ROW_IS_BLOCK || TPR * VPT <= kBlock8, "a row of several slots within a block");
-    static __device__ __forceinline__ int64_t col(int t, int i, int j) {
-        return ALIGNED ? (static_cast<int64_t>(i) * TPR + t) * V + j
-                       : ((static_cast<int64_t>(i) * (TPR / W) + t / W) * V + j) * W + t % W;
+
+    int t, c0, cols;  // thread of the row, its first column, the row's columns
+    __device__ __forceinline__ RowPart(int64_t columns) {
+        t = threadIdx.x % TPR;
+        c0 = ALIGNED ? t * V : t / W * W * V + t % W;
+        cols = static_cast<int>(columns);
+    }
+    __device__ __forceinline__ int col(int i, int j) const { return c0 + i * TPR * V + j * J; }
+    __device__ __forceinline__ bool has(int i, int j) const { return col(i, j) < cols; }
+    // Slot i exists for some thread (the same answer for all of them).
+    __device__ __forceinline__ bool any(int i) const { return i == 0 || i * TPR * V < cols; }
+    // The thread's slot i is all there.
+    __device__ __forceinline__ bool whole(int i) const { return col(i, V - 1) < cols; }
+
+    // Slots as they lie in memory (zeros where there is nothing; `live` false: all zeros).
+    __device__ __forceinline__ void fetch(const T* p, bool live, Raw<T, V> (&k)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (live && whole(i))
+                k[i] = ALIGNED ? load_raw<T, V>(p + col(i, 0)) : gather_raw<T, V>([&](int j) { return p[col(i, j)]; });
+            else
+                k[i] = gather_raw<T, V>([&](int j) { return live && has(i, j) ? p[col(i, j)] : from_f32<T>(0.0f); });
+        }
     }
     template <class P>
-    static __device__ __forceinline__ void load(const P* p, int t, int i, int64_t cols, float (&x)[V]) {
-        // P's slot is a vector load where P's elements are as wide as T's (aligned alike)
-        if (ALIGNED && sizeof(P) == sizeof(T) && col(t, i, 0) + V <= cols) {
-            load_v<P, V>(p + col(t, i, 0), x);
-            return;
-        }
+    __device__ __forceinline__ void load(const P* p, int i, float (&x)[V]) const {
+        if (ALIGNED && sizeof(P) == sizeof(T) && whole(i)) {
+            load_v<P, V>(p + col(i, 0), x);
+        } else if (ALIGNED && sizeof(P) == 4 && whole(i)) {  // fp32 parameters of 16-bit rows
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = col(t, i, j) < cols ? to_f32(p[col(t, i, j)]) : 0.0f;
+            for (int j = 0; j < V; j += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(p + col(i, j));
+                x[j] = q.x, x[j + 1] = q.y, x[j + 2] = q.z, x[j + 3] = q.w;
+            }
+        } else if (whole(i)) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = to_f32(p[col(i, j)]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = has(i, j) ? to_f32(p[col(i, j)]) : 0.0f;
+        }
     }
-    static __device__ __forceinline__ void store(T* p, int t, int i, int64_t cols, const float (&x)[V]) {
-        if (ALIGNED && col(t, i, 0) + V <= cols) {
-            store_v<T, V>(p + col(t, i, 0), x);
-            return;
-        }
+    __device__ __forceinline__ void store(T* p, int i, const float (&x)[V]) const {
+        if (whole(i)) {
+            if (ALIGNED) {
+                store_v<T, V>(p + col(i, 0), x);
+            } else {
+                Raw<T, V> k;
+                narrow(x, k);
+                scatter_raw(k, [&](int j, T v) { p[col(i, j)] = v; });
+            }
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (col(t, i, j) < cols) p[col(t, i, j)] = from_f32<T>(x[j]);
+            for (int j = 0; j < V; ++j)
+                if (has(i, j)) p[col(i, j)] = from_f32<T>(x[j]);
+        }
     }
 };
 
 // Sums a and b over the TPR threads of a row; every thread gets them.
-// `red`: 2 floats per warp of the block (TPR > 32 only, where a row is the block).
+// `red`: 2 floats per warp of the block (rows of several warps; the whole
+// block takes part).
 template <int TPR>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
     a = reduce_sum<float, (TPR < 32 ? TPR : 32)>(a);
@@ -87,146 +123,228 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
     }
     __syncthreads();
     a = b = 0.0f;
+    const float* mine = red + threadIdx.x / TPR * NW * 2;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-        a += red[2 * w];
-        b += red[2 * w + 1];
+        a += mine[2 * w];
+        b += mine[2 * w + 1];
     }
 }
 
 template <int TPR>
 constexpr int block_threads() { return TPR < 128 ? 128 : TPR; }
 
+// Blocks a SM: the kernels are compiled and launched for as many.
+template <int TPR, int VPT>
+constexpr int resident() { return TPR >= 256 ? 1024 / TPR : (VPT > 8 ? 5 : 8); }
+template <int TPR, int VPT>
+constexpr int resident_grad() { return TPR >= 256 ? 512 / TPR : (VPT > 8 ? 4 : 5); }
+
+// Rows' data is fetched one row ahead while it fits in registers.
+template <class T, int VPT>
+constexpr bool ahead() { return VPT * sizeof(T) <= 64; }
+
 template <class T, class P, bool ALIGNED, int TPR, int VPT>
-__global__ void __launch_bounds__(block_threads<TPR>()) norm_kernel(NormArgs a, const T* x, int64_t ldx, const P* gamma,
+__global__ void __launch_bounds__(block_threads<TPR>(), resident<TPR, VPT>()) norm_kernel(NormArgs a, const T* x, int64_t ldx, const P* gamma,
                                                                     const P* beta, T* y, int64_t ldy, float2* stats,
                                                                     Saved8 s) {
     using R = RowPart<T, ALIGNED, TPR, VPT>;
+    constexpr int V = R::V, N = R::N;
+    constexpr bool kKeep = VPT <= 8;  // gamma and beta stay in registers
     __shared__ float red[32];
     constexpr int RPB = block_threads<TPR>() / TPR;
-    const int t = threadIdx.x % TPR;
+    const R part(a.cols);
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPB; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * RPB) {
-        const int64_t row = row0 + threadIdx.x / TPR;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
+    float gk[kKeep ? N : 1][V], bk[kKeep ? N : 1][V];
+    if (kKeep) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            part.load(gamma, i, gk[kKeep ? i : 0]);
+            part.load(beta, i, bk[kKeep ? i : 0]);
+        }
+    }
+    // every thread takes part in the reductions: the loop runs on the block's first row
+    int64_t base = static_cast<int64_t>(blockIdx.x) * RPB, row = base + threadIdx.x / TPR;
+    Raw<T, V> k[N];
+    if (ahead<T, VPT>()) part.fetch(x + (row < a.rows ? row * ldx : 0), row < a.rows, k);
+    for (; base < a.rows; base += step, row += step) {
         const bool live = row < a.rows;
-        const int64_t cols = live ? a.cols : 0;  // every thread takes part in the reductions
-        const T* xr = x + (live ? row * ldx : 0);
-        float v[R::N][R::V];
+        if (!ahead<T, VPT>()) part.fetch(x + (live ? row * ldx : 0), live, k);
+        float v[N][V];
         float sum = 0.0f, none = 0.0f;
 #pragma unroll
-        for (int i = 0; i < R::N; ++i) {
-            R::load(xr, t, i, cols, v[i]);
+        for (int i = 0; i < N; ++i) {
+            widen(k[i], v[i]);
 #pragma unroll
-            for (int j = 0; j < R::V; ++j) sum += v[i][j];
+            for (int j = 0; j < V; ++j) sum += v[i][j];
+        }
+        if (ahead<T, VPT>()) {
+            const int64_t next = row + step;
+            part.fetch(x + (next < a.rows ? next * ldx : 0), next < a.rows, k);
         }
         row_sum2<TPR>(sum, none, red);
         const float mean = __fmul_rn(sum, inv_n);
         float sq = 0.0f;
 #pragma unroll
-        for (int i = 0; i < R::N; ++i)
+        for (int i = 0; i < N; ++i) {
+            if (!part.any(i)) break;
 #pragma unroll
-            for (int j = 0; j < R::V; ++j) {
-                v[i][j] = R::col(t, i, j) < cols ? __fsub_rn(v[i][j], mean) : 0.0f;
-                sq = fmaf(v[i][j], v[i][j], sq);
+            for (int j = 0; j < V; ++j) v[i][j] = __fsub_rn(v[i][j], mean);
+            if (!part.whole(i)) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] = part.has(i, j) ? v[i][j] : 0.0f;
             }
-        row_sum2<TPR>(sq, none, red);
-        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(sq, inv_n, a.eps)));
-        if (live && t == 0) stats[row] = make_float2(mean, rstd);
-        uint32_t row_max = 0;
 #pragma unroll
-        for (int i = 0; i < R::N; ++i) {
+            for (int j = 0; j < V; ++j) sq = fmaf(v[i][j], v[i][j], sq);
+        }
+        row_sum2<TPR>(sq, none, red);
+        const float rstd = rsqrtf(fmaf(sq, inv_n, a.eps));  // 2 ulp
+        if (live && part.t == 0) stats[row] = make_float2(mean, rstd);
+        float row_max = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
             map_v(v[i], [rstd](float u) { return __fmul_rn(u, rstd); });
             if (R::ROW_IS_BLOCK) {
 #pragma unroll
-                for (int j = 0; j < R::V; ++j) row_max = max(row_max, mag_bits(v[i][j]));
+                for (int j = 0; j < V; ++j) row_max = max_mag(row_max, v[i][j]);
             }
         }
+        const int64_t at = live ? row : 0;
+        T* yr = y + at * ldy;
+        int8_t* codes = s.codes + at * s.ld;
+        uint8_t* exps = s.exps + at * s.lde;
 #pragma unroll
-        for (int i = 0; i < R::N; ++i) {
+        for (int i = 0; i < N; ++i) {
+            if (!part.any(i)) break;
             if (s.codes) {
-                uint32_t m = row_max;
+                float m = row_max;
                 if (!R::ROW_IS_BLOCK) {
 #pragma unroll
-                    for (int j = 0; j < R::V; ++j) m = max(m, mag_bits(v[i][j]));
+                    for (int j = 0; j < V; ++j) m = max_mag(m, v[i][j]);
                 }
                 const int byte = exponent8(reduce_max<R::G>(m), a.r8.emin);
                 const float inv = encode8(byte);
-                if (ALIGNED && R::col(t, i, 0) + R::V <= cols) {
-                    Pack<int8_t, R::V> k;
+                if (!live) {
+                } else if (part.whole(i)) {
+                    if (ALIGNED) {
+                        store_codes<V>(codes + part.col(i, 0), v[i], inv, byte, a.r8.top);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < R::V; ++j) k.v[j] = code8(v[i][j], inv, byte, a.r8.top);
-                    *reinterpret_cast<Pack<int8_t, R::V>*>(s.codes + row * s.ld + R::col(t, i, 0)) = k;
+                        for (int j = 0; j < V; j += 4) {
+                            const uint32_t c = codes4(v[i][j], v[i][j + 1], v[i][j + 2], v[i][j + 3], inv, byte, a.r8.top);
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) codes[part.col(i, j + b)] = static_cast<int8_t>(c >> 8 * b);
+                        }
+                    }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < R::V; ++j)
-                        if (R::col(t, i, j) < cols) s.codes[row * s.ld + R::col(t, i, j)] = code8(v[i][j], inv, byte, a.r8.top);
+                    for (int j = 0; j < V; ++j)
+                        if (part.has(i, j)) codes[part.col(i, j)] = code8(v[i][j], inv, byte, a.r8.top);
                 }
                 // the first lane of the group that holds the block writes its exponent
-                if (t % R::G == 0 && (i == 0 || !R::ROW_IS_BLOCK) && R::col(t, i, 0) < cols)
-                    s.exps[row * s.lde + R::col(t, i, 0) / kBlock8] = static_cast<uint8_t>(byte);
+                if (live && part.t % R::G == 0 && (i == 0 || !R::ROW_IS_BLOCK) && part.has(i, 0))
+                    exps[part.col(i, 0) / kBlock8] = static_cast<uint8_t>(byte);
             }
-            float g[R::V], b[R::V];
-            R::load(gamma, t, i, cols, g);
-            R::load(beta, t, i, cols, b);
+            float g[V], b[V];
+            if (kKeep) {
 #pragma unroll
-            for (int j = 0; j < R::V; ++j) g[j] = fmaf(v[i][j], g[j], b[j]);
-            if (live) R::store(y + row * ldy, t, i, cols, g);
+                for (int j = 0; j < V; ++j) g[j] = gk[kKeep ? i : 0][j], b[j] = bk[kKeep ? i : 0][j];
+            } else {
+                part.load(gamma, i, g);
+                part.load(beta, i, b);
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[j] = fmaf(v[i][j], g[j], b[j]);
+            if (live) part.store(yr, i, g);
         }
+    }
+}
+
+// The saved copy's part of a row, and its blocks' exponents.
+template <class R>
+__device__ __forceinline__ void fetch_codes(const R& part, const int8_t* codes, const uint8_t* exps, bool live,
+                                            Raw<int8_t, R::V> (&k)[R::N], int (&e)[R::N]) {
+#pragma unroll
+    for (int i = 0; i < R::N; ++i) {
+        e[i] = live && part.has(i, 0) ? exps[part.col(i, 0) / kBlock8] : 127;
+        if (live && part.whole(i) && R::J == 1)
+            k[i] = *reinterpret_cast<const Raw<int8_t, R::V>*>(codes + part.col(i, 0));
+        else
+            k[i] = gather_codes<R::V>([&](int j) { return live && part.has(i, j) ? codes[part.col(i, j)] : int8_t(0); });
     }
 }
 
 // dx, and this block's partial sums of dgamma and dbeta: part[block][2][cols].
 template <class T, class P, bool ALIGNED, int TPR, int VPT, bool SAVED>
-__global__ void __launch_bounds__(block_threads<TPR>()) norm_grad_kernel(NormArgs a, const T* dy, int64_t lddy,
+__global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>()) norm_grad_kernel(NormArgs a, const T* dy, int64_t lddy,
                                                                          const T* x, int64_t ldx, Saved8 s,
                                                                          const float2* stats, const P* gamma, T* dx,
-                                                                         int64_t lddx, float* part) {
+                                                                         int64_t lddx, float* partial) {
     using R = RowPart<T, ALIGNED, TPR, VPT>;
-    constexpr int RPB = block_threads<TPR>() / TPR;
+    constexpr int V = R::V, N = R::N, RPB = block_threads<TPR>() / TPR;
+    constexpr bool kKeep = VPT <= 8, kAhead = ahead<T, 2 * VPT>();
     __shared__ float red[32];
     __shared__ float join[RPB > 1 ? RPB * TPR * VPT : 1];
-    const int t = threadIdx.x % TPR;
+    const R part(a.cols);
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
-    float ag[R::N][R::V], ab[R::N][R::V];
+    const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
+    float ag[N][V], ab[N][V], gk[kKeep ? N : 1][V];
 #pragma unroll
-    for (int i = 0; i < R::N; ++i)
+    for (int i = 0; i < N; ++i) {
+        if (kKeep) part.load(gamma, i, gk[kKeep ? i : 0]);
 #pragma unroll
-        for (int j = 0; j < R::V; ++j) ag[i][j] = ab[i][j] = 0.0f;
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPB; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * RPB) {
-        const int64_t row = row0 + threadIdx.x / TPR;
+        for (int j = 0; j < V; ++j) ag[i][j] = ab[i][j] = 0.0f;
+    }
+    Raw<T, V> kd[N], kx[SAVED ? 1 : N];
+    Raw<int8_t, V> kc[SAVED ? N : 1];
+    int ke[SAVED ? N : 1];
+    float2 st;
+    const auto fetch = [&](int64_t r) {
+        const bool live = r < a.rows;
+        const int64_t at = live ? r : 0;
+        st = stats[at];
+        part.fetch(dy + at * lddy, live, kd);
+        if constexpr (SAVED) fetch_codes(part, s.codes + at * s.ld, s.exps + at * s.lde, live, kc, ke);
+        else part.fetch(x + at * ldx, live, kx);
+    };
+    int64_t base = static_cast<int64_t>(blockIdx.x) * RPB, row = base + threadIdx.x / TPR;
+    if (kAhead) fetch(row);
+    for (; base < a.rows; base += step, row += step) {
         const bool live = row < a.rows;
-        const int64_t cols = live ? a.cols : 0;
-        const int64_t r0 = live ? row : 0;
-        const float2 st = stats[r0];
-        float h[R::N][R::V], g[R::N][R::V];
+        if (!kAhead) fetch(row);
+        const float mean = st.x, rstd = st.y;
+        float h[N][V], g[N][V];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (SAVED) {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) values4(kc[i].w[j / 4], ke[i], &h[i][j]);
+            } else {
+                widen(kx[i], h[i]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) h[i][j] = __fmul_rn(__fsub_rn(h[i][j], mean), rstd);
+                if (!part.whole(i)) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) h[i][j] = part.has(i, j) ? h[i][j] : 0.0f;
+                }
+            }
+            widen(kd[i], g[i]);
+        }
+        if (kAhead) fetch(row + step);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < R::N; ++i) {
-            R::load(dy + r0 * lddy, t, i, cols, g[i]);
-            if (SAVED) {
-                const int64_t c = R::col(t, i, 0);
-                const float scale = c < cols ? decode8(s.exps[r0 * s.lde + c / kBlock8]) : 0.0f;
-                if (ALIGNED && c + R::V <= cols) {
-                    const Pack<int8_t, R::V> k = *reinterpret_cast<const Pack<int8_t, R::V>*>(s.codes + r0 * s.ld + c);
+        for (int i = 0; i < N; ++i) {
+            if (!part.any(i)) break;
+            float w[V];
+            if (kKeep) {
 #pragma unroll
-                    for (int j = 0; j < R::V; ++j) h[i][j] = __fmul_rn(static_cast<float>(k.v[j]), scale);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < R::V; ++j)
-                        h[i][j] = R::col(t, i, j) < cols
-                                      ? __fmul_rn(static_cast<float>(s.codes[r0 * s.ld + R::col(t, i, j)]), scale)
-                                      : 0.0f;
-                }
+                for (int j = 0; j < V; ++j) w[j] = gk[kKeep ? i : 0][j];
             } else {
-                R::load(x + r0 * ldx, t, i, cols, h[i]);
-#pragma unroll
-                for (int j = 0; j < R::V; ++j)
-                    h[i][j] = R::col(t, i, j) < cols ? __fmul_rn(__fsub_rn(h[i][j], st.x), st.y) : 0.0f;
+                part.load(gamma, i, w);
             }
-            float w[R::V];
-            R::load(gamma, t, i, a.cols, w);
 #pragma unroll
-            for (int j = 0; j < R::V; ++j) {
+            for (int j = 0; j < V; ++j) {
                 ag[i][j] = fmaf(g[i][j], h[i][j], ag[i][j]);
                 ab[i][j] += g[i][j];
                 g[i][j] = __fmul_rn(g[i][j], w[j]);
@@ -236,41 +354,44 @@ __global__ void __launch_bounds__(block_threads<TPR>()) norm_grad_kernel(NormArg
         }
         row_sum2<TPR>(s1, s2, red);
         const float m1 = __fmul_rn(s1, inv_n), m2 = __fmul_rn(s2, inv_n);
+        T* out = dx + (live ? row * lddx : 0);
 #pragma unroll
-        for (int i = 0; i < R::N; ++i) {
+        for (int i = 0; i < N; ++i) {
+            if (!part.any(i)) break;
 #pragma unroll
-            for (int j = 0; j < R::V; ++j) g[i][j] = __fmul_rn(st.y, fmaf(-h[i][j], m2, __fsub_rn(g[i][j], m1)));
-            if (live) R::store(dx + row * lddx, t, i, cols, g[i]);
+            for (int j = 0; j < V; ++j) g[i][j] = __fmul_rn(rstd, fmaf(-h[i][j], m2, __fsub_rn(g[i][j], m1)));
+            if (live) part.store(out, i, g[i]);
         }
     }
-    float* out = part + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+    float* sums = partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
     if constexpr (RPB == 1) {
 #pragma unroll
-        for (int i = 0; i < R::N; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < R::V; ++j)
-                if (R::col(t, i, j) < a.cols) {
-                    out[R::col(t, i, j)] = ag[i][j];
-                    out[a.cols + R::col(t, i, j)] = ab[i][j];
+            for (int j = 0; j < V; ++j)
+                if (part.has(i, j)) {
+                    sums[part.col(i, j)] = ag[i][j];
+                    sums[a.cols + part.col(i, j)] = ab[i][j];
                 }
     } else {
-        // The block's row groups, joined through shared memory: slot k of
+        // The block's row groups, joined through shared memory: value k of
         // thread t of group q at (q * VPT + k) * TPR + t.
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < R::N; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int j = 0; j < R::V; ++j)
-                    join[(threadIdx.x / TPR * VPT + i * R::V + j) * TPR + t] = half ? ab[i][j] : ag[i][j];
+                for (int j = 0; j < V; ++j)
+                    join[(threadIdx.x / TPR * VPT + i * V + j) * TPR + part.t] = half ? ab[i][j] : ag[i][j];
             __syncthreads();
             for (int q = threadIdx.x; q < TPR * VPT; q += block_threads<TPR>()) {
                 float sum = 0.0f;
 #pragma unroll 4
                 for (int r = 0; r < RPB; ++r) sum += join[r * VPT * TPR + q];
-                const int64_t c = R::col(q % TPR, q / TPR / R::V, q / TPR % R::V);
-                if (c < a.cols) out[half * a.cols + c] = sum;
+                const int t = q % TPR, i = q / TPR / V, j = q / TPR % V;
+                const int c = (ALIGNED ? t * V : t / R::W * R::W * V + t % R::W) + i * TPR * V + j * R::J;
+                if (c < a.cols) sums[half * a.cols + c] = sum;
             }
         }
     }
@@ -295,17 +416,17 @@ __global__ void __launch_bounds__(512) norm_wide_kernel(NormArgs a, const T* x, 
             sq = fmaf(d, d, sq);
         }
         row_sum2<512>(sq, none, red);
-        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(sq, inv_n, a.eps)));
+        const float rstd = rsqrtf(fmaf(sq, inv_n, a.eps));
         if (threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
         // one warp per block of 128 columns
         for (int64_t b = warp; b * kBlock8 < a.cols; b += 16) {
             float h[4];
-            uint32_t m = 0;
+            float m = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int64_t c = b * kBlock8 + j * 32 + lane;
                 h[j] = c < a.cols ? __fmul_rn(__fsub_rn(to_f32(xr[c]), mean), rstd) : 0.0f;
-                m = max(m, mag_bits(h[j]));
+                m = max_mag(m, h[j]);
                 if (c < a.cols) y[row * ldy + c] = from_f32<T>(fmaf(h[j], to_f32(gamma[c]), to_f32(beta[c])));
             }
             if (s.codes) {
@@ -372,25 +493,24 @@ __global__ void __launch_bounds__(256) norm_wide_sums_kernel(NormArgs a, const T
 }
 
 // dgamma / dbeta = the sum of `parts` partial rows [2][cols], in their order
-// within each of 8 interleaved chains joined in order.
+// within each of 32 interleaved chains, which are joined in order.
 template <class P>
-__global__ void __launch_bounds__(256) norm_join_kernel(const float* part, int parts, int64_t cols, P* dgamma, P* dbeta) {
-    __shared__ float sh[8][33];
+__global__ void __launch_bounds__(1024) norm_join_kernel(const float* part, int parts, int64_t cols, P* dgamma, P* dbeta) {
+    __shared__ float sh[32][33];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // of 2 * cols
     float sum = 0.0f;
     if (c < 2 * cols) {
 #pragma unroll 8
-        for (int p = w; p < parts; p += 8) sum += part[static_cast<int64_t>(p) * 2 * cols + c];
+        for (int p = w; p < parts; p += 32) sum += part[static_cast<int64_t>(p) * 2 * cols + c];
     }
     sh[w][lane] = sum;
     __syncthreads();
-    if (w == 0 && c < 2 * cols) {
-        sum = 0.0f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) sum += sh[q][lane];
-        if (c < cols) dgamma[c] = from_f32<P>(sum);
-        else dbeta[c - cols] = from_f32<P>(sum);
+    sum = reduce_sum<float, 32>(sh[lane][w]);  // warp w: column w's 32 chains
+    const int64_t d = static_cast<int64_t>(blockIdx.x) * 32 + w;
+    if (lane == 0 && d < 2 * cols) {
+        if (d < cols) dgamma[d] = from_f32<P>(sum);
+        else dbeta[d - cols] = from_f32<P>(sum);
     }
 }
 
@@ -403,8 +523,10 @@ void by_width(int64_t cols, F&& f) {
     if (cols <= 32) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     else if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     else if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    else if (cols <= 1024) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
-    else if (cols <= 4096) f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
+    else if (cols <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    else if (cols <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
+    else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
     else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
 }
 
@@ -471,9 +593,10 @@ TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const 
                             rows_aligned16(gamma, 0, 1) && rows_aligned16(beta, 0, 1);
             by_width(cols, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
-                const int64_t blocks = ceil_div(rows, block_threads<TPR>() / TPR);
+                const int64_t blocks = std::min<int64_t>(ceil_div(rows, block_threads<TPR>() / TPR),
+                                                         int64_t(num_sms()) * resident<TPR, VPT>());
                 auto kern = al ? norm_kernel<T, P, true, TPR, VPT> : norm_kernel<T, P, false, TPR, VPT>;
-                launch("layer_norm", kern, dim3(static_cast<unsigned>(std::min<int64_t>(blocks, int64_t(1) << 30))),
+                launch("layer_norm", kern, dim3(static_cast<unsigned>(blocks)),
                        dim3(block_threads<TPR>()), 0, as_stream(stream), a, xp, ldx, gp, bp, yp, ldy, st, s);
             });
         });
@@ -516,7 +639,7 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
             int64_t parts = 0;
             const auto join = [&](const float* part) {
                 launch("layer_norm_join", norm_join_kernel<P>, dim3(static_cast<unsigned>(ceil_div(2 * cols, 32))),
-                       dim3(256), 0, str, part, static_cast<int>(parts), cols, static_cast<P*>(dgamma),
+                       dim3(1024), 0, str, part, static_cast<int>(parts), cols, static_cast<P*>(dgamma),
                        static_cast<P*>(dbeta));
             };
             if (cols > kRegisterCols) {
@@ -541,7 +664,7 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
                                         : norm_grad_kernel<T, P, false, TPR, VPT, true>)
                                   : (al ? norm_grad_kernel<T, P, true, TPR, VPT, false>
                                         : norm_grad_kernel<T, P, false, TPR, VPT, false>);
-                parts = std::min<int64_t>(ceil_div(rows, RPB), int64_t(num_sms()) * (BT == 512 ? 2 : 4));
+                parts = std::min<int64_t>(ceil_div(rows, RPB), int64_t(num_sms()) * resident_grad<TPR, VPT>());
                 Scratch<float> part(static_cast<size_t>(parts * 2 * cols), str);
                 launch("layer_norm_grad", kern, dim3(static_cast<unsigned>(parts)), dim3(BT), 0, str, a, dyp, lddy, xp,
                        ldx, s, st, gp, dxp, lddx, part.p);

@@ -3,10 +3,12 @@
 //  8 bits, the values back, and the activation's backward pass from them.
 //
 //  All three read and write each value once (the form is in values.cuh) and
-//  are bound by HBM.  A unit of work is one block of 128 columns of one row:
-//  its exponent needs the largest of the 128 magnitudes, which one warp's (or,
-//  at 8 values a lane, half a warp's) shuffles give, so values stay in
-//  registers between the read and the two writes.
+//  are bound by HBM.  A block of 128 columns of one row is the work of G lanes
+//  (16 bytes a lane: half a warp for 16-bit values, a warp for fp32): the
+//  block's exponent is a shuffle reduction over values that stay in registers
+//  between the read and the two writes.  A group keeps its columns and walks
+//  the rows R apart, U rows at a time: the loads of U rows are in flight
+//  together, and no row costs a division.
 // ============================================================================
 #include <algorithm>
 
@@ -22,51 +24,67 @@ template <class T, bool ALIGNED>
 struct Lanes {
     static constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
     static constexpr int G = kBlock8 / V;
-    static __device__ __forceinline__ int col(int lane, int j) { return ALIGNED ? lane * V + j : j * 32 + lane; }
-    // The lane's values of the block starting at p, of which `left` columns exist.
-    static __device__ __forceinline__ void load(const T* p, int lane, int64_t left, float (&x)[V]) {
-        if (ALIGNED && (lane + 1) * V <= left) {
-            load_v<T, V>(p + lane * V, x);
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = col(lane, j) < left ? to_f32(p[col(lane, j)]) : 0.0f;
+    static constexpr int U = ALIGNED ? 4 : 2;  // rows in flight
+    int lane, left;   // of the block's columns, `left` exist
+    bool full;        // the lane's values are all there, and contiguous
+
+    __device__ __forceinline__ Lanes(int64_t columns_left) {
+        lane = threadIdx.x % G;
+        left = columns_left < kBlock8 ? static_cast<int>(columns_left) : kBlock8;
+        full = ALIGNED && (lane + 1) * V <= left;
     }
-    static __device__ __forceinline__ void store(T* p, int lane, int64_t left, const float (&x)[V]) {
-        if (ALIGNED && (lane + 1) * V <= left) {
+    __device__ __forceinline__ int col(int j) const { return ALIGNED ? lane * V + j : j * 32 + lane; }
+    __device__ __forceinline__ Raw<T, V> load(const T* p, bool live) const {
+        if (full && live) return load_raw<T, V>(p + lane * V);
+        return gather_raw<T, V>([&](int j) { return col(j) < left && live ? p[col(j)] : from_f32<T>(0.0f); });
+    }
+    __device__ __forceinline__ void store(T* p, const float (&x)[V]) const {
+        if (full) {
             store_v<T, V>(p + lane * V, x);
             return;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (col(lane, j) < left) p[col(lane, j)] = from_f32<T>(x[j]);
+            if (col(j) < left) p[col(j)] = from_f32<T>(x[j]);
     }
-    static __device__ __forceinline__ void store_codes(int8_t* p, int lane, int64_t left, const float (&x)[V],
-                                                       float inv, int byte, int top) {
-        Pack<int8_t, V> k;
-#pragma unroll
-        for (int j = 0; j < V; ++j) k.v[j] = code8(x[j], inv, byte, top);
-        if (ALIGNED && (lane + 1) * V <= left) {
-            *reinterpret_cast<Pack<int8_t, V>*>(p + lane * V) = k;
+    __device__ __forceinline__ void save(int8_t* p, const float (&x)[V], int byte, int top) const {
+        const float inv = encode8(byte);
+        if (full) {
+            store_codes<V>(p + lane * V, x, inv, byte, top);
             return;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (col(lane, j) < left) p[col(lane, j)] = k.v[j];
+            if (col(j) < left) p[col(j)] = code8(x[j], inv, byte, top);
     }
-    static __device__ __forceinline__ void load_codes(const int8_t* p, int lane, int64_t left, float scale,
-                                                      float (&x)[V]) {
-        Pack<int8_t, V> k;
-        if (ALIGNED && (lane + 1) * V <= left) {
-            k = *reinterpret_cast<const Pack<int8_t, V>*>(p + lane * V);
-        } else {
+    __device__ __forceinline__ Raw<int8_t, V> load_codes(const int8_t* p, bool live) const {
+        if (full && live) return *reinterpret_cast<const Raw<int8_t, V>*>(p + lane * V);
+        return gather_codes<V>([&](int j) { return col(j) < left && live ? p[col(j)] : int8_t(0); });
+    }
+    static __device__ __forceinline__ void values(const Raw<int8_t, V>& k, int byte, float (&x)[V]) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) k.v[j] = col(lane, j) < left ? p[col(lane, j)] : int8_t(0);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = __fmul_rn(static_cast<float>(k.v[j]), scale);
+        for (int j = 0; j < V / 4; ++j) values4(k.w[j], byte, x + 4 * j);
     }
 };
+
+// The block of columns that this thread's group keeps, and its rows: row0,
+// row0 + step, ...  base: the least row0 of the warp (every lane of a warp
+// takes part in the shuffles, so a warp's loop runs on base).
+struct Walk {
+    int64_t b, row0, base, step;
+};
+template <int G>
+__device__ __forceinline__ Walk walk(int64_t rows, int64_t nb) {
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * (256 / G);
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * (256 / G) + threadIdx.x / G;
+    Walk w;
+    w.step = groups / nb;
+    w.row0 = id / nb;
+    w.b = id - w.row0 * nb;
+    w.base = __shfl_sync(0xffffffffu, w.row0, 0);
+    if (w.row0 >= w.step) w.row0 = rows;  // a group left over: no rows
+    return w;
+}
 
 struct ActArgs {
     int64_t rows, cols, nb;  // nb blocks a row
@@ -75,30 +93,45 @@ struct ActArgs {
     Range8 r8;
 };
 
-// y = act(x) (y nullable), saved = x in 8 bits.
-template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(256) save8_kernel(ActArgs a, const T* x, int64_t ldx, T* y, int64_t ldy, Saved8 o) {
+// y = act(x) (y nullable), saved = x in 8 bits.  ACT: as in act_forward.
+template <class T, bool ALIGNED, int ACT>
+__global__ void __launch_bounds__(256, 3) save8_kernel(ActArgs a, const T* x, int64_t ldx, T* y,
+                                                                     int64_t ldy, Saved8 o) {
     using L = Lanes<T, ALIGNED>;
-    const int lane = threadIdx.x % L::G;
-    const int64_t total = a.rows * a.nb, step = static_cast<int64_t>(gridDim.x) * (256 / L::G);
-    // Every lane of a warp takes part in the shuffles: the bound is the warp's first unit.
-    int64_t u = static_cast<int64_t>(blockIdx.x) * (256 / L::G) + threadIdx.x / L::G;
-    const int64_t first = static_cast<int>(threadIdx.x / 32 * (32 / L::G)) - static_cast<int>(threadIdx.x / L::G);  // this warp's first unit, less u
-    for (; u + first < total; u += step) {
-        const bool live = u < total;
-        const int64_t row = live ? u / a.nb : 0, b = live ? u - row * a.nb : 0;
-        const int64_t c0 = b * kBlock8, left = live ? a.cols - c0 : 0;
-        float v[L::V];
-        L::load(x + row * ldx + c0, lane, left, v);
-        uint32_t m = 0;
+    constexpr int V = L::V, U = L::U;
+    const Walk w = walk<L::G>(a.rows, a.nb);
+    const int64_t c0 = w.b * kBlock8;
+    const L l(a.cols - c0);
+    const bool forward = y != nullptr;
+    // pointers to the group's rows, a step at a time (multiples of the steps
+    // would be kept in registers)
+    const int64_t first = w.row0 < a.rows ? w.row0 : 0;
+    const T* px = x + first * ldx + c0;
+    T* py = y + (forward ? first * ldy + c0 : 0);
+    int8_t* pc = o.codes + first * o.ld + c0;
+    uint8_t* pe = o.exps + first * o.lde + w.b;
+    const int64_t dx = w.step * ldx, dy = w.step * ldy, dc = w.step * o.ld, de = w.step * o.lde;
+    for (int64_t base = w.base, row = w.row0; base < a.rows; base += U * w.step, row += U * w.step) {
+        Raw<T, V> k[U];
 #pragma unroll
-        for (int j = 0; j < L::V; ++j) m = max(m, mag_bits(v[j]));
-        const int byte = exponent8(reduce_max<L::G>(m), a.r8.emin);
-        L::store_codes(o.codes + row * o.ld + c0, lane, left, v, encode8(byte), byte, a.r8.top);
-        if (live && lane == 0) o.exps[row * o.lde + b] = static_cast<uint8_t>(byte);
-        if (y) {
-            act_forward(v, a.act, a.alpha);
-            L::store(y + row * ldy + c0, lane, left, v);
+        for (int u = 0; u < U; ++u, px += dx) k[u] = l.load(px, row + u * w.step < a.rows);
+#pragma unroll
+        for (int u = 0; u < U; ++u, py += dy, pc += dc, pe += de) {
+            float v[V];
+            widen(k[u], v);
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) m = max_mag(m, v[j]);
+            const int byte = exponent8(reduce_max<L::G>(m), a.r8.emin);
+            if (row + u * w.step < a.rows) {
+                l.save(pc, v, byte, a.r8.top);
+                if (l.lane == 0) *pe = static_cast<uint8_t>(byte);
+                if (forward) {
+                    act_forward<sizeof(T) == 2, ACT>(v, a.act, a.alpha);
+                    l.store(py, v);
+                }
+            }
+            __syncwarp();
         }
     }
 }
@@ -107,39 +140,71 @@ __global__ void __launch_bounds__(256) save8_kernel(ActArgs a, const T* x, int64
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) restore8_kernel(ActArgs a, Saved8 s, T* y, int64_t ldy) {
     using L = Lanes<T, ALIGNED>;
-    const int lane = threadIdx.x % L::G;
-    const int64_t total = a.rows * a.nb, step = static_cast<int64_t>(gridDim.x) * (256 / L::G);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (256 / L::G) + threadIdx.x / L::G; u < total; u += step) {
-        const int64_t row = u / a.nb, b = u - row * a.nb, c0 = b * kBlock8;
+    const Walk w = walk<L::G>(a.rows, a.nb);
+    const int64_t c0 = w.b * kBlock8;
+    const L l(a.cols - c0);
+    for (int64_t row = w.row0; row < a.rows; row += w.step) {
         float v[L::V];
-        L::load_codes(s.codes + row * s.ld + c0, lane, a.cols - c0, decode8(s.exps[row * s.lde + b]), v);
-        L::store(y + row * ldy + c0, lane, a.cols - c0, v);
+        L::values(l.load_codes(s.codes + row * s.ld + c0, true), s.exps[row * s.lde + w.b], v);
+        l.store(y + row * ldy + c0, v);
     }
 }
 
 // dx = dy * act'(x), x given as it was or in 8 bits.
-template <class T, bool ALIGNED, bool SAVED>
-__global__ void __launch_bounds__(256) act_grad_kernel(ActArgs a, const T* dy, int64_t lddy, const T* x, int64_t ldx,
-                                                       Saved8 s, T* dx, int64_t lddx) {
+template <class T, bool ALIGNED, bool SAVED, int ACT>
+__global__ void __launch_bounds__(256, 3) act_grad_kernel(ActArgs a, const T* dy, int64_t lddy,
+                                                                        const T* x, int64_t ldx, Saved8 s, T* dx,
+                                                                        int64_t lddx) {
     using L = Lanes<T, ALIGNED>;
-    const int lane = threadIdx.x % L::G;
-    const int64_t total = a.rows * a.nb, step = static_cast<int64_t>(gridDim.x) * (256 / L::G);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * (256 / L::G) + threadIdx.x / L::G; u < total; u += step) {
-        const int64_t row = u / a.nb, b = u - row * a.nb, c0 = b * kBlock8, left = a.cols - c0;
-        float v[L::V], g[L::V];
-        if (SAVED) L::load_codes(s.codes + row * s.ld + c0, lane, left, decode8(s.exps[row * s.lde + b]), v);
-        else L::load(x + row * ldx + c0, lane, left, v);
-        L::load(dy + row * lddy + c0, lane, left, g);
-        act_slope(v, a.act, a.alpha);
+    constexpr int V = L::V, U = L::U;
+    const Walk w = walk<L::G>(a.rows, a.nb);
+    const int64_t c0 = w.b * kBlock8;
+    const L l(a.cols - c0);
+    if (w.row0 >= a.rows) return;
+    const T *pg = dy + w.row0 * lddy + c0, *px = SAVED ? nullptr : x + w.row0 * ldx + c0;
+    const int8_t* pc = SAVED ? s.codes + w.row0 * s.ld + c0 : nullptr;
+    const uint8_t* pe = SAVED ? s.exps + w.row0 * s.lde + w.b : nullptr;
+    T* po = dx + w.row0 * lddx + c0;
+    const int64_t dg = w.step * lddy, dX = w.step * ldx, dc = w.step * s.ld, de = w.step * s.lde, dout = w.step * lddx;
+    for (int64_t row = w.row0; row < a.rows; row += U * w.step) {
+        Raw<T, V> g[U], k[SAVED ? 1 : U];
+        Raw<int8_t, V> c[SAVED ? U : 1];
+        int e[U];
 #pragma unroll
-        for (int j = 0; j < L::V; ++j) g[j] = __fmul_rn(g[j], v[j]);
-        L::store(dx + row * lddx + c0, lane, left, g);
+        for (int u = 0; u < U; ++u, pg += dg) {
+            const bool live = row + u * w.step < a.rows;
+            g[u] = l.load(pg, live);
+            if (SAVED) {
+                c[SAVED ? u : 0] = l.load_codes(pc, live);
+                e[u] = live ? *pe : 0;
+                pc += dc;
+                pe += de;
+            } else {
+                k[SAVED ? 0 : u] = l.load(px, live);
+                px += dX;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u, po += dout) {
+            if (row + u * w.step >= a.rows) break;
+            float v[V], d[V];
+            if (SAVED) L::values(c[SAVED ? u : 0], e[u], v);
+            else widen(k[SAVED ? 0 : u], v);
+            act_slope<sizeof(T) == 2, ACT>(v, a.act, a.alpha);
+            widen(g[u], d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) d[j] = __fmul_rn(d[j], v[j]);
+            l.store(po, d);
+        }
     }
 }
 
-unsigned grid_for(int64_t units, int per_block) {
-    const int64_t want = ceil_div(units, per_block);
-    return static_cast<unsigned>(std::min<int64_t>(want, int64_t(num_sms()) * 8));
+// Blocks of 256 threads for rows x nb groups of G lanes: all at once when
+// they fit, else three a SM (and one group for every column block).
+unsigned grid_for(int64_t rows, int64_t nb, int G) {
+    const int per = 256 / G;
+    const int64_t want = ceil_div(rows * nb, per), most = std::max<int64_t>(ceil_div(nb, per), int64_t(num_sms()) * 3);
+    return static_cast<unsigned>(std::min(want, most));
 }
 
 template <class T>
@@ -174,9 +239,10 @@ TG_API tg_status tg_save8(int64_t rows, int64_t cols, int32_t dtype, const void*
             const T* xp = static_cast<const T*>(x);
             T* yp = static_cast<T*>(y);
             const bool al = aligned<T>(x, ldx) && aligned<T>(y, ldy);
-            auto kern = al ? save8_kernel<T, true> : save8_kernel<T, false>;
-            const int per = 256 / (al ? Lanes<T, true>::G : Lanes<T, false>::G);
-            launch("save8", kern, dim3(grid_for(rows * a.nb, per)), dim3(256), 0, as_stream(stream), a, xp, ldx, yp,
+            auto kern = save8_kernel<T, false, -1>;
+            if (al) by_act(act, [&](auto k) { kern = save8_kernel<T, true, decltype(k)::value>; });
+            const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
+            launch("save8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, xp, ldx, yp,
                    ldy, o);
         });
     });
@@ -200,8 +266,8 @@ TG_API tg_status tg_restore8(int64_t rows, int64_t cols, const int8_t* codes, in
             using T = decltype(t);
             const bool al = aligned<T>(y, ldy);
             auto kern = al ? restore8_kernel<T, true> : restore8_kernel<T, false>;
-            const int per = 256 / (al ? Lanes<T, true>::G : Lanes<T, false>::G);
-            launch("restore8", kern, dim3(grid_for(rows * a.nb, per)), dim3(256), 0, as_stream(stream), a, s,
+            const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
+            launch("restore8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, s,
                    static_cast<T*>(y), ldy);
         });
     });
@@ -234,10 +300,14 @@ TG_API tg_status tg_activation_grad(int64_t rows, int64_t cols, int32_t dtype, c
             const T* xp = static_cast<const T*>(x);
             T* dxp = static_cast<T*>(dx);
             const bool al = aligned<T>(dy, lddy) && aligned<T>(x, ldx) && aligned<T>(dx, lddx);
-            auto kern = codes ? (al ? act_grad_kernel<T, true, true> : act_grad_kernel<T, false, true>)
-                              : (al ? act_grad_kernel<T, true, false> : act_grad_kernel<T, false, false>);
-            const int per = 256 / (al ? Lanes<T, true>::G : Lanes<T, false>::G);
-            launch("activation_grad", kern, dim3(grid_for(rows * a.nb, per)), dim3(256), 0, as_stream(stream), a, dyp,
+            auto kern = codes ? act_grad_kernel<T, false, true, -1> : act_grad_kernel<T, false, false, -1>;
+            if (al)
+                by_act(act, [&](auto k) {
+                    constexpr int A = decltype(k)::value;
+                    kern = codes ? act_grad_kernel<T, true, true, A> : act_grad_kernel<T, true, false, A>;
+                });
+            const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
+            launch("activation_grad", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, dyp,
                    lddy, xp, ldx, s, dxp, lddx);
         });
     });

@@ -20,23 +20,95 @@ namespace tg {
 
 namespace {
 
-// db of one type (blockIdx.y), 32 columns of it.
-template <class T, class O>
-__global__ void __launch_bounds__(256) typed_bias_kernel(WeightArgs<T, O> g) {
+// ── db ───────────────────────────────────────────────────────────────────
+// Column sums of each type's rows, in two steps of fixed order: chunks of
+// kChunk rows of one type (8 warps, a row each; the warps joined through
+// shared memory), then a type's chunks.  One read of dY: bound by HBM.
+constexpr int kChunk = 256;
+
+// Columns of a warp: 16 bytes a lane when rows are aligned, else 4 columns a
+// lane, 32 apart.
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(256) typed_bias_kernel(int64_t M, int64_t N, int types, const int32_t* offsets,
+                                                         const T* dY, int64_t lddy, float* part) {
+    constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
+    __shared__ int prefix[kMaxTypes + 1];
+    __shared__ float sh[8][32 * V];
+    const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+    if (w == 0) scan_types(offsets, types, M, kChunk, prefix);
+    __syncthreads();
+    const int p = blockIdx.x;
+    if (p >= prefix[types]) return;
+    const int t = find_type(prefix, types, p);
+    const int64_t r0 = clamp_row(offsets[t], M) + static_cast<int64_t>(p - prefix[t]) * kChunk;
+    const int64_t e = clamp_row(offsets[t + 1], M), r1 = r0 + kChunk < e ? r0 + kChunk : e;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.y) * 32 * V;
+    float sum[V] = {};
+    const auto col = [&](int j) { return n0 + (ALIGNED ? lane * V + j : j * 32 + lane); };
+    if (ALIGNED && col(0) + V <= N) {
+        const T* q = dY + col(0);
+#pragma unroll 8
+        for (int64_t r = r0 + w; r < r1; r += 8) {
+            float x[V];
+            load_v<T, V>(q + r * lddy, x);
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += x[j];
+        }
+    } else {
+#pragma unroll 4
+        for (int64_t r = r0 + w; r < r1; r += 8)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (col(j) < N) sum[j] += to_f32(dY[r * lddy + col(j)]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sh[w][j * 32 + lane] = sum[j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * V; c += 256) {
+        float all = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) all += sh[q][c];
+        const int64_t n = n0 + (ALIGNED ? c % 32 * V + c / 32 : c);
+        if (n < N) part[p * N + n] = all;
+    }
+}
+
+__global__ void __launch_bounds__(256) typed_bias_join_kernel(int64_t M, int64_t N, const int32_t* offsets,
+                                                              const float* part, float* db) {
+    __shared__ int prefix[kMaxTypes + 1];
     __shared__ float sh[8][33];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32, t = blockIdx.y;
-    const int64_t b = clamp_row(g.offsets[t], g.M), e = clamp_row(g.offsets[t + 1], g.M);
+    if (w == 0) scan_types(offsets, t + 1, M, kChunk, prefix);
+    __syncthreads();
     const int64_t n = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float sum = 0.0f;
-    if (n < g.N)
-        for (int64_t r = b + w; r < e; r += 8) sum += to_f32(g.dY[r * g.lddy + n]);
+    if (n < N) {
+#pragma unroll 4
+        for (int p = prefix[t] + w; p < prefix[t + 1]; p += 8) sum += part[p * N + n];
+    }
     sh[w][lane] = sum;
     __syncthreads();
-    if (w == 0 && n < g.N) {
+    if (w == 0 && n < N) {
         sum = 0.0f;
+#pragma unroll
         for (int q = 0; q < 8; ++q) sum += sh[q][lane];
-        g.db[t * g.N + n] = sum;
+        db[t * N + n] = sum;
     }
+}
+
+template <class T>
+void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T* dY, int64_t lddy, float* db,
+                cudaStream_t s) {
+    const int64_t chunks = M / kChunk + std::min<int64_t>(types, M);
+    Scratch<float> part(static_cast<size_t>(chunks * N), s);
+    const bool al = rows_aligned16(dY, lddy, sizeof(T));
+    const int64_t tile = al ? 32 * (16 / static_cast<int64_t>(sizeof(T))) : 128;
+    launch("typed_linear_grad_bias", al ? typed_bias_kernel<T, true> : typed_bias_kernel<T, false>,
+           dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(N, tile))), dim3(256), 0, s, M, N, types,
+           offsets, dY, lddy, part.p);
+    launch("typed_linear_grad_bias", typed_bias_join_kernel,
+           dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0, s, M, N, offsets,
+           part.p, db);
 }
 
 void check_typed(const char* fn, int64_t M, int64_t K, int64_t N, int64_t types, int dtype, const int32_t* offsets) {
@@ -140,13 +212,11 @@ TG_API tg_status tg_typed_linear_grad_weight(int64_t rows, int64_t K, int64_t N,
             using T = decltype(t);
             using O = decltype(o);
             const WeightArgs<T, O> g{rows, K, N, static_cast<int>(types), static_cast<const T*>(X), ldx, s,
-                                     static_cast<const T*>(dY), lddy, offsets, static_cast<O*>(dW), lddw, stride_dw,
-                                     db};
+                                     static_cast<const T*>(dY), lddy, offsets, static_cast<O*>(dW), lddw, stride_dw};
             typed_weight_tc<T, O>(g, as_stream(stream));
             if (db)
-                launch("typed_linear_grad_bias", typed_bias_kernel<T, O>,
-                       dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0,
-                       as_stream(stream), g);
+                typed_bias<T>(rows, N, static_cast<int>(types), offsets, static_cast<const T*>(dY), lddy, db,
+                              as_stream(stream));
         };
         by_dtype(dtype, [&](auto t) {
             if (dw_dtype == TG_F32) run(t, float{});

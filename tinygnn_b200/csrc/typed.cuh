@@ -14,6 +14,39 @@ __device__ __forceinline__ int clamp_row(int r, int64_t M) {
     return r < 0 ? 0 : (r > M ? static_cast<int>(M) : r);
 }
 
+// prefix[t] = number of pieces of `per` rows in the types before t (one warp).
+__device__ __forceinline__ void scan_types(const int32_t* offsets, int types, int64_t M, int64_t per, int* prefix) {
+    const int lane = threadIdx.x & 31;
+    int carry = 0;
+    if (lane == 0) prefix[0] = 0;
+    for (int t0 = 0; t0 < types; t0 += 32) {
+        const int t = t0 + lane;
+        int n = 0;
+        if (t < types) {
+            const int b = clamp_row(offsets[t], M), e = clamp_row(offsets[t + 1], M);
+            n = e > b ? static_cast<int>((e - b + per - 1) / per) : 0;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) n += up;
+        }
+        if (t < types) prefix[t + 1] = carry + n;
+        carry += __shfl_sync(0xffffffffu, n, 31);
+    }
+}
+
+// The type that piece p belongs to: the last t with prefix[t] <= p.
+__device__ __forceinline__ int find_type(const int* prefix, int types, int p) {
+    int lo = 0, hi = types;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (prefix[mid] <= p) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
 // C[r] = act(A[r] . B[t(r)] + bias[t(r)]), rows of A are K wide; B is W[t]
 // (K x N) in the forward pass and W[t]^T (W[t]: N x K) in the input gradient.
 template <class T>
@@ -48,7 +81,6 @@ struct WeightArgs {
     const int32_t* offsets;
     O* dW;
     int64_t lddw, stride_dw;
-    float* db;  // types x N, nullable
 };
 
 // On the tensor cores (typed_tc.cu).

@@ -59,39 +59,6 @@ struct Shared {
     int prefix[kMaxTypes + 1];
 };
 
-// prefix[t] = number of pieces of `per` rows in the types before t (one warp).
-__device__ __forceinline__ void scan_types(const int32_t* offsets, int types, int64_t M, int64_t per, int* prefix) {
-    const int lane = threadIdx.x & 31;
-    int carry = 0;
-    if (lane == 0) prefix[0] = 0;
-    for (int t0 = 0; t0 < types; t0 += 32) {
-        const int t = t0 + lane;
-        int n = 0;
-        if (t < types) {
-            const int b = clamp_row(offsets[t], M), e = clamp_row(offsets[t + 1], M);
-            n = e > b ? static_cast<int>((e - b + per - 1) / per) : 0;
-        }
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, n, o);
-            if (lane >= o) n += up;
-        }
-        if (t < types) prefix[t + 1] = carry + n;
-        carry += __shfl_sync(0xffffffffu, n, 31);
-    }
-}
-
-// The type that piece p belongs to: the last t with prefix[t] <= p.
-__device__ __forceinline__ int find_type(const int* prefix, int types, int p) {
-    int lo = 0, hi = types;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (prefix[mid] <= p) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
 // The MMAs of one stage: every plane product i + j <= 2, smallest first.
 template <int PA, int PB, int BN, bool A_OUTER, bool B_OUTER>
 __device__ __forceinline__ void stage_mmas(uint32_t stage, uint32_t acc, uint32_t id, bool first) {
@@ -121,10 +88,9 @@ __device__ __forceinline__ void store32(O* p, const float (&v)[32], int64_t left
 #pragma unroll
     for (int c = 0; c < 32; c += W) {
         if (mode > 0 && c + W <= left) {
-            Pack<O, W> k;
-#pragma unroll
-            for (int j = 0; j < W; ++j) k.v[j] = from_f32<O>(v[c + j]);
-            const uint32_t* r = reinterpret_cast<const uint32_t*>(&k);
+            Raw<O, W> k;
+            narrow(v + c, k);
+            const uint32_t* r = k.w;
             if (mode == 2) {
                 asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + c), "r"(r[0]),
                              "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -313,13 +279,13 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
                 int byte = 0;
                 float inv = 0.0f;
                 if (g.saved.codes) {  // the block's exponent needs all its columns first
-                    uint32_t m = 0;
+                    float m = 0.0f;
 #pragma unroll 1
                     for (int c0 = b0; c0 < b0 + W; c0 += 32) {
                         float v[32];
                         load_biased(addr + c0, g, t, n0 + c0, v);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) m = max(m, mag_bits(v[j]));
+                        for (int j = 0; j < 32; ++j) m = max_mag(m, v[j]);
                     }
                     byte = exponent8(m, g.r8.emin);
                     inv = encode8(byte);
@@ -331,22 +297,19 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
                     load_biased(addr + c0, g, t, n0 + c0, v);
                     const int64_t left = live ? g.N - n0 - c0 : 0;
                     if (g.saved.codes && left > 0) {
-                        Pack<int8_t, 16> k[2];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) k[j / 16].v[j % 16] = code8(v[j], inv, byte, g.r8.top);
                         int8_t* o = g.saved.codes + row * g.saved.ld + n0 + c0;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (16 * h + 16 <= left) {
-                                *reinterpret_cast<Pack<int8_t, 16>*>(o + 16 * h) = k[h];
+                        for (int h = 0; h < 32; h += 16) {
+                            if (h + 16 <= left) {
+                                store_codes<16>(o + h, v + h, inv, byte, g.r8.top);
                             } else {
 #pragma unroll
                                 for (int j = 0; j < 16; ++j)
-                                    if (16 * h + j < left) o[16 * h + j] = k[h].v[j];
+                                    if (h + j < left) o[h + j] = code8(v[h + j], inv, byte, g.r8.top);
                             }
                         }
                     }
-                    act_forward(v, g.act, g.alpha);
+                    act_forward<(P == 1)>(v, g.act, g.alpha);
                     store32(c + c0, v, left, g.mode);
                 }
             }
@@ -543,19 +506,20 @@ __global__ void __launch_bounds__(256) planes_kernel(int64_t rows, int64_t cols,
         for (int j = 0; j < 8; ++j) x[j] = c + j < cols ? to_f32(p[j]) : 0.0f;
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-            Pack<H, 8> k;
+            Raw<H, 8> k;
+            narrow(x, k);
+            if (P > 1) {
+                float top[8];
+                widen(k, top);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                k.v[j] = from_f32<H>(x[j]);
-                if (P > 1) {
+                for (int j = 0; j < 8; ++j) {
                     // a finite value above bf16's greatest rounds to infinity: take the greatest
-                    const float top = to_f32(k.v[j]);
-                    if (fabsf(top) > 3.4e38f && fabsf(x[j]) <= 3.4028235e38f)
-                        k.v[j] = from_f32<H>(copysignf(3.3895314e38f, x[j]));
-                    x[j] = __fsub_rn(x[j], to_f32(k.v[j]));
+                    if (isinf(top[j]) && !isinf(x[j])) top[j] = copysignf(3.3895314e38f, x[j]);
+                    x[j] = __fsub_rn(x[j], top[j]);
                 }
+                narrow(top, k);
             }
-            *reinterpret_cast<Pack<H, 8>*>(dst + (q * rows + r) * ld + c) = k;
+            *reinterpret_cast<Raw<H, 8>*>(dst + (q * rows + r) * ld + c) = k;
         }
     }
 }
@@ -567,11 +531,11 @@ __global__ void __launch_bounds__(256) saved_plane_kernel(int64_t rows, int64_t 
     for (int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; v < total;
          v += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = v / vecs, c = (v - r * vecs) * 8;
-        const float scale = decode8(s.exps[r * s.lde + c / kBlock8]);
-        const Pack<int8_t, 8> in = *reinterpret_cast<const Pack<int8_t, 8>*>(s.codes + r * s.ld + c);
+        const int byte = s.exps[r * s.lde + c / kBlock8];
+        const uint2 in = *reinterpret_cast<const uint2*>(s.codes + r * s.ld + c);
         float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = c + j < cols ? __fmul_rn(static_cast<float>(in.v[j]), scale) : 0.0f;
+        values4(in.x, byte, x);
+        values4(in.y, byte, x + 4);
         store_v<H, 8>(dst + r * ld + c, x);
     }
 }
@@ -656,7 +620,7 @@ void run_tc(const char* name, K kern, uint32_t smem, int64_t tiles, cudaStream_t
 template <class O>
 void join_pieces(const WeightTc<O>& g, int types, cudaStream_t s) {
     launch("typed_weight_join", typed_weight_join_kernel<O>,
-           dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(g.K * g.ldp / 4, 256), 64)),
+           dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(g.K * g.ldp / 4, 256), std::max(8, 16384 / types))),
                 static_cast<unsigned>(types)),
            dim3(256), 0, s, g);
 }

@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "launch.cuh"
 
 namespace tg {
@@ -48,33 +50,115 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
-// V consecutive values at p (aligned to V * sizeof(T)) to and from fp32.
+// V values as they lie in memory, in 32-bit words: where a kernel has a vector
+// load and an elementwise one for edges, 16-bit values kept one by one would
+// each take a register of their own (and an instruction to unpack).
 template <class T, int V>
-struct alignas(V * sizeof(T)) Pack {
-    T v[V];
+struct alignas(V * sizeof(T)) Raw {
+    static constexpr int N = V * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[N];
 };
+__device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ uint32_t bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+__device__ __forceinline__ uint32_t bits(__half x) { return __half_as_ushort(x); }
+
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p) {  // aligned to V * sizeof(T)
+    return *reinterpret_cast<const Raw<T, V>*>(p);
+}
+template <class T, int V, class F>  // value j = f(j)
+__device__ __forceinline__ Raw<T, V> gather_raw(F&& f) {
+    Raw<T, V> k;
+#pragma unroll
+    for (int i = 0; i < Raw<T, V>::N; ++i) {
+        if (sizeof(T) == 4) k.w[i] = bits(f(i));
+        else k.w[i] = bits(f(2 * i)) | bits(f(2 * i + 1)) << 16;
+    }
+    return k;
+}
+template <class T, int V, class F>  // f(j, value j)
+__device__ __forceinline__ void scatter_raw(const Raw<T, V>& k, F&& f) {
+    const T* v = reinterpret_cast<const T*>(k.w);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f(j, v[j]);
+}
+template <int V>
+__device__ __forceinline__ void widen(const Raw<float, V>& k, float* x) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = __uint_as_float(k.w[j]);
+}
+template <int V>
+__device__ __forceinline__ void widen(const Raw<__nv_bfloat16, V>& k, float* x) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+        x[j] = __uint_as_float(k.w[j / 2] << 16);
+        x[j + 1] = __uint_as_float(k.w[j / 2] & 0xffff0000u);
+    }
+}
+template <int V>
+__device__ __forceinline__ void widen(const Raw<__half, V>& k, float* x) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&k.w[j / 2]));
+        x[j] = t.x;
+        x[j + 1] = t.y;
+    }
+}
+// Rounded to T, two values an instruction where T has 16 bits.
+template <int V>
+__device__ __forceinline__ void narrow(const float* x, Raw<float, V>& k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) k.w[j] = __float_as_uint(x[j]);
+}
+template <int V>
+__device__ __forceinline__ void narrow(const float* x, Raw<__nv_bfloat16, V>& k) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(x[j], x[j + 1]);
+        k.w[j / 2] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+}
+template <int V>
+__device__ __forceinline__ void narrow(const float* x, Raw<__half, V>& k) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+        const __half2 t = __floats2half2_rn(x[j], x[j + 1]);
+        k.w[j / 2] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+}
 template <class T, int V>
 __device__ __forceinline__ void load_v(const T* p, float (&x)[V]) {
-    const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = to_f32(k.v[j]);
+    widen(load_raw<T, V>(p), x);
 }
 template <class T, int V>
 __device__ __forceinline__ void store_v(T* p, const float (&x)[V]) {
-    Pack<T, V> k;
-#pragma unroll
-    for (int j = 0; j < V; ++j) k.v[j] = from_f32<T>(x[j]);
-    *reinterpret_cast<Pack<T, V>*>(p) = k;
+    Raw<T, V> k;
+    narrow(x, k);
+    *reinterpret_cast<Raw<T, V>*>(p) = k;
 }
 
-// Magnitudes are compared as bit patterns: they order like the values, with
-// infinity above every number and NaN above infinity (fmaxf would drop NaN).
-__device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// max(a, |b|) that keeps a NaN (fmaxf drops it).
+__device__ __forceinline__ float max_mag(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
-// The exponent byte of a block whose largest magnitude has bits `m`.  127 is
+// The exponent byte of a block whose largest magnitude is `most`.  127 is
 // 1.984375 * 2^6, so e is the exponent of max|x| less 6, or one more when its
 // mantissa is above 1.984375.
-__device__ __forceinline__ int exponent8(uint32_t m, int emin) {
+__device__ __forceinline__ int exponent8(float most, int emin) {
+    const uint32_t m = __float_as_uint(most);
     if (m >= 0x7f800000u) return kBad8;
     const int e = static_cast<int>(m >> 23) - 133 + ((m & 0x7fffffu) > 0x7e0000u ? 1 : 0);
     return (e > emin ? e : emin) + 127;
@@ -86,12 +170,62 @@ __device__ __forceinline__ float encode8(int byte) { return byte == kBad8 ? 0.0f
 __device__ __forceinline__ float decode8(int byte) {
     return byte == kBad8 ? __uint_as_float(0x7fffffffu) : pow2f(byte - 127);
 }
-// The code of x (inv = encode8(byte); an infinity or NaN times 0 is NaN, which
-// converts to 0).  At the type's greatest exponent 64 * 2^e would overflow it.
+// Four codes as one word (inv = encode8(byte)).  x * inv + 1.5 * 2^23 rounds
+// x * inv to the nearest integer, ties to even, and leaves its two's
+// complement in the low bits: one FMA a value where a conversion instruction
+// runs at an eighth of that rate.  At the type's greatest exponent 64 * 2^e
+// would overflow it.
+__device__ __forceinline__ uint32_t codes4(float x0, float x1, float x2, float x3, float inv, int byte, int top) {
+    constexpr float kMagic = 12582912.0f;
+    float r[4] = {x0, x1, x2, x3};
+    if (byte == top) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = __fmul_rn(fminf(fmaxf(__fmul_rn(r[j], inv), -63.0f), 63.0f), pow2f(byte - 127));
+    }
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = __float_as_uint(fmaf(r[j], inv, kMagic));
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+}
 __device__ __forceinline__ int8_t code8(float x, float inv, int byte, int top) {
-    int c = __float2int_rn(__fmul_rn(x, inv));
-    if (byte == top) c = c > 63 ? 63 : (c < -63 ? -63 : c);
-    return static_cast<int8_t>(c);
+    return static_cast<int8_t>(codes4(x, x, x, x, inv, byte, top) & 0xff);
+}
+// The values of four codes: the byte b + 128 in the mantissa of 2^23, less
+// 2^23 + 128, is b; the product with 2^e is exact, so one FMA does both
+// (beyond 2^100 its addend would overflow).
+__device__ __forceinline__ void values4(uint32_t codes, int byte, float* x) {
+    const uint32_t u = codes ^ 0x80808080u;
+    const float scale = decode8(byte);
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + j));
+    if (byte <= 227) {
+        const float off = __fmul_rn(-8388736.0f, scale);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(f[j], scale, off);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __fmul_rn(__fsub_rn(f[j], 8388736.0f), scale);
+    }
+}
+// V codes (a multiple of 4), f(j) the byte j.
+template <int V, class F>
+__device__ __forceinline__ Raw<int8_t, V> gather_codes(F&& f) {
+    Raw<int8_t, V> k;
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        const auto byte = [&](int j) { return static_cast<uint32_t>(static_cast<uint8_t>(f(4 * i + j))); };
+        k.w[i] = byte(0) | byte(1) << 8 | byte(2) << 16 | byte(3) << 24;
+    }
+    return k;
+}
+// V codes at p, aligned to V bytes.
+template <int V>
+__device__ __forceinline__ void store_codes(int8_t* p, const float* x, float inv, int byte, int top) {
+    Raw<int8_t, V> k;
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) k.w[j] = codes4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3], inv, byte, top);
+    *reinterpret_cast<Raw<int8_t, V>*>(p) = k;
 }
 
 // The least exponent of a block: 2^-126, or 2^-24 for fp16 matrices, whose
@@ -110,9 +244,9 @@ __device__ __forceinline__ T reduce_sum(T x) {
     return x;
 }
 template <int W>
-__device__ __forceinline__ uint32_t reduce_max(uint32_t x) {
+__device__ __forceinline__ float reduce_max(float x) {
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+    for (int o = W / 2; o > 0; o >>= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, o));
     return x;
 }
 
@@ -128,12 +262,31 @@ struct Saved8 {
 // ── Activations and their slopes ─────────────────────────────────────────
 // The choice is made once for V values.  GELU's 1/2 (1 + tanh u) is computed
 // as 1 / (1 + e^-2u), which equals it, does not cancel where tanh u is near
-// -1, and costs one exponential and one reciprocal: with tanhf the 8-bit
-// activation passes are bound by arithmetic instead of memory.
-__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.0f, __fadd_rn(1.0f, expf(-x))); }
+// -1, and costs one exponential and one reciprocal.  FAST (for results of 16
+// bits) takes the hardware's exponential, whose error of 2^-19 or less here
+// is lost in the result's rounding of 2^-8 or 2^-11; with tanhf the 8-bit
+// activation passes were bound by arithmetic (0.52 ms for 131,072 x 1024
+// bf16, forward and backward).
+template <bool FAST>
+__device__ __forceinline__ float exp_f(float x) { return FAST ? __expf(x) : expf(x); }
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));  // 1 ulp; 1 / inf = 0
+    return r;
+}
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_f(float x) { return reciprocal(__fadd_rn(1.0f, exp_f<FAST>(-x))); }
 
-__device__ __forceinline__ float gelu_u(float x, float x2) {  // c (x + d x^3), c = sqrt(2 / pi)
-    return __fmul_rn(0.7978845608f, fmaf(__fmul_rn(0.044715f, x2), x, x));
+// 1 / (1 + e^-2u), 2u = 2 c (x + d x^3), c = sqrt(2 / pi), d = 0.044715; the
+// fast form takes 2^(-2u log2 e) with the factor in the constants.
+template <bool FAST>
+__device__ __forceinline__ float gelu_s(float x, float x2) {
+    if (FAST) {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(x, fmaf(-0.102943239f, x2, -2.302208198f))));
+        return reciprocal(__fadd_rn(1.0f, e));
+    }
+    return sigmoid_f<false>(__fmul_rn(x, fmaf(0.0713548162726f, x2, 1.5957691216f)));
 }
 
 template <int V, class F>
@@ -143,20 +296,22 @@ __device__ __forceinline__ void map_v(float (&x)[V], F&& f) {
 }
 
 // x <- act(x)
-template <int V>
+// ACT is the activation where it is known at compile time, else -1.
+template <bool FAST, int ACT = -1, int V>
 __device__ __forceinline__ void act_forward(float (&x)[V], int act, float alpha) {
-    switch (act) {
+    switch (ACT >= 0 ? ACT : act) {
         case TG_ACT_RELU: map_v(x, [](float v) { return v < 0.0f ? 0.0f : v; }); break;  // NaN stays NaN
         case TG_ACT_LEAKY_RELU: map_v(x, [alpha](float v) { return v >= 0.0f ? v : __fmul_rn(alpha, v); }); break;
         case TG_ACT_ELU:
-            map_v(x, [alpha](float v) { return v < 0.0f ? __fmul_rn(alpha, __fsub_rn(expf(v), 1.0f)) : v; });
+            map_v(x, [alpha](float v) { return v < 0.0f ? __fmul_rn(alpha, __fsub_rn(exp_f<FAST>(v), 1.0f)) : v; });
             break;
-        case TG_ACT_SIGMOID: map_v(x, [](float v) { return sigmoid_f(v); }); break;
+        case TG_ACT_SIGMOID: map_v(x, [](float v) { return sigmoid_f<FAST>(v); }); break;
         case TG_ACT_TANH: map_v(x, [](float v) { return tanhf(v); }); break;
         case TG_ACT_GELU:
+            // below -16 the product is 0 in fp32 (and -inf * 0 would not be)
             map_v(x, [](float v) {
-                const float s = sigmoid_f(__fmul_rn(2.0f, gelu_u(v, __fmul_rn(v, v))));
-                return s == 0.0f ? 0.0f : __fmul_rn(v, s);  // -inf: 0, not -inf * 0
+                v = max_nan(v, -16.0f);
+                return __fmul_rn(v, gelu_s<FAST>(v, __fmul_rn(v, v)));
             });
             break;
         default: break;
@@ -164,19 +319,19 @@ __device__ __forceinline__ void act_forward(float (&x)[V], int act, float alpha)
 }
 
 // x <- act'(x)
-template <int V>
+template <bool FAST, int ACT = -1, int V>
 __device__ __forceinline__ void act_slope(float (&x)[V], int act, float alpha) {
-    switch (act) {
+    switch (ACT >= 0 ? ACT : act) {
         case TG_ACT_RELU: map_v(x, [](float v) { return v > 0.0f ? 1.0f : (v <= 0.0f ? 0.0f : v); }); break;
         case TG_ACT_LEAKY_RELU:
             map_v(x, [alpha](float v) { return v >= 0.0f ? 1.0f : (v < 0.0f ? alpha : v); });
             break;
         case TG_ACT_ELU:
-            map_v(x, [alpha](float v) { return v < 0.0f ? __fmul_rn(alpha, expf(v)) : (v >= 0.0f ? 1.0f : v); });
+            map_v(x, [alpha](float v) { return v < 0.0f ? __fmul_rn(alpha, exp_f<FAST>(v)) : (v >= 0.0f ? 1.0f : v); });
             break;
         case TG_ACT_SIGMOID:
             map_v(x, [](float v) {
-                const float s = sigmoid_f(v);
+                const float s = sigmoid_f<FAST>(v);
                 return __fmul_rn(s, __fsub_rn(1.0f, s));
             });
             break;
@@ -187,17 +342,32 @@ __device__ __forceinline__ void act_slope(float (&x)[V], int act, float alpha) {
             });
             break;
         case TG_ACT_GELU:
-            // s = 1 / (1 + e^-2u): act' = s + 2 x s (1 - s) u',  u' = c (1 + 3 d x^2).
-            // Beyond |x| = 16 s is 0 or 1 in fp32, and u' may overflow.
+            // s = 1 / (1 + e^-2u): act' = s + x s (1 - s) (2u)',  (2u)' = 2 c (1 + 3 d x^2).
+            // Beyond |x| = 16 s is 0 or 1 in fp32, and (2u)' may overflow.
             map_v(x, [](float v) {
-                if (fabsf(v) > 16.0f) return v > 0.0f ? 1.0f : 0.0f;
+                v = min_nan(max_nan(v, -16.0f), 16.0f);
                 const float v2 = __fmul_rn(v, v);
-                const float s = sigmoid_f(__fmul_rn(2.0f, gelu_u(v, v2)));
-                const float du = __fmul_rn(0.7978845608f, fmaf(0.134145f, v2, 1.0f));
-                return fmaf(__fmul_rn(__fmul_rn(2.0f, v), __fmul_rn(s, __fsub_rn(1.0f, s))), du, s);
+                const float s = gelu_s<FAST>(v, v2);
+                const float du = fmaf(0.2140644488f, v2, 1.5957691216f);
+                return fmaf(__fmul_rn(v, fmaf(-s, s, s)), du, s);
             });
             break;
         default: map_v(x, [](float) { return 1.0f; }); break;
+    }
+}
+
+// Calls f with the activation as a compile-time constant.
+template <class F>
+void by_act(int act, F&& f) {
+    using std::integral_constant;
+    switch (act) {
+        case TG_ACT_RELU: f(integral_constant<int, TG_ACT_RELU>{}); break;
+        case TG_ACT_ELU: f(integral_constant<int, TG_ACT_ELU>{}); break;
+        case TG_ACT_LEAKY_RELU: f(integral_constant<int, TG_ACT_LEAKY_RELU>{}); break;
+        case TG_ACT_SIGMOID: f(integral_constant<int, TG_ACT_SIGMOID>{}); break;
+        case TG_ACT_TANH: f(integral_constant<int, TG_ACT_TANH>{}); break;
+        case TG_ACT_GELU: f(integral_constant<int, TG_ACT_GELU>{}); break;
+        default: f(integral_constant<int, TG_ACT_NONE>{});
     }
 }
 

@@ -42,19 +42,24 @@ def _matrix(t: torch.Tensor, fn: str, name: str, dtype=None, shape=None) -> torc
     if t.shape[1] < 1:
         raise _bad(f"{fn}: {name} has no columns")
     # Rows that overlap or run backwards (an expanded row) are laid out first.
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+    if not t.is_contiguous() and ((t.stride(1) != 1 and t.shape[1] > 1)
+                                  or (t.stride(0) < t.shape[1] and t.shape[0] > 1)):
         t = t.contiguous()
     return t
 
 
 def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    ld, cols = t.stride(0), t.shape[1]
+    return ld if ld >= cols else cols  # the stride of a single row is arbitrary
 
 
 def _stream(t: torch.Tensor) -> int:
-    if t.device.index != torch.cuda.current_device():
+    """The current stream's handle, by the calls under torch.cuda.current_stream
+    (which builds two objects a call: 7 us of a small operator's 20)."""
+    dev = t.get_device()
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"the tensors are on {t.device}, which is not the current CUDA device")
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _act(fn: str, act) -> int:
@@ -64,8 +69,9 @@ def _act(fn: str, act) -> int:
 
 
 def _same_device(fn: str, a: torch.Tensor, *others) -> None:
+    dev = a.get_device()
     for t in others:
-        if t is not None and t.device != a.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{fn}: tensors on {a.device} and {t.device}")
 
 
@@ -180,7 +186,7 @@ def _param(t: torch.Tensor, fn: str, name: str, dtype, cols: int) -> torch.Tenso
         raise _bad(f"{fn}: {name} must have {cols} elements, got {t.numel()}")
     if not t.is_cuda or t.dtype not in (torch.float32, dtype):
         raise ValueError(f"{fn}: {name} must be a float32 or {dtype} CUDA tensor")
-    return t.reshape(-1).contiguous()
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
 def layer_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, eps: float = 1e-5, save8: bool = False):
@@ -216,8 +222,8 @@ def layer_norm_backward(dy: torch.Tensor, saved: Union[torch.Tensor, Saved8], st
         raise _bad(f"{fn}: stats must be a contiguous float32 tensor of shape ({rows}, 2)")
     _same_device(fn, dy, gamma, stats, saved.codes if isinstance(saved, Saved8) else saved)
     dx = torch.empty((rows, cols), dtype=dy.dtype, device=dy.device)
-    dparams = torch.empty((2, cols), dtype=gamma.dtype, device=dy.device)
-    dgamma, dbeta = dparams[0], dparams[1]
+    dgamma = torch.empty((cols,), dtype=gamma.dtype, device=dy.device)
+    dbeta = torch.empty((cols,), dtype=gamma.dtype, device=dy.device)
     check(lib.tg_layer_norm_grad(rows, cols, DTYPE[dy.dtype], dy.data_ptr(), _ld(dy), *sargs, stats.data_ptr(),
                                  DTYPE[gamma.dtype], gamma.data_ptr(), dx.data_ptr(), _ld(dx), dgamma.data_ptr(),
                                  dbeta.data_ptr(), _stream(dy)))
