@@ -96,21 +96,6 @@ __global__ void __launch_bounds__(256) typed_bias_join_kernel(int64_t M, int64_t
     }
 }
 
-template <class T>
-void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T* dY, int64_t lddy, float* db,
-                cudaStream_t s) {
-    const int64_t chunks = M / kChunk + std::min<int64_t>(types, M);
-    Scratch<float> part(static_cast<size_t>(chunks * N), s);
-    const bool al = rows_aligned16(dY, lddy, sizeof(T));
-    const int64_t tile = al ? 32 * (16 / static_cast<int64_t>(sizeof(T))) : 128;
-    launch("typed_linear_grad_bias", al ? typed_bias_kernel<T, true> : typed_bias_kernel<T, false>,
-           dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(N, tile))), dim3(256), 0, s, M, N, types,
-           offsets, dY, lddy, part.p);
-    launch("typed_linear_grad_bias", typed_bias_join_kernel,
-           dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0, s, M, N, offsets,
-           part.p, db);
-}
-
 void check_typed(const char* fn, int64_t M, int64_t K, int64_t N, int64_t types, int dtype, const int32_t* offsets) {
     check_rows_cols(fn, M, K);
     check_rows_cols(fn, M, N);
@@ -128,6 +113,25 @@ void check_weight(const char* fn, const char* what, int64_t K, int64_t N, int64_
 }
 
 }  // namespace
+
+template <class T>
+void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T* dY, int64_t lddy, float* db,
+                cudaStream_t s) {
+    const int64_t chunks = M / kChunk + std::min<int64_t>(types, M);
+    Scratch<float> part(static_cast<size_t>(chunks * N), s);
+    const bool al = rows_aligned16(dY, lddy, sizeof(T));
+    const int64_t tile = al ? 32 * (16 / static_cast<int64_t>(sizeof(T))) : 128;
+    launch("typed_linear_grad_bias", al ? typed_bias_kernel<T, true> : typed_bias_kernel<T, false>,
+           dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(N, tile))), dim3(256), 0, s, M, N, types,
+           offsets, dY, lddy, part.p);
+    launch("typed_linear_grad_bias", typed_bias_join_kernel,
+           dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0, s, M, N, offsets,
+           part.p, db);
+}
+
+template void typed_bias<__nv_bfloat16>(int64_t, int64_t, int, const int32_t*, const __nv_bfloat16*, int64_t, float*,
+                                        cudaStream_t);
+template void typed_bias<__half>(int64_t, int64_t, int, const int32_t*, const __half*, int64_t, float*, cudaStream_t);
 
 }  // namespace tg
 
@@ -157,7 +161,7 @@ TG_API tg_status tg_typed_linear(int64_t rows, int64_t K, int64_t N, int64_t typ
             const RowsArgs<T> g{rows, K, N, static_cast<int>(types), static_cast<const T*>(X), ldx,
                                 static_cast<const T*>(W), ldw, stride_w, offsets, bias, act, alpha,
                                 static_cast<T*>(Y), ldy, s, range8(dtype)};
-            typed_rows_tc<T, false>(g, as_stream(stream));
+            typed_rows<T, false>(g, as_stream(stream));
         });
     });
 }
@@ -182,7 +186,7 @@ TG_API tg_status tg_typed_linear_grad_input(int64_t rows, int64_t K, int64_t N, 
             const RowsArgs<T> g{rows, N, K, static_cast<int>(types), static_cast<const T*>(dY), lddy,
                                 static_cast<const T*>(W), ldw, stride_w, offsets, nullptr, TG_ACT_NONE, 0.0f,
                                 static_cast<T*>(dX), lddx, Saved8{}, Range8{}};
-            typed_rows_tc<T, true>(g, as_stream(stream));
+            typed_rows<T, true>(g, as_stream(stream));
         });
     });
 }
@@ -212,11 +216,9 @@ TG_API tg_status tg_typed_linear_grad_weight(int64_t rows, int64_t K, int64_t N,
             using T = decltype(t);
             using O = decltype(o);
             const WeightArgs<T, O> g{rows, K, N, static_cast<int>(types), static_cast<const T*>(X), ldx, s,
-                                     static_cast<const T*>(dY), lddy, offsets, static_cast<O*>(dW), lddw, stride_dw};
-            typed_weight_tc<T, O>(g, as_stream(stream));
-            if (db)
-                typed_bias<T>(rows, N, static_cast<int>(types), offsets, static_cast<const T*>(dY), lddy, db,
-                              as_stream(stream));
+                                     static_cast<const T*>(dY), lddy, offsets, static_cast<O*>(dW), lddw, stride_dw,
+                                     db};
+            typed_weight<T, O>(g, as_stream(stream));
         };
         by_dtype(dtype, [&](auto t) {
             if (dw_dtype == TG_F32) run(t, float{});

@@ -81,13 +81,38 @@ struct WeightArgs {
     const int32_t* offsets;
     O* dW;
     int64_t lddw, stride_dw;
+    float* db;  // types x N, nullable
 };
 
-// On the tensor cores (typed_tc.cu).
+// How a weight gradient is cut up: pieces of at most `piece` rows of a type,
+// each summed by one CTA per tile of dW; types of several pieces leave partial
+// sums [piece][K][ldp] (and [piece][N] of db) that a second kernel adds up in
+// their order.
+struct WeightPlan {
+    int BN;  // columns of a tile
+    int tiles_k, tiles_n;
+    int64_t piece, ldp, items;
+    float *part, *db_part;
+    bool dy_by_tma;  // typed_weight_any: dY by TMA, db not summed on the way
+};
+
+// TMA-fed kernels and the choice between them and the others (typed_tc.cu).
 template <class T, bool TRANS>
-void typed_rows_tc(const RowsArgs<T>& a, cudaStream_t s);
+void typed_rows(const RowsArgs<T>& a, cudaStream_t s);
 template <class T, class O>
-void typed_weight_tc(const WeightArgs<T, O>& a, cudaStream_t s);
-int typed_take_error();
+void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s);
+int typed_tc_take_error();
+
+// Loader-fed kernels (typed_any.cu).
+template <class T, bool TRANS>
+void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s);
+template <class T, class O>
+void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s);
+int typed_any_take_error();
+
+// db alone (typed.cu).
+template <class T>
+void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T* dY, int64_t lddy, float* db,
+                cudaStream_t s);
 
 }  // namespace tg

@@ -1,0 +1,535 @@
+// ============================================================================
+//  typed_any.cu -- the typed products on the tensor cores for operands of any
+//  type and alignment, converted on their way into shared memory.
+//
+//  TMA needs 16-byte aligned rows and copies values as they are.  Here eight
+//  loader warps read the operands with plain loads and write the MMA's 16-bit
+//  tiles themselves, so one launch takes
+//   fp32       each value split into three bf16 parts (24 bits, exactly):
+//              x0 = x's upper half, x1 = bf16(x - x0), x2 = bf16(x - x0 - x1);
+//              a product is the six part products x_i y_j with i + j <= 2
+//              (what is left out is below 2^-23 of it and of random sign).  An
+//              infinity in an fp32 operand gives NaN;
+//   bf16, fp16 with rows of any alignment;
+//   8 bits     code * 2^e as one bf16 or fp16 value, exactly;
+//  and rows past a type's end and columns past the matrix are zeros.  Where
+//  dY passes through the loaders, they add up db on the way.
+//
+//    warps 0-7    loaders: the next stage's values are in registers (in
+//                 flight) while this stage's are converted and written;
+//    warp 8       the MMAs (one thread);
+//    warp 9       TMA for the second operand, where its rows are aligned;
+//    warps 12-15  the epilogue of one of two TMEM accumulators while the next
+//                 tile is multiplied.
+// ============================================================================
+#include <type_traits>
+
+#include "typed_mma.cuh"
+
+namespace tg {
+
+namespace {
+
+using namespace typed;
+
+enum Op { kForward, kGradInput, kGradWeight };
+
+constexpr int kLoaders = 256, kThreads = 512;
+
+template <class T>
+struct AnyArgs {
+    int64_t M, K, N;  // rows; inner length (weight: rows of dW); output columns
+    int types, tiles_m, tiles_n;  // tiles_m: of dW's rows (weight only)
+    const int32_t* offsets;
+    const T* A;
+    int64_t lda;
+    Saved8 a8;  // the first operand in 8 bits (weight only)
+    const T* B;
+    int64_t ldb, stride_b;
+    int a_vec, b_vec;  // rows 16-byte aligned
+    // weight
+    int64_t piece, stride_c, ldp;
+    float* part;
+    int out_f32;
+    float *db, *db_part;
+};
+
+// A tile's source: rows of 8-value chunks.
+template <class T>
+struct Source {
+    const T* p;
+    int64_t ld;
+    int rows, cols;  // of the tile, how many exist
+};
+
+// Eight values at p, of which the first `n` exist.
+template <class T>
+__device__ __forceinline__ Raw<T, 8> load8(const T* p, int n, bool vec) {
+    if (n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            Raw<T, 8> k;
+            if (vec) {
+                const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 4);
+                k.w[0] = a.x, k.w[1] = a.y, k.w[2] = a.z, k.w[3] = a.w;
+                k.w[4] = b.x, k.w[5] = b.y, k.w[6] = b.z, k.w[7] = b.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) k.w[j] = __float_as_uint(p[j]);
+            }
+            return k;
+        } else {
+            Raw<T, 8> k;
+            if (vec) {
+                const uint4 a = *reinterpret_cast<const uint4*>(p);
+                k.w[0] = a.x, k.w[1] = a.y, k.w[2] = a.z, k.w[3] = a.w;
+            } else {
+                // whole words: five, shifted by a half, where p is odd (each holds a value of the eight)
+                const uintptr_t u = reinterpret_cast<uintptr_t>(p);
+                const uint32_t* q = reinterpret_cast<const uint32_t*>(u & ~uintptr_t(3));
+                const bool odd = (u & 2) != 0;
+                uint32_t w[5];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = q[j];
+                w[4] = odd ? q[4] : 0u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) k.w[j] = odd ? __byte_perm(w[j], w[j + 1], 0x5432) : w[j];
+            }
+            return k;
+        }
+    }
+    return gather_raw<T, 8>([&](int j) { return j < n ? p[j] : from_f32<T>(0.0f); });
+}
+
+// Chunk c of row r of a plane: 128-byte rows, 16-byte chunks swizzled.  Tiles
+// of more than 64 columns are chunks of 8 KB.
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    return static_cast<uint32_t>(c >> 3) * tc::kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void store_chunk(uint32_t addr, const uint32_t (&w)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                 : "memory");
+}
+// Eight values into one plane (16-bit types) or three (fp32), `plane` bytes apart.
+template <class T>
+__device__ __forceinline__ void put8(uint32_t addr, uint32_t plane, const Raw<T, 8>& k) {
+    if constexpr (sizeof(T) == 2) {
+        store_chunk(addr, k.w);
+    } else {
+        float x[8];
+        Raw<__nv_bfloat16, 8> h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __fsub_rn(__uint_as_float(k.w[j]), __uint_as_float(k.w[j] & 0xffff0000u));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h.w[j] = __byte_perm(k.w[2 * j], k.w[2 * j + 1], 0x7632);
+        store_chunk(addr, h.w);
+        narrow(x, h);
+        store_chunk(addr + plane, h.w);
+        float y[8];
+        widen(h, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __fsub_rn(x[j], y[j]);
+        narrow(x, h);
+        store_chunk(addr + 2 * plane, h.w);
+    }
+}
+
+// The part of a tile of ROWS memory rows x CHUNKS 8-value chunks that one of
+// THREADS loader threads moves: one chunk of every STEP-th row.
+template <int ROWS, int CHUNKS, int THREADS>
+struct Part {
+    static constexpr int STEP = THREADS / CHUNKS, N = ROWS / STEP;
+    static __device__ __forceinline__ int chunk() { return threadIdx.x % CHUNKS; }
+    static __device__ __forceinline__ int row(int i) { return threadIdx.x % THREADS / CHUNKS + i * STEP; }
+};
+
+template <class P, class T>
+__device__ __forceinline__ void fetch_tile(const Source<T>& s, bool vec, Raw<T, 8> (&k)[P::N]) {
+    const T* p = s.p + P::row(0) * s.ld + P::chunk() * 8;
+    const int n = s.cols - P::chunk() * 8;
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+        k[i] = load8(p, P::row(i) < s.rows ? n : 0, vec);
+        p += P::STEP * s.ld;
+    }
+}
+template <class P>
+__device__ __forceinline__ void fetch_tile8(const Saved8& s, int64_t row0, int64_t col0, int rows, int cols,
+                                            Raw<int8_t, 8> (&k)[P::N], int (&e)[P::N]) {
+    const int c = P::chunk() * 8;
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+        const bool live = P::row(i) < rows && c < cols;
+        const int64_t r = row0 + P::row(i);
+        if (live) k[i] = *reinterpret_cast<const Raw<int8_t, 8>*>(s.codes + r * s.ld + col0 + c);
+        else k[i].w[0] = k[i].w[1] = 0u;
+        e[i] = live ? s.exps[r * s.lde + col0 / kBlock8] : 127;
+    }
+}
+
+// What a step of the loop over (tile, inner block) is.
+struct Item {
+    int t, p;
+    int64_t m0, n0;   // first row (rows products) or first row of dW; first column
+    int64_t r0, r1;   // the type's rows from the tile's (piece's) first to the end
+    int steps;
+    bool whole;       // weight: the type has this one piece
+};
+
+template <class T, int OP>
+__device__ __forceinline__ Item item_at(const AnyArgs<T>& g, const int* prefix, int64_t it, int BN) {
+    Item m;
+    const int per = OP == kGradWeight ? g.tiles_m * g.tiles_n : g.tiles_n;
+    m.p = static_cast<int>(it / per);
+    const int in = static_cast<int>(it - static_cast<int64_t>(m.p) * per);
+    m.t = find_type(prefix, g.types, m.p);
+    const int64_t b = clamp_row(g.offsets[m.t], g.M), e = clamp_row(g.offsets[m.t + 1], g.M);
+    const int64_t size = OP == kGradWeight ? g.piece : BM;
+    m.r0 = b + (m.p - prefix[m.t]) * size;
+    m.r1 = m.r0 + size < e ? m.r0 + size : e;
+    m.whole = prefix[m.t + 1] - prefix[m.t] == 1;
+    m.n0 = static_cast<int64_t>(in % g.tiles_n) * BN;
+    if (OP == kGradWeight) {
+        m.m0 = static_cast<int64_t>(in / g.tiles_n) * BM;
+        m.steps = static_cast<int>((m.r1 - m.r0 + tc::kInner - 1) / tc::kInner);
+    } else {
+        m.m0 = m.r0;
+        m.steps = static_cast<int>((g.K + tc::kInner - 1) / tc::kInner);
+    }
+    return m;
+}
+
+__device__ __forceinline__ int clip(int64_t n, int most) { return n < 0 ? 0 : (n < most ? static_cast<int>(n) : most); }
+
+// The two operands' sources for inner block kb.
+template <class T, int OP>
+__device__ __forceinline__ Source<T> source_a(const AnyArgs<T>& g, const Item& m, int kb, int) {
+    const int64_t k = static_cast<int64_t>(kb) * tc::kInner;
+    if (OP == kGradWeight)
+        return {g.A + (m.r0 + k) * g.lda + m.m0, g.lda, clip(m.r1 - m.r0 - k, tc::kInner), clip(g.K - m.m0, BM)};
+    return {g.A + m.m0 * g.lda + k, g.lda, clip(m.r1 - m.r0, BM), clip(g.K - k, tc::kInner)};
+}
+template <class T, int OP>
+__device__ __forceinline__ Source<T> source_b(const AnyArgs<T>& g, const Item& m, int kb, int BN) {
+    const int64_t k = static_cast<int64_t>(kb) * tc::kInner;
+    if (OP == kGradWeight)
+        return {g.B + (m.r0 + k) * g.ldb + m.n0, g.ldb, clip(m.r1 - m.r0 - k, tc::kInner), clip(g.N - m.n0, BN)};
+    const T* w = g.B + m.t * g.stride_b;
+    if (OP == kForward) return {w + k * g.ldb + m.n0, g.ldb, clip(g.K - k, tc::kInner), clip(g.N - m.n0, BN)};
+    return {w + m.n0 * g.ldb + k, g.ldb, clip(g.N - m.n0, BN), clip(g.K - k, tc::kInner)};
+}
+
+// dW and db of a type without rows, by n threads.
+template <class T>
+__device__ void zero_type(const AnyArgs<T>& g, const RowsOut<T>& out, int t, int e, int n) {
+    for (int64_t k = 0; k < g.K; ++k)
+        for (int64_t c = e; c < g.N; c += n) {
+            const int64_t at = t * g.stride_c + k * out.ldc + c;
+            if (sizeof(T) == 2 && g.out_f32) reinterpret_cast<float*>(out.C)[at] = 0.0f;
+            else out.C[at] = from_f32<T>(0.0f);
+        }
+    if (g.db)
+        for (int64_t c = e; c < g.N; c += n) g.db[t * g.N + c] = 0.0f;
+}
+
+// SAVED: the first operand in 8 bits.  TMA: the second by TMA (map mb).
+template <class T, int OP, int BN, bool SAVED, bool TMA>
+__global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_constant__ CUtensorMap map_b,
+                                                                const AnyArgs<T> g, const RowsOut<T> out) {
+    using H = typename Half<T>::type;
+    constexpr int PA = SAVED ? 1 : Half<T>::planes, PB = Half<T>::planes;
+    using S = Plan<PA, PB, BN>;
+    constexpr int STAGES = S::kStages;
+    constexpr bool W = OP == kGradWeight, A_OUTER = W, B_OUTER = OP != kGradInput;
+    static_assert(!TMA || (W && PB == 1), "TMA takes 16-bit dY");
+    constexpr uint32_t ID = tc::idesc(is_bf16<H>(), A_OUTER, B_OUTER, BM, BN);
+    // 16-bit values: the loaders are two groups that take the stages in turn,
+    // so that one group's loads are in flight while the other's arrive (fp32
+    // values would need twice the registers, and take six times as long to
+    // multiply).
+    constexpr int GROUPS = sizeof(T) == 2 ? 2 : 1, THREADS = kLoaders / GROUPS;
+    using PartA = Part<A_OUTER ? 64 : BM, A_OUTER ? BM / 8 : 8, THREADS>;
+    using PartB = Part<B_OUTER ? 64 : BN, B_OUTER ? BN / 8 : 8, THREADS>;
+
+    extern __shared__ uint8_t raw[];
+    __shared__ Shared s;
+    __shared__ float stage_out[4][(stage_bytes<float>() + 3) / 4];
+    __shared__ float db_rows[W && !TMA ? kLoaders * 8 : 1];
+    const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
+    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, W ? g.piece : BM,
+                                             8 / GROUPS + (TMA ? 1 : 0));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t items = static_cast<int64_t>(s.prefix[g.types]) * (W ? g.tiles_m * g.tiles_n : g.tiles_n);
+
+    if (warp < 8) {
+        // ── loaders ──
+        int64_t i = 0, it = blockIdx.x;
+        bool ok = true;
+        Raw<T, 8> ka[SAVED ? 1 : PartA::N], kb[TMA ? 1 : PartB::N];
+        Raw<int8_t, 8> k8[SAVED ? PartA::N : 1];
+        int e8[SAVED ? PartA::N : 1];
+        const auto fetch = [&](const Item& m, int step) {
+            if constexpr (SAVED) {
+                const int64_t k = static_cast<int64_t>(step) * tc::kInner;
+                fetch_tile8<PartA>(g.a8, m.r0 + k, m.m0, clip(m.r1 - m.r0 - k, tc::kInner), clip(g.K - m.m0, BM), k8,
+                                   e8);
+            } else {
+                fetch_tile<PartA>(source_a<T, OP>(g, m, step, BN), g.a_vec, ka);
+            }
+            if constexpr (!TMA) fetch_tile<PartB>(source_b<T, OP>(g, m, step, BN), g.b_vec, kb);
+        };
+        const int group = threadIdx.x / THREADS;
+        // This group's first step of an item whose first stage is number i0.
+        const auto first = [&](int64_t i0) { return GROUPS == 1 ? 0 : static_cast<int>((group + i0) & 1); };
+        Item m{};
+        bool fetched = false;  // the registers hold the next step's values
+        if (it < items) m = item_at<T, OP>(g, s.prefix, it, BN);
+        float sum[8];
+        while (it < items && ok) {
+            const bool sums = W && !TMA && g.db != nullptr && m.m0 == 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
+            const bool more = it + gridDim.x < items;
+            Item next = m;
+            if (more) next = item_at<T, OP>(g, s.prefix, it + gridDim.x, BN);
+            for (int step = first(i); step < m.steps; step += GROUPS) {
+                if (!fetched) fetch(m, step);
+                const int64_t n = i + step;
+                const int st = static_cast<int>(n % STAGES);
+                if (n >= STAGES) ok = mb::wait(&s.empty[st], (n / STAGES - 1) & 1, &g_error, 41);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                const uint32_t a = ring + st * S::kStage, b = a + PA * S::kA;
+#pragma unroll
+                for (int u = 0; u < PartA::N; ++u) {
+                    const uint32_t at = a + chunk_at(PartA::row(u), PartA::chunk());
+                    if constexpr (SAVED) {
+                        float x[8];
+                        values4(k8[u].w[0], e8[u], x);
+                        values4(k8[u].w[1], e8[u], x + 4);
+                        Raw<H, 8> h;
+                        narrow(x, h);
+                        store_chunk(at, h.w);
+                    } else {
+                        put8<T>(at, S::kA, ka[u]);
+                    }
+                }
+                if constexpr (!TMA) {
+#pragma unroll
+                    for (int u = 0; u < PartB::N; ++u) {
+                        put8<T>(b + chunk_at(PartB::row(u), PartB::chunk()), S::kB, kb[u]);
+                        if (sums) {
+                            float x[8];
+                            widen(kb[u], x);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) sum[j] += x[j];
+                        }
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mb::arrive(&s.full[st]);
+                // the next step's values, on their way while stages are
+                // multiplied (after the fence, which waits for loads too)
+                fetched = true;
+                if (step + GROUPS < m.steps) fetch(m, step + GROUPS);
+                else if (more && first(i + m.steps) < next.steps) fetch(next, first(i + m.steps));
+                else fetched = false;
+            }
+            i += m.steps;
+            if constexpr (W && !TMA) {
+                if (sums) {  // the same for every loader thread
+                    constexpr int G = kLoaders / (BN / 8);  // threads that share a column
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) db_rows[threadIdx.x / (BN / 8) * BN + PartB::chunk() * 8 + j] = sum[j];
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    if (ok && threadIdx.x < BN && m.n0 + threadIdx.x < g.N) {
+                        float all = 0.0f;
+#pragma unroll 4
+                        for (int q = 0; q < G; ++q) all += db_rows[q * BN + threadIdx.x];
+                        (m.whole ? g.db + m.t * g.N : g.db_part + m.p * g.N)[m.n0 + threadIdx.x] = all;
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                }
+            }
+            it += gridDim.x;
+            m = next;
+        }
+    } else if (warp == 8) {
+        // ── MMA issuer ──
+        int64_t i = 0;
+        int local = 0;
+        bool ok = true;
+        for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x, ++local) {
+            const Item m = item_at<T, OP>(g, s.prefix, it, BN);
+            const int acc = local & 1;
+            if (local >= 2) ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 42);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            tc::fence_after();
+            for (int k = 0; k < m.steps; ++k, ++i) {
+                const int st = static_cast<int>(i % STAGES);
+                ok = mb::wait(&s.full[st], (i / STAGES) & 1, &g_error, 43);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                tc::fence_after();
+                if constexpr (TMA) {
+                    // Rows of dY past the piece: the loaders' zeros would meet another type's values there, and
+                    // 0 x NaN is not 0.
+                    const int64_t valid = m.r1 - m.r0 - static_cast<int64_t>(k) * tc::kInner;
+                    if (valid < tc::kInner) zero_rows(ring + st * S::kStage + PA * S::kA, S::kB, static_cast<int>(valid));
+                }
+                if (lane == 0) {
+                    stage_mmas<PA, PB, BN, A_OUTER, B_OUTER>(ring + st * S::kStage, tmem + acc * BN, ID, k == 0);
+                    tc::commit(&s.empty[st]);
+                }
+                __syncwarp();
+            }
+            if (ok && lane == 0) tc::commit(&s.acc_full[acc]);
+        }
+    } else if (warp == 9) {
+        // ── TMA of dY ──
+        if (TMA && lane == 0) {
+            int64_t i = 0;
+            bool ok = true;
+            for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
+                const Item m = item_at<T, OP>(g, s.prefix, it, BN);
+                for (int k = 0; k < m.steps; ++k, ++i) {
+                    const int st = static_cast<int>(i % STAGES);
+                    if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_error, 44))) break;
+                    mb::arrive_expect_tx(&s.full[st], S::kB);
+#pragma unroll
+                    for (int c = 0; c < BN / 64; ++c)
+                        tc::tma3(ring + st * S::kStage + PA * S::kA + c * tc::kChunkBytes, &map_b,
+                                 static_cast<int>(m.n0) + c * 64, static_cast<int>(m.r0) + k * tc::kInner, 0,
+                                 &s.full[st]);
+                }
+            }
+            // every copy issued must have landed before the CTA may exit
+            for (int64_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
+                mb::wait(&s.full[j % STAGES], (j / STAGES) & 1, &g_error, 45);
+        }
+    } else if (warp >= 12) {
+        // ── epilogue ──
+        const int q = warp & 3;
+        T* buf = reinterpret_cast<T*>(stage_out[q]);
+        float* buf32 = stage_out[q];
+        int local = 0;
+        for (int64_t it = blockIdx.x; it < items; it += gridDim.x, ++local) {
+            const Item m = item_at<T, OP>(g, s.prefix, it, BN);
+            const int acc = local & 1;
+            bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 46);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc::fence_after();
+            const uint32_t addr = tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
+            const int64_t r = m.m0 + q * 32;
+            if constexpr (!W) {
+                finish_rows<T, BN, sizeof(T) == 2>(addr, out, m.t, r, clip(m.r1 - r, 32), m.n0, buf);
+            } else {
+                const int rows = clip(g.K - r, 32);
+#pragma unroll 1
+                for (int c0 = 0; c0 < BN && m.n0 + c0 < g.N; c0 += 32) {
+                    float v[32];
+                    tc::load32(addr + c0, v);
+                    const int64_t n = m.n0 + c0, left = g.N - n;
+                    if (!m.whole) {
+                        store_rows(g.part + (m.p * g.K + r) * g.ldp + n, g.ldp, rows, g.ldp - n, v, 2, buf32);
+                    } else if (sizeof(T) == 2 && g.out_f32) {
+                        store_rows(reinterpret_cast<float*>(out.C) + m.t * g.stride_c + r * out.ldc + n, out.ldc, rows,
+                                   left, v, out.mode, buf32);
+                    } else {
+                        store_rows(out.C + m.t * g.stride_c + r * out.ldc + n, out.ldc, rows, left, v, out.mode, buf);
+                    }
+                }
+            }
+            tc::fence_before();
+            mb::arrive(&s.acc_empty[acc]);
+        }
+        if constexpr (W) {
+            // types without rows: zero
+            const int e = threadIdx.x - 384;
+            for (int t = blockIdx.x; t < g.types; t += gridDim.x) {
+                if (s.prefix[t + 1] != s.prefix[t]) continue;
+                zero_type(g, out, t, e, 128);
+            }
+        }
+    }
+    tear_down<BN>(s, tmem, 8);
+}
+
+template <class T, int OP, int BN, bool SAVED, bool TMA>
+void go(const CUtensorMap& map, const AnyArgs<T>& g, const RowsOut<T>& out, int64_t items, cudaStream_t s) {
+    constexpr int PA = SAVED ? 1 : Half<T>::planes;
+    run("typed_any", typed_any_kernel<T, OP, BN, SAVED, TMA>, kThreads, Plan<PA, Half<T>::planes, BN>::kBytes, items,
+        s, map, g, out);
+}
+
+}  // namespace
+
+template <class T, bool TRANS>
+void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s) {
+    constexpr int OP = TRANS ? kGradInput : kForward;
+    AnyArgs<T> g{};
+    g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
+    g.A = a.A, g.lda = a.lda, g.B = a.W, g.ldb = a.ldw, g.stride_b = a.stride_w;
+    g.a_vec = rows_aligned16(a.A, a.lda, sizeof(T));
+    g.b_vec = rows_aligned16(a.W, a.ldw, sizeof(T)) && a.stride_w * sizeof(T) % 16 == 0;
+    const RowsOut<T> out{a.N, a.bias, a.act, a.alpha, a.C, a.ldc, store_mode(a.C, a.ldc * sizeof(T)), a.saved, a.r8};
+    const int64_t pieces = a.M / BM + std::min<int64_t>(a.types, a.M);
+    const int BN = tile_width(pieces, a.N, 128, a.saved.codes != nullptr);
+    g.tiles_m = 1;
+    g.tiles_n = static_cast<int>(ceil_div(a.N, BN));
+    const CUtensorMap none{};
+    if (BN == 64) go<T, OP, 64, false, false>(none, g, out, pieces * g.tiles_n, s);
+    else go<T, OP, 128, false, false>(none, g, out, pieces * g.tiles_n, s);
+}
+
+template <class T, class O>
+void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s) {
+    const bool saved = a.saved.codes != nullptr;
+    AnyArgs<T> g{};
+    g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
+    g.tiles_m = w.tiles_k, g.tiles_n = w.tiles_n;
+    g.A = a.X, g.lda = a.ldx, g.a8 = a.saved, g.B = a.dY, g.ldb = a.lddy;
+    g.a_vec = rows_aligned16(a.X, a.ldx, sizeof(T));
+    g.b_vec = rows_aligned16(a.dY, a.lddy, sizeof(T));
+    g.piece = w.piece, g.part = w.part, g.ldp = w.ldp, g.stride_c = a.stride_dw;
+    g.out_f32 = sizeof(O) == 4;
+    RowsOut<T> out{};
+    out.N = a.N;
+    out.C = reinterpret_cast<T*>(a.dW);
+    out.ldc = a.lddw;
+    out.mode = store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O));
+    const auto by_source = [&](auto bn) {
+        constexpr int BN = decltype(bn)::value;
+        if constexpr (sizeof(T) == 2) {
+            if (w.dy_by_tma) {
+                const int64_t dims[3] = {a.N, a.M, 1}, strides[2] = {a.lddy, std::max<int64_t>(a.M * a.lddy, 8)};
+                const int box[3] = {64, 64, 1};
+                const CUtensorMap map = tc::map16<3>(a.dY, is_bf16<T>(), dims, strides, box);
+                go<T, kGradWeight, BN, true, true>(map, g, out, w.items, s);
+                return;
+            }
+        }
+        if constexpr (BN <= 128) {
+            g.db = a.db, g.db_part = w.db_part;
+            const CUtensorMap none{};
+            if (saved) go<T, kGradWeight, BN, true, false>(none, g, out, w.items, s);
+            else go<T, kGradWeight, BN, false, false>(none, g, out, w.items, s);
+        }
+    };
+    if (w.BN == 64) by_source(std::integral_constant<int, 64>{});
+    else if (w.BN == 128) by_source(std::integral_constant<int, 128>{});
+    else if constexpr (sizeof(T) == 2) by_source(std::integral_constant<int, 256>{});
+}
+
+#define TG_TYPED_ANY(T)                                                   \
+    template void typed_rows_any<T, false>(const RowsArgs<T>&, cudaStream_t); \
+    template void typed_rows_any<T, true>(const RowsArgs<T>&, cudaStream_t);  \
+    template void typed_weight_any<T, T>(const WeightArgs<T, T>&, const WeightPlan&, cudaStream_t);
+TG_TYPED_ANY(float)
+TG_TYPED_ANY(__nv_bfloat16)
+TG_TYPED_ANY(__half)
+template void typed_weight_any<__nv_bfloat16, float>(const WeightArgs<__nv_bfloat16, float>&, const WeightPlan&,
+                                                     cudaStream_t);
+template void typed_weight_any<__half, float>(const WeightArgs<__half, float>&, const WeightPlan&, cudaStream_t);
+
+int typed_any_take_error() { return take_error(); }
+
+}  // namespace tg

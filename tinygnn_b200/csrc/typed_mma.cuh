@@ -1,0 +1,304 @@
+// ============================================================================
+//  typed_mma.cuh -- what the typed products' tensor-core kernels share: the
+//  shared-memory plan, set-up and tear-down, the MMAs of a stage, output
+//  stores and the epilogue of the rows products.
+// ============================================================================
+#pragma once
+
+#include <algorithm>
+
+#include "tcgen05.cuh"
+#include "typed.cuh"
+
+namespace tg {
+namespace typed {
+
+constexpr int BM = 128;
+
+// The error word of the including file's kernels: the first timeout code seen
+// (0 = none).
+namespace {
+__device__ int g_error = 0;
+}
+
+// Ring of stages (1024-byte aligned): PA planes of the A tile, PB of the B tile.
+template <int PA, int PB, int BN>
+struct Plan {
+    static constexpr uint32_t kA = BM * 128, kB = BN * 128;  // one plane's tile
+    static constexpr uint32_t kStage = PA * kA + PB * kB;
+    static constexpr int kStages = (192 * 1024) / kStage > 8 ? 8 : (192 * 1024) / kStage;
+    static constexpr uint32_t kBytes = kStages * kStage + 1024;
+    static_assert(kStages >= 2, "two stages");
+};
+
+struct Shared {
+    uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drain;
+    uint32_t tmem;
+    int prefix[kMaxTypes + 1];
+};
+
+template <int BN>
+constexpr uint32_t tmem_cols() { return 2 * BN < 64 ? 64 : 2 * BN; }
+
+// Barriers, TMEM (warp 2) and the scan of the types (warp 3); every thread
+// returns with them in place.
+template <int STAGES, int BN>
+__device__ __forceinline__ uint32_t set_up(Shared& s, const int32_t* offsets, int types, int64_t M, int64_t per,
+                                           int full_arrivals) {
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mb::init(&s.full[i], full_arrivals);
+            mb::init(&s.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mb::init(&s.acc_full[i], 1);
+            mb::init(&s.acc_empty[i], 128);
+        }
+        mb::init(&s.drain, 1);
+        mb::fence_init();
+    }
+    if (warp == 2) tc::alloc(&s.tmem, tmem_cols<BN>());
+    if (warp == 3) scan_types(offsets, types, M, per, s.prefix);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    return s.tmem;
+}
+
+// Every copy has landed; once every MMA of the issuing warp has retired, TMEM
+// goes back.
+template <int BN>
+__device__ __forceinline__ void tear_down(Shared& s, uint32_t tmem, int mma_warp) {
+    tc::fence_before();
+    __syncthreads();
+    const int warp = threadIdx.x >> 5;
+    if (warp == mma_warp && (threadIdx.x & 31) == 0) {
+        tc::commit(&s.drain);
+        mb::wait(&s.drain, 0, &g_error, 26);
+    }
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 2) tc::dealloc(tmem, tmem_cols<BN>());
+}
+
+// One warp: rows [valid, 64) of the 64-row chunks in `bytes` of shared memory
+// become zero, and the tensor cores see it.
+__device__ __forceinline__ void zero_rows(uint32_t base, uint32_t bytes, int valid) {
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t chunk = 0; chunk < bytes; chunk += tc::kChunkBytes)
+        for (uint32_t o = valid * 128 + lane * 16; o < tc::kChunkBytes; o += 512)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + chunk + o), "r"(0u) : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+// The MMAs of one stage: every plane product i + j <= 2, smallest first.
+template <int PA, int PB, int BN, bool A_OUTER, bool B_OUTER>
+__device__ __forceinline__ void stage_mmas(uint32_t stage, uint32_t acc, uint32_t id, bool first) {
+    using S = Plan<PA, PB, BN>;
+    bool add = !first;
+#pragma unroll
+    for (int order = PA + PB - 2 < 2 ? PA + PB - 2 : 2; order >= 0; --order)
+#pragma unroll
+        for (int i = PA - 1; i >= 0; --i) {
+            const int j = order - i;
+            if (j < 0 || j >= PB) continue;
+            const uint32_t a = stage + i * S::kA, b = stage + PA * S::kA + j * S::kB;
+#pragma unroll
+            for (int s = 0; s < tc::kInner / 16; ++s) {
+                tc::mma(acc, A_OUTER ? tc::desc_outer(a, s) : tc::desc_inner(a, s),
+                        B_OUTER ? tc::desc_outer(b, s) : tc::desc_inner(b, s), id, add);
+                add = true;
+            }
+        }
+}
+
+// How an output's rows are aligned: 2 = 32 bytes, 1 = 16 bytes, 0 = neither
+// (-1, for store_rows: neither, and there is no buffer to stage them in).
+inline int store_mode(const void* p, int64_t row_bytes, int64_t matrix_bytes = 0) {
+    const uint64_t b = reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(row_bytes) |
+                       static_cast<uint64_t>(matrix_bytes);
+    return b % 32 == 0 ? 2 : (b % 16 == 0 ? 1 : 0);
+}
+
+// Bytes of a warp's staging buffer for outputs whose rows are not aligned: 32
+// rows of 32 values, rows an odd number of words apart.
+template <class O>
+constexpr int stage_row() { return sizeof(O) == 4 ? 33 : 34; }
+template <class O>
+constexpr int stage_bytes() { return 32 * stage_row<O>() * static_cast<int>(sizeof(O)); }
+
+// A warp's 32 rows x 32 columns: lane l holds row l of `v`; rows [0, rows) and
+// columns [0, left) are stored at p + row * ld + column.  Aligned rows: each
+// lane stores its own, 32 bytes (whole sectors) or 16 at a time.  Others:
+// through `buf`, so that a warp's store covers 32 neighbouring columns of one
+// row (lane-per-row stores would send one sector for every 2 or 4 bytes).
+template <class O>
+__device__ __forceinline__ void store_rows(O* p, int64_t ld, int rows, int64_t left, const float (&v)[32], int mode,
+                                           O* buf) {
+    constexpr int W = 32 / sizeof(O);  // values per 32 bytes
+    const int lane = threadIdx.x & 31;
+    if (mode != 0) {
+        if (lane >= rows) return;
+        p += lane * ld;
+#pragma unroll
+        for (int c = 0; c < 32; c += W) {
+            if (mode > 0 && c + W <= left) {
+                Raw<O, W> k;
+                narrow(v + c, k);
+                const uint32_t* r = k.w;
+                if (mode == 2) {
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + c), "r"(r[0]),
+                                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                                 : "memory");
+                } else {
+                    uint4* q = reinterpret_cast<uint4*>(p + c);
+                    q[0] = make_uint4(r[0], r[1], r[2], r[3]);
+                    q[1] = make_uint4(r[4], r[5], r[6], r[7]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (c + j < left) p[c + j] = from_f32<O>(v[c + j]);
+            }
+        }
+        return;
+    }
+    constexpr int S = stage_row<O>();
+    __syncwarp();  // the previous chunk has been read
+#pragma unroll
+    for (int j = 0; j < 32; ++j) buf[lane * S + j] = from_f32<O>(v[j]);
+    __syncwarp();
+    if (lane < left) {
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) p[r * ld + lane] = buf[r * S + lane];
+    }
+}
+
+// ── epilogue of the rows products ────────────────────────────────────────
+template <class O>
+struct RowsOut {
+    int64_t N;
+    const float* bias;
+    int act;
+    float alpha;
+    O* C;
+    int64_t ldc;
+    int mode;
+    Saved8 saved;
+    Range8 r8;
+};
+
+// 32 accumulator columns from n (bias added; columns past N are zero).
+template <class O>
+__device__ __forceinline__ void load_biased(uint32_t addr, const RowsOut<O>& g, int type, int64_t n, float (&v)[32]) {
+    tc::load32(addr, v);
+    if (!g.bias) return;
+    const float* b = g.bias + type * g.N + n;
+    if (n + 32 <= g.N && g.N % 4 == 0 && reinterpret_cast<uintptr_t>(g.bias) % 16 == 0) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(b + j));
+            v[j] = __fadd_rn(v[j], q.x);
+            v[j + 1] = __fadd_rn(v[j + 1], q.y);
+            v[j + 2] = __fadd_rn(v[j + 2], q.z);
+            v[j + 3] = __fadd_rn(v[j + 3], q.w);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (n + j < g.N) v[j] = __fadd_rn(v[j], __ldg(b + j));
+    }
+}
+
+// One warp's 32 rows (row0 .. row0 + rows) and BN columns (from n0) of a tile.
+// FAST: act_forward's.
+template <class O, int BN, bool FAST>
+__device__ __forceinline__ void finish_rows(uint32_t addr, const RowsOut<O>& g, int type, int64_t row0, int rows,
+                                            int64_t n0, O* buf) {
+    const int lane = threadIdx.x & 31;
+    const bool live = lane < rows;
+    const int64_t row = live ? row0 + lane : 0;
+    constexpr int W = BN < kBlock8 ? BN : kBlock8;
+#pragma unroll 1
+    for (int b0 = 0; b0 < BN && n0 + b0 < g.N; b0 += kBlock8) {
+        int byte = 0;
+        float inv = 0.0f;
+        // An exponent's 128 columns may lie in two tiles of 64: then N <= 64
+        // and there is one tile (the callers see to it).
+        if (g.saved.codes) {  // the block's exponent needs all its columns first
+            float m = 0.0f;
+#pragma unroll 1
+            for (int c0 = b0; c0 < b0 + W; c0 += 32) {
+                float v[32];
+                load_biased(addr + c0, g, type, n0 + c0, v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) m = max_mag(m, v[j]);
+            }
+            byte = exponent8(m, g.r8.emin);
+            inv = encode8(byte);
+            if (live) g.saved.exps[row * g.saved.lde + (n0 + b0) / kBlock8] = static_cast<uint8_t>(byte);
+        }
+#pragma unroll 1
+        for (int c0 = b0; c0 < b0 + W; c0 += 32) {
+            const int64_t left = g.N - n0 - c0;
+            if (left <= 0) break;
+            float v[32];
+            load_biased(addr + c0, g, type, n0 + c0, v);
+            if (g.saved.codes && live) {
+                int8_t* o = g.saved.codes + row * g.saved.ld + n0 + c0;
+#pragma unroll
+                for (int h = 0; h < 32; h += 16) {
+                    if (h + 16 <= left) {
+                        store_codes<16>(o + h, v + h, inv, byte, g.r8.top);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (h + j < left) o[h + j] = code8(v[h + j], inv, byte, g.r8.top);
+                    }
+                }
+            }
+            act_forward<FAST>(v, g.act, g.alpha);
+            store_rows(g.C + row0 * g.ldc + n0 + c0, g.ldc, rows, left, v, g.mode, buf);
+        }
+    }
+}
+
+template <class T> struct Half { using type = T; static constexpr int planes = 1; };
+template <> struct Half<float> { using type = __nv_bfloat16; static constexpr int planes = 3; };
+template <class H>
+constexpr bool is_bf16() { return std::is_same<H, __nv_bfloat16>::value; }
+
+// Reads and clears the error word (the stream is idle).
+static int take_error() {
+    int h = 0;
+    TG_CUDA(cudaMemcpyFromSymbol(&h, g_error, sizeof(int)));
+    if (h) {
+        const int zero = 0;
+        TG_CUDA(cudaMemcpyToSymbol(g_error, &zero, sizeof(int)));
+    }
+    return h;
+}
+
+// Tile width of a product with N columns and `pieces` row tiles (or dW tiles):
+// the widest (it reads the rows fewest times) that still gives every SM a
+// tile, else the narrowest.  An exponent of a saved result needs its 128
+// columns in one tile.
+inline int tile_width(int64_t pieces, int64_t N, int widest, bool saved) {
+    const int least = saved && N > 64 ? 128 : 64;
+    for (int w = widest; w > least; w /= 2)
+        if (N > w / 2 && pieces * ceil_div(N, w) >= num_sms()) return w;
+    return least;
+}
+
+// A persistent grid of at most one CTA per SM.
+template <class K, class... A>
+void run(const char* name, K kern, int threads, uint32_t smem, int64_t items, cudaStream_t s, A... args) {
+    TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    launch(name, kern, dim3(static_cast<unsigned>(std::min<int64_t>(items, num_sms()))), dim3(threads), smem, s,
+           args...);
+}
+
+}  // namespace typed
+}  // namespace tg

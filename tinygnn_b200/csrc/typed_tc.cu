@@ -1,5 +1,6 @@
 // ============================================================================
-//  typed_tc.cu -- the typed linear map's products on the tensor cores.
+//  typed_tc.cu -- the typed linear map's products on the tensor cores, operands
+//  by TMA, and the choice of kernel for every product.
 //
 //  rows kernel    C[r] = act(A[r] . B[t(r)] + bias[t(r)]): the forward pass
 //                 (B = W[t], its columns contiguous) and the input gradient
@@ -7,15 +8,9 @@
 //  weight kernel  dW[t] = sum over the type's rows of X[r]^T dY[r]; both
 //                 operands have their outer index contiguous.
 //
-//  Operands are 16-bit.  bf16 and fp16 matrices are read where they lie when
-//  their rows start 16-byte aligned (TMA's rule), from an aligned copy
-//  otherwise.  An fp32 matrix is split into three bf16 planes,
-//      x = x0 + x1 + x2,   x0 = bf16(x), x1 = bf16(x - x0), x2 = bf16(x - x0 - x1),
-//  which holds its 24 bits exactly, and a product takes the six plane products
-//  x_i y_j with i + j <= 2 (the others are below 2^-24 of it), smallest first.
-//  A matrix saved in 8 bits is one bf16 (or fp16) plane, exactly.
-//
-//  Both kernels are persistent: CTAs walk tiles blockIdx.x, + gridDim.x, ...
+//  Operands are bf16 or fp16 with 16-byte aligned rows (TMA's rule); the other
+//  forms are typed_any.cu's.  Both kernels are persistent: CTAs walk tiles
+//  blockIdx.x, + gridDim.x, ...
 //    warp 0       TMA loads into a ring of stages (64 inner indexes each);
 //    warp 1       the MMAs (one thread), into one of two TMEM accumulators;
 //    warp 2       TMEM allocation;
@@ -29,182 +24,35 @@
 //  Every wait is bounded; one that runs out records a code in a device error
 //  word (tg_take_device_error), and the CTA drains its copies and returns.
 // ============================================================================
-#include <algorithm>
-
-#include "tcgen05.cuh"
-#include "typed.cuh"
+#include "typed_mma.cuh"
 
 namespace tg {
 
 namespace {
 
-__device__ int g_typed_error = 0;  // first timeout code seen (0 = none)
+using namespace typed;
 
-constexpr int BM = 128;
 constexpr int kThreads = 384;
 
-// Shared-memory plan: ring of stages (1024-byte aligned), then the rest.
-template <int PA, int PB, int BN>
-struct Plan {
-    static constexpr uint32_t kA = BM * 128, kB = BN * 128;  // one plane's tile
-    static constexpr uint32_t kStage = PA * kA + PB * kB;
-    static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
-    static constexpr uint32_t kBytes = kStages * kStage + 1024;
-    static_assert(kStages >= 2, "two stages");
-};
-
-struct Shared {
-    uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drain;
-    uint32_t tmem;
-    int prefix[kMaxTypes + 1];
-};
-
-// The MMAs of one stage: every plane product i + j <= 2, smallest first.
-template <int PA, int PB, int BN, bool A_OUTER, bool B_OUTER>
-__device__ __forceinline__ void stage_mmas(uint32_t stage, uint32_t acc, uint32_t id, bool first) {
-    using S = Plan<PA, PB, BN>;
-    bool add = !first;
-#pragma unroll
-    for (int order = PA + PB - 2 < 2 ? PA + PB - 2 : 2; order >= 0; --order)
-#pragma unroll
-        for (int i = PA - 1; i >= 0; --i) {
-            const int j = order - i;
-            if (j < 0 || j >= PB) continue;
-            const uint32_t a = stage + i * S::kA, b = stage + PA * S::kA + j * S::kB;
-#pragma unroll
-            for (int s = 0; s < tc::kInner / 16; ++s) {
-                tc::mma(acc, A_OUTER ? tc::desc_outer(a, s) : tc::desc_inner(a, s),
-                        B_OUTER ? tc::desc_outer(b, s) : tc::desc_inner(b, s), id, add);
-                add = true;
-            }
-        }
-}
-
-// 32 consecutive columns of one row, of which `left` exist.  mode: 2 = every
-// row 32-byte aligned, 1 = 16-byte, 0 = neither.
-template <class O>
-__device__ __forceinline__ void store32(O* p, const float (&v)[32], int64_t left, int mode) {
-    constexpr int W = 32 / sizeof(O);  // values per 32 bytes
-#pragma unroll
-    for (int c = 0; c < 32; c += W) {
-        if (mode > 0 && c + W <= left) {
-            Raw<O, W> k;
-            narrow(v + c, k);
-            const uint32_t* r = k.w;
-            if (mode == 2) {
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + c), "r"(r[0]),
-                             "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                             : "memory");
-            } else {
-                uint4* q = reinterpret_cast<uint4*>(p + c);
-                q[0] = make_uint4(r[0], r[1], r[2], r[3]);
-                q[1] = make_uint4(r[4], r[5], r[6], r[7]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (c + j < left) p[c + j] = from_f32<O>(v[c + j]);
-        }
-    }
-}
-
-template <class O>
-int store_mode(const O* p, int64_t ld) {
-    const uint64_t bits = reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(ld * sizeof(O));
-    return bits % 32 == 0 ? 2 : (bits % 16 == 0 ? 1 : 0);
-}
-
-template <int BN>
-constexpr uint32_t tmem_cols() { return 2 * BN < 64 ? 64 : 2 * BN; }
-
-// Barriers, TMEM and the scan; every thread returns with them in place.
-template <int STAGES, int BN>
-__device__ __forceinline__ uint32_t set_up(Shared& s, const int32_t* offsets, int types, int64_t M, int64_t per) {
-    const int warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) {
-            mb::init(&s.full[i], 1);
-            mb::init(&s.empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mb::init(&s.acc_full[i], 1);
-            mb::init(&s.acc_empty[i], 128);
-        }
-        mb::init(&s.drain, 1);
-        mb::fence_init();
-    }
-    if (warp == 2) tc::alloc(&s.tmem, tmem_cols<BN>());
-    if (warp == 3) scan_types(offsets, types, M, per, s.prefix);
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    return s.tmem;
-}
-
-// Every MMA has retired and every copy has landed: TMEM goes back.
-template <int BN>
-__device__ __forceinline__ void tear_down(Shared& s, uint32_t tmem) {
-    tc::fence_before();
-    __syncthreads();
-    const int warp = threadIdx.x >> 5;
-    if (warp == 1 && (threadIdx.x & 31) == 0) {
-        tc::commit(&s.drain);
-        mb::wait(&s.drain, 0, &g_typed_error, 26);
-    }
-    __syncthreads();
-    tc::fence_after();
-    if (warp == 2) tc::dealloc(tmem, tmem_cols<BN>());
-}
-
 // ── rows kernel ──────────────────────────────────────────────────────────
-template <class O>
 struct RowsTc {
-    int64_t M, K, N;
+    int64_t M, K;
     int types, tiles_n;
     const int32_t* offsets;
-    const float* bias;
-    int act;
-    float alpha;
-    O* C;
-    int64_t ldc;
-    int mode;
-    Saved8 saved;
-    Range8 r8;
 };
 
-// 32 accumulator columns from n (bias added; columns past N are zero).
-template <class O>
-__device__ __forceinline__ void load_biased(uint32_t addr, const RowsTc<O>& g, int type, int64_t n, float (&v)[32]) {
-    tc::load32(addr, v);
-    if (!g.bias) return;
-    const float* b = g.bias + type * g.N + n;
-    if (n + 32 <= g.N && g.N % 4 == 0 && reinterpret_cast<uintptr_t>(g.bias) % 16 == 0) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const float4 q = __ldg(reinterpret_cast<const float4*>(b + j));
-            v[j] = __fadd_rn(v[j], q.x);
-            v[j + 1] = __fadd_rn(v[j + 1], q.y);
-            v[j + 2] = __fadd_rn(v[j + 2], q.z);
-            v[j + 3] = __fadd_rn(v[j + 3], q.w);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (n + j < g.N) v[j] = __fadd_rn(v[j], __ldg(b + j));
-    }
-}
-
-template <class O, int P, int BN, bool TRANS, bool BF16>
+template <class T, int BN, bool TRANS>
 __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid_constant__ CUtensorMap ma,
                                                                     const __grid_constant__ CUtensorMap mw,
-                                                                    const RowsTc<O> g) {
-    using S = Plan<P, P, BN>;
+                                                                    const RowsTc g, const RowsOut<T> out) {
+    using S = Plan<1, 1, BN>;
     constexpr int STAGES = S::kStages;
-    constexpr uint32_t ID = tc::idesc(BF16, false, !TRANS, BM, BN);
+    constexpr uint32_t ID = tc::idesc(is_bf16<T>(), false, !TRANS, BM, BN);
     extern __shared__ uint8_t raw[];
     __shared__ Shared s;
+    __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, BM);
+    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, BM, 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tiles = static_cast<int64_t>(s.prefix[g.types]) * g.tiles_n;
     const int KB = static_cast<int>((g.K + tc::kInner - 1) / tc::kInner);
@@ -219,26 +67,22 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
                 const int row0 = clamp_row(g.offsets[t], g.M) + (p - s.prefix[t]) * BM;
                 for (int kb = 0; kb < KB; ++kb, ++i) {
                     const int st = static_cast<int>(i % STAGES);
-                    if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_typed_error, 21))) break;
-                    const uint32_t a = ring + st * S::kStage, b = a + P * S::kA;
+                    if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_error, 21))) break;
+                    const uint32_t a = ring + st * S::kStage, b = a + S::kA;
                     mb::arrive_expect_tx(&s.full[st], S::kStage);
+                    tc::tma3(a, &ma, kb * tc::kInner, row0, 0, &s.full[st]);
+                    if (TRANS) {
+                        tc::tma3(b, &mw, kb * tc::kInner, n0, t, &s.full[st]);
+                    } else {
 #pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        tc::tma3(a + q * S::kA, &ma, kb * tc::kInner, row0, q, &s.full[st]);
-                        if (TRANS) {
-                            tc::tma4(b + q * S::kB, &mw, kb * tc::kInner, n0, t, q, &s.full[st]);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < BN / 64; ++c)
-                                tc::tma4(b + q * S::kB + c * tc::kChunkBytes, &mw, n0 + c * 64, kb * tc::kInner, t, q,
-                                         &s.full[st]);
-                        }
+                        for (int c = 0; c < BN / 64; ++c)
+                            tc::tma3(b + c * tc::kChunkBytes, &mw, n0 + c * 64, kb * tc::kInner, t, &s.full[st]);
                     }
                 }
             }
             // Every copy issued must have landed before the CTA may exit.
             for (int64_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
-                mb::wait(&s.full[j % STAGES], (j / STAGES) & 1, &g_typed_error, 22);
+                mb::wait(&s.full[j % STAGES], (j / STAGES) & 1, &g_error, 22);
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -247,13 +91,13 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
             bool ok = true;
             for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++local) {
                 const int acc = local & 1;
-                if (local >= 2 && !(ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_typed_error, 23))) break;
+                if (local >= 2 && !(ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 23))) break;
                 tc::fence_after();
                 for (int kb = 0; kb < KB; ++kb, ++i) {
                     const int st = static_cast<int>(i % STAGES);
-                    if (!(ok = mb::wait(&s.full[st], (i / STAGES) & 1, &g_typed_error, 24))) break;
+                    if (!(ok = mb::wait(&s.full[st], (i / STAGES) & 1, &g_error, 24))) break;
                     tc::fence_after();
-                    stage_mmas<P, P, BN, false, !TRANS>(ring + st * S::kStage, tmem + acc * BN, ID, kb == 0);
+                    stage_mmas<1, 1, BN, false, !TRANS>(ring + st * S::kStage, tmem + acc * BN, ID, kb == 0);
                     tc::commit(&s.empty[st]);
                 }
                 if (ok) tc::commit(&s.acc_full[acc]);
@@ -265,59 +109,20 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
         for (int64_t tile = blockIdx.x + acc * static_cast<int64_t>(gridDim.x); tile < tiles;
              tile += 2 * static_cast<int64_t>(gridDim.x), local += 2) {
             const int p = static_cast<int>(tile / g.tiles_n);
-            const int64_t n0 = tile % g.tiles_n * BN;
             const int t = find_type(s.prefix, g.types, p);
-            const int64_t row = clamp_row(g.offsets[t], g.M) + static_cast<int64_t>(p - s.prefix[t]) * BM + q * 32 + lane;
-            const bool live = row < clamp_row(g.offsets[t + 1], g.M);
-            if (!mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_typed_error, 25)) break;
+            const int64_t row0 = clamp_row(g.offsets[t], g.M) + static_cast<int64_t>(p - s.prefix[t]) * BM + q * 32;
+            const int64_t left = clamp_row(g.offsets[t + 1], g.M) - row0;
+            const bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 25);
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc::fence_after();
-            const uint32_t addr = tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
-            O* c = g.C + (live ? row * g.ldc : 0) + n0;
-#pragma unroll 1
-            for (int b0 = 0; b0 < BN && n0 + b0 < g.N; b0 += kBlock8) {
-                constexpr int W = BN < kBlock8 ? BN : kBlock8;
-                int byte = 0;
-                float inv = 0.0f;
-                if (g.saved.codes) {  // the block's exponent needs all its columns first
-                    float m = 0.0f;
-#pragma unroll 1
-                    for (int c0 = b0; c0 < b0 + W; c0 += 32) {
-                        float v[32];
-                        load_biased(addr + c0, g, t, n0 + c0, v);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) m = max_mag(m, v[j]);
-                    }
-                    byte = exponent8(m, g.r8.emin);
-                    inv = encode8(byte);
-                    if (live) g.saved.exps[row * g.saved.lde + (n0 + b0) / kBlock8] = static_cast<uint8_t>(byte);
-                }
-#pragma unroll 1
-                for (int c0 = b0; c0 < b0 + W; c0 += 32) {
-                    float v[32];
-                    load_biased(addr + c0, g, t, n0 + c0, v);
-                    const int64_t left = live ? g.N - n0 - c0 : 0;
-                    if (g.saved.codes && left > 0) {
-                        int8_t* o = g.saved.codes + row * g.saved.ld + n0 + c0;
-#pragma unroll
-                        for (int h = 0; h < 32; h += 16) {
-                            if (h + 16 <= left) {
-                                store_codes<16>(o + h, v + h, inv, byte, g.r8.top);
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 16; ++j)
-                                    if (h + j < left) o[h + j] = code8(v[h + j], inv, byte, g.r8.top);
-                            }
-                        }
-                    }
-                    act_forward<(P == 1)>(v, g.act, g.alpha);
-                    store32(c + c0, v, left, g.mode);
-                }
-            }
+            finish_rows<T, BN, true>(tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16), out, t, row0,
+                                     left < 0 ? 0 : (left < 32 ? static_cast<int>(left) : 32), tile % g.tiles_n * BN,
+                                     stage_out[warp - 4]);
             tc::fence_before();
             mb::arrive(&s.acc_empty[acc]);
         }
     }
-    tear_down<BN>(s, tmem);
+    tear_down<BN>(s, tmem, 1);
 }
 
 // ── weight kernel ────────────────────────────────────────────────────────
@@ -326,26 +131,26 @@ struct WeightTc {
     int64_t M, K, N;
     int types, tiles_k, tiles_n;
     const int32_t* offsets;
-    int64_t piece;  // rows of a type that one sum takes
+    int64_t piece;
     O* dW;
     int64_t lddw, stride_dw;
     int mode;
-    float* part;  // sums of types with several pieces: [piece][K][ldp]
+    float* part;
     int64_t ldp;
 };
 
-template <class O, int PA, int PB, int BN, bool BF16>
+template <class T, class O, int BN>
 __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __grid_constant__ CUtensorMap mx,
                                                                       const __grid_constant__ CUtensorMap my,
                                                                       const WeightTc<O> g) {
-    using S = Plan<PA, PB, BN>;
+    using S = Plan<1, 1, BN>;
     constexpr int STAGES = S::kStages;
-    constexpr uint32_t ID = tc::idesc(BF16, true, true, BM, BN);
+    constexpr uint32_t ID = tc::idesc(is_bf16<T>(), true, true, BM, BN);
     extern __shared__ uint8_t raw[];
     __shared__ Shared s;
-    const uint32_t shift = (1024 - (mb::smem_u32(raw) & 1023)) & 1023;
-    const uint32_t ring = mb::smem_u32(raw) + shift;
-    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, g.piece);
+    __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
+    const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
+    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, g.piece, 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = g.tiles_k * g.tiles_n;
     const int64_t items = static_cast<int64_t>(s.prefix[g.types]) * per;
@@ -377,23 +182,19 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
                 const Item m = item_at(it);
                 for (int r = m.row0; r < m.row1; r += tc::kInner, ++i) {
                     const int st = static_cast<int>(i % STAGES);
-                    if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_typed_error, 31))) break;
-                    const uint32_t a = ring + st * S::kStage, b = a + PA * S::kA;
+                    if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_error, 31))) break;
+                    const uint32_t a = ring + st * S::kStage, b = a + S::kA;
                     mb::arrive_expect_tx(&s.full[st], S::kStage);
 #pragma unroll
-                    for (int q = 0; q < PA; ++q)
+                    for (int c = 0; c < BM / 64; ++c)
+                        tc::tma3(a + c * tc::kChunkBytes, &mx, m.k0 + c * 64, r, 0, &s.full[st]);
 #pragma unroll
-                        for (int c = 0; c < BM / 64; ++c)
-                            tc::tma3(a + q * S::kA + c * tc::kChunkBytes, &mx, m.k0 + c * 64, r, q, &s.full[st]);
-#pragma unroll
-                    for (int q = 0; q < PB; ++q)
-#pragma unroll
-                        for (int c = 0; c < BN / 64; ++c)
-                            tc::tma3(b + q * S::kB + c * tc::kChunkBytes, &my, m.n0 + c * 64, r, q, &s.full[st]);
+                    for (int c = 0; c < BN / 64; ++c)
+                        tc::tma3(b + c * tc::kChunkBytes, &my, m.n0 + c * 64, r, 0, &s.full[st]);
                 }
             }
             for (int64_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
-                mb::wait(&s.full[j % STAGES], (j / STAGES) & 1, &g_typed_error, 32);
+                mb::wait(&s.full[j % STAGES], (j / STAGES) & 1, &g_error, 32);
         }
     } else if (warp == 1) {
         int64_t i = 0;
@@ -402,29 +203,18 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
         for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x, ++local) {
             const Item m = item_at(it);
             const int acc = local & 1;
-            if (local >= 2) ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_typed_error, 33);
+            if (local >= 2) ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 33);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             tc::fence_after();
             for (int r = m.row0; r < m.row1; r += tc::kInner, ++i) {
                 const int st = static_cast<int>(i % STAGES);
-                ok = mb::wait(&s.full[st], (i / STAGES) & 1, &g_typed_error, 34);
+                ok = mb::wait(&s.full[st], (i / STAGES) & 1, &g_error, 34);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 tc::fence_after();
-                const int valid = m.row1 - r;
-                if (valid < tc::kInner) {
-                    // Rows of the next type (or piece): zero in both operands (0 x NaN would not do).
-                    uint8_t* base = raw + shift + st * S::kStage;
-                    for (uint32_t o = valid * 128 + lane * 16; o < S::kStage; o += 512) {
-                        // row o / 128 of its 64-row chunk; skip to the next chunk's first invalid row
-                        const uint32_t in = o % tc::kChunkBytes;
-                        if (in >= static_cast<uint32_t>(valid) * 128)
-                            *reinterpret_cast<uint4*>(base + o) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
+                // Rows of the next type (or piece): zero in both operands (0 x NaN would not do).
+                if (m.row1 - r < tc::kInner) zero_rows(ring + st * S::kStage, S::kStage, m.row1 - r);
                 if (lane == 0) {
-                    stage_mmas<PA, PB, BN, true, true>(ring + st * S::kStage, tmem + acc * BN, ID, r == m.row0);
+                    stage_mmas<1, 1, BN, true, true>(ring + st * S::kStage, tmem + acc * BN, ID, r == m.row0);
                     tc::commit(&s.empty[st]);
                 }
                 __syncwarp();
@@ -437,46 +227,71 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
         for (int64_t it = blockIdx.x + acc * static_cast<int64_t>(gridDim.x); it < items;
              it += 2 * static_cast<int64_t>(gridDim.x), local += 2) {
             const Item m = item_at(it);
-            if (!mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_typed_error, 35)) break;
+            const bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 35);
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc::fence_after();
             const uint32_t addr = tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
-            const int64_t k = m.k0 + q * 32 + lane;
-            const bool live = k < g.K;
+            const int64_t k = m.k0 + q * 32, left_k = g.K - k;
+            const int rows = left_k < 0 ? 0 : (left_k < 32 ? static_cast<int>(left_k) : 32);
 #pragma unroll 1
             for (int c0 = 0; c0 < BN && m.n0 + c0 < g.N; c0 += 32) {
                 float v[32];
                 tc::load32(addr + c0, v);
                 const int64_t n = m.n0 + c0;
-                if (!live) continue;
-                if (m.whole) store32(g.dW + m.t * g.stride_dw + k * g.lddw + n, v, g.N - n, g.mode);
-                else store32(g.part + (m.p * g.K + k) * g.ldp + n, v, g.ldp - n, 2);
+                if (m.whole) {
+                    O* o = g.dW + m.t * g.stride_dw + k * g.lddw + n;
+                    // shared memory has room to stage rows of T, not of fp32
+                    if constexpr (sizeof(O) == sizeof(T)) store_rows(o, g.lddw, rows, g.N - n, v, g.mode, stage_out[warp - 4]);
+                    else store_rows(o, g.lddw, rows, g.N - n, v, g.mode == 0 ? -1 : g.mode, static_cast<O*>(nullptr));
+                } else {
+                    store_rows(g.part + (m.p * g.K + k) * g.ldp + n, g.ldp, rows, g.ldp - n, v, 2,
+                               static_cast<float*>(nullptr));
+                }
             }
             tc::fence_before();
             mb::arrive(&s.acc_empty[acc]);
         }
+        // types without rows: zero
+        for (int t = blockIdx.x; t < g.types; t += gridDim.x) {
+            if (s.prefix[t + 1] != s.prefix[t]) continue;
+            for (int64_t k = 0; k < g.K; ++k)
+                for (int64_t n = threadIdx.x - 128; n < g.N; n += 256)
+                    g.dW[t * g.stride_dw + k * g.lddw + n] = from_f32<O>(0.0f);
+        }
     }
-    tear_down<BN>(s, tmem);
+    tear_down<BN>(s, tmem, 1);
 }
 
-// dW of the types that the weight kernel did not finish: the sum of a type's
-// pieces in their order, zero for a type without rows.
+// dW and db of the types with several pieces: the sum of the pieces in their order.
 template <class O>
-__global__ void __launch_bounds__(256) typed_weight_join_kernel(const WeightTc<O> g) {
+struct JoinArgs {
+    int64_t M, K, N, piece, ldp;
+    const int32_t* offsets;
+    const float *part, *db_part;
+    O* dW;
+    int64_t lddw, stride_dw;
+    float* db;  // nullable
+};
+
+template <class O>
+__global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O> g) {
     __shared__ int prefix[kMaxTypes + 1];
     const int t = blockIdx.y;
     const int b = clamp_row(g.offsets[t], g.M), e = clamp_row(g.offsets[t + 1], g.M);
-    const int64_t n = e > b ? (e - b + g.piece - 1) / g.piece : 0;
-    if (n == 1) return;
-    if (n > 1 && threadIdx.x < 32) scan_types(g.offsets, t, g.M, g.piece, prefix);
+    if (e - b <= g.piece) return;  // one piece: the weight kernel wrote it
+    const int n = static_cast<int>((e - b + g.piece - 1) / g.piece);
+    if (threadIdx.x < 32) scan_types(g.offsets, t, g.M, g.piece, prefix);
     __syncthreads();
-    const float* part = n > 1 ? g.part + static_cast<int64_t>(prefix[t]) * g.K * g.ldp : nullptr;
-    const int64_t vecs = g.ldp / 4, total = g.K * vecs;
+    const int64_t p = prefix[t];
+    const float* part = g.part + p * g.K * g.ldp;
+    const int64_t vecs = g.ldp / 4, total = g.K * vecs, next = g.K * g.ldp;
     for (int64_t v = blockIdx.x * 256 + threadIdx.x; v < total; v += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t k = v / vecs, c = (v - k * vecs) * 4;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int64_t q = 0; q < n; ++q) {
-            const float4 x = *reinterpret_cast<const float4*>(part + (q * g.K + k) * g.ldp + c);
+        const float* q = part + k * g.ldp + c;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i, q += next) {
+            const float4 x = *reinterpret_cast<const float4*>(q);
             sum.x += x.x;
             sum.y += x.y;
             sum.z += x.z;
@@ -484,253 +299,199 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const WeightTc<O
         }
         O* o = g.dW + t * g.stride_dw + k * g.lddw + c;
         const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (c + 4 <= g.N && (reinterpret_cast<uintptr_t>(o) % (4 * sizeof(O))) == 0) {
+            store_v<O, 4>(o, y);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + j < g.N) o[j] = from_f32<O>(y[j]);
+            for (int j = 0; j < 4; ++j)
+                if (c + j < g.N) o[j] = from_f32<O>(y[j]);
+        }
     }
+    if (g.db)
+        for (int64_t c = blockIdx.x * 256 + threadIdx.x; c < g.N; c += static_cast<int64_t>(gridDim.x) * 256) {
+            float sum = 0.0f;
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) sum += g.db_part[(p + i) * g.N + c];
+            g.db[t * g.N + c] = sum;
+        }
 }
 
 // ── operands ─────────────────────────────────────────────────────────────
-// P 16-bit planes [P][rows][ld] of a matrix whose row r lies at
+// A 16-bit matrix with 16-byte aligned rows, from one whose row r lies at
 // (r / inner) * stride + (r % inner) * lds.
-template <class T, class H, int P>
-__global__ void __launch_bounds__(256) planes_kernel(int64_t rows, int64_t cols, const T* src, int64_t inner,
-                                                     int64_t stride, int64_t lds, H* dst, int64_t ld) {
+template <class T>
+__global__ void __launch_bounds__(256) align_kernel(int64_t rows, int64_t cols, const T* src, int64_t inner,
+                                                    int64_t stride, int64_t lds, T* dst, int64_t ld) {
     const int64_t vecs = ld / 8, total = rows * vecs;
     for (int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; v < total;
          v += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = v / vecs, c = (v - r * vecs) * 8;
         const T* p = src + r / inner * stride + r % inner * lds + c;
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = c + j < cols ? to_f32(p[j]) : 0.0f;
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            Raw<H, 8> k;
-            narrow(x, k);
-            if (P > 1) {
-                float top[8];
-                widen(k, top);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    // a finite value above bf16's greatest rounds to infinity: take the greatest
-                    if (isinf(top[j]) && !isinf(x[j])) top[j] = copysignf(3.3895314e38f, x[j]);
-                    x[j] = __fsub_rn(x[j], top[j]);
-                }
-                narrow(top, k);
-            }
-            *reinterpret_cast<Raw<H, 8>*>(dst + (q * rows + r) * ld + c) = k;
-        }
+        *reinterpret_cast<Raw<T, 8>*>(dst + r * ld + c) =
+            gather_raw<T, 8>([&](int j) { return c + j < cols ? p[j] : from_f32<T>(0.0f); });
     }
 }
 
-// One 16-bit plane of a saved matrix, exactly.
-template <class H>
-__global__ void __launch_bounds__(256) saved_plane_kernel(int64_t rows, int64_t cols, Saved8 s, H* dst, int64_t ld) {
-    const int64_t vecs = ld / 8, total = rows * vecs;
-    for (int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; v < total;
-         v += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = v / vecs, c = (v - r * vecs) * 8;
-        const int byte = s.exps[r * s.lde + c / kBlock8];
-        const uint2 in = *reinterpret_cast<const uint2*>(s.codes + r * s.ld + c);
-        float x[8];
-        values4(in.x, byte, x);
-        values4(in.y, byte, x + 4);
-        store_v<H, 8>(dst + r * ld + c, x);
-    }
-}
-
-template <class T> struct Half { using type = T; static constexpr int planes = 1; };
-template <> struct Half<float> { using type = __nv_bfloat16; static constexpr int planes = 3; };
-
-// A matrix (or `types` of them) as 16-bit planes: in place, or in scratch.
-template <class H>
+// A matrix (or a batch of them) that TMA can read: in place, or a copy in scratch.
+template <class T>
 struct Operand {
-    const H* p = nullptr;
-    int64_t ld = 0, stride = 0, plane = 0;  // elements
-    H* own = nullptr;
+    const T* p = nullptr;
+    int64_t ld = 0, stride = 0;  // elements
+    T* own = nullptr;
     cudaStream_t s = nullptr;
+    Operand(int64_t batch, int64_t rows, int64_t cols, const T* src, int64_t lds, int64_t src_stride, cudaStream_t st)
+        : s(st) {
+        if (readable(batch, src, lds, src_stride)) {
+            p = src;
+            ld = lds;
+            stride = batch == 1 ? rows * lds : src_stride;
+            return;
+        }
+        ld = (cols + 7) / 8 * 8;
+        stride = rows * ld;
+        own = static_cast<T*>(scratch_alloc(static_cast<size_t>(batch * stride) * 2, st));
+        p = own;
+        const int64_t want = ceil_div(batch * rows * (ld / 8), 256);
+        launch("typed_align", align_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(want, num_sms() * 8))),
+               dim3(256), 0, st, batch * rows, cols, src, rows, src_stride, lds, own, ld);
+    }
     ~Operand() {
         if (own) scratch_free(own, s);
     }
-    Operand() = default;
     Operand(const Operand&) = delete;
     Operand& operator=(const Operand&) = delete;
 
-    void make(int64_t rows, int64_t cols, int planes, cudaStream_t st) {
-        s = st;
-        ld = (cols + 7) / 8 * 8;
-        plane = rows * ld;
-        own = static_cast<H*>(scratch_alloc(static_cast<size_t>(planes * plane) * 2, st));
-        p = own;
+    static bool readable(int64_t batch, const T* src, int64_t lds, int64_t stride) {
+        return rows_aligned16(src, lds, 2) && (batch == 1 || stride % 8 == 0);
+    }
+    CUtensorMap map(int64_t batch, int64_t rows, int64_t cols, int box_rows) const {
+        const int64_t dims[3] = {cols, rows, batch}, strides[2] = {ld, stride};
+        const int box[3] = {64, box_rows, 1};
+        return tc::map16<3>(p, is_bf16<T>(), dims, strides, box);
     }
 };
 
-unsigned prep_grid(int64_t rows, int64_t ld) {
-    return static_cast<unsigned>(std::min<int64_t>(ceil_div(rows * (ld / 8), 256), int64_t(num_sms()) * 8));
-}
-
-// `batch` matrices of rows x cols, ld and stride apart.
-template <class T>
-void make_operand(Operand<typename Half<T>::type>& o, int64_t batch, int64_t rows, int64_t cols, const T* src,
-                  int64_t ld, int64_t stride, cudaStream_t s) {
-    using H = typename Half<T>::type;
-    constexpr int P = Half<T>::planes;
-    if constexpr (P == 1) {
-        if (rows_aligned16(src, ld, 2) && (batch == 1 || stride % 8 == 0) && rows * ld * 2 < (int64_t(1) << 39) &&
-            stride * 2 < (int64_t(1) << 39)) {
-            o.p = src;
-            o.ld = ld;
-            o.stride = batch == 1 ? rows * ld : stride;
-            o.plane = batch * o.stride;
-            return;
-        }
-    }
-    o.make(batch * rows, cols, P, s);
-    o.stride = rows * o.ld;
-    launch("typed_operand", planes_kernel<T, H, P>, dim3(prep_grid(batch * rows, o.ld)), dim3(256), 0, s, batch * rows,
-           cols, src, rows, stride, ld, o.own, o.ld);
-}
-
-template <class H>
-void make_saved_operand(Operand<H>& o, int64_t rows, int64_t cols, const Saved8& saved, cudaStream_t s) {
-    o.make(rows, cols, 1, s);
-    o.stride = rows * o.ld;
-    launch("typed_operand", saved_plane_kernel<H>, dim3(prep_grid(rows, o.ld)), dim3(256), 0, s, rows, cols, saved,
-           o.own, o.ld);
-}
-
-template <class H>
-constexpr bool is_bf16() { return std::is_same<H, __nv_bfloat16>::value; }
-
-template <class H>
-CUtensorMap rows_map(const Operand<H>& o, int64_t rows, int64_t cols, int planes, int box_rows) {
-    const int64_t dims[3] = {cols, rows, planes}, strides[2] = {o.ld, std::max<int64_t>(o.plane, 8)};
-    const int box[3] = {64, box_rows, 1};
-    return tc::map16<3>(o.p, is_bf16<H>(), dims, strides, box);
-}
-
-template <class K, class... A>
-void run_tc(const char* name, K kern, uint32_t smem, int64_t tiles, cudaStream_t s, A... args) {
-    TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    launch(name, kern, dim3(static_cast<unsigned>(std::min<int64_t>(tiles, num_sms()))), dim3(kThreads), smem, s,
-           args...);
-}
-
-template <class O>
-void join_pieces(const WeightTc<O>& g, int types, cudaStream_t s) {
-    launch("typed_weight_join", typed_weight_join_kernel<O>,
-           dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(g.K * g.ldp / 4, 256), std::max(8, 16384 / types))),
-                static_cast<unsigned>(types)),
-           dim3(256), 0, s, g);
-}
-
-// Tile width.  Columns that no output has cost tensor time, and a wide tile
-// reads the rows fewer times.
-int tile_width(int64_t N, int widest) { return N <= 64 ? 64 : (N <= 128 || widest == 128 ? 128 : 256); }
-
-}  // namespace
-
 template <class T, bool TRANS>
-void typed_rows_tc(const RowsArgs<T>& a, cudaStream_t s) {
-    using H = typename Half<T>::type;
-    constexpr int P = Half<T>::planes;
-    Operand<H> A, W;
-    make_operand<T>(A, 1, a.M, a.K, a.A, a.lda, 0, s);
+void typed_rows_tma(const RowsArgs<T>& a, cudaStream_t s) {
+    const Operand<T> A(1, a.M, a.K, a.A, a.lda, 0, s);
     // W[t] is K x N in the forward pass, N x K in the input gradient.
     const int64_t wr = TRANS ? a.N : a.K, wc = TRANS ? a.K : a.N;
-    make_operand<T>(W, a.types, wr, wc, a.W, a.ldw, a.stride_w, s);
-    const CUtensorMap ma = rows_map(A, a.M, a.K, P, BM);
+    const Operand<T> W(a.types, wr, wc, a.W, a.ldw, a.stride_w, s);
+    const CUtensorMap ma = A.map(1, a.M, a.K, BM);
+    const int64_t pieces = a.M / BM + std::min<int64_t>(a.types, a.M);
+    const RowsOut<T> out{a.N, a.bias, a.act, a.alpha, a.C, a.ldc, store_mode(a.C, a.ldc * 2), a.saved, a.r8};
     const auto go = [&](auto bn) {
         constexpr int BN = decltype(bn)::value;
-        const int64_t dims[4] = {wc, wr, a.types, P}, strides[3] = {W.ld, W.stride, W.plane};
-        const int box[4] = {64, TRANS ? BN : 64, 1, 1};
-        const CUtensorMap mw = tc::map16<4>(W.p, is_bf16<H>(), dims, strides, box);
-        RowsTc<T> g{a.M, a.K, a.N, a.types, static_cast<int>(ceil_div(a.N, BN)), a.offsets, a.bias, a.act, a.alpha,
-                    a.C, a.ldc, store_mode(a.C, a.ldc), a.saved, a.r8};
-        run_tc("typed_rows", typed_rows_tc_kernel<T, P, BN, TRANS, is_bf16<H>()>, Plan<P, P, BN>::kBytes,
-               (a.M / BM + a.types) * g.tiles_n, s, ma, mw, g);
+        const CUtensorMap mw = W.map(a.types, wr, wc, TRANS ? BN : 64);
+        const RowsTc g{a.M, a.K, a.types, static_cast<int>(ceil_div(a.N, BN)), a.offsets};
+        run("typed_rows", typed_rows_tc_kernel<T, BN, TRANS>, kThreads, Plan<1, 1, BN>::kBytes, pieces * g.tiles_n, s,
+            ma, mw, g, out);
     };
-    switch (tile_width(a.N, P == 1 ? 256 : 128)) {
+    switch (tile_width(pieces, a.N, 256, a.saved.codes != nullptr)) {
         case 64: go(std::integral_constant<int, 64>{}); break;
         case 128: go(std::integral_constant<int, 128>{}); break;
-        default:
-            if constexpr (P == 1) go(std::integral_constant<int, 256>{});
+        default: go(std::integral_constant<int, 256>{});
     }
 }
 
 template <class T, class O>
-void typed_weight_tc(const WeightArgs<T, O>& a, cudaStream_t s) {
-    using H = typename Half<T>::type;
-    constexpr int PB = Half<T>::planes;
-    Operand<H> X, Y;
-    const bool saved = a.saved.codes != nullptr;
-    if (a.M == 0) {  // no rows: dW is zero
-        WeightTc<O> g{};
-        g.K = a.K;
-        g.N = a.N;
-        g.offsets = a.offsets;
-        g.piece = 1;
-        g.dW = a.dW;
-        g.lddw = a.lddw;
-        g.stride_dw = a.stride_dw;
-        g.ldp = (a.N + 7) / 8 * 8;
-        join_pieces(g, a.types, s);
-        return;
-    }
-    if (saved) make_saved_operand<H>(X, a.M, a.K, a.saved, s);
-    else make_operand<T>(X, 1, a.M, a.K, a.X, a.ldx, 0, s);
-    make_operand<T>(Y, 1, a.M, a.N, a.dY, a.lddy, 0, s);
-    const CUtensorMap my = rows_map(Y, a.M, a.N, PB, 64);
-    const auto go = [&](auto bn, auto pa) {
-        constexpr int BN = decltype(bn)::value, PA = decltype(pa)::value;
-        const CUtensorMap mx = rows_map(X, a.M, a.K, PA, 64);
-        WeightTc<O> g{a.M, a.K, a.N, a.types, static_cast<int>(ceil_div(a.K, BM)), static_cast<int>(ceil_div(a.N, BN)),
-                      a.offsets, 0, a.dW, a.lddw, a.stride_dw, store_mode(a.dW, a.lddw) , nullptr, (a.N + 7) / 8 * 8};
-        if (a.stride_dw * sizeof(O) % 32 != 0) g.mode = a.stride_dw * sizeof(O) % 16 == 0 ? std::min(g.mode, 1) : 0;
-        const int64_t per = int64_t(g.tiles_k) * g.tiles_n;
-        // About 2.5 sums per SM: enough to even out types of unequal sizes,
-        // few enough that the partial sums' traffic stays small.
-        g.piece = std::max<int64_t>(128, ceil_div(a.M * per * 2, int64_t(num_sms()) * 5 * 64) * 64);
-        const int64_t pieces = a.M / g.piece + std::min<int64_t>(a.types, a.M);
-        Scratch<float> part(a.M > g.piece ? static_cast<size_t>(pieces * a.K * g.ldp) : 1, s);
-        g.part = part.p;
-        run_tc("typed_weight", typed_weight_tc_kernel<O, PA, PB, BN, is_bf16<H>()>, Plan<PA, PB, BN>::kBytes,
-               pieces * per, s, mx, my, g);
-        join_pieces(g, a.types, s);
+void typed_weight_tma(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s) {
+    const Operand<T> X(1, a.M, a.K, a.X, a.ldx, 0, s), Y(1, a.M, a.N, a.dY, a.lddy, 0, s);
+    const CUtensorMap mx = X.map(1, a.M, a.K, 64), my = Y.map(1, a.M, a.N, 64);
+    const WeightTc<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, a.offsets, w.piece, a.dW, a.lddw, a.stride_dw,
+                        store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O)), w.part, w.ldp};
+    const auto go = [&](auto bn) {
+        constexpr int BN = decltype(bn)::value;
+        run("typed_weight", typed_weight_tc_kernel<T, O, BN>, kThreads, Plan<1, 1, BN>::kBytes, w.items, s, mx, my, g);
     };
-    const auto with_planes = [&](auto bn) {
-        if constexpr (PB == 1) go(bn, std::integral_constant<int, 1>{});
-        else if (saved) go(bn, std::integral_constant<int, 1>{});
-        else go(bn, std::integral_constant<int, PB>{});
-    };
-    switch (tile_width(a.N, PB == 1 ? 256 : 128)) {
-        case 64: with_planes(std::integral_constant<int, 64>{}); break;
-        case 128: with_planes(std::integral_constant<int, 128>{}); break;
-        default:
-            if constexpr (PB == 1) with_planes(std::integral_constant<int, 256>{});
+    switch (w.BN) {
+        case 64: go(std::integral_constant<int, 64>{}); break;
+        case 128: go(std::integral_constant<int, 128>{}); break;
+        default: go(std::integral_constant<int, 256>{});
     }
 }
 
-#define TG_TYPED(T)                                                  \
-    template void typed_rows_tc<T, false>(const RowsArgs<T>&, cudaStream_t); \
-    template void typed_rows_tc<T, true>(const RowsArgs<T>&, cudaStream_t);  \
-    template void typed_weight_tc<T, T>(const WeightArgs<T, T>&, cudaStream_t);
+// 2 M K N above which 16-bit operands that TMA cannot read are worth an
+// aligned copy, and dW's operands a kernel that does not add up db on the way.
+constexpr double kLargeFlops = 1e10;
+
+}  // namespace
+
+template <class T, bool TRANS>
+void typed_rows(const RowsArgs<T>& a, cudaStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        const bool readable = Operand<T>::readable(1, a.A, a.lda, 0) &&
+                              Operand<T>::readable(a.types, a.W, a.ldw, a.stride_w);
+        if (readable || 2.0 * a.M * a.K * a.N > kLargeFlops) {
+            typed_rows_tma<T, TRANS>(a, s);
+            return;
+        }
+    }
+    typed_rows_any<T, TRANS>(a, s);
+}
+
+template <class T, class O>
+void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
+    if (a.M == 0) {
+        for (int t = 0; t < a.types; ++t)
+            TG_CUDA(cudaMemset2DAsync(a.dW + t * a.stride_dw, a.lddw * sizeof(O), 0, a.N * sizeof(O), a.K, s));
+        if (a.db) TG_CUDA(cudaMemsetAsync(a.db, 0, static_cast<size_t>(a.types * a.N) * 4, s));
+        return;
+    }
+    const bool saved = a.saved.codes != nullptr;
+    const bool large = sizeof(T) == 2 && 2.0 * a.M * a.K * a.N > kLargeFlops;
+    WeightPlan w{};
+    const int widest = large ? 256 : 128;
+    w.BN = a.N <= 64 ? 64 : (a.N <= 128 || widest == 128 ? 128 : 256);
+    w.dy_by_tma = saved && large && rows_aligned16(a.dY, a.lddy, sizeof(T));
+    if (saved && !w.dy_by_tma) w.BN = std::min(w.BN, 128);
+    w.tiles_k = static_cast<int>(ceil_div(a.K, BM));
+    w.tiles_n = static_cast<int>(ceil_div(a.N, w.BN));
+    const int64_t per = int64_t(w.tiles_k) * w.tiles_n;
+    // About 2.5 sums per SM: enough to even out types of unequal sizes, few
+    // enough that the partial sums' traffic stays small.
+    w.piece = std::max<int64_t>(128, ceil_div(a.M * per * 2, int64_t(num_sms()) * 5 * 64) * 64);
+    const int64_t pieces = a.M / w.piece + std::min<int64_t>(a.types, a.M);
+    w.items = std::max<int64_t>(pieces * per, std::min(a.types, num_sms()));
+    w.ldp = (a.N + 7) / 8 * 8;
+    const bool joined = a.M > w.piece;
+    Scratch<float> part(joined ? static_cast<size_t>(pieces * (a.K * w.ldp + a.N)) : 1, s);
+    w.part = part.p;
+    w.db_part = part.p + (joined ? pieces * a.K * w.ldp : 0);
+    bool db_joined = a.db != nullptr;
+    if constexpr (sizeof(T) == 2) {
+        if ((large && !saved) || w.dy_by_tma) {
+            db_joined = false;
+            if (a.db) typed_bias<T>(a.M, a.N, a.types, a.offsets, a.dY, a.lddy, a.db, s);
+            if (saved) typed_weight_any<T, O>(a, w, s);
+            else typed_weight_tma<T, O>(a, w, s);
+        } else {
+            typed_weight_any<T, O>(a, w, s);
+        }
+    } else {
+        typed_weight_any<T, O>(a, w, s);
+    }
+    if (joined) {
+        const JoinArgs<O> j{a.M, a.K, a.N, w.piece, w.ldp, a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
+                            db_joined ? a.db : nullptr};
+        const int64_t want = ceil_div(a.K * w.ldp / 4, 256);
+        launch("typed_weight_join", typed_weight_join_kernel<O>,
+               dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(8, 16384 / a.types))),
+                    static_cast<unsigned>(a.types)),
+               dim3(256), 0, s, j);
+    }
+}
+
+#define TG_TYPED(T)                                                       \
+    template void typed_rows<T, false>(const RowsArgs<T>&, cudaStream_t); \
+    template void typed_rows<T, true>(const RowsArgs<T>&, cudaStream_t);  \
+    template void typed_weight<T, T>(const WeightArgs<T, T>&, cudaStream_t);
 TG_TYPED(float)
 TG_TYPED(__nv_bfloat16)
 TG_TYPED(__half)
-template void typed_weight_tc<__nv_bfloat16, float>(const WeightArgs<__nv_bfloat16, float>&, cudaStream_t);
-template void typed_weight_tc<__half, float>(const WeightArgs<__half, float>&, cudaStream_t);
+template void typed_weight<__nv_bfloat16, float>(const WeightArgs<__nv_bfloat16, float>&, cudaStream_t);
+template void typed_weight<__half, float>(const WeightArgs<__half, float>&, cudaStream_t);
 
-// Reads and clears the typed kernels' error word (the stream is idle).
-int typed_take_error() {
-    int h = 0;
-    TG_CUDA(cudaMemcpyFromSymbol(&h, g_typed_error, sizeof(int)));
-    if (h) {
-        const int zero = 0;
-        TG_CUDA(cudaMemcpyToSymbol(g_typed_error, &zero, sizeof(int)));
-    }
-    return h;
-}
+int typed_tc_take_error() { return take_error(); }
 
 }  // namespace tg
