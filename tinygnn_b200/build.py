@@ -4,7 +4,8 @@
 kernel with ``-gencode arch=compute_100a,code=sm_100a -lineinfo`` into
 tinygnn_b200/lib/libtinygnn_b200.so, then the pybind11 module
 tinygnn_b200/tinygnn/_core (TinyGNN's Python API over the C++ API in that
-library).  No GPU is needed to build.
+library) and tinygnn_b200/_torch_ops (the training operators on torch
+tensors).  No GPU is needed to build.
 
 This file imports nothing from the package, so it can be loaded by path
 (``__graft_entry__.build()``) before the library exists; the package's
@@ -31,6 +32,19 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 def pymodule_path() -> str:
     return os.path.join(PYMOD_DIR, "_core" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+
+
+def torchops_path() -> str:
+    return os.path.join(HERE, "_torch_ops" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+
+
+def _torch_flags() -> list[str]:
+    """torch's directories, without importing it (the build needs no more)."""
+    import importlib.util
+    root = os.path.dirname(importlib.util.find_spec("torch").origin)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include")]
+    # system headers: warnings in them are not this project's
+    return [f"TORCH_INCLUDES={' '.join('-isystem ' + i for i in inc)}", f"TORCH_LIB={os.path.join(root, 'lib')}"]
 
 
 def _python_flags() -> list[str]:
@@ -60,19 +74,19 @@ def _make(args: list[str], quiet: bool) -> None:
 
 
 def build(jobs: int = 0, quiet: bool = True) -> str:
-    """Compile (or bring up to date) the library and the Python module."""
+    """Compile (or bring up to date) the library and the Python modules."""
     jobs = jobs or min(32, os.cpu_count() or 8)
     with _lock():
         _make([f"-j{jobs}"], quiet)
-        _make(["pymodule", *_python_flags()], quiet)
+        _make([f"-j{jobs}", "pymodule", "torchops", *_python_flags(), *_torch_flags()], quiet)
     return LIB_PATH
 
 
 def ensure_built(pymodule: bool = False) -> str:
-    """Build the library (and, if asked, the Python module) when it is
+    """Build the library (and, if asked, TinyGNN's Python module) when it is
     missing.  Raises ImportError when it is missing and nvcc is not there
     to build it: the package has no CPU path."""
-    want = [LIB_PATH] + ([pymodule_path()] if pymodule else [])
+    want = [LIB_PATH, torchops_path()] + ([pymodule_path()] if pymodule else [])
     if all(os.path.exists(p) for p in want):
         return LIB_PATH
     if not (os.path.exists(NVCC) or shutil.which("nvcc")):
