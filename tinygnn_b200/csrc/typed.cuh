@@ -84,14 +84,108 @@ struct WeightArgs {
     float* db;  // types x N, nullable
 };
 
-// How a weight gradient is cut up: pieces of at most `piece` rows of a type,
-// each summed by one CTA per tile of dW; types of several pieces leave partial
-// sums [piece][K][ldp] (and [piece][N] of db) that a second kernel adds up in
+// ── How a weight gradient is cut up ──────────────────────────────────────
+// Each tile of each type's dW is a sum over the type's rows, in steps of 64.
+// An item is a tile and a piece of its type's rows, for one CTA.  A type is
+// one piece unless it has more steps than an SM's share of all the steps
+// (`slots` SMs, `per` tiles a type); then it is cut into the fewest equal
+// pieces that have no more.  Items run longest first, dealt out to the CTAs
+// back and forth, so the CTAs' totals come out nearly equal without a counter
+// in memory, and few types are cut at all: a cut type leaves partial sums
+// [piece][K][ldp] (and [piece][N] of db) that a second kernel adds up in
 // their order.
+constexpr int kStep = 64;
+constexpr int kSortTypes = 256;  // more types than this keep their order (many items even out anyway)
+
+__device__ __forceinline__ int rows_of(const int32_t* offsets, int t, int64_t M) {
+    const int b = clamp_row(offsets[t], M), e = clamp_row(offsets[t + 1], M);
+    return e > b ? e - b : 0;
+}
+// Rows of the longest piece, from the sum of all types' steps.
+__device__ __forceinline__ int64_t piece_limit(int64_t steps, int per, int slots) {
+    const int64_t share = (steps * per + slots - 1) / slots;
+    return (share < 2 ? 2 : share) * kStep;
+}
+__device__ __forceinline__ int piece_count(int n, int64_t limit) { return static_cast<int>((n + limit - 1) / limit); }
+// Rows of each piece (the last may have fewer; none is empty, since this is at most `limit`).
+__device__ __forceinline__ int piece_rows(int n, int count) {
+    return count <= 1 ? n : ((n + count - 1) / count + kStep - 1) / kStep * kStep;
+}
+// Whether type u's pieces come before type t's.
+__device__ __forceinline__ bool piece_before(int types, int rows_u, int u, int rows_t, int t) {
+    return types > kSortTypes ? u < t : rows_u > rows_t || (rows_u == rows_t && u < t);
+}
+
+// One warp: order[i] = the i-th type, prefix[i] = the pieces before it.
+__device__ __forceinline__ void plan_pieces(const int32_t* offsets, int types, int64_t M, int per, int slots,
+                                            int* prefix, uint16_t* order) {
+    const int lane = threadIdx.x & 31;
+    int64_t steps = 0;
+    for (int t = lane; t < types; t += 32) steps += (rows_of(offsets, t, M) + kStep - 1) / kStep;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, o);
+    const int64_t limit = piece_limit(steps, per, slots);
+    if (types > kSortTypes) {
+        for (int t = lane; t < types; t += 32) order[t] = static_cast<uint16_t>(t);
+    } else {
+        for (int t = lane; t < types; t += 32) {
+            const int n = rows_of(offsets, t, M);
+            prefix[t] = piece_rows(n, piece_count(n, limit));
+        }
+        __syncwarp();
+        for (int t = lane; t < types; t += 32) {
+            const int key = prefix[t];
+            int rank = 0;
+            for (int u = 0; u < types; ++u) rank += piece_before(types, prefix[u], u, key, t);
+            order[rank] = static_cast<uint16_t>(t);
+        }
+    }
+    __syncwarp();
+    int carry = 0;
+    for (int i0 = 0; i0 < types; i0 += 32) {
+        const int i = i0 + lane;
+        int n = i < types ? piece_count(rows_of(offsets, order[i], M), limit) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) n += up;
+        }
+        if (i < types) prefix[i + 1] = carry + n;
+        carry += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+}
+
+// Item number `it` in the order above.
+struct WeightItem {
+    int t, p;        // type, piece (of all)
+    int in;          // tile of the type
+    int64_t r0, r1;  // rows
+    bool whole;      // the type is one piece
+};
+__device__ __forceinline__ WeightItem weight_item(const int32_t* offsets, int types, int64_t M, int per,
+                                                  const int* prefix, const uint16_t* order, int64_t it) {
+    WeightItem m;
+    m.p = static_cast<int>(it / per);
+    m.in = static_cast<int>(it - static_cast<int64_t>(m.p) * per);
+    const int i = find_type(prefix, types, m.p);
+    m.t = order[i];
+    const int b = clamp_row(offsets[m.t], M), e = clamp_row(offsets[m.t + 1], M);
+    const int count = prefix[i + 1] - prefix[i], len = piece_rows(e - b, count);
+    m.r0 = b + static_cast<int64_t>(m.p - prefix[i]) * len;
+    m.r1 = m.r0 + len < e ? m.r0 + len : e;
+    m.whole = count == 1;
+    return m;
+}
+// The item that CTA `cta` of `ctas` takes in its round `r`: back and forth.
+__device__ __forceinline__ int64_t dealt(int64_t r, int64_t cta, int64_t ctas) {
+    return r * ctas + (r & 1 ? ctas - 1 - cta : cta);
+}
+
 struct WeightPlan {
     int BN;  // columns of a tile
-    int tiles_k, tiles_n;
-    int64_t piece, ldp, items;
+    int tiles_k, tiles_n, slots;
+    int64_t ldp, items;
     float *part, *db_part;
     bool dy_by_tma;  // typed_weight_any: dY by TMA, db not summed on the way
 };

@@ -46,9 +46,10 @@ struct AnyArgs {
     Saved8 a8;  // the first operand in 8 bits (weight only)
     const T* B;
     int64_t ldb, stride_b;
-    int a_vec, b_vec;  // rows 16-byte aligned
+    int a_align, b_align;
     // weight
-    int64_t piece, stride_c, ldp;
+    int slots;
+    int64_t stride_c, ldp;
     float* part;
     int out_f32;
     float *db, *db_part;
@@ -62,42 +63,39 @@ struct Source {
     int rows, cols;  // of the tile, how many exist
 };
 
+// How an operand's rows are aligned.
+enum Align { kElement, kPair, kVector };  // to one value, two values, 16 bytes
+
 // Eight values at p, of which the first `n` exist.
 template <class T>
-__device__ __forceinline__ Raw<T, 8> load8(const T* p, int n, bool vec) {
+__device__ __forceinline__ void load8(const T* p, int n, uint32_t* w) {
     if (n >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            Raw<T, 8> k;
-            if (vec) {
-                const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 4);
-                k.w[0] = a.x, k.w[1] = a.y, k.w[2] = a.z, k.w[3] = a.w;
-                k.w[4] = b.x, k.w[5] = b.y, k.w[6] = b.z, k.w[7] = b.w;
-            } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) k.w[j] = __float_as_uint(p[j]);
-            }
-            return k;
-        } else {
-            Raw<T, 8> k;
-            if (vec) {
-                const uint4 a = *reinterpret_cast<const uint4*>(p);
-                k.w[0] = a.x, k.w[1] = a.y, k.w[2] = a.z, k.w[3] = a.w;
-            } else {
-                // whole words: five, shifted by a half, where p is odd (each holds a value of the eight)
-                const uintptr_t u = reinterpret_cast<uintptr_t>(p);
-                const uint32_t* q = reinterpret_cast<const uint32_t*>(u & ~uintptr_t(3));
-                const bool odd = (u & 2) != 0;
-                uint32_t w[5];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = q[j];
-                w[4] = odd ? q[4] : 0u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) k.w[j] = odd ? __byte_perm(w[j], w[j + 1], 0x5432) : w[j];
-            }
-            return k;
+        for (int j = 0; j < 2 * static_cast<int>(sizeof(T)); j += 4) {
+            const uint4 q = *(reinterpret_cast<const uint4*>(p) + j / 4);
+            w[j] = q.x, w[j + 1] = q.y, w[j + 2] = q.z, w[j + 3] = q.w;
         }
+        return;
     }
-    return gather_raw<T, 8>([&](int j) { return j < n ? p[j] : from_f32<T>(0.0f); });
+    const Raw<T, 8> k = gather_raw<T, 8>([&](int j) { return j < n ? p[j] : from_f32<T>(0.0f); });
+#pragma unroll
+    for (int j = 0; j < Raw<T, 8>::N; ++j) w[j] = k.w[j];
+}
+// Two values at p.
+template <class T>
+__device__ __forceinline__ void load2(const T* p, int n, bool pair, uint32_t* w) {
+    if (pair && n >= 2) {
+        if (sizeof(T) == 4) {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            w[0] = q.x, w[sizeof(T) == 4] = q.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+        return;
+    }
+    const uint32_t lo = n > 0 ? bits(p[0]) : 0u, hi = n > 1 ? bits(p[1]) : 0u;
+    if (sizeof(T) == 4) w[0] = lo, w[sizeof(T) == 4] = hi;
+    else w[0] = lo | hi << 16;
 }
 
 // Chunk c of row r of a plane: 128-byte rows, 16-byte chunks swizzled.  Tiles
@@ -105,51 +103,147 @@ __device__ __forceinline__ Raw<T, 8> load8(const T* p, int n, bool vec) {
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
     return static_cast<uint32_t>(c >> 3) * tc::kChunkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
-__device__ __forceinline__ void store_chunk(uint32_t addr, const uint32_t (&w)[4]) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                 : "memory");
+// (plain stores: the compiler may mix the conversions of many values, which
+// volatile ones would run one chain after the other)
+__device__ __forceinline__ void store_chunk(uint8_t* at, const uint32_t (&w)[4]) {
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// N fp32 values (as words) to three bf16 parts, packed by twos: parts[q][N / 2].
+template <int N>
+__device__ __forceinline__ void split3(const uint32_t* w, uint32_t (&parts)[3][N / 2]) {
+    float x[N];
+    Raw<__nv_bfloat16, N> h;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = __fsub_rn(__uint_as_float(w[j]), __uint_as_float(w[j] & 0xffff0000u));
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) parts[0][j] = __byte_perm(w[2 * j], w[2 * j + 1], 0x7632);
+    narrow(x, h);
+    float y[N];
+    widen(h, y);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) parts[1][j] = h.w[j];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = __fsub_rn(x[j], y[j]);
+    narrow(x, h);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) parts[2][j] = h.w[j];
 }
 // Eight values into one plane (16-bit types) or three (fp32), `plane` bytes apart.
 template <class T>
-__device__ __forceinline__ void put8(uint32_t addr, uint32_t plane, const Raw<T, 8>& k) {
+__device__ __forceinline__ void put8(uint8_t* at, uint32_t plane, const uint32_t* w) {
     if constexpr (sizeof(T) == 2) {
-        store_chunk(addr, k.w);
+        store_chunk(at, {w[0], w[1], w[2], w[3]});
     } else {
-        float x[8];
-        Raw<__nv_bfloat16, 8> h;
+        uint32_t k[3][4];
+        split3<8>(w, k);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __fsub_rn(__uint_as_float(k.w[j]), __uint_as_float(k.w[j] & 0xffff0000u));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h.w[j] = __byte_perm(k.w[2 * j], k.w[2 * j + 1], 0x7632);
-        store_chunk(addr, h.w);
-        narrow(x, h);
-        store_chunk(addr + plane, h.w);
-        float y[8];
-        widen(h, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __fsub_rn(x[j], y[j]);
-        narrow(x, h);
-        store_chunk(addr + 2 * plane, h.w);
+        for (int q = 0; q < 3; ++q) store_chunk(at + q * plane, k[q]);
     }
+}
+template <class T>
+__device__ __forceinline__ void put2(uint8_t* at, uint32_t plane, const uint32_t* w) {
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint32_t*>(at) = w[0];
+    } else {
+        uint32_t k[3][1];
+        split3<2>(w, k);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(at + q * plane) = k[q][0];
+    }
+}
+template <class T>
+__device__ __forceinline__ float value_of(const uint32_t* w, int j) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    T v[2];
+    *reinterpret_cast<uint32_t*>(v) = w[j / 2];
+    return to_f32(v[j % 2]);
 }
 
 // The part of a tile of ROWS memory rows x CHUNKS 8-value chunks that one of
-// THREADS loader threads moves: one chunk of every STEP-th row.
+// THREADS loader threads moves.  Rows 16-byte aligned: one chunk of every
+// STEP-th row.  Others: a warp takes 64 columns of a row at a time, two
+// neighbouring ones a lane, so that its loads cover whole lines whatever the
+// alignment (a lane that read its own eight values of 4 bytes would touch each
+// line eight times); halves of 128 columns belong to warps of one parity, so
+// a lane keeps its columns.
 template <int ROWS, int CHUNKS, int THREADS>
 struct Part {
     static constexpr int STEP = THREADS / CHUNKS, N = ROWS / STEP;
+    static constexpr int HALVES = CHUNKS / 8, WARPS = THREADS / 32, PAIRS = ROWS * HALVES / WARPS;
+    static constexpr int PAIR_STEP = WARPS / HALVES;
+    static_assert(PAIRS == 4 * N && 8 % PAIR_STEP == 0, "both forms hold as many values");
+    static __device__ __forceinline__ constexpr int rows() { return ROWS; }
+    static __device__ __forceinline__ constexpr int cols() { return CHUNKS * 8; }
     static __device__ __forceinline__ int chunk() { return threadIdx.x % CHUNKS; }
     static __device__ __forceinline__ int row(int i) { return threadIdx.x % THREADS / CHUNKS + i * STEP; }
+    static __device__ __forceinline__ int warp() { return threadIdx.x % THREADS / 32; }
+    static __device__ __forceinline__ int pair_col() { return warp() % HALVES * 64 + threadIdx.x % 32 * 2; }
+    static __device__ __forceinline__ int pair_row(int i) { return warp() / HALVES + i * PAIR_STEP; }
 };
+template <class P, class T>
+constexpr int words() { return P::N * 2 * static_cast<int>(sizeof(T)); }
 
 template <class P, class T>
-__device__ __forceinline__ void fetch_tile(const Source<T>& s, bool vec, Raw<T, 8> (&k)[P::N]) {
-    const T* p = s.p + P::row(0) * s.ld + P::chunk() * 8;
-    const int n = s.cols - P::chunk() * 8;
+__device__ __forceinline__ void fetch_tile(const Source<T>& s, int align, uint32_t (&w)[words<P, T>()]) {
+    const bool whole = s.rows >= P::rows() && s.cols >= P::cols();  // the same for all threads
+    if (align == kVector) {
+        const T* p = s.p + P::row(0) * s.ld + P::chunk() * 8;
+        const int64_t step = P::STEP * s.ld;
+        if (whole) {
 #pragma unroll
-    for (int i = 0; i < P::N; ++i) {
-        k[i] = load8(p, P::row(i) < s.rows ? n : 0, vec);
-        p += P::STEP * s.ld;
+            for (int i = 0; i < P::N; ++i, p += step) load8(p, 8, w + i * 2 * sizeof(T));
+        } else {
+            const int n = s.cols - P::chunk() * 8;
+#pragma unroll
+            for (int i = 0; i < P::N; ++i, p += step) load8(p, P::row(i) < s.rows ? n : 0, w + i * 2 * sizeof(T));
+        }
+    } else {
+        const T* p = s.p + P::pair_row(0) * s.ld + P::pair_col();
+        const int64_t step = P::PAIR_STEP * s.ld;
+        if (whole && align == kPair) {
+#pragma unroll
+            for (int i = 0; i < P::PAIRS; ++i, p += step) load2(p, 2, true, w + i * sizeof(T) / 2);
+        } else {
+            const int n = s.cols - P::pair_col();
+#pragma unroll
+            for (int i = 0; i < P::PAIRS; ++i, p += step)
+                load2(p, P::pair_row(i) < s.rows ? n : 0, align == kPair, w + i * sizeof(T) / 2);
+        }
+    }
+}
+// The fetched values into the planes at `tile`; add: their column sums on top
+// of `sum`.  A row's place in the swizzle repeats every 8 rows, so the
+// addresses are a few and constant steps from them.
+template <class P, class T>
+__device__ __forceinline__ void put_tile(uint8_t* tile, uint32_t plane, int align,
+                                         const uint32_t (&w)[words<P, T>()], bool add, float (&sum)[8]) {
+    if (align == kVector) {
+        static_assert(P::STEP % 8 == 0, "whole swizzle periods");
+        uint8_t* at = tile + chunk_at(P::row(0), P::chunk());
+#pragma unroll
+        for (int i = 0; i < P::N; ++i) put8<T>(at + i * P::STEP * 128, plane, w + i * 2 * sizeof(T));
+        if (add) {
+#pragma unroll
+            for (int i = 0; i < P::N; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += value_of<T>(w + i * 2 * sizeof(T), j);
+        }
+    } else {
+        constexpr int PERIOD = 8 / P::PAIR_STEP;
+        const int c = P::pair_col();
+        uint8_t* at[PERIOD];
+#pragma unroll
+        for (int i = 0; i < PERIOD; ++i) at[i] = tile + chunk_at(P::pair_row(i), c >> 3) + (c & 7) * 2;
+#pragma unroll
+        for (int i = 0; i < P::PAIRS; ++i)
+            put2<T>(at[i % PERIOD] + i / PERIOD * 1024, plane, w + i * sizeof(T) / 2);
+        if (add) {
+#pragma unroll
+            for (int i = 0; i < P::PAIRS; ++i) {
+                sum[0] += value_of<T>(w + i * sizeof(T) / 2, 0);
+                sum[1] += value_of<T>(w + i * sizeof(T) / 2, 1);
+            }
+        }
     }
 }
 template <class P>
@@ -176,25 +270,24 @@ struct Item {
 };
 
 template <class T, int OP>
-__device__ __forceinline__ Item item_at(const AnyArgs<T>& g, const int* prefix, int64_t it, int BN) {
+__device__ __forceinline__ Item item_at(const AnyArgs<T>& g, const Shared& s, int64_t it, int BN) {
     Item m;
-    const int per = OP == kGradWeight ? g.tiles_m * g.tiles_n : g.tiles_n;
-    m.p = static_cast<int>(it / per);
-    const int in = static_cast<int>(it - static_cast<int64_t>(m.p) * per);
-    m.t = find_type(prefix, g.types, m.p);
-    const int64_t b = clamp_row(g.offsets[m.t], g.M), e = clamp_row(g.offsets[m.t + 1], g.M);
-    const int64_t size = OP == kGradWeight ? g.piece : BM;
-    m.r0 = b + (m.p - prefix[m.t]) * size;
-    m.r1 = m.r0 + size < e ? m.r0 + size : e;
-    m.whole = prefix[m.t + 1] - prefix[m.t] == 1;
-    m.n0 = static_cast<int64_t>(in % g.tiles_n) * BN;
     if (OP == kGradWeight) {
-        m.m0 = static_cast<int64_t>(in / g.tiles_n) * BM;
+        const WeightItem w = weight_item(g.offsets, g.types, g.M, g.tiles_m * g.tiles_n, s.prefix, s.order, it);
+        m.t = w.t, m.p = w.p, m.r0 = w.r0, m.r1 = w.r1, m.whole = w.whole;
+        m.m0 = static_cast<int64_t>(w.in / g.tiles_n) * BM;
+        m.n0 = static_cast<int64_t>(w.in % g.tiles_n) * BN;
         m.steps = static_cast<int>((m.r1 - m.r0 + tc::kInner - 1) / tc::kInner);
-    } else {
-        m.m0 = m.r0;
-        m.steps = static_cast<int>((g.K + tc::kInner - 1) / tc::kInner);
+        return m;
     }
+    m.p = static_cast<int>(it / g.tiles_n);
+    m.t = find_type(s.prefix, g.types, m.p);
+    const int64_t b = clamp_row(g.offsets[m.t], g.M), e = clamp_row(g.offsets[m.t + 1], g.M);
+    m.m0 = m.r0 = b + static_cast<int64_t>(m.p - s.prefix[m.t]) * BM;
+    m.r1 = m.r0 + BM < e ? m.r0 + BM : e;
+    m.n0 = (it - static_cast<int64_t>(m.p) * g.tiles_n) * BN;
+    m.steps = static_cast<int>((g.K + tc::kInner - 1) / tc::kInner);
+    m.whole = true;
     return m;
 }
 
@@ -242,104 +335,120 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
     constexpr bool W = OP == kGradWeight, A_OUTER = W, B_OUTER = OP != kGradInput;
     static_assert(!TMA || (W && PB == 1), "TMA takes 16-bit dY");
     constexpr uint32_t ID = tc::idesc(is_bf16<H>(), A_OUTER, B_OUTER, BM, BN);
-    // 16-bit values: the loaders are two groups that take the stages in turn,
-    // so that one group's loads are in flight while the other's arrive (fp32
-    // values would need twice the registers, and take six times as long to
-    // multiply).
-    constexpr int GROUPS = sizeof(T) == 2 ? 2 : 1, THREADS = kLoaders / GROUPS;
+    // 16-bit values: the loaders are two groups that take the stages in turn
+    // (four for 8-bit copies and dY by TMA), so that one group's loads are in
+    // flight while the other's arrive (fp32 values would need twice the
+    // registers, and take six times as long to multiply).
+    constexpr int GROUPS = TMA ? 4 : (sizeof(T) == 2 ? 2 : 1), THREADS = kLoaders / GROUPS;
     using PartA = Part<A_OUTER ? 64 : BM, A_OUTER ? BM / 8 : 8, THREADS>;
-    using PartB = Part<B_OUTER ? 64 : BN, B_OUTER ? BN / 8 : 8, THREADS>;
+    using PartB = Part<B_OUTER ? 64 : BN, B_OUTER ? BN / 8 : 8, TMA ? kLoaders : THREADS>;
 
     extern __shared__ uint8_t raw[];
     __shared__ Shared s;
     __shared__ float stage_out[4][(stage_bytes<float>() + 3) / 4];
     __shared__ float db_rows[W && !TMA ? kLoaders * 8 : 1];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, W ? g.piece : BM,
-                                             8 / GROUPS + (TMA ? 1 : 0));
+    uint8_t* const ring_p = raw + (ring - mb::smem_u32(raw));
+    const uint32_t tmem = set_up<STAGES, BN>(s, 8 / GROUPS + (TMA ? 1 : 0), [&] {
+        if (W) plan_pieces(g.offsets, g.types, g.M, g.tiles_m * g.tiles_n, g.slots, s.prefix, s.order);
+        else scan_types(g.offsets, g.types, g.M, BM, s.prefix);
+    });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t items = static_cast<int64_t>(s.prefix[g.types]) * (W ? g.tiles_m * g.tiles_n : g.tiles_n);
 
+    // Round r's item of this CTA (rows products: equal items, in order).
+    const auto item_of = [&](int64_t r) {
+        return W ? dealt(r, blockIdx.x, gridDim.x) : blockIdx.x + r * gridDim.x;
+    };
+
     if (warp < 8) {
         // ── loaders ──
-        int64_t i = 0, it = blockIdx.x;
+        int64_t i = 0, round = 0, it = item_of(0);
         bool ok = true;
-        Raw<T, 8> ka[SAVED ? 1 : PartA::N], kb[TMA ? 1 : PartB::N];
+        uint32_t ka[words<PartA, T>()], kb[words<PartB, T>()];
         Raw<int8_t, 8> k8[SAVED ? PartA::N : 1];
         int e8[SAVED ? PartA::N : 1];
-        const auto fetch = [&](const Item& m, int step) {
+        const auto fetch_a = [&](const Item& m, int step) {
             if constexpr (SAVED) {
                 const int64_t k = static_cast<int64_t>(step) * tc::kInner;
                 fetch_tile8<PartA>(g.a8, m.r0 + k, m.m0, clip(m.r1 - m.r0 - k, tc::kInner), clip(g.K - m.m0, BM), k8,
                                    e8);
             } else {
-                fetch_tile<PartA>(source_a<T, OP>(g, m, step, BN), g.a_vec, ka);
+                fetch_tile<PartA, T>(source_a<T, OP>(g, m, step, BN), g.a_align, ka);
             }
-            if constexpr (!TMA) fetch_tile<PartB>(source_b<T, OP>(g, m, step, BN), g.b_vec, kb);
+        };
+        const auto fetch_b = [&](const Item& m, int step) {
+            if constexpr (!TMA) fetch_tile<PartB, T>(source_b<T, OP>(g, m, step, BN), g.b_align, kb);
         };
         const int group = threadIdx.x / THREADS;
         // This group's first step of an item whose first stage is number i0.
-        const auto first = [&](int64_t i0) { return GROUPS == 1 ? 0 : static_cast<int>((group + i0) & 1); };
-        Item m{};
-        bool fetched = false;  // the registers hold the next step's values
-        if (it < items) m = item_at<T, OP>(g, s.prefix, it, BN);
+        const auto first = [&](int64_t i0) { return GROUPS == 1 ? 0 : static_cast<int>((group + GROUPS - i0 % GROUPS) % GROUPS); };
+        Item m{}, next{};
+        if (it < items) m = item_at<T, OP>(g, s, it, BN);
         float sum[8];
+        bool fetched = false;  // the registers hold the next step's values
         while (it < items && ok) {
             const bool sums = W && !TMA && g.db != nullptr && m.m0 == 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
-            const bool more = it + gridDim.x < items;
-            Item next = m;
-            if (more) next = item_at<T, OP>(g, s.prefix, it + gridDim.x, BN);
+            it = item_of(++round);
+            const bool more = it < items;
+            if (more) next = item_at<T, OP>(g, s, it, BN);
             for (int step = first(i); step < m.steps; step += GROUPS) {
-                if (!fetched) fetch(m, step);
+                if (!fetched) {
+                    fetch_a(m, step);
+                    fetch_b(m, step);
+                }
                 const int64_t n = i + step;
                 const int st = static_cast<int>(n % STAGES);
                 if (n >= STAGES) ok = mb::wait(&s.empty[st], (n / STAGES - 1) & 1, &g_error, 41);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                const uint32_t a = ring + st * S::kStage, b = a + PA * S::kA;
+                // The next step's values are asked for as soon as this step's
+                // have left their registers: A's are on their way while B is
+                // converted, B's while this thread waits for the next stage
+                // and converts A.
+                const bool here = step + GROUPS < m.steps;
+                const int after = here ? step + GROUPS : first(i + m.steps);
+                const Item then = here ? m : next;
+                fetched = here || (more && after < next.steps);
+                uint8_t* const a = ring_p + st * S::kStage;
+                if constexpr (SAVED) {
 #pragma unroll
-                for (int u = 0; u < PartA::N; ++u) {
-                    const uint32_t at = a + chunk_at(PartA::row(u), PartA::chunk());
-                    if constexpr (SAVED) {
+                    for (int u = 0; u < PartA::N; ++u) {
                         float x[8];
                         values4(k8[u].w[0], e8[u], x);
                         values4(k8[u].w[1], e8[u], x + 4);
                         Raw<H, 8> h;
                         narrow(x, h);
-                        store_chunk(at, h.w);
-                    } else {
-                        put8<T>(at, S::kA, ka[u]);
+                        store_chunk(a + chunk_at(PartA::row(u), PartA::chunk()), h.w);
                     }
+                } else {
+                    put_tile<PartA, T>(a, S::kA, g.a_align, ka, false, sum);
                 }
+                if (fetched) fetch_a(then, after);
                 if constexpr (!TMA) {
-#pragma unroll
-                    for (int u = 0; u < PartB::N; ++u) {
-                        put8<T>(b + chunk_at(PartB::row(u), PartB::chunk()), S::kB, kb[u]);
-                        if (sums) {
-                            float x[8];
-                            widen(kb[u], x);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) sum[j] += x[j];
-                        }
-                    }
+                    put_tile<PartB, T>(a + PA * S::kA, S::kB, g.b_align, kb, sums, sum);
+                    if (fetched) fetch_b(then, after);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                // (the MMA's thread passes the writes on to the tensor cores: a
+                // proxy fence here would wait for the loads just issued)
                 __syncwarp();
                 if (lane == 0) mb::arrive(&s.full[st]);
-                // the next step's values, on their way while stages are
-                // multiplied (after the fence, which waits for loads too)
-                fetched = true;
-                if (step + GROUPS < m.steps) fetch(m, step + GROUPS);
-                else if (more && first(i + m.steps) < next.steps) fetch(next, first(i + m.steps));
-                else fetched = false;
             }
             i += m.steps;
             if constexpr (W && !TMA) {
                 if (sums) {  // the same for every loader thread
-                    constexpr int G = kLoaders / (BN / 8);  // threads that share a column
+                    // threads that share a column, as rows of db_rows
+                    const bool vec = g.b_align == kVector;
+                    const int G = vec ? kLoaders / (BN / 8) : 8 / PartB::HALVES;
+                    if (vec) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) db_rows[threadIdx.x / (BN / 8) * BN + PartB::chunk() * 8 + j] = sum[j];
+                        for (int j = 0; j < 8; ++j) db_rows[threadIdx.x / (BN / 8) * BN + PartB::chunk() * 8 + j] = sum[j];
+                    } else {
+                        float* r = db_rows + threadIdx.x / 32 / PartB::HALVES * BN + PartB::pair_col();
+                        r[0] = sum[0];
+                        r[1] = sum[1];
+                    }
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                     if (ok && threadIdx.x < BN && m.n0 + threadIdx.x < g.N) {
                         float all = 0.0f;
@@ -350,7 +459,6 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                     asm volatile("bar.sync 1, 256;" ::: "memory");
                 }
             }
-            it += gridDim.x;
             m = next;
         }
     } else if (warp == 8) {
@@ -358,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
         int64_t i = 0;
         int local = 0;
         bool ok = true;
-        for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x, ++local) {
-            const Item m = item_at<T, OP>(g, s.prefix, it, BN);
+        for (int64_t it; (it = item_of(local)) < items && ok; ++local) {
+            const Item m = item_at<T, OP>(g, s, it, BN);
             const int acc = local & 1;
             if (local >= 2) ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 42);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -376,6 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                     if (valid < tc::kInner) zero_rows(ring + st * S::kStage + PA * S::kA, S::kB, static_cast<int>(valid));
                 }
                 if (lane == 0) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the loaders' writes -> MMA reads
                     stage_mmas<PA, PB, BN, A_OUTER, B_OUTER>(ring + st * S::kStage, tmem + acc * BN, ID, k == 0);
                     tc::commit(&s.empty[st]);
                 }
@@ -388,8 +497,8 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
         if (TMA && lane == 0) {
             int64_t i = 0;
             bool ok = true;
-            for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
-                const Item m = item_at<T, OP>(g, s.prefix, it, BN);
+            for (int64_t round = 0, it; (it = item_of(round)) < items && ok; ++round) {
+                const Item m = item_at<T, OP>(g, s, it, BN);
                 for (int k = 0; k < m.steps; ++k, ++i) {
                     const int st = static_cast<int>(i % STAGES);
                     if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_error, 44))) break;
@@ -411,8 +520,8 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
         T* buf = reinterpret_cast<T*>(stage_out[q]);
         float* buf32 = stage_out[q];
         int local = 0;
-        for (int64_t it = blockIdx.x; it < items; it += gridDim.x, ++local) {
-            const Item m = item_at<T, OP>(g, s.prefix, it, BN);
+        for (int64_t it; (it = item_of(local)) < items; ++local) {
+            const Item m = item_at<T, OP>(g, s, it, BN);
             const int acc = local & 1;
             bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 46);
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -445,12 +554,18 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
             // types without rows: zero
             const int e = threadIdx.x - 384;
             for (int t = blockIdx.x; t < g.types; t += gridDim.x) {
-                if (s.prefix[t + 1] != s.prefix[t]) continue;
+                if (rows_of(g.offsets, t, g.M) > 0) continue;
                 zero_type(g, out, t, e, 128);
             }
         }
     }
     tear_down<BN>(s, tmem, 8);
+}
+
+template <class T>
+int alignment(const T* p, int64_t ld) {
+    const uint64_t b = reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(ld * sizeof(T));
+    return b % 16 == 0 ? kVector : (b % (2 * sizeof(T)) == 0 ? kPair : kElement);
 }
 
 template <class T, int OP, int BN, bool SAVED, bool TMA>
@@ -468,8 +583,8 @@ void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s) {
     AnyArgs<T> g{};
     g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
     g.A = a.A, g.lda = a.lda, g.B = a.W, g.ldb = a.ldw, g.stride_b = a.stride_w;
-    g.a_vec = rows_aligned16(a.A, a.lda, sizeof(T));
-    g.b_vec = rows_aligned16(a.W, a.ldw, sizeof(T)) && a.stride_w * sizeof(T) % 16 == 0;
+    g.a_align = alignment(a.A, a.lda);
+    g.b_align = std::min(alignment(a.W, a.ldw), alignment(a.W, a.stride_w));
     const RowsOut<T> out{a.N, a.bias, a.act, a.alpha, a.C, a.ldc, store_mode(a.C, a.ldc * sizeof(T)), a.saved, a.r8};
     const int64_t pieces = a.M / BM + std::min<int64_t>(a.types, a.M);
     const int BN = tile_width(pieces, a.N, 128, a.saved.codes != nullptr);
@@ -487,9 +602,9 @@ void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream
     g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
     g.tiles_m = w.tiles_k, g.tiles_n = w.tiles_n;
     g.A = a.X, g.lda = a.ldx, g.a8 = a.saved, g.B = a.dY, g.ldb = a.lddy;
-    g.a_vec = rows_aligned16(a.X, a.ldx, sizeof(T));
-    g.b_vec = rows_aligned16(a.dY, a.lddy, sizeof(T));
-    g.piece = w.piece, g.part = w.part, g.ldp = w.ldp, g.stride_c = a.stride_dw;
+    g.a_align = alignment(a.X, a.ldx);
+    g.b_align = alignment(a.dY, a.lddy);
+    g.slots = w.slots, g.part = w.part, g.ldp = w.ldp, g.stride_c = a.stride_dw;
     g.out_f32 = sizeof(O) == 4;
     RowsOut<T> out{};
     out.N = a.N;

@@ -35,16 +35,16 @@ struct Shared {
     uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drain;
     uint32_t tmem;
     int prefix[kMaxTypes + 1];
+    uint16_t order[kMaxTypes];  // weight gradients only
 };
 
 template <int BN>
 constexpr uint32_t tmem_cols() { return 2 * BN < 64 ? 64 : 2 * BN; }
 
-// Barriers, TMEM (warp 2) and the scan of the types (warp 3); every thread
-// returns with them in place.
-template <int STAGES, int BN>
-__device__ __forceinline__ uint32_t set_up(Shared& s, const int32_t* offsets, int types, int64_t M, int64_t per,
-                                           int full_arrivals) {
+// Barriers, TMEM (warp 2) and the plan of the work (warp 3: plan(), over the
+// types' offsets); every thread returns with them in place.
+template <int STAGES, int BN, class F>
+__device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, F&& plan) {
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -59,7 +59,7 @@ __device__ __forceinline__ uint32_t set_up(Shared& s, const int32_t* offsets, in
         mb::fence_init();
     }
     if (warp == 2) tc::alloc(&s.tmem, tmem_cols<BN>());
-    if (warp == 3) scan_types(offsets, types, M, per, s.prefix);
+    if (warp == 3) plan();
     tc::fence_before();
     __syncthreads();
     tc::fence_after();

@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
     __shared__ Shared s;
     __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, BM, 1);
+    const uint32_t tmem = set_up<STAGES, BN>(s, 1, [&] { scan_types(g.offsets, g.types, g.M, BM, s.prefix); });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tiles = static_cast<int64_t>(s.prefix[g.types]) * g.tiles_n;
     const int KB = static_cast<int>((g.K + tc::kInner - 1) / tc::kInner);
@@ -129,9 +129,8 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
 template <class O>
 struct WeightTc {
     int64_t M, K, N;
-    int types, tiles_k, tiles_n;
+    int types, tiles_k, tiles_n, slots;
     const int32_t* offsets;
-    int64_t piece;
     O* dW;
     int64_t lddw, stride_dw;
     int mode;
@@ -150,35 +149,30 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
     __shared__ Shared s;
     __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t tmem = set_up<STAGES, BN>(s, g.offsets, g.types, g.M, g.piece, 1);
+    const uint32_t tmem = set_up<STAGES, BN>(s, 1, [&] {
+        plan_pieces(g.offsets, g.types, g.M, g.tiles_k * g.tiles_n, g.slots, s.prefix, s.order);
+    });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = g.tiles_k * g.tiles_n;
     const int64_t items = static_cast<int64_t>(s.prefix[g.types]) * per;
 
-    // Item -> type, piece, tile, rows.
     struct Item {
         int t, p, k0, n0, row0, row1;
         bool whole;
     };
     const auto item_at = [&](int64_t it) {
-        Item r;
-        r.p = static_cast<int>(it / per);
-        const int in = static_cast<int>(it % per);
-        r.k0 = in / g.tiles_n * BM;
-        r.n0 = in % g.tiles_n * BN;
-        r.t = find_type(s.prefix, g.types, r.p);
-        const int b = clamp_row(g.offsets[r.t], g.M), e = clamp_row(g.offsets[r.t + 1], g.M);
-        r.row0 = b + static_cast<int>((r.p - s.prefix[r.t]) * g.piece);
-        r.row1 = static_cast<int>(r.row0 + g.piece < e ? r.row0 + g.piece : e);
-        r.whole = s.prefix[r.t + 1] - s.prefix[r.t] == 1;
-        return r;
+        const WeightItem w = weight_item(g.offsets, g.types, g.M, per, s.prefix, s.order, it);
+        return Item{w.t, w.p, w.in / g.tiles_n * BM, w.in % g.tiles_n * BN, static_cast<int>(w.r0),
+                    static_cast<int>(w.r1), w.whole};
     };
+    // Round r's item of this CTA.
+    const auto dealt_item = [&](int64_t r) { return dealt(r, blockIdx.x, gridDim.x); };
 
     if (warp == 0) {
         if (lane == 0) {
             int64_t i = 0;
             bool ok = true;
-            for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
+            for (int64_t round = 0, it; (it = dealt_item(round)) < items && ok; ++round) {
                 const Item m = item_at(it);
                 for (int r = m.row0; r < m.row1; r += tc::kInner, ++i) {
                     const int st = static_cast<int>(i % STAGES);
@@ -200,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
         int64_t i = 0;
         int local = 0;
         bool ok = true;
-        for (int64_t it = blockIdx.x; it < items && ok; it += gridDim.x, ++local) {
+        for (int64_t it; (it = dealt_item(local)) < items && ok; ++local) {
             const Item m = item_at(it);
             const int acc = local & 1;
             if (local >= 2) ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 33);
@@ -224,8 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
     } else if (warp >= 4) {
         const int acc = (warp - 4) >> 2, q = warp & 3;
         int local = acc;
-        for (int64_t it = blockIdx.x + acc * static_cast<int64_t>(gridDim.x); it < items;
-             it += 2 * static_cast<int64_t>(gridDim.x), local += 2) {
+        for (int64_t it; (it = dealt_item(local)) < items; local += 2) {
             const Item m = item_at(it);
             const bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 35);
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -253,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
         }
         // types without rows: zero
         for (int t = blockIdx.x; t < g.types; t += gridDim.x) {
-            if (s.prefix[t + 1] != s.prefix[t]) continue;
+            if (rows_of(g.offsets, t, g.M) > 0) continue;
             for (int64_t k = 0; k < g.K; ++k)
                 for (int64_t n = threadIdx.x - 128; n < g.N; n += 256)
                     g.dW[t * g.stride_dw + k * g.lddw + n] = from_f32<O>(0.0f);
@@ -265,7 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
 // dW and db of the types with several pieces: the sum of the pieces in their order.
 template <class O>
 struct JoinArgs {
-    int64_t M, K, N, piece, ldp;
+    int64_t M, K, N, ldp;
+    int types, per, slots;
     const int32_t* offsets;
     const float *part, *db_part;
     O* dW;
@@ -275,14 +269,31 @@ struct JoinArgs {
 
 template <class O>
 __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O> g) {
-    __shared__ int prefix[kMaxTypes + 1];
-    const int t = blockIdx.y;
-    const int b = clamp_row(g.offsets[t], g.M), e = clamp_row(g.offsets[t + 1], g.M);
-    if (e - b <= g.piece) return;  // one piece: the weight kernel wrote it
-    const int n = static_cast<int>((e - b + g.piece - 1) / g.piece);
-    if (threadIdx.x < 32) scan_types(g.offsets, t, g.M, g.piece, prefix);
-    __syncthreads();
-    const int64_t p = prefix[t];
+    __shared__ int64_t sums[8];
+    __shared__ int first[8];
+    const int t = blockIdx.y, rows = rows_of(g.offsets, t, g.M);
+    const auto block_sum = [&](auto x, auto* sh) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = x;
+        __syncthreads();
+        x = 0;
+        for (int w = 0; w < 8; ++w) x += sh[w];
+        return x;
+    };
+    int64_t steps = 0;
+    for (int u = threadIdx.x; u < g.types; u += 256) steps += (rows_of(g.offsets, u, g.M) + kStep - 1) / kStep;
+    const int64_t limit = piece_limit(block_sum(steps, sums), g.per, g.slots);
+    const int n = piece_count(rows, limit);
+    if (n <= 1) return;  // the weight kernel wrote it
+    // this type's first piece
+    const int len = piece_rows(rows, n);
+    int before = 0;
+    for (int u = threadIdx.x; u < g.types; u += 256) {
+        const int ru = rows_of(g.offsets, u, g.M), nu = piece_count(ru, limit);
+        if (piece_before(g.types, piece_rows(ru, nu), u, len, t)) before += nu;
+    }
+    const int64_t p = block_sum(before, first);
     const float* part = g.part + p * g.K * g.ldp;
     const int64_t vecs = g.ldp / 4, total = g.K * vecs, next = g.K * g.ldp;
     for (int64_t v = blockIdx.x * 256 + threadIdx.x; v < total; v += static_cast<int64_t>(gridDim.x) * 256) {
@@ -398,7 +409,7 @@ template <class T, class O>
 void typed_weight_tma(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s) {
     const Operand<T> X(1, a.M, a.K, a.X, a.ldx, 0, s), Y(1, a.M, a.N, a.dY, a.lddy, 0, s);
     const CUtensorMap mx = X.map(1, a.M, a.K, 64), my = Y.map(1, a.M, a.N, 64);
-    const WeightTc<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, a.offsets, w.piece, a.dW, a.lddw, a.stride_dw,
+    const WeightTc<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, a.offsets, a.dW, a.lddw, a.stride_dw,
                         store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O)), w.part, w.ldp};
     const auto go = [&](auto bn) {
         constexpr int BN = decltype(bn)::value;
@@ -448,13 +459,14 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     w.tiles_k = static_cast<int>(ceil_div(a.K, BM));
     w.tiles_n = static_cast<int>(ceil_div(a.N, w.BN));
     const int64_t per = int64_t(w.tiles_k) * w.tiles_n;
-    // About 2.5 sums per SM: enough to even out types of unequal sizes, few
-    // enough that the partial sums' traffic stays small.
-    w.piece = std::max<int64_t>(128, ceil_div(a.M * per * 2, int64_t(num_sms()) * 5 * 64) * 64);
-    const int64_t pieces = a.M / w.piece + std::min<int64_t>(a.types, a.M);
+    w.slots = num_sms();
+    // A type is cut where it has more than an SM's share: at most slots / per
+    // pieces and one a type.
+    const int64_t used = std::min<int64_t>(a.types, a.M), pieces = w.slots / per + used;
     w.items = std::max<int64_t>(pieces * per, std::min(a.types, num_sms()));
     w.ldp = (a.N + 7) / 8 * 8;
-    const bool joined = a.M > w.piece;
+    // None is, if even all the rows in one type are an SM's share or two steps.
+    const bool joined = a.M > 2 * kStep && per < w.slots;
     Scratch<float> part(joined ? static_cast<size_t>(pieces * (a.K * w.ldp + a.N)) : 1, s);
     w.part = part.p;
     w.db_part = part.p + (joined ? pieces * a.K * w.ldp : 0);
@@ -472,11 +484,11 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
         typed_weight_any<T, O>(a, w, s);
     }
     if (joined) {
-        const JoinArgs<O> j{a.M, a.K, a.N, w.piece, w.ldp, a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
+        const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots, a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
                             db_joined ? a.db : nullptr};
         const int64_t want = ceil_div(a.K * w.ldp / 4, 256);
         launch("typed_weight_join", typed_weight_join_kernel<O>,
-               dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(8, 16384 / a.types))),
+               dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(1, 8 * num_sms() / a.types))),
                     static_cast<unsigned>(a.types)),
                dim3(256), 0, s, j);
     }
