@@ -479,6 +479,46 @@ def test_typed_more_rows_than_a_wave(tg):
             assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K,N", [(264, 328), (263, 329), (520, 160), (136, 640)])
+def test_typed_large_products(tg, dtype, K, N):
+    """Sizes that run on pairs of CTAs (aligned copies first where rows are not aligned): uneven types, one of a row,
+    one empty, one whose NaN and infinity must stay its own."""
+    sizes = [30001, 0, 1, 25000, 300, 14755, 130]
+    x, dy, w, bias, off = typed_inputs(sizes, K, N, dtype)
+    bad = sum(sizes[:4])
+    x[bad:bad + 300], dy[bad:bad + 300] = float("nan"), float("inf")
+    y, z8 = tg.typed_linear(x, w, off, bias, "relu", save8=True)
+    dx, dw, db = tg.typed_linear_backward(dy, x, w, off)
+    dw32, _ = tg.typed_linear_grad_weight(x, dy, off, dtype=torch.float32, bias=False)
+    s = tg.save8(x)
+    dws, dbs = tg.typed_linear_grad_weight(s, dy, off)
+    held = s.restore(torch.float32)
+    for t, a, b in spans(sizes):
+        if t == 4:
+            assert y[a:b].isnan().all() and dx[a:b].isnan().all()
+            continue
+        xd, dyd, wd = x[a:b].double(), dy[a:b].double(), w[t].double()
+        pre, mag = xd @ wd + bias[t].double(), xd.abs() @ wd.abs() + bias[t].double().abs()
+        ref = torch.clamp(pre, min=0)
+        err = (K + 16) * 2.0 ** -23 * mag
+        assert_within(y[a:b], ref, U[dtype] * ref.abs() + err + TINY[dtype], f"y[{t}]")
+        part = tg.Saved8(z8.codes[a:b], z8.exponents[a:b], dtype)
+        step = torch.exp2(spread(part.exponents.double() - 127, N))
+        assert_within(part.restore(torch.float32), pre, 0.5 * step + err, f"saved[{t}]")
+        assert_product(dx[a:b], dyd @ wd.T, dyd.abs() @ wd.abs().T, N, dtype, f"dx[{t}]")
+        want, mag = xd.T @ dyd, xd.abs().T @ dyd.abs()
+        assert_product(dw[t], want, mag, b - a, dtype, f"dw[{t}]")
+        assert_product(dw32[t], want, mag, b - a, torch.float32, f"fp32 dw[{t}]")
+        hd = held[a:b].double()
+        assert_product(dws[t], hd.T @ dyd, hd.abs().T @ dyd.abs(), b - a, dtype, f"dw[{t}] from 8 bits")
+        assert_within(db[t], dyd.sum(0), 1024 * 2.0 ** -24 * dyd.abs().sum(0), f"db[{t}]")
+        assert_within(dbs[t], dyd.sum(0), 1024 * 2.0 ** -24 * dyd.abs().sum(0), f"db[{t}] from 8 bits")
+    again = tg.typed_linear(x, w, off, bias, "relu"), *tg.typed_linear_backward(dy, x, w, off)
+    for p, q in zip((y, dx, dw, db), again):
+        assert torch.equal(p.nan_to_num(7.0), q.nan_to_num(7.0))
+
+
 def test_typed_offsets_out_of_range_stay_inside(tg):
     """Offsets are clamped: nothing outside the outputs is touched and no address past the inputs is read."""
     x, dy, w, bias, _ = typed_inputs([40, 50], 32, 24, torch.float32)

@@ -196,6 +196,7 @@ int gather_take_error(cudaStream_t s);
 int peer_take_error(cudaStream_t s);
 int typed_tc_take_error();
 int typed_any_take_error();
+int typed_pair_take_error();
 void gemm_tc(int64_t M, int64_t N, int64_t K, const float* A, int64_t lda, const float* B, int64_t ldb, float* C,
              int64_t ldc, const float* bias, int act, float alpha, cudaStream_t s, const PeerOut& peers = PeerOut{},
              bool c_cols_padded = false, const float* row_scale = nullptr);
@@ -385,8 +386,9 @@ TG_API tg_status tg_take_device_error(void* stream) {
         const int code = gemm_tc_take_error(as_stream(stream));
         const int gcode = gather_take_error(as_stream(stream));
         const int pcode = peer_take_error(as_stream(stream));
-        const int tcode1 = typed_tc_take_error(), tcode2 = typed_any_take_error();
-        if (const int tcode = tcode1 ? tcode1 : tcode2)
+        const int tcode1 = typed_tc_take_error(), tcode2 = typed_any_take_error(),
+                  tcode3 = typed_pair_take_error();
+        if (const int tcode = tcode1 ? tcode1 : (tcode2 ? tcode2 : tcode3))
             fail(TG_ERR_TIMEOUT, "a typed product's pipeline wait ran out (code " + std::to_string(tcode) +
                                      "); its output is invalid");
         if (code)

@@ -99,6 +99,83 @@ __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* m, int x, 
         : "memory");
 }
 
+// ── CTA pairs ────────────────────────────────────────────────────────────
+// Two CTAs of a cluster multiply one tile of 256 rows (cta_group::2): each
+// holds its 128 rows of A and half of B's columns in its own shared memory
+// and its 128 rows of the accumulator in its own TMEM.  The CTA of rank 0
+// issues the MMAs; its full barriers count both CTAs' copies.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of `bar` in the CTA of rank `rank`.
+__device__ __forceinline__ uint32_t in_rank(const void* bar, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(mb::smem_u32(bar)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void arrive_expect_tx_at(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Bounded wait (as mb::wait) that sees what the other CTA did before it arrived.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err, int code) {
+    const uint32_t a = mb::smem_u32(bar);
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (i == 0) t0 = mb::global_ns();
+        if ((i & 15) == 15 && mb::global_ns() - t0 > mb::kWaitNs) break;
+        if (i > 32) __nanosleep(64);
+    }
+    atomicCAS(err, 0, code);
+    return false;
+}
+// A copy into this CTA's shared memory that completes on a barrier of either CTA.
+__device__ __forceinline__ void tma3_pair(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4}], [%5];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(acc)));
+}
+// Arrives on `bar` (the same offset) of both CTAs once the MMAs so far have retired.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(mb::smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+__device__ __forceinline__ void alloc_pair(uint32_t* out, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(mb::smem_u32(out)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void dealloc_pair(uint32_t tmem, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+}
+
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;

@@ -187,6 +187,7 @@ struct WeightPlan {
     int tiles_k, tiles_n, slots;
     int64_t ldp, items;
     float *part, *db_part;
+    bool pairs;      // on CTA pairs (tiles of 256 x 256)
     bool dy_by_tma;  // typed_weight_any: dY by TMA, db not summed on the way
 };
 
@@ -196,6 +197,21 @@ void typed_rows(const RowsArgs<T>& a, cudaStream_t s);
 template <class T, class O>
 void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s);
 int typed_tc_take_error();
+
+// A batch of 16-bit matrices that TMA can read (rows and matrices 16-byte aligned).
+template <class T>
+struct TmaMatrix {
+    const T* p;
+    int64_t ld, stride;
+};
+
+// TMA-fed kernels on CTA pairs (typed_pair.cu).
+template <class T, bool TRANS>
+void typed_rows_pair(const RowsArgs<T>& a, const TmaMatrix<T>& A, const TmaMatrix<T>& W, cudaStream_t s);
+template <class T, class O>
+void typed_weight_pair(const WeightArgs<T, O>& a, const WeightPlan& w, const TmaMatrix<T>& X, const TmaMatrix<T>& Y,
+                       cudaStream_t s);
+int typed_pair_take_error();
 
 // Loader-fed kernels (typed_any.cu).
 template <class T, bool TRANS>

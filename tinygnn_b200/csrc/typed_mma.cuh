@@ -270,6 +270,14 @@ template <> struct Half<float> { using type = __nv_bfloat16; static constexpr in
 template <class H>
 constexpr bool is_bf16() { return std::is_same<H, __nv_bfloat16>::value; }
 
+// Boxes of 64 columns x box_rows rows of a batch of matrices.
+template <class T>
+CUtensorMap tma_map(const TmaMatrix<T>& m, int64_t batch, int64_t rows, int64_t cols, int box_rows) {
+    const int64_t dims[3] = {cols, rows, batch}, strides[2] = {m.ld, m.stride};
+    const int box[3] = {64, box_rows, 1};
+    return tc::map16<3>(m.p, is_bf16<T>(), dims, strides, box);
+}
+
 // Reads and clears the error word (the stream is idle).
 static int take_error() {
     int h = 0;

@@ -375,11 +375,7 @@ struct Operand {
     static bool readable(int64_t batch, const T* src, int64_t lds, int64_t stride) {
         return rows_aligned16(src, lds, 2) && (batch == 1 || stride % 8 == 0);
     }
-    CUtensorMap map(int64_t batch, int64_t rows, int64_t cols, int box_rows) const {
-        const int64_t dims[3] = {cols, rows, batch}, strides[2] = {ld, stride};
-        const int box[3] = {64, box_rows, 1};
-        return tc::map16<3>(p, is_bf16<T>(), dims, strides, box);
-    }
+    TmaMatrix<T> matrix() const { return {p, ld, stride}; }
 };
 
 template <class T, bool TRANS>
@@ -388,12 +384,18 @@ void typed_rows_tma(const RowsArgs<T>& a, cudaStream_t s) {
     // W[t] is K x N in the forward pass, N x K in the input gradient.
     const int64_t wr = TRANS ? a.N : a.K, wc = TRANS ? a.K : a.N;
     const Operand<T> W(a.types, wr, wc, a.W, a.ldw, a.stride_w, s);
-    const CUtensorMap ma = A.map(1, a.M, a.K, BM);
+    // Pairs of CTAs, where 256-row tiles of 256 columns are enough for all of
+    // them and the types long enough not to leave much of a tile empty.
+    if (a.N > 128 && a.M / 512 >= a.types && (a.M / 256) * ceil_div(a.N, 256) >= num_sms()) {
+        typed_rows_pair<T, TRANS>(a, A.matrix(), W.matrix(), s);
+        return;
+    }
+    const CUtensorMap ma = tma_map(A.matrix(), 1, a.M, a.K, BM);
     const int64_t pieces = a.M / BM + std::min<int64_t>(a.types, a.M);
     const RowsOut<T> out{a.N, a.bias, a.act, a.alpha, a.C, a.ldc, store_mode(a.C, a.ldc * 2), a.saved, a.r8};
     const auto go = [&](auto bn) {
         constexpr int BN = decltype(bn)::value;
-        const CUtensorMap mw = W.map(a.types, wr, wc, TRANS ? BN : 64);
+        const CUtensorMap mw = tma_map(W.matrix(), a.types, wr, wc, TRANS ? BN : 64);
         const RowsTc g{a.M, a.K, a.types, static_cast<int>(ceil_div(a.N, BN)), a.offsets};
         run("typed_rows", typed_rows_tc_kernel<T, BN, TRANS>, kThreads, Plan<1, 1, BN>::kBytes, pieces * g.tiles_n, s,
             ma, mw, g, out);
@@ -408,7 +410,11 @@ void typed_rows_tma(const RowsArgs<T>& a, cudaStream_t s) {
 template <class T, class O>
 void typed_weight_tma(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s) {
     const Operand<T> X(1, a.M, a.K, a.X, a.ldx, 0, s), Y(1, a.M, a.N, a.dY, a.lddy, 0, s);
-    const CUtensorMap mx = X.map(1, a.M, a.K, 64), my = Y.map(1, a.M, a.N, 64);
+    if (w.pairs) {
+        typed_weight_pair<T, O>(a, w, X.matrix(), Y.matrix(), s);
+        return;
+    }
+    const CUtensorMap mx = tma_map(X.matrix(), 1, a.M, a.K, 64), my = tma_map(Y.matrix(), 1, a.M, a.N, 64);
     const WeightTc<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, a.offsets, a.dW, a.lddw, a.stride_dw,
                         store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O)), w.part, w.ldp};
     const auto go = [&](auto bn) {
@@ -456,10 +462,11 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     w.BN = a.N <= 64 ? 64 : (a.N <= 128 || widest == 128 ? 128 : 256);
     w.dy_by_tma = saved && large && rows_aligned16(a.dY, a.lddy, sizeof(T));
     if (saved && !w.dy_by_tma) w.BN = std::min(w.BN, 128);
-    w.tiles_k = static_cast<int>(ceil_div(a.K, BM));
+    w.pairs = large && !saved && a.K > 128 && a.N > 128;
+    w.tiles_k = static_cast<int>(ceil_div(a.K, w.pairs ? 2 * BM : BM));
     w.tiles_n = static_cast<int>(ceil_div(a.N, w.BN));
     const int64_t per = int64_t(w.tiles_k) * w.tiles_n;
-    w.slots = num_sms();
+    w.slots = w.pairs ? num_sms() / 2 : num_sms();
     // A type is cut where it has more than an SM's share: at most slots / per
     // pieces and one a type.
     const int64_t used = std::min<int64_t>(a.types, a.M), pieces = w.slots / per + used;
