@@ -33,32 +33,26 @@ struct NormArgs {
     Range8 r8;
 };
 
-// The part of a row that one of TPR threads holds: N slots of V values.
-// Aligned rows: a slot is 16 contiguous bytes.  Others: 4 values, one column
-// per lane, W (= lanes of the row within a warp) columns apart.  Either way a
-// block of 128 columns lies in one slot of 128 / V neighbouring lanes, so its
-// largest magnitude is a shuffle reduction (ROW_IS_BLOCK: the TPR lanes of a
-// row of at most 128 columns, and all their slots).
+// The part of a row that one of TPR threads holds: N slots of V neighbouring
+// values (16 bytes of aligned rows, 4 values of others).  A block of 128
+// columns lies in one slot of 128 / V neighbouring lanes, so its largest
+// magnitude is a shuffle reduction (ROW_IS_BLOCK: the TPR lanes of a row of at
+// most 128 columns, and all their slots).
 template <class T, bool ALIGNED, int TPR, int VPT>
 struct RowPart {
     static constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
     static constexpr int N = VPT / V;
     static constexpr int W = TPR < 32 ? TPR : 32;
-    static constexpr int J = ALIGNED ? 1 : W;  // columns between a slot's values
     static constexpr bool ROW_IS_BLOCK = TPR * V < kBlock8;
     static constexpr int G = ROW_IS_BLOCK ? TPR : kBlock8 / V;
     static_assert(!ROW_IS_BLOCK || TPR * VPT <= kBlock8, "a row of several slots within a block");
 
-    int t, c0, cols;  // thread of the row, its first column, the row's columns
-    __device__ __forceinline__ RowPart(int64_t columns) {
-        t = threadIdx.x % TPR;
-        c0 = ALIGNED ? t * V : t / W * W * V + t % W;
-        cols = static_cast<int>(columns);
-    }
-    __device__ __forceinline__ int col(int i, int j) const { return c0 + i * TPR * V + j * J; }
+    int t, cols;  // thread of the row, the row's columns
+    __device__ __forceinline__ RowPart(int64_t columns) : t(threadIdx.x % TPR), cols(static_cast<int>(columns)) {}
+    __device__ __forceinline__ int col(int i, int j) const { return (i * TPR + t) * V + j; }
     __device__ __forceinline__ bool has(int i, int j) const { return col(i, j) < cols; }
-    // Slot i exists for some thread (the same answer for all of them).
-    __device__ __forceinline__ bool any(int i) const { return i == 0 || i * TPR * V < cols; }
+    // Slot i exists for some thread of the warp (the same answer for all of them).
+    __device__ __forceinline__ bool any(int i) const { return (i * TPR + t / W * W) * V < cols; }
     // The thread's slot i is all there.
     __device__ __forceinline__ bool whole(int i) const { return col(i, V - 1) < cols; }
 
@@ -66,25 +60,29 @@ struct RowPart {
     __device__ __forceinline__ void fetch(const T* p, bool live, Raw<T, V> (&k)[N]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (live && whole(i))
-                k[i] = ALIGNED ? load_raw<T, V>(p + col(i, 0)) : gather_raw<T, V>([&](int j) { return p[col(i, j)]; });
-            else
+            if (live && whole(i)) {
+                if constexpr (ALIGNED) k[i] = load_raw<T, V>(p + col(i, 0));
+                else k[i] = load4_any(p + col(i, 0));
+            } else if (any(i)) {
                 k[i] = gather_raw<T, V>([&](int j) { return live && has(i, j) ? p[col(i, j)] : from_f32<T>(0.0f); });
+            } else {
+                k[i] = gather_raw<T, V>([](int) { return from_f32<T>(0.0f); });
+            }
         }
     }
+    // A slot of gamma or beta.
     template <class P>
     __device__ __forceinline__ void load(const P* p, int i, float (&x)[V]) const {
-        if (ALIGNED && sizeof(P) == sizeof(T) && whole(i)) {
-            load_v<P, V>(p + col(i, 0), x);
-        } else if (ALIGNED && sizeof(P) == 4 && whole(i)) {  // fp32 parameters of 16-bit rows
+        if (whole(i) && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+            if constexpr (V * sizeof(P) <= 16) {
+                load_v<P, V>(p + col(i, 0), x);
+            } else {
 #pragma unroll
-            for (int j = 0; j < V; j += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(p + col(i, j));
-                x[j] = q.x, x[j + 1] = q.y, x[j + 2] = q.z, x[j + 3] = q.w;
+                for (int j = 0; j < V; j += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(p + col(i, j));
+                    x[j] = q.x, x[j + 1] = q.y, x[j + 2] = q.z, x[j + 3] = q.w;
+                }
             }
-        } else if (whole(i)) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = to_f32(p[col(i, j)]);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) x[j] = has(i, j) ? to_f32(p[col(i, j)]) : 0.0f;
@@ -92,13 +90,8 @@ struct RowPart {
     }
     __device__ __forceinline__ void store(T* p, int i, const float (&x)[V]) const {
         if (whole(i)) {
-            if (ALIGNED) {
-                store_v<T, V>(p + col(i, 0), x);
-            } else {
-                Raw<T, V> k;
-                narrow(x, k);
-                scatter_raw(k, [&](int j, T v) { p[col(i, j)] = v; });
-            }
+            if constexpr (ALIGNED) store_v<T, V>(p + col(i, 0), x);
+            else store4_any(p + col(i, 0), x);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -107,30 +100,27 @@ struct RowPart {
     }
 };
 
-// Sums a and b over the TPR threads of a row; every thread gets them.
-// `red`: 2 floats per warp of the block (rows of several warps; the whole
+// Sums of S values over the TPR threads of a row; every thread gets them.
+// `red`: S floats per warp of the block (rows of several warps; the whole
 // block takes part).
-template <int TPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
-    a = reduce_sum<float, (TPR < 32 ? TPR : 32)>(a);
-    b = reduce_sum<float, (TPR < 32 ? TPR : 32)>(b);
-    if (TPR <= 32) return;
-    constexpr int NW = TPR > 32 ? TPR / 32 : 1;
-    __syncthreads();  // the previous sum has been read
-    if (threadIdx.x % 32 == 0) {
-        red[threadIdx.x / 32 * 2] = a;
-        red[threadIdx.x / 32 * 2 + 1] = b;
-    }
-    __syncthreads();
-    a = b = 0.0f;
-    const float* mine = red + threadIdx.x / TPR * NW * 2;
+template <int TPR, int S>
+__device__ __forceinline__ void row_sum(float (&x)[S], float* red) {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        a += mine[2 * w];
-        b += mine[2 * w + 1];
+    for (int k = 0; k < S; ++k) x[k] = reduce_sum<float, (TPR < 32 ? TPR : 32)>(x[k]);
+    if constexpr (TPR > 32) {
+        constexpr int NW = TPR / 32;
+        const int lane = threadIdx.x % 32;
+        __syncthreads();  // the previous sum has been read
+        if (lane < S) red[threadIdx.x / 32 * S + lane] = S == 1 || lane == 0 ? x[0] : x[S - 1];
+        __syncthreads();
+        // each warp adds up the row's warps, one a lane
+        const float* mine = red + threadIdx.x / TPR * NW * S;
+#pragma unroll
+        for (int k = 0; k < S; ++k) x[k] = reduce_sum<float, NW>(mine[lane % NW * S + k]);
     }
 }
 
+// Threads of a block.
 template <int TPR>
 constexpr int block_threads() { return TPR < 128 ? 128 : TPR; }
 
@@ -140,123 +130,128 @@ constexpr int resident() { return TPR >= 256 ? 1024 / TPR : (VPT > 8 ? 5 : 8); }
 template <int TPR, int VPT>
 constexpr int resident_grad() { return TPR >= 256 ? 512 / TPR : (VPT > 8 ? 4 : 5); }
 
-// Rows' data is fetched one row ahead while it fits in registers.
-template <class T, int VPT>
-constexpr bool ahead() { return VPT * sizeof(T) <= 64; }
+// How many of its next rows a group of threads has asked for: as many as keep
+// about 16 KB of loads in flight a SM (one row at a time left HBM at 45 %).
+template <class T, int TPR, int VPT>
+constexpr int rows_ahead() { return TPR >= 256 ? 1 : VPT * sizeof(T) <= 16 ? 4 : (VPT * sizeof(T) <= 32 ? 2 : 1); }
+
+// gamma and beta as they lie in memory, kept in registers where they are few.
+template <class R, class T, class P>
+struct Params {
+    static constexpr bool kKeep = R::N * R::V * sizeof(P) <= 32;
+    Raw<P, R::V> k[kKeep ? R::N : 1];
+    const P* p;
+    __device__ __forceinline__ Params(const R& part, const P* q) : p(q) {
+        if (kKeep) {
+#pragma unroll
+            for (int i = 0; i < R::N; ++i)
+                k[kKeep ? i : 0] = gather_raw<P, R::V>(
+                    [&](int j) { return part.has(i, j) ? p[part.col(i, j)] : from_f32<P>(0.0f); });
+        }
+    }
+    __device__ __forceinline__ void get(const R& part, int i, float (&x)[R::V]) const {
+        if (kKeep) widen(k[kKeep ? i : 0], x);
+        else part.load(p, i, x);
+    }
+};
 
 template <class T, class P, bool ALIGNED, int TPR, int VPT>
 __global__ void __launch_bounds__(block_threads<TPR>(), resident<TPR, VPT>()) norm_kernel(NormArgs a, const T* x, int64_t ldx, const P* gamma,
                                                                     const P* beta, T* y, int64_t ldy, float2* stats,
                                                                     Saved8 s) {
     using R = RowPart<T, ALIGNED, TPR, VPT>;
-    constexpr int V = R::V, N = R::N;
-    constexpr bool kKeep = VPT <= 8;  // gamma and beta stay in registers
+    constexpr int V = R::V, N = R::N, D = rows_ahead<T, TPR, VPT>();
     __shared__ float red[32];
     constexpr int RPB = block_threads<TPR>() / TPR;
     const R part(a.cols);
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
     const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
-    float gk[kKeep ? N : 1][V], bk[kKeep ? N : 1][V];
-    if (kKeep) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            part.load(gamma, i, gk[kKeep ? i : 0]);
-            part.load(beta, i, bk[kKeep ? i : 0]);
-        }
-    }
+    const Params<R, T, P> g(part, gamma), b(part, beta);
     // every thread takes part in the reductions: the loop runs on the block's first row
     int64_t base = static_cast<int64_t>(blockIdx.x) * RPB, row = base + threadIdx.x / TPR;
-    Raw<T, V> k[N];
-    if (ahead<T, VPT>()) part.fetch(x + (row < a.rows ? row * ldx : 0), row < a.rows, k);
-    for (; base < a.rows; base += step, row += step) {
-        const bool live = row < a.rows;
-        if (!ahead<T, VPT>()) part.fetch(x + (live ? row * ldx : 0), live, k);
-        float v[N][V];
-        float sum = 0.0f, none = 0.0f;
+    Raw<T, V> ring[D][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            widen(k[i], v[i]);
+    for (int d = 0; d < D; ++d) {
+        const int64_t r = row + d * step;
+        part.fetch(x + (r < a.rows ? r * ldx : 0), r < a.rows, ring[d]);
+    }
+    while (base < a.rows) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum += v[i][j];
-        }
-        if (ahead<T, VPT>()) {
-            const int64_t next = row + step;
-            part.fetch(x + (next < a.rows ? next * ldx : 0), next < a.rows, k);
-        }
-        row_sum2<TPR>(sum, none, red);
-        const float mean = __fmul_rn(sum, inv_n);
-        float sq = 0.0f;
+        for (int d = 0; d < D; ++d, base += step, row += step) {
+            if (base >= a.rows) break;
+            const bool live = row < a.rows;
+            float v[N][V];
+            float sum[1] = {0.0f};
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (!part.any(i)) break;
+            for (int i = 0; i < N; ++i) {
+                widen(ring[d][i], v[i]);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i][j] = __fsub_rn(v[i][j], mean);
-            if (!part.whole(i)) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[i][j] = part.has(i, j) ? v[i][j] : 0.0f;
+                for (int j = 0; j < V; ++j) sum[0] += v[i][j];
             }
+            const int64_t next = row + D * step;
+            part.fetch(x + (next < a.rows ? next * ldx : 0), next < a.rows, ring[d]);
+            row_sum<TPR>(sum, red);
+            const float mean = __fmul_rn(sum[0], inv_n);
+            float sq[1] = {0.0f};
 #pragma unroll
-            for (int j = 0; j < V; ++j) sq = fmaf(v[i][j], v[i][j], sq);
-        }
-        row_sum2<TPR>(sq, none, red);
-        const float rstd = rsqrtf(fmaf(sq, inv_n, a.eps));  // 2 ulp
-        if (live && part.t == 0) stats[row] = make_float2(mean, rstd);
-        float row_max = 0.0f;
+            for (int i = 0; i < N; ++i) {
+                if (!part.any(i)) break;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            map_v(v[i], [rstd](float u) { return __fmul_rn(u, rstd); });
-            if (R::ROW_IS_BLOCK) {
+                for (int j = 0; j < V; ++j) v[i][j] = __fsub_rn(v[i][j], mean);
+                if (!part.whole(i)) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) row_max = max_mag(row_max, v[i][j]);
-            }
-        }
-        const int64_t at = live ? row : 0;
-        T* yr = y + at * ldy;
-        int8_t* codes = s.codes + at * s.ld;
-        uint8_t* exps = s.exps + at * s.lde;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (!part.any(i)) break;
-            if (s.codes) {
-                float m = row_max;
-                if (!R::ROW_IS_BLOCK) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) m = max_mag(m, v[i][j]);
+                    for (int j = 0; j < V; ++j) v[i][j] = part.has(i, j) ? v[i][j] : 0.0f;
                 }
-                const int byte = exponent8(reduce_max<R::G>(m), a.r8.emin);
-                const float inv = encode8(byte);
-                if (!live) {
-                } else if (part.whole(i)) {
-                    if (ALIGNED) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
+            }
+            row_sum<TPR>(sq, red);
+            const float rstd = rsqrtf(fmaf(sq[0], inv_n, a.eps));  // 2 ulp
+            if (live && part.t == 0) stats[row] = make_float2(mean, rstd);
+            float row_max = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (!part.any(i)) break;
+                map_v(v[i], [rstd](float u) { return __fmul_rn(u, rstd); });
+                if (R::ROW_IS_BLOCK) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) row_max = max_mag(row_max, v[i][j]);
+                }
+            }
+            const int64_t at = live ? row : 0;
+            T* yr = y + at * ldy;
+            int8_t* codes = s.codes + at * s.ld;
+            uint8_t* exps = s.exps + at * s.lde;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (!part.any(i)) break;
+                if (s.codes) {
+                    float m = row_max;
+                    if (!R::ROW_IS_BLOCK) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) m = max_mag(m, v[i][j]);
+                    }
+                    const int byte = exponent8(reduce_max<R::G>(m), a.r8.emin);
+                    const float inv = encode8(byte);
+                    if (!live) {
+                    } else if (part.whole(i)) {
                         store_codes<V>(codes + part.col(i, 0), v[i], inv, byte, a.r8.top);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < V; j += 4) {
-                            const uint32_t c = codes4(v[i][j], v[i][j + 1], v[i][j + 2], v[i][j + 3], inv, byte, a.r8.top);
-#pragma unroll
-                            for (int b = 0; b < 4; ++b) codes[part.col(i, j + b)] = static_cast<int8_t>(c >> 8 * b);
-                        }
+                        for (int j = 0; j < V; ++j)
+                            if (part.has(i, j)) codes[part.col(i, j)] = code8(v[i][j], inv, byte, a.r8.top);
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (part.has(i, j)) codes[part.col(i, j)] = code8(v[i][j], inv, byte, a.r8.top);
+                    // the first lane of the group that holds the block writes its exponent
+                    if (live && part.t % R::G == 0 && (i == 0 || !R::ROW_IS_BLOCK) && part.has(i, 0))
+                        exps[part.col(i, 0) / kBlock8] = static_cast<uint8_t>(byte);
                 }
-                // the first lane of the group that holds the block writes its exponent
-                if (live && part.t % R::G == 0 && (i == 0 || !R::ROW_IS_BLOCK) && part.has(i, 0))
-                    exps[part.col(i, 0) / kBlock8] = static_cast<uint8_t>(byte);
-            }
-            float g[V], b[V];
-            if (kKeep) {
+                float w[V], c[V];
+                g.get(part, i, w);
+                b.get(part, i, c);
 #pragma unroll
-                for (int j = 0; j < V; ++j) g[j] = gk[kKeep ? i : 0][j], b[j] = bk[kKeep ? i : 0][j];
-            } else {
-                part.load(gamma, i, g);
-                part.load(beta, i, b);
+                for (int j = 0; j < V; ++j) w[j] = fmaf(v[i][j], w[j], c[j]);
+                if (live) part.store(yr, i, w);
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) g[j] = fmaf(v[i][j], g[j], b[j]);
-            if (live) part.store(yr, i, g);
         }
     }
 }
@@ -267,8 +262,13 @@ __device__ __forceinline__ void fetch_codes(const R& part, const int8_t* codes, 
                                             Raw<int8_t, R::V> (&k)[R::N], int (&e)[R::N]) {
 #pragma unroll
     for (int i = 0; i < R::N; ++i) {
-        e[i] = live && part.has(i, 0) ? exps[part.col(i, 0) / kBlock8] : 127;
-        if (live && part.whole(i) && R::J == 1)
+        e[i] = 127;
+        if (!part.any(i)) {
+            k[i] = gather_codes<R::V>([](int) { return int8_t(0); });
+            continue;
+        }
+        if (live && part.has(i, 0)) e[i] = exps[part.col(i, 0) / kBlock8];
+        if (live && part.whole(i))
             k[i] = *reinterpret_cast<const Raw<int8_t, R::V>*>(codes + part.col(i, 0));
         else
             k[i] = gather_codes<R::V>([&](int j) { return live && part.has(i, j) ? codes[part.col(i, j)] : int8_t(0); });
@@ -282,85 +282,82 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
                                                                          const float2* stats, const P* gamma, T* dx,
                                                                          int64_t lddx, float* partial) {
     using R = RowPart<T, ALIGNED, TPR, VPT>;
-    constexpr int V = R::V, N = R::N, RPB = block_threads<TPR>() / TPR;
-    constexpr bool kKeep = VPT <= 8, kAhead = ahead<T, 2 * VPT>();
+    constexpr int V = R::V, N = R::N, RPB = block_threads<TPR>() / TPR, D = (rows_ahead<T, TPR, VPT>() + 1) / 2;
     __shared__ float red[32];
     __shared__ float join[RPB > 1 ? RPB * TPR * VPT : 1];
     const R part(a.cols);
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
     const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
-    float ag[N][V], ab[N][V], gk[kKeep ? N : 1][V];
+    const Params<R, T, P> w8(part, gamma);
+    float ag[N][V], ab[N][V];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (kKeep) part.load(gamma, i, gk[kKeep ? i : 0]);
+    for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) ag[i][j] = ab[i][j] = 0.0f;
-    }
-    Raw<T, V> kd[N], kx[SAVED ? 1 : N];
-    Raw<int8_t, V> kc[SAVED ? N : 1];
-    int ke[SAVED ? N : 1];
-    float2 st;
-    const auto fetch = [&](int64_t r) {
+    Raw<T, V> kd[D][N], kx[SAVED ? 1 : D][N];
+    Raw<int8_t, V> kc[SAVED ? D : 1][N];
+    int ke[SAVED ? D : 1][N];
+    float2 st[D];
+    const auto fetch = [&](int d, int64_t r) {
         const bool live = r < a.rows;
         const int64_t at = live ? r : 0;
-        st = stats[at];
-        part.fetch(dy + at * lddy, live, kd);
-        if constexpr (SAVED) fetch_codes(part, s.codes + at * s.ld, s.exps + at * s.lde, live, kc, ke);
-        else part.fetch(x + at * ldx, live, kx);
+        st[d] = stats[at];
+        part.fetch(dy + at * lddy, live, kd[d]);
+        if constexpr (SAVED) fetch_codes(part, s.codes + at * s.ld, s.exps + at * s.lde, live, kc[SAVED ? d : 0], ke[SAVED ? d : 0]);
+        else part.fetch(x + at * ldx, live, kx[SAVED ? 0 : d]);
     };
     int64_t base = static_cast<int64_t>(blockIdx.x) * RPB, row = base + threadIdx.x / TPR;
-    if (kAhead) fetch(row);
-    for (; base < a.rows; base += step, row += step) {
-        const bool live = row < a.rows;
-        if (!kAhead) fetch(row);
-        const float mean = st.x, rstd = st.y;
-        float h[N][V], g[N][V];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if constexpr (SAVED) {
+    for (int d = 0; d < D; ++d) fetch(d, row + d * step);
+    while (base < a.rows) {
 #pragma unroll
-                for (int j = 0; j < V; j += 4) values4(kc[i].w[j / 4], ke[i], &h[i][j]);
-            } else {
-                widen(kx[i], h[i]);
+        for (int d = 0; d < D; ++d, base += step, row += step) {
+            if (base >= a.rows) break;
+            const bool live = row < a.rows;
+            const float mean = st[d].x, rstd = st[d].y;
+            float h[N][V], g[N][V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) h[i][j] = __fmul_rn(__fsub_rn(h[i][j], mean), rstd);
-                if (!part.whole(i)) {
+            for (int i = 0; i < N; ++i) {
+                if constexpr (SAVED) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) h[i][j] = part.has(i, j) ? h[i][j] : 0.0f;
+                    for (int j = 0; j < V; j += 4) values4(kc[SAVED ? d : 0][i].w[j / 4], ke[SAVED ? d : 0][i], &h[i][j]);
+                } else {
+                    widen(kx[SAVED ? 0 : d][i], h[i]);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) h[i][j] = __fmul_rn(__fsub_rn(h[i][j], mean), rstd);
+                    if (!part.whole(i)) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) h[i][j] = part.has(i, j) ? h[i][j] : 0.0f;
+                    }
+                }
+                widen(kd[d][i], g[i]);
+            }
+            fetch(d, row + D * step);
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (!part.any(i)) break;
+                float w[V];
+                w8.get(part, i, w);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    ag[i][j] = fmaf(g[i][j], h[i][j], ag[i][j]);
+                    ab[i][j] += g[i][j];
+                    g[i][j] = __fmul_rn(g[i][j], w[j]);
+                    sum[0] += g[i][j];
+                    sum[1] = fmaf(g[i][j], h[i][j], sum[1]);
                 }
             }
-            widen(kd[i], g[i]);
-        }
-        if (kAhead) fetch(row + step);
-        float s1 = 0.0f, s2 = 0.0f;
+            row_sum<TPR>(sum, red);
+            const float m1 = __fmul_rn(sum[0], inv_n), m2 = __fmul_rn(sum[1], inv_n);
+            T* out = dx + (live ? row * lddx : 0);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (!part.any(i)) break;
-            float w[V];
-            if (kKeep) {
+            for (int i = 0; i < N; ++i) {
+                if (!part.any(i)) break;
 #pragma unroll
-                for (int j = 0; j < V; ++j) w[j] = gk[kKeep ? i : 0][j];
-            } else {
-                part.load(gamma, i, w);
+                for (int j = 0; j < V; ++j) g[i][j] = __fmul_rn(rstd, fmaf(-h[i][j], m2, __fsub_rn(g[i][j], m1)));
+                if (live) part.store(out, i, g[i]);
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                ag[i][j] = fmaf(g[i][j], h[i][j], ag[i][j]);
-                ab[i][j] += g[i][j];
-                g[i][j] = __fmul_rn(g[i][j], w[j]);
-                s1 += g[i][j];
-                s2 = fmaf(g[i][j], h[i][j], s2);
-            }
-        }
-        row_sum2<TPR>(s1, s2, red);
-        const float m1 = __fmul_rn(s1, inv_n), m2 = __fmul_rn(s2, inv_n);
-        T* out = dx + (live ? row * lddx : 0);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (!part.any(i)) break;
-#pragma unroll
-            for (int j = 0; j < V; ++j) g[i][j] = __fmul_rn(rstd, fmaf(-h[i][j], m2, __fsub_rn(g[i][j], m1)));
-            if (live) part.store(out, i, g[i]);
         }
     }
     float* sums = partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
@@ -390,7 +387,7 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
 #pragma unroll 4
                 for (int r = 0; r < RPB; ++r) sum += join[r * VPT * TPR + q];
                 const int t = q % TPR, i = q / TPR / V, j = q / TPR % V;
-                const int c = (ALIGNED ? t * V : t / R::W * R::W * V + t % R::W) + i * TPR * V + j * R::J;
+                const int c = (i * TPR + t) * V + j;
                 if (c < a.cols) sums[half * a.cols + c] = sum;
             }
         }
@@ -406,17 +403,17 @@ __global__ void __launch_bounds__(512) norm_wide_kernel(NormArgs a, const T* x, 
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* xr = x + row * ldx;
-        float sum = 0.0f, none = 0.0f;
-        for (int64_t c = threadIdx.x; c < a.cols; c += 512) sum += to_f32(xr[c]);
-        row_sum2<512>(sum, none, red);
-        const float mean = __fmul_rn(sum, inv_n);
-        float sq = 0.0f;
+        float sum[1] = {0.0f};
+        for (int64_t c = threadIdx.x; c < a.cols; c += 512) sum[0] += to_f32(xr[c]);
+        row_sum<512>(sum, red);
+        const float mean = __fmul_rn(sum[0], inv_n);
+        float sq[1] = {0.0f};
         for (int64_t c = threadIdx.x; c < a.cols; c += 512) {
             const float d = __fsub_rn(to_f32(xr[c]), mean);
-            sq = fmaf(d, d, sq);
+            sq[0] = fmaf(d, d, sq[0]);
         }
-        row_sum2<512>(sq, none, red);
-        const float rstd = rsqrtf(fmaf(sq, inv_n, a.eps));
+        row_sum<512>(sq, red);
+        const float rstd = rsqrtf(fmaf(sq[0], inv_n, a.eps));
         if (threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
         // one warp per block of 128 columns
         for (int64_t b = warp; b * kBlock8 < a.cols; b += 16) {
@@ -458,14 +455,14 @@ __global__ void __launch_bounds__(512) norm_wide_grad_kernel(NormArgs a, const T
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const float2 st = stats[row];
-        float s1 = 0.0f, s2 = 0.0f;
+        float sum[2] = {0.0f, 0.0f};
         for (int64_t c = threadIdx.x; c < a.cols; c += 512) {
             const float g = __fmul_rn(to_f32(dy[row * lddy + c]), to_f32(gamma[c]));
-            s1 += g;
-            s2 = fmaf(g, wide_h<T, SAVED>(x, ldx, s, st, row, c), s2);
+            sum[0] += g;
+            sum[1] = fmaf(g, wide_h<T, SAVED>(x, ldx, s, st, row, c), sum[1]);
         }
-        row_sum2<512>(s1, s2, red);
-        const float m1 = __fmul_rn(s1, inv_n), m2 = __fmul_rn(s2, inv_n);
+        row_sum<512>(sum, red);
+        const float m1 = __fmul_rn(sum[0], inv_n), m2 = __fmul_rn(sum[1], inv_n);
         for (int64_t c = threadIdx.x; c < a.cols; c += 512) {
             const float g = __fmul_rn(to_f32(dy[row * lddy + c]), to_f32(gamma[c]));
             const float h = wide_h<T, SAVED>(x, ldx, s, st, row, c);
@@ -521,7 +518,8 @@ template <class F>
 void by_width(int64_t cols, F&& f) {
     using std::integral_constant;
     if (cols <= 32) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
-    else if (cols <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (cols <= 64) f(integral_constant<int, 4>{}, integral_constant<int, 16>{});
+    else if (cols <= 128) f(integral_constant<int, 8>{}, integral_constant<int, 16>{});
     else if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
     else if (cols <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
     else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});

@@ -18,29 +18,33 @@ namespace tg {
 
 namespace {
 
-// Lane mapping of one block: G lanes, V values each.  Aligned rows: 16 bytes
-// a lane, contiguous.  Others: 32 lanes, 4 values each, 32 columns apart.
+// Lane mapping of one block: G lanes, V neighbouring values each: 16 bytes of
+// aligned rows, 4 values of others.
 template <class T, bool ALIGNED>
 struct Lanes {
     static constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
     static constexpr int G = kBlock8 / V;
-    static constexpr int U = ALIGNED ? 4 : 2;  // rows in flight
+    static constexpr int U = 4;  // rows in flight
     int lane, left;   // of the block's columns, `left` exist
-    bool full;        // the lane's values are all there, and contiguous
+    bool full;        // the lane's values are all there
 
     __device__ __forceinline__ Lanes(int64_t columns_left) {
         lane = threadIdx.x % G;
         left = columns_left < kBlock8 ? static_cast<int>(columns_left) : kBlock8;
-        full = ALIGNED && (lane + 1) * V <= left;
+        full = (lane + 1) * V <= left;
     }
-    __device__ __forceinline__ int col(int j) const { return ALIGNED ? lane * V + j : j * 32 + lane; }
+    __device__ __forceinline__ int col(int j) const { return lane * V + j; }
     __device__ __forceinline__ Raw<T, V> load(const T* p, bool live) const {
-        if (full && live) return load_raw<T, V>(p + lane * V);
+        if (full && live) {
+            if constexpr (ALIGNED) return load_raw<T, V>(p + lane * V);
+            else return load4_any(p + lane * V);
+        }
         return gather_raw<T, V>([&](int j) { return col(j) < left && live ? p[col(j)] : from_f32<T>(0.0f); });
     }
     __device__ __forceinline__ void store(T* p, const float (&x)[V]) const {
         if (full) {
-            store_v<T, V>(p + lane * V, x);
+            if constexpr (ALIGNED) store_v<T, V>(p + lane * V, x);
+            else store4_any(p + lane * V, x);
             return;
         }
 #pragma unroll

@@ -118,10 +118,6 @@ __device__ __forceinline__ uint32_t in_rank(const void* bar, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(mb::smem_u32(bar)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void arrive_expect_tx_at(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
-}
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }

@@ -87,8 +87,8 @@ struct WeightArgs {
 // ── How a weight gradient is cut up ──────────────────────────────────────
 // Each tile of each type's dW is a sum over the type's rows, in steps of 64.
 // An item is a tile and a piece of its type's rows, for one CTA.  A type is
-// one piece unless it has more steps than an SM's share of all the steps
-// (`slots` SMs, `per` tiles a type); then it is cut into the fewest equal
+// one piece unless it has more steps than 5/4 of an SM's share of all the
+// steps (`slots` SMs, `per` tiles a type); then it is cut into the fewest equal
 // pieces that have no more.  Items run longest first, dealt out to the CTAs
 // back and forth, so the CTAs' totals come out nearly equal without a counter
 // in memory, and few types are cut at all: a cut type leaves partial sums
@@ -102,8 +102,8 @@ __device__ __forceinline__ int rows_of(const int32_t* offsets, int t, int64_t M)
     return e > b ? e - b : 0;
 }
 // Rows of the longest piece, from the sum of all types' steps.
-__device__ __forceinline__ int64_t piece_limit(int64_t steps, int per, int slots) {
-    const int64_t share = (steps * per + slots - 1) / slots;
+__host__ __device__ __forceinline__ int64_t piece_limit(int64_t steps, int per, int slots) {
+    const int64_t share = (steps * per * 5 + slots * 4 - 1) / (slots * 4);
     return (share < 2 ? 2 : share) * kStep;
 }
 __device__ __forceinline__ int piece_count(int n, int64_t limit) { return static_cast<int>((n + limit - 1) / limit); }

@@ -32,7 +32,7 @@ struct PairPlan {
 constexpr int STAGES = PairPlan::kStages;
 
 struct PairShared {
-    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain, tail;
+    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain, tail, tail_peer;
     uint32_t tmem;
     int prefix[kMaxTypes + 1];
     uint16_t order[kMaxTypes];  // weight gradients only
@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t set_up_pair(PairShared& s, F&& plan) {
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mb::init(&s.full[i], 2);   // both CTAs' producers
+            mb::init(&s.full[i], 1);
             mb::init(&s.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -52,6 +52,7 @@ __device__ __forceinline__ uint32_t set_up_pair(PairShared& s, F&& plan) {
         }
         mb::init(&s.drain, 1);
         mb::init(&s.tail, 1);
+        mb::init(&s.tail_peer, 1);
         mb::fence_init();
     }
     if (warp == 2) tc::alloc_pair(&s.tmem, 2 * BN);
@@ -123,8 +124,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     const int st = static_cast<int>(i % STAGES);
                     if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_error, 51))) break;
                     const uint32_t a = ring + st * PairPlan::kStage, b = a + PairPlan::kA;
+                    // rank 0 expects both CTAs' bytes (a remote arrival would wait
+                    // for this thread's earlier operations: 0.6 us a stage)
                     const uint32_t bar = tc::in_rank(&s.full[st], 0);
-                    tc::arrive_expect_tx_at(bar, PairPlan::kStage);
+                    if (rank == 0) mb::arrive_expect_tx(&s.full[st], 2 * PairPlan::kStage);
                     tc::tma3_pair(a, &ma, kb * tc::kInner, row0, 0, bar);
                     if (TRANS) {
                         tc::tma3_pair(b, &mw, kb * tc::kInner, n0, t, bar);
@@ -236,7 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (lane == 0) {
                     const uint32_t on = cut ? mb::smem_u32(&s.tail) : bar;
                     if (cut) mb::arrive_expect_tx(&s.tail, PairPlan::kStage);
-                    else tc::arrive_expect_tx_at(bar, PairPlan::kStage);
+                    else if (rank == 0) mb::arrive_expect_tx(&s.full[st], 2 * PairPlan::kStage);
 #pragma unroll
                     for (int c = 0; c < BM / 64; ++c)
                         tc::tma3_pair(a + c * tc::kChunkBytes, &mx, k0 + c * 64, static_cast<int>(r), 0, on);
@@ -248,10 +251,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (cut) {
                     // The piece's last rows are followed by another's: zero in
                     // both operands (0 x NaN would not do), then pass them on.
-                    ok = mb::wait(&s.tail, tails++ & 1, &g_error, 62);
+                    ok = mb::wait(&s.tail, tails & 1, &g_error, 62);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
                     zero_rows(a, PairPlan::kStage, static_cast<int>(m.r1 - r));
-                    if (lane == 0) tc::arrive_at(bar);
+                    if (rank != 0) {
+                        if (lane == 0) tc::arrive_at(tc::in_rank(&s.tail_peer, 0));
+                    } else {
+                        ok = tc::wait_cluster(&s.tail_peer, tails & 1, &g_error, 67);
+                        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                        if (lane == 0) mb::arrive(&s.full[st]);
+                    }
+                    ++tails;
                     __syncwarp();
                 }
             }

@@ -260,6 +260,7 @@ template <class O>
 struct JoinArgs {
     int64_t M, K, N, ldp;
     int types, per, slots;
+    int64_t least;  // no type of fewer rows is cut (the limit when no step is ragged)
     const int32_t* offsets;
     const float *part, *db_part;
     O* dW;
@@ -272,6 +273,7 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O
     __shared__ int64_t sums[8];
     __shared__ int first[8];
     const int t = blockIdx.y, rows = rows_of(g.offsets, t, g.M);
+    if (rows <= g.least) return;
     const auto block_sum = [&](auto x, auto* sh) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -295,29 +297,32 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O
     }
     const int64_t p = block_sum(before, first);
     const float* part = g.part + p * g.K * g.ldp;
-    const int64_t vecs = g.ldp / 4, total = g.K * vecs, next = g.K * g.ldp;
-    for (int64_t v = blockIdx.x * 256 + threadIdx.x; v < total; v += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t k = v / vecs, c = (v - k * vecs) * 4;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float* q = part + k * g.ldp + c;
+    // four columns a thread; a block takes as many rows of dW at a time as it has threads for
+    const int vecs = static_cast<int>(g.ldp / 4), wide = vecs < 256 ? vecs : 256, rpb = 256 / wide;
+    const int64_t next = g.K * g.ldp;
+    const int r = threadIdx.x / wide;
+    for (int64_t k = blockIdx.x * rpb + r; r < rpb && k < g.K; k += static_cast<int64_t>(gridDim.x) * rpb)
+        for (int64_t c = (threadIdx.x - r * wide) * 4; c < g.N; c += wide * 4) {
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float* q = part + k * g.ldp + c;
 #pragma unroll 8
-        for (int i = 0; i < n; ++i, q += next) {
-            const float4 x = *reinterpret_cast<const float4*>(q);
-            sum.x += x.x;
-            sum.y += x.y;
-            sum.z += x.z;
-            sum.w += x.w;
-        }
-        O* o = g.dW + t * g.stride_dw + k * g.lddw + c;
-        const float y[4] = {sum.x, sum.y, sum.z, sum.w};
-        if (c + 4 <= g.N && (reinterpret_cast<uintptr_t>(o) % (4 * sizeof(O))) == 0) {
-            store_v<O, 4>(o, y);
-        } else {
+            for (int i = 0; i < n; ++i, q += next) {
+                const float4 x = *reinterpret_cast<const float4*>(q);
+                sum.x += x.x;
+                sum.y += x.y;
+                sum.z += x.z;
+                sum.w += x.w;
+            }
+            O* o = g.dW + t * g.stride_dw + k * g.lddw + c;
+            const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+            if (c + 4 <= g.N && (reinterpret_cast<uintptr_t>(o) % (4 * sizeof(O))) == 0) {
+                store_v<O, 4>(o, y);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c + j < g.N) o[j] = from_f32<O>(y[j]);
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < g.N) o[j] = from_f32<O>(y[j]);
+            }
         }
-    }
     if (g.db)
         for (int64_t c = blockIdx.x * 256 + threadIdx.x; c < g.N; c += static_cast<int64_t>(gridDim.x) * 256) {
             float sum = 0.0f;
@@ -491,9 +496,10 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
         typed_weight_any<T, O>(a, w, s);
     }
     if (joined) {
-        const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots, a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
+        const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots,
+                            piece_limit(a.M / kStep, static_cast<int>(per), w.slots), a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
                             db_joined ? a.db : nullptr};
-        const int64_t want = ceil_div(a.K * w.ldp / 4, 256);
+        const int64_t want = ceil_div(a.K * std::min<int64_t>(w.ldp / 4, 256), 256);
         launch("typed_weight_join", typed_weight_join_kernel<O>,
                dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(1, 8 * num_sms() / a.types))),
                     static_cast<unsigned>(a.types)),

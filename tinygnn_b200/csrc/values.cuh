@@ -137,6 +137,49 @@ __device__ __forceinline__ void store_v(T* p, const float (&x)[V]) {
     *reinterpret_cast<Raw<T, V>*>(p) = k;
 }
 
+// Four values at p of any alignment (of T's): 16-bit ones in whole words,
+// shifted by half a word where p is odd.  The first and the last word then
+// reach one value past the four, in words that hold one of them.
+template <class T>
+__device__ __forceinline__ Raw<T, 4> load4_any(const T* p) {
+    Raw<T, 4> k;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k.w[j] = bits(p[j]);
+    } else {
+        const uintptr_t u = reinterpret_cast<uintptr_t>(p);
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(u & ~uintptr_t(3));
+        const uint32_t a = q[0], b = q[1];
+        if (u & 2) {
+            const uint32_t c = q[2];
+            k.w[0] = __byte_perm(a, b, 0x5432);
+            k.w[1] = __byte_perm(b, c, 0x5432);
+        } else {
+            k.w[0] = a;
+            k.w[1] = b;
+        }
+    }
+    return k;
+}
+template <class T>
+__device__ __forceinline__ void store4_any(T* p, const float (&x)[4]) {
+    Raw<T, 4> k;
+    narrow(x, k);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = x[j];
+    } else if (reinterpret_cast<uintptr_t>(p) & 2) {
+        uint16_t* q = reinterpret_cast<uint16_t*>(p);
+        q[0] = static_cast<uint16_t>(k.w[0]);
+        *reinterpret_cast<uint32_t*>(q + 1) = __byte_perm(k.w[0], k.w[1], 0x5432);
+        q[3] = static_cast<uint16_t>(k.w[1] >> 16);
+    } else {
+        uint32_t* q = reinterpret_cast<uint32_t*>(p);
+        q[0] = k.w[0];
+        q[1] = k.w[1];
+    }
+}
+
 // max(a, |b|) that keeps a NaN (fmaxf drops it).
 __device__ __forceinline__ float max_mag(float a, float b) {
     float r;
