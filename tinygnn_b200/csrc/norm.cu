@@ -34,13 +34,13 @@ struct NormArgs {
 };
 
 // The part of a row that one of TPR threads holds: N slots of V neighbouring
-// values (16 bytes of aligned rows, 4 values of others).  A block of 128
+// values, 16 bytes (ALIGNED: one access).  A block of 128
 // columns lies in one slot of 128 / V neighbouring lanes, so its largest
 // magnitude is a shuffle reduction (ROW_IS_BLOCK: the TPR lanes of a row of at
 // most 128 columns, and all their slots).
 template <class T, bool ALIGNED, int TPR, int VPT>
 struct RowPart {
-    static constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
+    static constexpr int V = 16 / static_cast<int>(sizeof(T));
     static constexpr int N = VPT / V;
     static constexpr int W = TPR < 32 ? TPR : 32;
     static constexpr bool ROW_IS_BLOCK = TPR * V < kBlock8;
@@ -56,18 +56,14 @@ struct RowPart {
     // The thread's slot i is all there.
     __device__ __forceinline__ bool whole(int i) const { return col(i, V - 1) < cols; }
 
-    // Slots as they lie in memory (zeros where there is nothing; `live` false: all zeros).
-    __device__ __forceinline__ void fetch(const T* p, bool live, Raw<T, V> (&k)[N]) const {
+    // The row's slots (zeros where there is nothing; `live` false: all zeros).
+    using Slot = Held<T, V, ALIGNED>;
+    __device__ __forceinline__ void fetch(const T* p, bool live, Slot (&k)[N]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (live && whole(i)) {
-                if constexpr (ALIGNED) k[i] = load_raw<T, V>(p + col(i, 0));
-                else k[i] = load4_any(p + col(i, 0));
-            } else if (any(i)) {
-                k[i] = gather_raw<T, V>([&](int j) { return live && has(i, j) ? p[col(i, j)] : from_f32<T>(0.0f); });
-            } else {
-                k[i] = gather_raw<T, V>([](int) { return from_f32<T>(0.0f); });
-            }
+            if (live && whole(i)) k[i].fetch(p + col(i, 0));
+            else if (live && has(i, 0)) k[i].fetch(p + col(i, 0), cols - col(i, 0));
+            else k[i].zero();
         }
     }
     // A slot of gamma or beta.
@@ -91,7 +87,7 @@ struct RowPart {
     __device__ __forceinline__ void store(T* p, int i, const float (&x)[V]) const {
         if (whole(i)) {
             if constexpr (ALIGNED) store_v<T, V>(p + col(i, 0), x);
-            else store4_any(p + col(i, 0), x);
+            else store_any<T, V>(p + col(i, 0), x);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -163,13 +159,14 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident<TPR, VPT>()) no
     constexpr int V = R::V, N = R::N, D = rows_ahead<T, TPR, VPT>();
     __shared__ float red[32];
     constexpr int RPB = block_threads<TPR>() / TPR;
+    wait_for_previous();
     const R part(a.cols);
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
     const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
     const Params<R, T, P> g(part, gamma), b(part, beta);
     // every thread takes part in the reductions: the loop runs on the block's first row
     int64_t base = static_cast<int64_t>(blockIdx.x) * RPB, row = base + threadIdx.x / TPR;
-    Raw<T, V> ring[D][N];
+    typename R::Slot ring[D][N];
 #pragma unroll
     for (int d = 0; d < D; ++d) {
         const int64_t r = row + d * step;
@@ -184,7 +181,8 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident<TPR, VPT>()) no
             float sum[1] = {0.0f};
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                widen(ring[d][i], v[i]);
+                if (!part.any(i)) break;
+                ring[d][i].values(R::Slot::odd(x + row * ldx), v[i]);
 #pragma unroll
                 for (int j = 0; j < V; ++j) sum[0] += v[i][j];
             }
@@ -285,6 +283,7 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
     constexpr int V = R::V, N = R::N, RPB = block_threads<TPR>() / TPR, D = (rows_ahead<T, TPR, VPT>() + 1) / 2;
     __shared__ float red[32];
     __shared__ float join[RPB > 1 ? RPB * TPR * VPT : 1];
+    wait_for_previous();
     const R part(a.cols);
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
     const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
@@ -294,7 +293,7 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
     for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) ag[i][j] = ab[i][j] = 0.0f;
-    Raw<T, V> kd[D][N], kx[SAVED ? 1 : D][N];
+    typename R::Slot kd[D][N], kx[SAVED ? 1 : D][N];
     Raw<int8_t, V> kc[SAVED ? D : 1][N];
     int ke[SAVED ? D : 1][N];
     float2 st[D];
@@ -318,11 +317,12 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
             float h[N][V], g[N][V];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
+                if (!part.any(i)) break;
                 if constexpr (SAVED) {
 #pragma unroll
                     for (int j = 0; j < V; j += 4) values4(kc[SAVED ? d : 0][i].w[j / 4], ke[SAVED ? d : 0][i], &h[i][j]);
                 } else {
-                    widen(kx[SAVED ? 0 : d][i], h[i]);
+                    kx[SAVED ? 0 : d][i].values(R::Slot::odd(x + row * ldx), h[i]);
 #pragma unroll
                     for (int j = 0; j < V; ++j) h[i][j] = __fmul_rn(__fsub_rn(h[i][j], mean), rstd);
                     if (!part.whole(i)) {
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
                         for (int j = 0; j < V; ++j) h[i][j] = part.has(i, j) ? h[i][j] : 0.0f;
                     }
                 }
-                widen(kd[d][i], g[i]);
+                kd[d][i].values(R::Slot::odd(dy + row * lddy), g[i]);
             }
             fetch(d, row + D * step);
             float sum[2] = {0.0f, 0.0f};
@@ -399,6 +399,7 @@ template <class T, class P>
 __global__ void __launch_bounds__(512) norm_wide_kernel(NormArgs a, const T* x, int64_t ldx, const P* gamma,
                                                         const P* beta, T* y, int64_t ldy, float2* stats, Saved8 s) {
     __shared__ float red[32];
+    wait_for_previous();
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -452,6 +453,7 @@ __global__ void __launch_bounds__(512) norm_wide_grad_kernel(NormArgs a, const T
                                                              int64_t ldx, Saved8 s, const float2* stats, const P* gamma,
                                                              T* dx, int64_t lddx) {
     __shared__ float red[32];
+    wait_for_previous();
     const float inv_n = __fdiv_rn(1.0f, static_cast<float>(a.cols));
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const float2 st = stats[row];
@@ -476,6 +478,7 @@ __global__ void __launch_bounds__(512) norm_wide_grad_kernel(NormArgs a, const T
 template <class T, bool SAVED>
 __global__ void __launch_bounds__(256) norm_wide_sums_kernel(NormArgs a, const T* dy, int64_t lddy, const T* x,
                                                              int64_t ldx, Saved8 s, const float2* stats, float* part) {
+    wait_for_previous();
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (c >= a.cols) return;
     float sg = 0.0f, sb = 0.0f;
@@ -494,6 +497,7 @@ __global__ void __launch_bounds__(256) norm_wide_sums_kernel(NormArgs a, const T
 template <class P>
 __global__ void __launch_bounds__(1024) norm_join_kernel(const float* part, int parts, int64_t cols, P* dgamma, P* dbeta) {
     __shared__ float sh[32][33];
+    wait_for_previous();
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // of 2 * cols
     float sum = 0.0f;
@@ -583,7 +587,7 @@ TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const 
             T* yp = static_cast<T*>(y);
             const P *gp = static_cast<const P*>(gamma), *bp = static_cast<const P*>(beta);
             if (cols > kRegisterCols) {
-                launch("layer_norm", norm_wide_kernel<T, P>, dim3(static_cast<unsigned>(std::min<int64_t>(rows, num_sms() * 4))),
+                launch_dependent("layer_norm", norm_wide_kernel<T, P>, dim3(static_cast<unsigned>(std::min<int64_t>(rows, num_sms() * 4))),
                        dim3(512), 0, as_stream(stream), a, xp, ldx, gp, bp, yp, ldy, st, s);
                 return;
             }
@@ -594,7 +598,7 @@ TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const 
                 const int64_t blocks = std::min<int64_t>(ceil_div(rows, block_threads<TPR>() / TPR),
                                                          int64_t(num_sms()) * resident<TPR, VPT>());
                 auto kern = al ? norm_kernel<T, P, true, TPR, VPT> : norm_kernel<T, P, false, TPR, VPT>;
-                launch("layer_norm", kern, dim3(static_cast<unsigned>(blocks)),
+                launch_dependent("layer_norm", kern, dim3(static_cast<unsigned>(blocks)),
                        dim3(block_threads<TPR>()), 0, as_stream(stream), a, xp, ldx, gp, bp, yp, ldy, st, s);
             });
         });
@@ -636,7 +640,7 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
             const P* gp = static_cast<const P*>(gamma);
             int64_t parts = 0;
             const auto join = [&](const float* part) {
-                launch("layer_norm_join", norm_join_kernel<P>, dim3(static_cast<unsigned>(ceil_div(2 * cols, 32))),
+                launch_dependent("layer_norm_join", norm_join_kernel<P>, dim3(static_cast<unsigned>(ceil_div(2 * cols, 32))),
                        dim3(1024), 0, str, part, static_cast<int>(parts), cols, static_cast<P*>(dgamma),
                        static_cast<P*>(dbeta));
             };
@@ -644,10 +648,10 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
                 parts = std::min<int64_t>(std::max<int64_t>(ceil_div(rows, 16), 0), 64);
                 Scratch<float> part(static_cast<size_t>(parts * 2 * cols), str);
                 auto kern = codes ? norm_wide_grad_kernel<T, P, true> : norm_wide_grad_kernel<T, P, false>;
-                launch("layer_norm_grad", kern, dim3(static_cast<unsigned>(std::min<int64_t>(rows, num_sms() * 4))),
+                launch_dependent("layer_norm_grad", kern, dim3(static_cast<unsigned>(std::min<int64_t>(rows, num_sms() * 4))),
                        dim3(512), 0, str, a, dyp, lddy, xp, ldx, s, st, gp, dxp, lddx);
                 auto sums = codes ? norm_wide_sums_kernel<T, true> : norm_wide_sums_kernel<T, false>;
-                launch("layer_norm_sums", sums,
+                launch_dependent("layer_norm_sums", sums,
                        dim3(static_cast<unsigned>(ceil_div(cols, 256)), static_cast<unsigned>(parts)), dim3(256), 0,
                        str, a, dyp, lddy, xp, ldx, s, st, part.p);
                 join(part.p);
@@ -664,7 +668,7 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
                                         : norm_grad_kernel<T, P, false, TPR, VPT, false>);
                 parts = std::min<int64_t>(ceil_div(rows, RPB), int64_t(num_sms()) * resident_grad<TPR, VPT>());
                 Scratch<float> part(static_cast<size_t>(parts * 2 * cols), str);
-                launch("layer_norm_grad", kern, dim3(static_cast<unsigned>(parts)), dim3(BT), 0, str, a, dyp, lddy, xp,
+                launch_dependent("layer_norm_grad", kern, dim3(static_cast<unsigned>(parts)), dim3(BT), 0, str, a, dyp, lddy, xp,
                        ldx, s, st, gp, dxp, lddx, part.p);
                 join(part.p);
             });

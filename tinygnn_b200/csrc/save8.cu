@@ -18,11 +18,11 @@ namespace tg {
 
 namespace {
 
-// Lane mapping of one block: G lanes, V neighbouring values each: 16 bytes of
-// aligned rows, 4 values of others.
+// Lane mapping of one block: G lanes, 16 bytes of neighbouring values each
+// (ALIGNED: one access).
 template <class T, bool ALIGNED>
 struct Lanes {
-    static constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
+    static constexpr int V = 16 / static_cast<int>(sizeof(T));
     static constexpr int G = kBlock8 / V;
     static constexpr int U = 4;  // rows in flight
     int lane, left;   // of the block's columns, `left` exist
@@ -34,17 +34,19 @@ struct Lanes {
         full = (lane + 1) * V <= left;
     }
     __device__ __forceinline__ int col(int j) const { return lane * V + j; }
-    __device__ __forceinline__ Raw<T, V> load(const T* p, bool live) const {
-        if (full && live) {
-            if constexpr (ALIGNED) return load_raw<T, V>(p + lane * V);
-            else return load4_any(p + lane * V);
-        }
-        return gather_raw<T, V>([&](int j) { return col(j) < left && live ? p[col(j)] : from_f32<T>(0.0f); });
+    // Of the row whose block starts at p.
+    __device__ __forceinline__ void load(const T* p, bool live, Held<T, V, ALIGNED>& k) const {
+        if (full && live) k.fetch(p + lane * V);
+        else if (live && lane * V < left) k.fetch(p + lane * V, left - lane * V);
+        else k.zero();
+    }
+    __device__ __forceinline__ void values(const Held<T, V, ALIGNED>& k, const T* p, float (&x)[V]) const {
+        k.values(k.odd(p + lane * V), x);
     }
     __device__ __forceinline__ void store(T* p, const float (&x)[V]) const {
         if (full) {
             if constexpr (ALIGNED) store_v<T, V>(p + lane * V, x);
-            else store4_any(p + lane * V, x);
+            else store_any<T, V>(p + lane * V, x);
             return;
         }
 #pragma unroll
@@ -99,10 +101,11 @@ struct ActArgs {
 
 // y = act(x) (y nullable), saved = x in 8 bits.  ACT: as in act_forward.
 template <class T, bool ALIGNED, int ACT>
-__global__ void __launch_bounds__(256, 3) save8_kernel(ActArgs a, const T* x, int64_t ldx, T* y,
+__global__ void __launch_bounds__(256, ALIGNED ? 3 : 2) save8_kernel(ActArgs a, const T* x, int64_t ldx, T* y,
                                                                      int64_t ldy, Saved8 o) {
     using L = Lanes<T, ALIGNED>;
     constexpr int V = L::V, U = L::U;
+    wait_for_previous();
     const Walk w = walk<L::G>(a.rows, a.nb);
     const int64_t c0 = w.b * kBlock8;
     const L l(a.cols - c0);
@@ -116,13 +119,14 @@ __global__ void __launch_bounds__(256, 3) save8_kernel(ActArgs a, const T* x, in
     uint8_t* pe = o.exps + first * o.lde + w.b;
     const int64_t dx = w.step * ldx, dy = w.step * ldy, dc = w.step * o.ld, de = w.step * o.lde;
     for (int64_t base = w.base, row = w.row0; base < a.rows; base += U * w.step, row += U * w.step) {
-        Raw<T, V> k[U];
+        Held<T, V, ALIGNED> k[U];
+        const T* at = px;
 #pragma unroll
-        for (int u = 0; u < U; ++u, px += dx) k[u] = l.load(px, row + u * w.step < a.rows);
+        for (int u = 0; u < U; ++u, px += dx) l.load(px, row + u * w.step < a.rows, k[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u, py += dy, pc += dc, pe += de) {
+        for (int u = 0; u < U; ++u, at += dx, py += dy, pc += dc, pe += de) {
             float v[V];
-            widen(k[u], v);
+            l.values(k[u], at, v);
             float m = 0.0f;
 #pragma unroll
             for (int j = 0; j < V; ++j) m = max_mag(m, v[j]);
@@ -144,6 +148,7 @@ __global__ void __launch_bounds__(256, 3) save8_kernel(ActArgs a, const T* x, in
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) restore8_kernel(ActArgs a, Saved8 s, T* y, int64_t ldy) {
     using L = Lanes<T, ALIGNED>;
+    wait_for_previous();
     const Walk w = walk<L::G>(a.rows, a.nb);
     const int64_t c0 = w.b * kBlock8;
     const L l(a.cols - c0);
@@ -156,11 +161,12 @@ __global__ void __launch_bounds__(256) restore8_kernel(ActArgs a, Saved8 s, T* y
 
 // dx = dy * act'(x), x given as it was or in 8 bits.
 template <class T, bool ALIGNED, bool SAVED, int ACT>
-__global__ void __launch_bounds__(256, 3) act_grad_kernel(ActArgs a, const T* dy, int64_t lddy,
+__global__ void __launch_bounds__(256, ALIGNED ? 3 : 2) act_grad_kernel(ActArgs a, const T* dy, int64_t lddy,
                                                                         const T* x, int64_t ldx, Saved8 s, T* dx,
                                                                         int64_t lddx) {
     using L = Lanes<T, ALIGNED>;
     constexpr int V = L::V, U = L::U;
+    wait_for_previous();
     const Walk w = walk<L::G>(a.rows, a.nb);
     const int64_t c0 = w.b * kBlock8;
     const L l(a.cols - c0);
@@ -171,31 +177,32 @@ __global__ void __launch_bounds__(256, 3) act_grad_kernel(ActArgs a, const T* dy
     T* po = dx + w.row0 * lddx + c0;
     const int64_t dg = w.step * lddy, dX = w.step * ldx, dc = w.step * s.ld, de = w.step * s.lde, dout = w.step * lddx;
     for (int64_t row = w.row0; row < a.rows; row += U * w.step) {
-        Raw<T, V> g[U], k[SAVED ? 1 : U];
+        Held<T, V, ALIGNED> g[U], k[SAVED ? 1 : U];
+        const T *at_g = pg, *at_x = px;
         Raw<int8_t, V> c[SAVED ? U : 1];
         int e[U];
 #pragma unroll
         for (int u = 0; u < U; ++u, pg += dg) {
             const bool live = row + u * w.step < a.rows;
-            g[u] = l.load(pg, live);
+            l.load(pg, live, g[u]);
             if (SAVED) {
                 c[SAVED ? u : 0] = l.load_codes(pc, live);
                 e[u] = live ? *pe : 0;
                 pc += dc;
                 pe += de;
             } else {
-                k[SAVED ? 0 : u] = l.load(px, live);
+                l.load(px, live, k[SAVED ? 0 : u]);
                 px += dX;
             }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u, po += dout) {
+        for (int u = 0; u < U; ++u, po += dout, at_g += dg, at_x += dX) {
             if (row + u * w.step >= a.rows) break;
             float v[V], d[V];
             if (SAVED) L::values(c[SAVED ? u : 0], e[u], v);
-            else widen(k[SAVED ? 0 : u], v);
+            else l.values(k[SAVED ? 0 : u], at_x, v);
             act_slope<sizeof(T) == 2, ACT>(v, a.act, a.alpha);
-            widen(g[u], d);
+            l.values(g[u], at_g, d);
 #pragma unroll
             for (int j = 0; j < V; ++j) d[j] = __fmul_rn(d[j], v[j]);
             l.store(po, d);
@@ -246,7 +253,7 @@ TG_API tg_status tg_save8(int64_t rows, int64_t cols, int32_t dtype, const void*
             auto kern = save8_kernel<T, false, -1>;
             if (al) by_act(act, [&](auto k) { kern = save8_kernel<T, true, decltype(k)::value>; });
             const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
-            launch("save8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, xp, ldx, yp,
+            launch_dependent("save8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, xp, ldx, yp,
                    ldy, o);
         });
     });
@@ -271,7 +278,7 @@ TG_API tg_status tg_restore8(int64_t rows, int64_t cols, const int8_t* codes, in
             const bool al = aligned<T>(y, ldy);
             auto kern = al ? restore8_kernel<T, true> : restore8_kernel<T, false>;
             const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
-            launch("restore8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, s,
+            launch_dependent("restore8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, s,
                    static_cast<T*>(y), ldy);
         });
     });
@@ -311,7 +318,7 @@ TG_API tg_status tg_activation_grad(int64_t rows, int64_t cols, int32_t dtype, c
                     kern = codes ? act_grad_kernel<T, true, true, A> : act_grad_kernel<T, true, false, A>;
                 });
             const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
-            launch("activation_grad", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, dyp,
+            launch_dependent("activation_grad", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, dyp,
                    lddy, xp, ldx, s, dxp, lddx);
         });
     });

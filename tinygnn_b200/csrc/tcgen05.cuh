@@ -85,20 +85,15 @@ __device__ __forceinline__ void load32(uint32_t addr, float (&v)[32]) {
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
 __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(mb::smem_u32(bar))
         : "memory");
 }
-__device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(mb::smem_u32(bar))
-        : "memory");
-}
-
 // ── CTA pairs ────────────────────────────────────────────────────────────
 // Two CTAs of a cluster multiply one tile of 256 rows (cta_group::2): each
 // holds its 128 rows of A and half of B's columns in its own shared memory

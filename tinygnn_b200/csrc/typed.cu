@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(256) typed_bias_kernel(int64_t M, int64_t N, i
     __shared__ int prefix[kMaxTypes + 1];
     __shared__ float sh[8][32 * V];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+    wait_for_previous();
     if (w == 0) scan_types(offsets, types, M, kChunk, prefix);
     __syncthreads();
     const int p = blockIdx.x;
@@ -78,6 +79,7 @@ __global__ void __launch_bounds__(256) typed_bias_join_kernel(int64_t M, int64_t
     __shared__ int prefix[kMaxTypes + 1];
     __shared__ float sh[8][33];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32, t = blockIdx.y;
+    wait_for_previous();
     if (w == 0) scan_types(offsets, t + 1, M, kChunk, prefix);
     __syncthreads();
     const int64_t n = static_cast<int64_t>(blockIdx.x) * 32 + lane;
@@ -121,10 +123,10 @@ void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T
     Scratch<float> part(static_cast<size_t>(chunks * N), s);
     const bool al = rows_aligned16(dY, lddy, sizeof(T));
     const int64_t tile = al ? 32 * (16 / static_cast<int64_t>(sizeof(T))) : 128;
-    launch("typed_linear_grad_bias", al ? typed_bias_kernel<T, true> : typed_bias_kernel<T, false>,
+    launch_dependent("typed_linear_grad_bias", al ? typed_bias_kernel<T, true> : typed_bias_kernel<T, false>,
            dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(N, tile))), dim3(256), 0, s, M, N, types,
            offsets, dY, lddy, part.p);
-    launch("typed_linear_grad_bias", typed_bias_join_kernel,
+    launch_dependent("typed_linear_grad_bias", typed_bias_join_kernel,
            dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0, s, M, N, offsets,
            part.p, db);
 }

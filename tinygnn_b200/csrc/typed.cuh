@@ -15,24 +15,33 @@ __device__ __forceinline__ int clamp_row(int r, int64_t M) {
 }
 
 // prefix[t] = number of pieces of `per` rows in the types before t (one warp).
+// The offsets of 128 types are asked for at once: a warp that went 32 at a
+// time would wait for memory four times.
 __device__ __forceinline__ void scan_types(const int32_t* offsets, int types, int64_t M, int64_t per, int* prefix) {
     const int lane = threadIdx.x & 31;
     int carry = 0;
     if (lane == 0) prefix[0] = 0;
-    for (int t0 = 0; t0 < types; t0 += 32) {
-        const int t = t0 + lane;
-        int n = 0;
-        if (t < types) {
-            const int b = clamp_row(offsets[t], M), e = clamp_row(offsets[t + 1], M);
-            n = e > b ? static_cast<int>((e - b + per - 1) / per) : 0;
+    for (int t0 = 0; t0 < types; t0 += 128) {
+        int b[4], e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = t0 + i * 32 + lane;
+            b[i] = t < types ? offsets[t] : 0;
+            e[i] = t < types ? offsets[t + 1] : 0;
         }
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, n, o);
-            if (lane >= o) n += up;
+        for (int i = 0; i < 4; ++i) {
+            if (t0 + i * 32 >= types) break;
+            const int t = t0 + i * 32 + lane, rows = clamp_row(e[i], M) - clamp_row(b[i], M);
+            int n = rows > 0 ? static_cast<int>((rows + per - 1) / per) : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, n, o);
+                if (lane >= o) n += up;
+            }
+            if (t < types) prefix[t + 1] = carry + n;
+            carry += __shfl_sync(0xffffffffu, n, 31);
         }
-        if (t < types) prefix[t + 1] = carry + n;
-        carry += __shfl_sync(0xffffffffu, n, 31);
     }
 }
 

@@ -523,6 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
         for (int64_t it; (it = item_of(local)) < items; ++local) {
             const Item m = item_at<T, OP>(g, s, it, BN);
             const int acc = local & 1;
+            if (!W) prefetch_bias<T, BN>(out, m.t, m.n0);
             bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 46);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc::fence_after();

@@ -59,6 +59,7 @@ __device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, F&& pla
         mb::fence_init();
     }
     if (warp == 2) tc::alloc(&s.tmem, tmem_cols<BN>());
+    wait_for_previous();
     if (warp == 3) plan();
     tc::fence_before();
     __syncthreads();
@@ -212,6 +213,14 @@ __device__ __forceinline__ void load_biased(uint32_t addr, const RowsOut<O>& g, 
     }
 }
 
+// Asks for a tile's bias while its products are still being summed (a warp).
+template <class O, int BN>
+__device__ __forceinline__ void prefetch_bias(const RowsOut<O>& g, int type, int64_t n0) {
+    const int64_t n = n0 + (threadIdx.x & 31) * 32;
+    if (g.bias && n < n0 + BN && n < g.N)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(g.bias + type * g.N + n));
+}
+
 // One warp's 32 rows (row0 .. row0 + rows) and BN columns (from n0) of a tile.
 // FAST: act_forward's.
 template <class O, int BN, bool FAST>
@@ -304,7 +313,7 @@ inline int tile_width(int64_t pieces, int64_t N, int widest, bool saved) {
 template <class K, class... A>
 void run(const char* name, K kern, int threads, uint32_t smem, int64_t items, cudaStream_t s, A... args) {
     TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    launch(name, kern, dim3(static_cast<unsigned>(std::min<int64_t>(items, num_sms()))), dim3(threads), smem, s,
+    launch_dependent(name, kern, dim3(static_cast<unsigned>(std::min<int64_t>(items, num_sms()))), dim3(threads), smem, s,
            args...);
 }
 

@@ -56,6 +56,7 @@ __device__ __forceinline__ uint32_t set_up_pair(PairShared& s, F&& plan) {
         mb::fence_init();
     }
     if (warp == 2) tc::alloc_pair(&s.tmem, 2 * BN);
+    wait_for_previous();
     if (warp == 3) plan();
     tc::fence_before();
     __syncthreads();
@@ -340,7 +341,7 @@ template <class K, class... A>
 void run_pairs(const char* name, K kern, int64_t items, cudaStream_t s, A... args) {
     TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(PairPlan::kBytes)));
-    launch(name, kern, dim3(pair_grid(items)), dim3(kThreads), PairPlan::kBytes, s, args...);
+    launch_dependent(name, kern, dim3(pair_grid(items)), dim3(kThreads), PairPlan::kBytes, s, args...);
 }
 
 }  // namespace

@@ -52,6 +52,10 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
     __shared__ Shared s;
     __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
+    if (threadIdx.x == 0) {
+        tc::prefetch_map(&ma);
+        tc::prefetch_map(&mw);
+    }
     const uint32_t tmem = set_up<STAGES, BN>(s, 1, [&] { scan_types(g.offsets, g.types, g.M, BM, s.prefix); });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tiles = static_cast<int64_t>(s.prefix[g.types]) * g.tiles_n;
@@ -112,6 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
             const int t = find_type(s.prefix, g.types, p);
             const int64_t row0 = clamp_row(g.offsets[t], g.M) + static_cast<int64_t>(p - s.prefix[t]) * BM + q * 32;
             const int64_t left = clamp_row(g.offsets[t + 1], g.M) - row0;
+            prefetch_bias<T, BN>(out, t, tile % g.tiles_n * BN);
             const bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 25);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc::fence_after();
@@ -272,6 +277,7 @@ template <class O>
 __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O> g) {
     __shared__ int64_t sums[8];
     __shared__ int first[8];
+    wait_for_previous();
     const int t = blockIdx.y, rows = rows_of(g.offsets, t, g.M);
     if (rows <= g.least) return;
     const auto block_sum = [&](auto x, auto* sh) {
@@ -338,6 +344,7 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O
 template <class T>
 __global__ void __launch_bounds__(256) align_kernel(int64_t rows, int64_t cols, const T* src, int64_t inner,
                                                     int64_t stride, int64_t lds, T* dst, int64_t ld) {
+    wait_for_previous();
     const int64_t vecs = ld / 8, total = rows * vecs;
     for (int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; v < total;
          v += static_cast<int64_t>(gridDim.x) * 256) {
@@ -368,7 +375,7 @@ struct Operand {
         own = static_cast<T*>(scratch_alloc(static_cast<size_t>(batch * stride) * 2, st));
         p = own;
         const int64_t want = ceil_div(batch * rows * (ld / 8), 256);
-        launch("typed_align", align_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(want, num_sms() * 8))),
+        launch_dependent("typed_align", align_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(want, num_sms() * 8))),
                dim3(256), 0, st, batch * rows, cols, src, rows, src_stride, lds, own, ld);
     }
     ~Operand() {
@@ -500,7 +507,7 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
                             piece_limit(a.M / kStep, static_cast<int>(per), w.slots), a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
                             db_joined ? a.db : nullptr};
         const int64_t want = ceil_div(a.K * std::min<int64_t>(w.ldp / 4, 256), 256);
-        launch("typed_weight_join", typed_weight_join_kernel<O>,
+        launch_dependent("typed_weight_join", typed_weight_join_kernel<O>,
                dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(1, 8 * num_sms() / a.types))),
                     static_cast<unsigned>(a.types)),
                dim3(256), 0, s, j);

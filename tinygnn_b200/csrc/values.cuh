@@ -137,46 +137,79 @@ __device__ __forceinline__ void store_v(T* p, const float (&x)[V]) {
     *reinterpret_cast<Raw<T, V>*>(p) = k;
 }
 
-// Four values at p of any alignment (of T's): 16-bit ones in whole words,
-// shifted by half a word where p is odd.  The first and the last word then
-// reach one value past the four, in words that hold one of them.
-template <class T>
-__device__ __forceinline__ Raw<T, 4> load4_any(const T* p) {
-    Raw<T, 4> k;
-    if constexpr (sizeof(T) == 4) {
+// V values as they were fetched from rows of any alignment (ALIGNED: from
+// aligned ones).  16-bit values are fetched in whole words; where p is odd they
+// start half a word in, and are shifted into place when they are widened, not
+// when they are fetched: a kernel can ask for many before it waits for one.
+template <class T, int V, bool ALIGNED>
+struct Held {
+    static constexpr bool kShift = !ALIGNED && sizeof(T) == 2;
+    uint32_t w[V * static_cast<int>(sizeof(T)) / 4 + kShift];
+
+    static __device__ __forceinline__ bool odd(const T* p) { return kShift && (reinterpret_cast<uintptr_t>(p) & 2); }
+    // All V values are there.  (The first and the last word then reach one
+    // value past the V, in words that hold one of them.)
+    __device__ __forceinline__ void fetch(const T* p) {
+        if constexpr (ALIGNED) {
+            const Raw<T, V> k = load_raw<T, V>(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k.w[j] = bits(p[j]);
-    } else {
-        const uintptr_t u = reinterpret_cast<uintptr_t>(p);
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(u & ~uintptr_t(3));
-        const uint32_t a = q[0], b = q[1];
-        if (u & 2) {
-            const uint32_t c = q[2];
-            k.w[0] = __byte_perm(a, b, 0x5432);
-            k.w[1] = __byte_perm(b, c, 0x5432);
+            for (int j = 0; j < Raw<T, V>::N; ++j) w[j] = k.w[j];
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = bits(p[j]);
         } else {
-            k.w[0] = a;
-            k.w[1] = b;
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) w[j] = q[j];
+            w[V / 2] = odd(p) ? q[V / 2] : 0u;
         }
     }
-    return k;
-}
-template <class T>
-__device__ __forceinline__ void store4_any(T* p, const float (&x)[4]) {
-    Raw<T, 4> k;
+    // The first n values are there; zeros after them.
+    __device__ __forceinline__ void fetch(const T* p, int n) {
+        const int shift = odd(p);
+#pragma unroll
+        for (int j = 0; j < V * static_cast<int>(sizeof(T)) / 4 + kShift; ++j) {
+            if constexpr (sizeof(T) == 4) {
+                w[j] = j < n ? bits(p[j]) : 0u;
+            } else {
+                const int e = 2 * j - shift;
+                w[j] = (e >= 0 && e < n ? bits(p[e]) : 0u) | (e + 1 < n ? bits(p[e + 1]) : 0u) << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < V * static_cast<int>(sizeof(T)) / 4 + kShift; ++j) w[j] = 0u;
+    }
+    // odd: of the pointer they were fetched from.
+    __device__ __forceinline__ void values(bool odd, float* x) const {
+        Raw<T, V> k;
+#pragma unroll
+        for (int j = 0; j < Raw<T, V>::N; ++j) {
+            if constexpr (kShift) k.w[j] = odd ? __byte_perm(w[j], w[j + 1], 0x5432) : w[j];
+            else k.w[j] = w[j];
+        }
+        widen(k, x);
+    }
+};
+// V values to p of any alignment (of T's).
+template <class T, int V>
+__device__ __forceinline__ void store_any(T* p, const float (&x)[V]) {
+    Raw<T, V> k;
     narrow(x, k);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = x[j];
+        for (int j = 0; j < V; ++j) p[j] = x[j];
     } else if (reinterpret_cast<uintptr_t>(p) & 2) {
         uint16_t* q = reinterpret_cast<uint16_t*>(p);
         q[0] = static_cast<uint16_t>(k.w[0]);
-        *reinterpret_cast<uint32_t*>(q + 1) = __byte_perm(k.w[0], k.w[1], 0x5432);
-        q[3] = static_cast<uint16_t>(k.w[1] >> 16);
+#pragma unroll
+        for (int j = 0; j + 1 < V / 2; ++j)
+            *reinterpret_cast<uint32_t*>(q + 1 + 2 * j) = __byte_perm(k.w[j], k.w[j + 1], 0x5432);
+        q[V - 1] = static_cast<uint16_t>(k.w[V / 2 - 1] >> 16);
     } else {
-        uint32_t* q = reinterpret_cast<uint32_t*>(p);
-        q[0] = k.w[0];
-        q[1] = k.w[1];
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) reinterpret_cast<uint32_t*>(p)[j] = k.w[j];
     }
 }
 
