@@ -229,6 +229,13 @@ template <class T, class O>
 void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s);
 int typed_any_take_error();
 
+// At most kFewRows rows (typed_few.cu).
+constexpr int64_t kFewRows = 16;
+template <class T, bool TRANS>
+void typed_rows_few(const RowsArgs<T>& a, cudaStream_t s);
+template <class T, class O>
+void typed_weight_few(const WeightArgs<T, O>& a, cudaStream_t s);
+
 // db alone (typed.cu).
 template <class T>
 void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T* dY, int64_t lddy, float* db,

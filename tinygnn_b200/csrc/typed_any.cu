@@ -311,19 +311,6 @@ __device__ __forceinline__ Source<T> source_b(const AnyArgs<T>& g, const Item& m
     return {w + m.n0 * g.ldb + k, g.ldb, clip(g.N - m.n0, BN), clip(g.K - k, tc::kInner)};
 }
 
-// dW and db of a type without rows, by n threads.
-template <class T>
-__device__ void zero_type(const AnyArgs<T>& g, const RowsOut<T>& out, int t, int e, int n) {
-    for (int64_t k = 0; k < g.K; ++k)
-        for (int64_t c = e; c < g.N; c += n) {
-            const int64_t at = t * g.stride_c + k * out.ldc + c;
-            if (sizeof(T) == 2 && g.out_f32) reinterpret_cast<float*>(out.C)[at] = 0.0f;
-            else out.C[at] = from_f32<T>(0.0f);
-        }
-    if (g.db)
-        for (int64_t c = e; c < g.N; c += n) g.db[t * g.N + c] = 0.0f;
-}
-
 // SAVED: the first operand in 8 bits.  TMA: the second by TMA (map mb).
 template <class T, int OP, int BN, bool SAVED, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_constant__ CUtensorMap map_b,
@@ -552,12 +539,15 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
             mb::arrive(&s.acc_empty[acc]);
         }
         if constexpr (W) {
-            // types without rows: zero
             const int e = threadIdx.x - 384;
-            for (int t = blockIdx.x; t < g.types; t += gridDim.x) {
-                if (rows_of(g.offsets, t, g.M) > 0) continue;
-                zero_type(g, out, t, e, 128);
-            }
+            if (sizeof(T) == 2 && g.out_f32)
+                zero_empty_types(g.offsets, g.types, g.M, g.K, g.N, reinterpret_cast<float*>(out.C), out.ldc, g.stride_c,
+                                 out.mode, e, 128);
+            else zero_empty_types(g.offsets, g.types, g.M, g.K, g.N, out.C, out.ldc, g.stride_c, out.mode, e, 128);
+            if (g.db)
+                for (int t = blockIdx.x; t < g.types; t += gridDim.x)
+                    if (rows_of(g.offsets, t, g.M) == 0)
+                        for (int64_t n = e; n < g.N; n += 128) g.db[t * g.N + n] = 0.0f;
         }
     }
     tear_down<BN>(s, tmem, 8);

@@ -177,6 +177,26 @@ __device__ __forceinline__ void store_rows(O* p, int64_t ld, int rows, int64_t l
     }
 }
 
+// dW of the types without rows is zero: every CTA's threads (id < n) write
+// their share of all of them.
+template <class O>
+__device__ __forceinline__ void zero_empty_types(const int32_t* offsets, int types, int64_t M, int64_t K, int64_t N,
+                                                 O* dW, int64_t ld, int64_t stride, int mode, int id, int n) {
+    for (int t = 0; t < types; ++t) {
+        if (rows_of(offsets, t, M) > 0) continue;
+        for (int64_t k = blockIdx.x; k < K; k += gridDim.x) {
+            O* row = dW + t * stride + k * ld;
+            constexpr int W = 16 / static_cast<int>(sizeof(O));
+            int64_t c = 0;
+            if (mode > 0) {
+                c = N / W * W;
+                for (int64_t i = id * W; i < c; i += n * W) *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
+            }
+            for (int64_t i = c + id; i < N; i += n) row[i] = from_f32<O>(0.0f);
+        }
+    }
+}
+
 // ── epilogue of the rows products ────────────────────────────────────────
 template <class O>
 struct RowsOut {

@@ -321,13 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) tc::arrive_at(freed);
         }
-        // types without rows: zero
-        for (int t = blockIdx.x; t < g.types; t += gridDim.x) {
-            if (rows_of(g.offsets, t, g.M) > 0) continue;
-            for (int64_t k = 0; k < g.K; ++k)
-                for (int64_t n = threadIdx.x - 128; n < g.N; n += 256)
-                    g.dW[t * g.stride_dw + k * g.lddw + n] = from_f32<O>(0.0f);
-        }
+        zero_empty_types(g.offsets, g.types, g.M, g.K, g.N, g.dW, g.lddw, g.stride_dw, g.mode, threadIdx.x - 128, 256);
     }
     tear_down_pair(s, tmem, rank);
 }

@@ -249,13 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
             tc::fence_before();
             mb::arrive(&s.acc_empty[acc]);
         }
-        // types without rows: zero
-        for (int t = blockIdx.x; t < g.types; t += gridDim.x) {
-            if (rows_of(g.offsets, t, g.M) > 0) continue;
-            for (int64_t k = 0; k < g.K; ++k)
-                for (int64_t n = threadIdx.x - 128; n < g.N; n += 256)
-                    g.dW[t * g.stride_dw + k * g.lddw + n] = from_f32<O>(0.0f);
-        }
+        zero_empty_types(g.offsets, g.types, g.M, g.K, g.N, g.dW, g.lddw, g.stride_dw, g.mode, threadIdx.x - 128, 256);
     }
     tear_down<BN>(s, tmem, 1);
 }
@@ -448,6 +442,10 @@ constexpr double kLargeFlops = 1e10;
 
 template <class T, bool TRANS>
 void typed_rows(const RowsArgs<T>& a, cudaStream_t s) {
+    if (a.M <= kFewRows) {
+        typed_rows_few<T, TRANS>(a, s);
+        return;
+    }
     if constexpr (sizeof(T) == 2) {
         const bool readable = Operand<T>::readable(1, a.A, a.lda, 0) &&
                               Operand<T>::readable(a.types, a.W, a.ldw, a.stride_w);
@@ -461,10 +459,8 @@ void typed_rows(const RowsArgs<T>& a, cudaStream_t s) {
 
 template <class T, class O>
 void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
-    if (a.M == 0) {
-        for (int t = 0; t < a.types; ++t)
-            TG_CUDA(cudaMemset2DAsync(a.dW + t * a.stride_dw, a.lddw * sizeof(O), 0, a.N * sizeof(O), a.K, s));
-        if (a.db) TG_CUDA(cudaMemsetAsync(a.db, 0, static_cast<size_t>(a.types * a.N) * 4, s));
+    if (a.M <= kFewRows) {  // none among them: dW and db are zero
+        typed_weight_few<T, O>(a, s);
         return;
     }
     const bool saved = a.saved.codes != nullptr;
