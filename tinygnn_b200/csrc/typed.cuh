@@ -110,10 +110,12 @@ __device__ __forceinline__ int rows_of(const int32_t* offsets, int t, int64_t M)
     const int b = clamp_row(offsets[t], M), e = clamp_row(offsets[t + 1], M);
     return e > b ? e - b : 0;
 }
-// Rows of the longest piece, from the sum of all types' steps.
-__host__ __device__ __forceinline__ int64_t piece_limit(int64_t steps, int per, int slots) {
+// Rows of the longest piece, from the sum of all types' steps.  `longest`: the
+// steps that a sum may take (kernels that cannot add up parts of it themselves,
+// where the result is fp32).
+__host__ __device__ __forceinline__ int64_t piece_limit(int64_t steps, int per, int slots, int longest) {
     const int64_t share = (steps * per * 5 + slots * 4 - 1) / (slots * 4);
-    return (share < 2 ? 2 : share) * kStep;
+    return (share < 2 ? 2 : (share < longest ? share : longest)) * kStep;
 }
 __device__ __forceinline__ int piece_count(int n, int64_t limit) { return static_cast<int>((n + limit - 1) / limit); }
 // Rows of each piece (the last may have fewer; none is empty, since this is at most `limit`).
@@ -127,13 +129,13 @@ __device__ __forceinline__ bool piece_before(int types, int rows_u, int u, int r
 
 // One warp: order[i] = the i-th type, prefix[i] = the pieces before it.
 __device__ __forceinline__ void plan_pieces(const int32_t* offsets, int types, int64_t M, int per, int slots,
-                                            int* prefix, uint16_t* order) {
+                                            int longest, int* prefix, uint16_t* order) {
     const int lane = threadIdx.x & 31;
     int64_t steps = 0;
     for (int t = lane; t < types; t += 32) steps += (rows_of(offsets, t, M) + kStep - 1) / kStep;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, o);
-    const int64_t limit = piece_limit(steps, per, slots);
+    const int64_t limit = piece_limit(steps, per, slots, longest);
     if (types > kSortTypes) {
         for (int t = lane; t < types; t += 32) order[t] = static_cast<uint16_t>(t);
     } else {
@@ -193,7 +195,7 @@ __device__ __forceinline__ int64_t dealt(int64_t r, int64_t cta, int64_t ctas) {
 
 struct WeightPlan {
     int BN;  // columns of a tile
-    int tiles_k, tiles_n, slots;
+    int tiles_k, tiles_n, slots, longest;
     int64_t ldp, items;
     float *part, *db_part;
     bool pairs;      // on CTA pairs (tiles of 256 x 256)

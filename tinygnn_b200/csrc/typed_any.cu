@@ -8,8 +8,10 @@
 //   fp32       each value split into three bf16 parts (24 bits, exactly):
 //              x0 = x's upper half, x1 = bf16(x - x0), x2 = bf16(x - x0 - x1);
 //              a product is the six part products x_i y_j with i + j <= 2
-//              (what is left out is below 2^-23 of it and of random sign).  An
-//              infinity in an fp32 operand gives NaN;
+//              (what is left out is below 2^-23 of it and of random sign), in
+//              parts of 768 inner indexes that are added up in fp32, rounded
+//              to nearest (see stage_mmas).  An infinity in an fp32 operand
+//              gives NaN;
 //   bf16, fp16 with rows of any alignment;
 //   8 bits     code * 2^e as one bf16 or fp16 value, exactly;
 //  and rows past a type's end and columns past the matrix are zeros.  Where
@@ -66,20 +68,14 @@ struct Source {
 // How an operand's rows are aligned.
 enum Align { kElement, kPair, kVector };  // to one value, two values, 16 bytes
 
-// Eight values at p, of which the first `n` exist.
+// 16 bytes of values at p, of which the first `n` values exist.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, int n, uint32_t* w) {
-    if (n >= 8) {
+__device__ __forceinline__ void load16(const T* p, int n, uint32_t* w) {
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    const Raw<T, V> k = n >= V ? load_raw<T, V>(p)
+                               : gather_raw<T, V>([&](int j) { return j < n ? p[j] : from_f32<T>(0.0f); });
 #pragma unroll
-        for (int j = 0; j < 2 * static_cast<int>(sizeof(T)); j += 4) {
-            const uint4 q = *(reinterpret_cast<const uint4*>(p) + j / 4);
-            w[j] = q.x, w[j + 1] = q.y, w[j + 2] = q.z, w[j + 3] = q.w;
-        }
-        return;
-    }
-    const Raw<T, 8> k = gather_raw<T, 8>([&](int j) { return j < n ? p[j] : from_f32<T>(0.0f); });
-#pragma unroll
-    for (int j = 0; j < Raw<T, 8>::N; ++j) w[j] = k.w[j];
+    for (int j = 0; j < 4; ++j) w[j] = k.w[j];
 }
 // Two values at p.
 template <class T>
@@ -128,16 +124,17 @@ __device__ __forceinline__ void split3(const uint32_t* w, uint32_t (&parts)[3][N
 #pragma unroll
     for (int j = 0; j < N / 2; ++j) parts[2][j] = h.w[j];
 }
-// Eight values into one plane (16-bit types) or three (fp32), `plane` bytes apart.
+// 16 bytes of values into one plane (16-bit types: 16 bytes of it) or three
+// (fp32: 8 bytes of each), `plane` bytes apart.
 template <class T>
-__device__ __forceinline__ void put8(uint8_t* at, uint32_t plane, const uint32_t* w) {
+__device__ __forceinline__ void put16(uint8_t* at, uint32_t plane, const uint32_t* w) {
     if constexpr (sizeof(T) == 2) {
         store_chunk(at, {w[0], w[1], w[2], w[3]});
     } else {
-        uint32_t k[3][4];
-        split3<8>(w, k);
+        uint32_t k[3][2];
+        split3<4>(w, k);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) store_chunk(at + q * plane, k[q]);
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(at + q * plane) = make_uint2(k[q][0], k[q][1]);
     }
 }
 template <class T>
@@ -159,43 +156,44 @@ __device__ __forceinline__ float value_of(const uint32_t* w, int j) {
     return to_f32(v[j % 2]);
 }
 
-// The part of a tile of ROWS memory rows x CHUNKS 8-value chunks that one of
-// THREADS loader threads moves.  Rows 16-byte aligned: one chunk of every
-// STEP-th row.  Others: a warp takes 64 columns of a row at a time, two
-// neighbouring ones a lane, so that its loads cover whole lines whatever the
-// alignment (a lane that read its own eight values of 4 bytes would touch each
-// line eight times); halves of 128 columns belong to warps of one parity, so
-// a lane keeps its columns.
-template <int ROWS, int CHUNKS, int THREADS>
+// The part of a tile of ROWS memory rows x COLS columns that one of THREADS
+// loader threads moves.  Rows 16-byte aligned: VAL neighbouring columns (16
+// bytes; 8 of an 8-bit copy) of every STEP-th row.  Others: a warp takes 64
+// columns of a row at a time, two neighbouring ones a lane, so that its loads
+// cover whole lines whatever the alignment (a lane that read its own eight
+// values of 4 bytes would touch each line eight times); halves of 128 columns
+// belong to warps of one parity, so a lane keeps its columns.
+template <int ROWS, int COLS, int THREADS, int VAL>
 struct Part {
-    static constexpr int STEP = THREADS / CHUNKS, N = ROWS / STEP;
-    static constexpr int HALVES = CHUNKS / 8, WARPS = THREADS / 32, PAIRS = ROWS * HALVES / WARPS;
-    static constexpr int PAIR_STEP = WARPS / HALVES;
-    static_assert(PAIRS == 4 * N && 8 % PAIR_STEP == 0, "both forms hold as many values");
+    static constexpr int LANES = COLS / VAL, STEP = THREADS / LANES, N = ROWS / STEP;
+    static constexpr int HALVES = COLS / 64, WARPS = THREADS / 32, PAIRS = ROWS * HALVES / WARPS;
+    static constexpr int PAIR_STEP = WARPS / HALVES, kVal = VAL;
+    static_assert(2 * PAIRS == VAL * N && 8 % PAIR_STEP == 0, "both forms hold as many values");
     static __device__ __forceinline__ constexpr int rows() { return ROWS; }
-    static __device__ __forceinline__ constexpr int cols() { return CHUNKS * 8; }
-    static __device__ __forceinline__ int chunk() { return threadIdx.x % CHUNKS; }
-    static __device__ __forceinline__ int row(int i) { return threadIdx.x % THREADS / CHUNKS + i * STEP; }
+    static __device__ __forceinline__ constexpr int cols() { return COLS; }
+    static __device__ __forceinline__ int col() { return threadIdx.x % LANES * VAL; }
+    static __device__ __forceinline__ int row(int i) { return threadIdx.x % THREADS / LANES + i * STEP; }
     static __device__ __forceinline__ int warp() { return threadIdx.x % THREADS / 32; }
     static __device__ __forceinline__ int pair_col() { return warp() % HALVES * 64 + threadIdx.x % 32 * 2; }
     static __device__ __forceinline__ int pair_row(int i) { return warp() / HALVES + i * PAIR_STEP; }
 };
+// Words that one thread's values take.
 template <class P, class T>
-constexpr int words() { return P::N * 2 * static_cast<int>(sizeof(T)); }
+constexpr int words() { return P::N * P::kVal * static_cast<int>(sizeof(T)) / 4; }
 
 template <class P, class T>
 __device__ __forceinline__ void fetch_tile(const Source<T>& s, int align, uint32_t (&w)[words<P, T>()]) {
     const bool whole = s.rows >= P::rows() && s.cols >= P::cols();  // the same for all threads
     if (align == kVector) {
-        const T* p = s.p + P::row(0) * s.ld + P::chunk() * 8;
+        const T* p = s.p + P::row(0) * s.ld + P::col();
         const int64_t step = P::STEP * s.ld;
         if (whole) {
 #pragma unroll
-            for (int i = 0; i < P::N; ++i, p += step) load8(p, 8, w + i * 2 * sizeof(T));
+            for (int i = 0; i < P::N; ++i, p += step) load16(p, P::kVal, w + i * 4);
         } else {
-            const int n = s.cols - P::chunk() * 8;
+            const int n = s.cols - P::col();
 #pragma unroll
-            for (int i = 0; i < P::N; ++i, p += step) load8(p, P::row(i) < s.rows ? n : 0, w + i * 2 * sizeof(T));
+            for (int i = 0; i < P::N; ++i, p += step) load16(p, P::row(i) < s.rows ? n : 0, w + i * 4);
         }
     } else {
         const T* p = s.p + P::pair_row(0) * s.ld + P::pair_col();
@@ -219,14 +217,14 @@ __device__ __forceinline__ void put_tile(uint8_t* tile, uint32_t plane, int alig
                                          const uint32_t (&w)[words<P, T>()], bool add, float (&sum)[8]) {
     if (align == kVector) {
         static_assert(P::STEP % 8 == 0, "whole swizzle periods");
-        uint8_t* at = tile + chunk_at(P::row(0), P::chunk());
+        uint8_t* at = tile + chunk_at(P::row(0), P::col() / 8) + P::col() % 8 * 2;
 #pragma unroll
-        for (int i = 0; i < P::N; ++i) put8<T>(at + i * P::STEP * 128, plane, w + i * 2 * sizeof(T));
+        for (int i = 0; i < P::N; ++i) put16<T>(at + i * P::STEP * 128, plane, w + i * 4);
         if (add) {
 #pragma unroll
             for (int i = 0; i < P::N; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sum[j] += value_of<T>(w + i * 2 * sizeof(T), j);
+                for (int j = 0; j < P::kVal; ++j) sum[j] += value_of<T>(w + i * 4, j);
         }
     } else {
         constexpr int PERIOD = 8 / P::PAIR_STEP;
@@ -249,7 +247,7 @@ __device__ __forceinline__ void put_tile(uint8_t* tile, uint32_t plane, int alig
 template <class P>
 __device__ __forceinline__ void fetch_tile8(const Saved8& s, int64_t row0, int64_t col0, int rows, int cols,
                                             Raw<int8_t, 8> (&k)[P::N], int (&e)[P::N]) {
-    const int c = P::chunk() * 8;
+    const int c = P::col();
 #pragma unroll
     for (int i = 0; i < P::N; ++i) {
         const bool live = P::row(i) < rows && c < cols;
@@ -319,7 +317,10 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
     constexpr int PA = SAVED ? 1 : Half<T>::planes, PB = Half<T>::planes;
     using S = Plan<PA, PB, BN>;
     constexpr int STAGES = S::kStages;
-    constexpr bool W = OP == kGradWeight, A_OUTER = W, B_OUTER = OP != kGradInput;
+    constexpr bool W = OP == kGradWeight, A_OUTER = W, B_OUTER = OP != kGradInput, SPLIT = PB > 1;
+    // Steps that one accumulator takes; sums of more are added up in the output.
+    const int part = SPLIT ? 12 : (W && g.out_f32 ? 32 : 1 << 30);
+    constexpr int ACC = SPLIT ? 2 * BN : BN;  // TMEM columns of a buffer
     static_assert(!TMA || (W && PB == 1), "TMA takes 16-bit dY");
     constexpr uint32_t ID = tc::idesc(is_bf16<H>(), A_OUTER, B_OUTER, BM, BN);
     // 16-bit values: the loaders are two groups that take the stages in turn
@@ -327,8 +328,9 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
     // flight while the other's arrive (fp32 values would need twice the
     // registers, and take six times as long to multiply).
     constexpr int GROUPS = TMA ? 4 : (sizeof(T) == 2 ? 2 : 1), THREADS = kLoaders / GROUPS;
-    using PartA = Part<A_OUTER ? 64 : BM, A_OUTER ? BM / 8 : 8, THREADS>;
-    using PartB = Part<B_OUTER ? 64 : BN, B_OUTER ? BN / 8 : 8, TMA ? kLoaders : THREADS>;
+    constexpr int VAL = 16 / static_cast<int>(sizeof(T));
+    using PartA = Part<A_OUTER ? 64 : BM, A_OUTER ? BM : 64, THREADS, SAVED ? 8 : VAL>;
+    using PartB = Part<B_OUTER ? 64 : BN, B_OUTER ? BN : 64, TMA ? kLoaders : THREADS, VAL>;
 
     extern __shared__ uint8_t raw[];
     __shared__ Shared s;
@@ -336,8 +338,8 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
     __shared__ float db_rows[W && !TMA ? kLoaders * 8 : 1];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
     uint8_t* const ring_p = raw + (ring - mb::smem_u32(raw));
-    const uint32_t tmem = set_up<STAGES, BN>(s, 8 / GROUPS + (TMA ? 1 : 0), [&] {
-        if (W) plan_pieces(g.offsets, g.types, g.M, g.tiles_m * g.tiles_n, g.slots, s.prefix, s.order);
+    const uint32_t tmem = set_up<STAGES, BN, SPLIT>(s, 8 / GROUPS + (TMA ? 1 : 0), [&] {
+        if (W) plan_pieces(g.offsets, g.types, g.M, g.tiles_m * g.tiles_n, g.slots, 1 << 30, s.prefix, s.order);
         else scan_types(g.offsets, g.types, g.M, BM, s.prefix);
     });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                         values4(k8[u].w[1], e8[u], x + 4);
                         Raw<H, 8> h;
                         narrow(x, h);
-                        store_chunk(a + chunk_at(PartA::row(u), PartA::chunk()), h.w);
+                        store_chunk(a + chunk_at(PartA::row(u), PartA::col() / 8), h.w);
                     }
                 } else {
                     put_tile<PartA, T>(a, S::kA, g.a_align, ka, false, sum);
@@ -427,10 +429,11 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                 if (sums) {  // the same for every loader thread
                     // threads that share a column, as rows of db_rows
                     const bool vec = g.b_align == kVector;
-                    const int G = vec ? kLoaders / (BN / 8) : 8 / PartB::HALVES;
+                    const int G = vec ? kLoaders / PartB::LANES : 8 / PartB::HALVES;
                     if (vec) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) db_rows[threadIdx.x / (BN / 8) * BN + PartB::chunk() * 8 + j] = sum[j];
+                        for (int j = 0; j < VAL; ++j)
+                            db_rows[threadIdx.x / PartB::LANES * BN + PartB::col() + j] = sum[j];
                     } else {
                         float* r = db_rows + threadIdx.x / 32 / PartB::HALVES * BN + PartB::pair_col();
                         r[0] = sum[0];
@@ -451,15 +454,17 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
     } else if (warp == 8) {
         // ── MMA issuer ──
         int64_t i = 0;
-        int local = 0;
+        int local = 0;  // accumulators filled
         bool ok = true;
-        for (int64_t it; (it = item_of(local)) < items && ok; ++local) {
+        for (int64_t round = 0, it; (it = item_of(round)) < items && ok; ++round) {
             const Item m = item_at<T, OP>(g, s, it, BN);
-            const int acc = local & 1;
-            if (local >= 2) ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 42);
-            if (!(ok = __all_sync(0xffffffffu, ok))) break;
-            tc::fence_after();
             for (int k = 0; k < m.steps; ++k, ++i) {
+                const int acc = local & 1;
+                if (k % part == 0) {
+                    if (local >= 2) ok = mb::wait(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 42);
+                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                    tc::fence_after();
+                }
                 const int st = static_cast<int>(i % STAGES);
                 ok = mb::wait(&s.full[st], (i / STAGES) & 1, &g_error, 43);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -470,14 +475,16 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                     const int64_t valid = m.r1 - m.r0 - static_cast<int64_t>(k) * tc::kInner;
                     if (valid < tc::kInner) zero_rows(ring + st * S::kStage + PA * S::kA, S::kB, static_cast<int>(valid));
                 }
+                const bool done = k + 1 == m.steps || (k + 1) % part == 0;
                 if (lane == 0) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the loaders' writes -> MMA reads
-                    stage_mmas<PA, PB, BN, A_OUTER, B_OUTER>(ring + st * S::kStage, tmem + acc * BN, ID, k == 0);
+                    stage_mmas<PA, PB, BN, A_OUTER, B_OUTER>(ring + st * S::kStage, tmem + acc * ACC, ID, k % part == 0);
                     tc::commit(&s.empty[st]);
+                    if (done) tc::commit(&s.acc_full[acc]);
                 }
+                local += done;
                 __syncwarp();
             }
-            if (ok && lane == 0) tc::commit(&s.acc_full[acc]);
         }
     } else if (warp == 9) {
         // ── TMA of dY ──
@@ -507,36 +514,42 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
         T* buf = reinterpret_cast<T*>(stage_out[q]);
         float* buf32 = stage_out[q];
         int local = 0;
-        for (int64_t it; (it = item_of(local)) < items; ++local) {
+        bool ok = true;
+        for (int64_t round = 0, it; (it = item_of(round)) < items && ok; ++round) {
             const Item m = item_at<T, OP>(g, s, it, BN);
-            const int acc = local & 1;
             if (!W) prefetch_bias<T, BN>(out, m.t, m.n0);
-            bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 46);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            tc::fence_after();
-            const uint32_t addr = tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
             const int64_t r = m.m0 + q * 32;
-            if constexpr (!W) {
-                finish_rows<T, BN, sizeof(T) == 2>(addr, out, m.t, r, clip(m.r1 - r, 32), m.n0, buf);
-            } else {
-                const int rows = clip(g.K - r, 32);
+            for (int k = 0; k < m.steps; k += part, ++local) {
+                const bool first = k == 0, last = k + part >= m.steps;
+                const int acc = local & 1;
+                ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 46);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                tc::fence_after();
+                const uint32_t addr = tmem + acc * ACC + (static_cast<uint32_t>(q * 32) << 16);
+                if constexpr (!W) {
+                    finish_rows<T, BN, sizeof(T) == 2, SPLIT>(addr, out, m.t, r, clip(m.r1 - r, 32), m.n0, buf, first,
+                                                              last);
+                } else {
+                    const int rows = clip(g.K - r, 32);
 #pragma unroll 1
-                for (int c0 = 0; c0 < BN && m.n0 + c0 < g.N; c0 += 32) {
-                    float v[32];
-                    tc::load32(addr + c0, v);
-                    const int64_t n = m.n0 + c0, left = g.N - n;
-                    if (!m.whole) {
-                        store_rows(g.part + (m.p * g.K + r) * g.ldp + n, g.ldp, rows, g.ldp - n, v, 2, buf32);
-                    } else if (sizeof(T) == 2 && g.out_f32) {
-                        store_rows(reinterpret_cast<float*>(out.C) + m.t * g.stride_c + r * out.ldc + n, out.ldc, rows,
-                                   left, v, out.mode, buf32);
-                    } else {
-                        store_rows(out.C + m.t * g.stride_c + r * out.ldc + n, out.ldc, rows, left, v, out.mode, buf);
+                    for (int c0 = 0; c0 < BN && m.n0 + c0 < g.N; c0 += 32) {
+                        float v[32];
+                        load_acc<BN, SPLIT>(addr + c0, v);
+                        const int64_t n = m.n0 + c0, left = g.N - n;
+                        if (!m.whole) {
+                            store_rows(g.part + (m.p * g.K + r) * g.ldp + n, g.ldp, rows, g.ldp - n, v, 2, buf32, !first);
+                        } else if (sizeof(T) == 2 && g.out_f32) {
+                            store_rows(reinterpret_cast<float*>(out.C) + m.t * g.stride_c + r * out.ldc + n, out.ldc,
+                                       rows, left, v, out.mode, buf32, !first);
+                        } else {
+                            store_rows(out.C + m.t * g.stride_c + r * out.ldc + n, out.ldc, rows, left, v, out.mode, buf,
+                                       !first);
+                        }
                     }
                 }
+                tc::fence_before();
+                mb::arrive(&s.acc_empty[acc]);
             }
-            tc::fence_before();
-            mb::arrive(&s.acc_empty[acc]);
         }
         if constexpr (W) {
             const int e = threadIdx.x - 384;
@@ -550,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                         for (int64_t n = e; n < g.N; n += 128) g.db[t * g.N + n] = 0.0f;
         }
     }
-    tear_down<BN>(s, tmem, 8);
+    tear_down<BN, SPLIT>(s, tmem, 8);
 }
 
 template <class T>

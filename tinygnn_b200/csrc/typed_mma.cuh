@@ -38,12 +38,13 @@ struct Shared {
     uint16_t order[kMaxTypes];  // weight gradients only
 };
 
-template <int BN>
-constexpr uint32_t tmem_cols() { return 2 * BN < 64 ? 64 : 2 * BN; }
+// TMEM columns: two buffers of an accumulator (SPLIT: of two, see stage_mmas).
+template <int BN, bool SPLIT = false>
+constexpr uint32_t tmem_cols() { return 2 * BN * (SPLIT ? 2 : 1); }
 
 // Barriers, TMEM (warp 2) and the plan of the work (warp 3: plan(), over the
 // types' offsets); every thread returns with them in place.
-template <int STAGES, int BN, class F>
+template <int STAGES, int BN, bool SPLIT = false, class F>
 __device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, F&& plan) {
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
@@ -58,7 +59,7 @@ __device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, F&& pla
         mb::init(&s.drain, 1);
         mb::fence_init();
     }
-    if (warp == 2) tc::alloc(&s.tmem, tmem_cols<BN>());
+    if (warp == 2) tc::alloc(&s.tmem, tmem_cols<BN, SPLIT>());
     wait_for_previous();
     if (warp == 3) plan();
     tc::fence_before();
@@ -69,7 +70,7 @@ __device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, F&& pla
 
 // Every copy has landed; once every MMA of the issuing warp has retired, TMEM
 // goes back.
-template <int BN>
+template <int BN, bool SPLIT = false>
 __device__ __forceinline__ void tear_down(Shared& s, uint32_t tmem, int mma_warp) {
     tc::fence_before();
     __syncthreads();
@@ -80,7 +81,7 @@ __device__ __forceinline__ void tear_down(Shared& s, uint32_t tmem, int mma_warp
     }
     __syncthreads();
     tc::fence_after();
-    if (warp == 2) tc::dealloc(tmem, tmem_cols<BN>());
+    if (warp == 2) tc::dealloc(tmem, tmem_cols<BN, SPLIT>());
 }
 
 // One warp: rows [valid, 64) of the 64-row chunks in `bytes` of shared memory
@@ -94,13 +95,19 @@ __device__ __forceinline__ void zero_rows(uint32_t base, uint32_t bytes, int val
     __syncwarp();
 }
 
-// The MMAs of one stage: every plane product i + j <= 2, smallest first.
+// The MMAs of one stage: every plane product i + j <= 2.  An MMA truncates as
+// it adds to the accumulator: about 2^-25 of it is lost each time, always
+// towards zero.  So with several planes the products x_0 y_0 have an
+// accumulator of their own and all the small ones another (BN columns on),
+// where the same loss is 2^-8 as large; one accumulator for all six was ten
+// times less exact (4e-6 of the result for 602 inner indexes).
 template <int PA, int PB, int BN, bool A_OUTER, bool B_OUTER>
 __device__ __forceinline__ void stage_mmas(uint32_t stage, uint32_t acc, uint32_t id, bool first) {
     using S = Plan<PA, PB, BN>;
     bool add = !first;
 #pragma unroll
-    for (int order = PA + PB - 2 < 2 ? PA + PB - 2 : 2; order >= 0; --order)
+    for (int order = PA + PB - 2 < 2 ? PA + PB - 2 : 2; order >= 0; --order) {
+        if (order == 0) add = !first;
 #pragma unroll
         for (int i = PA - 1; i >= 0; --i) {
             const int j = order - i;
@@ -108,11 +115,24 @@ __device__ __forceinline__ void stage_mmas(uint32_t stage, uint32_t acc, uint32_
             const uint32_t a = stage + i * S::kA, b = stage + PA * S::kA + j * S::kB;
 #pragma unroll
             for (int s = 0; s < tc::kInner / 16; ++s) {
-                tc::mma(acc, A_OUTER ? tc::desc_outer(a, s) : tc::desc_inner(a, s),
+                tc::mma(acc + (order > 0 ? BN : 0), A_OUTER ? tc::desc_outer(a, s) : tc::desc_inner(a, s),
                         B_OUTER ? tc::desc_outer(b, s) : tc::desc_inner(b, s), id, add);
                 add = true;
             }
         }
+    }
+}
+
+// 32 columns of an accumulator (SPLIT: of the two).
+template <int BN, bool SPLIT>
+__device__ __forceinline__ void load_acc(uint32_t addr, float (&v)[32]) {
+    tc::load32(addr, v);
+    if constexpr (SPLIT) {
+        float u[32];
+        tc::load32(addr + BN, u);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], u[j]);
+    }
 }
 
 // How an output's rows are aligned: 2 = 32 bytes, 1 = 16 bytes, 0 = neither
@@ -135,14 +155,30 @@ constexpr int stage_bytes() { return 32 * stage_row<O>() * static_cast<int>(size
 // lane stores its own, 32 bytes (whole sectors) or 16 at a time.  Others:
 // through `buf`, so that a warp's store covers 32 neighbouring columns of one
 // row (lane-per-row stores would send one sector for every 2 or 4 bytes).
+// add (fp32 only): on top of what this warp stored there before.
 template <class O>
-__device__ __forceinline__ void store_rows(O* p, int64_t ld, int rows, int64_t left, const float (&v)[32], int mode,
-                                           O* buf) {
+__device__ __forceinline__ void store_rows(O* p, int64_t ld, int rows, int64_t left, float (&v)[32], int mode, O* buf,
+                                           bool add = false) {
     constexpr int W = 32 / sizeof(O);  // values per 32 bytes
     const int lane = threadIdx.x & 31;
     if (mode != 0) {
         if (lane >= rows) return;
         p += lane * ld;
+        if constexpr (sizeof(O) == 4) {
+            if (add) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    if (mode > 0 && c + 4 <= left) {
+                        const float4 q = *reinterpret_cast<const float4*>(p + c);
+                        v[c] += q.x, v[c + 1] += q.y, v[c + 2] += q.z, v[c + 3] += q.w;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (c + j < left) v[c + j] += p[c + j];
+                    }
+                }
+            }
+        }
 #pragma unroll
         for (int c = 0; c < 32; c += W) {
             if (mode > 0 && c + W <= left) {
@@ -172,6 +208,13 @@ __device__ __forceinline__ void store_rows(O* p, int64_t ld, int rows, int64_t l
     for (int j = 0; j < 32; ++j) buf[lane * S + j] = from_f32<O>(v[j]);
     __syncwarp();
     if (lane < left) {
+        if constexpr (sizeof(O) == 4) {
+            if (add) {
+#pragma unroll 8
+                for (int r = 0; r < rows; ++r) p[r * ld + lane] += buf[r * S + lane];
+                return;
+            }
+        }
 #pragma unroll 8
         for (int r = 0; r < rows; ++r) p[r * ld + lane] = buf[r * S + lane];
     }
@@ -211,10 +254,19 @@ struct RowsOut {
     Range8 r8;
 };
 
-// 32 accumulator columns from n (bias added; columns past N are zero).
-template <class O>
-__device__ __forceinline__ void load_biased(uint32_t addr, const RowsOut<O>& g, int type, int64_t n, float (&v)[32]) {
-    tc::load32(addr, v);
+// 32 accumulator columns from n, and what `before` (this lane's row of C, if
+// not null) holds of the sum so far; bias added; columns past N are zero.
+template <class O, int BN, bool SPLIT>
+__device__ __forceinline__ void load_biased(uint32_t addr, const RowsOut<O>& g, int type, int64_t n, const O* before,
+                                            float (&v)[32]) {
+    load_acc<BN, SPLIT>(addr, v);
+    if constexpr (SPLIT) {
+        if (before) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (n + j < g.N) v[j] = __fadd_rn(v[j], before[n + j]);
+        }
+    }
     if (!g.bias) return;
     const float* b = g.bias + type * g.N + n;
     if (n + 32 <= g.N && g.N % 4 == 0 && reinterpret_cast<uintptr_t>(g.bias) % 16 == 0) {
@@ -242,13 +294,28 @@ __device__ __forceinline__ void prefetch_bias(const RowsOut<O>& g, int type, int
 }
 
 // One warp's 32 rows (row0 .. row0 + rows) and BN columns (from n0) of a tile.
-// FAST: act_forward's.
-template <class O, int BN, bool FAST>
+// FAST: act_forward's.  SPLIT (fp32): the accumulators hold part of the inner
+// indexes; parts but the last (`last` false) only add to C, and `first` tells
+// that C holds nothing yet.
+template <class O, int BN, bool FAST, bool SPLIT = false>
 __device__ __forceinline__ void finish_rows(uint32_t addr, const RowsOut<O>& g, int type, int64_t row0, int rows,
-                                            int64_t n0, O* buf) {
+                                            int64_t n0, O* buf, bool first = true, bool last = true) {
     const int lane = threadIdx.x & 31;
     const bool live = lane < rows;
     const int64_t row = live ? row0 + lane : 0;
+    if constexpr (SPLIT) {
+        if (!last) {
+#pragma unroll 1
+            for (int c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 32) {
+                float v[32];
+                load_acc<BN, SPLIT>(addr + c0, v);
+                store_rows(g.C + row0 * g.ldc + n0 + c0, g.ldc, rows, g.N - n0 - c0, v, g.mode, buf, !first);
+            }
+            return;
+        }
+        __syncwarp();  // C's rows may have been stored by other lanes
+    }
+    const O* before = SPLIT && !first && live ? g.C + row * g.ldc : nullptr;
     constexpr int W = BN < kBlock8 ? BN : kBlock8;
 #pragma unroll 1
     for (int b0 = 0; b0 < BN && n0 + b0 < g.N; b0 += kBlock8) {
@@ -261,7 +328,7 @@ __device__ __forceinline__ void finish_rows(uint32_t addr, const RowsOut<O>& g, 
 #pragma unroll 1
             for (int c0 = b0; c0 < b0 + W; c0 += 32) {
                 float v[32];
-                load_biased(addr + c0, g, type, n0 + c0, v);
+                load_biased<O, BN, SPLIT>(addr + c0, g, type, n0 + c0, before, v);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) m = max_mag(m, v[j]);
             }
@@ -274,7 +341,7 @@ __device__ __forceinline__ void finish_rows(uint32_t addr, const RowsOut<O>& g, 
             const int64_t left = g.N - n0 - c0;
             if (left <= 0) break;
             float v[32];
-            load_biased(addr + c0, g, type, n0 + c0, v);
+            load_biased<O, BN, SPLIT>(addr + c0, g, type, n0 + c0, before, v);
             if (g.saved.codes && live) {
                 int8_t* o = g.saved.codes + row * g.saved.ld + n0 + c0;
 #pragma unroll

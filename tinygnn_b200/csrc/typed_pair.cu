@@ -191,7 +191,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 template <class O>
 struct WeightPair {
     int64_t M, K, N;
-    int types, tiles_k, tiles_n, slots;
+    int types, tiles_k, tiles_n, slots, longest;
     const int32_t* offsets;
     O* dW;
     int64_t lddw, stride_dw;
@@ -212,7 +212,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t rank = tc::cluster_rank();
     const int per = g.tiles_k * g.tiles_n;
     const uint32_t tmem = set_up_pair(s, [&] {
-        plan_pieces(g.offsets, g.types, g.M, per, g.slots, s.prefix, s.order);
+        plan_pieces(g.offsets, g.types, g.M, per, g.slots, g.longest, s.prefix, s.order);
     });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t items = static_cast<int64_t>(s.prefix[g.types]) * per;
@@ -354,7 +354,7 @@ template <class T, class O>
 void typed_weight_pair(const WeightArgs<T, O>& a, const WeightPlan& w, const TmaMatrix<T>& X, const TmaMatrix<T>& Y,
                        cudaStream_t s) {
     const CUtensorMap mx = tma_map(X, 1, a.M, a.K, 64), my = tma_map(Y, 1, a.M, a.N, 64);
-    const WeightPair<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, a.offsets, a.dW, a.lddw, a.stride_dw,
+    const WeightPair<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, w.longest, a.offsets, a.dW, a.lddw, a.stride_dw,
                           store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O)), w.part, w.ldp};
     run_pairs("typed_weight_pair", typed_weight_pair_kernel<T, O>, w.items, s, mx, my, g);
 }

@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
 template <class O>
 struct WeightTc {
     int64_t M, K, N;
-    int types, tiles_k, tiles_n, slots;
+    int types, tiles_k, tiles_n, slots, longest;
     const int32_t* offsets;
     O* dW;
     int64_t lddw, stride_dw;
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
     __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
     const uint32_t tmem = set_up<STAGES, BN>(s, 1, [&] {
-        plan_pieces(g.offsets, g.types, g.M, g.tiles_k * g.tiles_n, g.slots, s.prefix, s.order);
+        plan_pieces(g.offsets, g.types, g.M, g.tiles_k * g.tiles_n, g.slots, g.longest, s.prefix, s.order);
     });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = g.tiles_k * g.tiles_n;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
 template <class O>
 struct JoinArgs {
     int64_t M, K, N, ldp;
-    int types, per, slots;
+    int types, per, slots, longest;
     int64_t least;  // no type of fewer rows is cut (the limit when no step is ragged)
     const int32_t* offsets;
     const float *part, *db_part;
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O
     };
     int64_t steps = 0;
     for (int u = threadIdx.x; u < g.types; u += 256) steps += (rows_of(g.offsets, u, g.M) + kStep - 1) / kStep;
-    const int64_t limit = piece_limit(block_sum(steps, sums), g.per, g.slots);
+    const int64_t limit = piece_limit(block_sum(steps, sums), g.per, g.slots, g.longest);
     const int n = piece_count(rows, limit);
     if (n <= 1) return;  // the weight kernel wrote it
     // this type's first piece
@@ -421,7 +421,7 @@ void typed_weight_tma(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream
         return;
     }
     const CUtensorMap mx = tma_map(X.matrix(), 1, a.M, a.K, 64), my = tma_map(Y.matrix(), 1, a.M, a.N, 64);
-    const WeightTc<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, a.offsets, a.dW, a.lddw, a.stride_dw,
+    const WeightTc<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, w.longest, a.offsets, a.dW, a.lddw, a.stride_dw,
                         store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O)), w.part, w.ldp};
     const auto go = [&](auto bn) {
         constexpr int BN = decltype(bn)::value;
@@ -477,11 +477,14 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     w.slots = w.pairs ? num_sms() / 2 : num_sms();
     // A type is cut where it has more than an SM's share: at most slots / per
     // pieces and one a type.
-    const int64_t used = std::min<int64_t>(a.types, a.M), pieces = w.slots / per + used;
+    const bool by_tma = large && !saved;
+    w.longest = by_tma && sizeof(O) == 4 ? 64 : 1 << 30;
+    const int64_t used = std::min<int64_t>(a.types, a.M);
+    const int64_t pieces = std::max<int64_t>(w.slots / per, a.M / (int64_t(w.longest) * kStep)) + used;
     w.items = std::max<int64_t>(pieces * per, std::min(a.types, num_sms()));
     w.ldp = (a.N + 7) / 8 * 8;
     // None is, if even all the rows in one type are an SM's share or two steps.
-    const bool joined = a.M > 2 * kStep && per < w.slots;
+    const bool joined = a.M > 2 * kStep && (per < w.slots || a.M > int64_t(w.longest) * kStep);
     Scratch<float> part(joined ? static_cast<size_t>(pieces * (a.K * w.ldp + a.N)) : 1, s);
     w.part = part.p;
     w.db_part = part.p + (joined ? pieces * a.K * w.ldp : 0);
@@ -499,8 +502,8 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
         typed_weight_any<T, O>(a, w, s);
     }
     if (joined) {
-        const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots,
-                            piece_limit(a.M / kStep, static_cast<int>(per), w.slots), a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
+        const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots, w.longest,
+                            piece_limit(a.M / kStep, static_cast<int>(per), w.slots, w.longest), a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
                             db_joined ? a.db : nullptr};
         const int64_t want = ceil_div(a.K * std::min<int64_t>(w.ldp / 4, 256), 256);
         launch_dependent("typed_weight_join", typed_weight_join_kernel<O>,
