@@ -122,7 +122,7 @@ constexpr int block_threads() { return TPR < 128 ? 128 : TPR; }
 
 // Blocks a SM: the kernels are compiled and launched for as many.
 template <int TPR, int VPT>
-constexpr int resident() { return TPR >= 256 ? 1024 / TPR : (VPT > 8 ? 5 : 8); }
+constexpr int resident() { return VPT > 16 ? 512 / block_threads<TPR>() : (TPR >= 256 ? 1024 / TPR : (VPT > 8 ? 5 : 8)); }
 template <int TPR, int VPT>
 constexpr int resident_grad() { return TPR >= 256 ? 512 / TPR : (VPT > 8 ? 4 : 5); }
 
@@ -532,6 +532,18 @@ void by_width(int64_t cols, F&& f) {
     else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
 }
 
+// The forward pass holds half as much a value: twice the values a thread, half
+// the warps that a row's sums have to cross.
+template <class F>
+void by_width_forward(int64_t cols, F&& f) {
+    using std::integral_constant;
+    if (cols <= 512) by_width(cols, f);
+    else if (cols <= 1024) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (cols <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
+    else if (cols <= 4096) f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
+    else f(integral_constant<int, 256>{}, integral_constant<int, 32>{});
+}
+
 // gamma and beta are fp32 or of the rows' own type.
 template <class F>
 void by_types(int dtype, int param_dtype, F&& f) {
@@ -593,7 +605,7 @@ TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const 
             }
             const bool al = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(y, ldy, sizeof(T)) &&
                             rows_aligned16(gamma, 0, 1) && rows_aligned16(beta, 0, 1);
-            by_width(cols, [&](auto tpr, auto vpt) {
+            by_width_forward(cols, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
                 const int64_t blocks = std::min<int64_t>(ceil_div(rows, block_threads<TPR>() / TPR),
                                                          int64_t(num_sms()) * resident<TPR, VPT>());

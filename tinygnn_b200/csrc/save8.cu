@@ -152,10 +152,25 @@ __global__ void __launch_bounds__(256) restore8_kernel(ActArgs a, Saved8 s, T* y
     const Walk w = walk<L::G>(a.rows, a.nb);
     const int64_t c0 = w.b * kBlock8;
     const L l(a.cols - c0);
-    for (int64_t row = w.row0; row < a.rows; row += w.step) {
-        float v[L::V];
-        L::values(l.load_codes(s.codes + row * s.ld + c0, true), s.exps[row * s.lde + w.b], v);
-        l.store(y + row * ldy + c0, v);
+    constexpr int U = L::U;
+    for (int64_t row = w.row0; row < a.rows; row += U * w.step) {
+        Raw<int8_t, L::V> c[U];
+        int e[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = row + u * w.step;
+            const bool live = r < a.rows;
+            c[u] = l.load_codes(s.codes + (live ? r : row) * s.ld + c0, live);
+            e[u] = live ? s.exps[r * s.lde + w.b] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = row + u * w.step;
+            if (r >= a.rows) break;
+            float v[L::V];
+            L::values(c[u], e[u], v);
+            l.store(y + r * ldy + c0, v);
+        }
     }
 }
 
@@ -225,6 +240,18 @@ bool aligned(const void* p, int64_t ld) {
 
 }  // namespace
 
+template <class T>
+void restore8(int64_t rows, int64_t cols, const Saved8& s, T* y, int64_t ldy, cudaStream_t stream) {
+    const ActArgs a{rows, cols, ceil_div(cols, kBlock8), TG_ACT_NONE, 0.0f, Range8{}};
+    const bool al = aligned<T>(y, ldy);
+    const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
+    launch_dependent("restore8", al ? restore8_kernel<T, true> : restore8_kernel<T, false>,
+                     dim3(grid_for(rows, a.nb, G)), dim3(256), 0, stream, a, s, y, ldy);
+}
+template void restore8<float>(int64_t, int64_t, const Saved8&, float*, int64_t, cudaStream_t);
+template void restore8<__nv_bfloat16>(int64_t, int64_t, const Saved8&, __nv_bfloat16*, int64_t, cudaStream_t);
+template void restore8<__half>(int64_t, int64_t, const Saved8&, __half*, int64_t, cudaStream_t);
+
 }  // namespace tg
 
 extern "C" {
@@ -272,14 +299,9 @@ TG_API tg_status tg_restore8(int64_t rows, int64_t cols, const int8_t* codes, in
         check_ld(fn, "y", ldy, cols);
         const Saved8 s{const_cast<int8_t*>(codes), ld_codes, const_cast<uint8_t*>(exponents), ld_exponents};
         check_saved8(fn, cols, s, rows > 0);
-        const ActArgs a{rows, cols, ceil_div(cols, kBlock8), TG_ACT_NONE, 0.0f, range8(dtype)};
         by_dtype(dtype, [&](auto t) {
             using T = decltype(t);
-            const bool al = aligned<T>(y, ldy);
-            auto kern = al ? restore8_kernel<T, true> : restore8_kernel<T, false>;
-            const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
-            launch_dependent("restore8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, s,
-                   static_cast<T*>(y), ldy);
+            restore8<T>(rows, cols, s, static_cast<T*>(y), ldy, as_stream(stream));
         });
     });
 }

@@ -198,8 +198,7 @@ struct WeightPlan {
     int tiles_k, tiles_n, slots, longest;
     int64_t ldp, items;
     float *part, *db_part;
-    bool pairs;      // on CTA pairs (tiles of 256 x 256)
-    bool dy_by_tma;  // typed_weight_any: dY by TMA, db not summed on the way
+    bool pairs;  // on CTA pairs (tiles of 256 x 256)
 };
 
 // TMA-fed kernels and the choice between them and the others (typed_tc.cu).

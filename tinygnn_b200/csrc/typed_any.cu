@@ -20,7 +20,6 @@
 //    warps 0-7    loaders: the next stage's values are in registers (in
 //                 flight) while this stage's are converted and written;
 //    warp 8       the MMAs (one thread);
-//    warp 9       TMA for the second operand, where its rows are aligned;
 //    warps 12-15  the epilogue of one of two TMEM accumulators while the next
 //                 tile is multiplied.
 // ============================================================================
@@ -309,10 +308,9 @@ __device__ __forceinline__ Source<T> source_b(const AnyArgs<T>& g, const Item& m
     return {w + m.n0 * g.ldb + k, g.ldb, clip(g.N - m.n0, BN), clip(g.K - k, tc::kInner)};
 }
 
-// SAVED: the first operand in 8 bits.  TMA: the second by TMA (map mb).
-template <class T, int OP, int BN, bool SAVED, bool TMA>
-__global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_constant__ CUtensorMap map_b,
-                                                                const AnyArgs<T> g, const RowsOut<T> out) {
+// SAVED: the first operand in 8 bits.
+template <class T, int OP, int BN, bool SAVED>
+__global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T> g, const RowsOut<T> out) {
     using H = typename Half<T>::type;
     constexpr int PA = SAVED ? 1 : Half<T>::planes, PB = Half<T>::planes;
     using S = Plan<PA, PB, BN>;
@@ -321,24 +319,23 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
     // Steps that one accumulator takes; sums of more are added up in the output.
     const int part = SPLIT ? 12 : (W && g.out_f32 ? 32 : 1 << 30);
     constexpr int ACC = SPLIT ? 2 * BN : BN;  // TMEM columns of a buffer
-    static_assert(!TMA || (W && PB == 1), "TMA takes 16-bit dY");
     constexpr uint32_t ID = tc::idesc(is_bf16<H>(), A_OUTER, B_OUTER, BM, BN);
-    // 16-bit values: the loaders are two groups that take the stages in turn
-    // (four for 8-bit copies and dY by TMA), so that one group's loads are in
-    // flight while the other's arrive (fp32 values would need twice the
-    // registers, and take six times as long to multiply).
-    constexpr int GROUPS = TMA ? 4 : (sizeof(T) == 2 ? 2 : 1), THREADS = kLoaders / GROUPS;
+    // 16-bit values: the loaders are two groups that take the stages in turn, so
+    // that one group's loads are in flight while the other's arrive (fp32
+    // values would need twice the registers, and take six times as long to
+    // multiply).
+    constexpr int GROUPS = sizeof(T) == 2 ? 2 : 1, THREADS = kLoaders / GROUPS;
     constexpr int VAL = 16 / static_cast<int>(sizeof(T));
     using PartA = Part<A_OUTER ? 64 : BM, A_OUTER ? BM : 64, THREADS, SAVED ? 8 : VAL>;
-    using PartB = Part<B_OUTER ? 64 : BN, B_OUTER ? BN : 64, TMA ? kLoaders : THREADS, VAL>;
+    using PartB = Part<B_OUTER ? 64 : BN, B_OUTER ? BN : 64, THREADS, VAL>;
 
     extern __shared__ uint8_t raw[];
     __shared__ Shared s;
     __shared__ float stage_out[4][(stage_bytes<float>() + 3) / 4];
-    __shared__ float db_rows[W && !TMA ? kLoaders * 8 : 1];
+    __shared__ float db_rows[W ? kLoaders * 8 : 1];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
     uint8_t* const ring_p = raw + (ring - mb::smem_u32(raw));
-    const uint32_t tmem = set_up<STAGES, BN, SPLIT>(s, 8 / GROUPS + (TMA ? 1 : 0), [&] {
+    const uint32_t tmem = set_up<STAGES, BN, SPLIT>(s, 8 / GROUPS, [&] {
         if (W) plan_pieces(g.offsets, g.types, g.M, g.tiles_m * g.tiles_n, g.slots, 1 << 30, s.prefix, s.order);
         else scan_types(g.offsets, g.types, g.M, BM, s.prefix);
     });
@@ -367,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
             }
         };
         const auto fetch_b = [&](const Item& m, int step) {
-            if constexpr (!TMA) fetch_tile<PartB, T>(source_b<T, OP>(g, m, step, BN), g.b_align, kb);
+            fetch_tile<PartB, T>(source_b<T, OP>(g, m, step, BN), g.b_align, kb);
         };
         const int group = threadIdx.x / THREADS;
         // This group's first step of an item whose first stage is number i0.
@@ -377,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
         float sum[8];
         bool fetched = false;  // the registers hold the next step's values
         while (it < items && ok) {
-            const bool sums = W && !TMA && g.db != nullptr && m.m0 == 0;
+            const bool sums = W && g.db != nullptr && m.m0 == 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
             it = item_of(++round);
@@ -415,17 +412,15 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                     put_tile<PartA, T>(a, S::kA, g.a_align, ka, false, sum);
                 }
                 if (fetched) fetch_a(then, after);
-                if constexpr (!TMA) {
-                    put_tile<PartB, T>(a + PA * S::kA, S::kB, g.b_align, kb, sums, sum);
-                    if (fetched) fetch_b(then, after);
-                }
+                put_tile<PartB, T>(a + PA * S::kA, S::kB, g.b_align, kb, sums, sum);
+                if (fetched) fetch_b(then, after);
                 // (the MMA's thread passes the writes on to the tensor cores: a
                 // proxy fence here would wait for the loads just issued)
                 __syncwarp();
                 if (lane == 0) mb::arrive(&s.full[st]);
             }
             i += m.steps;
-            if constexpr (W && !TMA) {
+            if constexpr (W) {
                 if (sums) {  // the same for every loader thread
                     // threads that share a column, as rows of db_rows
                     const bool vec = g.b_align == kVector;
@@ -469,12 +464,6 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                 ok = mb::wait(&s.full[st], (i / STAGES) & 1, &g_error, 43);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 tc::fence_after();
-                if constexpr (TMA) {
-                    // Rows of dY past the piece: the loaders' zeros would meet another type's values there, and
-                    // 0 x NaN is not 0.
-                    const int64_t valid = m.r1 - m.r0 - static_cast<int64_t>(k) * tc::kInner;
-                    if (valid < tc::kInner) zero_rows(ring + st * S::kStage + PA * S::kA, S::kB, static_cast<int>(valid));
-                }
                 const bool done = k + 1 == m.steps || (k + 1) % part == 0;
                 if (lane == 0) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the loaders' writes -> MMA reads
@@ -485,28 +474,6 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const __grid_con
                 local += done;
                 __syncwarp();
             }
-        }
-    } else if (warp == 9) {
-        // ── TMA of dY ──
-        if (TMA && lane == 0) {
-            int64_t i = 0;
-            bool ok = true;
-            for (int64_t round = 0, it; (it = item_of(round)) < items && ok; ++round) {
-                const Item m = item_at<T, OP>(g, s, it, BN);
-                for (int k = 0; k < m.steps; ++k, ++i) {
-                    const int st = static_cast<int>(i % STAGES);
-                    if (i >= STAGES && !(ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_error, 44))) break;
-                    mb::arrive_expect_tx(&s.full[st], S::kB);
-#pragma unroll
-                    for (int c = 0; c < BN / 64; ++c)
-                        tc::tma3(ring + st * S::kStage + PA * S::kA + c * tc::kChunkBytes, &map_b,
-                                 static_cast<int>(m.n0) + c * 64, static_cast<int>(m.r0) + k * tc::kInner, 0,
-                                 &s.full[st]);
-                }
-            }
-            // every copy issued must have landed before the CTA may exit
-            for (int64_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
-                mb::wait(&s.full[j % STAGES], (j / STAGES) & 1, &g_error, 45);
         }
     } else if (warp >= 12) {
         // ── epilogue ──
@@ -572,11 +539,11 @@ int alignment(const T* p, int64_t ld) {
     return b % 16 == 0 ? kVector : (b % (2 * sizeof(T)) == 0 ? kPair : kElement);
 }
 
-template <class T, int OP, int BN, bool SAVED, bool TMA>
-void go(const CUtensorMap& map, const AnyArgs<T>& g, const RowsOut<T>& out, int64_t items, cudaStream_t s) {
+template <class T, int OP, int BN, bool SAVED>
+void go(const AnyArgs<T>& g, const RowsOut<T>& out, int64_t items, cudaStream_t s) {
     constexpr int PA = SAVED ? 1 : Half<T>::planes;
-    run("typed_any", typed_any_kernel<T, OP, BN, SAVED, TMA>, kThreads, Plan<PA, Half<T>::planes, BN>::kBytes, items,
-        s, map, g, out);
+    run("typed_any", typed_any_kernel<T, OP, BN, SAVED>, kThreads, Plan<PA, Half<T>::planes, BN>::kBytes, items, s, g,
+        out);
 }
 
 }  // namespace
@@ -594,9 +561,8 @@ void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s) {
     const int BN = tile_width(pieces, a.N, 128, a.saved.codes != nullptr);
     g.tiles_m = 1;
     g.tiles_n = static_cast<int>(ceil_div(a.N, BN));
-    const CUtensorMap none{};
-    if (BN == 64) go<T, OP, 64, false, false>(none, g, out, pieces * g.tiles_n, s);
-    else go<T, OP, 128, false, false>(none, g, out, pieces * g.tiles_n, s);
+    if (BN == 64) go<T, OP, 64, false>(g, out, pieces * g.tiles_n, s);
+    else go<T, OP, 128, false>(g, out, pieces * g.tiles_n, s);
 }
 
 template <class T, class O>
@@ -615,27 +581,14 @@ void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream
     out.C = reinterpret_cast<T*>(a.dW);
     out.ldc = a.lddw;
     out.mode = store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O));
+    g.db = a.db, g.db_part = w.db_part;
     const auto by_source = [&](auto bn) {
         constexpr int BN = decltype(bn)::value;
-        if constexpr (sizeof(T) == 2) {
-            if (w.dy_by_tma) {
-                const int64_t dims[3] = {a.N, a.M, 1}, strides[2] = {a.lddy, std::max<int64_t>(a.M * a.lddy, 8)};
-                const int box[3] = {64, 64, 1};
-                const CUtensorMap map = tc::map16<3>(a.dY, is_bf16<T>(), dims, strides, box);
-                go<T, kGradWeight, BN, true, true>(map, g, out, w.items, s);
-                return;
-            }
-        }
-        if constexpr (BN <= 128) {
-            g.db = a.db, g.db_part = w.db_part;
-            const CUtensorMap none{};
-            if (saved) go<T, kGradWeight, BN, true, false>(none, g, out, w.items, s);
-            else go<T, kGradWeight, BN, false, false>(none, g, out, w.items, s);
-        }
+        if (saved) go<T, kGradWeight, BN, true>(g, out, w.items, s);
+        else go<T, kGradWeight, BN, false>(g, out, w.items, s);
     };
     if (w.BN == 64) by_source(std::integral_constant<int, 64>{});
-    else if (w.BN == 128) by_source(std::integral_constant<int, 128>{});
-    else if constexpr (sizeof(T) == 2) by_source(std::integral_constant<int, 256>{});
+    else by_source(std::integral_constant<int, 128>{});
 }
 
 #define TG_TYPED_ANY(T)                                                   \

@@ -372,6 +372,21 @@ struct Operand {
         launch_dependent("typed_align", align_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(want, num_sms() * 8))),
                dim3(256), 0, st, batch * rows, cols, src, rows, src_stride, lds, own, ld);
     }
+    // A weight gradient's first operand.
+    template <class O>
+    Operand(const WeightArgs<T, O>& a, cudaStream_t st) : s(st) {
+        if (!a.saved.codes) {
+            Operand x(1, a.M, a.K, a.X, a.ldx, 0, st);
+            p = x.p, ld = x.ld, stride = x.stride, own = x.own;
+            x.own = nullptr;
+            return;
+        }
+        ld = (a.K + 7) / 8 * 8;
+        stride = a.M * ld;
+        own = static_cast<T*>(scratch_alloc(static_cast<size_t>(stride) * 2, st));
+        p = own;
+        restore8<T>(a.M, a.K, a.saved, own, ld, st);
+    }
     ~Operand() {
         if (own) scratch_free(own, s);
     }
@@ -415,7 +430,10 @@ void typed_rows_tma(const RowsArgs<T>& a, cudaStream_t s) {
 
 template <class T, class O>
 void typed_weight_tma(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s) {
-    const Operand<T> X(1, a.M, a.K, a.X, a.ldx, 0, s), Y(1, a.M, a.N, a.dY, a.lddy, 0, s);
+    // X in 8 bits: its values as a 16-bit matrix, exactly (33 us for 65,536 x
+    // 1,024 at HBM rate; a kernel whose loaders decoded the codes into shared
+    // memory for every tile of columns took 193 us where pairs take 126).
+    const Operand<T> X(a, s), Y(1, a.M, a.N, a.dY, a.lddy, 0, s);
     if (w.pairs) {
         typed_weight_pair<T, O>(a, w, X.matrix(), Y.matrix(), s);
         return;
@@ -463,22 +481,18 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
         typed_weight_few<T, O>(a, s);
         return;
     }
-    const bool saved = a.saved.codes != nullptr;
     const bool large = sizeof(T) == 2 && 2.0 * a.M * a.K * a.N > kLargeFlops;
     WeightPlan w{};
     const int widest = large ? 256 : 128;
     w.BN = a.N <= 64 ? 64 : (a.N <= 128 || widest == 128 ? 128 : 256);
-    w.dy_by_tma = saved && large && rows_aligned16(a.dY, a.lddy, sizeof(T));
-    if (saved && !w.dy_by_tma) w.BN = std::min(w.BN, 128);
-    w.pairs = large && !saved && a.K > 128 && a.N > 128;
+    w.pairs = large && a.K > 128 && a.N > 128;
     w.tiles_k = static_cast<int>(ceil_div(a.K, w.pairs ? 2 * BM : BM));
     w.tiles_n = static_cast<int>(ceil_div(a.N, w.BN));
     const int64_t per = int64_t(w.tiles_k) * w.tiles_n;
     w.slots = w.pairs ? num_sms() / 2 : num_sms();
     // A type is cut where it has more than an SM's share: at most slots / per
     // pieces and one a type.
-    const bool by_tma = large && !saved;
-    w.longest = by_tma && sizeof(O) == 4 ? 64 : 1 << 30;
+    w.longest = large && sizeof(O) == 4 ? 64 : 1 << 30;
     const int64_t used = std::min<int64_t>(a.types, a.M);
     const int64_t pieces = std::max<int64_t>(w.slots / per, a.M / (int64_t(w.longest) * kStep)) + used;
     w.items = std::max<int64_t>(pieces * per, std::min(a.types, num_sms()));
@@ -488,23 +502,19 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     Scratch<float> part(joined ? static_cast<size_t>(pieces * (a.K * w.ldp + a.N)) : 1, s);
     w.part = part.p;
     w.db_part = part.p + (joined ? pieces * a.K * w.ldp : 0);
-    bool db_joined = a.db != nullptr;
+    bool done = false;
     if constexpr (sizeof(T) == 2) {
-        if ((large && !saved) || w.dy_by_tma) {
-            db_joined = false;
+        if (large) {
             if (a.db) typed_bias<T>(a.M, a.N, a.types, a.offsets, a.dY, a.lddy, a.db, s);
-            if (saved) typed_weight_any<T, O>(a, w, s);
-            else typed_weight_tma<T, O>(a, w, s);
-        } else {
-            typed_weight_any<T, O>(a, w, s);
+            typed_weight_tma<T, O>(a, w, s);
+            done = true;
         }
-    } else {
-        typed_weight_any<T, O>(a, w, s);
     }
+    if (!done) typed_weight_any<T, O>(a, w, s);
     if (joined) {
         const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots, w.longest,
                             piece_limit(a.M / kStep, static_cast<int>(per), w.slots, w.longest), a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
-                            db_joined ? a.db : nullptr};
+                            large ? nullptr : a.db};
         const int64_t want = ceil_div(a.K * std::min<int64_t>(w.ldp / 4, 256), 256);
         launch_dependent("typed_weight_join", typed_weight_join_kernel<O>,
                dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(1, 8 * num_sms() / a.types))),

@@ -335,6 +335,10 @@ struct Saved8 {
     int64_t lde;
 };
 
+// y = the values of a saved matrix (save8.cu).
+template <class T>
+void restore8(int64_t rows, int64_t cols, const Saved8& s, T* y, int64_t ldy, cudaStream_t stream);
+
 // ── Activations and their slopes ─────────────────────────────────────────
 // The choice is made once for V values.  GELU's 1/2 (1 + tanh u) is computed
 // as 1 / (1 + e^-2u), which equals it, does not cancel where tanh u is near
