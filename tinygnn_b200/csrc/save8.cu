@@ -24,7 +24,8 @@ template <class T, bool ALIGNED>
 struct Lanes {
     static constexpr int V = 16 / static_cast<int>(sizeof(T));
     static constexpr int G = kBlock8 / V;
-    static constexpr int U = 4;  // rows in flight
+    static constexpr int U = ALIGNED ? 4 : 2;  // rows in flight
+    static constexpr int kResident = ALIGNED ? 3 : 4;  // blocks of 256 threads a SM
     int lane, left;   // of the block's columns, `left` exist
     bool full;        // the lane's values are all there
 
@@ -101,7 +102,7 @@ struct ActArgs {
 
 // y = act(x) (y nullable), saved = x in 8 bits.  ACT: as in act_forward.
 template <class T, bool ALIGNED, int ACT>
-__global__ void __launch_bounds__(256, ALIGNED ? 3 : 2) save8_kernel(ActArgs a, const T* x, int64_t ldx, T* y,
+__global__ void __launch_bounds__(256, Lanes<T, ALIGNED>::kResident) save8_kernel(ActArgs a, const T* x, int64_t ldx, T* y,
                                                                      int64_t ldy, Saved8 o) {
     using L = Lanes<T, ALIGNED>;
     constexpr int V = L::V, U = L::U;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(256) restore8_kernel(ActArgs a, Saved8 s, T* y
 
 // dx = dy * act'(x), x given as it was or in 8 bits.
 template <class T, bool ALIGNED, bool SAVED, int ACT>
-__global__ void __launch_bounds__(256, ALIGNED ? 3 : 2) act_grad_kernel(ActArgs a, const T* dy, int64_t lddy,
+__global__ void __launch_bounds__(256, Lanes<T, ALIGNED>::kResident) act_grad_kernel(ActArgs a, const T* dy, int64_t lddy,
                                                                         const T* x, int64_t ldx, Saved8 s, T* dx,
                                                                         int64_t lddx) {
     using L = Lanes<T, ALIGNED>;
@@ -225,11 +226,14 @@ __global__ void __launch_bounds__(256, ALIGNED ? 3 : 2) act_grad_kernel(ActArgs 
     }
 }
 
-// Blocks of 256 threads for rows x nb groups of G lanes: all at once when
-// they fit, else three a SM (and one group for every column block).
-unsigned grid_for(int64_t rows, int64_t nb, int G) {
-    const int per = 256 / G;
-    const int64_t want = ceil_div(rows * nb, per), most = std::max<int64_t>(ceil_div(nb, per), int64_t(num_sms()) * 3);
+// Blocks of 256 threads for rows x nb blocks of columns: a group each when all
+// are resident at once, else as many as are (and one group for every block of
+// columns).
+template <class L>
+unsigned grid_for(int64_t rows, int64_t nb) {
+    const int per = 256 / L::G;
+    const int64_t want = ceil_div(rows * nb, per),
+                  most = std::max<int64_t>(ceil_div(nb, per), int64_t(num_sms()) * L::kResident);
     return static_cast<unsigned>(std::min(want, most));
 }
 
@@ -244,9 +248,9 @@ template <class T>
 void restore8(int64_t rows, int64_t cols, const Saved8& s, T* y, int64_t ldy, cudaStream_t stream) {
     const ActArgs a{rows, cols, ceil_div(cols, kBlock8), TG_ACT_NONE, 0.0f, Range8{}};
     const bool al = aligned<T>(y, ldy);
-    const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
+    const unsigned grid = al ? grid_for<Lanes<T, true>>(rows, a.nb) : grid_for<Lanes<T, false>>(rows, a.nb);
     launch_dependent("restore8", al ? restore8_kernel<T, true> : restore8_kernel<T, false>,
-                     dim3(grid_for(rows, a.nb, G)), dim3(256), 0, stream, a, s, y, ldy);
+                     dim3(grid), dim3(256), 0, stream, a, s, y, ldy);
 }
 template void restore8<float>(int64_t, int64_t, const Saved8&, float*, int64_t, cudaStream_t);
 template void restore8<__nv_bfloat16>(int64_t, int64_t, const Saved8&, __nv_bfloat16*, int64_t, cudaStream_t);
@@ -279,8 +283,8 @@ TG_API tg_status tg_save8(int64_t rows, int64_t cols, int32_t dtype, const void*
             const bool al = aligned<T>(x, ldx) && aligned<T>(y, ldy);
             auto kern = save8_kernel<T, false, -1>;
             if (al) by_act(act, [&](auto k) { kern = save8_kernel<T, true, decltype(k)::value>; });
-            const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
-            launch_dependent("save8", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, xp, ldx, yp,
+            const unsigned grid = al ? grid_for<Lanes<T, true>>(rows, a.nb) : grid_for<Lanes<T, false>>(rows, a.nb);
+            launch_dependent("save8", kern, dim3(grid), dim3(256), 0, as_stream(stream), a, xp, ldx, yp,
                    ldy, o);
         });
     });
@@ -339,8 +343,8 @@ TG_API tg_status tg_activation_grad(int64_t rows, int64_t cols, int32_t dtype, c
                     constexpr int A = decltype(k)::value;
                     kern = codes ? act_grad_kernel<T, true, true, A> : act_grad_kernel<T, true, false, A>;
                 });
-            const int G = al ? Lanes<T, true>::G : Lanes<T, false>::G;
-            launch_dependent("activation_grad", kern, dim3(grid_for(rows, a.nb, G)), dim3(256), 0, as_stream(stream), a, dyp,
+            const unsigned grid = al ? grid_for<Lanes<T, true>>(rows, a.nb) : grid_for<Lanes<T, false>>(rows, a.nb);
+            launch_dependent("activation_grad", kern, dim3(grid), dim3(256), 0, as_stream(stream), a, dyp,
                    lddy, xp, ldx, s, dxp, lddx);
         });
     });

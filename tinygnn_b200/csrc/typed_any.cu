@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
     __shared__ float db_rows[W ? kLoaders * 8 : 1];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
     uint8_t* const ring_p = raw + (ring - mb::smem_u32(raw));
-    const uint32_t tmem = set_up<STAGES, BN, SPLIT>(s, 8 / GROUPS, [&] {
+    const uint32_t tmem = set_up<STAGES, BN, SPLIT>(s, 8 / GROUPS, 128, [&] {
         if (W) plan_pieces(g.offsets, g.types, g.M, g.tiles_m * g.tiles_n, g.slots, 1 << 30, s.prefix, s.order);
         else scan_types(g.offsets, g.types, g.M, BM, s.prefix);
     });
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
 
     if (warp < 8) {
         // ── loaders ──
-        int64_t i = 0, round = 0, it = item_of(0);
+        int64_t round = 0, it = item_of(0);
         bool ok = true;
         uint32_t ka[words<PartA, T>()], kb[words<PartB, T>()];
         Raw<int8_t, 8> k8[SAVED ? PartA::N : 1];
@@ -369,35 +369,63 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
         const int group = threadIdx.x / THREADS;
         // This group's first step of an item whose first stage is number i0.
         const auto first = [&](int64_t i0) { return GROUPS == 1 ? 0 : static_cast<int>((group + GROUPS - i0 % GROUPS) % GROUPS); };
-        Item m{}, next{};
-        if (it < items) m = item_at<T, OP>(g, s, it, BN);
+        // `now` is the step whose values the registers hold, `next` the one
+        // that is asked for while they are converted.  Values leave their
+        // registers into the stage, and the next step's are asked for as soon
+        // as they have: A's are on their way while B is converted, B's while
+        // this thread waits for the next stage and converts A.  (One place
+        // that fetches and one that converts: small products are bound by
+        // instructions being fetched for the first time.)
+        Item now{}, next{};
+        int step = 0, next_step = 0;
+        int64_t base = 0, next_base = 0;  // numbers of the items' first stages
+        bool have = false, more = it < items;
+        if (more) {
+            next = item_at<T, OP>(g, s, it, BN);
+            next_step = first(0);
+        }
         float sum[8];
-        bool fetched = false;  // the registers hold the next step's values
-        while (it < items && ok) {
-            const bool sums = W && g.db != nullptr && m.m0 == 0;
+        const auto clear = [&] {
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
-            it = item_of(++round);
-            const bool more = it < items;
-            if (more) next = item_at<T, OP>(g, s, it, BN);
-            for (int step = first(i); step < m.steps; step += GROUPS) {
-                if (!fetched) {
-                    fetch_a(m, step);
-                    fetch_b(m, step);
+        };
+        clear();
+        // Adds the item's column sums of dY up (every loader thread calls it).
+        const auto finish_sums = [&](const Item& m) {
+            if constexpr (W) {
+                if (g.db == nullptr || m.m0 != 0) return;
+                // threads that share a column, as rows of db_rows
+                const bool vec = g.b_align == kVector;
+                const int G = vec ? kLoaders / PartB::LANES : 8 / PartB::HALVES;
+                if (vec) {
+#pragma unroll
+                    for (int j = 0; j < VAL; ++j) db_rows[threadIdx.x / PartB::LANES * BN + PartB::col() + j] = sum[j];
+                } else {
+                    float* r = db_rows + threadIdx.x / 32 / PartB::HALVES * BN + PartB::pair_col();
+                    r[0] = sum[0];
+                    r[1] = sum[1];
                 }
-                const int64_t n = i + step;
-                const int st = static_cast<int>(n % STAGES);
-                if (n >= STAGES) ok = mb::wait(&s.empty[st], (n / STAGES - 1) & 1, &g_error, 41);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                // The next step's values are asked for as soon as this step's
-                // have left their registers: A's are on their way while B is
-                // converted, B's while this thread waits for the next stage
-                // and converts A.
-                const bool here = step + GROUPS < m.steps;
-                const int after = here ? step + GROUPS : first(i + m.steps);
-                const Item then = here ? m : next;
-                fetched = here || (more && after < next.steps);
-                uint8_t* const a = ring_p + st * S::kStage;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (ok && threadIdx.x < BN && m.n0 + threadIdx.x < g.N) {
+                    float all = 0.0f;
+#pragma unroll 4
+                    for (int q = 0; q < G; ++q) all += db_rows[q * BN + threadIdx.x];
+                    (m.whole ? g.db + m.t * g.N : g.db_part + m.p * g.N)[m.n0 + threadIdx.x] = all;
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                clear();
+            }
+        };
+        while (have || more) {
+            // A group may have no step in an item (two groups, one step).
+            const bool fetch_next = more && next_step < next.steps;
+            uint8_t* const a = ring_p + static_cast<int>((base + step) % STAGES) * S::kStage;
+            const int64_t n = base + step;
+            if (have) {
+                // (after a wait that ran out the loop goes on without waiting: the
+                // loaders meet at barriers)
+                if (ok && n >= STAGES) ok = mb::wait(&s.empty[n % STAGES], (n / STAGES - 1) & 1, &g_error, 41);
+                ok = __all_sync(0xffffffffu, ok);
                 if constexpr (SAVED) {
 #pragma unroll
                     for (int u = 0; u < PartA::N; ++u) {
@@ -411,40 +439,38 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
                 } else {
                     put_tile<PartA, T>(a, S::kA, g.a_align, ka, false, sum);
                 }
-                if (fetched) fetch_a(then, after);
-                put_tile<PartB, T>(a + PA * S::kA, S::kB, g.b_align, kb, sums, sum);
-                if (fetched) fetch_b(then, after);
+            }
+            if (fetch_next) fetch_a(next, next_step);
+            if (have) put_tile<PartB, T>(a + PA * S::kA, S::kB, g.b_align, kb, W && g.db != nullptr && now.m0 == 0, sum);
+            if (fetch_next) fetch_b(next, next_step);
+            if (have) {
                 // (the MMA's thread passes the writes on to the tensor cores: a
                 // proxy fence here would wait for the loads just issued)
                 __syncwarp();
-                if (lane == 0) mb::arrive(&s.full[st]);
+                if (lane == 0 && ok) mb::arrive(&s.full[n % STAGES]);
             }
-            i += m.steps;
-            if constexpr (W) {
-                if (sums) {  // the same for every loader thread
-                    // threads that share a column, as rows of db_rows
-                    const bool vec = g.b_align == kVector;
-                    const int G = vec ? kLoaders / PartB::LANES : 8 / PartB::HALVES;
-                    if (vec) {
-#pragma unroll
-                        for (int j = 0; j < VAL; ++j)
-                            db_rows[threadIdx.x / PartB::LANES * BN + PartB::col() + j] = sum[j];
-                    } else {
-                        float* r = db_rows + threadIdx.x / 32 / PartB::HALVES * BN + PartB::pair_col();
-                        r[0] = sum[0];
-                        r[1] = sum[1];
+            // the sums of every item that `next` is about to leave behind are
+            // complete once its last step has been converted
+            if (have && (!more || next_base != base)) finish_sums(now);
+            have = fetch_next;
+            if (fetch_next || more) {
+                if (fetch_next) {
+                    now = next;
+                    step = next_step;
+                    base = next_base;
+                }
+                next_step += GROUPS;
+                if (next_step >= next.steps) {
+                    if (!fetch_next) finish_sums(next);  // nothing of this item was this group's
+                    next_base += next.steps;
+                    it = item_of(++round);
+                    more = it < items;
+                    if (more) {
+                        next = item_at<T, OP>(g, s, it, BN);
+                        next_step = first(next_base);
                     }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    if (ok && threadIdx.x < BN && m.n0 + threadIdx.x < g.N) {
-                        float all = 0.0f;
-#pragma unroll 4
-                        for (int q = 0; q < G; ++q) all += db_rows[q * BN + threadIdx.x];
-                        (m.whole ? g.db + m.t * g.N : g.db_part + m.p * g.N)[m.n0 + threadIdx.x] = all;
-                    }
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
                 }
             }
-            m = next;
         }
     } else if (warp == 8) {
         // ── MMA issuer ──

@@ -45,7 +45,7 @@ constexpr uint32_t tmem_cols() { return 2 * BN * (SPLIT ? 2 : 1); }
 // Barriers, TMEM (warp 2) and the plan of the work (warp 3: plan(), over the
 // types' offsets); every thread returns with them in place.
 template <int STAGES, int BN, bool SPLIT = false, class F>
-__device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, F&& plan) {
+__device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, int acc_arrivals, F&& plan) {
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
@@ -54,7 +54,7 @@ __device__ __forceinline__ uint32_t set_up(Shared& s, int full_arrivals, F&& pla
         }
         for (int i = 0; i < 2; ++i) {
             mb::init(&s.acc_full[i], 1);
-            mb::init(&s.acc_empty[i], 128);
+            mb::init(&s.acc_empty[i], acc_arrivals);
         }
         mb::init(&s.drain, 1);
         mb::fence_init();

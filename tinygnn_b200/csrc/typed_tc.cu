@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
         tc::prefetch_map(&ma);
         tc::prefetch_map(&mw);
     }
-    const uint32_t tmem = set_up<STAGES, BN>(s, 1, [&] { scan_types(g.offsets, g.types, g.M, BM, s.prefix); });
+    const uint32_t tmem = set_up<STAGES, BN>(s, 1, BN == 256 ? 256 : 128, [&] { scan_types(g.offsets, g.types, g.M, BM, s.prefix); });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tiles = static_cast<int64_t>(s.prefix[g.types]) * g.tiles_n;
     const int KB = static_cast<int>((g.K + tc::kInner - 1) / tc::kInner);
@@ -108,21 +108,26 @@ __global__ void __launch_bounds__(kThreads, 1) typed_rows_tc_kernel(const __grid
             }
         }
     } else if (warp >= 4) {
-        const int acc = (warp - 4) >> 2, q = warp & 3;
-        int local = acc;
-        for (int64_t tile = blockIdx.x + acc * static_cast<int64_t>(gridDim.x); tile < tiles;
-             tile += 2 * static_cast<int64_t>(gridDim.x), local += 2) {
+        // 256 columns: every tile is split between the two groups of four warps
+        // (a lone tile's results leave in half the time); fewer: in turn.
+        constexpr bool SHARE = BN == 256;
+        constexpr int WIDTH = SHARE ? BN / 2 : BN;
+        const int group = (warp - 4) >> 2, q = warp & 3, c0 = SHARE ? group * WIDTH : 0;
+        int local = SHARE ? 0 : group;
+        for (int64_t tile = blockIdx.x + local * static_cast<int64_t>(gridDim.x); tile < tiles;
+             tile += (SHARE ? 1 : 2) * static_cast<int64_t>(gridDim.x), local += SHARE ? 1 : 2) {
+            const int acc = local & 1;
             const int p = static_cast<int>(tile / g.tiles_n);
             const int t = find_type(s.prefix, g.types, p);
             const int64_t row0 = clamp_row(g.offsets[t], g.M) + static_cast<int64_t>(p - s.prefix[t]) * BM + q * 32;
-            const int64_t left = clamp_row(g.offsets[t + 1], g.M) - row0;
-            prefetch_bias<T, BN>(out, t, tile % g.tiles_n * BN);
+            const int64_t left = clamp_row(g.offsets[t + 1], g.M) - row0, n0 = tile % g.tiles_n * BN + c0;
+            prefetch_bias<T, WIDTH>(out, t, n0);
             const bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 25);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc::fence_after();
-            finish_rows<T, BN, true>(tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16), out, t, row0,
-                                     left < 0 ? 0 : (left < 32 ? static_cast<int>(left) : 32), tile % g.tiles_n * BN,
-                                     stage_out[warp - 4]);
+            finish_rows<T, WIDTH, true>(tmem + acc * BN + c0 + (static_cast<uint32_t>(q * 32) << 16), out, t, row0,
+                                        left < 0 ? 0 : (left < 32 ? static_cast<int>(left) : 32), n0,
+                                        stage_out[warp - 4]);
             tc::fence_before();
             mb::arrive(&s.acc_empty[acc]);
         }
@@ -154,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_weight_tc_kernel(const __gr
     __shared__ Shared s;
     __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
     const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t tmem = set_up<STAGES, BN>(s, 1, [&] {
+    const uint32_t tmem = set_up<STAGES, BN>(s, 1, 128, [&] {
         plan_pieces(g.offsets, g.types, g.M, g.tiles_k * g.tiles_n, g.slots, g.longest, s.prefix, s.order);
     });
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
