@@ -198,7 +198,6 @@ struct WeightPlan {
     int tiles_k, tiles_n, slots, longest;
     int64_t ldp, items;
     float *part, *db_part;
-    bool pairs;  // on CTA pairs (tiles of 256 x 256)
 };
 
 // TMA-fed kernels and the choice between them and the others (typed_tc.cu).
@@ -218,9 +217,6 @@ struct TmaMatrix {
 // TMA-fed kernels on CTA pairs (typed_pair.cu).
 template <class T, bool TRANS>
 void typed_rows_pair(const RowsArgs<T>& a, const TmaMatrix<T>& A, const TmaMatrix<T>& W, cudaStream_t s);
-template <class T, class O>
-void typed_weight_pair(const WeightArgs<T, O>& a, const WeightPlan& w, const TmaMatrix<T>& X, const TmaMatrix<T>& Y,
-                       cudaStream_t s);
 int typed_pair_take_error();
 
 // Loader-fed kernels (typed_any.cu).
@@ -230,8 +226,8 @@ template <class T, class O>
 void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s);
 int typed_any_take_error();
 
-// At most kFewRows rows (typed_few.cu).
-constexpr int64_t kFewRows = 16;
+// A few rows (typed_few.cu).
+constexpr int64_t kFewRows = 32;
 template <class T, bool TRANS>
 void typed_rows_few(const RowsArgs<T>& a, cudaStream_t s);
 template <class T, class O>

@@ -1,10 +1,10 @@
 // ============================================================================
-//  typed_any.cu -- the typed products on the tensor cores for operands of any
-//  type and alignment, converted on their way into shared memory.
+//  typed_any.cu -- the typed products on the tensor cores for operands that are
+//  converted on their way into shared memory.
 //
-//  TMA needs 16-byte aligned rows and copies values as they are.  Here eight
-//  loader warps read the operands with plain loads and write the MMA's 16-bit
-//  tiles themselves, so one launch takes
+//  TMA copies values as they are.  Here eight loader warps read the operands
+//  with plain loads and write the MMA's 16-bit tiles themselves, so one launch
+//  takes
 //   fp32       each value split into three bf16 parts (24 bits, exactly):
 //              x0 = x's upper half, x1 = bf16(x - x0), x2 = bf16(x - x0 - x1);
 //              a product is the six part products x_i y_j with i + j <= 2
@@ -12,7 +12,7 @@
 //              parts of 768 inner indexes that are added up in fp32, rounded
 //              to nearest (see stage_mmas).  An infinity in an fp32 operand
 //              gives NaN;
-//   bf16, fp16 with rows of any alignment;
+//   bf16, fp16 (weight gradients of moderate size: db is added up on the way);
 //   8 bits     code * 2^e as one bf16 or fp16 value, exactly;
 //  and rows past a type's end and columns past the matrix are zeros.  Where
 //  dY passes through the loaders, they add up db on the way.
@@ -47,7 +47,7 @@ struct AnyArgs {
     Saved8 a8;  // the first operand in 8 bits (weight only)
     const T* B;
     int64_t ldb, stride_b;
-    int a_align, b_align;
+    bool a_pair, b_pair;  // rows aligned to two values, not to 16 bytes (fp32)
     // weight
     int slots;
     int64_t stride_c, ldp;
@@ -63,35 +63,6 @@ struct Source {
     int64_t ld;
     int rows, cols;  // of the tile, how many exist
 };
-
-// How an operand's rows are aligned.
-enum Align { kElement, kPair, kVector };  // to one value, two values, 16 bytes
-
-// 16 bytes of values at p, of which the first `n` values exist.
-template <class T>
-__device__ __forceinline__ void load16(const T* p, int n, uint32_t* w) {
-    constexpr int V = 16 / static_cast<int>(sizeof(T));
-    const Raw<T, V> k = n >= V ? load_raw<T, V>(p)
-                               : gather_raw<T, V>([&](int j) { return j < n ? p[j] : from_f32<T>(0.0f); });
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = k.w[j];
-}
-// Two values at p.
-template <class T>
-__device__ __forceinline__ void load2(const T* p, int n, bool pair, uint32_t* w) {
-    if (pair && n >= 2) {
-        if (sizeof(T) == 4) {
-            const uint2 q = *reinterpret_cast<const uint2*>(p);
-            w[0] = q.x, w[sizeof(T) == 4] = q.y;
-        } else {
-            w[0] = *reinterpret_cast<const uint32_t*>(p);
-        }
-        return;
-    }
-    const uint32_t lo = n > 0 ? bits(p[0]) : 0u, hi = n > 1 ? bits(p[1]) : 0u;
-    if (sizeof(T) == 4) w[0] = lo, w[sizeof(T) == 4] = hi;
-    else w[0] = lo | hi << 16;
-}
 
 // Chunk c of row r of a plane: 128-byte rows, 16-byte chunks swizzled.  Tiles
 // of more than 64 columns are chunks of 8 KB.
@@ -136,16 +107,12 @@ __device__ __forceinline__ void put16(uint8_t* at, uint32_t plane, const uint32_
         for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(at + q * plane) = make_uint2(k[q][0], k[q][1]);
     }
 }
-template <class T>
+// Two fp32 values into three planes.
 __device__ __forceinline__ void put2(uint8_t* at, uint32_t plane, const uint32_t* w) {
-    if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint32_t*>(at) = w[0];
-    } else {
-        uint32_t k[3][1];
-        split3<2>(w, k);
+    uint32_t k[3][1];
+    split3<2>(w, k);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(at + q * plane) = k[q][0];
-    }
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(at + q * plane) = k[q][0];
 }
 template <class T>
 __device__ __forceinline__ float value_of(const uint32_t* w, int j) {
@@ -157,11 +124,12 @@ __device__ __forceinline__ float value_of(const uint32_t* w, int j) {
 
 // The part of a tile of ROWS memory rows x COLS columns that one of THREADS
 // loader threads moves.  Rows 16-byte aligned: VAL neighbouring columns (16
-// bytes; 8 of an 8-bit copy) of every STEP-th row.  Others: a warp takes 64
-// columns of a row at a time, two neighbouring ones a lane, so that its loads
-// cover whole lines whatever the alignment (a lane that read its own eight
-// values of 4 bytes would touch each line eight times); halves of 128 columns
-// belong to warps of one parity, so a lane keeps its columns.
+// bytes; 8 of an 8-bit copy) of every STEP-th row.  fp32 rows aligned to two
+// values (602 columns; a copy would cost as much as the product): a warp takes
+// 64 columns of a row at a time, two neighbouring ones a lane, so that its
+// loads cover whole lines; halves of 128 columns belong to warps of one parity,
+// so a lane keeps its columns.  No access is partly past a row's end (other
+// matrices are copied first).
 template <int ROWS, int COLS, int THREADS, int VAL>
 struct Part {
     static constexpr int LANES = COLS / VAL, STEP = THREADS / LANES, N = ROWS / STEP;
@@ -180,31 +148,26 @@ struct Part {
 template <class P, class T>
 constexpr int words() { return P::N * P::kVal * static_cast<int>(sizeof(T)) / 4; }
 
+// pair: rows aligned to two values (fp32 only).
 template <class P, class T>
-__device__ __forceinline__ void fetch_tile(const Source<T>& s, int align, uint32_t (&w)[words<P, T>()]) {
-    const bool whole = s.rows >= P::rows() && s.cols >= P::cols();  // the same for all threads
-    if (align == kVector) {
+__device__ __forceinline__ void fetch_tile(const Source<T>& s, bool pair, uint32_t (&w)[words<P, T>()]) {
+    if (sizeof(T) == 2 || !pair) {
         const T* p = s.p + P::row(0) * s.ld + P::col();
         const int64_t step = P::STEP * s.ld;
-        if (whole) {
+        const bool there = P::col() < s.cols;
 #pragma unroll
-            for (int i = 0; i < P::N; ++i, p += step) load16(p, P::kVal, w + i * 4);
-        } else {
-            const int n = s.cols - P::col();
-#pragma unroll
-            for (int i = 0; i < P::N; ++i, p += step) load16(p, P::row(i) < s.rows ? n : 0, w + i * 4);
+        for (int i = 0; i < P::N; ++i, p += step) {
+            const uint4 q = there && P::row(i) < s.rows ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
         }
     } else {
         const T* p = s.p + P::pair_row(0) * s.ld + P::pair_col();
         const int64_t step = P::PAIR_STEP * s.ld;
-        if (whole && align == kPair) {
+        const bool there = P::pair_col() < s.cols;
 #pragma unroll
-            for (int i = 0; i < P::PAIRS; ++i, p += step) load2(p, 2, true, w + i * sizeof(T) / 2);
-        } else {
-            const int n = s.cols - P::pair_col();
-#pragma unroll
-            for (int i = 0; i < P::PAIRS; ++i, p += step)
-                load2(p, P::pair_row(i) < s.rows ? n : 0, align == kPair, w + i * sizeof(T) / 2);
+        for (int i = 0; i < words<P, T>() / 2; ++i, p += step) {
+            const uint2 q = there && P::pair_row(i) < s.rows ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+            w[2 * i] = q.x, w[2 * i + 1] = q.y;
         }
     }
 }
@@ -212,9 +175,9 @@ __device__ __forceinline__ void fetch_tile(const Source<T>& s, int align, uint32
 // of `sum`.  A row's place in the swizzle repeats every 8 rows, so the
 // addresses are a few and constant steps from them.
 template <class P, class T>
-__device__ __forceinline__ void put_tile(uint8_t* tile, uint32_t plane, int align,
+__device__ __forceinline__ void put_tile(uint8_t* tile, uint32_t plane, bool pair,
                                          const uint32_t (&w)[words<P, T>()], bool add, float (&sum)[8]) {
-    if (align == kVector) {
+    if (sizeof(T) == 2 || !pair) {
         static_assert(P::STEP % 8 == 0, "whole swizzle periods");
         uint8_t* at = tile + chunk_at(P::row(0), P::col() / 8) + P::col() % 8 * 2;
 #pragma unroll
@@ -232,13 +195,12 @@ __device__ __forceinline__ void put_tile(uint8_t* tile, uint32_t plane, int alig
 #pragma unroll
         for (int i = 0; i < PERIOD; ++i) at[i] = tile + chunk_at(P::pair_row(i), c >> 3) + (c & 7) * 2;
 #pragma unroll
-        for (int i = 0; i < P::PAIRS; ++i)
-            put2<T>(at[i % PERIOD] + i / PERIOD * 1024, plane, w + i * sizeof(T) / 2);
+        for (int i = 0; i < words<P, T>() / 2; ++i) put2(at[i % PERIOD] + i / PERIOD * 1024, plane, w + i * 2);
         if (add) {
 #pragma unroll
-            for (int i = 0; i < P::PAIRS; ++i) {
-                sum[0] += value_of<T>(w + i * sizeof(T) / 2, 0);
-                sum[1] += value_of<T>(w + i * sizeof(T) / 2, 1);
+            for (int i = 0; i < words<P, T>() / 2; ++i) {
+                sum[0] += value_of<T>(w + i * 2, 0);
+                sum[1] += value_of<T>(w + i * 2, 1);
             }
         }
     }
@@ -360,11 +322,11 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
                 fetch_tile8<PartA>(g.a8, m.r0 + k, m.m0, clip(m.r1 - m.r0 - k, tc::kInner), clip(g.K - m.m0, BM), k8,
                                    e8);
             } else {
-                fetch_tile<PartA, T>(source_a<T, OP>(g, m, step, BN), g.a_align, ka);
+                fetch_tile<PartA, T>(source_a<T, OP>(g, m, step, BN), g.a_pair, ka);
             }
         };
         const auto fetch_b = [&](const Item& m, int step) {
-            fetch_tile<PartB, T>(source_b<T, OP>(g, m, step, BN), g.b_align, kb);
+            fetch_tile<PartB, T>(source_b<T, OP>(g, m, step, BN), g.b_pair, kb);
         };
         const int group = threadIdx.x / THREADS;
         // This group's first step of an item whose first stage is number i0.
@@ -395,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
             if constexpr (W) {
                 if (g.db == nullptr || m.m0 != 0) return;
                 // threads that share a column, as rows of db_rows
-                const bool vec = g.b_align == kVector;
+                const bool vec = sizeof(T) == 2 || !g.b_pair;
                 const int G = vec ? kLoaders / PartB::LANES : 8 / PartB::HALVES;
                 if (vec) {
 #pragma unroll
@@ -437,11 +399,11 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
                         store_chunk(a + chunk_at(PartA::row(u), PartA::col() / 8), h.w);
                     }
                 } else {
-                    put_tile<PartA, T>(a, S::kA, g.a_align, ka, false, sum);
+                    put_tile<PartA, T>(a, S::kA, g.a_pair, ka, false, sum);
                 }
             }
             if (fetch_next) fetch_a(next, next_step);
-            if (have) put_tile<PartB, T>(a + PA * S::kA, S::kB, g.b_align, kb, W && g.db != nullptr && now.m0 == 0, sum);
+            if (have) put_tile<PartB, T>(a + PA * S::kA, S::kB, g.b_pair, kb, W && g.db != nullptr && now.m0 == 0, sum);
             if (fetch_next) fetch_b(next, next_step);
             if (have) {
                 // (the MMA's thread passes the writes on to the tensor cores: a
@@ -559,11 +521,9 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
     tear_down<BN, SPLIT>(s, tmem, 8);
 }
 
+// The least alignment that the loaders take, in bytes.
 template <class T>
-int alignment(const T* p, int64_t ld) {
-    const uint64_t b = reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(ld * sizeof(T));
-    return b % 16 == 0 ? kVector : (b % (2 * sizeof(T)) == 0 ? kPair : kElement);
-}
+constexpr int64_t least() { return sizeof(T) == 4 ? 8 : 16; }
 
 template <class T, int OP, int BN, bool SAVED>
 void go(const AnyArgs<T>& g, const RowsOut<T>& out, int64_t items, cudaStream_t s) {
@@ -579,9 +539,13 @@ void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s) {
     constexpr int OP = TRANS ? kGradInput : kForward;
     AnyArgs<T> g{};
     g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
-    g.A = a.A, g.lda = a.lda, g.B = a.W, g.ldb = a.ldw, g.stride_b = a.stride_w;
-    g.a_align = alignment(a.A, a.lda);
-    g.b_align = std::min(alignment(a.W, a.ldw), alignment(a.W, a.stride_w));
+    // W[t] is K x N in the forward pass, N x K in the input gradient.
+    const int64_t wr = TRANS ? a.N : a.K, wc = TRANS ? a.K : a.N;
+    const Operand<T> A(1, a.M, a.K, a.A, a.lda, 0, s, least<T>()),
+        W(a.types, wr, wc, a.W, a.ldw, a.stride_w, s, least<T>());
+    g.A = A.p, g.lda = A.ld, g.B = W.p, g.ldb = W.ld, g.stride_b = W.stride;
+    g.a_pair = !in_place(1, A.own ? A.ld : a.K, A.p, A.ld, 0);
+    g.b_pair = !in_place(a.types, W.own ? W.ld : wc, W.p, W.ld, W.stride);
     const RowsOut<T> out{a.N, a.bias, a.act, a.alpha, a.C, a.ldc, store_mode(a.C, a.ldc * sizeof(T)), a.saved, a.r8};
     const int64_t pieces = a.M / BM + std::min<int64_t>(a.types, a.M);
     const int BN = tile_width(pieces, a.N, 128, a.saved.codes != nullptr);
@@ -597,9 +561,9 @@ void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream
     AnyArgs<T> g{};
     g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
     g.tiles_m = w.tiles_k, g.tiles_n = w.tiles_n;
-    g.A = a.X, g.lda = a.ldx, g.a8 = a.saved, g.B = a.dY, g.ldb = a.lddy;
-    g.a_align = alignment(a.X, a.ldx);
-    g.b_align = alignment(a.dY, a.lddy);
+    const Operand<T> Y(1, a.M, a.N, a.dY, a.lddy, 0, s, least<T>());
+    g.a8 = a.saved, g.B = Y.p, g.ldb = Y.ld;
+    g.b_pair = !in_place(1, Y.own ? Y.ld : a.N, Y.p, Y.ld, 0);
     g.slots = w.slots, g.part = w.part, g.ldp = w.ldp, g.stride_c = a.stride_dw;
     g.out_f32 = sizeof(O) == 4;
     RowsOut<T> out{};
@@ -610,8 +574,14 @@ void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream
     g.db = a.db, g.db_part = w.db_part;
     const auto by_source = [&](auto bn) {
         constexpr int BN = decltype(bn)::value;
-        if (saved) go<T, kGradWeight, BN, true>(g, out, w.items, s);
-        else go<T, kGradWeight, BN, false>(g, out, w.items, s);
+        if (saved) {
+            go<T, kGradWeight, BN, true>(g, out, w.items, s);
+        } else {
+            const Operand<T> X(1, a.M, a.K, a.X, a.ldx, 0, s, least<T>());
+            g.A = X.p, g.lda = X.ld;
+            g.a_pair = !in_place(1, X.own ? X.ld : a.K, X.p, X.ld, 0);
+            go<T, kGradWeight, BN, false>(g, out, w.items, s);
+        }
     };
     if (w.BN == 64) by_source(std::integral_constant<int, 64>{});
     else by_source(std::integral_constant<int, 128>{});

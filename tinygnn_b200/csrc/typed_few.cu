@@ -2,7 +2,7 @@
 //  typed_few.cu -- the typed products of a few rows (serving: single tokens or
 //  nodes, each through its type's weight).
 //
-//  With at most kFewRows rows the products read the used weights (or write all
+//  With a few rows (see few_rows()) the products read the used weights (or write all
 //  of dW) and do next to no arithmetic: they are bound by HBM and by latency,
 //  and a 128-row tensor-core tile would be filled for a row or two.  These
 //  kernels stream the weights through FP32 FMAs.  Each row finds its type by

@@ -374,6 +374,105 @@ CUtensorMap tma_map(const TmaMatrix<T>& m, int64_t batch, int64_t rows, int64_t 
     return tc::map16<3>(m.p, is_bf16<T>(), dims, strides, box);
 }
 
+// ── operands ─────────────────────────────────────────────────────────────
+// Whether the kernels read a batch of matrices where they lie: rows and
+// matrices 16-byte aligned, and no row that ends inside 16 bytes (fp32 rows
+// for the loaders may be aligned to, and end at, two values).
+template <class T>
+bool in_place(int64_t batch, int64_t cols, const T* p, int64_t ld, int64_t stride, int64_t bytes = 16) {
+    const uint64_t b = reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(ld * sizeof(T)) |
+                       static_cast<uint64_t>(cols * sizeof(T)) |
+                       (batch > 1 ? static_cast<uint64_t>(stride * sizeof(T)) : 0);
+    return b % bytes == 0;
+}
+
+// A copy with 16-byte aligned rows (zeros to their end) of a batch of matrices
+// whose row r lies at (r / inner) * stride + (r % inner) * lds.  A warp a row.
+template <class T>
+__global__ void __launch_bounds__(256) align_kernel(int64_t rows, int64_t cols, const T* src, int64_t inner,
+                                                    int64_t stride, int64_t lds, T* dst, int64_t ld) {
+    constexpr int V = 16 / static_cast<int>(sizeof(T)), U = 4;
+    wait_for_previous();
+    const int lane = threadIdx.x % 32;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; r < rows; r += warps) {
+        const T* p = src + r / inner * stride + r % inner * lds;
+        const bool odd = Held<T, V, false>::odd(p);
+        for (int64_t c0 = lane * V; c0 < ld; c0 += U * 32 * V) {
+            Held<T, V, false> h[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = c0 + u * 32 * V;
+                if (c + V <= cols) h[u].fetch(p + c);
+                else h[u].fetch(p + c, c < cols ? static_cast<int>(cols - c) : 0);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = c0 + u * 32 * V;
+                if (c >= ld) break;
+                float x[V];
+                h[u].values(odd, x);
+                store_v<T, V>(dst + r * ld + c, x);
+            }
+        }
+    }
+}
+
+// A matrix (or a batch) in place, or an aligned copy of it in scratch.
+template <class T>
+struct Operand {
+    const T* p = nullptr;
+    int64_t ld = 0, stride = 0;  // elements
+    T* own = nullptr;
+    cudaStream_t s = nullptr;
+
+    // least: the alignment in bytes that the kernel can do with.
+    Operand(int64_t batch, int64_t rows, int64_t cols, const T* src, int64_t lds, int64_t src_stride, cudaStream_t st,
+            int64_t least = 16)
+        : s(st) {
+        take(batch, rows, cols, src, lds, src_stride, least);
+    }
+    // A matrix given as it is or in 8 bits.
+    Operand(int64_t rows, int64_t cols, const T* src, int64_t lds, const Saved8& saved, cudaStream_t st) : s(st) {
+        if (!saved.codes) {
+            take(1, rows, cols, src, lds, 0, 16);
+            return;
+        }
+        make(1, rows, cols);
+        restore8<T>(rows, cols, saved, own, ld, s);
+    }
+    ~Operand() {
+        if (own) scratch_free(own, s);
+    }
+    Operand(const Operand&) = delete;
+    Operand& operator=(const Operand&) = delete;
+    TmaMatrix<T> matrix() const { return {p, ld, stride}; }
+
+  private:
+    void make(int64_t batch, int64_t rows, int64_t cols) {
+        constexpr int64_t V = 16 / sizeof(T);
+        ld = (cols + V - 1) / V * V;
+        stride = rows * ld;
+        own = static_cast<T*>(scratch_alloc(static_cast<size_t>(batch * stride) * sizeof(T), s));
+        p = own;
+    }
+    void take(int64_t batch, int64_t rows, int64_t cols, const T* src, int64_t lds, int64_t src_stride, int64_t least) {
+        // (TMA zero-fills past a row's end itself)
+        const bool there = sizeof(T) == 2 ? rows_aligned16(src, lds, 2) && (batch == 1 || src_stride % 8 == 0)
+                                          : in_place(batch, cols, src, lds, src_stride, least);
+        if (there) {
+            p = src;
+            ld = lds;
+            stride = batch == 1 ? rows * lds : src_stride;
+            return;
+        }
+        make(batch, rows, cols);
+        launch_dependent("typed_align", align_kernel<T>,
+                         dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(batch * rows, 8), num_sms() * 8))),
+                         dim3(256), 0, s, batch * rows, cols, src, rows, src_stride, lds, own, ld);
+    }
+};
+
 // Reads and clears the error word (the stream is idle).
 static int take_error() {
     int h = 0;

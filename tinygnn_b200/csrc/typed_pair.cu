@@ -1,13 +1,13 @@
 // ============================================================================
-//  typed_pair.cu -- the large typed products on pairs of CTAs: tiles of 256
-//  rows x 256 columns, 16-bit operands by TMA.
+//  typed_pair.cu -- the large typed products (forward pass, input gradient) on
+//  pairs of CTAs: tiles of 256 rows x 256 columns, 16-bit operands by TMA.
 //
-//  A lone CTA's 128 x 256 tile reads 12 KB of shared memory per MMA of 16 inner
-//  indexes (128 cycles) and takes as much from L2: about 190 bytes a cycle
-//  where shared memory gives 128.  In a pair each CTA holds 128 rows and 128
-//  of the 256 columns, 8 KB per MMA and 8 KB from L2, and the tensor cores are
-//  the bound again.  Measured (B200): dX of 65,536 x 1,024 x 1,024, 8 types,
-//  bf16: see the table in the class comment of choose().
+//  A lone CTA's 128 x 256 tile takes 12 KB of operands per MMA of 16 inner
+//  indexes (128 cycles); in a pair each CTA holds 128 rows and 128 of the 256
+//  columns and takes 8 KB.  A step of 64 inner indexes takes 615 cycles (512 at
+//  the tensor cores' peak), at the 1.29 GHz that the power cap leaves: 65,536 x
+//  2,048 x 2,048 bf16 in 437-459 us, 1.2 PFLOP/s, where single CTAs take
+//  481-485 (fewer bytes moved is less power and a higher clock).
 //
 //  The structure is typed_tc.cu's: warp 0 loads, warp 1 of rank 0 issues the
 //  MMAs for both CTAs, warps 4-11 empty the two accumulators.
@@ -32,10 +32,9 @@ struct PairPlan {
 constexpr int STAGES = PairPlan::kStages;
 
 struct PairShared {
-    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain, tail, tail_peer;
+    uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain;
     uint32_t tmem;
     int prefix[kMaxTypes + 1];
-    uint16_t order[kMaxTypes];  // weight gradients only
 };
 
 template <class F>
@@ -51,8 +50,6 @@ __device__ __forceinline__ uint32_t set_up_pair(PairShared& s, F&& plan) {
             mb::init(&s.acc_empty[i], 8);  // both CTAs' four epilogue warps
         }
         mb::init(&s.drain, 1);
-        mb::init(&s.tail, 1);
-        mb::init(&s.tail_peer, 1);
         mb::fence_init();
     }
     if (warp == 2) tc::alloc_pair(&s.tmem, 2 * BN);
@@ -187,145 +184,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tear_down_pair(s, tmem, rank);
 }
 
-// ── weight kernel ────────────────────────────────────────────────────────
-template <class O>
-struct WeightPair {
-    int64_t M, K, N;
-    int types, tiles_k, tiles_n, slots, longest;
-    const int32_t* offsets;
-    O* dW;
-    int64_t lddw, stride_dw;
-    int mode;
-    float* part;
-    int64_t ldp;
-};
-
-template <class T, class O>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    typed_weight_pair_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap my,
-                             const WeightPair<O> g) {
-    constexpr uint32_t ID = tc::idesc(is_bf16<T>(), true, true, kRows, BN);
-    extern __shared__ uint8_t raw[];
-    __shared__ PairShared s;
-    __shared__ T stage_out[8][stage_bytes<T>() / sizeof(T)];
-    const uint32_t ring = (mb::smem_u32(raw) + 1023) & ~1023u;
-    const uint32_t rank = tc::cluster_rank();
-    const int per = g.tiles_k * g.tiles_n;
-    const uint32_t tmem = set_up_pair(s, [&] {
-        plan_pieces(g.offsets, g.types, g.M, per, g.slots, g.longest, s.prefix, s.order);
-    });
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t items = static_cast<int64_t>(s.prefix[g.types]) * per;
-    const int64_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-    const auto dealt_item = [&](int64_t r) { return dealt(r, pair, pairs); };
-    const auto item_at = [&](int64_t it) {
-        return weight_item(g.offsets, g.types, g.M, per, s.prefix, s.order, it);
-    };
-
-    if (warp == 0) {
-        int64_t i = 0;
-        uint32_t tails = 0;
-        bool ok = true;
-        for (int64_t round = 0, it; (it = dealt_item(round)) < items && ok; ++round) {
-            const WeightItem m = item_at(it);
-            const int k0 = m.in / g.tiles_n * kRows + static_cast<int>(rank) * BM;
-            const int n0 = m.in % g.tiles_n * BN + static_cast<int>(rank) * HN;
-            for (int64_t r = m.r0; r < m.r1; r += tc::kInner, ++i) {
-                const int st = static_cast<int>(i % STAGES);
-                if (i >= STAGES) ok = mb::wait(&s.empty[st], (i / STAGES - 1) & 1, &g_error, 61);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                const uint32_t a = ring + st * PairPlan::kStage, b = a + PairPlan::kA;
-                const uint32_t bar = tc::in_rank(&s.full[st], 0);
-                const bool cut = m.r1 - r < tc::kInner;
-                if (lane == 0) {
-                    const uint32_t on = cut ? mb::smem_u32(&s.tail) : bar;
-                    if (cut) mb::arrive_expect_tx(&s.tail, PairPlan::kStage);
-                    else if (rank == 0) mb::arrive_expect_tx(&s.full[st], 2 * PairPlan::kStage);
-#pragma unroll
-                    for (int c = 0; c < BM / 64; ++c)
-                        tc::tma3_pair(a + c * tc::kChunkBytes, &mx, k0 + c * 64, static_cast<int>(r), 0, on);
-#pragma unroll
-                    for (int c = 0; c < HN / 64; ++c)
-                        tc::tma3_pair(b + c * tc::kChunkBytes, &my, n0 + c * 64, static_cast<int>(r), 0, on);
-                }
-                __syncwarp();
-                if (cut) {
-                    // The piece's last rows are followed by another's: zero in
-                    // both operands (0 x NaN would not do), then pass them on.
-                    ok = mb::wait(&s.tail, tails & 1, &g_error, 62);
-                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                    zero_rows(a, PairPlan::kStage, static_cast<int>(m.r1 - r));
-                    if (rank != 0) {
-                        if (lane == 0) tc::arrive_at(tc::in_rank(&s.tail_peer, 0));
-                    } else {
-                        ok = tc::wait_cluster(&s.tail_peer, tails & 1, &g_error, 67);
-                        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                        if (lane == 0) mb::arrive(&s.full[st]);
-                    }
-                    ++tails;
-                    __syncwarp();
-                }
-            }
-        }
-        for (int64_t j = i > STAGES ? i - STAGES : 0; j < i && ok; ++j)
-            ok = mb::wait(&s.empty[j % STAGES], (j / STAGES) & 1, &g_error, 63);
-    } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            int64_t i = 0;
-            int local = 0;
-            bool ok = true;
-            for (int64_t it; (it = dealt_item(local)) < items && ok; ++local) {
-                const WeightItem m = item_at(it);
-                const int acc = local & 1;
-                if (local >= 2 && !(ok = tc::wait_cluster(&s.acc_empty[acc], (local / 2 - 1) & 1, &g_error, 64))) break;
-                tc::fence_after();
-                for (int64_t r = m.r0; r < m.r1; r += tc::kInner, ++i) {
-                    const int st = static_cast<int>(i % STAGES);
-                    if (!(ok = tc::wait_cluster(&s.full[st], (i / STAGES) & 1, &g_error, 65))) break;
-                    tc::fence_after();
-                    stage_mmas_pair<true, true>(ring + st * PairPlan::kStage, tmem + acc * BN, ID, r == m.r0);
-                    tc::commit_pair(&s.empty[st]);
-                }
-                if (ok) tc::commit_pair(&s.acc_full[acc]);
-            }
-        }
-    } else if (warp >= 4) {
-        const int acc = (warp - 4) >> 2, q = warp & 3;
-        const uint32_t freed = tc::in_rank(&s.acc_empty[acc], 0);
-        int local = acc;
-        for (int64_t it; (it = dealt_item(local)) < items; local += 2) {
-            const WeightItem m = item_at(it);
-            const int64_t n0 = m.in % g.tiles_n * BN;
-            const bool ok = mb::wait(&s.acc_full[acc], (local / 2) & 1, &g_error, 66);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            tc::fence_after();
-            const uint32_t addr = tmem + acc * BN + (static_cast<uint32_t>(q * 32) << 16);
-            const int64_t k = m.in / g.tiles_n * kRows + rank * BM + q * 32, left_k = g.K - k;
-            const int rows = left_k < 0 ? 0 : (left_k < 32 ? static_cast<int>(left_k) : 32);
-#pragma unroll 1
-            for (int c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 32) {
-                float v[32];
-                tc::load32(addr + c0, v);
-                const int64_t n = n0 + c0;
-                if (m.whole) {
-                    O* o = g.dW + m.t * g.stride_dw + k * g.lddw + n;
-                    // shared memory has room to stage rows of T, not of fp32
-                    if constexpr (sizeof(O) == sizeof(T)) store_rows(o, g.lddw, rows, g.N - n, v, g.mode, stage_out[warp - 4]);
-                    else store_rows(o, g.lddw, rows, g.N - n, v, g.mode == 0 ? -1 : g.mode, static_cast<O*>(nullptr));
-                } else {
-                    store_rows(g.part + (m.p * g.K + k) * g.ldp + n, g.ldp, rows, g.ldp - n, v, 2,
-                               static_cast<float*>(nullptr));
-                }
-            }
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::arrive_at(freed);
-        }
-        zero_empty_types(g.offsets, g.types, g.M, g.K, g.N, g.dW, g.lddw, g.stride_dw, g.mode, threadIdx.x - 128, 256);
-    }
-    tear_down_pair(s, tmem, rank);
-}
-
 // A grid of pairs, at most one CTA per SM.
 unsigned pair_grid(int64_t items) {
     return static_cast<unsigned>(2 * std::min<int64_t>(items, num_sms() / 2));
@@ -350,24 +208,11 @@ void typed_rows_pair(const RowsArgs<T>& a, const TmaMatrix<T>& A, const TmaMatri
               (a.M / kRows + std::min<int64_t>(a.types, a.M)) * g.tiles_n, s, ma, mw, g, out);
 }
 
-template <class T, class O>
-void typed_weight_pair(const WeightArgs<T, O>& a, const WeightPlan& w, const TmaMatrix<T>& X, const TmaMatrix<T>& Y,
-                       cudaStream_t s) {
-    const CUtensorMap mx = tma_map(X, 1, a.M, a.K, 64), my = tma_map(Y, 1, a.M, a.N, 64);
-    const WeightPair<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, w.longest, a.offsets, a.dW, a.lddw, a.stride_dw,
-                          store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O)), w.part, w.ldp};
-    run_pairs("typed_weight_pair", typed_weight_pair_kernel<T, O>, w.items, s, mx, my, g);
-}
-
-#define TG_TYPED_PAIR(T)                                                                                         \
-    template void typed_rows_pair<T, false>(const RowsArgs<T>&, const TmaMatrix<T>&, const TmaMatrix<T>&,        \
-                                            cudaStream_t);                                                       \
-    template void typed_rows_pair<T, true>(const RowsArgs<T>&, const TmaMatrix<T>&, const TmaMatrix<T>&,         \
-                                           cudaStream_t);                                                        \
-    template void typed_weight_pair<T, T>(const WeightArgs<T, T>&, const WeightPlan&, const TmaMatrix<T>&,       \
-                                          const TmaMatrix<T>&, cudaStream_t);                                    \
-    template void typed_weight_pair<T, float>(const WeightArgs<T, float>&, const WeightPlan&, const TmaMatrix<T>&, \
-                                              const TmaMatrix<T>&, cudaStream_t);
+#define TG_TYPED_PAIR(T)                                                                                  \
+    template void typed_rows_pair<T, false>(const RowsArgs<T>&, const TmaMatrix<T>&, const TmaMatrix<T>&, \
+                                            cudaStream_t);                                                \
+    template void typed_rows_pair<T, true>(const RowsArgs<T>&, const TmaMatrix<T>&, const TmaMatrix<T>&,  \
+                                           cudaStream_t);
 TG_TYPED_PAIR(__nv_bfloat16)
 TG_TYPED_PAIR(__half)
 

@@ -337,82 +337,20 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O
         }
 }
 
-// ── operands ─────────────────────────────────────────────────────────────
-// A 16-bit matrix with 16-byte aligned rows, from one whose row r lies at
-// (r / inner) * stride + (r % inner) * lds.
-template <class T>
-__global__ void __launch_bounds__(256) align_kernel(int64_t rows, int64_t cols, const T* src, int64_t inner,
-                                                    int64_t stride, int64_t lds, T* dst, int64_t ld) {
-    wait_for_previous();
-    const int64_t vecs = ld / 8, total = rows * vecs;
-    for (int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; v < total;
-         v += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = v / vecs, c = (v - r * vecs) * 8;
-        const T* p = src + r / inner * stride + r % inner * lds + c;
-        *reinterpret_cast<Raw<T, 8>*>(dst + r * ld + c) =
-            gather_raw<T, 8>([&](int j) { return c + j < cols ? p[j] : from_f32<T>(0.0f); });
-    }
-}
-
-// A matrix (or a batch of them) that TMA can read: in place, or a copy in scratch.
-template <class T>
-struct Operand {
-    const T* p = nullptr;
-    int64_t ld = 0, stride = 0;  // elements
-    T* own = nullptr;
-    cudaStream_t s = nullptr;
-    Operand(int64_t batch, int64_t rows, int64_t cols, const T* src, int64_t lds, int64_t src_stride, cudaStream_t st)
-        : s(st) {
-        if (readable(batch, src, lds, src_stride)) {
-            p = src;
-            ld = lds;
-            stride = batch == 1 ? rows * lds : src_stride;
-            return;
-        }
-        ld = (cols + 7) / 8 * 8;
-        stride = rows * ld;
-        own = static_cast<T*>(scratch_alloc(static_cast<size_t>(batch * stride) * 2, st));
-        p = own;
-        const int64_t want = ceil_div(batch * rows * (ld / 8), 256);
-        launch_dependent("typed_align", align_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(want, num_sms() * 8))),
-               dim3(256), 0, st, batch * rows, cols, src, rows, src_stride, lds, own, ld);
-    }
-    // A weight gradient's first operand.
-    template <class O>
-    Operand(const WeightArgs<T, O>& a, cudaStream_t st) : s(st) {
-        if (!a.saved.codes) {
-            Operand x(1, a.M, a.K, a.X, a.ldx, 0, st);
-            p = x.p, ld = x.ld, stride = x.stride, own = x.own;
-            x.own = nullptr;
-            return;
-        }
-        ld = (a.K + 7) / 8 * 8;
-        stride = a.M * ld;
-        own = static_cast<T*>(scratch_alloc(static_cast<size_t>(stride) * 2, st));
-        p = own;
-        restore8<T>(a.M, a.K, a.saved, own, ld, st);
-    }
-    ~Operand() {
-        if (own) scratch_free(own, s);
-    }
-    Operand(const Operand&) = delete;
-    Operand& operator=(const Operand&) = delete;
-
-    static bool readable(int64_t batch, const T* src, int64_t lds, int64_t stride) {
-        return rows_aligned16(src, lds, 2) && (batch == 1 || stride % 8 == 0);
-    }
-    TmaMatrix<T> matrix() const { return {p, ld, stride}; }
-};
-
 template <class T, bool TRANS>
 void typed_rows_tma(const RowsArgs<T>& a, cudaStream_t s) {
     const Operand<T> A(1, a.M, a.K, a.A, a.lda, 0, s);
     // W[t] is K x N in the forward pass, N x K in the input gradient.
     const int64_t wr = TRANS ? a.N : a.K, wc = TRANS ? a.K : a.N;
     const Operand<T> W(a.types, wr, wc, a.W, a.ldw, a.stride_w, s);
-    // Pairs of CTAs, where 256-row tiles of 256 columns are enough for all of
-    // them and the types long enough not to leave much of a tile empty.
-    if (a.N > 128 && a.M / 512 >= a.types && (a.M / 256) * ceil_div(a.N, 256) >= num_sms()) {
+    // Pairs of CTAs for long sums, where 256-row tiles of 256 columns are enough
+    // for all of them and the types long enough not to leave much of a tile
+    // empty.  Measured, back to back, pairs against single CTAs: 65,536 x 2,048
+    // x 2,048 437-459 against 481-485 us, 65,536 x 1,024 x 1,024 128 against
+    // 140, 16,384 x 1,024 x 1,024 38.5 against 39.0, 65,536 x 512 x 512 47.2
+    // both, 100,000 x 256 x 256 28.8 against 28.0.  (Weight gradients gained
+    // nothing: 149 against 139 us for 65,536 x 1,024 x 1,024.)
+    if (a.K > 512 && a.N > 128 && a.M / 512 >= a.types && (a.M / 256) * ceil_div(a.N, 256) >= num_sms()) {
         typed_rows_pair<T, TRANS>(a, A.matrix(), W.matrix(), s);
         return;
     }
@@ -437,12 +375,8 @@ template <class T, class O>
 void typed_weight_tma(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s) {
     // X in 8 bits: its values as a 16-bit matrix, exactly (33 us for 65,536 x
     // 1,024 at HBM rate; a kernel whose loaders decoded the codes into shared
-    // memory for every tile of columns took 193 us where pairs take 126).
-    const Operand<T> X(a, s), Y(1, a.M, a.N, a.dY, a.lddy, 0, s);
-    if (w.pairs) {
-        typed_weight_pair<T, O>(a, w, X.matrix(), Y.matrix(), s);
-        return;
-    }
+    // memory for every tile of columns took 60 us longer than this and TMA).
+    const Operand<T> X(a.M, a.K, a.X, a.ldx, a.saved, s), Y(1, a.M, a.N, a.dY, a.lddy, 0, s);
     const CUtensorMap mx = tma_map(X.matrix(), 1, a.M, a.K, 64), my = tma_map(Y.matrix(), 1, a.M, a.N, 64);
     const WeightTc<O> g{a.M, a.K, a.N, a.types, w.tiles_k, w.tiles_n, w.slots, w.longest, a.offsets, a.dW, a.lddw, a.stride_dw,
                         store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O)), w.part, w.ldp};
@@ -457,47 +391,52 @@ void typed_weight_tma(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream
     }
 }
 
-// 2 M K N above which 16-bit operands that TMA cannot read are worth an
-// aligned copy, and dW's operands a kernel that does not add up db on the way.
+// 2 M K N above which dW's 16-bit operands go by TMA, and db in kernels of its
+// own: 16,384 x 512 x 512 bf16 without db, 26.9 by TMA and 29.7 us by loaders;
+// 8,192 x 512 x 512 23.9 and 20.8 (and db's two kernels take 8 us more).
 constexpr double kLargeFlops = 1e10;
 
 }  // namespace
 
+// Few rows: measured against the tile kernels (bf16, 64 types and one, K = N),
+//   forward   1,024: 8 rows 7.2 against 12.3 us, 32 rows 9.7 against 20.9, 64
+//             rows of one type 15.9 against 9.3; 256: 5.9 against 6.9
+//   dX        1,024: 4 rows 9.5 against 10.0, 8 rows 16.5 against 12.5; 256: 16
+//             rows 5.5 against 6.4, 32 rows 8.9 against 6.9
+//   dW        8 rows of one type 9.8 against 9.9, 16 rows 17.6 against 9.9; 64
+//             rows over 64 types 48 against 93
+bool few_rows(int64_t M, int64_t K, int64_t N, bool trans) {
+    return trans ? M <= 4 || (M <= kFewRows && M * K * N <= 1 << 20) : M <= kFewRows;
+}
+
 template <class T, bool TRANS>
 void typed_rows(const RowsArgs<T>& a, cudaStream_t s) {
-    if (a.M <= kFewRows) {
-        typed_rows_few<T, TRANS>(a, s);
-        return;
-    }
-    if constexpr (sizeof(T) == 2) {
-        const bool readable = Operand<T>::readable(1, a.A, a.lda, 0) &&
-                              Operand<T>::readable(a.types, a.W, a.ldw, a.stride_w);
-        if (readable || 2.0 * a.M * a.K * a.N > kLargeFlops) {
-            typed_rows_tma<T, TRANS>(a, s);
-            return;
-        }
-    }
-    typed_rows_any<T, TRANS>(a, s);
+    if (few_rows(a.M, a.K, a.N, TRANS)) typed_rows_few<T, TRANS>(a, s);
+    else if constexpr (sizeof(T) == 2) typed_rows_tma<T, TRANS>(a, s);
+    else typed_rows_any<T, TRANS>(a, s);
 }
 
 template <class T, class O>
 void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
-    if (a.M <= kFewRows) {  // none among them: dW and db are zero
+    if (a.M <= 8 || a.M <= a.types) {  // no rows: dW and db are zero
         typed_weight_few<T, O>(a, s);
         return;
     }
-    const bool large = sizeof(T) == 2 && 2.0 * a.M * a.K * a.N > kLargeFlops;
+    // by TMA; the rows that only a copy makes readable are worth it at any size
+    // (8,192 x 511 x 513 bf16: 43 us, and 257 by loaders that take any alignment)
+    const bool by_tma = sizeof(T) == 2 && (2.0 * a.M * a.K * a.N > kLargeFlops ||
+                                           !(a.saved.codes || in_place(1, a.K, a.X, a.ldx, 0)) ||
+                                           !in_place(1, a.N, a.dY, a.lddy, 0));
     WeightPlan w{};
-    const int widest = large ? 256 : 128;
+    const int widest = by_tma ? 256 : 128;
     w.BN = a.N <= 64 ? 64 : (a.N <= 128 || widest == 128 ? 128 : 256);
-    w.pairs = large && a.K > 128 && a.N > 128;
-    w.tiles_k = static_cast<int>(ceil_div(a.K, w.pairs ? 2 * BM : BM));
+    w.tiles_k = static_cast<int>(ceil_div(a.K, BM));
     w.tiles_n = static_cast<int>(ceil_div(a.N, w.BN));
     const int64_t per = int64_t(w.tiles_k) * w.tiles_n;
-    w.slots = w.pairs ? num_sms() / 2 : num_sms();
+    w.slots = num_sms();
     // A type is cut where it has more than an SM's share: at most slots / per
     // pieces and one a type.
-    w.longest = large && sizeof(O) == 4 ? 64 : 1 << 30;
+    w.longest = by_tma && sizeof(O) == 4 ? 64 : 1 << 30;
     const int64_t used = std::min<int64_t>(a.types, a.M);
     const int64_t pieces = std::max<int64_t>(w.slots / per, a.M / (int64_t(w.longest) * kStep)) + used;
     w.items = std::max<int64_t>(pieces * per, std::min(a.types, num_sms()));
@@ -509,7 +448,7 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     w.db_part = part.p + (joined ? pieces * a.K * w.ldp : 0);
     bool done = false;
     if constexpr (sizeof(T) == 2) {
-        if (large) {
+        if (by_tma) {
             if (a.db) typed_bias<T>(a.M, a.N, a.types, a.offsets, a.dY, a.lddy, a.db, s);
             typed_weight_tma<T, O>(a, w, s);
             done = true;
@@ -518,13 +457,13 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     if (!done) typed_weight_any<T, O>(a, w, s);
     if (joined) {
         const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots, w.longest,
-                            piece_limit(a.M / kStep, static_cast<int>(per), w.slots, w.longest), a.offsets, w.part, w.db_part, a.dW, a.lddw, a.stride_dw,
-                            large ? nullptr : a.db};
+                            piece_limit(a.M / kStep, static_cast<int>(per), w.slots, w.longest), a.offsets, w.part,
+                            w.db_part, a.dW, a.lddw, a.stride_dw, by_tma ? nullptr : a.db};
         const int64_t want = ceil_div(a.K * std::min<int64_t>(w.ldp / 4, 256), 256);
         launch_dependent("typed_weight_join", typed_weight_join_kernel<O>,
-               dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(1, 8 * num_sms() / a.types))),
-                    static_cast<unsigned>(a.types)),
-               dim3(256), 0, s, j);
+                         dim3(static_cast<unsigned>(std::min<int64_t>(want, std::max(1, 8 * num_sms() / a.types))),
+                              static_cast<unsigned>(a.types)),
+                         dim3(256), 0, s, j);
     }
 }
 
