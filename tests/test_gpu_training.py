@@ -408,6 +408,37 @@ def test_typed_single_rows(tg, dtype):
         assert_product(tg.typed_linear_grad_input(dy, w, off), dx, mag, N, dtype, "dx")
 
 
+LONG = [  # sizes of the types, K, N: sums of more than one part, forward and for dX; limits between few rows and tiles
+    ([40, 0, 90], 1700, 72),
+    ([40, 0, 90], 1699, 41),
+    ([130, 1, 70], 72, 1604),
+    ([33, 64], 770, 1537),
+    ([0, 17, 0], 801, 130),
+    ([0, 31, 1, 0], 200, 1000),
+    ([16, 17, 18], 1024, 1024),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_typed_long_sums(tg, dtype, case):
+    """Long inner lengths: fp32 products add several parts in the output."""
+    sizes, K, N = LONG[case]
+    x, dy, w, bias, off = typed_inputs(sizes, K, N, dtype)
+    z = torch.cat([x[a:b].double() @ w[t].double() + bias[t].double() for t, a, b in spans(sizes)])
+    mag = torch.cat([x[a:b].double().abs() @ w[t].double().abs() + bias[t].double().abs() for t, a, b in spans(sizes)])
+    assert_product(tg.typed_linear(x, w, off, bias), z, mag, K, dtype, "y")
+    y, s = tg.typed_linear(x, w, off, bias, "elu", 0.5, save8=True)
+    assert torch.equal(y, tg.typed_linear(x, w, off, bias, "elu", 0.5))
+    err = (K + 16) * 2.0 ** -23 * mag
+    ref = act64(z, "elu", 0.5)
+    assert_within(y, ref, U[dtype] * ref.abs() + err * 1.2 + 2.0 ** -20 + TINY[dtype], "elu(y)")
+    assert_within(s.restore(torch.float32), z, 0.5 * torch.exp2(spread(s.exponents.double() - 127, N)) + err, "saved")
+    dx = torch.cat([dy[a:b].double() @ w[t].double().T for t, a, b in spans(sizes)])
+    mag = torch.cat([dy[a:b].double().abs() @ w[t].double().abs().T for t, a, b in spans(sizes)])
+    assert_product(tg.typed_linear_grad_input(dy, w, off), dx, mag, N, dtype, "dx")
+
+
 def test_typed_rows_of_other_types_do_not_leak(tg):
     """NaN and infinity in one type's rows and weight stay there."""
     for dtype in DTYPES:
@@ -581,6 +612,49 @@ def test_operators_capture_into_a_graph(tg):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_example_trains_and_8_bits_keep_up(tg):
+    """examples/train_typed_block.py: the loss falls, and with the saved activations in 8 bits it follows the run that
+    keeps them whole (each step's gradients are perturbed by about 1 %)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_typed_block.py")
+    spec = importlib.util.spec_from_file_location("train_typed_block", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    kept = example.train(nodes=3000, width=96, types=5, steps=25, save8=True, report=None)
+    whole = example.train(nodes=3000, width=96, types=5, steps=25, save8=False, report=None)
+    assert kept[-1] < 0.8 * kept[0] and whole[-1] < 0.8 * whole[0]
+    assert abs(kept[-1] - whole[-1]) < 0.05 * whole[-1]
+
+
+def test_block_gradients_against_the_whole_formula(tg):
+    """The example's block, fp32, against automatic differentiation in 64 bits."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_typed_block.py")
+    spec = importlib.util.spec_from_file_location("train_typed_block", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    sizes = [40, 0, 90]
+    block = example.TypedBlock(3, 64, 128, dtype=torch.float32, save8=False, seed=3)
+    x, dy, off = rand(130, 64, seed=1), rand(130, 64, seed=2), offsets_of(sizes)
+    y, kept = block.forward(x, off)
+    dx, grads = block.backward(dy, kept)
+    p = {k: v.double().requires_grad_(True) for k, v in block.params.items()}
+    xd = x.double().requires_grad_(True)
+    h, _, _ = norm64(xd, 1e-5)
+    n = h * p["gamma"] + p["beta"]
+    out = torch.cat([xd[a:b] + act64(n[a:b] @ p["w1"][t] + p["b1"][t], "gelu", 0.0) @ p["w2"][t] + p["b2"][t]
+                     for t, a, b in spans(sizes)])
+    out.backward(dy.double())
+    # a chain of two products of 64 and 128 terms and a norm: 2^-23 (8 + sqrt K) each of their terms' norm, which is
+    # within a factor of 8 of the result's for these inputs of random sign
+    tol = 8 * 4 * 2.0 ** -23 * (8 + math.sqrt(128))
+    for name, got, want in (("y", y, out.detach()), ("dx", dx, xd.grad), *((k, grads[k], p[k].grad) for k in grads)):
+        off_by = float((got.double() - want).norm() / want.norm())
+        assert off_by <= tol, f"{name}: {off_by}"
 
 
 def test_refusals(tg):
