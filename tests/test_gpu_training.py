@@ -564,6 +564,25 @@ def test_typed_offsets_out_of_range_stay_inside(tg):
     assert tg.check_row_offsets(good, 90) is good
 
 
+def test_typed_offsets_that_overlap_stay_inside(tg):
+    """Types that own the same rows, or leave rows out: the partial sums stay within their buffers, and types whose rows
+    are their own (or owned twice) still get their gradients."""
+    M, K, N = 30000, 256, 384  # weight gradients by TMA (bf16), and by loaders (fp32)
+    for dtype, out in ((torch.bfloat16, torch.float32), (torch.bfloat16, None), (torch.float32, None)):
+        x, dy, w, bias, _ = typed_inputs([M] + [0] * 31, K, N, dtype)
+        twice = torch.tensor([0, M] * 16 + [0], dtype=torch.int32, device="cuda")
+        assert tg.typed_linear(x, w, twice, bias).shape == (M, N)
+        dx, dw, db = tg.typed_linear_backward(dy, x, w, twice, dtype=out)
+        part = offsets_of([1000] + [0] * 30 + [500])  # rows from 1500 on are no type's
+        _, dw, db = tg.typed_linear_backward(dy, x, w, part, dtype=out)
+        for t, a, b in ((0, 0, 1000), (31, 1000, 1500)):
+            xd, dyd = x[a:b].double(), dy[a:b].double()
+            assert_product(dw[t], xd.T @ dyd, xd.abs().T @ dyd.abs(), b - a, dw.dtype, f"dw[{t}]")
+            assert_within(db[t], dyd.sum(0), (b - a + 16) * 2.0 ** -24 * dyd.abs().sum(0), f"db[{t}]")
+        assert dw[1:31].eq(0).all() and db[1:31].eq(0).all()
+    torch.cuda.synchronize()
+
+
 # ── streams, graphs, refusals ────────────────────────────────────────────────
 def _everything(tg, x, dy, gamma, beta, w, w2, off):
     y, stats, h8 = tg.layer_norm(x, gamma, beta, save8=True)

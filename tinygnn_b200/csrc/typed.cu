@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) typed_bias_kernel(int64_t M, int64_t N, i
 }
 
 __global__ void __launch_bounds__(256) typed_bias_join_kernel(int64_t M, int64_t N, const int32_t* offsets,
-                                                              const float* part, float* db) {
+                                                              const float* part, int chunks, float* db) {
     __shared__ int prefix[kMaxTypes + 1];
     __shared__ float sh[8][33];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32, t = blockIdx.y;
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256) typed_bias_join_kernel(int64_t M, int64_t
     float sum = 0.0f;
     if (n < N) {
 #pragma unroll 4
-        for (int p = prefix[t] + w; p < prefix[t + 1]; p += 8) sum += part[p * N + n];
+        for (int p = prefix[t] + w; p < (prefix[t + 1] < chunks ? prefix[t + 1] : chunks); p += 8) sum += part[p * N + n];
     }
     sh[w][lane] = sum;
     __syncthreads();
@@ -128,7 +128,7 @@ void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T
            offsets, dY, lddy, part.p);
     launch_dependent("typed_linear_grad_bias", typed_bias_join_kernel,
            dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0, s, M, N, offsets,
-           part.p, db);
+           part.p, static_cast<int>(chunks), db);
 }
 
 template void typed_bias<__nv_bfloat16>(int64_t, int64_t, int, const int32_t*, const __nv_bfloat16*, int64_t, float*,

@@ -3,6 +3,8 @@
 // ============================================================================
 #pragma once
 
+#include <algorithm>
+
 #include "values.cuh"
 
 namespace tg {
@@ -112,10 +114,20 @@ __device__ __forceinline__ int rows_of(const int32_t* offsets, int t, int64_t M)
 }
 // Rows of the longest piece, from the sum of all types' steps.  `longest`: the
 // steps that a sum may take (kernels that cannot add up parts of it themselves,
-// where the result is fp32).
-__host__ __device__ __forceinline__ int64_t piece_limit(int64_t steps, int per, int slots, int longest) {
+// where the result is fp32).  Offsets that leave rows out or own rows twice
+// keep within the same bounds: a type of at most the limit for M / 64 steps is
+// never cut, and there are at most max_pieces().
+__host__ __device__ __forceinline__ int64_t piece_limit(int64_t steps, int64_t M, int types, int per, int slots,
+                                                        int longest) {
+    if (steps < M / kStep) steps = M / kStep;
+    if (steps > M / kStep + types) longest = 1 << 30;
     const int64_t share = (steps * per * 5 + slots * 4 - 1) / (slots * 4);
     return (share < 2 ? 2 : (share < longest ? share : longest)) * kStep;
+}
+// A type of n rows has fewer than n / limit + 1 pieces, and a limit is at least
+// 5/4 of slots / per equal shares of the rows, or `longest` steps.
+inline int64_t max_pieces(int64_t M, int types, int64_t per, int slots, int longest) {
+    return types + std::max<int64_t>(slots / per, (M / kStep + types) / longest + 1);
 }
 __device__ __forceinline__ int piece_count(int n, int64_t limit) { return static_cast<int>((n + limit - 1) / limit); }
 // Rows of each piece (the last may have fewer; none is empty, since this is at most `limit`).
@@ -135,7 +147,7 @@ __device__ __forceinline__ void plan_pieces(const int32_t* offsets, int types, i
     for (int t = lane; t < types; t += 32) steps += (rows_of(offsets, t, M) + kStep - 1) / kStep;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, o);
-    const int64_t limit = piece_limit(steps, per, slots, longest);
+    const int64_t limit = piece_limit(steps, M, types, per, slots, longest);
     if (types > kSortTypes) {
         for (int t = lane; t < types; t += 32) order[t] = static_cast<uint16_t>(t);
     } else {

@@ -264,7 +264,7 @@ template <class O>
 struct JoinArgs {
     int64_t M, K, N, ldp;
     int types, per, slots, longest;
-    int64_t least;  // no type of fewer rows is cut (the limit when no step is ragged)
+    int64_t least;  // no type of at most as many rows is cut (the limit when no step is ragged)
     const int32_t* offsets;
     const float *part, *db_part;
     O* dW;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O
     };
     int64_t steps = 0;
     for (int u = threadIdx.x; u < g.types; u += 256) steps += (rows_of(g.offsets, u, g.M) + kStep - 1) / kStep;
-    const int64_t limit = piece_limit(block_sum(steps, sums), g.per, g.slots, g.longest);
+    const int64_t limit = piece_limit(block_sum(steps, sums), g.M, g.types, g.per, g.slots, g.longest);
     const int n = piece_count(rows, limit);
     if (n <= 1) return;  // the weight kernel wrote it
     // this type's first piece
@@ -434,11 +434,8 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     w.tiles_n = static_cast<int>(ceil_div(a.N, w.BN));
     const int64_t per = int64_t(w.tiles_k) * w.tiles_n;
     w.slots = num_sms();
-    // A type is cut where it has more than an SM's share: at most slots / per
-    // pieces and one a type.
     w.longest = by_tma && sizeof(O) == 4 ? 64 : 1 << 30;
-    const int64_t used = std::min<int64_t>(a.types, a.M);
-    const int64_t pieces = std::max<int64_t>(w.slots / per, a.M / (int64_t(w.longest) * kStep)) + used;
+    const int64_t pieces = max_pieces(a.M, a.types, per, w.slots, w.longest);
     w.items = std::max<int64_t>(pieces * per, std::min(a.types, num_sms()));
     w.ldp = (a.N + 7) / 8 * 8;
     // None is, if even all the rows in one type are an SM's share or two steps.
@@ -457,7 +454,7 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     if (!done) typed_weight_any<T, O>(a, w, s);
     if (joined) {
         const JoinArgs<O> j{a.M, a.K, a.N, w.ldp, a.types, static_cast<int>(per), w.slots, w.longest,
-                            piece_limit(a.M / kStep, static_cast<int>(per), w.slots, w.longest), a.offsets, w.part,
+                            piece_limit(a.M / kStep, a.M, a.types, static_cast<int>(per), w.slots, w.longest), a.offsets, w.part,
                             w.db_part, a.dW, a.lddw, a.stride_dw, by_tma ? nullptr : a.db};
         const int64_t want = ceil_div(a.K * std::min<int64_t>(w.ldp / 4, 256), 256);
         launch_dependent("typed_weight_join", typed_weight_join_kernel<O>,
