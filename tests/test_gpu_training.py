@@ -191,8 +191,8 @@ def test_activation_extremes(tg):
 
 
 # ── layer norm ───────────────────────────────────────────────────────────────
-WIDTHS = [1, 2, 7, 16, 31, 32, 33, 64, 128, 129, 200, 256, 257, 602, 1000, 1024, 1025, 2048, 4096, 4099, 8192, 8193,
-          20000]
+WIDTHS = [1, 2, 7, 16, 31, 32, 33, 64, 128, 129, 200, 256, 257, 602, 1000, 1024, 1025, 1280, 2048, 2560, 4096,
+          4099, 4104, 5119, 5120, 5128, 8192, 8193, 20000]
 
 
 def norm_slack(x, cols):

@@ -9,8 +9,8 @@
 //  The forward pass keeps (mu, r) of each row in fp32 and, if asked, h in 8
 //  bits (values.cuh); the backward pass takes x or that copy.  Both read each
 //  operand once and write each result once: a row stays in the registers of
-//  the TPR threads that share it (4 threads for 32 columns up to 512 threads
-//  for 8192), so the variance is a second pass over registers, not memory.
+//  the TPR threads that share it (4 threads for 32 columns up to 256 for 8192,
+//  512 in the gradient), so the variance is a second pass over registers, not memory.
 //  The bound is HBM.  Rows wider than 8192 columns are walked three times by
 //  one block each (the second and third walk come from L2).
 //
@@ -34,7 +34,7 @@ struct NormArgs {
 };
 
 // The part of a row that one of TPR threads holds: N slots of V neighbouring
-// values, 16 bytes (ALIGNED: one access).  A block of 128
+// values, 16 bytes (ALIGNED: one access, and no row ends inside a slot).  A block of 128
 // columns lies in one slot of 128 / V neighbouring lanes, so its largest
 // magnitude is a shuffle reduction (ROW_IS_BLOCK: the TPR lanes of a row of at
 // most 128 columns, and all their slots).
@@ -42,6 +42,7 @@ template <class T, bool ALIGNED, int TPR, int VPT>
 struct RowPart {
     static constexpr int V = 16 / static_cast<int>(sizeof(T));
     static constexpr int N = VPT / V;
+    static constexpr bool kAligned = ALIGNED;
     static constexpr int W = TPR < 32 ? TPR : 32;
     static constexpr bool ROW_IS_BLOCK = TPR * V < kBlock8;
     static constexpr int G = ROW_IS_BLOCK ? TPR : kBlock8 / V;
@@ -53,23 +54,31 @@ struct RowPart {
     __device__ __forceinline__ bool has(int i, int j) const { return col(i, j) < cols; }
     // Slot i exists for some thread of the warp (the same answer for all of them).
     __device__ __forceinline__ bool any(int i) const { return (i * TPR + t / W * W) * V < cols; }
-    // The thread's slot i is all there.
-    __device__ __forceinline__ bool whole(int i) const { return col(i, V - 1) < cols; }
+    // Slot i is all there for every thread of the warp's rows (the same answer
+    // for all of them: a warp does not do both the whole and the ragged form).
+    __device__ __forceinline__ bool whole(int i) const { return (i * TPR + t / W * W + W) * V <= cols; }
+    // How many values of slot i the row has (may be more than V, or negative).
+    __device__ __forceinline__ int left(int i) const { return cols - col(i, 0); }
 
     // The row's slots (zeros where there is nothing; `live` false: all zeros).
     using Slot = Held<T, V, ALIGNED>;
     __device__ __forceinline__ void fetch(const T* p, bool live, Slot (&k)[N]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (live && whole(i)) k[i].fetch(p + col(i, 0));
-            else if (live && has(i, 0)) k[i].fetch(p + col(i, 0), cols - col(i, 0));
+            if (live && (ALIGNED ? has(i, 0) : whole(i))) k[i].fetch(p + col(i, 0));
+            else if (!ALIGNED && live && any(i)) k[i].fetch(p + col(i, 0), left(i));
             else k[i].zero();
         }
+    }
+    // Slot i of row p, fetched: zeros past the row's end.
+    __device__ __forceinline__ void values(const Slot& k, const T* p, int i, float (&x)[V]) const {
+        if (ALIGNED || whole(i)) k.values(Slot::odd(p), x);
+        else k.values(Slot::odd(p), x, left(i));
     }
     // A slot of gamma or beta.
     template <class P>
     __device__ __forceinline__ void load(const P* p, int i, float (&x)[V]) const {
-        if (whole(i) && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+        if (ALIGNED ? has(i, 0) : whole(i) && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
             if constexpr (V * sizeof(P) <= 16) {
                 load_v<P, V>(p + col(i, 0), x);
             } else {
@@ -79,19 +88,22 @@ struct RowPart {
                     x[j] = q.x, x[j + 1] = q.y, x[j + 2] = q.z, x[j + 3] = q.w;
                 }
             }
-        } else {
+        } else if (ALIGNED) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = has(i, j) ? to_f32(p[col(i, j)]) : 0.0f;
+            for (int j = 0; j < V; ++j) x[j] = 0.0f;
+        } else {
+            Held<P, V, false> k;
+            k.fetch(p + col(i, 0), left(i));
+            k.values(k.odd(p), x, left(i));
         }
     }
     __device__ __forceinline__ void store(T* p, int i, const float (&x)[V]) const {
-        if (whole(i)) {
-            if constexpr (ALIGNED) store_v<T, V>(p + col(i, 0), x);
-            else store_any<T, V>(p + col(i, 0), x);
+        if constexpr (ALIGNED) {
+            if (has(i, 0)) store_v<T, V>(p + col(i, 0), x);
+        } else if (whole(i)) {
+            store_any<T, V>(p + col(i, 0), x);
         } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (has(i, j)) p[col(i, j)] = from_f32<T>(x[j]);
+            store_some<T, V>(p + col(i, 0), x, left(i));
         }
     }
 };
@@ -112,7 +124,10 @@ __device__ __forceinline__ void row_sum(float (&x)[S], float* red) {
         // each warp adds up the row's warps, one a lane
         const float* mine = red + threadIdx.x / TPR * NW * S;
 #pragma unroll
-        for (int k = 0; k < S; ++k) x[k] = reduce_sum<float, NW>(mine[lane % NW * S + k]);
+        for (int k = 0; k < S; ++k) {
+            constexpr int P = NW <= 2 ? 2 : (NW <= 4 ? 4 : (NW <= 8 ? 8 : 16));
+            x[k] = reduce_sum<float, P>(lane % P < NW ? mine[lane % P * S + k] : 0.0f);
+        }
     }
 }
 
@@ -124,7 +139,7 @@ constexpr int block_threads() { return TPR < 128 ? 128 : TPR; }
 template <int TPR, int VPT>
 constexpr int resident() { return VPT > 16 ? 512 / block_threads<TPR>() : (TPR >= 256 ? 1024 / TPR : (VPT > 8 ? 5 : 8)); }
 template <int TPR, int VPT>
-constexpr int resident_grad() { return TPR >= 256 ? 512 / TPR : (VPT > 8 ? 4 : 5); }
+constexpr int resident_grad() { return TPR == 320 ? 2 : TPR >= 256 ? 512 / TPR : (VPT > 8 ? 4 : 5); }
 
 // How many of its next rows a group of threads has asked for: as many as keep
 // about 16 KB of loads in flight a SM (one row at a time left HBM at 45 %).
@@ -182,7 +197,7 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident<TPR, VPT>()) no
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (!part.any(i)) break;
-                ring[d][i].values(R::Slot::odd(x + row * ldx), v[i]);
+                part.values(ring[d][i], x + row * ldx, i, v[i]);
 #pragma unroll
                 for (int j = 0; j < V; ++j) sum[0] += v[i][j];
             }
@@ -232,12 +247,10 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident<TPR, VPT>()) no
                     const int byte = exponent8(reduce_max<R::G>(m), a.r8.emin);
                     const float inv = encode8(byte);
                     if (!live) {
-                    } else if (part.whole(i)) {
+                    } else if (ALIGNED ? part.has(i, 0) : part.whole(i)) {
                         store_codes<V>(codes + part.col(i, 0), v[i], inv, byte, a.r8.top);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < V; ++j)
-                            if (part.has(i, j)) codes[part.col(i, j)] = code8(v[i][j], inv, byte, a.r8.top);
+                    } else if (!ALIGNED) {
+                        store_codes<V>(codes + part.col(i, 0), v[i], inv, byte, a.r8.top, part.left(i));
                     }
                     // the first lane of the group that holds the block writes its exponent
                     if (live && part.t % R::G == 0 && (i == 0 || !R::ROW_IS_BLOCK) && part.has(i, 0))
@@ -260,16 +273,10 @@ __device__ __forceinline__ void fetch_codes(const R& part, const int8_t* codes, 
                                             Raw<int8_t, R::V> (&k)[R::N], int (&e)[R::N]) {
 #pragma unroll
     for (int i = 0; i < R::N; ++i) {
-        e[i] = 127;
-        if (!part.any(i)) {
-            k[i] = gather_codes<R::V>([](int) { return int8_t(0); });
-            continue;
-        }
-        if (live && part.has(i, 0)) e[i] = exps[part.col(i, 0) / kBlock8];
-        if (live && part.whole(i))
+        e[i] = live && part.has(i, 0) ? exps[part.col(i, 0) / kBlock8] : 127;
+        if (live && (R::kAligned ? part.has(i, 0) : part.whole(i)))
             k[i] = *reinterpret_cast<const Raw<int8_t, R::V>*>(codes + part.col(i, 0));
-        else
-            k[i] = gather_codes<R::V>([&](int j) { return live && part.has(i, j) ? codes[part.col(i, j)] : int8_t(0); });
+        else k[i] = load_codes<R::V>(codes + part.col(i, 0), live && !R::kAligned ? part.left(i) : 0);
     }
 }
 
@@ -322,7 +329,7 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
 #pragma unroll
                     for (int j = 0; j < V; j += 4) values4(kc[SAVED ? d : 0][i].w[j / 4], ke[SAVED ? d : 0][i], &h[i][j]);
                 } else {
-                    kx[SAVED ? 0 : d][i].values(R::Slot::odd(x + row * ldx), h[i]);
+                    part.values(kx[SAVED ? 0 : d][i], x + row * ldx, i, h[i]);
 #pragma unroll
                     for (int j = 0; j < V; ++j) h[i][j] = __fmul_rn(__fsub_rn(h[i][j], mean), rstd);
                     if (!part.whole(i)) {
@@ -330,7 +337,7 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
                         for (int j = 0; j < V; ++j) h[i][j] = part.has(i, j) ? h[i][j] : 0.0f;
                     }
                 }
-                kd[d][i].values(R::Slot::odd(dy + row * lddy), g[i]);
+                part.values(kd[d][i], dy + row * lddy, i, g[i]);
             }
             fetch(d, row + D * step);
             float sum[2] = {0.0f, 0.0f};
@@ -517,18 +524,29 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const float* part, int 
 
 constexpr int64_t kRegisterCols = 8192;
 
-// Calls f(TPR, VPT) with the row split for `cols` columns.
+// Calls f(TPR, VPT) with the row split for `cols` columns.  The steps double up
+// to 4,096 columns; from there a row is a block, and a step that leaves half
+// the threads without a value halves the rows in flight: 8,191 x 4,099 fp16
+// with the 8-bit copy, forward 119 us by 256 threads and 98 by 160, gradient
+// 154 by 512 and 136 by 320 (two blocks a SM).
 template <class F>
-void by_width(int64_t cols, F&& f) {
+void by_width_narrow(int64_t cols, F&& f) {
     using std::integral_constant;
     if (cols <= 32) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     else if (cols <= 64) f(integral_constant<int, 4>{}, integral_constant<int, 16>{});
     else if (cols <= 128) f(integral_constant<int, 8>{}, integral_constant<int, 16>{});
     else if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    else if (cols <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+}
+
+template <class F>
+void by_width_grad(int64_t cols, F&& f) {
+    using std::integral_constant;
+    if (cols <= 512) by_width_narrow(cols, f);
     else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
     else if (cols <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
     else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+    else if (cols <= 5120) f(integral_constant<int, 320>{}, integral_constant<int, 16>{});
     else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
 }
 
@@ -537,10 +555,11 @@ void by_width(int64_t cols, F&& f) {
 template <class F>
 void by_width_forward(int64_t cols, F&& f) {
     using std::integral_constant;
-    if (cols <= 512) by_width(cols, f);
+    if (cols <= 512) by_width_narrow(cols, f);
     else if (cols <= 1024) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
     else if (cols <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
     else if (cols <= 4096) f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
+    else if (cols <= 5120) f(integral_constant<int, 160>{}, integral_constant<int, 32>{});
     else f(integral_constant<int, 256>{}, integral_constant<int, 32>{});
 }
 
@@ -603,7 +622,10 @@ TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const 
                        dim3(512), 0, as_stream(stream), a, xp, ldx, gp, bp, yp, ldy, st, s);
                 return;
             }
-            const bool al = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(y, ldy, sizeof(T)) &&
+            // (8,191 x 4,096 fp16 with the 8-bit copy: 43 us, 55 with the code
+            // for rows that end inside a slot, 68 where no row is aligned)
+            const bool al = cols * sizeof(T) % 16 == 0 && rows_aligned16(x, ldx, sizeof(T)) &&
+                            rows_aligned16(y, ldy, sizeof(T)) &&
                             rows_aligned16(gamma, 0, 1) && rows_aligned16(beta, 0, 1);
             by_width_forward(cols, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
@@ -669,9 +691,10 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
                 join(part.p);
                 return;
             }
-            const bool al = rows_aligned16(dy, lddy, sizeof(T)) && (codes || rows_aligned16(x, ldx, sizeof(T))) &&
+            const bool al = cols * sizeof(T) % 16 == 0 && rows_aligned16(dy, lddy, sizeof(T)) &&
+                            (codes || rows_aligned16(x, ldx, sizeof(T))) &&
                             rows_aligned16(dx, lddx, sizeof(T)) && rows_aligned16(gamma, 0, 1);
-            by_width(cols, [&](auto tpr, auto vpt) {
+            by_width_grad(cols, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
                 constexpr int BT = block_threads<TPR>(), RPB = BT / TPR;
                 auto kern = codes ? (al ? norm_grad_kernel<T, P, true, TPR, VPT, true>

@@ -19,7 +19,7 @@ namespace tg {
 namespace {
 
 // Lane mapping of one block: G lanes, 16 bytes of neighbouring values each
-// (ALIGNED: one access).
+// (ALIGNED: one access, and no row ends inside a lane's).
 template <class T, bool ALIGNED>
 struct Lanes {
     static constexpr int V = 16 / static_cast<int>(sizeof(T));
@@ -34,39 +34,33 @@ struct Lanes {
         left = columns_left < kBlock8 ? static_cast<int>(columns_left) : kBlock8;
         full = (lane + 1) * V <= left;
     }
-    __device__ __forceinline__ int col(int j) const { return lane * V + j; }
     // Of the row whose block starts at p.
     __device__ __forceinline__ void load(const T* p, bool live, Held<T, V, ALIGNED>& k) const {
         if (full && live) k.fetch(p + lane * V);
-        else if (live && lane * V < left) k.fetch(p + lane * V, left - lane * V);
+        else if (!ALIGNED) k.fetch(p + lane * V, live ? left - lane * V : 0);
         else k.zero();
     }
     __device__ __forceinline__ void values(const Held<T, V, ALIGNED>& k, const T* p, float (&x)[V]) const {
-        k.values(k.odd(p + lane * V), x);
+        if (ALIGNED) k.values(false, x);
+        else k.values(k.odd(p + lane * V), x, left - lane * V);
     }
     __device__ __forceinline__ void store(T* p, const float (&x)[V]) const {
-        if (full) {
-            if constexpr (ALIGNED) store_v<T, V>(p + lane * V, x);
-            else store_any<T, V>(p + lane * V, x);
-            return;
+        if constexpr (ALIGNED) {
+            if (full) store_v<T, V>(p + lane * V, x);
+        } else if (full) {
+            store_any<T, V>(p + lane * V, x);
+        } else {
+            store_some<T, V>(p + lane * V, x, left - lane * V);
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (col(j) < left) p[col(j)] = from_f32<T>(x[j]);
     }
     __device__ __forceinline__ void save(int8_t* p, const float (&x)[V], int byte, int top) const {
         const float inv = encode8(byte);
-        if (full) {
-            store_codes<V>(p + lane * V, x, inv, byte, top);
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (col(j) < left) p[col(j)] = code8(x[j], inv, byte, top);
+        if (full) store_codes<V>(p + lane * V, x, inv, byte, top);
+        else if (!ALIGNED) store_codes<V>(p + lane * V, x, inv, byte, top, left - lane * V);
     }
-    __device__ __forceinline__ Raw<int8_t, V> load_codes(const int8_t* p, bool live) const {
+    __device__ __forceinline__ Raw<int8_t, V> codes(const int8_t* p, bool live) const {
         if (full && live) return *reinterpret_cast<const Raw<int8_t, V>*>(p + lane * V);
-        return gather_codes<V>([&](int j) { return col(j) < left && live ? p[col(j)] : int8_t(0); });
+        return load_codes<V>(p + lane * V, live && !ALIGNED ? left - lane * V : 0);
     }
     static __device__ __forceinline__ void values(const Raw<int8_t, V>& k, int byte, float (&x)[V]) {
 #pragma unroll
@@ -161,7 +155,7 @@ __global__ void __launch_bounds__(256) restore8_kernel(ActArgs a, Saved8 s, T* y
         for (int u = 0; u < U; ++u) {
             const int64_t r = row + u * w.step;
             const bool live = r < a.rows;
-            c[u] = l.load_codes(s.codes + (live ? r : row) * s.ld + c0, live);
+            c[u] = l.codes(s.codes + (live ? r : row) * s.ld + c0, live);
             e[u] = live ? s.exps[r * s.lde + w.b] : 0;
         }
 #pragma unroll
@@ -202,7 +196,7 @@ __global__ void __launch_bounds__(256, Lanes<T, ALIGNED>::kResident) act_grad_ke
             const bool live = row + u * w.step < a.rows;
             l.load(pg, live, g[u]);
             if (SAVED) {
-                c[SAVED ? u : 0] = l.load_codes(pc, live);
+                c[SAVED ? u : 0] = l.codes(pc, live);
                 e[u] = live ? *pe : 0;
                 pc += dc;
                 pe += de;
@@ -237,9 +231,10 @@ unsigned grid_for(int64_t rows, int64_t nb) {
     return static_cast<unsigned>(std::min(want, most));
 }
 
+// Rows that start, and end, at multiples of 16 bytes.
 template <class T>
-bool aligned(const void* p, int64_t ld) {
-    return p == nullptr || rows_aligned16(p, ld, sizeof(T));
+bool aligned(const void* p, int64_t ld, int64_t cols) {
+    return p == nullptr || (cols * sizeof(T) % 16 == 0 && rows_aligned16(p, ld, sizeof(T)));
 }
 
 }  // namespace
@@ -247,7 +242,7 @@ bool aligned(const void* p, int64_t ld) {
 template <class T>
 void restore8(int64_t rows, int64_t cols, const Saved8& s, T* y, int64_t ldy, cudaStream_t stream) {
     const ActArgs a{rows, cols, ceil_div(cols, kBlock8), TG_ACT_NONE, 0.0f, Range8{}};
-    const bool al = aligned<T>(y, ldy);
+    const bool al = aligned<T>(y, ldy, cols);
     const unsigned grid = al ? grid_for<Lanes<T, true>>(rows, a.nb) : grid_for<Lanes<T, false>>(rows, a.nb);
     launch_dependent("restore8", al ? restore8_kernel<T, true> : restore8_kernel<T, false>,
                      dim3(grid), dim3(256), 0, stream, a, s, y, ldy);
@@ -280,7 +275,7 @@ TG_API tg_status tg_save8(int64_t rows, int64_t cols, int32_t dtype, const void*
             using T = decltype(t);
             const T* xp = static_cast<const T*>(x);
             T* yp = static_cast<T*>(y);
-            const bool al = aligned<T>(x, ldx) && aligned<T>(y, ldy);
+            const bool al = aligned<T>(x, ldx, cols) && aligned<T>(y, ldy, cols);
             auto kern = save8_kernel<T, false, -1>;
             if (al) by_act(act, [&](auto k) { kern = save8_kernel<T, true, decltype(k)::value>; });
             const unsigned grid = al ? grid_for<Lanes<T, true>>(rows, a.nb) : grid_for<Lanes<T, false>>(rows, a.nb);
@@ -336,7 +331,7 @@ TG_API tg_status tg_activation_grad(int64_t rows, int64_t cols, int32_t dtype, c
             const T* dyp = static_cast<const T*>(dy);
             const T* xp = static_cast<const T*>(x);
             T* dxp = static_cast<T*>(dx);
-            const bool al = aligned<T>(dy, lddy) && aligned<T>(x, ldx) && aligned<T>(dx, lddx);
+            const bool al = aligned<T>(dy, lddy, cols) && aligned<T>(x, ldx, cols) && aligned<T>(dx, lddx, cols);
             auto kern = codes ? act_grad_kernel<T, false, true, -1> : act_grad_kernel<T, false, false, -1>;
             if (al)
                 by_act(act, [&](auto k) {

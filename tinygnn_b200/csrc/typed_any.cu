@@ -21,7 +21,13 @@
 //                 flight) while this stage's are converted and written;
 //    warp 8       the MMAs (one thread);
 //    warps 12-15  the epilogue of one of two TMEM accumulators while the next
-//                 tile is multiplied.
+//                 tile is multiplied (warps 9-11 only take part in the set-up:
+//                 a warp reads the TMEM lanes of its number modulo 4).
+//
+//  fp32 is bound by shared memory: a stage's MMAs read its planes at its full
+//  rate, and the loaders' conversions write beside them.  232,965 x 602 x 128
+//  forward takes 334 us, 0.11 PFLOP/s of fp32 products and six times that
+//  of MMAs (the tensor cores' measured rate would allow 126 us).
 // ============================================================================
 #include <type_traits>
 

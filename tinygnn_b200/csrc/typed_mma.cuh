@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(256) align_kernel(int64_t rows, int64_t cols, 
                 const int64_t c = c0 + u * 32 * V;
                 if (c >= ld) break;
                 float x[V];
-                h[u].values(odd, x);
+                h[u].values(odd, x, c < cols ? static_cast<int>(cols - c < V ? cols - c : V) : 0);
                 store_v<T, V>(dst + r * ld + c, x);
             }
         }
@@ -485,13 +485,16 @@ static int take_error() {
 }
 
 // Tile width of a product with N columns and `pieces` row tiles (or dW tiles):
-// the widest (it reads the rows fewest times) that still gives every SM a
-// tile, else the narrowest.  An exponent of a saved result needs its 128
-// columns in one tile.
+// the widest (it reads the rows fewest times) that still gives four of five
+// SMs a tile, else the narrowest.  Forward, 4 types, us for widths 64 / 128 /
+// 256 (tiles): bf16, K = N = 512: 4,096 rows 14.3 (288), 12.3 (144), 14.4 (72);
+// 8,192 rows 18.4, 16.4 (272), 14.3 (136); fp32: 2,048 rows 22.5 (160), 26.6
+// (80); 4,096 rows 34.8, 28.6 (144).  An exponent of a saved result needs its
+// 128 columns in one tile.
 inline int tile_width(int64_t pieces, int64_t N, int widest, bool saved) {
     const int least = saved && N > 64 ? 128 : 64;
     for (int w = widest; w > least; w /= 2)
-        if (N > w / 2 && pieces * ceil_div(N, w) >= num_sms()) return w;
+        if (N > w / 2 && 5 * pieces * ceil_div(N, w) >= 4 * num_sms()) return w;
     return least;
 }
 

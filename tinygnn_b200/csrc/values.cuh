@@ -26,8 +26,6 @@ namespace tg {
 constexpr int kBlock8 = 128;   // columns that share an exponent
 constexpr int kBad8 = 255;     // exponent byte of a block that held inf or NaN
 
-inline size_t dtype_size(int dtype) { return dtype == TG_F32 ? 4 : 2; }
-
 inline void check_dtype(const char* fn, const char* what, int dtype) {
     if (dtype != TG_F32 && dtype != TG_BF16 && dtype != TG_F16)
         invalid(std::string(fn) + ": " + what + " has no such type (" + std::to_string(dtype) + ")");
@@ -75,12 +73,6 @@ __device__ __forceinline__ Raw<T, V> gather_raw(F&& f) {
         else k.w[i] = bits(f(2 * i)) | bits(f(2 * i + 1)) << 16;
     }
     return k;
-}
-template <class T, int V, class F>  // f(j, value j)
-__device__ __forceinline__ void scatter_raw(const Raw<T, V>& k, F&& f) {
-    const T* v = reinterpret_cast<const T*>(k.w);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f(j, v[j]);
 }
 template <int V>
 __device__ __forceinline__ void widen(const Raw<float, V>& k, float* x) {
@@ -164,30 +156,34 @@ struct Held {
             w[V / 2] = odd(p) ? q[V / 2] : 0u;
         }
     }
-    // The first n values are there; zeros after them.
+    // The first n values (all, for more; none, for n <= 0) are there.  Whole
+    // words that hold one of them are read and kept as they are: values() with
+    // n clears the rest, since an instruction on a word here would wait for it
+    // (a layer norm that picked a row's last values out as it asked for the
+    // next rows took OLDFWD us for 65,536 x 511, and 33 for 512).
     __device__ __forceinline__ void fetch(const T* p, int n) {
-        const int shift = odd(p);
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < V * static_cast<int>(sizeof(T)) / 4 + kShift; ++j) {
-            if constexpr (sizeof(T) == 4) {
-                w[j] = j < n ? bits(p[j]) : 0u;
-            } else {
-                const int e = 2 * j - shift;
-                w[j] = (e >= 0 && e < n ? bits(p[e]) : 0u) | (e + 1 < n ? bits(p[e + 1]) : 0u) << 16;
-            }
+            for (int j = 0; j < V; ++j) w[j] = j < n ? bits(p[j]) : 0u;
+        } else {
+            const int shift = odd(p);
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+#pragma unroll
+            for (int j = 0; j < V / 2 + kShift; ++j) w[j] = n > 0 && 2 * j < (n < V ? n : V) + shift ? q[j] : 0u;
         }
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int j = 0; j < V * static_cast<int>(sizeof(T)) / 4 + kShift; ++j) w[j] = 0u;
     }
-    // odd: of the pointer they were fetched from.
-    __device__ __forceinline__ void values(bool odd, float* x) const {
+    // odd: of the pointer they were fetched from.  n: zeros after the first n.
+    __device__ __forceinline__ void values(bool odd, float* x, int n = V) const {
         Raw<T, V> k;
 #pragma unroll
         for (int j = 0; j < Raw<T, V>::N; ++j) {
             if constexpr (kShift) k.w[j] = odd ? __byte_perm(w[j], w[j + 1], 0x5432) : w[j];
             else k.w[j] = w[j];
+            if (sizeof(T) == 2 && 2 * j + 2 > n) k.w[j] = 2 * j + 1 == n ? k.w[j] & 0xffffu : 0u;
         }
         widen(k, x);
     }
@@ -210,6 +206,34 @@ __device__ __forceinline__ void store_any(T* p, const float (&x)[V]) {
     } else {
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) reinterpret_cast<uint32_t*>(p)[j] = k.w[j];
+    }
+}
+
+// The first n of V values (all, for more; none, for n <= 0).
+template <class T, int V>
+__device__ __forceinline__ void store_some(T* p, const float (&x)[V], int n) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < n) p[j] = x[j];
+    } else {
+        Raw<T, V> k;
+        narrow(x, k);
+        n = n < V ? n : V;
+        const int shift = (reinterpret_cast<uintptr_t>(p) >> 1) & 1;
+        uint16_t* q = reinterpret_cast<uint16_t*>(p);
+        if (shift && n > 0) q[0] = static_cast<uint16_t>(k.w[0]);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const uint32_t u = shift && j + 1 < V / 2 ? __byte_perm(k.w[j], k.w[j + 1 < V / 2 ? j + 1 : j], 0x5432) : k.w[j];
+            if (2 * j + 1 + shift < n) *reinterpret_cast<uint32_t*>(q + 2 * j + shift) = u;
+        }
+        if (n > shift && (n - shift) % 2) {  // the last value is alone in its word
+            uint32_t u = k.w[0];
+#pragma unroll
+            for (int j = 1; j < V / 2; ++j) u = (n - 1) / 2 == j ? k.w[j] : u;
+            q[n - 1] = static_cast<uint16_t>((n - 1) % 2 ? u >> 16 : u);
+        }
     }
 }
 
@@ -284,17 +308,6 @@ __device__ __forceinline__ void values4(uint32_t codes, int byte, float* x) {
         for (int j = 0; j < 4; ++j) x[j] = __fmul_rn(__fsub_rn(f[j], 8388736.0f), scale);
     }
 }
-// V codes (a multiple of 4), f(j) the byte j.
-template <int V, class F>
-__device__ __forceinline__ Raw<int8_t, V> gather_codes(F&& f) {
-    Raw<int8_t, V> k;
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-        const auto byte = [&](int j) { return static_cast<uint32_t>(static_cast<uint8_t>(f(4 * i + j))); };
-        k.w[i] = byte(0) | byte(1) << 8 | byte(2) << 16 | byte(3) << 24;
-    }
-    return k;
-}
 // V codes at p, aligned to V bytes.
 template <int V>
 __device__ __forceinline__ void store_codes(int8_t* p, const float* x, float inv, int byte, int top) {
@@ -302,6 +315,30 @@ __device__ __forceinline__ void store_codes(int8_t* p, const float* x, float inv
 #pragma unroll
     for (int j = 0; j < V / 4; ++j) k.w[j] = codes4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3], inv, byte, top);
     *reinterpret_cast<Raw<int8_t, V>*>(p) = k;
+}
+// The first n of them.
+template <int V>
+__device__ __forceinline__ void store_codes(int8_t* p, const float* x, float inv, int byte, int top, int n) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+        const uint32_t u = codes4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3], inv, byte, top);
+        if (4 * j + 4 <= n) {
+            *reinterpret_cast<uint32_t*>(p + 4 * j) = u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (4 * j + i < n) p[4 * j + i] = static_cast<int8_t>(u >> 8 * i & 0xff);
+        }
+    }
+}
+// The first n of V codes at p (all, for more); p is aligned to 4 bytes.  Whole
+// words that hold one of them are read: what follows the n is any code.
+template <int V>
+__device__ __forceinline__ Raw<int8_t, V> load_codes(const int8_t* p, int n) {
+    Raw<int8_t, V> k;
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) k.w[j] = 4 * j < n ? reinterpret_cast<const uint32_t*>(p)[j] : 0u;
+    return k;
 }
 
 // The least exponent of a block: 2^-126, or 2^-24 for fp16 matrices, whose
@@ -345,8 +382,8 @@ void restore8(int64_t rows, int64_t cols, const Saved8& s, T* y, int64_t ldy, cu
 // -1, and costs one exponential and one reciprocal.  FAST (for results of 16
 // bits) takes the hardware's exponential, whose error of 2^-19 or less here
 // is lost in the result's rounding of 2^-8 or 2^-11; with tanhf the 8-bit
-// activation passes were bound by arithmetic (0.52 ms for 131,072 x 1024
-// bf16, forward and backward).
+// activation passes were bound by arithmetic (131,072 x 1024 bf16, forward and
+// backward: 0.52 ms, and 0.29 with it).
 template <bool FAST>
 __device__ __forceinline__ float exp_f(float x) { return FAST ? __expf(x) : expf(x); }
 __device__ __forceinline__ float reciprocal(float x) {
