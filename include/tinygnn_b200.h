@@ -193,8 +193,8 @@ TG_API tg_status tg_add_bias_f32(float* X, int64_t rows, int64_t cols, int64_t l
  * the least exponent whose 127 * 2^e reaches the block's largest magnitude
  * (not below 2^-126, for fp16 matrices 2^-24) and codes rounded to nearest
  * even (at most 63 where 64 * 2^e would overflow the matrix's type), so that
- * fp32, bf16 and the matrix's own type hold every value.  Exponent 255 marks a block that held an infinity or a NaN: all its
- * values are NaN. */
+ * fp32, bf16 and the matrix's own type hold every value.  Exponent 255 marks
+ * a block that held an infinity or a NaN: all its values are NaN. */
 
 /* y = act(x) (y nullable: only save), and x in the saved form. */
 TG_API tg_status tg_save8(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ldx,
@@ -236,7 +236,10 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
  * offsets: types + 1 device integers, non-decreasing from 0 to rows (checked
  * by tg_typed_check_offsets, not here: a bound outside [0, rows] is clamped,
  * and rows of no type are not written).  codes and exponents (nullable)
- * receive the pre-activation in the saved form.  At most 1024 types. */
+ * receive the pre-activation in the saved form.  At most 1024 types.  fp32
+ * rows are multiplied on the tensor cores in three bf16 parts each (within
+ * fp32 tolerance; a row or column that holds an infinity gives NaN), a few
+ * rows in fp32; so are the gradients below. */
 TG_API tg_status tg_typed_linear(int64_t rows, int64_t K, int64_t N, int64_t types, int32_t dtype,
                                  const void* X, int64_t ldx, const void* W, int64_t ldw,
                                  int64_t stride_w, const int32_t* offsets, const float* bias,
