@@ -139,7 +139,7 @@ constexpr int block_threads() { return TPR < 128 ? 128 : TPR; }
 template <int TPR, int VPT>
 constexpr int resident() { return VPT > 16 ? 512 / block_threads<TPR>() : (TPR >= 256 ? 1024 / TPR : (VPT > 8 ? 5 : 8)); }
 template <int TPR, int VPT>
-constexpr int resident_grad() { return TPR == 320 ? 2 : TPR >= 256 ? 512 / TPR : (VPT > 8 ? 4 : 5); }
+constexpr int resident_grad() { return TPR >= 512 ? 1 : (TPR >= 256 ? 2 : (VPT > 8 ? 4 : 5)); }
 
 // How many of its next rows a group of threads has asked for: as many as keep
 // about 16 KB of loads in flight a SM (one row at a time left HBM at 45 %).
@@ -524,11 +524,13 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const float* part, int 
 
 constexpr int64_t kRegisterCols = 8192;
 
-// Calls f(TPR, VPT) with the row split for `cols` columns.  The steps double up
-// to 4,096 columns; from there a row is a block, and a step that leaves half
-// the threads without a value halves the rows in flight: 8,191 x 4,099 fp16
-// with the 8-bit copy, forward 119 us by 256 threads and 98 by 160, gradient
-// 154 by 512 and 136 by 320 (two blocks a SM).
+// Calls f(TPR, VPT) with the row split for `cols` columns.  The steps double;
+// above 4,096 columns, where a row is a block, there is one more at 5,120, which
+// leaves fewer threads without a value.  8,191 rows fp16, with the 8-bit copy:
+// forward by 160 threads 98 us for 4,099 columns, 53 for 4,104, by 256 131 and
+// 61.  The gradient from the copy, by 320 (two blocks a SM) 136 for 4,099, by
+// 512 148; from x 129 and 142; but aligned rows of 5,120 from x 99 and 88, so
+// there they stay with 512.
 template <class F>
 void by_width_narrow(int64_t cols, F&& f) {
     using std::integral_constant;
@@ -539,14 +541,16 @@ void by_width_narrow(int64_t cols, F&& f) {
     else f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
 }
 
+constexpr int kRaggedThreads = 320;
+
 template <class F>
-void by_width_grad(int64_t cols, F&& f) {
+void by_width_grad(int64_t cols, bool aligned, F&& f) {
     using std::integral_constant;
     if (cols <= 512) by_width_narrow(cols, f);
     else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
     else if (cols <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
     else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
-    else if (cols <= 5120) f(integral_constant<int, 320>{}, integral_constant<int, 16>{});
+    else if (cols <= 5120 && !aligned) f(integral_constant<int, kRaggedThreads>{}, integral_constant<int, 16>{});
     else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
 }
 
@@ -622,8 +626,8 @@ TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const 
                        dim3(512), 0, as_stream(stream), a, xp, ldx, gp, bp, yp, ldy, st, s);
                 return;
             }
-            // (8,191 x 4,096 fp16 with the 8-bit copy: 43 us, 55 with the code
-            // for rows that end inside a slot, 68 where no row is aligned)
+            // (8,191 x 4,096 fp16 with the 8-bit copy: 43 us; 59 with code for
+            // rows that end inside a slot, 69 where the rows are not aligned)
             const bool al = cols * sizeof(T) % 16 == 0 && rows_aligned16(x, ldx, sizeof(T)) &&
                             rows_aligned16(y, ldy, sizeof(T)) &&
                             rows_aligned16(gamma, 0, 1) && rows_aligned16(beta, 0, 1);
@@ -694,12 +698,13 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
             const bool al = cols * sizeof(T) % 16 == 0 && rows_aligned16(dy, lddy, sizeof(T)) &&
                             (codes || rows_aligned16(x, ldx, sizeof(T))) &&
                             rows_aligned16(dx, lddx, sizeof(T)) && rows_aligned16(gamma, 0, 1);
-            by_width_grad(cols, [&](auto tpr, auto vpt) {
+            by_width_grad(cols, al, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
                 constexpr int BT = block_threads<TPR>(), RPB = BT / TPR;
-                auto kern = codes ? (al ? norm_grad_kernel<T, P, true, TPR, VPT, true>
+                constexpr bool AL = TPR != kRaggedThreads;
+                auto kern = codes ? (al ? norm_grad_kernel<T, P, AL, TPR, VPT, true>
                                         : norm_grad_kernel<T, P, false, TPR, VPT, true>)
-                                  : (al ? norm_grad_kernel<T, P, true, TPR, VPT, false>
+                                  : (al ? norm_grad_kernel<T, P, AL, TPR, VPT, false>
                                         : norm_grad_kernel<T, P, false, TPR, VPT, false>);
                 parts = std::min<int64_t>(ceil_div(rows, RPB), int64_t(num_sms()) * resident_grad<TPR, VPT>());
                 Scratch<float> part(static_cast<size_t>(parts * 2 * cols), str);
