@@ -26,7 +26,7 @@
 //
 //  fp32 is bound by shared memory: a stage's MMAs read its planes at its full
 //  rate, and the loaders' conversions write beside them.  232,965 x 602 x 128
-//  forward takes 334 us, 0.11 PFLOP/s of fp32 products and six times that
+//  forward takes 334-341 us, 0.11 PFLOP/s of fp32 products and six times that
 //  of MMAs (the tensor cores' measured rate would allow 126 us).
 // ============================================================================
 #include <type_traits>
