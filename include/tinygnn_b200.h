@@ -214,8 +214,8 @@ TG_API tg_status tg_activation_grad(int64_t rows, int64_t cols, int32_t dtype, c
 /* y = h * gamma + beta with h = (x - mean) * rstd over the columns of each
  * row, rstd = 1 / sqrt(mean (x - mean)^2 + eps).  gamma and beta are fp32 or
  * of the rows' type (param_dtype).  stats[2 i], stats[2 i + 1] receive row
- * i's mean and rstd; codes and exponents (nullable) receive h in the saved
- * form. */
+ * i's mean and rstd; codes (nullable) and, with them, exponents receive h
+ * in the saved form. */
 TG_API tg_status tg_layer_norm(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ldx,
                                int32_t param_dtype, const void* gamma, const void* beta, float eps,
                                void* y, int64_t ldy, float* stats, int8_t* codes, int64_t ld_codes,
@@ -235,8 +235,8 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
  * W + t * stride_w (rows ldw apart); bias (nullable) is types x N, fp32.
  * offsets: types + 1 device integers, non-decreasing from 0 to rows (checked
  * by tg_typed_check_offsets, not here: a bound outside [0, rows] is clamped,
- * and rows of no type are not written).  codes and exponents (nullable)
- * receive the pre-activation in the saved form.  At most 1024 types.  fp32
+ * and rows of no type are not written).  codes (nullable) and, with them,
+ * exponents receive the pre-activation in the saved form.  At most 1024 types.  fp32
  * rows are multiplied on the tensor cores in three bf16 parts each (within
  * fp32 tolerance; a row or column that holds an infinity gives NaN), a few
  * rows in fp32; so are the gradients below. */

@@ -505,9 +505,11 @@ inline void check_rows_cols(const char* fn, int64_t rows, int64_t cols) {
                 " columns is outside [0, 2^31) x [1, 2^31)");
 }
 
+// Without codes (where they are not `needed`) nothing is saved; with them the
+// exponents have to be there too.
 inline void check_saved8(const char* fn, int64_t cols, const Saved8& s, bool needed) {
     check_ptr(fn, "codes", s.codes, needed);
-    check_ptr(fn, "exponents", s.exps, needed);
+    check_ptr(fn, "exponents", s.exps, needed || s.codes);
     if (!s.codes) return;
     check_ld(fn, "codes", s.ld, cols);
     check_ld(fn, "exponents", s.lde, ceil_div(cols, kBlock8));
