@@ -47,3 +47,22 @@ def test_codes_without_exponents_are_refused(tg):
         assert call() == _lib.INVALID_ARGUMENT, k
         assert "exponents is NULL" in _lib.last_error(), k
     assert lib.tg_kernel_launch_count() == before
+
+
+def test_layer_norm_gradient_of_large_constant_rows(tg):
+    """Rows whose mean times 1 / sqrt(eps) overflows fp32: h is 0, so dx = rstd * (g - mean g) and dgamma = 0, whatever
+    the number of rows (a block's threads may have fewer rows than they could take).  Sums of 16 and 3 terms: 2^-20."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for rows in (1, 2, 3, 33):
+            x = torch.full((rows, 16), 2.0 ** 121, dtype=dtype, device="cuda")
+            dy, gamma, beta = rand(rows, 16, seed=1, dtype=dtype), rand(16, seed=2), rand(16, seed=3)
+            y, stats = tg.layer_norm(x, gamma, beta)
+            assert torch.equal(y, beta.to(dtype).expand(rows, 16))
+            dx, dg, db = tg.layer_norm_backward(dy, x, stats, gamma)
+            assert dg.eq(0).all(), rows
+            want = dy.double().sum(0)
+            assert ((db - want).abs() <= 2.0 ** -20 * dy.double().abs().sum(0)).all()
+            g = dy.double() * gamma.double()
+            want = 1e-5 ** -0.5 * (g - g.mean(1, keepdim=True))
+            mag = 1e-5 ** -0.5 * (g.abs() + g.abs().mean(1, keepdim=True))
+            assert ((dx.double() - want).abs() <= U[dtype] * want.abs() + 2.0 ** -20 * mag).all()

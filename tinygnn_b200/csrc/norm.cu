@@ -307,7 +307,9 @@ __global__ void __launch_bounds__(block_threads<TPR>(), resident_grad<TPR, VPT>(
     const auto fetch = [&](int d, int64_t r) {
         const bool live = r < a.rows;
         const int64_t at = live ? r : 0;
-        st[d] = stats[at];
+        // (of a row that is not there h is 0, not what row 0's statistics make
+        // of zeros: an infinity times its zero gradient would be NaN)
+        st[d] = live ? stats[at] : make_float2(0.0f, 0.0f);
         part.fetch(dy + at * lddy, live, kd[d]);
         if constexpr (SAVED) fetch_codes(part, s.codes + at * s.ld, s.exps + at * s.lde, live, kc[SAVED ? d : 0], ke[SAVED ? d : 0]);
         else part.fetch(x + at * ldx, live, kx[SAVED ? 0 : d]);
