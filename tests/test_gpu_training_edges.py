@@ -66,3 +66,35 @@ def test_layer_norm_gradient_of_large_constant_rows(tg):
             want = 1e-5 ** -0.5 * (g - g.mean(1, keepdim=True))
             mag = 1e-5 ** -0.5 * (g.abs() + g.abs().mean(1, keepdim=True))
             assert ((dx.double() - want).abs() <= U[dtype] * want.abs() + 2.0 ** -20 * mag).all()
+
+
+def small_and_large(dtype, most):
+    """Values of both signs, evenly spread over their exponents from 2^-30 to `most`, as one row per 64 values."""
+    n = 64 * 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    low, high = -30.0, torch.tensor(float(most)).log2().item()
+    x = torch.exp2(low + (high - low) * torch.rand(n, device="cuda", generator=g))
+    return torch.where(torch.rand(n, device="cuda", generator=g) < 0.5, x, -x).to(dtype).view(64, 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_elu_keeps_its_digits_near_zero(tg, dtype):
+    """ELU to a relative tolerance, by the activation kernels and by a typed product's epilogue (x times 1: few rows and
+    tiles).  fp32: 1 - e^x by CUDA's function (1 ulp), a product with alpha, and two sums of the three parts a tile's
+    product has: 2^-21.  16 bits: the rounding and 2^-16 (the exponential's 2^-22 against 1/16, and alpha)."""
+    x = small_and_large(dtype, 20.0)
+    for alpha in (1.0, 0.7):
+        xd = x.double()
+        want = torch.where(xd < 0, alpha * torch.expm1(xd), xd)
+        tol = (2.0 ** -21 if dtype == torch.float32 else U[dtype] + 2.0 ** -16) * want.abs() + TINY[dtype]
+        got = [tg.activation_save8(x, "elu", alpha)[0],
+               tg.activation_save8(x[:, :61], "elu", alpha)[0]]  # rows that end inside 16 bytes
+        one = torch.ones(1, 1, 1, dtype=dtype, device="cuda")
+        for rows in (16, 64 * 64):
+            off = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+            y = tg.typed_linear(x.view(-1, 1)[:rows].contiguous(), one, off, None, "elu", alpha)
+            got.append(y)
+        for y, w, t in zip(got, (want, want[:, :61], want.view(-1, 1)[:16], want.view(-1, 1)),
+                           (tol, tol[:, :61], tol.view(-1, 1)[:16], tol.view(-1, 1))):
+            bad = ~((y.double() - w).abs() <= t)
+            assert not bad.any(), (alpha, y[bad][:4], w[bad][:4])

@@ -381,11 +381,39 @@ void restore8(int64_t rows, int64_t cols, const Saved8& s, T* y, int64_t ldy, cu
 // as 1 / (1 + e^-2u), which equals it, does not cancel where tanh u is near
 // -1, and costs one exponential and one reciprocal.  FAST (for results of 16
 // bits) takes the hardware's exponential, whose error of 2^-19 or less here
-// is lost in the result's rounding of 2^-8 or 2^-11; with tanhf the 8-bit
-// activation passes were bound by arithmetic (131,072 x 1024 bf16, forward and
-// backward: 0.52 ms, and 0.29 with it).
+// is lost in the result's rounding of 2^-8 or 2^-11 where nothing cancels (for
+// ELU near zero see expm1_f); with tanhf the 8-bit activation passes were bound
+// by arithmetic (131,072 x 1024 bf16, forward and backward: 0.52 ms, and 0.29
+// with it).
+__device__ __forceinline__ float exp2_hw(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));  // within 2^-22; 2^-inf = 0
+    return r;
+}
 template <bool FAST>
 __device__ __forceinline__ float exp_f(float x) { return FAST ? __expf(x) : expf(x); }
+// e^x - 1 for x <= 0.  The difference loses what 1 has more bits than e^x - 1;
+// where that would show the series is summed instead.  FAST: four terms above
+// -1/16 (the fifth is below 2^-22 of the sum; below -1/16 the difference is
+// within 2^-17).  fp32: nine terms above -1/2 (the tenth is below 2^-30 of the
+// sum; below, the hardware's exponential is within 2^-22 and the difference
+// within 2^-21).  131,072 x 1,024 fp32 with the 8-bit copy: 223 us, 270 with
+// expm1f, and 240 by expf's difference alone.
+template <bool FAST>
+__device__ __forceinline__ float expm1_f(float x) {
+    float q = FAST ? 1.0f / 24.0f : 1.0f / 362880.0f;
+    if (!FAST) {
+        q = fmaf(x, q, 1.0f / 40320.0f);
+        q = fmaf(x, q, 1.0f / 5040.0f);
+        q = fmaf(x, q, 1.0f / 720.0f);
+        q = fmaf(x, q, 1.0f / 120.0f);
+        q = fmaf(x, q, 1.0f / 24.0f);
+    }
+    q = fmaf(x, q, 1.0f / 6.0f);
+    q = fmaf(x, q, 0.5f);
+    q = fmaf(__fmul_rn(x, x), q, x);
+    return x > (FAST ? -0.0625f : -0.5f) ? q : __fsub_rn(exp2_hw(__fmul_rn(x, 1.4426950409f)), 1.0f);
+}
 __device__ __forceinline__ float reciprocal(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));  // 1 ulp; 1 / inf = 0
@@ -399,9 +427,7 @@ __device__ __forceinline__ float sigmoid_f(float x) { return reciprocal(__fadd_r
 template <bool FAST>
 __device__ __forceinline__ float gelu_s(float x, float x2) {
     if (FAST) {
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(x, fmaf(-0.102943239f, x2, -2.302208198f))));
-        return reciprocal(__fadd_rn(1.0f, e));
+        return reciprocal(__fadd_rn(1.0f, exp2_hw(__fmul_rn(x, fmaf(-0.102943239f, x2, -2.302208198f)))));
     }
     return sigmoid_f<false>(__fmul_rn(x, fmaf(0.0713548162726f, x2, 1.5957691216f)));
 }
@@ -420,7 +446,11 @@ __device__ __forceinline__ void act_forward(float (&x)[V], int act, float alpha)
         case TG_ACT_RELU: map_v(x, [](float v) { return v < 0.0f ? 0.0f : v; }); break;  // NaN stays NaN
         case TG_ACT_LEAKY_RELU: map_v(x, [alpha](float v) { return v >= 0.0f ? v : __fmul_rn(alpha, v); }); break;
         case TG_ACT_ELU:
-            map_v(x, [alpha](float v) { return v < 0.0f ? __fmul_rn(alpha, __fsub_rn(exp_f<FAST>(v), 1.0f)) : v; });
+            // (without a branch: a warp's values have both signs)
+            map_v(x, [alpha](float v) {
+                const float e = __fmul_rn(alpha, expm1_f<FAST>(fminf(v, 0.0f)));
+                return v < 0.0f ? e : v;
+            });
             break;
         case TG_ACT_SIGMOID: map_v(x, [](float v) { return sigmoid_f<FAST>(v); }); break;
         case TG_ACT_TANH: map_v(x, [](float v) { return tanhf(v); }); break;
