@@ -98,3 +98,28 @@ def test_elu_keeps_its_digits_near_zero(tg, dtype):
                            (tol, tol[:, :61], tol.view(-1, 1)[:16], tol.view(-1, 1))):
             bad = ~((y.double() - w).abs() <= t)
             assert not bad.any(), (alpha, y[bad][:4], w[bad][:4])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["sigmoid", "tanh"])
+def test_slopes_far_from_zero_keep_their_digits(tg, dtype, act):
+    """Slopes of sigmoid and tanh to a relative tolerance where they are small.  e^-a with a up to 40 in fp32: its
+    argument's rounding is 40 2^-24 of it, and six more roundings: 2^-18.  Results of 16 bits add their rounding."""
+    most = 40.0 if act == "sigmoid" else 20.0
+    x = small_and_large(dtype, most)
+    xd = x.double()
+    e = torch.exp(-xd.abs() * (1 if act == "sigmoid" else 2))
+    slope = (1 if act == "sigmoid" else 4) * e / (1 + e) ** 2
+    # scaled, so that fp16 (least step 2^-24) can tell more of the small ones from zero
+    dy = torch.full_like(x, 2.0 ** 14)
+    want = 2.0 ** 14 * slope
+    tol = (2.0 ** -18 if dtype == torch.float32 else U[dtype] + 2.0 ** -18) * want + TINY[dtype]
+    for cols in (64, 61):
+        got = tg.activation_backward(dy[:, :cols], x[:, :cols], act)
+        bad = ~((got.double() - want[:, :cols]).abs() <= tol[:, :cols])
+        assert not bad.any(), (x[:, :cols][bad][:4], got[bad][:4], want[:, :cols][bad][:4])
+    # infinities, NaN and zeros
+    v = torch.tensor([[float("inf"), -float("inf"), float("nan"), 0.0, -0.0, 200.0, -200.0, 3.0]], device="cuda").to(dtype)
+    got = tg.activation_backward(torch.ones_like(v), v, act)
+    assert got[0, :2].eq(0).all() and got[0, 2].isnan() and got[0, 3:5].eq(0.25 if act == "sigmoid" else 1.0).all()
+    assert got[0, 5:7].eq(0).all() and got[0, 7] > 0

@@ -478,14 +478,16 @@ __device__ __forceinline__ void act_slope(float (&x)[V], int act, float alpha) {
             break;
         case TG_ACT_SIGMOID:
             map_v(x, [](float v) {
-                const float s = sigmoid_f<FAST>(v);
-                return __fmul_rn(s, __fsub_rn(1.0f, s));
+                // s (1 - s) = e / (1 + e)^2, e = e^-|v|: 1 - s would cancel
+                const float e = exp_f<FAST>(-fabsf(v)), s = reciprocal(__fadd_rn(1.0f, e));
+                return __fmul_rn(__fmul_rn(e, s), s);
             });
             break;
         case TG_ACT_TANH:
             map_v(x, [](float v) {
-                const float t = tanhf(v);
-                return fmaf(-t, t, 1.0f);
+                // 1 - tanh^2 = 4 e / (1 + e)^2, e = e^-2|v|
+                const float e = exp_f<FAST>(__fmul_rn(-2.0f, fabsf(v))), s = reciprocal(__fadd_rn(1.0f, e));
+                return __fmul_rn(__fmul_rn(4.0f, e), __fmul_rn(s, s));
             });
             break;
         case TG_ACT_GELU:
