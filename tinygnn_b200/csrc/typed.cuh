@@ -4,6 +4,7 @@
 #pragma once
 
 #include <algorithm>
+#include <climits>
 
 #include "values.cuh"
 
@@ -16,9 +17,16 @@ __device__ __forceinline__ int clamp_row(int r, int64_t M) {
     return r < 0 ? 0 : (r > M ? static_cast<int>(M) : r);
 }
 
-// prefix[t] = number of pieces of `per` rows in the types before t (one warp).
-// The offsets of 128 types are asked for at once: a warp that went 32 at a
-// time would wait for memory four times.
+// Pieces so far and n more (n below 2^29), at most INT_MAX: types that overlap
+// own more than M rows between them, and a count that wrapped around would
+// lead a block out of its type.  Pieces past the limit are not worked on.
+__host__ __device__ __forceinline__ int add_pieces(int so_far, int n) {
+    return n > INT_MAX - so_far ? INT_MAX : so_far + n;
+}
+
+// prefix[t] = number of pieces of `per` rows (128 or more) in the types before
+// t (one warp).  The offsets of 128 types are asked for at once: a warp that
+// went 32 at a time would wait for memory four times.
 __device__ __forceinline__ void scan_types(const int32_t* offsets, int types, int64_t M, int64_t per, int* prefix) {
     const int lane = threadIdx.x & 31;
     int carry = 0;
@@ -41,8 +49,8 @@ __device__ __forceinline__ void scan_types(const int32_t* offsets, int types, in
                 const int up = __shfl_up_sync(0xffffffffu, n, o);
                 if (lane >= o) n += up;
             }
-            if (t < types) prefix[t + 1] = carry + n;
-            carry += __shfl_sync(0xffffffffu, n, 31);
+            if (t < types) prefix[t + 1] = add_pieces(carry, n);
+            carry = add_pieces(carry, __shfl_sync(0xffffffffu, n, 31));
         }
     }
 }
@@ -129,9 +137,9 @@ __host__ __device__ __forceinline__ int64_t piece_limit(int64_t steps, int64_t M
 inline int64_t max_pieces(int64_t M, int types, int64_t per, int slots, int longest) {
     return types + std::max<int64_t>(slots / per, (M / kStep + types) / longest + 1);
 }
-__device__ __forceinline__ int piece_count(int n, int64_t limit) { return static_cast<int>((n + limit - 1) / limit); }
+__host__ __device__ __forceinline__ int piece_count(int n, int64_t limit) { return static_cast<int>((n + limit - 1) / limit); }
 // Rows of each piece (the last may have fewer; none is empty, since this is at most `limit`).
-__device__ __forceinline__ int piece_rows(int n, int count) {
+__host__ __device__ __forceinline__ int piece_rows(int n, int count) {
     return count <= 1 ? n : ((n + count - 1) / count + kStep - 1) / kStep * kStep;
 }
 // Whether type u's pieces come before type t's.
