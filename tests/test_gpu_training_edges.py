@@ -123,3 +123,91 @@ def test_slopes_far_from_zero_keep_their_digits(tg, dtype, act):
     got = tg.activation_backward(torch.ones_like(v), v, act)
     assert got[0, :2].eq(0).all() and got[0, 2].isnan() and got[0, 3:5].eq(0.25 if act == "sigmoid" else 1.0).all()
     assert got[0, 5:7].eq(0).all() and got[0, 7] > 0
+
+
+class Guarded:
+    """A matrix (or a batch) in a buffer with `room` sentinel elements before it, after it and between its rows."""
+
+    def __init__(self, shape, dtype, pad=8, room=4096):
+        self.rows, self.cols = 1, shape[-1]
+        for n in shape[:-1]:
+            self.rows *= n
+        self.ld = self.cols + pad
+        self.buf = torch.full((2 * room + self.rows * self.ld,), 77.0, dtype=dtype, device="cuda")
+        self.all = self.buf[room:room + self.rows * self.ld].view(self.rows, self.ld)
+        self.t = self.all[:, :self.cols].unflatten(0, shape[:-1]) if len(shape) > 2 else self.all[:, :self.cols]
+        self.p = self.all.data_ptr()
+        self.room = room
+
+    def check(self, what):
+        assert self.buf[:self.room].eq(77).all() and self.buf[-self.room:].eq(77).all(), what
+        assert self.all[:, self.cols:].eq(77).all(), what
+
+
+def typed_calls(lib, x, dy, w, bias, off, y, dx, dw, db):
+    """The three typed products by the C entry points into guarded buffers (db has no leading dimension: pad 0)."""
+    (M, K), N, T, d = x.shape, dy.shape[1], w.shape[0], {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[x.dtype]
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.tg_typed_linear(M, K, N, T, d, x.data_ptr(), K, w.data_ptr(), N, K * N, off.data_ptr(), bias.data_ptr(), 0,
+                               0.0, y.p, y.ld, None, 0, None, 0, st) == 0
+    assert lib.tg_typed_linear_grad_input(M, K, N, T, d, dy.data_ptr(), N, w.data_ptr(), N, K * N, off.data_ptr(), dx.p,
+                                          dx.ld, st) == 0
+    assert lib.tg_typed_linear_grad_weight(M, K, N, T, d, x.data_ptr(), K, None, 0, None, 0, dy.data_ptr(), N,
+                                           off.data_ptr(), d, dw.p, dw.ld, K * dw.ld, db.p, st) == 0
+    torch.cuda.synchronize()
+    for what, g in (("y", y), ("dx", dx), ("dw", dw), ("db", db)):
+        g.check(what)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(30000, 256, 384), (3000, 72, 41), (40, 24, 136)])
+def test_types_that_overlap(tg, dtype, M, K, N):
+    """Sixteen types that each own all rows (and sixteen that own none): every one gets the whole gradients, with the
+    same weight everywhere the rows' products are right too, and nothing around the outputs is written.  Sums of n terms
+    to n 2^-23 of their magnitude (the tensor cores may truncate)."""
+    from tinygnn_b200 import _lib
+    T = 32
+    x, dy = rand(M, K, seed=1, dtype=dtype), rand(M, N, seed=2, dtype=dtype)
+    w = rand(1, K, N, seed=3, scale=K ** -0.5, dtype=dtype).repeat(T, 1, 1)
+    bias = rand(1, N, seed=4).repeat(T, 1)
+    off = torch.tensor([0, M] * 16 + [0], dtype=torch.int32, device="cuda")
+    y, dx = Guarded((M, N), dtype), Guarded((M, K), dtype)
+    dw, db = Guarded((T, K, N), dtype), Guarded((T, N), torch.float32, pad=0)
+    typed_calls(_lib.lib, x, dy, w, bias, off, y, dx, dw, db)
+    xd, dyd, wd = x.double(), dy.double(), w[0].double()
+
+    def near(got, want, mag, terms, u):
+        bad = ~((got.double() - want).abs() <= u * want.abs() + (terms + 16) * 2.0 ** -23 * mag + TINY[got.dtype])
+        assert not bad.any(), (int(bad.sum()), got[bad][:3], want[bad][:3])
+
+    near(y.t, xd @ wd + bias[0].double(), xd.abs() @ wd.abs() + bias[0].double().abs(), K, U[dtype])
+    near(dx.t, dyd @ wd.T, dyd.abs() @ wd.abs().T, N, U[dtype])
+    dw_want, dw_mag, db_want, db_mag = xd.T @ dyd, xd.abs().T @ dyd.abs(), dyd.sum(0), dyd.abs().sum(0)
+    for t in range(T):
+        if t % 2:
+            assert dw.t[t].eq(0).all() and db.t[t].eq(0).all(), t
+        else:
+            near(dw.t[t], dw_want, dw_mag, M, U[dtype])
+            near(db.t[t], db_want, db_mag, M, U[torch.float32])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_out_of_range_write_nothing_outside(tg, dtype):
+    """Bounds outside [0, rows], decreasing ones, rows of no type: nothing around the outputs is written, and rows of no
+    type stay as they were."""
+    from tinygnn_b200 import _lib
+    for M in (20, 90, 700):
+        for off in ([0, 40, 5000], [-7, 10, M], [0, M - 5, 12], [M, M, M], [3, 9, M - 4], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1]):
+            K, N = 32, 24
+            x, dy, w, bias = rand(M, K, seed=1, dtype=dtype), rand(M, N, seed=2, dtype=dtype), rand(2, K, N, seed=3, dtype=dtype), rand(2, N, seed=4)
+            y, dx = Guarded((M, N), dtype), Guarded((M, K), dtype)
+            dw, db = Guarded((2, K, N), dtype), Guarded((2, N), torch.float32, pad=0)
+            typed_calls(_lib.lib, x, dy, w, bias, torch.tensor(off, dtype=torch.int32, device="cuda"), y, dx, dw, db)
+            c = [min(max(o, 0), M) for o in off]
+            own = torch.zeros(M, dtype=torch.bool, device="cuda")
+            for t in range(2):
+                own[c[t]:max(c[t], c[t + 1])] = True
+                n = max(0, c[t + 1] - c[t])
+                want = dy[c[t]:c[t] + n].double().sum(0)
+                assert ((db.t[t] - want).abs() <= (n + 16) * 2.0 ** -24 * dy[c[t]:c[t] + n].double().abs().sum(0)).all()
+            assert y.t[~own].eq(77).all() and dx.t[~own].eq(77).all()

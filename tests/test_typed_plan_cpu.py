@@ -60,6 +60,12 @@ int main() {
             }
         }
         CHECK(pieces <= max_pieces(M, types, per, slots, longest));
+        // bias gradients: partial sums of M / kBiasChunk + types chunks
+        const int64_t rows = bias_chunk(owned, M);
+        int64_t chunks = 0;
+        for (int t = 0; t < types; ++t) chunks += (n[t] + rows - 1) / rows;
+        CHECK(chunks <= M / kBiasChunk + types);
+        CHECK(owned > M || rows == kBiasChunk);
         // counts of pieces never wrap around
         int sum = 0;
         int64_t exact = 0;

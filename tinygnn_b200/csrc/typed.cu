@@ -22,27 +22,49 @@ namespace {
 
 // ── db ───────────────────────────────────────────────────────────────────
 // Column sums of each type's rows, in two steps of fixed order: chunks of
-// kChunk rows of one type (8 warps, a row each; the warps joined through
+// kBiasChunk rows of one type (8 warps, a row each; the warps joined through
 // shared memory), then a type's chunks.  One read of dY: bound by HBM.
-constexpr int kChunk = 256;
+
+// One warp: prefix[t] = the chunks before type t, at most `chunks` of them in
+// all; the rows of a chunk.
+__device__ __forceinline__ int64_t scan_chunks(const int32_t* offsets, int types, int64_t M, int chunks, int* prefix) {
+    scan_types(offsets, types, M, kBiasChunk, prefix);
+    __syncwarp();
+    if (prefix[types] <= chunks) return kBiasChunk;
+    int64_t owned = 0;  // types overlap
+    for (int t = threadIdx.x & 31; t < types; t += 32) owned += rows_of(offsets, t, M);
+    owned = reduce_sum<int64_t, 32>(owned);
+    const int64_t per = bias_chunk(owned, M);
+    __syncwarp();
+    scan_types(offsets, types, M, per, prefix);
+    return per;
+}
 
 // Columns of a warp: 16 bytes a lane when rows are aligned, else 4 columns a
 // lane, 32 apart.
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) typed_bias_kernel(int64_t M, int64_t N, int types, const int32_t* offsets,
-                                                         const T* dY, int64_t lddy, float* part) {
+                                                         const T* dY, int64_t lddy, float* part, int chunks,
+                                                         int64_t* chunk_rows) {
     constexpr int V = ALIGNED ? 16 / static_cast<int>(sizeof(T)) : 4;
     __shared__ int prefix[kMaxTypes + 1];
     __shared__ float sh[8][32 * V];
+    __shared__ int64_t rows;
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
     wait_for_previous();
-    if (w == 0) scan_types(offsets, types, M, kChunk, prefix);
+    if (w == 0) {
+        const int64_t per = scan_chunks(offsets, types, M, chunks, prefix);
+        if (lane == 0) {
+            rows = per;
+            if (blockIdx.x == 0 && blockIdx.y == 0) *chunk_rows = per;
+        }
+    }
     __syncthreads();
     const int p = blockIdx.x;
     if (p >= prefix[types]) return;
     const int t = find_type(prefix, types, p);
-    const int64_t r0 = clamp_row(offsets[t], M) + static_cast<int64_t>(p - prefix[t]) * kChunk;
-    const int64_t e = clamp_row(offsets[t + 1], M), r1 = r0 + kChunk < e ? r0 + kChunk : e;
+    const int64_t r0 = clamp_row(offsets[t], M) + (p - prefix[t]) * rows;
+    const int64_t e = clamp_row(offsets[t + 1], M), r1 = r0 + rows < e ? r0 + rows : e;
     const int64_t n0 = static_cast<int64_t>(blockIdx.y) * 32 * V;
     float sum[V] = {};
     const auto col = [&](int j) { return n0 + (ALIGNED ? lane * V + j : j * 32 + lane); };
@@ -75,18 +97,18 @@ __global__ void __launch_bounds__(256) typed_bias_kernel(int64_t M, int64_t N, i
 }
 
 __global__ void __launch_bounds__(256) typed_bias_join_kernel(int64_t M, int64_t N, const int32_t* offsets,
-                                                              const float* part, int chunks, float* db) {
+                                                              const float* part, const int64_t* chunk_rows, float* db) {
     __shared__ int prefix[kMaxTypes + 1];
     __shared__ float sh[8][33];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32, t = blockIdx.y;
     wait_for_previous();
-    if (w == 0) scan_types(offsets, t + 1, M, kChunk, prefix);
+    if (w == 0) scan_types(offsets, t + 1, M, *chunk_rows, prefix);
     __syncthreads();
     const int64_t n = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float sum = 0.0f;
     if (n < N) {
 #pragma unroll 4
-        for (int p = prefix[t] + w; p < (prefix[t + 1] < chunks ? prefix[t + 1] : chunks); p += 8) sum += part[p * N + n];
+        for (int p = prefix[t] + w; p < prefix[t + 1]; p += 8) sum += part[p * N + n];
     }
     sh[w][lane] = sum;
     __syncthreads();
@@ -119,16 +141,18 @@ void check_weight(const char* fn, const char* what, int64_t K, int64_t N, int64_
 template <class T>
 void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T* dY, int64_t lddy, float* db,
                 cudaStream_t s) {
-    const int64_t chunks = M / kChunk + std::min<int64_t>(types, M);
-    Scratch<float> part(static_cast<size_t>(chunks * N), s);
+    const int64_t chunks = M / kBiasChunk + types;
+    Scratch<float> scratch(static_cast<size_t>(2 + chunks * N), s);
+    int64_t* const chunk_rows = reinterpret_cast<int64_t*>(scratch.p);
+    float* const part = scratch.p + 2;
     const bool al = rows_aligned16(dY, lddy, sizeof(T));
     const int64_t tile = al ? 32 * (16 / static_cast<int64_t>(sizeof(T))) : 128;
     launch_dependent("typed_linear_grad_bias", al ? typed_bias_kernel<T, true> : typed_bias_kernel<T, false>,
            dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(N, tile))), dim3(256), 0, s, M, N, types,
-           offsets, dY, lddy, part.p);
+           offsets, dY, lddy, part, static_cast<int>(chunks), chunk_rows);
     launch_dependent("typed_linear_grad_bias", typed_bias_join_kernel,
            dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0, s, M, N, offsets,
-           part.p, static_cast<int>(chunks), db);
+           part, chunk_rows, db);
 }
 
 template void typed_bias<__nv_bfloat16>(int64_t, int64_t, int, const int32_t*, const __nv_bfloat16*, int64_t, float*,

@@ -55,6 +55,14 @@ __device__ __forceinline__ void scan_types(const int32_t* offsets, int types, in
     }
 }
 
+// Rows of a chunk of the bias gradient's sums when the types own `owned` rows
+// of M between them: more than kBiasChunk where they overlap, so that there are
+// never more than M / kBiasChunk + types chunks.
+constexpr int kBiasChunk = 256;
+__host__ __device__ __forceinline__ int64_t bias_chunk(int64_t owned, int64_t M) {
+    return kBiasChunk * (owned <= M ? 1 : (owned + M - 1) / M);
+}
+
 // The type that piece p belongs to: the last t with prefix[t] <= p.
 __device__ __forceinline__ int find_type(const int* prefix, int types, int p) {
     int lo = 0, hi = types;
