@@ -160,7 +160,7 @@ def typed_calls(lib, x, dy, w, bias, off, y, dx, dw, db):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M,K,N", [(30000, 256, 384), (3000, 72, 41), (40, 24, 136)])
+@pytest.mark.parametrize("M,K,N", [(60000, 256, 384), (30000, 256, 384), (3000, 72, 41), (40, 24, 136)])
 def test_types_that_overlap(tg, dtype, M, K, N):
     """Sixteen types that each own all rows (and sixteen that own none): every one gets the whole gradients, with the
     same weight everywhere the rows' products are right too, and nothing around the outputs is written.  Sums of n terms
@@ -211,3 +211,17 @@ def test_offsets_out_of_range_write_nothing_outside(tg, dtype):
                 want = dy[c[t]:c[t] + n].double().sum(0)
                 assert ((db.t[t] - want).abs() <= (n + 16) * 2.0 ** -24 * dy[c[t]:c[t] + n].double().abs().sum(0)).all()
             assert y.t[~own].eq(77).all() and dx.t[~own].eq(77).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_a_type_are_written_whatever_follows_them(tg, dtype):
+    """Types whose bounds fall again after their rows: by the few-row kernels (20 rows, 3 for dX) as by tiles (90)."""
+    K, N = 32, 24
+    for M in (3, 20, 90):
+        x, dy, w = rand(M, K, seed=1, dtype=dtype), rand(M, N, seed=2, dtype=dtype), rand(3, K, N, seed=3, dtype=dtype)
+        off = torch.tensor([0, M - 1, 1, 1], dtype=torch.int32, device="cuda")  # type 0 owns all rows but the last
+        y, dx = tg.typed_linear(x, w, off)[:M - 1], tg.typed_linear_grad_input(dy, w, off)[:M - 1]
+        xd, dyd, wd = x[:M - 1].double(), dy[:M - 1].double(), w[0].double()
+        for got, a, b in ((y, xd, wd), (dx, dyd, wd.T)):
+            tol = U[dtype] * (a @ b).abs() + 48 * 2.0 ** -23 * (a.abs() @ b.abs()) + TINY[dtype]
+            assert ((got.double() - a @ b).abs() <= tol).all(), M

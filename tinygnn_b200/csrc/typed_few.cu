@@ -5,9 +5,9 @@
 //  With a few rows (see few_rows()) the products read the used weights (or write all
 //  of dW) and do next to no arithmetic: they are bound by HBM and by latency,
 //  and a 128-row tensor-core tile would be filled for a row or two.  These
-//  kernels stream the weights through FP32 FMAs.  Each row finds its type by
-//  counting the offsets below it (one load a thread).  Rows of one type read
-//  its weight again, from L2.
+//  kernels stream the weights through FP32 FMAs.  Each row looks for its type
+//  among all of them (one a thread).  Rows of one type read its weight again,
+//  from L2.
 // ============================================================================
 #include <algorithm>
 
@@ -21,18 +21,18 @@ constexpr int kFewThreads = 512;
 constexpr int kFewCols = 128;    // columns of a forward block (one exponent of the saved form)
 constexpr int kFewChunk = 2048;  // inner indexes of a row held in shared memory at a time
 
-// The type of row r: how many types end at or before it.  Every thread calls it.
+// The type that owns row r (the last, of types that overlap), -1 if none does.
+// Every thread calls it.
 __device__ __forceinline__ int type_of_row(const int32_t* offsets, int types, int64_t M, int64_t r) {
-    int n = 0;
-    for (int t = threadIdx.x; t < types; t += blockDim.x) n += clamp_row(offsets[t + 1], M) <= r;
-    __shared__ int count[kFewThreads / 32];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (threadIdx.x % 32 == 0) count[threadIdx.x / 32] = n;
+    int n = -1;
+    for (int t = threadIdx.x; t < types; t += blockDim.x)
+        if (clamp_row(offsets[t], M) <= r && r < clamp_row(offsets[t + 1], M)) n = t;
+    __shared__ int owner[kFewThreads / 32];
+    n = __reduce_max_sync(0xffffffffu, n);
+    if (threadIdx.x % 32 == 0) owner[threadIdx.x / 32] = n;
     __syncthreads();
-    n = 0;
 #pragma unroll
-    for (int w = 0; w < kFewThreads / 32; ++w) n += count[w];
+    for (int w = 0; w < kFewThreads / 32; ++w) n = owner[w] > n ? owner[w] : n;
     return n;
 }
 
@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kFewThreads) few_forward_kernel(const RowsArgs
     wait_for_previous();
     const int64_t r = blockIdx.y, n0 = static_cast<int64_t>(blockIdx.x) * kFewCols;
     const int t = type_of_row(g.offsets, g.types, g.M, r);
-    if (t >= g.types || r < clamp_row(g.offsets[t], g.M)) return;  // no type owns the row
+    if (t < 0) return;
     const int lane = threadIdx.x % LANES, k_first = threadIdx.x / LANES;
     const int64_t n = n0 + lane * V;
     const int left = n + V <= g.N ? V : (n < g.N ? static_cast<int>(g.N - n) : 0);
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kFewThreads) few_grad_input_kernel(const RowsA
     wait_for_previous();
     const int64_t r = blockIdx.y;
     const int t = type_of_row(g.offsets, g.types, g.M, r);
-    if (t >= g.types || r < clamp_row(g.offsets[t], g.M)) return;
+    if (t < 0) return;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t out0 = static_cast<int64_t>(blockIdx.x) * kFewOut + warp * 2;
     float acc[2] = {0.0f, 0.0f};
