@@ -137,9 +137,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
             }
             // Every copy issued must have landed before the CTA may exit: the
-            // MMAs that read a stage free it.
-            for (int64_t j = i > STAGES ? i - STAGES : 0; j < i && ok; ++j)
-                ok = mb::wait(&s.empty[j % STAGES], (j / STAGES) & 1, &g_error, 52);
+            // MMAs that read a stage free it.  (After a wait that ran out too:
+            // each of these is bounded by itself.)
+            for (int64_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
+                mb::wait(&s.empty[j % STAGES], (j / STAGES) & 1, &g_error, 52);
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
