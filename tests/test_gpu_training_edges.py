@@ -225,3 +225,75 @@ def test_rows_of_a_type_are_written_whatever_follows_them(tg, dtype):
         for got, a, b in ((y, xd, wd), (dx, dyd, wd.T)):
             tol = U[dtype] * (a @ b).abs() + 48 * 2.0 ** -23 * (a.abs() @ b.abs()) + TINY[dtype]
             assert ((got.double() - a @ b).abs() <= tol).all(), M
+
+
+def lay_out(rows, types, spread):
+    """Offsets of `rows` rows over `types` types: a few rows each, or all in the third (first, of fewer) type."""
+    if spread:
+        o = [rows * t // types for t in range(types + 1)]
+    else:
+        at = min(2, types - 1)
+        o = [0] * (at + 1) + [rows] * (types - at)
+    return torch.tensor(o, dtype=torch.int32, device="cuda"), o
+
+
+# rows, types, K, N at and past the limits between the few-row kernels and tiles (forward, dX, dW), 16-bit and fp32
+LIMITS = [(4, 1, 2048, 2048), (5, 1, 2560, 2624), (8, 3, 2048, 2048), (9, 3, 2048, 2048), (32, 2, 1024, 1024),
+          (32, 40, 1024, 1032), (4, 5, 1024, 1024), (4, 5, 1024, 1025), (32, 7, 128, 256), (32, 7, 129, 257), (8, 1, 520, 2056),
+          (32, 1, 4096, 4096), (32, 1, 4096, 4104), (32, 2, 4096, 4104), (33, 40, 264, 136), (40, 40, 264, 136), (41, 40, 264, 136),
+          (200, 200, 41, 43), (1000, 1024, 72, 40)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,types,K,N", LIMITS)
+@pytest.mark.parametrize("spread", [True, False])
+def test_few_rows_at_the_limits(tg, dtype, rows, types, K, N, spread):
+    """Sums of n terms to (n + 16) 2^-23 of their magnitude, and the result's rounding."""
+    off, o = lay_out(rows, types, spread)
+    x, dy = rand(rows, K, seed=1, dtype=dtype), rand(rows, N, seed=2, dtype=dtype)
+    w, bias = rand(types, K, N, seed=3, scale=K ** -0.5, dtype=dtype), rand(types, N, seed=4)
+
+    def near(got, want, mag, terms, u):
+        bad = ~((got.double() - want).abs() <= u * want.abs() + (terms + 16) * 2.0 ** -23 * mag + TINY[got.dtype])
+        assert not bad.any(), (int(bad.sum()), got[bad][:3], want[bad][:3])
+
+    y, (dx, dw, db) = tg.typed_linear(x, w, off, bias), tg.typed_linear_backward(dy, x, w, off)
+    for t in range(types):
+        a, b = o[t], o[t + 1]
+        if a == b:
+            assert dw[t].eq(0).all() and db[t].eq(0).all()
+            continue
+        xd, dyd, wd = x[a:b].double(), dy[a:b].double(), w[t].double()
+        near(y[a:b], xd @ wd + bias[t].double(), xd.abs() @ wd.abs() + bias[t].double().abs(), K, U[dtype])
+        near(dx[a:b], dyd @ wd.T, dyd.abs() @ wd.abs().T, N, U[dtype])
+        near(dw[t], xd.T @ dyd, xd.abs().T @ dyd.abs(), b - a, U[dtype])
+        near(db[t], dyd.sum(0), dyd.abs().sum(0), b - a, U[torch.float32])
+
+
+def device_us(f, n=5):
+    """Median device time of f in us."""
+    f()
+    times = []
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    return sorted(times)[n // 2]
+
+
+def test_few_rows_have_no_cliffs(tg):
+    """Time, to a factor that a busy machine does not reach: rows that share a large weight take no longer than a tile
+    of them (33 rows); rows that all lie in one of many types no longer than a few times what they take when spread."""
+    w = rand(1, 4096, 4096, seed=1, dtype=torch.bfloat16)
+    x = rand(33, 4096, seed=2, dtype=torch.bfloat16)
+    off = [torch.tensor([0, r], dtype=torch.int32, device="cuda") for r in range(34)]
+    for f, few in ((tg.typed_linear, 32), (tg.typed_linear_grad_input, 4)):
+        tile = device_us(lambda: f(x, w, off[33]))
+        assert device_us(lambda: f(x[:few], w, off[few])) <= 2 * tile + 10, few
+    rows = 256
+    x, dy = rand(rows, 1024, seed=3, dtype=torch.bfloat16), rand(rows, 1024, seed=4, dtype=torch.bfloat16)
+    one, spread = (device_us(lambda o=lay_out(rows, 256, s)[0]: tg.typed_linear_grad_weight(x, dy, o)) for s in (False, True))
+    assert one <= 6 * spread, (one, spread)

@@ -223,8 +223,10 @@ void typed_weight_few(const WeightArgs<T, O>& a, cudaStream_t s) {
     const int wide = static_cast<int>(std::min<int64_t>(ceil_div(a.N, 8), 256)), rpb = 256 / wide;
     const int vec = reinterpret_cast<uintptr_t>(a.dW) % 16 == 0 && a.lddw * sizeof(O) % 16 == 0 &&
                     (a.types == 1 || a.stride_dw * sizeof(O) % 16 == 0);
-    // enough blocks for every SM several times over, each with a few rows of dW
-    const int64_t want = ceil_div(a.K, rpb * 4), most = std::max<int64_t>(1, int64_t(num_sms()) * 32 / a.types);
+    // Enough blocks for every SM several times over, each with a few rows of dW;
+    // and 64 a type, since all rows may lie in one (256 rows, 1,024 types, 1,024
+    // x 1,024 bf16: 858 us in one type, 395 spread; 4 blocks a type 6,505, 392).
+    const int64_t want = ceil_div(a.K, rpb * 4), most = std::max<int64_t>(64, int64_t(num_sms()) * 32 / a.types);
     launch_dependent("typed_few_weight",
                      a.saved.codes ? few_grad_weight_kernel<T, O, true> : few_grad_weight_kernel<T, O, false>,
                      dim3(static_cast<unsigned>(std::min(want, most)), static_cast<unsigned>(a.types)), dim3(256), 0,

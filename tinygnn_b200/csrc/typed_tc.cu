@@ -398,27 +398,51 @@ constexpr double kLargeFlops = 1e10;
 
 }  // namespace
 
-// Few rows: measured against the tile kernels (bf16, 64 types and one, K = N),
-//   forward   1,024: 8 rows 7.2 against 12.3 us, 32 rows 9.7 against 20.9, 64
-//             rows of one type 15.9 against 9.3; 256: 5.9 against 6.9
-//   dX        1,024: 4 rows 9.5 against 10.0, 8 rows 16.5 against 12.5; 256: 16
-//             rows 5.5 against 6.4, 32 rows 8.9 against 6.9
-//   dW        8 rows of one type 9.8 against 9.9, 16 rows 17.6 against 9.9; 64
-//             rows over 64 types 48 against 93
-bool few_rows(int64_t M, int64_t K, int64_t N, bool trans) {
-    return trans ? M <= 4 || (M <= kFewRows && M * K * N <= 1 << 20) : M <= kFewRows;
+// Which products of a few rows stream the weights (typed_few.cu): those kernels
+// read a row's weight from L2 or HBM for every row, so they lose to a tile when
+// rows share a large weight; where rows have weights of their own the tiles are
+// mostly empty.  The host does not see how the rows lie (unless there is one
+// type), so each limit is where the worse of the two loses least.  us by few
+// rows / by tiles, rows of one type | each in a type of its own (K = N = 2,048
+// unless given; other weights in between, not in L2):
+//   forward, 16 bits  8 rows 14.5 / 13.6 | 13.9 / 21.4;  16 rows 15.5 / 13.8 |
+//                     24 / 30;  32 rows 28 / 13.5 | 45 / 44;  1,024: 32 rows
+//                     9.3 / 8.9 | 13.9 / 17.7;  4,096: 4 rows 27 / 26 | 31 / 41,
+//                     32 rows 93 / 23 | 165 / 160
+//   forward, fp32     32 rows 36 / 55 | 81 / 235;  8,192: 8 rows 136 / 191 |
+//                     300 / 899, 32 rows 445 / 193 | 663 / 1,897
+//   dX, 16 bits       1 row 13.2 / 13.7 | 12.3 / 13.9;  4 rows 30 / 13.5 | 30 /
+//                     19.5;  1,024: 4 rows 9.8 / 8.9 | 9.5 / 10.0, 8 rows 16.8 /
+//                     8.8 | 16.8 / 12.5;  256: 16 rows 5.0 / 5.9 | 5.5 / 6.2, 32
+//                     rows 8.3 / 5.9 | 8.4 / 6.8
+//   dX, fp32          8 rows 26 / 53 | 28 / 69;  32 rows 82 / 54 | 86 / 234;
+//                     1,024: 32 rows 24 / 29 | 27 / 70;  4,096 x 512: 32 rows
+//                     55 / 16.5 | 56 / 111
+bool few_rows(int64_t M, int64_t K, int64_t N, int types, size_t size, bool trans) {
+    const double work = static_cast<double>(M) * K * N;
+    if (M > kFewRows) return false;
+    if (size == 2) return trans ? work <= (M <= 4 ? 1 << 22 : 1 << 20) : M <= 4 || work <= 1 << 25;
+    return trans ? M <= 4 || work <= 1 << 25 : types > 1 || work <= 1 << 29;
 }
+// The weight gradients that go there: 8 rows, or no more rows than types (most
+// of dW is zeros, and a tile kernel's CTAs walk all types for them).
+// Measured as above, rows each in a type of its own | all in one: bf16, 1,024 x
+// 1,024: 64 rows 47 / 78 | 143 / 94, 256 rows 172 / 320 | 716 / 648, 1,024 rows
+// 667 / 1,250 | 2,886 / 2,474;  128 x 128: 64 rows 5.6 / 16 | 51 / 27, 1,024 rows
+// 16 / 140 | 915 / 329;  fp32, 1,024 x 1,024: 1,024 rows 1,416 / 1,910 | 4,386 /
+// 2,421.
+bool few_weight_rows(int64_t M, int types) { return M <= 8 || M <= types; }
 
 template <class T, bool TRANS>
 void typed_rows(const RowsArgs<T>& a, cudaStream_t s) {
-    if (few_rows(a.M, a.K, a.N, TRANS)) typed_rows_few<T, TRANS>(a, s);
+    if (few_rows(a.M, a.K, a.N, a.types, sizeof(T), TRANS)) typed_rows_few<T, TRANS>(a, s);
     else if constexpr (sizeof(T) == 2) typed_rows_tma<T, TRANS>(a, s);
     else typed_rows_any<T, TRANS>(a, s);
 }
 
 template <class T, class O>
 void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
-    if (a.M <= 8 || a.M <= a.types) {  // no rows: dW and db are zero
+    if (few_weight_rows(a.M, a.types)) {  // no rows: dW and db are zero
         typed_weight_few<T, O>(a, s);
         return;
     }
