@@ -297,3 +297,36 @@ def test_few_rows_have_no_cliffs(tg):
     x, dy = rand(rows, 1024, seed=3, dtype=torch.bfloat16), rand(rows, 1024, seed=4, dtype=torch.bfloat16)
     one, spread = (device_us(lambda o=lay_out(rows, 256, s)[0]: tg.typed_linear_grad_weight(x, dy, o)) for s in (False, True))
     assert one <= 6 * spread, (one, spread)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [513, 2049, 2056, 2304, 3071, 3073, 4095, 4112, 5121, 5632, 6143, 6144, 6145, 6152, 8191])
+def test_layer_norm_at_the_steps_of_its_row_split(tg, dtype, cols):
+    """Widths on both sides of every step, aligned and not, more rows than blocks, all outputs.  Sums of at most 32 terms a
+    thread and 12 joins of values up to max |x|: 2^-24 * 48 against the row's deviation, doubled for the gradient's."""
+    for rows, pad in ((700, 0), (3, 3)):
+        x, dy = rand(rows, cols + pad, seed=1, scale=2.0, shift=0.5, dtype=dtype)[:, :cols], rand(rows, cols + pad, seed=2, dtype=dtype)[:, :cols]
+        gamma, beta = rand(cols, seed=3, scale=0.3, shift=1.0, dtype=dtype), rand(cols, seed=4, dtype=dtype)
+        y, stats, saved = tg.layer_norm(x, gamma, beta, save8=True)
+        assert torch.equal(y, tg.layer_norm(x, gamma, beta)[0])
+        xd, dyd, g, b = x.double(), dy.double(), gamma.double(), beta.double()
+        mean = xd.mean(1, keepdim=True)
+        rstd = ((xd - mean) ** 2).mean(1, keepdim=True).add(1e-5) ** -0.5
+        h = (xd - mean) * rstd
+        slack = 2.0 ** -24 * 48 * (1 + xd.abs().amax(1, keepdim=True) * rstd)
+        want = h * g + b
+        assert ((y.double() - want).abs() <= U[dtype] * want.abs() + slack * (g.abs() * (1 + h.abs()) + b.abs()) + TINY[dtype]).all()
+        held = saved.restore(torch.float32).double()
+        step = torch.exp2(saved.exponents.double() - 127).repeat_interleave(128, 1)[:, :cols]
+        assert ((held - h).abs() <= 0.5 * step + 2 * slack * (1 + h.abs())).all()
+        for given, hh, rough in ((x, h, slack), (saved, held, torch.full_like(slack, 2.0 ** -24 * 48))):
+            dx, dg, db = tg.layer_norm_backward(dy, given, stats, gamma)
+            gy = dyd * g
+            want = rstd * (gy - gy.mean(1, keepdim=True) - hh * (gy * hh).mean(1, keepdim=True))
+            mag = gy.abs() + gy.abs().mean(1, keepdim=True) + hh.abs() * (gy * hh).abs().mean(1, keepdim=True)
+            tol = U[dtype] * want.abs() + rstd * 4 * (rough + slack) * (1 + hh.abs()) * mag + TINY[dtype]
+            assert ((dx.double() - want).abs() <= tol).all()
+            n = (rows + 16) * 2.0 ** -24
+            for got, want, mag in ((dg, (dyd * hh).sum(0), (dyd * hh).abs() * n + dyd.abs() * rough * (1 + hh.abs())),
+                                   (db, dyd.sum(0), dyd.abs() * n)):
+                assert ((got.double() - want).abs() <= U[dtype] * want.abs() + mag.sum(0) + TINY[dtype]).all()

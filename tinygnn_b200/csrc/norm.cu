@@ -131,15 +131,15 @@ __device__ __forceinline__ void row_sum(float (&x)[S], float* red) {
     }
 }
 
-// Threads of a block.
+// Threads of a block: whole rows.
 template <int TPR>
-constexpr int block_threads() { return TPR < 128 ? 128 : TPR; }
+constexpr int block_threads() { return TPR < 128 && 128 % TPR == 0 ? 128 : TPR; }
 
 // Blocks a SM: the kernels are compiled and launched for as many.
 template <int TPR, int VPT>
 constexpr int resident() { return VPT > 16 ? 512 / block_threads<TPR>() : (TPR >= 256 ? 1024 / TPR : (VPT > 8 ? 5 : 8)); }
 template <int TPR, int VPT>
-constexpr int resident_grad() { return TPR >= 512 ? 1 : (TPR >= 256 ? 2 : (VPT > 8 ? 4 : 5)); }
+constexpr int resident_grad() { return TPR >= 384 ? 1 : (TPR >= 256 ? 2 : (VPT > 8 ? 4 : 5)); }
 
 // How many of its next rows a group of threads has asked for: as many as keep
 // about 16 KB of loads in flight a SM (one row at a time left HBM at 45 %).
@@ -526,13 +526,7 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const float* part, int 
 
 constexpr int64_t kRegisterCols = 8192;
 
-// Calls f(TPR, VPT) with the row split for `cols` columns.  The steps double;
-// above 4,096 columns, where a row is a block, there is one more at 5,120, which
-// leaves fewer threads without a value.  8,191 rows fp16, with the 8-bit copy:
-// forward by 160 threads 98 us for 4,099 columns, 53 for 4,104, by 256 131 and
-// 61.  The gradient from the copy, by 320 (two blocks a SM) 136 for 4,099, by
-// 512 148; from x 129 and 142; but aligned rows of 5,120 from x 99 and 88, so
-// there they stay with 512.
+// Calls f(TPR, VPT) with the row split for `cols` columns.
 template <class F>
 void by_width_narrow(int64_t cols, F&& f) {
     using std::integral_constant;
@@ -543,29 +537,43 @@ void by_width_narrow(int64_t cols, F&& f) {
     else f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
 }
 
-constexpr int kRaggedThreads = 320;
-
+// Above 4,096 columns, where one block has an SM to itself, 384 threads as far
+// as they reach: with 512 a thread has 128 registers for a row's values and its
+// sums.  33.5 million values, from x / from the 8-bit copy, us by 384 and 512
+// threads: fp16, 4,104 columns 68, 76 / 69, 80;  6,144: 59, 65 / 59, 67;  4,099:
+// 116, 136 / 134, 142;  5,121: 109, 121 / 122, 125;  half as many in fp32, 4,104:
+// 48, 62 / 46, 47;  4,099: 82, 87 / 79, 79.  (Two blocks of 320: fp16, 4,104: 87 /
+// 80;  4,099: 126 / 133;  fp32, 4,099: 75 / 69.  Three of 192 for 2,049: 136 / 140
+// where 256 take 122 / 128.)
 template <class F>
-void by_width_grad(int64_t cols, bool aligned, F&& f) {
+void by_width_grad(int64_t cols, F&& f) {
     using std::integral_constant;
     if (cols <= 512) by_width_narrow(cols, f);
-    else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
-    else if (cols <= 2048) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
-    else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
-    else if (cols <= 5120 && !aligned) f(integral_constant<int, kRaggedThreads>{}, integral_constant<int, 16>{});
+    else if (cols <= 64 * 16) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    else if (cols <= 128 * 16) f(integral_constant<int, 128>{}, integral_constant<int, 16>{});
+    else if (cols <= 256 * 16) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+    else if (cols <= 384 * 16) f(integral_constant<int, 384>{}, integral_constant<int, 16>{});
     else f(integral_constant<int, 512>{}, integral_constant<int, 16>{});
 }
 
 // The forward pass holds half as much a value: twice the values a thread, half
-// the warps that a row's sums have to cross.
+// the warps that a row's sums have to cross.  An SM holds 512 such threads; the
+// steps are the multiples of 32 threads whose blocks fill at least 15/16 of
+// them (96 by five, 160 by three; not 192 and 224).  33.5 million fp16 values
+// without / with the 8-bit copy, us by that step and by the next power of two:
+// 2,049 columns by 96 71 / 89, by 128 98 / 124;  2,056: 33 / 48, 36 / 55;  4,099
+// by 160 73 / 95, by 256 102 / 127;  4,104: 33 / 49, 38 / 57;  5,120: 29 / 42, 33 /
+// 47;  5,128 by 192 36 / 55, by 224 34 / 50, by 256 34 / 49;  6,144 by 224 33 / 49,
+// by 256 31 / 44.
 template <class F>
 void by_width_forward(int64_t cols, F&& f) {
     using std::integral_constant;
     if (cols <= 512) by_width_narrow(cols, f);
-    else if (cols <= 1024) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
-    else if (cols <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
-    else if (cols <= 4096) f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
-    else if (cols <= 5120) f(integral_constant<int, 160>{}, integral_constant<int, 32>{});
+    else if (cols <= 32 * 32) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (cols <= 64 * 32) f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
+    else if (cols <= 96 * 32) f(integral_constant<int, 96>{}, integral_constant<int, 32>{});
+    else if (cols <= 128 * 32) f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
+    else if (cols <= 160 * 32) f(integral_constant<int, 160>{}, integral_constant<int, 32>{});
     else f(integral_constant<int, 256>{}, integral_constant<int, 32>{});
 }
 
@@ -700,13 +708,12 @@ TG_API tg_status tg_layer_norm_grad(int64_t rows, int64_t cols, int32_t dtype, c
             const bool al = cols * sizeof(T) % 16 == 0 && rows_aligned16(dy, lddy, sizeof(T)) &&
                             (codes || rows_aligned16(x, ldx, sizeof(T))) &&
                             rows_aligned16(dx, lddx, sizeof(T)) && rows_aligned16(gamma, 0, 1);
-            by_width_grad(cols, al, [&](auto tpr, auto vpt) {
+            by_width_grad(cols, [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
                 constexpr int BT = block_threads<TPR>(), RPB = BT / TPR;
-                constexpr bool AL = TPR != kRaggedThreads;
-                auto kern = codes ? (al ? norm_grad_kernel<T, P, AL, TPR, VPT, true>
+                auto kern = codes ? (al ? norm_grad_kernel<T, P, true, TPR, VPT, true>
                                         : norm_grad_kernel<T, P, false, TPR, VPT, true>)
-                                  : (al ? norm_grad_kernel<T, P, AL, TPR, VPT, false>
+                                  : (al ? norm_grad_kernel<T, P, true, TPR, VPT, false>
                                         : norm_grad_kernel<T, P, false, TPR, VPT, false>);
                 parts = std::min<int64_t>(ceil_div(rows, RPB), int64_t(num_sms()) * resident_grad<TPR, VPT>());
                 Scratch<float> part(static_cast<size_t>(parts * 2 * cols), str);
