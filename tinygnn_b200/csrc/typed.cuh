@@ -247,9 +247,10 @@ template <class T, bool TRANS>
 void typed_rows_pair(const RowsArgs<T>& a, const TmaMatrix<T>& A, const TmaMatrix<T>& W, cudaStream_t s);
 int typed_pair_take_error();
 
-// Loader-fed kernels (typed_any.cu).
-template <class T, bool TRANS>
-void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s);
+// Loader-fed kernels (typed_any.cu): all products of fp32 rows, weight gradients
+// of 16-bit ones.
+template <bool TRANS>
+void typed_rows_any(const RowsArgs<float>& a, cudaStream_t s);
 template <class T, class O>
 void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s);
 int typed_any_take_error();

@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
                 tc::fence_after();
                 const uint32_t addr = tmem + acc * ACC + (static_cast<uint32_t>(q * 32) << 16);
                 if constexpr (!W) {
-                    finish_rows<T, BN, sizeof(T) == 2, SPLIT>(addr, out, m.t, r, clip(m.r1 - r, 32), m.n0, buf, first,
+                    finish_rows<T, BN, false, SPLIT>(addr, out, m.t, r, clip(m.r1 - r, 32), m.n0, buf, first,
                                                               last);
                 } else {
                     const int rows = clip(g.K - r, 32);
@@ -527,9 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1) typed_any_kernel(const AnyArgs<T>
     tear_down<BN, SPLIT>(s, tmem, 8);
 }
 
-// The least alignment that the loaders take, in bytes.
-template <class T>
-constexpr int64_t least() { return sizeof(T) == 4 ? 8 : 16; }
+// The least alignment of fp32 rows that the loaders take, in bytes.
+constexpr int64_t kLeast = 8;
 
 template <class T, int OP, int BN, bool SAVED>
 void go(const AnyArgs<T>& g, const RowsOut<T>& out, int64_t items, cudaStream_t s) {
@@ -540,15 +539,16 @@ void go(const AnyArgs<T>& g, const RowsOut<T>& out, int64_t items, cudaStream_t 
 
 }  // namespace
 
-template <class T, bool TRANS>
-void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s) {
+template <bool TRANS>
+void typed_rows_any(const RowsArgs<float>& a, cudaStream_t s) {
+    using T = float;
     constexpr int OP = TRANS ? kGradInput : kForward;
     AnyArgs<T> g{};
     g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
     // W[t] is K x N in the forward pass, N x K in the input gradient.
     const int64_t wr = TRANS ? a.N : a.K, wc = TRANS ? a.K : a.N;
-    const Operand<T> A(1, a.M, a.K, a.A, a.lda, 0, s, least<T>()),
-        W(a.types, wr, wc, a.W, a.ldw, a.stride_w, s, least<T>());
+    const Operand<T> A(1, a.M, a.K, a.A, a.lda, 0, s, kLeast),
+        W(a.types, wr, wc, a.W, a.ldw, a.stride_w, s, kLeast);
     g.A = A.p, g.lda = A.ld, g.B = W.p, g.ldb = W.ld, g.stride_b = W.stride;
     g.a_pair = !in_place(1, A.own ? A.ld : a.K, A.p, A.ld, 0);
     g.b_pair = !in_place(a.types, W.own ? W.ld : wc, W.p, W.ld, W.stride);
@@ -563,13 +563,10 @@ void typed_rows_any(const RowsArgs<T>& a, cudaStream_t s) {
 
 template <class T, class O>
 void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream_t s) {
-    const bool saved = a.saved.codes != nullptr;
     AnyArgs<T> g{};
     g.M = a.M, g.K = a.K, g.N = a.N, g.types = a.types, g.offsets = a.offsets;
     g.tiles_m = w.tiles_k, g.tiles_n = w.tiles_n;
-    const Operand<T> Y(1, a.M, a.N, a.dY, a.lddy, 0, s, least<T>());
-    g.a8 = a.saved, g.B = Y.p, g.ldb = Y.ld;
-    g.b_pair = !in_place(1, Y.own ? Y.ld : a.N, Y.p, Y.ld, 0);
+    g.a8 = a.saved;
     g.slots = w.slots, g.part = w.part, g.ldp = w.ldp, g.stride_c = a.stride_dw;
     g.out_f32 = sizeof(O) == 4;
     RowsOut<T> out{};
@@ -578,28 +575,39 @@ void typed_weight_any(const WeightArgs<T, O>& a, const WeightPlan& w, cudaStream
     out.ldc = a.lddw;
     out.mode = store_mode(a.dW, a.lddw * sizeof(O), a.stride_dw * sizeof(O));
     g.db = a.db, g.db_part = w.db_part;
-    const auto by_source = [&](auto bn) {
-        constexpr int BN = decltype(bn)::value;
-        if (saved) {
-            go<T, kGradWeight, BN, true>(g, out, w.items, s);
-        } else {
-            const Operand<T> X(1, a.M, a.K, a.X, a.ldx, 0, s, least<T>());
-            g.A = X.p, g.lda = X.ld;
-            g.a_pair = !in_place(1, X.own ? X.ld : a.K, X.p, X.ld, 0);
-            go<T, kGradWeight, BN, false>(g, out, w.items, s);
-        }
+    const auto by_width = [&](auto saved) {
+        constexpr bool SAVED = decltype(saved)::value;
+        if (w.BN == 64) go<T, kGradWeight, 64, SAVED>(g, out, w.items, s);
+        else go<T, kGradWeight, 128, SAVED>(g, out, w.items, s);
     };
-    if (w.BN == 64) by_source(std::integral_constant<int, 64>{});
-    else by_source(std::integral_constant<int, 128>{});
+    const auto by_source = [&] {
+        if (a.saved.codes) by_width(std::true_type{});
+        else by_width(std::false_type{});
+    };
+    if constexpr (sizeof(T) == 2) {  // (rows that the loaders cannot read where they lie go by TMA)
+        g.A = a.X, g.lda = a.ldx, g.B = a.dY, g.ldb = a.lddy;
+        by_source();
+    } else {
+        const Operand<T> Y(1, a.M, a.N, a.dY, a.lddy, 0, s, kLeast);
+        g.B = Y.p, g.ldb = Y.ld;
+        g.b_pair = !in_place(1, Y.own ? Y.ld : a.N, Y.p, Y.ld, 0);
+        if (a.saved.codes) {
+            by_source();
+            return;
+        }
+        const Operand<T> X(1, a.M, a.K, a.X, a.ldx, 0, s, kLeast);
+        g.A = X.p, g.lda = X.ld;
+        g.a_pair = !in_place(1, X.own ? X.ld : a.K, X.p, X.ld, 0);
+        by_source();
+    }
 }
 
-#define TG_TYPED_ANY(T)                                                   \
-    template void typed_rows_any<T, false>(const RowsArgs<T>&, cudaStream_t); \
-    template void typed_rows_any<T, true>(const RowsArgs<T>&, cudaStream_t);  \
-    template void typed_weight_any<T, T>(const WeightArgs<T, T>&, const WeightPlan&, cudaStream_t);
-TG_TYPED_ANY(float)
-TG_TYPED_ANY(__nv_bfloat16)
-TG_TYPED_ANY(__half)
+template void typed_rows_any<false>(const RowsArgs<float>&, cudaStream_t);
+template void typed_rows_any<true>(const RowsArgs<float>&, cudaStream_t);
+template void typed_weight_any<float, float>(const WeightArgs<float, float>&, const WeightPlan&, cudaStream_t);
+template void typed_weight_any<__nv_bfloat16, __nv_bfloat16>(const WeightArgs<__nv_bfloat16, __nv_bfloat16>&,
+                                                             const WeightPlan&, cudaStream_t);
+template void typed_weight_any<__half, __half>(const WeightArgs<__half, __half>&, const WeightPlan&, cudaStream_t);
 template void typed_weight_any<__nv_bfloat16, float>(const WeightArgs<__nv_bfloat16, float>&, const WeightPlan&,
                                                      cudaStream_t);
 template void typed_weight_any<__half, float>(const WeightArgs<__half, float>&, const WeightPlan&, cudaStream_t);

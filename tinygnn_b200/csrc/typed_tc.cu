@@ -437,7 +437,7 @@ template <class T, bool TRANS>
 void typed_rows(const RowsArgs<T>& a, cudaStream_t s) {
     if (few_rows(a.M, a.K, a.N, a.types, sizeof(T), TRANS)) typed_rows_few<T, TRANS>(a, s);
     else if constexpr (sizeof(T) == 2) typed_rows_tma<T, TRANS>(a, s);
-    else typed_rows_any<T, TRANS>(a, s);
+    else typed_rows_any<TRANS>(a, s);
 }
 
 template <class T, class O>
