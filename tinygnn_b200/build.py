@@ -38,10 +38,35 @@ def torchops_path() -> str:
     return os.path.join(HERE, "_torch_ops" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
+def _torch_root() -> str:
+    import importlib.util
+    return os.path.dirname(importlib.util.find_spec("torch").origin)
+
+
+def _torch_version() -> str:
+    """torch's version, without importing it."""
+    scope: dict = {}
+    with open(os.path.join(_torch_root(), "version.py")) as f:
+        exec(f.read(), scope)  # noqa: S102  (a generated file of assignments)
+    return str(scope["__version__"])
+
+
+# The torch that _torch_ops was built against (its C++ ABI is that version's).
+TORCH_STAMP = os.path.join(HERE, "_build", "torch_ops_torch_version")
+
+
+def _torchops_stale() -> bool:
+    """Whether _torch_ops is known to have been built against another torch."""
+    try:
+        with open(TORCH_STAMP) as f:
+            return f.read() != _torch_version()
+    except OSError:
+        return False  # built elsewhere: nothing is known
+
+
 def _torch_flags() -> list[str]:
     """torch's directories, without importing it (the build needs no more)."""
-    import importlib.util
-    root = os.path.dirname(importlib.util.find_spec("torch").origin)
+    root = _torch_root()
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include")]
     # system headers: warnings in them are not this project's
     return [f"TORCH_INCLUDES={' '.join('-isystem ' + i for i in inc)}", f"TORCH_LIB={os.path.join(root, 'lib')}"]
@@ -78,22 +103,30 @@ def build(jobs: int = 0, quiet: bool = True) -> str:
     jobs = jobs or min(32, os.cpu_count() or 8)
     with _lock():
         _make([f"-j{jobs}"], quiet)
-        _make([f"-j{jobs}", "pymodule", "torchops", *_python_flags(), *_torch_flags()], quiet)
+        again = ["-W", "api/torchops.cpp"] if _torchops_stale() else []  # as if its source were newer
+        _make([f"-j{jobs}", *again, "pymodule", "torchops", *_python_flags(), *_torch_flags()], quiet)
+        with open(TORCH_STAMP, "w") as f:
+            f.write(_torch_version())
     return LIB_PATH
 
 
-def ensure_built(pymodule: bool = False) -> str:
-    """Build the library (and, if asked, TinyGNN's Python module) when it is
-    missing.  Raises ImportError when it is missing and nvcc is not there
-    to build it: the package has no CPU path."""
-    want = [LIB_PATH, torchops_path()] + ([pymodule_path()] if pymodule else [])
-    if all(os.path.exists(p) for p in want):
+def ensure_built(pymodule: bool = False, torchops: bool = False) -> str:
+    """Build the library (and, if asked, TinyGNN's Python module, or the
+    training operators' one) when it is missing, the latter also when it was
+    built against another torch.  Raises ImportError when there is no nvcc to
+    build it: the package has no CPU path."""
+    want = [LIB_PATH] + ([pymodule_path()] if pymodule else []) + ([torchops_path()] if torchops else [])
+
+    def there() -> bool:
+        return all(os.path.exists(p) for p in want) and not (torchops and _torchops_stale())
+
+    if there():
         return LIB_PATH
     if not (os.path.exists(NVCC) or shutil.which("nvcc")):
-        raise ImportError(f"tinygnn_b200: {LIB_PATH} is missing and nvcc is not available to build it "
-                          "(there is no CPU fallback)")
+        raise ImportError(f"tinygnn_b200: {', '.join(want)}: missing, or built against another torch, and nvcc is not "
+                          "available to build it (there is no CPU fallback)")
     with _lock():
-        if all(os.path.exists(p) for p in want):  # another process built it meanwhile
+        if there():  # another process built it meanwhile
             return LIB_PATH
     try:
         build()

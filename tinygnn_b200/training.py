@@ -21,8 +21,11 @@ from typing import NamedTuple, Optional, Union
 import torch
 
 from . import _lib
-from . import _torch_ops as _ops
+from . import build as _build
 from .ops import ACT
+
+_build.ensure_built(torchops=True)
+from . import _torch_ops as _ops  # noqa: E402
 
 _ops.set_errors(_lib.InvalidArgument, _lib.TinyGNNError)
 
