@@ -330,3 +330,14 @@ def test_layer_norm_at_the_steps_of_its_row_split(tg, dtype, cols):
             for got, want, mag in ((dg, (dyd * hh).sum(0), (dyd * hh).abs() * n + dyd.abs() * rough * (1 + hh.abs())),
                                    (db, dyd.sum(0), dyd.abs() * n)):
                 assert ((got.double() - want).abs() <= U[dtype] * want.abs() + mag.sum(0) + TINY[dtype]).all()
+
+
+def test_what_is_no_truth_value_is_refused(tg):
+    """A flag whose truth cannot be told (several elements), and an x of the wrong rank: InvalidArgument, like the others."""
+    x, g, off = rand(4, 8), rand(8, seed=1), torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    w, several = rand(1, 8, 8, seed=2), torch.zeros(2)
+    for call in (lambda: tg.layer_norm(x, g, g, save8=several), lambda: tg.typed_linear(x, w, off, save8=several),
+                 lambda: tg.typed_linear_grad_weight(x, x, off, bias=several),
+                 lambda: tg.typed_linear_backward(x, x[0], w, off)):
+        with pytest.raises(tg.InvalidArgument):
+            call()

@@ -211,6 +211,15 @@ float number(const char* fn, PyObject* o) {
     return static_cast<float>(v);
 }
 
+bool truth(const char* fn, PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        refuse(fn, "a truth value is needed");
+    }
+    return v == 1;
+}
+
 PyObject* wrap(at::Tensor t) { return THPVariable_Wrap(std::move(t)); }
 template <class... A>
 PyObject* pack(A&&... a) {
@@ -309,7 +318,7 @@ PyObject* py_layer_norm(PyObject*, Args a, Py_ssize_t n) {
         const Matrix x = matrix(fn, "x", a[0]);
         const at::Tensor gamma = param(fn, "gamma", a[1], x), beta = param(fn, "beta", a[2], x);
         same_type(fn, "beta", beta, gamma);
-        const bool save = PyObject_IsTrue(a[4]) == 1;
+        const bool save = truth(fn, a[4]);
         void* st = stream_of(fn, x.t);
         at::Tensor y = fresh({x.rows, x.cols}, x.t.scalar_type(), x.t), stats = fresh({x.rows, 2}, at::kFloat, x.t);
         Saved s{};
@@ -398,7 +407,7 @@ PyObject* py_typed_linear(PyObject*, Args a, Py_ssize_t n) {
             same_device(fn, x.t, bias);
             bias = bias.contiguous();
         }
-        const bool save = PyObject_IsTrue(a[6]) == 1;
+        const bool save = truth(fn, a[6]);
         void* st = stream_of(fn, x.t);
         at::Tensor y = fresh({x.rows, w.N}, x.t.scalar_type(), x.t);
         Saved s{};
@@ -440,7 +449,7 @@ PyObject* py_typed_linear_grad_weight(PyObject*, Args a, Py_ssize_t n) {
         const int32_t* off = offsets_of(fn, a[4], -1, dy.t);
         const int64_t types = THPVariable_Unpack(a[4]).numel() - 1;
         if (types < 1) refuse(fn, "offsets need at least two elements");
-        const bool wide = PyObject_IsTrue(a[5]) == 1, bias = PyObject_IsTrue(a[6]) == 1;
+        const bool wide = truth(fn, a[5]), bias = truth(fn, a[6]);
         void* st = stream_of(fn, dy.t);
         at::Tensor dw = fresh({types, K, N}, wide ? at::kFloat : dy.t.scalar_type(), dy.t), db;
         if (bias) db = fresh({types, N}, at::kFloat, dy.t);

@@ -159,8 +159,8 @@ def typed_linear_backward(dy: torch.Tensor, x: Matrix, w: torch.Tensor, offsets:
                           dtype: Optional[torch.dtype] = None, bias: bool = True):
     """(dx, dw, db) of ``x @ w + bias`` (dy: the gradient before the activation,
     :func:`activation_backward`)."""
-    if w.dim() == 3 and w.shape[1] != x.shape[1]:
-        raise _bad(f"typed_linear_backward: dimension mismatch — x has {x.shape[1]} columns, w {tuple(w.shape)}")
+    if w.dim() == 3 and (len(x.shape) != 2 or w.shape[1] != x.shape[1]):
+        raise _bad(f"typed_linear_backward: dimension mismatch — x has shape {tuple(x.shape)}, w {tuple(w.shape)}")
     dx = _ops.typed_linear_grad_input(dy, w, offsets)
     dw, db = typed_linear_grad_weight(x, dy, offsets, dtype, bias)
     return dx, dw, db
