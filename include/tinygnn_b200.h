@@ -101,6 +101,9 @@ TG_API int32_t tg_device_count(void);
 /* How many kernels this library has launched in this process (all devices);
  * used by benchmarks to count their own launches. */
 TG_API uint64_t tg_kernel_launch_count(void);
+/* The library's name for the kernel that the calling thread launched last (""
+ * before its first): which of an entry point's routes a call took. */
+TG_API const char* tg_last_kernel_name(void);
 
 /* Input CSR checks.  Every entry point that reads a caller's CSR first
  * checks it on the device -- Tensor::sparse_csr's checks (src/tensor.cpp:

@@ -341,3 +341,108 @@ def test_what_is_no_truth_value_is_refused(tg):
                  lambda: tg.typed_linear_backward(x, x[0], w, off)):
         with pytest.raises(tg.InvalidArgument):
             call()
+
+
+# Sizes of the types, K, N: products on pairs of CTAs in both directions, more than one tile of 256 columns: last tiles
+# of 88 and 8 columns, of 89 and 7 (rows that TMA cannot read: aligned copies first), of one column and of half a tile,
+# and whole tiles; types of one row, of none, and one whose values are its own.
+PAIRS = [([6001, 0, 1, 5000, 300, 4755, 130], 776, 600), ([6001, 0, 1, 5000, 300, 4755, 130], 775, 601),
+         ([9001, 7000, 0, 300], 640, 513), ([20000], 1024, 768)]
+
+
+def last_kernel():
+    from tinygnn_b200 import _lib
+    return _lib.lib.tg_last_kernel_name().decode()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(PAIRS)))
+def test_products_on_pairs_of_ctas(tg, dtype, case):
+    """Sums of n terms to (n + 16) 2^-23 of their magnitude (the tensor cores may truncate) and the result's rounding; the
+    8-bit copy to half a step more."""
+    sizes, K, N = PAIRS[case]
+    M, T = sum(sizes), len(sizes)
+    o = [0]
+    for n in sizes:
+        o.append(o[-1] + n)
+    off = torch.tensor(o, dtype=torch.int32, device="cuda")
+    x, dy = rand(M, K, seed=1, dtype=dtype), rand(M, N, seed=2, dtype=dtype)
+    w, bias = rand(T, K, N, seed=3, scale=K ** -0.5, dtype=dtype), rand(T, N, seed=4)
+    bad = next((t for t, n in enumerate(sizes) if n == 300), None)
+    if bad is not None:
+        x[o[bad]:o[bad + 1]], dy[o[bad]:o[bad + 1]] = float("nan"), float("inf")
+    y, saved = tg.typed_linear(x, w, off, bias, "relu", save8=True)
+    assert last_kernel() == "typed_rows_pair"
+    plain = tg.typed_linear(x, w, off)
+    assert last_kernel() == "typed_rows_pair"
+    dx = tg.typed_linear_grad_input(dy, w, off)
+    assert last_kernel() == "typed_rows_pair"
+
+    def near(got, want, tol, what):
+        off_by = ~((got.double() - want).abs() <= tol)
+        assert not off_by.any(), (what, int(off_by.sum()), off_by.nonzero()[:3], got[off_by][:3], want[off_by][:3])
+
+    for t in range(T):
+        r = slice(o[t], o[t + 1])
+        if t == bad:
+            assert y[r].isnan().all() and dx[r].isnan().all() and plain[r].isnan().all() and saved.exponents[r].eq(255).all()
+            continue
+        xd, dyd, wd, b = x[r].double(), dy[r].double(), w[t].double(), bias[t].double()
+        z, mag = xd @ wd, xd.abs() @ wd.abs()
+        near(plain[r], z, U[dtype] * z.abs() + (K + 16) * 2.0 ** -23 * mag + TINY[dtype], f"plain {t}")
+        z, err = z + b, (K + 16) * 2.0 ** -23 * (mag + b.abs())
+        want = z.clamp(min=0)
+        near(y[r], want, U[dtype] * want + err + TINY[dtype], f"y {t}")
+        held = tg.Saved8(saved.codes[r], saved.exponents[r], dtype).restore(torch.float32)
+        step = torch.exp2(saved.exponents[r].double() - 127).repeat_interleave(128, 1)[:, :N]
+        near(held, z, 0.5 * step + err, f"saved {t}")
+        top = torch.nn.functional.pad(z.abs(), (0, -N % 128)).view(z.shape[0], (N + 127) // 128, 128).amax(2)
+        room = torch.nn.functional.pad(err, (0, -N % 128)).view(z.shape[0], (N + 127) // 128, 128).amax(2)
+        e = torch.exp2(saved.exponents[r].double() - 127)
+        assert (127 * e >= top - room).all() and (63.5 * e <= top + room).all(), f"exponents {t}"
+        near(dx[r], dyd @ wd.T, U[dtype] * (dyd @ wd.T).abs() + (N + 16) * 2.0 ** -23 * (dyd.abs() @ wd.abs().T) + TINY[dtype], f"dx {t}")
+    again = tg.typed_linear(x, w, off, bias, "relu"), tg.typed_linear_grad_input(dy, w, off)
+    assert torch.equal(again[0].nan_to_num(7.0), y.nan_to_num(7.0)) and torch.equal(again[1].nan_to_num(7.0), dx.nan_to_num(7.0))
+
+
+def test_routes_of_the_typed_products(tg):
+    """Which kernels run on which sides of the rules, so that a test of one of them cannot silently test another."""
+    def rows(M, T, K, N, dtype):
+        off, _ = lay_out(M, T, True)
+        tg.typed_linear(rand(M, K, dtype=dtype), rand(T, K, N, dtype=dtype), off)
+        return last_kernel()
+    b, f = torch.bfloat16, torch.float32
+    assert rows(32, 1, 1024, 1024, b) == "typed_few" and rows(33, 1, 1024, 1024, b) == "typed_rows"
+    assert rows(32, 1, 2048, 2048, b) == "typed_rows" and rows(32, 2, 2048, 2048, f) == "typed_few"
+    assert rows(33, 2, 256, 256, f) == "typed_any" and rows(20000, 4, 512, 512, b) == "typed_rows"
+    assert rows(20000, 4, 520, 512, b) == "typed_rows_pair" and rows(20000, 40, 520, 512, b) == "typed_rows"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,alpha", [("relu", 0.0), ("gelu", 0.0), ("elu", 0.7), (None, 0.0)])
+@pytest.mark.parametrize("rows,cols,pad", [(20011, 1000, 0), (20011, 1003, 0), (6001, 1000, 1), (70001, 41, 0), (3, 9000, 0)])
+def test_activations_over_many_steps(tg, dtype, act, alpha, rows, cols, pad):
+    """More rows than the activation kernels' groups take at once, blocks of columns that do not divide the groups: codes
+    and exponents bit for bit, values to the exponential's 2^-20 of max(|x|, 1) and the result's rounding."""
+    x, dy = rand(rows, cols + pad, seed=1, scale=2.0, dtype=dtype)[:, :cols], rand(rows, cols + pad, seed=2, dtype=dtype)[:, :cols]
+    y, saved = tg.activation_save8(x, act, alpha)
+    nb = (cols + 127) // 128
+    m, e = torch.frexp(torch.nn.functional.pad(x.float().abs(), (0, nb * 128 - cols)).view(rows, nb, 128).amax(2))
+    e = (e - 7 + (m > 127 / 128).int()).clamp(min=-24 if dtype == torch.float16 else -126)
+    assert torch.equal(saved.exponents.int(), e + 127)
+    scale = torch.exp2(e.double()).repeat_interleave(128, 1)[:, :cols]
+    assert torch.equal(saved.codes.double(), torch.round(x.double() / scale))
+    assert torch.equal(saved.restore(torch.float32).double(), saved.codes.double() * scale)
+
+    def forms(z):
+        zd = z.double().requires_grad_(True)
+        v = {"relu": torch.relu, "elu": lambda a: torch.where(a < 0, alpha * torch.expm1(a), a), None: lambda a: a * 1,
+             "gelu": lambda a: 0.5 * a * (1 + torch.tanh(0.7978845608 * (a + 0.044715 * a ** 3)))}[act](zd)
+        return v.detach(), torch.autograd.grad(v.sum(), zd)[0]
+
+    want, slope = forms(x)
+    slack = 2.0 ** -20 * x.double().abs().clamp(min=1)
+    assert ((y.double() - want).abs() <= U[dtype] * want.abs() + slack + TINY[dtype]).all()
+    for given, s in ((x, slope), (saved, forms(saved.restore(torch.float32))[1])):
+        got, want = tg.activation_backward(dy, given, act, alpha), dy.double() * s
+        assert ((got.double() - want).abs() <= U[dtype] * want.abs() + slack * dy.double().abs() + TINY[dtype]).all()

@@ -35,6 +35,7 @@ SIGNATURES = {
     "tg_abi_version": (i32, []),
     "tg_device_count": (i32, []),
     "tg_kernel_launch_count": (u64, []),
+    "tg_last_kernel_name": (C.c_char_p, []),
     "tg_gemm_f32": (i32, [i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, i32, f32, i32, vp]),
     "tg_gemm_pair_f32": (i32, [i64, i64, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i32, vp]),
     "tg_gemm_cat_f32": (i32, [i64, i64, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i32, f32, i32, vp]),

@@ -7,7 +7,7 @@
 
 namespace tg {
 
-void count_launch();     // one per kernel launch (tg_kernel_launch_count)
+void count_launch(const char* name);  // one per kernel launch (tg_kernel_launch_count, tg_last_kernel_name)
 void require_device();   // throws TG_ERR_NO_DEVICE without a GPU
 
 // Launch `kernel<<<grid, block, smem, stream>>>(args...)`, count it and check
@@ -17,7 +17,7 @@ inline void launch(const char* name, K kernel, dim3 grid, dim3 block, size_t sme
                    cudaStream_t s, A... args) {
     if (grid.x == 0 || grid.y == 0 || grid.z == 0) return;
     kernel<<<grid, block, smem, s>>>(args...);
-    count_launch();
+    count_launch(name);
     TG_LAUNCH_CHECK(name);
 }
 
@@ -39,7 +39,7 @@ inline void launch_dependent(const char* name, K kernel, dim3 grid, dim3 block, 
     cfg.attrs = at;
     cfg.numAttrs = 1;
     cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), name);
-    count_launch();
+    count_launch(name);
 }
 
 #ifdef __CUDACC__

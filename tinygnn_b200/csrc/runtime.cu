@@ -16,6 +16,7 @@ namespace {
 thread_local std::string g_last_error;
 thread_local bool g_csr_checks = true;
 std::atomic<uint64_t> g_launches{0};
+thread_local const char* g_last_kernel = "";
 std::mutex g_dev_mu;
 std::vector<int> g_sms;           // per device, 0 = not queried yet
 std::vector<char> g_pool_ready;   // per device
@@ -25,7 +26,10 @@ void set_last_error(const std::string& m) { g_last_error = m; }
 
 bool csr_checks_enabled() { return g_csr_checks; }
 
-void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+void count_launch(const char* name) {
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    g_last_kernel = name;
+}
 
 static int current_device() {
     int dev = 0;
@@ -121,6 +125,8 @@ TG_API int32_t tg_device_count(void) {
 TG_API uint64_t tg_kernel_launch_count(void) {
     return tg::g_launches.load(std::memory_order_relaxed);
 }
+
+TG_API const char* tg_last_kernel_name(void) { return tg::g_last_kernel; }
 
 TG_API int32_t tg_set_csr_checks(int32_t enabled) {
     const int32_t prev = tg::g_csr_checks ? 1 : 0;
