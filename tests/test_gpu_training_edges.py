@@ -446,3 +446,67 @@ def test_activations_over_many_steps(tg, dtype, act, alpha, rows, cols, pad):
     for given, s in ((x, slope), (saved, forms(saved.restore(torch.float32))[1])):
         got, want = tg.activation_backward(dy, given, act, alpha), dy.double() * s
         assert ((got.double() - want).abs() <= U[dtype] * want.abs() + slack * dy.double().abs() + TINY[dtype]).all()
+
+
+def scratch_high(f):
+    """The most bytes of the device's default memory pool (the library's scratch) in use while f runs."""
+    import ctypes
+    cu = ctypes.CDLL("libcuda.so.1")
+    pool, value = ctypes.c_void_p(), ctypes.c_uint64(0)
+    assert cu.cuDeviceGetDefaultMemPool(ctypes.byref(pool), torch.cuda.current_device()) == 0
+    high = 8  # CU_MEMPOOL_ATTR_USED_MEM_HIGH
+    torch.cuda.synchronize()
+    assert cu.cuMemPoolSetAttribute(pool, high, ctypes.byref(value)) == 0
+    f()
+    torch.cuda.synchronize()
+    assert cu.cuMemPoolGetAttribute(pool, high, ctypes.byref(value)) == 0
+    return value.value
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradient_scratch_is_for_cut_types(tg, dtype):
+    """400 types of 512 x 512, one of them long enough to be cut: partial sums for its pieces, not for every type."""
+    T, K, N = 400, 512, 512
+    sizes = [3] * T
+    sizes[7] = 6000
+    M = sum(sizes)
+    off = torch.tensor([0] + torch.tensor(sizes).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    x, dy = rand(M, K, seed=1, dtype=dtype), rand(M, N, seed=2, dtype=dtype)
+    out = []
+    used = scratch_high(lambda: out.append(tg.typed_linear_grad_weight(x, dy, off)))
+    # 2 (148 / 8 tiles + 1) pieces of a MiB and the aligned copies that the route makes (none here)
+    assert 0 < used <= 64 << 20, used
+    dw, db = out[0]
+    for t in (0, 6, 7, 8, 399):
+        a, b = int(off[t]), int(off[t + 1])
+        xd, dyd = x[a:b].double(), dy[a:b].double()
+        want, mag = xd.T @ dyd, xd.abs().T @ dyd.abs()
+        assert ((dw[t].double() - want).abs() <= U[dtype] * want.abs() + (b - a + 16) * 2.0 ** -23 * mag + TINY[dtype]).all(), t
+        assert ((db[t].double() - dyd.sum(0)).abs() <= (b - a + 16) * 2.0 ** -24 * dyd.abs().sum(0)).all(), t
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("types", [37, 300])
+@pytest.mark.parametrize("K,N", [(40, 72), (264, 200)])
+def test_weight_gradients_of_cut_whole_and_empty_types(tg, dtype, types, K, N):
+    """Types of every kind in one call (more than 256 keep their order, fewer run longest first): each whole type's
+    gradient and each cut one's sum of pieces, from both forms of x, dW of both types."""
+    g = torch.Generator().manual_seed(types)
+    sizes = [(0, 1, 63, 64, 65, 200, 1500, 9000)[int(k)] for k in torch.randint(8, (types,), generator=g)]
+    if types > 256:
+        sizes = [n if t % 9 == 0 else n % 64 for t, n in enumerate(sizes)]
+    M = sum(sizes)
+    o = [0] + torch.tensor(sizes).cumsum(0).tolist()
+    off = torch.tensor(o, dtype=torch.int32, device="cuda")
+    x, dy = rand(M, K, seed=1, dtype=dtype), rand(M, N, seed=2, dtype=dtype)
+    saved = tg.save8(x)
+    for given, wide in ((x, None), (saved, None), (x, torch.float32)):
+        dw, db = tg.typed_linear_grad_weight(given, dy, off, dtype=wide)
+        xs = given.double() if given is x else given.restore(torch.float32).double()
+        for t in range(types):
+            xd, dyd, n = xs[o[t]:o[t + 1]], dy[o[t]:o[t + 1]].double(), sizes[t]
+            want, mag = xd.T @ dyd, xd.abs().T @ dyd.abs()
+            assert ((dw[t].double() - want).abs() <= U[dw.dtype] * want.abs() + (n + 16) * 2.0 ** -23 * mag + TINY[dw.dtype]).all(), t
+            assert ((db[t].double() - dyd.sum(0)).abs() <= (n + 16) * 2.0 ** -24 * dyd.abs().sum(0)).all(), t
+        again = tg.typed_linear_grad_weight(given, dy, off, dtype=wide)
+        assert torch.equal(again[0], dw) and torch.equal(again[1], db)

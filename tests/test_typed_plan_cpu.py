@@ -45,14 +45,15 @@ int main() {
             steps += (n[t] + kStep - 1) / kStep;
         }
         overlapping += owned > M;
-        // weight gradients: partial sums of max_pieces() pieces
+        // weight gradients: items of max_pieces() pieces, partial sums of max_slots()
         const int64_t limit = piece_limit(steps, M, types, per, slots, longest);
         const int64_t least = piece_limit(M / kStep, M, types, per, slots, longest);
-        int64_t pieces = 0;
+        int64_t pieces = 0, kept = 0;
         for (int t = 0; t < types; ++t) {
             const int count = piece_count(n[t], limit);
             pieces += count;
             cut += count > 1;
+            kept += count > 1 ? count : 0;
             CHECK(count <= 1 || n[t] > least);  // the join looks at no shorter type
             if (count > 1) {
                 const int64_t len = piece_rows(n[t], count);
@@ -60,6 +61,7 @@ int main() {
             }
         }
         CHECK(pieces <= max_pieces(M, types, per, slots, longest));
+        CHECK(kept <= max_slots(M, types, per, slots, longest));
         // bias gradients: partial sums of M / kBiasChunk + types chunks
         const int64_t rows = bias_chunk(owned, M);
         int64_t chunks = 0;

@@ -118,9 +118,11 @@ struct WeightArgs {
 // steps (`slots` SMs, `per` tiles a type); then it is cut into the fewest equal
 // pieces that have no more.  Items run longest first, dealt out to the CTAs
 // back and forth, so the CTAs' totals come out nearly equal without a counter
-// in memory, and few types are cut at all: a cut type leaves partial sums
-// [piece][K][ldp] (and [piece][N] of db) that a second kernel adds up in
-// their order.
+// in memory, and few types are cut at all: a cut type's pieces leave partial
+// sums [slot][K][ldp] (and [slot][N] of db) that a second kernel adds up in
+// their order.  Slots count the cut types' pieces only (with one for every
+// piece, 1,024 types of 1,024 x 1,024 took 4.3 GB of scratch, most of it for
+// types that are not cut).
 constexpr int kStep = 64;
 constexpr int kSortTypes = 256;  // more types than this keep their order (many items even out anyway)
 
@@ -145,6 +147,10 @@ __host__ __device__ __forceinline__ int64_t piece_limit(int64_t steps, int64_t M
 inline int64_t max_pieces(int64_t M, int types, int64_t per, int slots, int longest) {
     return types + std::max<int64_t>(slots / per, (M / kStep + types) / longest + 1);
 }
+// A cut type has fewer than 2 n / limit pieces.
+inline int64_t max_slots(int64_t M, int types, int64_t per, int slots, int longest) {
+    return 2 * std::max<int64_t>(slots / per + 1, (M / kStep + types) / longest + 1);
+}
 __host__ __device__ __forceinline__ int piece_count(int n, int64_t limit) { return static_cast<int>((n + limit - 1) / limit); }
 // Rows of each piece (the last may have fewer; none is empty, since this is at most `limit`).
 __host__ __device__ __forceinline__ int piece_rows(int n, int count) {
@@ -155,9 +161,10 @@ __device__ __forceinline__ bool piece_before(int types, int rows_u, int u, int r
     return types > kSortTypes ? u < t : rows_u > rows_t || (rows_u == rows_t && u < t);
 }
 
-// One warp: order[i] = the i-th type, prefix[i] = the pieces before it.
+// One warp: order[i] = the i-th type, and above its 16 bits how many types
+// before it are one piece; prefix[i] = the pieces before it.
 __device__ __forceinline__ void plan_pieces(const int32_t* offsets, int types, int64_t M, int per, int slots,
-                                            int longest, int* prefix, uint16_t* order) {
+                                            int longest, int* prefix, uint32_t* order) {
     const int lane = threadIdx.x & 31;
     int64_t steps = 0;
     for (int t = lane; t < types; t += 32) steps += (rows_of(offsets, t, M) + kStep - 1) / kStep;
@@ -165,7 +172,7 @@ __device__ __forceinline__ void plan_pieces(const int32_t* offsets, int types, i
     for (int o = 16; o > 0; o >>= 1) steps += __shfl_xor_sync(0xffffffffu, steps, o);
     const int64_t limit = piece_limit(steps, M, types, per, slots, longest);
     if (types > kSortTypes) {
-        for (int t = lane; t < types; t += 32) order[t] = static_cast<uint16_t>(t);
+        for (int t = lane; t < types; t += 32) order[t] = static_cast<uint32_t>(t);
     } else {
         for (int t = lane; t < types; t += 32) {
             const int n = rows_of(offsets, t, M);
@@ -176,14 +183,17 @@ __device__ __forceinline__ void plan_pieces(const int32_t* offsets, int types, i
             const int key = prefix[t];
             int rank = 0;
             for (int u = 0; u < types; ++u) rank += piece_before(types, prefix[u], u, key, t);
-            order[rank] = static_cast<uint16_t>(t);
+            order[rank] = static_cast<uint32_t>(t);
         }
     }
     __syncwarp();
-    int carry = 0;
+    int carry = 0, whole = 0;
     for (int i0 = 0; i0 < types; i0 += 32) {
         const int i = i0 + lane;
         int n = i < types ? piece_count(rows_of(offsets, order[i], M), limit) : 0;
+        const uint32_t ones = __ballot_sync(0xffffffffu, n == 1);
+        if (i < types) order[i] |= static_cast<uint32_t>(whole + __popc(ones & ((1u << lane) - 1))) << 16;
+        whole += __popc(ones);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, n, o);
@@ -197,21 +207,22 @@ __device__ __forceinline__ void plan_pieces(const int32_t* offsets, int types, i
 
 // Item number `it` in the order above.
 struct WeightItem {
-    int t, p;        // type, piece (of all)
+    int t, p;        // type, slot (of a cut type's piece)
     int in;          // tile of the type
     int64_t r0, r1;  // rows
     bool whole;      // the type is one piece
 };
 __device__ __forceinline__ WeightItem weight_item(const int32_t* offsets, int types, int64_t M, int per,
-                                                  const int* prefix, const uint16_t* order, int64_t it) {
+                                                  const int* prefix, const uint32_t* order, int64_t it) {
     WeightItem m;
-    m.p = static_cast<int>(it / per);
-    m.in = static_cast<int>(it - static_cast<int64_t>(m.p) * per);
-    const int i = find_type(prefix, types, m.p);
-    m.t = order[i];
+    const int p = static_cast<int>(it / per);
+    m.in = static_cast<int>(it - static_cast<int64_t>(p) * per);
+    const int i = find_type(prefix, types, p);
+    m.t = order[i] & 0xffff;
+    m.p = p - static_cast<int>(order[i] >> 16);
     const int b = clamp_row(offsets[m.t], M), e = clamp_row(offsets[m.t + 1], M);
     const int count = prefix[i + 1] - prefix[i], len = piece_rows(e - b, count);
-    m.r0 = b + static_cast<int64_t>(m.p - prefix[i]) * len;
+    m.r0 = b + static_cast<int64_t>(p - prefix[i]) * len;
     m.r1 = m.r0 + len < e ? m.r0 + len : e;
     m.whole = count == 1;
     return m;

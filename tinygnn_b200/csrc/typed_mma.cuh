@@ -35,7 +35,7 @@ struct Shared {
     uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drain;
     uint32_t tmem;
     int prefix[kMaxTypes + 1];
-    uint16_t order[kMaxTypes];  // weight gradients only
+    uint32_t order[kMaxTypes];  // weight gradients only
 };
 
 // TMEM columns: two buffers of an accumulator (SPLIT: of two, see stage_mmas).

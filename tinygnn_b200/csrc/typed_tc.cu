@@ -293,12 +293,12 @@ __global__ void __launch_bounds__(256) typed_weight_join_kernel(const JoinArgs<O
     const int64_t limit = piece_limit(block_sum(steps, sums), g.M, g.types, g.per, g.slots, g.longest);
     const int n = piece_count(rows, limit);
     if (n <= 1) return;  // the weight kernel wrote it
-    // this type's first piece
+    // this type's first slot
     const int len = piece_rows(rows, n);
     int before = 0;
     for (int u = threadIdx.x; u < g.types; u += 256) {
         const int ru = rows_of(g.offsets, u, g.M), nu = piece_count(ru, limit);
-        if (piece_before(g.types, piece_rows(ru, nu), u, len, t)) before += nu;
+        if (nu > 1 && piece_before(g.types, piece_rows(ru, nu), u, len, t)) before += nu;
     }
     const int64_t p = block_sum(before, first);
     const float* part = g.part + p * g.K * g.ldp;
@@ -464,9 +464,10 @@ void typed_weight(const WeightArgs<T, O>& a, cudaStream_t s) {
     w.ldp = (a.N + 7) / 8 * 8;
     // None is, if even all the rows in one type are an SM's share or two steps.
     const bool joined = a.M > 2 * kStep && (per < w.slots || a.M > int64_t(w.longest) * kStep);
-    Scratch<float> part(joined ? static_cast<size_t>(pieces * (a.K * w.ldp + a.N)) : 1, s);
+    const int64_t slots = joined ? max_slots(a.M, a.types, per, w.slots, w.longest) : 0;
+    Scratch<float> part(static_cast<size_t>(slots * (a.K * w.ldp + a.N)), s);
     w.part = part.p;
-    w.db_part = part.p + (joined ? pieces * a.K * w.ldp : 0);
+    w.db_part = part.p + slots * a.K * w.ldp;
     bool done = false;
     if constexpr (sizeof(T) == 2) {
         if (by_tma) {
