@@ -510,3 +510,25 @@ def test_weight_gradients_of_cut_whole_and_empty_types(tg, dtype, types, K, N):
             assert ((db[t].double() - dyd.sum(0)).abs() <= (n + 16) * 2.0 ** -24 * dyd.abs().sum(0)).all(), t
         again = tg.typed_linear_grad_weight(given, dy, off, dtype=wide)
         assert torch.equal(again[0], dw) and torch.equal(again[1], db)
+
+
+def test_a_refused_cuda_call_is_not_reported_again(tg):
+    """A call that the CUDA runtime refuses (a synchronisation inside a capture) fails by itself; the next call, which
+    has nothing wrong, succeeds."""
+    import ctypes
+    from tinygnn_b200 import _lib
+    cu, lib = ctypes.CDLL("libcuda.so.1"), _lib.lib
+    off, x = torch.tensor([0, 4], dtype=torch.int32, device="cuda"), rand(4, 8)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    handle, graph = ctypes.c_void_p(stream.cuda_stream), ctypes.c_void_p()
+    assert cu.cuStreamBeginCapture_v2(handle, 2) == 0  # relaxed: this stream only
+    try:
+        status = lib.tg_typed_check_offsets(4, 1, off.data_ptr(), stream.cuda_stream)
+    finally:
+        cu.cuStreamEndCapture(handle, ctypes.byref(graph))
+    assert status == _lib.CUDA
+    y = x.clone()
+    tg.relu_(y)  # (checks the runtime's last error after its launch)
+    assert torch.equal(y, x.clamp(min=0))
+    tg.check_row_offsets(off, 4)

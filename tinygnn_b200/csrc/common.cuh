@@ -29,9 +29,9 @@ struct Error : std::runtime_error {
 void set_last_error(const std::string& m);
 
 inline void cuda_check(cudaError_t e, const char* what) {
-    if (e != cudaSuccess)
-        fail(TG_ERR_CUDA, std::string(what) + ": " + cudaGetErrorName(e) + " (" +
-                              cudaGetErrorString(e) + ")");
+    if (e == cudaSuccess) return;
+    cudaGetLastError();  // reported here: the next launch's check must not find it again
+    fail(TG_ERR_CUDA, std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")");
 }
 #define TG_CUDA(call) ::tg::cuda_check((call), #call)
 #define TG_LAUNCH_CHECK(name) ::tg::cuda_check(cudaGetLastError(), name)
