@@ -532,3 +532,24 @@ def test_a_refused_cuda_call_is_not_reported_again(tg):
     tg.relu_(y)  # (checks the runtime's last error after its launch)
     assert torch.equal(y, x.clamp(min=0))
     tg.check_row_offsets(off, 4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_very_wide_outputs(tg, dtype):
+    """More columns than 65,535 tiles of any kernel: products of one input column, exact but for the result's rounding;
+    sums of nine rows."""
+    M, N = 9, 65536 * 256 + 300
+    x, dy = rand(M, 1, seed=1, dtype=dtype), rand(M, N, seed=2, dtype=dtype)
+    w, off = rand(1, 1, N, seed=3, dtype=dtype), torch.tensor([0, M], dtype=torch.int32, device="cuda")
+    dw, db = tg.typed_linear_grad_weight(x, dy, off)
+    for c in (slice(0, 1000), slice(N - 1000, N)):
+        xd, dyd = x.double(), dy[:, c].double()
+        want, mag = (xd * dyd).sum(0), (xd * dyd).abs().sum(0)
+        assert ((dw[0, 0, c].double() - want).abs() <= U[dtype] * want.abs() + 25 * 2.0 ** -23 * mag + TINY[dtype]).all()
+        assert ((db[0, c].double() - dyd.sum(0)).abs() <= 25 * 2.0 ** -24 * dyd.abs().sum(0)).all()
+    for rows in (M, 40):
+        xs = rand(rows, 1, seed=4, dtype=dtype)
+        y = tg.typed_linear(xs, w, torch.tensor([0, rows], dtype=torch.int32, device="cuda"))
+        want = xs.double() * w[0, 0, -1000:].double()
+        assert ((y[:, -1000:].double() - want).abs() <= (U[dtype] + 2.0 ** -22) * want.abs() + TINY[dtype]).all()
+        del y

@@ -56,16 +56,16 @@ __global__ void __launch_bounds__(256) typed_bias_kernel(int64_t M, int64_t N, i
         const int64_t per = scan_chunks(offsets, types, M, chunks, prefix);
         if (lane == 0) {
             rows = per;
-            if (blockIdx.x == 0 && blockIdx.y == 0) *chunk_rows = per;
+            if (blockIdx.x == 0) *chunk_rows = per;
         }
     }
     __syncthreads();
-    const int p = blockIdx.x;
+    const int p = blockIdx.x % chunks;  // (a grid's y is too short for the widest matrices)
     if (p >= prefix[types]) return;
     const int t = find_type(prefix, types, p);
     const int64_t r0 = clamp_row(offsets[t], M) + (p - prefix[t]) * rows;
     const int64_t e = clamp_row(offsets[t + 1], M), r1 = r0 + rows < e ? r0 + rows : e;
-    const int64_t n0 = static_cast<int64_t>(blockIdx.y) * 32 * V;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x / chunks) * 32 * V;
     float sum[V] = {};
     const auto col = [&](int j) { return n0 + (ALIGNED ? lane * V + j : j * 32 + lane); };
     if (ALIGNED && col(0) + V <= N) {
@@ -148,7 +148,7 @@ void typed_bias(int64_t M, int64_t N, int types, const int32_t* offsets, const T
     const bool al = rows_aligned16(dY, lddy, sizeof(T));
     const int64_t tile = al ? 32 * (16 / static_cast<int64_t>(sizeof(T))) : 128;
     launch_dependent("typed_linear_grad_bias", al ? typed_bias_kernel<T, true> : typed_bias_kernel<T, false>,
-           dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(ceil_div(N, tile))), dim3(256), 0, s, M, N, types,
+           dim3(static_cast<unsigned>(chunks * ceil_div(N, tile))), dim3(256), 0, s, M, N, types,
            offsets, dY, lddy, part, static_cast<int>(chunks), chunk_rows);
     launch_dependent("typed_linear_grad_bias", typed_bias_join_kernel,
            dim3(static_cast<unsigned>(ceil_div(N, 32)), static_cast<unsigned>(types)), dim3(256), 0, s, M, N, offsets,
