@@ -7,7 +7,8 @@
 //  columns and takes 8 KB.  A step of 64 inner indexes takes 615 cycles (512 at
 //  the tensor cores' peak), at the 1.29 GHz that the power cap leaves: 65,536 x
 //  2,048 x 2,048 bf16 in 437-459 us, 1.2 PFLOP/s, where single CTAs take
-//  481-485 (fewer bytes moved is less power and a higher clock).
+//  481-485 (fewer bytes moved is less power and a higher clock).  For seconds on
+//  end it takes 465 us at 1.28 GHz, with bias, GELU and the 8-bit copy 564.
 //
 //  The structure is typed_tc.cu's: warp 0 loads, warp 1 of rank 0 issues the
 //  MMAs for both CTAs, warps 4-11 empty the two accumulators.

@@ -4,7 +4,8 @@
 //
 //  Saved form of a rows x cols matrix: for each row and each block of 128
 //  columns the least exponent e with max|x| <= 127 * 2^e, and one signed byte
-//  round-to-even(x / 2^e) per value.  A power of two (rather than max|x| / 127)
+//  round-to-even(x / 2^e) per value (at the type's greatest exponent clamped to
+//  63, since 64 * 2^e would overflow it).  A power of two (rather than max|x| / 127)
 //  costs up to one bit of resolution and buys an exact form: every value
 //  code * 2^e has at most 7 significant bits, so bf16 holds it exactly and a
 //  product on the tensor cores reads it with no second rounding; coding is a
@@ -159,8 +160,8 @@ struct Held {
     // The first n values (all, for more; none, for n <= 0) are there.  Whole
     // words that hold one of them are read and kept as they are: values() with
     // n clears the rest, since an instruction on a word here would wait for it
-    // (a layer norm that picked a row's last values out as it asked for the
-    // next rows took OLDFWD us for 65,536 x 511, and 33 for 512).
+    // (a layer norm's gradient that picked a row's last values out as it asked
+    // for the next rows took 92 us for 65,536 x 511, and 76 without).
     __device__ __forceinline__ void fetch(const T* p, int n) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -264,7 +265,8 @@ __device__ __forceinline__ int exponent8(float most, int emin) {
     return (e > emin ? e : emin) + 127;
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
-// 2^-e, the factor from values to codes (0 for a bad block: its codes are 0).
+// 2^-e, the factor from values to codes (0 for a bad block: its finite values
+// get the code 0, the others any; all of them restore as NaN).
 __device__ __forceinline__ float encode8(int byte) { return byte == kBad8 ? 0.0f : pow2f(127 - byte); }
 // 2^e, the factor from codes to values (NaN for a bad block).
 __device__ __forceinline__ float decode8(int byte) {
