@@ -102,7 +102,11 @@ __global__ void __launch_bounds__(256) typed_bias_join_kernel(int64_t M, int64_t
     __shared__ float sh[8][33];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32, t = blockIdx.y;
     wait_for_previous();
-    if (w == 0) scan_types(offsets, t + 1, M, *chunk_rows, prefix);
+    if (w == 0) {  // (a division by a constant where it can be one)
+        const int64_t per = *chunk_rows;
+        if (per == kBiasChunk) scan_types(offsets, t + 1, M, kBiasChunk, prefix);
+        else scan_types(offsets, t + 1, M, per, prefix);
+    }
     __syncthreads();
     const int64_t n = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float sum = 0.0f;
