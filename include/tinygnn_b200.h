@@ -270,6 +270,68 @@ TG_API tg_status tg_typed_linear_grad_weight(int64_t rows, int64_t K, int64_t N,
 TG_API tg_status tg_typed_check_offsets(int64_t rows, int64_t types, const int32_t* offsets,
                                         void* stream);
 
+/* Group norm with an activation: y = act(h * gamma + beta), h = (x - mean) *
+ * rstd over the rows of a graph and the cols / groups neighbouring columns of
+ * a group.  Graph g has the rows [offsets[g], offsets[g + 1]) (graphs + 1
+ * device integers, as for tg_typed_linear; NULL, with graphs 1: all rows); rows
+ * of no graph are not written.  gamma and beta (cols each) are fp32 or of the
+ * rows' type (param_dtype).  stats[2 (g * groups + j)] and the next float receive the
+ * mean and rstd of graph g's group j (zeros for a graph without rows).
+ * At most 2^24 graphs. */
+TG_API tg_status tg_group_norm(int64_t rows, int64_t cols, int64_t groups, int64_t graphs,
+                               const int32_t* offsets, int32_t dtype, const void* x, int64_t ldx,
+                               int32_t param_dtype, const void* gamma, const void* beta, float eps,
+                               int32_t act, float alpha, void* y, int64_t ldy, float* stats,
+                               void* stream);
+/* The backward pass from x and the forward pass's stats (the pre-activation
+ * is computed again): dx, and dgamma and dbeta (param_dtype) over all graphs'
+ * rows, summed in a fixed order. */
+TG_API tg_status tg_group_norm_grad(int64_t rows, int64_t cols, int64_t groups, int64_t graphs,
+                                    const int32_t* offsets, int32_t dtype, const void* dy,
+                                    int64_t lddy, const void* x, int64_t ldx, const float* stats,
+                                    int32_t param_dtype, const void* gamma, const void* beta,
+                                    int32_t act, float alpha, void* dx, int64_t lddx, void* dgamma,
+                                    void* dbeta, void* stream);
+
+/* Rows of class scores (`logits`, rows x classes).  A score of -inf is a
+ * masked class: its probability and its gradient are 0.  A row of masked
+ * classes alone has no probabilities: their logarithms are NaN, its entropy and
+ * its gradient 0; a row with a NaN or +inf gives NaN.
+ *
+ * log_probs[i] = log softmax(logits[i])[labels[i]] (labels of label_bytes 4 or
+ * 8 bytes; one outside [0, classes) is none: 0), entropy[i] = -sum p log p,
+ * stats[2 i] and stats[2 i + 1] the row's maximum and log sum e^(z - max) for
+ * the backward pass.  With top > 0 (at most 128) top_log_probs and top_classes
+ * (rows x top) receive the best classes in falling order, equal scores in the
+ * order of their classes (a NaN counts as the greatest). */
+TG_API tg_status tg_label_log_probs(int64_t rows, int64_t classes, int32_t dtype, const void* logits,
+                                    int64_t ldz, const void* labels, int32_t label_bytes, int64_t top,
+                                    float* log_probs, float* entropy, float* stats,
+                                    float* top_log_probs, int32_t* top_classes, void* stream);
+/* dlogits from the gradients of log_probs and (nullable; entropy is then not
+ * read) of entropy. */
+TG_API tg_status tg_label_log_probs_grad(int64_t rows, int64_t classes, int32_t dtype,
+                                         const float* dlog_probs, const float* dentropy,
+                                         const void* logits, int64_t ldz, const void* labels,
+                                         int32_t label_bytes, const float* stats,
+                                         const float* entropy, void* dlogits, int64_t lddz,
+                                         void* stream);
+
+/* Distillation from a teacher's best logits of each row (top_classes, of
+ * class_bytes 4 or 8 bytes, and top_logits, fp32 or of the logits' type; rows x
+ * k, k at most 128): with q = softmax(top_logits / temperature) over the row's
+ * k classes and p = softmax(logits / temperature) over all classes,
+ * loss[i] = temperature^2 sum q (log q - log p), and dlogits (nullable: the loss
+ * alone) = weights[i] (nullable: 1) times its gradient.  A class outside
+ * [0, classes), and one whose logit is -inf, is none; a row without any has
+ * loss and gradient 0.  A class named twice has both its probabilities.  A row
+ * of masked scores alone has a NaN for its loss and no gradient. */
+TG_API tg_status tg_distill_loss(int64_t rows, int64_t classes, int32_t dtype, const void* logits,
+                                 int64_t ldz, int64_t k, const void* top_classes, int32_t class_bytes,
+                                 int64_t ld_classes, int32_t teacher_dtype, const void* top_logits,
+                                 int64_t ld_logits, float temperature, const float* weights,
+                                 float* loss, void* dlogits, int64_t lddz, void* stream);
+
 /* ── sparse ops ──────────────────────────────────────────────────────────── */
 
 /* C[M,F] = A . B for CSR A (M x K, int32 row_ptr[M+1] / col_ind[nnz], fp32

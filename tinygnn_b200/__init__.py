@@ -15,7 +15,8 @@ from .ops import (CSR, add_bias_, add_self_loops, csr_validate, degree_order, ed
                   spmm, tanh_)
 # The training operators' names, imported on their first use: their module is
 # built against one torch, and the rest of the package needs none of it.
-_TRAINING = ("Saved8", "activation_backward", "activation_save8", "check_row_offsets", "layer_norm",
+_TRAINING = ("Saved8", "activation_backward", "activation_save8", "check_row_offsets", "distill_loss", "group_norm",
+             "group_norm_backward", "label_log_probs", "label_log_probs_backward", "layer_norm",
              "layer_norm_backward", "save8", "typed_linear", "typed_linear_backward", "typed_linear_grad_input",
              "typed_linear_grad_weight")
 

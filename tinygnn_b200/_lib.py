@@ -110,6 +110,12 @@ SIGNATURES = {
     "tg_typed_linear_grad_weight": (i32, [i64, i64, i64, i64, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, i32, vp,
                                           i64, i64, vp, vp]),
     "tg_typed_check_offsets": (i32, [i64, i64, vp, vp]),
+    "tg_group_norm": (i32, [i64, i64, i64, i64, vp, i32, vp, i64, i32, vp, vp, f32, i32, f32, vp, i64, vp, vp]),
+    "tg_group_norm_grad": (i32, [i64, i64, i64, i64, vp, i32, vp, i64, vp, i64, vp, i32, vp, vp, i32, f32, vp, i64, vp,
+                                 vp, vp]),
+    "tg_label_log_probs": (i32, [i64, i64, i32, vp, i64, vp, i32, i64, vp, vp, vp, vp, vp, vp]),
+    "tg_label_log_probs_grad": (i32, [i64, i64, i32, vp, vp, vp, i64, vp, i32, vp, vp, vp, i64, vp]),
+    "tg_distill_loss": (i32, [i64, i64, i32, vp, i64, i64, vp, i32, i64, i32, vp, i64, f32, vp, vp, vp, i64, vp]),
     "tg_take_device_error": (i32, [vp]),
     "tg_ipc_get_handle": (i32, [vp, vp, P64]),
     "tg_ipc_open_handle": (i32, [vp, C.POINTER(vp)]),

@@ -469,6 +469,181 @@ PyObject* py_typed_linear_grad_weight(PyObject*, Args a, Py_ssize_t n) {
     });
 }
 
+// ── group norm ───────────────────────────────────────────────────────────
+// Offsets of the graphs in x's rows; without them one graph has all rows.
+struct Graphs {
+    int64_t n = 1;
+    const int32_t* offsets = nullptr;
+};
+Graphs graphs_of(const char* fn, PyObject* o, const at::Tensor& like) {
+    Graphs g;
+    if (o == Py_None) return g;
+    g.offsets = offsets_of(fn, o, -1, like);
+    g.n = THPVariable_Unpack(o).numel() - 1;
+    if (g.n < 0) refuse(fn, "offsets must have at least one element");
+    return g;
+}
+
+// group_norm(x, gamma, beta, groups, offsets, act, alpha, eps) -> (y, stats)
+PyObject* py_group_norm(PyObject*, Args a, Py_ssize_t n) {
+    return guarded([&] {
+        const char* fn = "group_norm";
+        arity(fn, n, 8);
+        const Matrix x = matrix(fn, "x", a[0]);
+        const at::Tensor gamma = param(fn, "gamma", a[1], x), beta = param(fn, "beta", a[2], x);
+        same_type(fn, "beta", beta, gamma);
+        const int64_t groups = integer(fn, a[3]);
+        if (groups < 1 || x.cols % groups != 0)
+            refuse(fn, std::to_string(x.cols) + " columns cannot be cut into " + std::to_string(groups) + " groups");
+        const Graphs g = graphs_of(fn, a[4], x.t);
+        void* st = stream_of(fn, x.t);
+        at::Tensor y = fresh({x.rows, x.cols}, x.t.scalar_type(), x.t), stats = fresh({g.n, groups, 2}, at::kFloat, x.t);
+        check(tg_group_norm(x.rows, x.cols, groups, g.n, g.offsets, x.dtype, x.p(), x.ld,
+                            dtype_of(fn, "gamma", gamma.scalar_type()), gamma.data_ptr(), beta.data_ptr(),
+                            number(fn, a[7]), static_cast<int>(integer(fn, a[5])), number(fn, a[6]), y.data_ptr(), x.cols,
+                            static_cast<float*>(stats.data_ptr()), st));
+        return pack(y, stats);
+    });
+}
+
+// group_norm_backward(dy, x, stats, gamma, beta, groups, offsets, act, alpha) -> (dx, dgamma, dbeta)
+PyObject* py_group_norm_backward(PyObject*, Args a, Py_ssize_t n) {
+    return guarded([&] {
+        const char* fn = "group_norm_backward";
+        arity(fn, n, 9);
+        const Matrix dy = matrix(fn, "dy", a[0]), x = matrix(fn, "x", a[1]);
+        same_type(fn, "x", x.t, dy.t);
+        same_shape(fn, "x", x.t, dy.rows, dy.cols);
+        same_device(fn, dy.t, x.t);
+        const at::Tensor gamma = param(fn, "gamma", a[3], dy), beta = param(fn, "beta", a[4], dy);
+        same_type(fn, "beta", beta, gamma);
+        const int64_t groups = integer(fn, a[5]);
+        const Graphs g = graphs_of(fn, a[6], dy.t);
+        const at::Tensor& stats = tensor(fn, "stats", a[2]);
+        if (stats.dim() != 3 || stats.size(0) != g.n || stats.size(1) != groups || stats.size(2) != 2 ||
+            stats.scalar_type() != at::kFloat || !stats.is_contiguous() || !stats.is_cuda())
+            refuse(fn, "stats must be a contiguous float32 CUDA tensor of shape (" + std::to_string(g.n) + ", " +
+                           std::to_string(groups) + ", 2)");
+        same_device(fn, dy.t, stats);
+        void* st = stream_of(fn, dy.t);
+        at::Tensor dx = fresh({dy.rows, dy.cols}, dy.t.scalar_type(), dy.t),
+                   dg = fresh({dy.cols}, gamma.scalar_type(), dy.t), db = fresh({dy.cols}, gamma.scalar_type(), dy.t);
+        check(tg_group_norm_grad(dy.rows, dy.cols, groups, g.n, g.offsets, dy.dtype, dy.p(), dy.ld, x.p(), x.ld,
+                                 static_cast<const float*>(stats.data_ptr()), dtype_of(fn, "gamma", gamma.scalar_type()),
+                                 gamma.data_ptr(), beta.data_ptr(), static_cast<int>(integer(fn, a[7])), number(fn, a[8]),
+                                 dx.data_ptr(), dy.cols, dg.data_ptr(), db.data_ptr(), st));
+        return pack(dx, dg, db);
+    });
+}
+
+// ── losses on class scores ───────────────────────────────────────────────
+// One float32 for each row.
+at::Tensor row_values(const char* fn, const char* what, PyObject* o, const Matrix& z) {
+    const at::Tensor& t = tensor(fn, what, o);
+    if (t.dim() != 1 || t.size(0) != z.rows || t.scalar_type() != at::kFloat || !t.is_cuda())
+        refuse(fn, std::string(what) + " must be a float32 CUDA tensor of " + std::to_string(z.rows) + " elements, got shape " +
+                       shape_text(t));
+    same_device(fn, z.t, t);
+    return t.contiguous();
+}
+int int_bytes(const char* fn, const char* what, const at::Tensor& t) {
+    if (!t.is_cuda() || (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong))
+        refuse(fn, std::string(what) + " must be an int32 or int64 CUDA tensor");
+    return t.scalar_type() == at::kLong ? 8 : 4;
+}
+at::Tensor labels_of(const char* fn, PyObject* o, const Matrix& z) {
+    const at::Tensor& t = tensor(fn, "labels", o);
+    int_bytes(fn, "labels", t);
+    if (t.dim() != 1 || t.size(0) != z.rows)
+        refuse(fn, "labels must have shape (" + std::to_string(z.rows) + ",), got " + shape_text(t));
+    same_device(fn, z.t, t);
+    return t.contiguous();
+}
+template <class T>
+T* data(const at::Tensor& t) {
+    return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
+}
+
+// label_log_probs(logits, labels, top) -> (log_probs, entropy, stats[, top_log_probs, top_classes])
+PyObject* py_label_log_probs(PyObject*, Args a, Py_ssize_t n) {
+    return guarded([&] {
+        const char* fn = "label_log_probs";
+        arity(fn, n, 3);
+        const Matrix z = matrix(fn, "logits", a[0]);
+        const at::Tensor labels = labels_of(fn, a[1], z);
+        const int64_t top = integer(fn, a[2]);
+        if (top < 0 || top > z.cols)
+            refuse(fn, "top = " + std::to_string(top) + " is outside [0, " + std::to_string(z.cols) + "]");
+        void* st = stream_of(fn, z.t);
+        at::Tensor lp = fresh({z.rows}, at::kFloat, z.t), entropy = fresh({z.rows}, at::kFloat, z.t),
+                   stats = fresh({z.rows, 2}, at::kFloat, z.t), best, classes;
+        if (top) {
+            best = fresh({z.rows, top}, at::kFloat, z.t);
+            classes = fresh({z.rows, top}, at::kInt, z.t);
+        }
+        check(tg_label_log_probs(z.rows, z.cols, z.dtype, z.p(), z.ld, labels.data_ptr(), int_bytes(fn, "labels", labels),
+                                 top, data<float>(lp), data<float>(entropy), data<float>(stats), data<float>(best),
+                                 data<int32_t>(classes), st));
+        return top ? pack(lp, entropy, stats, best, classes) : pack(lp, entropy, stats);
+    });
+}
+
+// label_log_probs_backward(dlog_probs, logits, labels, stats, dentropy, entropy) -> dlogits
+PyObject* py_label_log_probs_backward(PyObject*, Args a, Py_ssize_t n) {
+    return guarded([&] {
+        const char* fn = "label_log_probs_backward";
+        arity(fn, n, 6);
+        const Matrix z = matrix(fn, "logits", a[1]);
+        const at::Tensor dlog = row_values(fn, "dlog_probs", a[0], z), labels = labels_of(fn, a[2], z);
+        const at::Tensor& stats = tensor(fn, "stats", a[3]);
+        if (stats.dim() != 2 || stats.size(0) != z.rows || stats.size(1) != 2 || stats.scalar_type() != at::kFloat ||
+            !stats.is_contiguous() || !stats.is_cuda())
+            refuse(fn, "stats must be a contiguous float32 CUDA tensor of shape (" + std::to_string(z.rows) + ", 2)");
+        same_device(fn, z.t, stats);
+        at::Tensor dent, entropy;
+        if (a[4] != Py_None) {
+            dent = row_values(fn, "dentropy", a[4], z);
+            if (a[5] == Py_None) refuse(fn, "dentropy needs the forward pass's entropy");
+            entropy = row_values(fn, "entropy", a[5], z);
+        }
+        void* st = stream_of(fn, z.t);
+        at::Tensor dz = fresh({z.rows, z.cols}, z.t.scalar_type(), z.t);
+        check(tg_label_log_probs_grad(z.rows, z.cols, z.dtype, data<float>(dlog), data<float>(dent), z.p(), z.ld,
+                                      labels.data_ptr(), int_bytes(fn, "labels", labels), data<float>(stats),
+                                      data<float>(entropy), dz.data_ptr(), z.cols, st));
+        return wrap(dz);
+    });
+}
+
+// distill_loss(logits, top_classes, top_logits, temperature, weights, grad) -> loss or (loss, dlogits)
+PyObject* py_distill_loss(PyObject*, Args a, Py_ssize_t n) {
+    return guarded([&] {
+        const char* fn = "distill_loss";
+        arity(fn, n, 6);
+        const Matrix z = matrix(fn, "logits", a[0]), t = matrix(fn, "top_logits", a[2]);
+        at::Tensor classes = tensor(fn, "top_classes", a[1]);
+        const int bytes = int_bytes(fn, "top_classes", classes);
+        if (classes.dim() != 2 || classes.size(0) != z.rows || classes.size(1) < 1)
+            refuse(fn, "top_classes must have " + std::to_string(z.rows) + " rows of one class or more, got shape " +
+                           shape_text(classes));
+        const int64_t k = classes.size(1);
+        same_shape(fn, "top_logits", t.t, z.rows, k);
+        if (t.dtype != TG_F32 && t.dtype != z.dtype) refuse(fn, "top_logits must be float32 or of the logits' type");
+        same_device(fn, z.t, classes);
+        same_device(fn, z.t, t.t);
+        classes = classes.contiguous();
+        at::Tensor weights;
+        if (a[4] != Py_None) weights = row_values(fn, "weights", a[4], z);
+        const bool grad = truth(fn, a[5]);
+        void* st = stream_of(fn, z.t);
+        at::Tensor loss = fresh({z.rows}, at::kFloat, z.t), dz;
+        if (grad) dz = fresh({z.rows, z.cols}, z.t.scalar_type(), z.t);
+        check(tg_distill_loss(z.rows, z.cols, z.dtype, z.p(), z.ld, k, classes.data_ptr(), bytes, k, t.dtype, t.p(), t.ld,
+                              number(fn, a[3]), data<float>(weights), data<float>(loss), data<void>(dz), z.cols, st));
+        return grad ? pack(loss, dz) : wrap(loss);
+    });
+}
+
 // check_row_offsets(offsets, rows)
 PyObject* py_check_row_offsets(PyObject*, Args a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -503,6 +678,11 @@ PyMethodDef kMethods[] = {FAST(save8),
                           FAST(typed_linear),
                           FAST(typed_linear_grad_input),
                           FAST(typed_linear_grad_weight),
+                          FAST(group_norm),
+                          FAST(group_norm_backward),
+                          FAST(label_log_probs),
+                          FAST(label_log_probs_backward),
+                          FAST(distill_loss),
                           FAST(check_row_offsets),
                           {"set_errors", py_set_errors, METH_VARARGS, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

@@ -1,0 +1,541 @@
+// ============================================================================
+//  label.cu -- log probabilities of each row's label, with the row's entropy
+//  and its best classes, and the gradient of the first two.
+//
+//      log p_j = d_j - log s,  d_j = z_j - max z,  s = sum e^d_j
+//      H = log s - (sum d_j e^d_j) / s
+//      dz_j = a ([j = label] - p_j) - b p_j (log p_j + H),
+//      a, b the gradients of log p_label and of H
+//
+//  The forward pass reads the scores once.  The best classes come from that
+//  pass too: the k-th greatest of the threads' maxima is not above the k-th
+//  greatest score, so only the threads whose maximum reaches it can hold one
+//  of the k, and only their scores (about k / threads of the row, from L2) are
+//  read again.  The scores above that bound are ranked by (score descending,
+//  class ascending) against each other; those equal to it fill up what is left
+//  in the order of their classes.
+// ============================================================================
+#include <algorithm>
+
+#include <cooperative_groups.h>
+
+#include "logits.cuh"
+
+namespace tg {
+
+namespace {
+
+using namespace logits;
+namespace cg = cooperative_groups;
+
+struct LabelArgs {
+    int64_t rows;
+    int n;             // classes
+    const void* labels;
+    bool wide_labels;  // of 8 bytes
+    int top;
+    float *log_probs, *entropy;
+    float2* stats;     // (max, log s)
+    float* top_log_probs;
+    int32_t* top_classes;
+};
+
+struct RowResult {
+    float m, log_s, entropy;
+};
+template <bool FAST>
+__device__ __forceinline__ RowResult finish_row(const Soft& a) {
+    if (a.m == -INFINITY) return {a.m, 0.0f, 0.0f};  // no class is left
+    const float log_s = logf(a.s);
+    return {a.m, log_s, __fsub_rn(log_s, __fmul_rn(kUnit<FAST>, __fdiv_rn(a.t, a.s)))};
+}
+__device__ __forceinline__ float log_prob(float z, const RowResult& r) {
+    return __fsub_rn(__fsub_rn(z, r.m), r.log_s);  // (NaN where no class is left)
+}
+// What a row's first thread writes.  z: the row.
+template <class T>
+__device__ __forceinline__ void write_row(const LabelArgs& a, int64_t row, const T* z, const RowResult& r) {
+    const int label = class_at(a.labels, row, a.wide_labels);
+    a.log_probs[row] = label >= 0 && label < a.n ? log_prob(to_f32(z[label]), r) : 0.0f;
+    a.entropy[row] = r.entropy;
+    a.stats[row] = make_float2(r.m, r.log_s);
+}
+
+// ── narrow rows ──────────────────────────────────────────────────────────
+template <class T, int LPR, int E, bool TOP>
+__global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const LabelArgs a, const T* x, int64_t ldx) {
+    constexpr bool FAST = sizeof(T) == 2;
+    constexpr float C = FAST ? kLog2e : 1.0f;
+    constexpr int RPB = kNarrowThreads / LPR;
+    extern __shared__ __align__(16) uint8_t sh[];
+    wait_for_previous();
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
+        const int rows = a.rows - r0 < RPB ? static_cast<int>(a.rows - r0) : RPB;
+        const T* st = stage_in(sh, x, ldx, r0, rows, a.n);
+        __syncthreads();
+        float z[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int j = lane + i * LPR;
+            z[i] = sub < rows && j < a.n ? to_f32(st[sub * a.n + j]) : -INFINITY;
+        }
+        Soft s;
+        add_scores<FAST, true>(s, z, C);
+        lanes_soft<FAST, true, LPR>(s, C);
+        const RowResult r = finish_row<FAST>(s);
+        const int64_t row = r0 + sub;
+        if (lane == 0 && sub < rows) write_row(a, row, st + sub * a.n, r);
+        if constexpr (TOP) {
+            uint32_t rank[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) rank[i] = lane + i * LPR < a.n ? rank_of(z[i]) : 0u;
+            uint32_t kept = 0;
+            int kept_class = 0;
+            for (int k = 0; k < a.top; ++k) {
+                uint32_t best = rank[0];
+                int at = 0;
+#pragma unroll
+                for (int i = 1; i < E; ++i)
+                    if (rank[i] > best) best = rank[i], at = i;
+                int j = lane + at * LPR;
+                if (LPR == 32) {
+                    const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+                    j = __reduce_min_sync(0xffffffffu, best == most ? j : INT_MAX);
+                    best = most;
+                } else {
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) {
+                        const uint32_t other = __shfl_xor_sync(0xffffffffu, best, o);
+                        const int oj = __shfl_xor_sync(0xffffffffu, j, o);
+                        if (other > best || (other == best && oj < j)) best = other, j = oj;
+                    }
+                }
+                if (lane == j % LPR) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (i == j / LPR) rank[i] = 0u;
+                }
+                if (lane == k % LPR) kept = best, kept_class = j;
+                if ((k % LPR == LPR - 1 || k == a.top - 1) && k - k % LPR + lane <= k && sub < rows) {
+                    const int64_t o = row * a.top + k - k % LPR + lane;
+                    a.top_log_probs[o] = log_prob(score_of(kept), r);
+                    a.top_classes[o] = kept_class;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ── wide rows ────────────────────────────────────────────────────────────
+constexpr int kCandidates = 1024;  // scores above the bound that are ranked at a time
+constexpr int kEquals = 256;       // scores equal to it that are ranked at a time
+
+// A score and its class as one number: greater for a greater score, and among
+// equal scores for a lower class.  0: none.
+__device__ __forceinline__ uint64_t entry(uint32_t rank, int column) {
+    return static_cast<uint64_t>(rank) << 32 | (0xffffffffu - static_cast<uint32_t>(column));
+}
+__device__ __forceinline__ uint32_t entry_rank(uint64_t e) { return static_cast<uint32_t>(e >> 32); }
+__device__ __forceinline__ int entry_column(uint64_t e) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(e)); }
+
+template <int NT>
+struct TopShared {
+    uint64_t best[kMaxTop];  // this CTA's best, in order
+    uint64_t above[kCandidates];
+    int equal[kEquals];
+    int n_above, n_equal, n_threads;
+    int threads[NT];
+    int sums[NT / 32];
+    uint32_t bound;
+};
+
+// The `k` best scores of the part into sh.best, 0 where it has fewer.  `most`:
+// the rank of this thread's greatest score among its vectors (0 without one).
+template <class T, int NT>
+__device__ __forceinline__ void part_top(TopShared<NT>& sh, const Part<T>& p, uint32_t most, int k) {
+    constexpr int V = kVec<T>;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid < k) sh.best[tid] = 0;
+    // The greatest bound that k maxima reach, bit by bit (any that exactly k
+    // reach will do).
+    uint32_t bound = 0;
+    if (__syncthreads_count(most != 0) >= k) {
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t next = bound | 1u << bit;
+            const int reached = __syncthreads_count(most >= next);
+            if (reached >= k) bound = next;
+            if (reached == k) break;
+        }
+    }
+    int above;
+    for (;;) {
+        if (tid == 0) sh.n_above = sh.n_equal = sh.n_threads = 0;
+        __syncthreads();
+        if (most != 0 && most >= bound) sh.threads[atomicAdd(&sh.n_threads, 1)] = tid;
+        const auto look = [&](float z, int column) {
+            const uint32_t r = rank_of(z);
+            if (r > bound) {
+                const int i = atomicAdd(&sh.n_above, 1);
+                if (i < kCandidates) sh.above[i] = entry(r, column);
+            } else if (r == bound) {
+                const int i = atomicAdd(&sh.n_equal, 1);
+                if (i < kEquals) sh.equal[i] = column;
+            }
+        };
+        if (tid < p.extra) look(to_f32(p.row[p.extra_column(tid)]), p.extra_column(tid));
+        __syncthreads();
+        // A warp for each of those threads' vectors.
+        for (int i = warp; i < sh.n_threads; i += NT / 32)
+            for (int64_t v = p.v0 + sh.threads[i] + static_cast<int64_t>(lane) * NT; v < p.v1; v += 32 * NT) {
+                float z[V];
+                widen(p.load(v), z);
+#pragma unroll
+                for (int j = 0; j < V; ++j) look(z[j], p.column(v) + j);
+            }
+        __syncthreads();
+        above = sh.n_above;
+        const int held = above < kCandidates ? above : kCandidates;
+        // The rank of each among them is its place.
+        for (int i = tid; i < held; i += NT) {
+            const uint64_t e = sh.above[i];
+            int place = 0;
+            for (int j = 0; j < held; ++j) place += sh.above[j] > e;
+            if (place < k) sh.best[place] = e;
+            if (place == k - 1) sh.bound = entry_rank(e);
+        }
+        __syncthreads();
+        if (above <= kCandidates) break;
+        // Too many, as where a row's greatest scores lie with few threads: k of
+        // those that were kept reach a greater bound.
+        bound = sh.bound;
+        __syncthreads();
+    }
+    const int missing = k - above;
+    if (missing <= 0 || bound == 0) return;
+    const int equal = sh.n_equal;
+    if (equal <= kEquals) {
+        for (int i = tid; i < equal; i += NT) {
+            const int column = sh.equal[i];
+            int place = 0;
+            for (int j = 0; j < equal; ++j) place += sh.equal[j] < column;
+            if (place < missing) sh.best[above + place] = entry(bound, column);
+        }
+    } else {
+        // Many equal scores: the first of them in the order of the columns.
+        int found = 0;
+        const auto step = [&](int count, auto&& put) {  // count: this thread's; put(i): its i-th
+            int before = count;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += x;
+            }
+            if (lane == 31) sh.sums[warp] = before;
+            __syncthreads();
+            int total = 0;
+            before -= count;
+            for (int w = 0; w < NT / 32; ++w) {
+                if (w < warp) before += sh.sums[w];
+                total += sh.sums[w];
+            }
+            for (int i = 0; i < count && found + before + i < missing; ++i)
+                sh.best[above + found + before + i] = entry(bound, put(i));
+            found += total;
+            __syncthreads();
+        };
+        const auto is = [&](int column) { return rank_of(to_f32(p.row[column])) == bound; };
+        if (p.extra) step(tid < p.head && is(tid), [&](int) { return tid; });
+        for (int64_t v = p.v0 + tid; v - tid < p.v1 && found < missing; v += NT) {
+            uint32_t mask = 0;
+            if (v < p.v1) {
+                float z[V];
+                widen(p.load(v), z);
+#pragma unroll
+                for (int j = 0; j < V; ++j) mask |= (rank_of(z[j]) == bound ? 1u : 0u) << j;
+            }
+            step(__popc(mask), [&](int i) { return p.column(v) + static_cast<int>(__fns(mask, 0, i + 1)); });
+        }
+        if (p.extra && found < missing)
+            step(tid < p.extra - p.head && is(p.tail + tid), [&](int) { return p.tail + tid; });
+    }
+}
+
+template <int NT, bool TOP>
+struct LabelShared {
+    SoftShared soft;
+    SoftCell mine[2];  // this CTA's state, of even and odd rounds
+    TopShared<NT> top;
+    uint64_t joined[8 * kMaxTop];
+};
+template <int NT>
+struct LabelShared<NT, false> {
+    SoftShared soft;
+    SoftCell mine[2];
+};
+
+template <class T, int NT, bool TOP>
+__global__ void __launch_bounds__(NT, 1024 / NT) label_wide_kernel(const LabelArgs a, const T* x, int64_t ldx) {
+    constexpr bool FAST = sizeof(T) == 2;
+    constexpr float C = FAST ? kLog2e : 1.0f;
+    __shared__ LabelShared<NT, TOP> sh;
+    wait_for_previous();
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
+    const int64_t clusters = gridDim.x / ranks;
+    int round = 0;
+    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += clusters, ++round) {
+        const Part<T> p(x + row * ldx, a.n, rank, ranks);
+        Soft s = scan_part<T, NT, 4, true>(p, C);
+        const float most = s.m;
+        if (threadIdx.x < p.extra) {
+            const float z[1] = {to_f32(p.row[p.extra_column(threadIdx.x)])};
+            add_scores<FAST, true>(s, z, C);
+        }
+        block_soft<FAST, true, NT>(s, C, sh.soft);
+        if (ranks > 1 && threadIdx.x == 0) sh.mine[round & 1].set(s);
+        if constexpr (TOP) part_top<T, NT>(sh.top, p, p.v0 + threadIdx.x < p.v1 ? rank_of(most) : 0u, a.top);
+        if (ranks > 1) {
+            cluster.sync();
+            if (rank == 0) {
+                s = Soft{};
+                if (threadIdx.x % 32 < ranks) s = cluster.map_shared_rank(&sh.mine[round & 1], threadIdx.x % 32)->get();
+                lanes_soft<FAST, true, 32>(s, C);
+            }
+        }
+        if (rank == 0) {
+            const RowResult r = finish_row<FAST>(s);
+            if (threadIdx.x == 0) write_row(a, row, p.row, r);
+            if constexpr (TOP) {
+                __syncthreads();
+                const auto put = [&](int i, uint64_t e) {
+                    a.top_log_probs[row * a.top + i] = log_prob(score_of(entry_rank(e)), r);
+                    a.top_classes[row * a.top + i] = entry_column(e);
+                };
+                if (ranks == 1) {
+                    for (int i = threadIdx.x; i < a.top; i += NT) put(i, sh.top.best[i]);
+                } else {
+                    const int all = ranks * a.top;
+                    for (int i = threadIdx.x; i < all; i += NT)
+                        sh.joined[i] = cluster.map_shared_rank(sh.top.best, i / a.top)[i % a.top];
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < all; i += NT) {
+                        const uint64_t e = sh.joined[i];
+                        int place = 0;
+                        for (int j = 0; j < all; ++j) place += sh.joined[j] > e;
+                        if (place < a.top && e) put(place, e);
+                    }
+                }
+            }
+        }
+        if (TOP && ranks > 1) cluster.sync();  // the CTAs' best have been read
+        __syncthreads();
+    }
+    if (ranks > 1) cluster.sync();  // no CTA leaves while its state may be read
+}
+
+// ── gradient ─────────────────────────────────────────────────────────────
+struct GradArgs {
+    int64_t rows;
+    int n;
+    const void* labels;
+    bool wide_labels;
+    const float2* stats;
+    const float *dlog, *dentropy, *entropy;  // dentropy nullable, then entropy is not read
+};
+// dz_j = a [j = label] - p_j (c0 + c1 d_j), d_j = log p_j in units.
+struct RowGrad {
+    float m, log_s, a, c0, c1;
+    int label;
+};
+template <bool FAST>
+__device__ __forceinline__ RowGrad row_grad(const GradArgs& g, int64_t row) {
+    const float2 s = g.stats[row];
+    RowGrad r{s.x, __fmul_rn(s.y, FAST ? kLog2e : 1.0f), 0.0f, 0.0f, 0.0f, class_at(g.labels, row, g.wide_labels)};
+    if (r.label >= g.n) r.label = -1;
+    if (s.x == -INFINITY) {  // no class is left, no gradient
+        r.m = 0.0f;
+        r.label = -1;
+        return r;
+    }
+    r.a = r.label >= 0 ? g.dlog[row] : 0.0f;
+    r.c0 = r.a;
+    if (g.dentropy) {
+        const float b = g.dentropy[row];
+        r.c0 = fmaf(b, g.entropy[row], r.a);
+        r.c1 = __fmul_rn(b, kUnit<FAST>);
+    }
+    return r;
+}
+template <bool FAST>
+__device__ __forceinline__ float grad_of(float z, const RowGrad& r) {
+    const float d = max_nan(__fsub_rn(__fmul_rn(__fsub_rn(z, r.m), FAST ? kLog2e : 1.0f), r.log_s), -200.0f);
+    return __fmul_rn(-expo<FAST>(d), fmaf(r.c1, d, r.c0));
+}
+
+template <class T, int LPR, int E>
+__global__ void __launch_bounds__(kNarrowThreads) label_grad_narrow_kernel(const GradArgs g, const T* x, int64_t ldx, T* dx,
+                                                                           int64_t lddx) {
+    constexpr bool FAST = sizeof(T) == 2;
+    constexpr int RPB = kNarrowThreads / LPR;
+    extern __shared__ __align__(16) uint8_t sh[];
+    wait_for_previous();
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < g.rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
+        const int rows = g.rows - r0 < RPB ? static_cast<int>(g.rows - r0) : RPB;
+        RowGrad r{};
+        if (sub < rows) r = row_grad<FAST>(g, r0 + sub);
+        T* st = stage_in(sh, x, ldx, r0, rows, g.n);
+        __syncthreads();
+        if (sub < rows) {
+            T* p = st + sub * g.n;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int j = lane + i * LPR;
+                if (j < g.n) {
+                    float y = grad_of<FAST>(to_f32(p[j]), r);
+                    if (j == r.label) y = __fadd_rn(y, r.a);
+                    p[j] = from_f32<T>(y);
+                }
+            }
+        }
+        __syncthreads();
+        stage_out(st, dx, lddx, r0, rows, g.n);
+        __syncthreads();
+    }
+}
+
+// Item i of a row: `per` vectors of it.
+template <class T, int NT, int U>
+__global__ void __launch_bounds__(NT) label_grad_wide_kernel(const GradArgs g, const T* x, int64_t ldx, T* dx, int64_t lddx,
+                                                             int parts) {
+    constexpr bool FAST = sizeof(T) == 2;
+    constexpr int V = kVec<T>;
+    wait_for_previous();
+    const int64_t row = blockIdx.x / parts;
+    const Part<T> p(x + row * ldx, g.n, static_cast<int>(blockIdx.x % parts), parts);
+    T* out = dx + row * lddx;
+    const RowGrad r = row_grad<FAST>(g, row);
+    const bool aligned = (reinterpret_cast<uintptr_t>(out + p.head) & 15) == 0;
+    for_vectors<T, NT, U>(p, [&](int64_t v, float (&z)[V]) {
+        const int first = p.column(v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = grad_of<FAST>(z[j], r);
+        if (static_cast<unsigned>(r.label - first) < V) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (first + j == r.label) z[j] = __fadd_rn(z[j], r.a);
+        }
+        if (aligned) store_v<T, V>(out + first, z);
+        else store_any<T, V>(out + first, z);
+    });
+    if (threadIdx.x < p.extra) {
+        const int j = p.extra_column(threadIdx.x);
+        float y = grad_of<FAST>(to_f32(p.row[j]), r);
+        if (j == r.label) y = __fadd_rn(y, r.a);
+        out[j] = from_f32<T>(y);
+    }
+}
+
+size_t staged_bytes(int rows, int64_t n, size_t size) { return static_cast<size_t>(rows * n) * size + 32; }
+
+}  // namespace
+
+}  // namespace tg
+
+extern "C" {
+
+TG_API tg_status tg_label_log_probs(int64_t rows, int64_t classes, int32_t dtype, const void* logits, int64_t ldz,
+                                    const void* labels, int32_t label_bytes, int64_t top, float* log_probs,
+                                    float* entropy, float* stats, float* top_log_probs, int32_t* top_classes,
+                                    void* stream) {
+    return tg::guard([&] {
+        tg::require_device();
+        using namespace tg;
+        const char* fn = "label_log_probs";
+        logits::check_row_args(fn, rows, classes, dtype, logits, ldz);
+        logits::check_int_bytes(fn, "labels", label_bytes);
+        check_ptr(fn, "labels", labels, rows > 0);
+        check_ptr(fn, "log_probs", log_probs, rows > 0);
+        check_ptr(fn, "entropy", entropy, rows > 0);
+        check_ptr(fn, "stats", stats, rows > 0);
+        if (top < 0 || top > logits::kMaxTop || top > classes)
+            invalid(std::string(fn) + ": top = " + std::to_string(top) + " is outside [0, min(" +
+                    std::to_string(logits::kMaxTop) + ", classes)]");
+        check_ptr(fn, "top_log_probs", top_log_probs, rows > 0 && top > 0);
+        check_ptr(fn, "top_classes", top_classes, rows > 0 && top > 0);
+        if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) invalid(std::string(fn) + ": stats must be 8-byte aligned");
+        const LabelArgs a{rows, static_cast<int>(classes), labels, label_bytes == 8, static_cast<int>(top), log_probs,
+                          entropy, reinterpret_cast<float2*>(stats), top_log_probs, top_classes};
+        cudaStream_t s = as_stream(stream);
+        by_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            const T* x = static_cast<const T*>(logits);
+            if (classes <= logits::kNarrow) {
+                logits::by_narrow(classes, [&](auto lpr, auto e) {
+                    constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = logits::kNarrowThreads / LPR;
+                    auto kern = top ? label_narrow_kernel<T, LPR, E, true> : label_narrow_kernel<T, LPR, E, false>;
+                    launch_dependent("label_log_probs", kern,
+                                     dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB), num_sms() * 16))),
+                                     dim3(logits::kNarrowThreads), staged_bytes(RPB, classes, sizeof(T)), s, a, x, ldz);
+                });
+                return;
+            }
+            const int ranks = logits::row_ranks(rows, classes, 4096);
+            const auto go = [&](auto nt) {
+                constexpr int NT = decltype(nt)::value;
+                const int64_t clusters = std::min<int64_t>(rows, std::max<int64_t>(1, int64_t(num_sms()) * (1024 / NT) * 2 / ranks));
+                auto kern = top ? label_wide_kernel<T, NT, true> : label_wide_kernel<T, NT, false>;
+                logits::launch_clusters("label_log_probs", kern, clusters, ranks, NT, 0, s, a, x, ldz);
+            };
+            if (classes / ranks <= 8192) go(std::integral_constant<int, 128>{});
+            else go(std::integral_constant<int, 512>{});
+        });
+    });
+}
+
+TG_API tg_status tg_label_log_probs_grad(int64_t rows, int64_t classes, int32_t dtype, const float* dlog_probs,
+                                         const float* dentropy, const void* logits, int64_t ldz, const void* labels,
+                                         int32_t label_bytes, const float* stats, const float* entropy, void* dlogits,
+                                         int64_t lddz, void* stream) {
+    return tg::guard([&] {
+        tg::require_device();
+        using namespace tg;
+        const char* fn = "label_log_probs_grad";
+        logits::check_row_args(fn, rows, classes, dtype, logits, ldz);
+        logits::check_int_bytes(fn, "labels", label_bytes);
+        check_ptr(fn, "labels", labels, rows > 0);
+        check_ptr(fn, "dlog_probs", dlog_probs, rows > 0);
+        check_ptr(fn, "stats", stats, rows > 0);
+        check_ptr(fn, "entropy", entropy, rows > 0 && dentropy);
+        check_ptr(fn, "dlogits", dlogits, rows > 0);
+        check_ld(fn, "dlogits", lddz, classes);
+        if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) invalid(std::string(fn) + ": stats must be 8-byte aligned");
+        const GradArgs g{rows, static_cast<int>(classes), labels, label_bytes == 8,
+                         reinterpret_cast<const float2*>(stats), dlog_probs, dentropy, entropy};
+        cudaStream_t s = as_stream(stream);
+        by_dtype(dtype, [&](auto t) {
+            using T = decltype(t);
+            const T* x = static_cast<const T*>(logits);
+            T* dx = static_cast<T*>(dlogits);
+            if (classes <= logits::kNarrow) {
+                logits::by_narrow(classes, [&](auto lpr, auto e) {
+                    constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = logits::kNarrowThreads / LPR;
+                    launch_dependent("label_log_probs_grad", label_grad_narrow_kernel<T, LPR, E>,
+                                     dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB), num_sms() * 16))),
+                                     dim3(logits::kNarrowThreads), staged_bytes(RPB, classes, sizeof(T)), s, g, x, ldz, dx,
+                                     lddz);
+                });
+                return;
+            }
+            constexpr int NT = 256, U = 4;
+            const int parts = static_cast<int>(ceil_div(classes, int64_t(NT) * U * logits::kVec<T>));
+            if (rows * parts > INT32_MAX) invalid(std::string(fn) + ": more than 2^31 blocks of the gradient");
+            launch_dependent("label_log_probs_grad", label_grad_wide_kernel<T, NT, U>,
+                             dim3(static_cast<unsigned>(rows * parts)), dim3(NT), 0, s, g, x, ldz, dx, lddz, parts);
+        });
+    });
+}
+
+}  // extern "C"

@@ -1,5 +1,6 @@
-"""Training operators on torch tensors: layer norm, typed linear maps and 8-bit
-saved activations, each with its backward pass.
+"""Training operators on torch tensors: layer norm, group norm, typed linear maps,
+8-bit saved activations and the losses on class scores, each with its backward
+pass.
 
 Matrices are 2-D CUDA tensors of float32, bfloat16 or float16 with unit column
 stride (any row stride; other orders are copied).  Every function runs on
@@ -164,3 +165,71 @@ def typed_linear_backward(dy: torch.Tensor, x: Matrix, w: torch.Tensor, offsets:
     dx = _ops.typed_linear_grad_input(dy, w, offsets)
     dw, db = typed_linear_grad_weight(x, dy, offsets, dtype, bias)
     return dx, dw, db
+
+
+# ── group norm ───────────────────────────────────────────────────────────────
+def group_norm(x: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, groups: int,
+               offsets: Optional[torch.Tensor] = None, act=None, alpha: float = 0.0, eps: float = 1e-5):
+    """(y, stats): y = act(h * gamma + beta), h = (x - mean) * rstd over the rows
+    of each graph and the cols / groups neighbouring columns of each group.
+
+    x: rows x cols.  offsets: graphs + 1 int32 (:func:`check_row_offsets`),
+    graph g has the rows offsets[g] .. offsets[g + 1]; without them all rows are
+    one graph.  (A batch of N images or sequences of L places, channels last, is
+    ``x.view(N * L, C)`` with the offsets 0, L, 2 L, ...; ``groups=1`` normalises
+    whole graphs, ``groups=cols`` each column of a graph.)  gamma and beta are
+    float32 or of x's type.  stats (graphs x groups x 2, float32) holds (mean,
+    rstd) for the backward pass."""
+    return _ops.group_norm(x, gamma, beta, groups, offsets, _act("group_norm", act), alpha, eps)
+
+
+def group_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, gamma: torch.Tensor,
+                        beta: torch.Tensor, groups: int, offsets: Optional[torch.Tensor] = None, act=None,
+                        alpha: float = 0.0):
+    """(dx, dgamma, dbeta) from the forward pass's x, stats and arguments (the
+    pre-activation is computed again).  dgamma and dbeta have gamma's type."""
+    return _ops.group_norm_backward(dy, x, stats, gamma, beta, groups, offsets, _act("group_norm_backward", act), alpha)
+
+
+# ── losses on class scores ───────────────────────────────────────────────────
+def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top: int = 0):
+    """(log_probs, entropy, stats), with ``top`` also (top_log_probs, top_classes):
+    of each row of scores the log probability of its label, the entropy of its
+    probabilities and its ``top`` (at most 128) best classes in falling order,
+    equal scores in the order of their classes.
+
+    logits: rows x classes.  labels: int32 or int64; one outside the classes is
+    none (log probability 0).  -inf masks a class; a row of masked classes alone
+    has NaNs for log probabilities, the entropy 0 and no gradient, a row with a NaN
+    or +inf NaNs throughout.
+    Results are float32 (top_classes int32); stats (rows x 2) holds (max, log of
+    the sum of e^(z - max)) for the backward pass."""
+    return _ops.label_log_probs(logits, labels, top)
+
+
+def label_log_probs_backward(dlog_probs: torch.Tensor, logits: torch.Tensor, labels: torch.Tensor,
+                             stats: torch.Tensor, dentropy: Optional[torch.Tensor] = None,
+                             entropy: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dlogits from the gradients of log_probs (cross entropy: minus the rows'
+    weights) and, with ``dentropy``, of entropy (both float32, one a row; then the
+    forward pass's ``entropy`` is needed too).  The top alternatives take none."""
+    return _ops.label_log_probs_backward(dlog_probs, logits, labels, stats, dentropy, entropy)
+
+
+def distill_loss(logits: torch.Tensor, top_classes: torch.Tensor, top_logits: torch.Tensor, temperature: float = 1.0,
+                 weights: Optional[torch.Tensor] = None, grad: bool = True):
+    """(loss, dlogits), or the loss alone without ``grad``: each row's divergence
+    from a teacher of which its best logits are known,
+
+        temperature^2 sum_i q_i (log q_i - log p[c_i]),
+        q = softmax(top_logits / temperature), p = softmax(logits / temperature),
+
+    and ``weights`` (float32, one a row; 1 without them) times its gradient: for
+    the mean over the rows they are 1 / rows each.
+
+    top_classes, top_logits: rows x k, k at most 128 (:func:`label_log_probs` with
+    ``top`` gives both: log probabilities will do).  A class outside the logits'
+    classes, or one with a logit of -inf, is none; a row without any has loss and
+    gradient 0; a class that occurs twice has both its probabilities.  A row of
+    masked logits (-inf) alone has a NaN for its loss and no gradient."""
+    return _ops.distill_loss(logits, top_classes, top_logits, temperature, weights, grad)
