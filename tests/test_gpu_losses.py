@@ -271,6 +271,10 @@ def distill64(z, classes, teacher, temperature, weights):
     want = w * (p - qs)
     ln = math.log(n) + 1
     rel = 2.0 ** -21 + 2.0 ** -24 * (chain(n) + 12 + 2 * ln + 6 * (d.nan_to_num(neginf=0.0).abs() + logs))
+    if z.dtype != torch.float32:
+        # w p may be one power of two, its exponent's addend K = max / temperature + log s - log w rounded to fp32 (|K| < 256)
+        k = (z.double().amax(1, keepdim=True).nan_to_num(neginf=0.0).abs() / temperature + logs + w.abs().clamp(min=2.0 ** -64).log().abs()) * 1.4427
+        rel = rel + 2.0 ** -24 * 2 * k.clamp(max=256)
     tq = 2.0 ** -24 * 24 * (1 + (t - t.amax(1, keepdim=True)).nan_to_num(neginf=0.0, nan=0.0).abs().amax(1, keepdim=True))
     tol = U[z.dtype] * want.abs() + w.abs() * (rel * p + (tq + 2.0 ** -23) * qs) + TINY[z.dtype]
     mag = torch.where(q > 0, q * (torch.where(q > 0, q, 1.0).log().abs() + lc.abs() + 1), 0.0).nan_to_num(posinf=0.0).sum(1)
@@ -284,7 +288,8 @@ def check_distill(tg, z, classes, teacher, temperature, weights, what=""):
     assert_within(loss, want_loss, tol_loss, f"{what} loss")
     assert_within(dz, want, tol, f"{what} dlogits")
     alone = tg.distill_loss(z, classes, teacher, temperature, weights, grad=False)
-    assert torch.equal(alone.nan_to_num(nan=-1.0), loss.nan_to_num(nan=-1.0))
+    # (not the same bits: without a gradient a row is shared by other threads, and its sum is in another order)
+    assert_within(alone, want_loss, tol_loss, f"{what} loss alone")
     return loss, dz
 
 

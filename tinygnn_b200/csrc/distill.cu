@@ -38,216 +38,462 @@ struct DistillArgs {
     float* loss;
 };
 
-// The teacher's entry i of a row: a class outside the row is none (-1).
-template <class U>
-__device__ __forceinline__ int teacher_class(const DistillArgs& a, int64_t row, int i) {
-    const int c = class_at(a.classes, row * a.ldc + i, a.wide_classes);
-    return c < a.n ? c : -1;
-}
-template <class U>
-__device__ __forceinline__ float teacher_logit(const DistillArgs& a, int64_t row, int i) {
-    return to_f32(static_cast<const U*>(a.teacher)[row * a.ldt + i]);
-}
+constexpr int kAhead = 4;  // slots of a ring that holds no row
 
-// One row's teacher in shared memory.
+// One row's teacher in shared memory, 16-byte aligned.
 struct Teacher {
-    int* c;      // the classes, -1 for none
-    float* q;    // their probabilities, 0 for none
-    float* sum;  // of the probabilities: 1, or 0 without any
+    int* c;        // the classes, -1 for none
+    float* q;      // their probabilities, 0 for none
+    float* z;      // the student's scores of the classes
+    float* scale;  // the row's weight times the temperature; 0 for a row without entries
+
+    // Room for k entries and the scale, and where they lie in it.
+    static __host__ __device__ constexpr int floats(int k) { return (3 * k + 4) / 4 * 4; }
+    static __device__ __forceinline__ Teacher in(float* room, int k) {
+        return {reinterpret_cast<int*>(room), room + k, room + 2 * k, room + 3 * k};
+    }
 };
 
-// Fills `t` with W lanes; each lane's part of sum q (log q) is returned.
-template <class U, int W>
-__device__ __forceinline__ float read_teacher(const DistillArgs& a, int64_t row, int lane, const Teacher& t) {
+// A lane's entries lane, lane + W, ... of a row as they were read.  They are
+// kept as they lie in memory: an instruction on them would wait for them.
+template <class T, class U, int W>
+struct Entries {
+    static constexpr int N = (kMaxTop + W - 1) / W;
+    uint2 c[N];
+    U v[N];
+    T z[N];  // the student's scores of the classes
+    float weight;
+
+    __device__ __forceinline__ void fetch(const DistillArgs& a, int64_t row, int lane) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = lane + i * W;
+            c[i] = make_uint2(0xffffffffu, 0xffffffffu);
+            if (e >= a.k) continue;
+            if (a.wide_classes) c[i] = static_cast<const uint2*>(a.classes)[row * a.ldc + e];
+            else c[i].x = static_cast<const uint32_t*>(a.classes)[row * a.ldc + e];
+            v[i] = static_cast<const U*>(a.teacher)[row * a.ldt + e];
+        }
+        weight = a.weights ? a.weights[row] : 1.0f;
+    }
+    // Entry i's class; one outside the row is none (-1).
+    __device__ __forceinline__ int class_of(const DistillArgs& a, int i) const {
+        const int j = static_cast<int>(c[i].x);
+        return j >= 0 && j < a.n && (!a.wide_classes || c[i].y == 0) ? j : -1;
+    }
+    __device__ __forceinline__ void fetch_scores(const DistillArgs& a, const T* row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (class_of(a, i) >= 0) z[i] = row[class_of(a, i)];
+    }
+};
+
+// From a row's classes and logits in t.c and t.q (-inf for none), W lanes set
+// their probabilities and the row's scale; each lane's part of sum q (log q) is
+// returned.  (A lane reads what it wrote, and t.c of all lanes.)
+template <int W>
+__device__ __forceinline__ float finish_teacher(const DistillArgs& a, int lane, const Teacher& t, float weight) {
     const float c = __fdiv_rn(1.0f, a.temperature);
     float most = -INFINITY;
-    for (int i = lane; i < a.k; i += W) {
-        const int j = teacher_class<U>(a, row, i);
-        const float v = j >= 0 ? teacher_logit<U>(a, row, i) : -INFINITY;
-        t.c[i] = v == -INFINITY ? -1 : j;
-        t.q[i] = v;
-        most = max_nan(most, v);
-    }
+    for (int i = lane; i < a.k; i += W) most = max_nan(most, t.q[i]);
     most = reduce_max<W>(most);
     float s = 0.0f;
     for (int i = lane; i < a.k; i += W) s = __fadd_rn(s, t.c[i] >= 0 ? expf(distance(t.q[i], most, c)) : 0.0f);
     s = reduce_sum<float, W>(s);
     const float log_s = logf(s);
     float entropy = 0.0f;
+    bool twice = false;
     for (int i = lane; i < a.k; i += W) {
         float q = 0.0f;
-        if (t.c[i] >= 0) {
+        const int j = t.c[i];
+        if (j >= 0) {
             const float l = __fsub_rn(distance(t.q[i], most, c), log_s);
             q = expf(l);
             if (q != 0.0f) entropy = fmaf(q, l, entropy);
         }
         t.q[i] = q;
     }
-    if (lane == 0) *t.sum = most == -INFINITY ? 0.0f : 1.0f;
+    __syncwarp();
+    // Classes that occur more than once: the first entry takes all their probabilities.
+    for (int i = lane; i < a.k; i += W) {
+        const int j = t.c[i];
+        int same = 0;
+        int o = 0;
+        for (; o + 4 <= a.k; o += 4) {
+            const int4 c4 = *reinterpret_cast<const int4*>(t.c + o);
+            same += (c4.x == j) + (c4.y == j) + (c4.z == j) + (c4.w == j);
+        }
+        for (; o < a.k; ++o) same += t.c[o] == j;
+        twice |= j >= 0 && same > 1;
+    }
+    if (__any_sync(0xffffffffu, twice)) {
+        // First the later ones are marked (-2 - class: lanes still read classes), then the first adds theirs up.
+        const auto class_in = [&](int e) { return t.c[e] < -1 ? -2 - t.c[e] : t.c[e]; };
+        for (int i = lane; i < a.k; i += W) {
+            const int j = class_in(i);
+            bool later = false;
+            for (int o = 0; o < i; ++o) later |= class_in(o) == j;
+            if (j >= 0 && later) t.c[i] = -2 - j;
+        }
+        __syncwarp();
+        for (int i = lane; i < a.k; i += W)
+            if (t.c[i] >= 0)
+                for (int o = i + 1; o < a.k; ++o)
+                    if (t.c[o] == -2 - t.c[i]) t.q[i] = __fadd_rn(t.q[i], t.q[o]);
+        __syncwarp();
+        for (int i = lane; i < a.k; i += W)
+            if (t.c[i] < 0) t.c[i] = -1, t.q[i] = 0.0f;
+    }
+    if (lane == 0) *t.scale = most == -INFINITY ? 0.0f : __fmul_rn(a.temperature, weight);
+    __syncwarp();
     return entropy;
 }
 
-// log p of a score in natural units (the row's maximum m, log of its sum);
-// NaN in a row without any score above -inf.
-__device__ __forceinline__ float log_p(float z, float m, float log_s, float c) {
-    return __fsub_rn(__fmul_rn(__fsub_rn(z, m), c), log_s);
+// Fills `t` from a warp's entries; returned as above.
+template <class T, class U>
+__device__ __forceinline__ float read_teacher(const DistillArgs& a, const Entries<T, U, 32>& in, int lane, const Teacher& t) {
+#pragma unroll
+    for (int i = 0; i < in.N; ++i) {
+        const int e = lane + i * 32, j = in.class_of(a, i);
+        if (e >= a.k) continue;
+        const float v = j >= 0 ? to_f32(in.v[i]) : -INFINITY;
+        t.z[e] = j >= 0 ? to_f32(in.z[i]) : 0.0f;
+        t.c[e] = v == -INFINITY ? -1 : j;
+        t.q[e] = v;
+    }
+    return finish_teacher<32>(a, lane, t, in.weight);
 }
 
+// What a row's gradient takes from its softmax.  c: the exponential's units in
+// 1 / T.
+template <bool FAST>
 struct RowScale {
-    float m, c, log_s, w;  // origin, factor and log of the sum in the exponential's units; w T, 0 for rows without gradient
+    Origin o;
+    float c, log_s;  // log of the sum, in the exponential's units
+    float w;         // w T; 0 for a row without gradient
+    // Where fp32 holds them well the origin, the sum and the weight go into one
+    // addend: w p = +-2^(z c - K).  (|M| <= 64 and a weight above 2^-64 keep |K|
+    // below 256, and its rounding, 2^-17 at most, far below a 16-bit result's 2^-12.)
+    float K;
+    bool quick;
+    uint32_t sign;  // of two 16-bit results
+
+    __device__ __forceinline__ RowScale(const Soft& s, float c_, float scale) : o(s.m, c_), c(c_) {
+        log_s = __fmul_rn(logf(s.s), FAST ? kLog2e : 1.0f);
+        w = s.m == -INFINITY ? 0.0f : scale;  // (no class is left, no gradient)
+        quick = FAST && fabsf(o.M) <= 64.0f && fabsf(w) > 5.421e-20f;
+        K = __fsub_rn(__fadd_rn(o.M, log_s), __log2f(fabsf(w)));
+        sign = w < 0.0f ? 0x80008000u : 0u;
+    }
+    // log p of a score in natural units; NaN in a row without any score above -inf.
+    __device__ __forceinline__ float log_p(float z) const {
+        if (!FAST) return __fsub_rn(__fmul_rn(__fsub_rn(z, o.m), c), log_s);
+        return __fmul_rn(__fsub_rn(o.d(z, c), log_s), kLn2);
+    }
+    __device__ __forceinline__ float prob(float z) const {
+        const float d = FAST ? o.d(z, c) : __fmul_rn(__fsub_rn(z, o.m), c);
+        return expo<FAST>(max_nan(__fsub_rn(d, log_s), -200.0f));
+    }
 };
+// The gradient at a class that the teacher does not name.
 template <bool FAST>
-__device__ __forceinline__ RowScale row_scale(const DistillArgs& a, int64_t row, const Soft& s, float sum_q) {
-    RowScale r;
-    r.m = origin(s.m);
-    r.c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
-    r.log_s = s.m == -INFINITY ? 0.0f : __fmul_rn(logf(s.s), FAST ? kLog2e : 1.0f);
-    r.w = sum_q == 0.0f || s.m == -INFINITY ? 0.0f : __fmul_rn(a.temperature, a.weights ? a.weights[row] : 1.0f);
-    return r;
+__device__ __forceinline__ float grad_of(float z, const RowScale<FAST>& r) {
+    return r.w == 0.0f ? 0.0f : __fmul_rn(r.w, r.prob(z));
 }
+// The gradient at the teacher's entry i.
 template <bool FAST>
-__device__ __forceinline__ float prob(float z, const RowScale& r) {
-    return expo<FAST>(max_nan(__fsub_rn(__fmul_rn(__fsub_rn(z, r.m), r.c), r.log_s), -200.0f));
+__device__ __forceinline__ float entry_grad(const Teacher& t, int i, const RowScale<FAST>& r) {
+    return __fmul_rn(r.w, __fsub_rn(r.prob(t.z[i]), t.q[i]));
 }
-// The gradient at the teacher's entry i, whose score is z: where the class
-// occurs more than once the first entry answers for all (false for the others).
-template <bool FAST>
-__device__ __forceinline__ bool entry_grad(const Teacher& t, int i, float z, const RowScale& r, int k, float& y) {
-    const int c = t.c[i];
-    for (int j = 0; j < i; ++j)
-        if (t.c[j] == c) return false;
-    float q = t.q[i];
-    for (int j = i + 1; j < k; ++j)
-        if (t.c[j] == c) q = __fadd_rn(q, t.q[j]);
-    y = __fmul_rn(r.w, __fsub_rn(prob<FAST>(z, r), q));
-    return true;
+// The same for this thread's vectors of a row in the ring, of which slot `at` is
+// the first and which has `have` vectors; each slot is asked into again.
+// Returns the slot after the last.
+template <bool FAST, class T, int NT>
+__device__ __forceinline__ int write_grad(Stream<T, NT>& in, int at, int steps, int have, const RowScale<FAST>& r, T* to, bool aligned,
+                                          bool wait = false) {
+    constexpr int V = kVec<T>, W = Stream<T, NT>::W;
+    const Pair c(r.c, r.c), k(-r.K, -r.K);
+    for (int i = 0; i < steps; ++i, have -= NT * W) {
+        if (wait) in.template wait<kAhead - 1>();
+        uint32_t raw[4 * W];
+        float z[W * V];
+        in.read(at, have, raw);
+        in.scores(raw, z);
+        if (r.quick) {
+#pragma unroll
+            for (int j = 0; j < W * V; j += 2) {
+                float x, y;
+                fma2(Pair(z[j], z[j + 1]), c, k).get(x, y);
+                z[j] = expo<FAST>(x), z[j + 1] = expo<FAST>(y);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < W * V; ++j) z[j] = grad_of<FAST>(z[j], r);
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            float y[V];
+            Raw<T, V> out;
+#pragma unroll
+            for (int j = 0; j < V; ++j) y[j] = z[w * V + j];
+            narrow(y, out);
+            if (sizeof(T) == 2 && r.quick) {
+#pragma unroll
+                for (int j = 0; j < out.N; ++j) out.w[j] ^= r.sign;
+            }
+            if (have <= w * NT + Team<NT>::thread()) continue;
+            if (aligned) *reinterpret_cast<Raw<T, V>*>(to + w * NT * V) = out;
+            else store_words(to + w * NT * V, out);
+        }
+        to += NT * W * V;
+        at = in.next(at);
+        in.ask();
+    }
+    return at;
 }
 
 // ── narrow rows ──────────────────────────────────────────────────────────
 template <class T, class U, int LPR, int E, bool GRAD>
 __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const DistillArgs a, const T* x, int64_t ldx, T* dx,
-                                                                        int64_t lddx, int stage) {
+                                                                        int64_t lddx, int turns, int stage) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int RPB = kNarrowThreads / LPR;
     extern __shared__ __align__(16) uint8_t sh[];
     wait_for_previous();
-    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    int* room = reinterpret_cast<int*>(sh + stage) + sub * (2 * a.k + 1);
-    const Teacher t{room, reinterpret_cast<float*>(room + a.k), reinterpret_cast<float*>(room + 2 * a.k)};
-    const float cn = __fdiv_rn(1.0f, a.temperature), c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
-        const int rows = a.rows - r0 < RPB ? static_cast<int>(a.rows - r0) : RPB;
-        const int64_t row = r0 + (sub < rows ? sub : 0);
+    const int lane = threadIdx.x % LPR, place = threadIdx.x / LPR, per = RPB * turns;
+    const Teacher t = Teacher::in(reinterpret_cast<float*>(sh + stage) + place * Teacher::floats(a.k), a.k);
+    const float c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
+        const int rows = a.rows - r0 < per ? static_cast<int>(a.rows - r0) : per;
         T* st = stage_in(sh, x, ldx, r0, rows, a.n);
-        float loss = read_teacher<U, LPR>(a, row, lane, t);
         __syncthreads();
-        T* p = st + (sub < rows ? sub : 0) * a.n;
-        float z[E];
+        for (int first = 0; first < rows; first += RPB) {
+            // (lanes without a row compute the first one's, and write nothing)
+            const bool here = first + place < rows;
+            const int sub = here ? first + place : first;
+            const int64_t row = r0 + sub;
+            T* p = st + sub * a.n;
+            for (int i = lane; i < a.k; i += LPR) {
+                const int j = class_at(a.classes, row * a.ldc + i, a.wide_classes);
+                const bool in = j >= 0 && j < a.n;
+                const float v = in ? to_f32(static_cast<const U*>(a.teacher)[row * a.ldt + i]) : -INFINITY;
+                t.z[i] = in ? to_f32(p[j]) : 0.0f;
+                t.c[i] = v == -INFINITY ? -1 : j;
+                t.q[i] = v;
+            }
+            float z[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int j = lane + i * LPR;
-            z[i] = j < a.n ? to_f32(p[j]) : -INFINITY;
-        }
-        Soft s;
-        add_scores<FAST, false>(s, z, c);
-        lanes_soft<FAST, false, LPR>(s, c);
-        const float log_s = logf(s.s);
-        for (int i = lane; i < a.k; i += LPR)
-            if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], log_p(to_f32(p[t.c[i]]), s.m, log_s, cn), loss);
-        loss = reduce_sum<float, LPR>(loss);
-        if (lane == 0 && sub < rows) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
-        if constexpr (GRAD) {
-            const RowScale r = row_scale<FAST>(a, row, s, *t.sum);
-            __syncwarp();
-            if (sub < rows) {
+            for (int i = 0; i < E; ++i) {
+                const int j = lane + i * LPR;
+                z[i] = j < a.n ? to_f32(p[j]) : -INFINITY;
+            }
+            __syncwarp();  // (before the row's first lanes write over its scores)
+            float loss = finish_teacher<LPR>(a, lane, t, a.weights ? a.weights[row] : 1.0f);
+            Soft s;
+            add_scores<FAST, false>(s, z, c);
+            lanes_soft<FAST, false, LPR>(s, c);
+            const RowScale<FAST> r(s, c, *t.scale);
+            for (int i = lane; i < a.k; i += LPR)
+                if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.log_p(t.z[i]), loss);
+            loss = reduce_sum<float, LPR>(loss);
+            if (lane == 0 && here) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
+            if constexpr (GRAD) {
+                if (here) {
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const int j = lane + i * LPR;
-                    if (j < a.n) p[j] = from_f32<T>(r.w == 0.0f ? 0.0f : __fmul_rn(r.w, prob<FAST>(z[i], r)));
+                    for (int i = 0; i < E; ++i) {
+                        const int j = lane + i * LPR;
+                        if (j < a.n) p[j] = from_f32<T>(grad_of<FAST>(z[i], r));
+                    }
                 }
+                __syncwarp();
+                if (here && r.w != 0.0f)
+                    for (int i = lane; i < a.k; i += LPR)
+                        if (t.c[i] >= 0) p[t.c[i]] = from_f32<T>(entry_grad<FAST>(t, i, r));
             }
-            __syncwarp();
-            if (sub < rows && r.w != 0.0f) {
-                const T* from = x + row * ldx;
-                float y;
-                for (int i = lane; i < a.k; i += LPR)
-                    if (t.c[i] >= 0 && entry_grad<FAST>(t, i, to_f32(from[t.c[i]]), r, a.k, y)) p[t.c[i]] = from_f32<T>(y);
-            }
-            __syncthreads();
-            stage_out(st, dx, lddx, r0, rows, a.n);
+            __syncwarp();  // (before the next row's entries)
         }
         __syncthreads();
+        if constexpr (GRAD) {
+            stage_out(st, dx, lddx, r0, rows, a.n);
+            __syncthreads();
+        }
+    }
+}
+
+// ── rows of a warp ───────────────────────────────────────────────────────
+// As the wide rows' kernel below, with a warp in the place of the block: of the
+// ring's slots kAhead are for the next rows.
+constexpr int kTeams = 4;
+
+template <class T, class U, bool GRAD>
+__global__ void __launch_bounds__(32 * kTeams, 5) distill_warp_kernel(const DistillArgs a, const T* x, int64_t ldx, T* dx,
+                                                                      int64_t lddx, int slots) {
+    constexpr bool FAST = sizeof(T) == 2;
+    extern __shared__ __align__(16) uint8_t room[];
+    wait_for_previous();
+    const int lane = threadIdx.x & 31, team = threadIdx.x >> 5;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kTeams, first = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+    const float c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
+    Stream<T, 32> in(x, ldx, a.rows, a.n, first, step, 0, 0, room + team * slots * Stream<T, 32>::kSlot, slots, false);
+    const Teacher t = Teacher::in(
+        reinterpret_cast<float*>(room + kTeams * slots * Stream<T, 32>::kSlot) + team * Teacher::floats(a.k), a.k);
+    // (a row's entries are asked for a row ahead, the scores of their classes at its start)
+    Entries<T, U, 32> entries;
+    if (first < a.rows) entries.fetch(a, first, lane);
+    for (int64_t row = first; row < a.rows; row += step) {
+        const Part<T> p(x + row * ldx, a.n, 0, 0);
+        T beside{};
+        if (lane < p.extra) beside = p.row[p.extra_column(lane)];
+        entries.fetch_scores(a, p.row);
+        Soft s;
+        const int steps = in.steps_of(p), mine_first = in.from, count = p.v1 - p.v0;
+        in.template wait<kAhead>();
+        for (int i = 0, have = count; i < steps; ++i, have -= 32 * in.W) {
+            in.template add<false>(s, in.from, have, c);
+            in.from = in.next(in.from);
+            if (!GRAD) in.ask();
+        }
+        if (lane < p.extra) {
+            const float z[1] = {to_f32(beside)};
+            add_scores<FAST, false>(s, z, c);
+        }
+        lanes_soft<FAST, false, 32>(s, c);
+        float loss = read_teacher<T, U>(a, entries, lane, t);
+        if (row + step < a.rows) entries.fetch(a, row + step, lane);
+        const RowScale<FAST> r(s, c, *t.scale);
+        for (int i = lane; i < a.k; i += 32)
+            if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.log_p(t.z[i]), loss);
+        loss = reduce_sum<float, 32>(loss);
+        if (lane == 0) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
+        if constexpr (GRAD) {
+            T* out = dx + row * lddx;
+            write_grad<FAST, T, 32>(in, mine_first, steps, count, r, out + p.column(p.v0 + lane),
+                                    (reinterpret_cast<uintptr_t>(out + p.head) & 15) == 0);
+            if (lane < p.extra) out[p.extra_column(lane)] = from_f32<T>(grad_of<FAST>(to_f32(beside), r));
+            __syncwarp();
+            if (r.w != 0.0f)
+                for (int i = lane; i < a.k; i += 32)
+                    if (t.c[i] >= 0) out[t.c[i]] = from_f32<T>(entry_grad<FAST>(t, i, r));
+        }
+        __syncwarp();  // (before the next row's entries)
     }
 }
 
 // ── wide rows ────────────────────────────────────────────────────────────
+// NT threads read the row (Stream), and one warp more has the teacher: it sets
+// the entries' gradients right once the row's p are written, and reads the next
+// row's entries, while the others read the next row.
+//
+// With `hold` a CTA's part of the row fills the ring and stays there until its p
+// are written, slot by slot the next row's after that; the other CTAs of the SM
+// keep it busy meanwhile (three of 256 threads: 1,004 us for 8,192 x 131,072 bf16;
+// two with four slots for the next row 1,147, one of 512 threads 1,286).  Without
+// it (parts that do not fit) the row is read twice.
+
+struct alignas(16) TeacherShared {
+    int c[2][kMaxTop];
+    float q[2][kMaxTop], z[2][kMaxTop], scale[2];
+};
+
 template <class T, class U, int NT, bool GRAD>
-__global__ void __launch_bounds__(NT, 1024 / NT) distill_wide_kernel(const DistillArgs a, const T* x, int64_t ldx, T* dx,
-                                                                     int64_t lddx) {
+__global__ void __launch_bounds__(NT + 32, 768 / NT) distill_wide_kernel(const DistillArgs a, const T* x, int64_t ldx, T* dx, int64_t lddx,
+                                                               int slots, bool hold) {
     constexpr bool FAST = sizeof(T) == 2;
-    constexpr int V = kVec<T>;
     __shared__ SoftShared soft;
     __shared__ SoftCell mine[2];  // this CTA's state, of even and odd rounds
-    __shared__ int tc[kMaxTop];
-    __shared__ float tq[kMaxTop];
-    __shared__ float tsum;
-    const Teacher t{tc, tq, &tsum};
+    __shared__ TeacherShared teacher;
+    extern __shared__ __align__(16) uint8_t room[];
     wait_for_previous();
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
-    const int64_t clusters = gridDim.x / ranks;
-    const float cn = __fdiv_rn(1.0f, a.temperature), c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
+    const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks()), log_ranks = __ffs(ranks) - 1;
+    const int64_t clusters = gridDim.x / ranks, first = blockIdx.x / ranks;
+    const float c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
+    const auto meet = [] { asm volatile("bar.sync 2, %0;" ::"n"(NT + 32) : "memory"); };
+    const auto all = [&] {  // the CTAs' states are there
+        if (ranks > 1) cluster.sync();
+        else meet();
+    };
+    const auto joined = [&](int b) {
+        Soft s;
+        const int lane = threadIdx.x % 32;
+        if (ranks == 1) return mine[b].get();
+        if (lane < ranks) s = cluster.map_shared_rank(&mine[b], lane)->get();
+        lanes_soft<FAST, false, 32>(s, c);
+        return s;
+    };
     int round = 0;
-    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += clusters, ++round) {
-        float loss = 0.0f;
-        if (threadIdx.x < 32) loss = read_teacher<U, 32>(a, row, threadIdx.x, t);
-        const Part<T> p(x + row * ldx, a.n, rank, ranks);
-        Soft s = scan_part<T, NT, 4, false>(p, c);
-        if (threadIdx.x < p.extra) {
-            const float z[1] = {to_f32(p.row[p.extra_column(threadIdx.x)])};
-            add_scores<FAST, false>(s, z, c);
-        }
-        block_soft<FAST, false, NT>(s, c, soft);
-        if (ranks > 1) {
-            if (threadIdx.x == 0) mine[round & 1].set(s);
-            cluster.sync();
-            s = Soft{};
-            if (threadIdx.x % 32 < ranks) s = cluster.map_shared_rank(&mine[round & 1], threadIdx.x % 32)->get();
-            lanes_soft<FAST, false, 32>(s, c);
-        }
-        if (rank == 0 && threadIdx.x < 32) {
-            const float log_s = logf(s.s);
-            for (int i = threadIdx.x; i < a.k; i += 32)
-                if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], log_p(to_f32(p.row[t.c[i]]), s.m, log_s, cn), loss);
-            loss = reduce_sum<float, 32>(loss);
-            if (threadIdx.x == 0) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
-        }
-        if constexpr (GRAD) {
-            T* out = dx + row * lddx;
-            const RowScale r = row_scale<FAST>(a, row, s, *t.sum);
-            const bool aligned = (reinterpret_cast<uintptr_t>(out + p.head) & 15) == 0;
-            const auto grad = [&](float z) { return r.w == 0.0f ? 0.0f : __fmul_rn(r.w, prob<FAST>(z, r)); };
-            for_vectors<T, NT, 4>(p, [&](int64_t v, float (&z)[V]) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) z[j] = grad(z[j]);
-                if (aligned) store_v<T, V>(out + p.column(v), z);
-                else store_any<T, V>(out + p.column(v), z);
-            });
+    if (threadIdx.x < NT) {
+        Stream<T, NT> in(x, ldx, a.rows, a.n, first, clusters, rank, log_ranks, room, slots, GRAD && !hold);
+        for (int64_t row = first; row < a.rows; row += clusters, ++round) {
+            const int b = round & 1;
+            const Part<T> p(x + row * ldx, a.n, rank, log_ranks);
+            T beside{};
+            if (threadIdx.x < p.extra) beside = p.row[p.extra_column(threadIdx.x)];
+            Soft s;
+            const int steps = in.steps_of(p), mine_first = in.from;
+            const int count = p.v1 - p.v0;
+            if (GRAD && hold) in.template wait<0>();
+            for (int i = 0, have = count; i < steps; ++i, have -= NT * in.W) {
+                if (!(GRAD && hold)) in.template wait<kAhead - 1>();
+                in.template add<false>(s, in.from, have, c);
+                in.from = in.next(in.from);
+                if (!(GRAD && hold)) in.ask();
+            }
             if (threadIdx.x < p.extra) {
-                const int j = p.extra_column(threadIdx.x);
-                out[j] = from_f32<T>(grad(to_f32(p.row[j])));
+                const float z[1] = {to_f32(beside)};
+                add_scores<FAST, false>(s, z, c);
             }
-            __syncthreads();  // the block's p are written
-            if (threadIdx.x < a.k && r.w != 0.0f) {
-                const int j = t.c[threadIdx.x];
-                const bool here = j >= 0 && (j < p.head || j >= p.tail
-                                                 ? rank == 0
-                                                 : (j - p.head) / V >= p.v0 && (j - p.head) / V < p.v1);
-                float y;
-                if (here && entry_grad<FAST>(t, threadIdx.x, to_f32(p.row[j]), r, a.k, y)) out[j] = from_f32<T>(y);
+            team_soft<FAST, false, NT>(s, c, soft);
+            if (threadIdx.x == 0) mine[b].set(s);
+            all();
+            if constexpr (GRAD) {
+                s = joined(b);
+                const RowScale<FAST> r(s, c, teacher.scale[b]);
+                T* out = dx + row * lddx;
+                const int end = write_grad<FAST, T, NT>(in, hold ? mine_first : in.from, steps, count, r,
+                                                        out + p.column(p.v0 + threadIdx.x),
+                                                        (reinterpret_cast<uintptr_t>(out + p.head) & 15) == 0, !hold);
+                if (!hold) in.from = end;
+                if (threadIdx.x < p.extra) out[p.extra_column(threadIdx.x)] = from_f32<T>(grad_of<FAST>(to_f32(beside), r));
             }
+            meet();  // the row's p are written
         }
-        __syncthreads();
+    } else {
+        const int lane = threadIdx.x - NT;
+        const auto entries = [&](int b) { return Teacher{teacher.c[b], teacher.q[b], teacher.z[b], &teacher.scale[b]}; };
+        // A row's entries are asked for two rows ahead, the scores of their classes
+        // while the row before is read, and put into shared memory after it.
+        Entries<T, U, 32> next;
+        float own = 0.0f;
+        if (first < a.rows) {
+            next.fetch(a, first, lane);
+            next.fetch_scores(a, x + first * ldx);
+            own = read_teacher<T, U>(a, next, lane, entries(0));
+        }
+        if (first + clusters < a.rows) next.fetch(a, first + clusters, lane);
+        for (int64_t row = first; row < a.rows; row += clusters, ++round) {
+            const int b = round & 1;
+            const Teacher t = entries(b);
+            if (row + clusters < a.rows) next.fetch_scores(a, x + (row + clusters) * ldx);
+            all();
+            const Soft s = joined(b);
+            const RowScale<FAST> r(s, c, *t.scale);
+            float loss = own;
+            if (rank == 0) {
+                for (int i = lane; i < a.k; i += 32)
+                    if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.log_p(t.z[i]), loss);
+                loss = reduce_sum<float, 32>(loss);
+                if (lane == 0) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
+            }
+            meet();
+            if constexpr (GRAD) {
+                const Part<T> p(x + row * ldx, a.n, rank, log_ranks);
+                for (int e = lane; e < a.k; e += 32)
+                    if (t.c[e] >= 0 && r.w != 0.0f && p.has(t.c[e])) dx[row * lddx + t.c[e]] = from_f32<T>(entry_grad<FAST>(t, e, r));
+            }
+            if (row + clusters < a.rows) own = read_teacher<T, U>(a, next, lane, entries(b ^ 1));
+            if (row + 2 * clusters < a.rows) next.fetch(a, row + 2 * clusters, lane);
+        }
     }
     if (ranks > 1) cluster.sync();  // no CTA leaves while its state may be read
 }
@@ -258,24 +504,48 @@ void distill(const DistillArgs& a, const T* x, int64_t ldx, T* dx, int64_t lddx,
         by_narrow(a.n, [&](auto lpr, auto e) {
             constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = kNarrowThreads / LPR;
             auto kern = dx ? distill_narrow_kernel<T, U, LPR, E, true> : distill_narrow_kernel<T, U, LPR, E, false>;
-            const int stage = static_cast<int>((RPB * a.n * sizeof(T) + 32 + 15) / 16 * 16);
-            const size_t bytes = stage + RPB * (2 * a.k + 1) * sizeof(float);
+            const int turns = narrow_turns(RPB, a.n, sizeof(T), a.rows);
+            const int stage = static_cast<int>((RPB * turns * a.n * sizeof(T) + 32 + 15) / 16 * 16);
+            const size_t bytes = stage + RPB * Teacher::floats(a.k) * sizeof(float);
             if (bytes > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
             launch_dependent("distill_loss", kern,
-                             dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(a.rows, RPB), num_sms() * 16))),
-                             dim3(kNarrowThreads), bytes, s, a, x, ldx, dx, lddx, stage);
+                             dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(a.rows, RPB * turns), num_sms() * 8))),
+                             dim3(kNarrowThreads), bytes, s, a, x, ldx, dx, lddx, turns, stage);
         });
         return;
     }
-    const int ranks = row_ranks(a.rows, a.n, 4096);
+    if (a.n <= kWarp && a.rows > num_sms()) {
+        using In = Stream<T, 32>;
+        const int slots = (dx ? static_cast<int>(ceil_div(a.n / kVec<T>, 32 * In::W)) : 0) + kAhead;
+        const int bytes = kTeams * (slots * In::kSlot + Teacher::floats(a.k) * 4);
+        auto kern = dx ? distill_warp_kernel<T, U, true> : distill_warp_kernel<T, U, false>;
+        launch_rows("distill_loss", kern, ceil_div(a.rows, kTeams), 1, std::min(5, kSharedSm / (bytes + 1024)), 32 * kTeams, bytes, s, a, x, ldx, dx,
+                    lddx, slots);
+        return;
+    }
     const auto go = [&](auto nt) {
-        constexpr int NT = decltype(nt)::value;
-        const int64_t clusters = std::min<int64_t>(a.rows, std::max<int64_t>(1, int64_t(num_sms()) * (1024 / NT) / ranks));
+        constexpr int NT = decltype(nt)::value, kSlot = Stream<T, NT>::kSlot;
+        constexpr int kMost = 212 * 1024 * NT / 768 / kSlot;  // slots, with 768 reading threads an SM
+        // Enough CTAs a row for the SMs to be busy, and for each to hold its part.
+        int ranks = row_ranks(a.rows, a.n, 4096);
+        const auto steps = [&] {
+            return static_cast<int>(ceil_div(ceil_div(a.n / kVec<T>, ranks), NT * Stream<T, NT>::W));
+        };
+        while (dx && ranks < 8 && steps() > kMost) ranks *= 2;
+        const bool hold = dx && steps() <= kMost;
+        const int slots = hold ? steps() : kAhead;
+        // (by registers, and by shared memory)
+        const int resident = std::max(1, std::min(dx ? 768 / NT : 1024 / (NT + 32), kSharedSm / (slots * kSlot + 4608)));
         auto kern = dx ? distill_wide_kernel<T, U, NT, true> : distill_wide_kernel<T, U, NT, false>;
-        launch_clusters("distill_loss", kern, clusters, ranks, NT, 0, s, a, x, ldx, dx, lddx);
+        launch_rows("distill_loss", kern, a.rows, ranks, resident, NT + 32, slots * kSlot, s, a, x, ldx, dx, lddx, slots, hold);
     };
-    if (a.n / ranks <= 8192) go(std::integral_constant<int, 128>{});
-    else go(std::integral_constant<int, 512>{});
+    if (!dx) {
+        if (a.n / row_ranks(a.rows, a.n, 4096) <= 8192) go(std::integral_constant<int, 128>{});
+        else go(std::integral_constant<int, 256>{});
+        return;
+    }
+    if (a.n * sizeof(T) <= 32 * 1024) go(std::integral_constant<int, 128>{});
+    else go(std::integral_constant<int, 256>{});
 }
 
 }  // namespace

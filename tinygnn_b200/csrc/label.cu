@@ -52,75 +52,79 @@ __device__ __forceinline__ RowResult finish_row(const Soft& a) {
 __device__ __forceinline__ float log_prob(float z, const RowResult& r) {
     return __fsub_rn(__fsub_rn(z, r.m), r.log_s);  // (NaN where no class is left)
 }
-// What a row's first thread writes.  z: the row.
-template <class T>
-__device__ __forceinline__ void write_row(const LabelArgs& a, int64_t row, const T* z, const RowResult& r) {
-    const int label = class_at(a.labels, row, a.wide_labels);
-    a.log_probs[row] = label >= 0 && label < a.n ? log_prob(to_f32(z[label]), r) : 0.0f;
+// What a row's first thread writes.  z: the score of its label.
+__device__ __forceinline__ void write_row(const LabelArgs& a, int64_t row, bool labelled, float z, const RowResult& r) {
+    a.log_probs[row] = labelled ? log_prob(z, r) : 0.0f;
     a.entropy[row] = r.entropy;
     a.stats[row] = make_float2(r.m, r.log_s);
 }
 
 // ── narrow rows ──────────────────────────────────────────────────────────
 template <class T, int LPR, int E, bool TOP>
-__global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const LabelArgs a, const T* x, int64_t ldx) {
+__global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const LabelArgs a, const T* x, int64_t ldx, int turns) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr float C = FAST ? kLog2e : 1.0f;
     constexpr int RPB = kNarrowThreads / LPR;
     extern __shared__ __align__(16) uint8_t sh[];
     wait_for_previous();
-    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
-        const int rows = a.rows - r0 < RPB ? static_cast<int>(a.rows - r0) : RPB;
+    const int lane = threadIdx.x % LPR, per = RPB * turns;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
+        const int rows = a.rows - r0 < per ? static_cast<int>(a.rows - r0) : per;
         const T* st = stage_in(sh, x, ldx, r0, rows, a.n);
         __syncthreads();
-        float z[E];
+        for (int sub = threadIdx.x / LPR; sub - static_cast<int>(threadIdx.x) / LPR < rows; sub += RPB) {
+            float z[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int j = lane + i * LPR;
-            z[i] = sub < rows && j < a.n ? to_f32(st[sub * a.n + j]) : -INFINITY;
-        }
-        Soft s;
-        add_scores<FAST, true>(s, z, C);
-        lanes_soft<FAST, true, LPR>(s, C);
-        const RowResult r = finish_row<FAST>(s);
-        const int64_t row = r0 + sub;
-        if (lane == 0 && sub < rows) write_row(a, row, st + sub * a.n, r);
-        if constexpr (TOP) {
-            uint32_t rank[E];
+            for (int i = 0; i < E; ++i) {
+                const int j = lane + i * LPR;
+                z[i] = sub < rows && j < a.n ? to_f32(st[sub * a.n + j]) : -INFINITY;
+            }
+            Soft s;
+            add_scores<FAST, true>(s, z, C);
+            lanes_soft<FAST, true, LPR>(s, C);
+            const RowResult r = finish_row<FAST>(s);
+            const int64_t row = r0 + sub;
+            if (lane == 0 && sub < rows) {
+                const int label = class_at(a.labels, row, a.wide_labels);
+                const bool labelled = label >= 0 && label < a.n;
+                write_row(a, row, labelled, labelled ? to_f32(st[sub * a.n + label]) : 0.0f, r);
+            }
+            if constexpr (TOP) {
+                uint32_t rank[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) rank[i] = lane + i * LPR < a.n ? rank_of(z[i]) : 0u;
-            uint32_t kept = 0;
-            int kept_class = 0;
-            for (int k = 0; k < a.top; ++k) {
-                uint32_t best = rank[0];
-                int at = 0;
+                for (int i = 0; i < E; ++i) rank[i] = lane + i * LPR < a.n ? rank_of(z[i]) : 0u;
+                uint32_t kept = 0;
+                int kept_class = 0;
+                for (int k = 0; k < a.top; ++k) {
+                    uint32_t best = rank[0];
+                    int at = 0;
 #pragma unroll
-                for (int i = 1; i < E; ++i)
-                    if (rank[i] > best) best = rank[i], at = i;
-                int j = lane + at * LPR;
-                if (LPR == 32) {
-                    const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-                    j = __reduce_min_sync(0xffffffffu, best == most ? j : INT_MAX);
-                    best = most;
-                } else {
+                    for (int i = 1; i < E; ++i)
+                        if (rank[i] > best) best = rank[i], at = i;
+                    int j = lane + at * LPR;
+                    if (LPR == 32) {
+                        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+                        j = __reduce_min_sync(0xffffffffu, best == most ? j : INT_MAX);
+                        best = most;
+                    } else {
 #pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1) {
-                        const uint32_t other = __shfl_xor_sync(0xffffffffu, best, o);
-                        const int oj = __shfl_xor_sync(0xffffffffu, j, o);
-                        if (other > best || (other == best && oj < j)) best = other, j = oj;
+                        for (int o = LPR / 2; o > 0; o >>= 1) {
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, best, o);
+                            const int oj = __shfl_xor_sync(0xffffffffu, j, o);
+                            if (other > best || (other == best && oj < j)) best = other, j = oj;
+                        }
                     }
-                }
-                if (lane == j % LPR) {
+                    if (lane == j % LPR) {
 #pragma unroll
-                    for (int i = 0; i < E; ++i)
-                        if (i == j / LPR) rank[i] = 0u;
-                }
-                if (lane == k % LPR) kept = best, kept_class = j;
-                if ((k % LPR == LPR - 1 || k == a.top - 1) && k - k % LPR + lane <= k && sub < rows) {
-                    const int64_t o = row * a.top + k - k % LPR + lane;
-                    a.top_log_probs[o] = log_prob(score_of(kept), r);
-                    a.top_classes[o] = kept_class;
+                        for (int i = 0; i < E; ++i)
+                            if (i == j / LPR) rank[i] = 0u;
+                    }
+                    if (lane == k % LPR) kept = best, kept_class = j;
+                    if ((k % LPR == LPR - 1 || k == a.top - 1) && k - k % LPR + lane <= k && sub < rows) {
+                        const int64_t o = row * a.top + k - k % LPR + lane;
+                        a.top_log_probs[o] = log_prob(score_of(kept), r);
+                        a.top_classes[o] = kept_class;
+                    }
                 }
             }
         }
@@ -129,8 +133,11 @@ __global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const Labe
 }
 
 // ── wide rows ────────────────────────────────────────────────────────────
-constexpr int kCandidates = 1024;  // scores above the bound that are ranked at a time
-constexpr int kEquals = 256;       // scores equal to it that are ranked at a time
+// Scores above the bound, and equal to it, that a team ranks at a time.
+template <int NT>
+constexpr int kCandidates = NT == 32 ? 256 : 512;
+template <int NT>
+constexpr int kEquals = NT == 32 ? 64 : 256;
 
 // A score and its class as one number: greater for a greater score, and among
 // equal scores for a lower class.  0: none.
@@ -143,79 +150,107 @@ __device__ __forceinline__ int entry_column(uint64_t e) { return static_cast<int
 template <int NT>
 struct TopShared {
     uint64_t best[kMaxTop];  // this CTA's best, in order
-    uint64_t above[kCandidates];
-    int equal[kEquals];
+    uint64_t above[NT == 32 ? kCandidates<NT> : 8 * kMaxTop];  // candidates; then the best of all CTAs of the row
+    int equal[kEquals<NT>];
     int n_above, n_equal, n_threads;
-    int threads[NT];
+    int threads[NT == 32 ? 1 : NT];
     int sums[NT / 32];
     uint32_t bound;
 };
+
+// How many of the first n entries are greater than e.
+__device__ __forceinline__ int place_of(const uint64_t* entries, int n, uint64_t e) {
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) place += entries[j] > e;
+    return place;
+}
 
 // The `k` best scores of the part into sh.best, 0 where it has fewer.  `most`:
 // the rank of this thread's greatest score among its vectors (0 without one).
 template <class T, int NT>
 __device__ __forceinline__ void part_top(TopShared<NT>& sh, const Part<T>& p, uint32_t most, int k) {
     constexpr int V = kVec<T>;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    using Team = logits::Team<NT>;
+    const int tid = Team::thread(), warp = tid >> 5, lane = tid & 31;
     if (tid < k) sh.best[tid] = 0;
-    // The greatest bound that k maxima reach, bit by bit (any that exactly k
+    // The greatest bound that k maxima reach, bit by bit (any that not many more
     // reach will do).
     uint32_t bound = 0;
-    if (__syncthreads_count(most != 0) >= k) {
-        for (int bit = 31; bit >= 0; --bit) {
+    if (Team::count(most != 0) >= k) {
+        // (the lowest bits of a 16-bit type's scores are alike)
+        constexpr int kLow = sizeof(T) == 4 ? 0 : (std::is_same<T, __half>::value ? 13 : 16);
+        for (int bit = 31; bit >= kLow; --bit) {
             const uint32_t next = bound | 1u << bit;
-            const int reached = __syncthreads_count(most >= next);
+            const int reached = Team::count(most >= next);
             if (reached >= k) bound = next;
-            if (reached == k) break;
+            if (reached >= k && reached <= k + NT / 16) break;
         }
+        if (bound >> 31 == 0) bound |= (1u << kLow) - 1;  // (of negative scores' ranks they are ones)
     }
     int above;
     for (;;) {
         if (tid == 0) sh.n_above = sh.n_equal = sh.n_threads = 0;
-        __syncthreads();
-        if (most != 0 && most >= bound) sh.threads[atomicAdd(&sh.n_threads, 1)] = tid;
+        // Where many threads reach the bound its score is a common one: then
+        // only those above it are looked at, and the equal ones found below.
+        const bool common = Team::count(most != 0 && most >= bound) > (NT == 32 ? NT : 2 * k + 32);
+        const bool mine = most != 0 && (common ? most > bound : most >= bound);
+        if (NT > 32 && mine) sh.threads[atomicAdd(&sh.n_threads, 1)] = tid;
+        if (common && tid == 0) sh.n_equal = kEquals<NT> + 1;
+        const volatile int *above_now = &sh.n_above, *equal_now = &sh.n_equal;
         const auto look = [&](float z, int column) {
             const uint32_t r = rank_of(z);
+            // (once there are too many, no more are counted: a row of equal
+            // scores would queue up at the counter)
             if (r > bound) {
-                const int i = atomicAdd(&sh.n_above, 1);
-                if (i < kCandidates) sh.above[i] = entry(r, column);
+                if (*above_now <= kCandidates<NT>) {
+                    const int i = atomicAdd(&sh.n_above, 1);
+                    if (i < kCandidates<NT>) sh.above[i] = entry(r, column);
+                }
             } else if (r == bound) {
-                const int i = atomicAdd(&sh.n_equal, 1);
-                if (i < kEquals) sh.equal[i] = column;
+                if (*equal_now <= kEquals<NT>) {
+                    const int i = atomicAdd(&sh.n_equal, 1);
+                    if (i < kEquals<NT>) sh.equal[i] = column;
+                }
             }
         };
         if (tid < p.extra) look(to_f32(p.row[p.extra_column(tid)]), p.extra_column(tid));
-        __syncthreads();
-        // A warp for each of those threads' vectors.
-        for (int i = warp; i < sh.n_threads; i += NT / 32)
-            for (int64_t v = p.v0 + sh.threads[i] + static_cast<int64_t>(lane) * NT; v < p.v1; v += 32 * NT) {
-                float z[V];
-                widen(p.load(v), z);
+        Team::sync();
+        const auto look_at = [&](int v) {
+            float z[V];
+            widen(p.load(v), z);
 #pragma unroll
-                for (int j = 0; j < V; ++j) look(z[j], p.column(v) + j);
-            }
-        __syncthreads();
+            for (int j = 0; j < V; ++j) look(z[j], p.column(v) + j);
+        };
+        if (NT == 32) {
+            if (mine)
+                for (int v = p.v0 + tid; v < p.v1; v += 32) look_at(v);
+        } else {
+            // A warp for each of those threads' vectors.
+            for (int i = warp; i < sh.n_threads; i += NT / 32)
+                for (int v = p.v0 + sh.threads[i] + lane * NT; v < p.v1; v += 32 * NT) look_at(v);
+        }
+        Team::sync();
         above = sh.n_above;
-        const int held = above < kCandidates ? above : kCandidates;
+        const int held = above < kCandidates<NT> ? above : kCandidates<NT>;
         // The rank of each among them is its place.
         for (int i = tid; i < held; i += NT) {
             const uint64_t e = sh.above[i];
-            int place = 0;
-            for (int j = 0; j < held; ++j) place += sh.above[j] > e;
+            const int place = place_of(sh.above, held, e);
             if (place < k) sh.best[place] = e;
             if (place == k - 1) sh.bound = entry_rank(e);
         }
-        __syncthreads();
-        if (above <= kCandidates) break;
+        Team::sync();
+        if (above <= kCandidates<NT>) break;
         // Too many, as where a row's greatest scores lie with few threads: k of
         // those that were kept reach a greater bound.
         bound = sh.bound;
-        __syncthreads();
+        Team::sync();
     }
     const int missing = k - above;
     if (missing <= 0 || bound == 0) return;
     const int equal = sh.n_equal;
-    if (equal <= kEquals) {
+    if (equal <= kEquals<NT>) {
         for (int i = tid; i < equal; i += NT) {
             const int column = sh.equal[i];
             int place = 0;
@@ -233,7 +268,7 @@ __device__ __forceinline__ void part_top(TopShared<NT>& sh, const Part<T>& p, ui
                 if (lane >= o) before += x;
             }
             if (lane == 31) sh.sums[warp] = before;
-            __syncthreads();
+            Team::sync();
             int total = 0;
             before -= count;
             for (int w = 0; w < NT / 32; ++w) {
@@ -243,11 +278,11 @@ __device__ __forceinline__ void part_top(TopShared<NT>& sh, const Part<T>& p, ui
             for (int i = 0; i < count && found + before + i < missing; ++i)
                 sh.best[above + found + before + i] = entry(bound, put(i));
             found += total;
-            __syncthreads();
+            Team::sync();
         };
         const auto is = [&](int column) { return rank_of(to_f32(p.row[column])) == bound; };
         if (p.extra) step(tid < p.head && is(tid), [&](int) { return tid; });
-        for (int64_t v = p.v0 + tid; v - tid < p.v1 && found < missing; v += NT) {
+        for (int v = p.v0 + tid; v - tid < p.v1 && found < missing; v += NT) {
             uint32_t mask = 0;
             if (v < p.v1) {
                 float z[V];
@@ -267,7 +302,6 @@ struct LabelShared {
     SoftShared soft;
     SoftCell mine[2];  // this CTA's state, of even and odd rounds
     TopShared<NT> top;
-    uint64_t joined[8 * kMaxTop];
 };
 template <int NT>
 struct LabelShared<NT, false> {
@@ -275,27 +309,50 @@ struct LabelShared<NT, false> {
     SoftCell mine[2];
 };
 
-template <class T, int NT, bool TOP>
-__global__ void __launch_bounds__(NT, 1024 / NT) label_wide_kernel(const LabelArgs a, const T* x, int64_t ldx) {
+constexpr int kAhead = 4;  // slots of the ring: 32 KB of a block of 256 threads
+
+template <class T, int NT, int TEAMS, bool TOP>
+__global__ void __launch_bounds__(NT * TEAMS, 1024 / (NT * TEAMS)) label_wide_kernel(const LabelArgs a, const T* x, int64_t ldx) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr float C = FAST ? kLog2e : 1.0f;
-    __shared__ LabelShared<NT, TOP> sh;
+    using Team = logits::Team<NT>;
+    __shared__ LabelShared<NT, TOP> shared[TEAMS];
+    extern __shared__ __align__(16) uint8_t room[];
     wait_for_previous();
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
-    const int64_t clusters = gridDim.x / ranks;
+    const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks()), log_ranks = __ffs(ranks) - 1;
+    const int team = TEAMS > 1 ? threadIdx.x / NT : 0, tid = Team::thread();
+    const int64_t step = static_cast<int64_t>(gridDim.x / ranks) * TEAMS, first = static_cast<int64_t>(blockIdx.x / ranks) * TEAMS + team;
+    LabelShared<NT, TOP>& sh = shared[team];
+    Stream<T, NT> in(x, ldx, a.rows, a.n, first, step, rank, log_ranks, room + team * kAhead * Stream<T, NT>::kSlot, kAhead, false);
+    // (a row's label is asked for a row ahead, its score at the row's start)
+    int label = first < a.rows ? class_at(a.labels, first, a.wide_labels) : -1;
     int round = 0;
-    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += clusters, ++round) {
-        const Part<T> p(x + row * ldx, a.n, rank, ranks);
-        Soft s = scan_part<T, NT, 4, true>(p, C);
+    for (int64_t row = first; row < a.rows; row += step, ++round) {
+        const Part<T> p(x + row * ldx, a.n, rank, log_ranks);
+        const bool labelled = label >= 0 && label < a.n;
+        T at_label{}, beside{};
+        if (rank == 0) {
+            if (labelled && tid == 0) at_label = p.row[label];
+            if (tid < p.extra) beside = p.row[p.extra_column(tid)];
+            label = row + step < a.rows ? class_at(a.labels, row + step, a.wide_labels) : -1;
+        }
+        Soft s;
+        const int steps = in.steps_of(p);
+        for (int i = 0, have = p.v1 - p.v0; i < steps; ++i, have -= NT * in.W) {
+            in.template wait<kAhead - 1>();
+            in.template add<true>(s, in.from, have, C);
+            in.from = in.next(in.from);
+            in.ask();
+        }
         const float most = s.m;
-        if (threadIdx.x < p.extra) {
-            const float z[1] = {to_f32(p.row[p.extra_column(threadIdx.x)])};
+        if (tid < p.extra) {
+            const float z[1] = {to_f32(beside)};
             add_scores<FAST, true>(s, z, C);
         }
-        block_soft<FAST, true, NT>(s, C, sh.soft);
-        if (ranks > 1 && threadIdx.x == 0) sh.mine[round & 1].set(s);
-        if constexpr (TOP) part_top<T, NT>(sh.top, p, p.v0 + threadIdx.x < p.v1 ? rank_of(most) : 0u, a.top);
+        team_soft<FAST, true, NT>(s, C, sh.soft);
+        if (ranks > 1 && tid == 0) sh.mine[round & 1].set(s);
+        if constexpr (TOP) part_top<T, NT>(sh.top, p, p.v0 + tid < p.v1 ? rank_of(most) : 0u, a.top);
         if (ranks > 1) {
             cluster.sync();
             if (rank == 0) {
@@ -306,31 +363,30 @@ __global__ void __launch_bounds__(NT, 1024 / NT) label_wide_kernel(const LabelAr
         }
         if (rank == 0) {
             const RowResult r = finish_row<FAST>(s);
-            if (threadIdx.x == 0) write_row(a, row, p.row, r);
+            if (tid == 0) write_row(a, row, labelled, to_f32(at_label), r);
             if constexpr (TOP) {
-                __syncthreads();
+                Team::sync();
                 const auto put = [&](int i, uint64_t e) {
                     a.top_log_probs[row * a.top + i] = log_prob(score_of(entry_rank(e)), r);
                     a.top_classes[row * a.top + i] = entry_column(e);
                 };
                 if (ranks == 1) {
-                    for (int i = threadIdx.x; i < a.top; i += NT) put(i, sh.top.best[i]);
+                    for (int i = tid; i < a.top; i += NT) put(i, sh.top.best[i]);
                 } else {
+                    // (the candidates' room is free by now)
                     const int all = ranks * a.top;
-                    for (int i = threadIdx.x; i < all; i += NT)
-                        sh.joined[i] = cluster.map_shared_rank(sh.top.best, i / a.top)[i % a.top];
-                    __syncthreads();
-                    for (int i = threadIdx.x; i < all; i += NT) {
-                        const uint64_t e = sh.joined[i];
-                        int place = 0;
-                        for (int j = 0; j < all; ++j) place += sh.joined[j] > e;
+                    for (int i = tid; i < all; i += NT) sh.top.above[i] = cluster.map_shared_rank(sh.top.best, i / a.top)[i % a.top];
+                    Team::sync();
+                    for (int i = tid; i < all; i += NT) {
+                        const uint64_t e = sh.top.above[i];
+                        const int place = place_of(sh.top.above, all, e);
                         if (place < a.top && e) put(place, e);
                     }
                 }
             }
         }
         if (TOP && ranks > 1) cluster.sync();  // the CTAs' best have been read
-        __syncthreads();
+        Team::sync();
     }
     if (ranks > 1) cluster.sync();  // no CTA leaves while its state may be read
 }
@@ -376,19 +432,18 @@ __device__ __forceinline__ float grad_of(float z, const RowGrad& r) {
 
 template <class T, int LPR, int E>
 __global__ void __launch_bounds__(kNarrowThreads) label_grad_narrow_kernel(const GradArgs g, const T* x, int64_t ldx, T* dx,
-                                                                           int64_t lddx) {
+                                                                           int64_t lddx, int turns) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int RPB = kNarrowThreads / LPR;
     extern __shared__ __align__(16) uint8_t sh[];
     wait_for_previous();
-    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * RPB; r0 < g.rows; r0 += static_cast<int64_t>(gridDim.x) * RPB) {
-        const int rows = g.rows - r0 < RPB ? static_cast<int>(g.rows - r0) : RPB;
-        RowGrad r{};
-        if (sub < rows) r = row_grad<FAST>(g, r0 + sub);
+    const int lane = threadIdx.x % LPR, per = RPB * turns;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < g.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
+        const int rows = g.rows - r0 < per ? static_cast<int>(g.rows - r0) : per;
         T* st = stage_in(sh, x, ldx, r0, rows, g.n);
         __syncthreads();
-        if (sub < rows) {
+        for (int sub = threadIdx.x / LPR; sub < rows; sub += RPB) {
+            const RowGrad r = row_grad<FAST>(g, r0 + sub);
             T* p = st + sub * g.n;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
@@ -406,20 +461,32 @@ __global__ void __launch_bounds__(kNarrowThreads) label_grad_narrow_kernel(const
     }
 }
 
-// Item i of a row: `per` vectors of it.
-template <class T, int NT, int U>
-__global__ void __launch_bounds__(NT) label_grad_wide_kernel(const GradArgs g, const T* x, int64_t ldx, T* dx, int64_t lddx,
-                                                             int parts) {
+// A warp has U vectors a lane of one row.
+template <class T, int U>
+__global__ void __launch_bounds__(256) label_grad_wide_kernel(const GradArgs g, const T* x, int64_t ldx, T* dx, int64_t lddx,
+                                                              int64_t items, int parts) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int V = kVec<T>;
     wait_for_previous();
-    const int64_t row = blockIdx.x / parts;
-    const Part<T> p(x + row * ldx, g.n, static_cast<int>(blockIdx.x % parts), parts);
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), row = item / parts;
+    if (item >= items) return;
+    const int lane = threadIdx.x & 31;
+    const Part<T> p = Part<T>::of_size(x + row * ldx, g.n, static_cast<int>(item - row * parts), 32 * U);
+    Raw<T, V> raw[U];
+    T beside{};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (p.v0 + lane + u * 32 < p.v1) raw[u] = p.load(p.v0 + lane + u * 32);
+    if (lane < p.extra) beside = p.row[p.extra_column(lane)];
     T* out = dx + row * lddx;
     const RowGrad r = row_grad<FAST>(g, row);
     const bool aligned = (reinterpret_cast<uintptr_t>(out + p.head) & 15) == 0;
-    for_vectors<T, NT, U>(p, [&](int64_t v, float (&z)[V]) {
-        const int first = p.column(v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int v = p.v0 + lane + u * 32, first = p.column(v);
+        if (v >= p.v1) break;
+        float z[V];
+        widen(raw[u], z);
 #pragma unroll
         for (int j = 0; j < V; ++j) z[j] = grad_of<FAST>(z[j], r);
         if (static_cast<unsigned>(r.label - first) < V) {
@@ -429,10 +496,10 @@ __global__ void __launch_bounds__(NT) label_grad_wide_kernel(const GradArgs g, c
         }
         if (aligned) store_v<T, V>(out + first, z);
         else store_any<T, V>(out + first, z);
-    });
-    if (threadIdx.x < p.extra) {
-        const int j = p.extra_column(threadIdx.x);
-        float y = grad_of<FAST>(to_f32(p.row[j]), r);
+    }
+    if (lane < p.extra) {
+        const int j = p.extra_column(lane);
+        float y = grad_of<FAST>(to_f32(beside), r);
         if (j == r.label) y = __fadd_rn(y, r.a);
         out[j] = from_f32<T>(y);
     }
@@ -476,21 +543,28 @@ TG_API tg_status tg_label_log_probs(int64_t rows, int64_t classes, int32_t dtype
                 logits::by_narrow(classes, [&](auto lpr, auto e) {
                     constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = logits::kNarrowThreads / LPR;
                     auto kern = top ? label_narrow_kernel<T, LPR, E, true> : label_narrow_kernel<T, LPR, E, false>;
+                    const int turns = logits::narrow_turns(RPB, classes, sizeof(T), rows);
                     launch_dependent("label_log_probs", kern,
-                                     dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB), num_sms() * 16))),
-                                     dim3(logits::kNarrowThreads), staged_bytes(RPB, classes, sizeof(T)), s, a, x, ldz);
+                                     dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB * turns), num_sms() * 8))),
+                                     dim3(logits::kNarrowThreads), staged_bytes(RPB * turns, classes, sizeof(T)), s, a, x, ldz,
+                                     turns);
                 });
                 return;
             }
             const int ranks = logits::row_ranks(rows, classes, 4096);
-            const auto go = [&](auto nt) {
-                constexpr int NT = decltype(nt)::value;
-                const int64_t clusters = std::min<int64_t>(rows, std::max<int64_t>(1, int64_t(num_sms()) * (1024 / NT) * 2 / ranks));
-                auto kern = top ? label_wide_kernel<T, NT, true> : label_wide_kernel<T, NT, false>;
-                logits::launch_clusters("label_log_probs", kern, clusters, ranks, NT, 0, s, a, x, ldz);
+            const auto go = [&](auto nt, auto teams) {
+                constexpr int NT = decltype(nt)::value, TEAMS = decltype(teams)::value;
+                auto kern = top ? label_wide_kernel<T, NT, TEAMS, true> : label_wide_kernel<T, NT, TEAMS, false>;
+                const int room = TEAMS * kAhead * logits::Stream<T, NT>::kSlot;
+                const int fixed = TEAMS * static_cast<int>(top ? sizeof(LabelShared<NT, true>) : sizeof(LabelShared<NT, false>));
+                logits::launch_rows("label_log_probs", kern, ceil_div(rows, TEAMS), NT == 32 ? 1 : ranks,
+                                    std::min(1024 / (NT * TEAMS), logits::kSharedSm / (room + fixed + 1024)), NT * TEAMS, room, s, a,
+                                    x, ldz);
             };
-            if (classes / ranks <= 8192) go(std::integral_constant<int, 128>{});
-            else go(std::integral_constant<int, 512>{});
+            using std::integral_constant;
+            if (classes <= logits::kWarp && rows > num_sms()) go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+            else if (classes / ranks <= 8192) go(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+            else go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
         });
     });
 }
@@ -522,18 +596,20 @@ TG_API tg_status tg_label_log_probs_grad(int64_t rows, int64_t classes, int32_t 
             if (classes <= logits::kNarrow) {
                 logits::by_narrow(classes, [&](auto lpr, auto e) {
                     constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = logits::kNarrowThreads / LPR;
+                    const int turns = logits::narrow_turns(RPB, classes, sizeof(T), rows);
                     launch_dependent("label_log_probs_grad", label_grad_narrow_kernel<T, LPR, E>,
-                                     dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB), num_sms() * 16))),
-                                     dim3(logits::kNarrowThreads), staged_bytes(RPB, classes, sizeof(T)), s, g, x, ldz, dx,
-                                     lddz);
+                                     dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB * turns), num_sms() * 8))),
+                                     dim3(logits::kNarrowThreads), staged_bytes(RPB * turns, classes, sizeof(T)), s, g, x, ldz, dx,
+                                     lddz, turns);
                 });
                 return;
             }
-            constexpr int NT = 256, U = 4;
-            const int parts = static_cast<int>(ceil_div(classes, int64_t(NT) * U * logits::kVec<T>));
-            if (rows * parts > INT32_MAX) invalid(std::string(fn) + ": more than 2^31 blocks of the gradient");
-            launch_dependent("label_log_probs_grad", label_grad_wide_kernel<T, NT, U>,
-                             dim3(static_cast<unsigned>(rows * parts)), dim3(NT), 0, s, g, x, ldz, dx, lddz, parts);
+            constexpr int U = 4;
+            const int64_t parts = ceil_div(classes, int64_t(32) * U * logits::kVec<T>), items = rows * parts;
+            if (ceil_div(items, 8) > INT32_MAX) invalid(std::string(fn) + ": more than 2^31 blocks of the gradient");
+            launch_dependent("label_log_probs_grad", label_grad_wide_kernel<T, U>,
+                             dim3(static_cast<unsigned>(ceil_div(items, 8))), dim3(256), 0, s, g, x, ldz, dx, lddz, items,
+                             static_cast<int>(parts));
         });
     });
 }

@@ -8,23 +8,29 @@
 //  log p = d - log s and the entropy log s - t / s.  A new maximum m' scales s
 //  and t by e^((m - m') c).
 //
-//  Rows of at most kNarrow classes go through shared memory, several rows of
+//  Rows of at most kNarrow classes go through shared memory, many rows of
 //  contiguous memory at a time (rows of 41 floats begin anywhere, and
 //  16-byte loads of the whole block do not mind), and a row is then shared by
-//  LPR lanes that keep E scores each in registers.  Wider rows are shared by
-//  the CTAs of a cluster, which read them in 16-byte vectors: the few scores
-//  before the first and after the last aligned vector are the first CTA's.
+//  LPR lanes that keep E scores each in registers.  Wider rows are read in
+//  16-byte vectors by a team: a warp up to kWarp classes (a row's sums then need
+//  no barrier, and the SM has 16 to 32 rows under way), a block or the blocks of
+//  a cluster beyond.  The few scores before the first and after the last aligned
+//  vector are read one by one.
 // ============================================================================
 #pragma once
+
+#include <algorithm>
 
 #include "values.cuh"
 
 namespace tg {
 namespace logits {
 
-constexpr int kNarrow = 1024;   // widest row that a warp keeps in registers
+constexpr int kNarrow = 256;    // widest row that goes through shared memory with others
+constexpr int kWarp = 4096;     // widest row that a warp has alone
 constexpr int kMaxTop = 128;    // most alternatives of a row
 constexpr int kNarrowThreads = 256;
+constexpr int kSharedSm = 228 * 1024;  // shared memory of an SM; each block takes 1 KB of it for itself
 
 constexpr float kLn2 = 0.6931471806f, kLog2e = 1.4426950409f;
 
@@ -47,6 +53,35 @@ __device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.0f 
 struct Soft {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
 };
+
+// 16-bit scores whose entropy is not asked for (FUSED): d = z c - M with M = m c
+// rounded once, one instruction a score.  M's rounding shifts all of a row's d
+// alike and falls out of log p = d - log s; only a maximum whose product with c
+// leaves fp32's range (`far`) takes (z - m) c.  (With the entropy, whose log p of
+// a sure label is to be 0, all rows take the latter.)
+template <bool FAST, bool ENTROPY>
+constexpr bool kFused = FAST && !ENTROPY;
+struct Origin {
+    float m, M;
+    bool far;
+    __device__ __forceinline__ Origin(float most, float c) : m(origin(most)) {
+        M = __fmul_rn(m, c);
+        far = !(fabsf(M) <= 1e38f);  // (or NaN)
+    }
+    // At least -inf: its exponential is 0.
+    __device__ __forceinline__ float d(float z, float c) const {
+        return far ? __fmul_rn(__fsub_rn(z, m), c) : fmaf(z, c, -M);
+    }
+};
+// d of the maximum `from` as seen from the maximum `to`.
+template <bool FUSED>
+__device__ __forceinline__ float between(float from, float to, float c) {
+    if (FUSED && from != -INFINITY) {
+        const Origin a(from, c), b(to, c);
+        if (!a.far && !b.far) return __fsub_rn(a.M, b.M);
+    }
+    return distance(from, to, c);
+}
 // A CTA's state where the other CTAs of its cluster read it.
 struct SoftCell {
     float m, s, t;
@@ -58,36 +93,105 @@ struct SoftCell {
     }
 };
 
-// Adds V scores (those that are not there are -inf).
+// Two floats an instruction.
+struct Pair {
+    uint64_t v;
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Pair(uint64_t x) : v(x) {}
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return Pair(r);
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return Pair(r);
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return Pair(r);
+}
+
+// The greatest of N words' scores (a NaN, if there is one).
+template <class T, int N>
+__device__ __forceinline__ float top_of(const uint32_t (&w)[N]) {
+    uint32_t top = w[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+        if (std::is_same<T, float>::value) top = __float_as_uint(max_nan(__uint_as_float(top), __uint_as_float(w[i])));
+        else if (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i]));
+        else asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i]));
+    }
+    if (sizeof(T) == 4) return __uint_as_float(top);
+    Raw<T, 2> r;
+    r.w[0] = top;
+    float z[2];
+    widen(r, z);
+    return max_nan(z[0], z[1]);
+}
+
+// The state with the maximum `top`, if that is not below its own.
+template <bool FAST, bool ENTROPY>
+__device__ __forceinline__ void see_top(Soft& a, float top, float c) {
+    if (!(top <= a.m)) {
+        top = max_nan(top, a.m);  // (a NaN stays the maximum)
+        const float d = between<kFused<FAST, ENTROPY>>(a.m, top, c), f = expo<FAST>(d);
+        if (ENTROPY) a.t = __fmul_rn(f, fmaf(d, a.s, a.t));
+        a.s = __fmul_rn(a.s, f);
+        a.m = top;
+    }
+}
+
+// Adds V scores, of which `top` is the greatest (those that are not there are -inf).
+template <bool FAST, bool ENTROPY, int V>
+__device__ __forceinline__ void add_scores(Soft& a, const float (&z)[V], float top, float c) {
+    see_top<FAST, ENTROPY>(a, top, c);
+    Pair s(0.0f, 0.0f), t(0.0f, 0.0f);
+    float x, y;
+    const Origin o(a.m, c);
+    if (kFused<FAST, ENTROPY> && !o.far) {
+        const Pair k(-o.M, -o.M), cc(c, c);
+#pragma unroll
+        for (int j = 0; j + 1 < V; j += 2) {
+            fma2(Pair(z[j], z[j + 1]), cc, k).get(x, y);
+            s = add2(s, Pair(expo<FAST>(x), expo<FAST>(y)));
+        }
+        if (V % 2) s = add2(s, Pair(expo<FAST>(fmaf(z[V - 1], c, -o.M)), 0.0f));
+    } else {
+        const Pair k(-o.m, -o.m), cc(c, c);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            mul2(add2(Pair(z[j], z[j + 1 < V ? j + 1 : j]), k), cc).get(x, y);
+            x = max_nan(x, -200.0f), y = max_nan(y, -200.0f);
+            const Pair e(expo<FAST>(x), j + 1 < V ? expo<FAST>(y) : 0.0f);
+            s = add2(s, e);
+            if (ENTROPY) t = fma2(Pair(x, y), e, t);
+        }
+    }
+    s.get(x, y);
+    a.s = __fadd_rn(a.s, __fadd_rn(x, y));
+    if (ENTROPY) {
+        t.get(x, y);
+        a.t = __fadd_rn(a.t, __fadd_rn(x, y));
+    }
+}
 template <bool FAST, bool ENTROPY, int V>
 __device__ __forceinline__ void add_scores(Soft& a, const float (&z)[V], float c) {
     float top = z[0];
 #pragma unroll
     for (int j = 1; j < V; ++j) top = max_nan(top, z[j]);
-    if (!(top <= a.m)) {
-        top = max_nan(top, a.m);  // (a NaN stays the maximum)
-        const float d = distance(a.m, top, c), f = expo<FAST>(d);
-        if (ENTROPY) a.t = __fmul_rn(f, fmaf(d, a.s, a.t));
-        a.s = __fmul_rn(a.s, f);
-        a.m = top;
-    }
-    const float m = origin(a.m);
-    float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float d = distance(z[j], m, c), e = expo<FAST>(d);
-        s[j & 1] = __fadd_rn(s[j & 1], e);
-        if (ENTROPY) t[j & 1] = fmaf(d, e, t[j & 1]);
-    }
-    a.s = __fadd_rn(a.s, __fadd_rn(s[0], s[1]));
-    if (ENTROPY) a.t = __fadd_rn(a.t, __fadd_rn(t[0], t[1]));
+    add_scores<FAST, ENTROPY, V>(a, z, top, c);
 }
 
 // The state with the maximum m, which is at least its own.
 template <bool FAST, bool ENTROPY>
 __device__ __forceinline__ void raise_to(Soft& a, float m, float c) {
     if (a.m == m) return;
-    const float d = distance(a.m, m, c), f = expo<FAST>(d);
+    const float d = between<kFused<FAST, ENTROPY>>(a.m, m, c), f = expo<FAST>(d);
     if (ENTROPY) a.t = __fmul_rn(f, fmaf(d, a.s, a.t));
     a.s = __fmul_rn(a.s, f);
     a.m = m;
@@ -101,21 +205,46 @@ __device__ __forceinline__ void lanes_soft(Soft& a, float c) {
     if (ENTROPY) a.t = reduce_sum<float, W>(a.t);
 }
 
+// The threads that share a row within a block: a warp (NT = 32; a block then has
+// several teams), or the block's first NT threads.
+template <int NT>
+struct Team {
+    static __device__ __forceinline__ int thread() { return NT == 32 ? threadIdx.x & 31 : threadIdx.x; }
+    static __device__ __forceinline__ void sync() {
+        if (NT == 32) __syncwarp();
+        else asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
+    }
+    // How many of them; and a sync.
+    static __device__ __forceinline__ int count(bool x) {
+        if (NT == 32) return __popc(__ballot_sync(0xffffffffu, x));
+        int n;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.u32 p, %1, 0;\n\t"
+            "bar.red.popc.u32 %0, 1, %2, p;\n\t}"
+            : "=r"(n)
+            : "r"(static_cast<uint32_t>(x)), "n"(NT)
+            : "memory");
+        return n;
+    }
+};
+
 struct SoftShared {
     float m[32], s[32], t[32];
 };
-// The state of a block of NT threads, in each of them.
+// The state of a team, in each of its threads.
 template <bool FAST, bool ENTROPY, int NT>
-__device__ __forceinline__ void block_soft(Soft& a, float c, SoftShared& sh) {
+__device__ __forceinline__ void team_soft(Soft& a, float c, SoftShared& sh) {
     constexpr int W = NT / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     lanes_soft<FAST, ENTROPY, 32>(a, c);
+    if (NT == 32) return;
     if (lane == 0) {
         sh.m[warp] = a.m;
         sh.s[warp] = a.s;
         if (ENTROPY) sh.t[warp] = a.t;
     }
-    __syncthreads();
+    Team<NT>::sync();
     a = Soft{};
     if (lane < W) {
         a.m = sh.m[lane];
@@ -154,70 +283,158 @@ template <class T>
 struct Part {
     const T *row, *body;
     int head, tail, extra;
-    int64_t v0, v1;
+    int v0, v1;
 
-    __device__ __forceinline__ Part(const T* p, int64_t n, int rank, int ranks) : row(p) {
-        const int lead = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / static_cast<int>(sizeof(T));
-        head = lead < n ? lead : static_cast<int>(n);
-        body = p + head;
-        const int64_t nv = (n - head) / kVec<T>;
-        tail = static_cast<int>(head + nv * kVec<T>);
-        extra = rank == 0 ? head + static_cast<int>(n - tail) : 0;
-        v0 = nv * rank / ranks;
-        v1 = nv * (rank + 1) / ranks;
+    // Part `rank` of 2^log_ranks alike.
+    __device__ __forceinline__ Part(const T* p, int n, int rank, int log_ranks) : row(p) {
+        const int64_t nv = vectors(n, rank);
+        v0 = static_cast<int>(nv * rank >> log_ranks);
+        v1 = static_cast<int>(nv * (rank + 1) >> log_ranks);
+    }
+    // Part `rank` of those of `per` vectors.
+    static __device__ __forceinline__ Part of_size(const T* p, int n, int rank, int per) {
+        Part r(p);
+        const int nv = r.vectors(n, rank);
+        r.v0 = rank * per < nv ? rank * per : nv;
+        r.v1 = nv - r.v0 < per ? nv : r.v0 + per;
+        return r;
+    }
+    __device__ __forceinline__ bool has(int column) const {
+        if (column < head || column >= tail) return extra > 0;
+        const int v = (column - head) / kVec<T>;
+        return v >= v0 && v < v1;
     }
     __device__ __forceinline__ int extra_column(int i) const { return i < head ? i : tail + i - head; }
-    __device__ __forceinline__ int column(int64_t v) const { return head + static_cast<int>(v) * kVec<T>; }
-    __device__ __forceinline__ Raw<T, kVec<T>> load(int64_t v) const { return load_raw<T, kVec<T>>(body + v * kVec<T>); }
+    __device__ __forceinline__ int column(int v) const { return head + v * kVec<T>; }
+    __device__ __forceinline__ Raw<T, kVec<T>> load(int v) const {
+        return load_raw<T, kVec<T>>(body + static_cast<int64_t>(v) * kVec<T>);
+    }
+
+  private:
+    __device__ __forceinline__ explicit Part(const T* p) : row(p) {}
+    __device__ __forceinline__ int vectors(int n, int rank) {
+        const int lead = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T));
+        head = lead < n ? lead : n;
+        body = row + head;
+        const int nv = (n - head) / kVec<T>;
+        tail = head + nv * kVec<T>;
+        extra = rank == 0 ? head + n - tail : 0;
+        return nv;
+    }
 };
 
-// Calls f(v, V scores) for this thread's vectors, v0 + thread, + NT, ...; U are
-// asked for before the first is looked at.
-template <class T, int NT, int U, class F>
-__device__ __forceinline__ void for_vectors(const Part<T>& p, F&& f) {
-    constexpr int V = kVec<T>;
-    for (int64_t v = p.v0 + threadIdx.x; v < p.v1; v += NT * U) {
-        Raw<T, V> r[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v + u * NT < p.v1) r[u] = p.load(v + u * NT);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v + u * NT < p.v1) {
-                float z[V];
-                widen(r[u], z);
-                f(v + u * NT, z);
-            }
-    }
-}
+// The parts of rows first, first + step, ... that one team has, read through a
+// ring in shared memory by asynchronous copies, across the rows' ends: while a
+// row's statistics are joined the next row's scores are on their way.  Each
+// thread copies and reads the vectors part.v0 + thread, + NT, ..., two a slot of
+// the ring, so that nobody waits for another thread's copies; one group of
+// copies (empty after the last row) is committed a slot.
+template <class T, int NT>
+struct Stream {
+    static constexpr int W = 2;                       // vectors of a slot
+    static constexpr int kSlot = NT * W * 16;         // bytes
+    const T* x;
+    int64_t ldx, rows, step;
+    int n, rank, log_ranks, slots;
+    bool twice;      // each row is read twice
+    uint32_t base;   // of this thread's vector in the first slot
+    // what is asked for next
+    int64_t row;
+    const T* at;
+    int left, steps, again, slot;
+    // the slot that is read next
+    int from;
 
-// This thread's running softmax over its part (and, for the first threads of
-// the first CTA, of one of the scores beside the vectors).
-template <class T, int NT, int U, bool ENTROPY>
-__device__ __forceinline__ Soft scan_part(const Part<T>& p, float c) {
-    constexpr bool FAST = sizeof(T) == 2;
-    constexpr int V = kVec<T>;
-    Soft a;
-    for (int64_t v = p.v0 + threadIdx.x; v < p.v1; v += NT * U) {
-        Raw<T, V> r[U];
+    __device__ __forceinline__ Stream(const T* x_, int64_t ldx_, int64_t rows_, int n_, int64_t first, int64_t step_, int rank_,
+                                      int log_ranks_, uint8_t* room, int slots_, bool twice_)
+        : x(x_), ldx(ldx_), rows(rows_), step(step_), n(n_), rank(rank_), log_ranks(log_ranks_), slots(slots_), twice(twice_),
+          base(static_cast<uint32_t>(__cvta_generic_to_shared(room)) + Team<NT>::thread() * 16), row(first), at(nullptr), left(0),
+          steps(0), again(twice_ ? 2 : 1), slot(0), from(0) {
+        open();
+        for (int i = 0; i < slots; ++i) ask();
+    }
+    static __device__ __forceinline__ int steps_of(const Part<T>& p) {
+        return (p.v1 - p.v0 + NT * W - 1) / (NT * W);
+    }
+    __device__ __forceinline__ void open() {
+        while (row < rows) {
+            const Part<T> p(x + row * ldx, n, rank, log_ranks);
+            steps = steps_of(p);
+            if (steps > 0) {
+                at = p.body + (static_cast<int64_t>(p.v0) + Team<NT>::thread()) * kVec<T>;
+                left = p.v1 - p.v0 - Team<NT>::thread() - (steps - 1) * NT * W;  // (of the last step's)
+                return;
+            }
+            row += step;
+        }
+    }
+    __device__ __forceinline__ uint32_t address(int s, int w) const { return base + (s * W + w) * (NT * 16); }
+    // Asks for the next vectors, into the oldest slot (whose vectors have been used).
+    __device__ __forceinline__ void ask() {
+        if (steps > 0) {
+            const uint32_t to = address(slot, 0);
+            if (steps > 1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (v + u * NT < p.v1) {
-                r[u] = p.load(v + u * NT);
+                for (int w = 0; w < W; ++w) copy(to + w * NT * 16, at + w * NT * kVec<T>);
             } else {
 #pragma unroll
-                for (int j = 0; j < Raw<T, V>::N; ++j) r[u].w[j] = masked_word<T>();
+                for (int w = 0; w < W; ++w)
+                    if (left > w * NT) copy(to + w * NT * 16, at + w * NT * kVec<T>);
+            }
+            at += W * NT * kVec<T>;
+            if (--steps == 0) {
+                if (--again == 0) {
+                    again = twice ? 2 : 1;
+                    row += step;
+                }
+                open();
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        slot = next(slot);
+    }
+    static __device__ __forceinline__ void copy(uint32_t to, const T* from) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    }
+    // Waits until at most N of the groups asked for are on their way.
+    template <int N>
+    __device__ __forceinline__ void wait() const {
+        asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    }
+    // Slot s as it lies in memory; vectors from `have` threads on are masked.
+    __device__ __forceinline__ void read(int s, int have, uint32_t (&r)[4 * W]) const {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float z[V];
-            widen(r[u], z);
-            add_scores<FAST, ENTROPY>(a, z, c);
+        for (int w = 0; w < W; ++w)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(r[4 * w]), "=r"(r[4 * w + 1]), "=r"(r[4 * w + 2]), "=r"(r[4 * w + 3])
+                         : "r"(address(s, w))
+                         : "memory");
+        if (have < NT * W) {  // (the last slot of a row)
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+                if (have <= w * NT + Team<NT>::thread()) r[4 * w] = r[4 * w + 1] = r[4 * w + 2] = r[4 * w + 3] = masked_word<T>();
         }
     }
-    return a;
-}
+    static __device__ __forceinline__ void scores(const uint32_t (&r)[4 * W], float (&z)[W * kVec<T>]) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            Raw<T, kVec<T>> x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.w[j] = r[4 * w + j];
+            widen(x, z + w * kVec<T>);
+        }
+    }
+    // Adds slot s to the running softmax.
+    template <bool ENTROPY>
+    __device__ __forceinline__ void add(Soft& a, int s, int have, float c) const {
+        uint32_t r[4 * W];
+        float z[W * kVec<T>];
+        read(s, have, r);
+        scores(r, z);
+        add_scores<sizeof(T) == 2, ENTROPY>(a, z, top_of<T>(r), c);
+    }
+    __device__ __forceinline__ int next(int s) const { return s + 1 == slots ? 0 : s + 1; }
+};
 
 // Copies `rows` rows of n classes from row r0 on into shared memory (of n rows,
 // and 16 bytes): returns the address of the first, the others follow n apart.
@@ -277,8 +494,13 @@ void by_narrow(int64_t n, F&& f) {
     using std::integral_constant;
     if (n <= 16) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
     else if (n <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-    else if (n <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (n <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+}
+// How often RPB rows of n classes, taken together, make up about 16 KB.
+inline int narrow_turns(int rpb, int64_t n, size_t size, int64_t rows) {
+    const int64_t fit = std::max<int64_t>(1, 16384 / (rpb * n * static_cast<int64_t>(size)));
+    return static_cast<int>(std::max<int64_t>(1, std::min({fit, int64_t(8), ceil_div(rows, int64_t(rpb) * num_sms() * 4)})));
 }
 
 // An integer of 4 or 8 bytes; what does not fit an int is none (-1).
@@ -288,14 +510,16 @@ __device__ __forceinline__ int class_at(const void* p, int64_t i, bool wide) {
     return v < 0 || v > INT32_MAX ? -1 : static_cast<int>(v);
 }
 
-// Launches clusters of `ranks` blocks, `clusters` of them, dependent on the
-// previous kernel (wait_for_previous).
+// Launches clusters of `ranks` blocks for `rows` rows, at most as many as run at
+// a time (`resident` blocks an SM: each cluster walks rows, and one that had to
+// wait for another to end would come last), dependent on the previous kernel
+// (wait_for_previous).
 template <class K, class... A>
-void launch_clusters(const char* name, K kernel, int64_t clusters, int ranks, int block, size_t smem, cudaStream_t s,
-                     A... args) {
-    if (clusters == 0) return;
+void launch_rows(const char* name, K kernel, int64_t rows, int ranks, int resident, int block, size_t smem, cudaStream_t s,
+                 A... args) {
+    if (rows == 0) return;
+    if (smem > 32 * 1024) TG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(clusters * ranks));
     cfg.blockDim = dim3(static_cast<unsigned>(block));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -307,6 +531,15 @@ void launch_clusters(const char* name, K kernel, int64_t clusters, int ranks, in
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = ranks > 1 ? 2 : 1;
+    int64_t clusters = std::max<int64_t>(1, int64_t(num_sms()) * resident / ranks);
+    if (ranks > 1 && rows > clusters / 2) {
+        // (not every SM finds partners)
+        int most = 0;
+        cfg.gridDim = dim3(static_cast<unsigned>(ranks));
+        cuda_check(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg), name);
+        clusters = std::max(1, most);
+    }
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(rows, clusters) * ranks));
     cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), name);
     count_launch(name);
 }

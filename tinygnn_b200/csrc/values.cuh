@@ -189,14 +189,12 @@ struct Held {
         widen(k, x);
     }
 };
-// V values to p of any alignment (of T's).
+// V values to p of any alignment (of T's), as they lie in memory.
 template <class T, int V>
-__device__ __forceinline__ void store_any(T* p, const float (&x)[V]) {
-    Raw<T, V> k;
-    narrow(x, k);
+__device__ __forceinline__ void store_words(T* p, const Raw<T, V>& k) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = x[j];
+        for (int j = 0; j < V; ++j) p[j] = __uint_as_float(k.w[j]);
     } else if (reinterpret_cast<uintptr_t>(p) & 2) {
         uint16_t* q = reinterpret_cast<uint16_t*>(p);
         q[0] = static_cast<uint16_t>(k.w[0]);
@@ -208,6 +206,12 @@ __device__ __forceinline__ void store_any(T* p, const float (&x)[V]) {
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) reinterpret_cast<uint32_t*>(p)[j] = k.w[j];
     }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_any(T* p, const float (&x)[V]) {
+    Raw<T, V> k;
+    narrow(x, k);
+    store_words(p, k);
 }
 
 // The first n of V values (all, for more; none, for n <= 0).
