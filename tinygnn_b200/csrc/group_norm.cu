@@ -11,17 +11,24 @@
 //
 //  Graphs have any sizes, which only the device knows, so the work is cut by
 //  rows: a block walks chunks of R rows, thread (tx, ty) the V columns of one
-//  vector in every TY-th row of it, and splits a chunk where a graph ends.  The
-//  first pass leaves one partial result for each vector of columns, chunk and
-//  graph in it; chunk c's part of graph g is slot c + g, which no other part
-//  has, and there are at most chunks + graphs of them.  A second, small kernel
-//  joins a graph's slots in their order (no atomics, the same bits every run),
-//  and a third applies the statistics.
+//  16-byte vector in every ty-th row of it, and splits a chunk where a graph ends.
+//  The first pass leaves one partial result for each column, chunk and graph in
+//  it; chunk c's part of graph g is slot c + g, which no other part has, and there
+//  are at most chunks + graphs of them.  A second, small kernel joins a graph's
+//  slots in their order (no atomics, the same bits every run), and a third applies
+//  the statistics.  Many small graphs are a block's each instead, in one kernel
+//  (and one more that joins dgamma and dbeta): see small_graphs below.
 //
 //  A part's mean and sum of squared deviations come from one pass: each thread
-//  sums x - k and (x - k)^2 with k its own first value, which cannot lose the
-//  deviations (k is one of the few values it is subtracted from), and parts are
-//  joined by their means and deviations, not by sums of squares.
+//  sums x - k and (x - k)^2 with k its first value of the column, which cannot
+//  lose the deviations (k is one of the few values it is subtracted from), and
+//  parts are joined by their means and deviations, not by sums of squares.
+//
+//  What is applied to a value is linear in its distance from the mean, with
+//  factors of its column (the mean is not folded into the addend: a constant
+//  graph's y is beta):
+//      u = A (x - mean) + beta,  A = r gamma
+//      dx = A du - E (x - mean) - D,  E = r^2 mean(g h),  D = r mean g
 // ============================================================================
 #include <algorithm>
 
@@ -31,26 +38,9 @@ namespace tg {
 
 namespace {
 
-// V values (or one of any alignment) in loads of at most 16 bytes.
-template <class T, int V>
-__device__ __forceinline__ void load_cols(const T* p, float (&x)[V]) {
-    constexpr int N = V * static_cast<int>(sizeof(T)) > 16 ? 16 / static_cast<int>(sizeof(T)) : V;
-    if constexpr (V == 1) {
-        x[0] = to_f32(*p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i += N) widen(load_raw<T, N>(p + i), x + i);
-    }
-}
-template <class T, int V>
-__device__ __forceinline__ void store_cols(T* p, const float (&x)[V]) {
-    if constexpr (V == 1) *p = from_f32<T>(x[0]);
-    else store_v<T, V>(p, x);
-}
-
 struct GroupArgs {
     int64_t rows;
-    int cols, groups, graphs;
+    int cols, groups, per, graphs;  // per: columns of a group
     const int32_t* offsets;  // nullable: one graph of all rows
     int act;
     float alpha, eps;
@@ -95,102 +85,178 @@ __device__ __forceinline__ void for_parts(const GroupArgs& a, int c, F&& f) {
     }
 }
 
-// A thread's place.
+constexpr int kMaxThreads = 256;
+
+// A thread's place: V columns from `col` on, of which `n` are there (ALIGNED: all
+// or none), in the rows ty, ty + a.ty, ... of a part.
+template <class T, bool ALIGNED>
 struct Place {
-    int tx, ty, vec;
-    bool here;  // it has columns
+    static constexpr int V = 16 / static_cast<int>(sizeof(T));
+    using Values = Held<T, V, ALIGNED>;
+    int tx, ty, col, n;
     __device__ __forceinline__ explicit Place(const GroupArgs& a) {
         tx = threadIdx.x % a.tx;
         ty = threadIdx.x / a.tx;
-        vec = blockIdx.y * a.tx + tx;
-        here = ty < a.ty && vec < a.nv;
+        col = (blockIdx.y * a.tx + tx) * V;
+        n = ty < a.ty ? min(V, a.cols - col) : 0;
+    }
+    __device__ __forceinline__ void fetch(Values& v, const T* row) const {
+        if (ALIGNED) v.fetch(row + col);
+        else v.fetch(row + col, n);
+    }
+    __device__ __forceinline__ void values(const Values& v, const T* row, float (&x)[V]) const {
+        v.values(Values::odd(row + col), x, ALIGNED ? V : n);
+    }
+    __device__ __forceinline__ void store(T* row, const float (&x)[V]) const {
+        if (ALIGNED) store_v<T, V>(row + col, x);
+        else store_some<T, V>(row + col, x, n);
+    }
+    template <class P>
+    __device__ __forceinline__ void params(const P* p, float (&x)[V]) const {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = j < n ? to_f32(p[col + j]) : 0.0f;
+    }
+    // Calls f(row, values) for this thread's rows of [lo, hi); U rows are asked
+    // for before the first is looked at.
+    template <int U, class F>
+    __device__ __forceinline__ void for_rows(const GroupArgs& a, int lo, int hi, const T* x, int64_t ldx, F&& f) const {
+        if (n <= 0) return;
+        for (int r = lo + ty; r < hi; r += a.ty * U) {
+            Values v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r + u * a.ty < hi) fetch(v[u], x + (r + u * a.ty) * ldx);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r + u * a.ty < hi) {
+                    float z[V];
+                    values(v[u], x + (r + u * a.ty) * ldx, z);
+                    f(r + u * a.ty, z);
+                }
+        }
+    }
+    // The same for two matrices.
+    template <int U, class F>
+    __device__ __forceinline__ void for_rows(const GroupArgs& a, int lo, int hi, const T* x, int64_t ldx, const T* y, int64_t ldy,
+                                             F&& f) const {
+        if (n <= 0) return;
+        for (int r = lo + ty; r < hi; r += a.ty * U) {
+            Values v[U], w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r + u * a.ty < hi) {
+                    fetch(v[u], x + (r + u * a.ty) * ldx);
+                    fetch(w[u], y + (r + u * a.ty) * ldy);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r + u * a.ty < hi) {
+                    float z[V], d[V];
+                    values(v[u], x + (r + u * a.ty) * ldx, z);
+                    values(w[u], y + (r + u * a.ty) * ldy, d);
+                    f(r + u * a.ty, z, d);
+                }
+        }
     }
 };
 
-// The sum over the row lanes of a block of two values a thread, in those of the first.
-__device__ __forceinline__ float2 over_lanes(const GroupArgs& a, const Place& p, float2 v, float2* sh) {
-    __syncthreads();
-    sh[threadIdx.x] = v;
-    __syncthreads();
-    float2 s = make_float2(0.0f, 0.0f);
-    if (p.ty == 0)
-        for (int y = 0; y < a.ty; ++y) {
-            const float2 o = sh[y * a.tx + p.tx];
-            s.x = __fadd_rn(s.x, o.x);
-            s.y = __fadd_rn(s.y, o.y);
-        }
-    return s;
-}
-
-constexpr int kMaxThreads = 256;
+// Two sums of every column of a block's threads, before they are joined over
+// the row lanes.  (One pair more a plane: neighbouring columns lie in other banks.)
+template <class T>
+struct Sums {
+    static constexpr int V = 16 / static_cast<int>(sizeof(T));
+    float2 at[V][kMaxThreads + 1];
+    // Column c of the block's in row lane y.
+    __device__ __forceinline__ float2 get(const GroupArgs& a, int c, int y) const { return at[c % V][y * a.tx + c / V]; }
+};
 
 // ── forward ──────────────────────────────────────────────────────────────
-// part[slot * nv + vec] = (mean, sum of squared deviations) of the part's values.
-template <class T, int V>
-__global__ void __launch_bounds__(kMaxThreads) group_parts_kernel(const GroupArgs a, const T* x, int64_t ldx, float2* part) {
-    __shared__ float2 sh[kMaxThreads];
+// This thread's columns' means and sums of squared deviations over its rows of [lo, hi).
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void part_sums(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* x, int64_t ldx, int lo, int hi,
+                                          Sums<T>& sh) {
+    constexpr int V = Place<T, ALIGNED>::V;
+    float k[V], s[V], q[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) k[j] = s[j] = q[j] = 0.0f;
+    int n = 0;
+    p.template for_rows<4>(a, lo, hi, x, ldx, [&](int, const float (&z)[V]) {
+        if (n++ == 0) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) k[j] = z[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = __fsub_rn(z[j], k[j]);
+                s[j] = __fadd_rn(s[j], d);
+                q[j] = fmaf(d, d, q[j]);
+            }
+        }
+    });
+    // (a value that is not finite: x - x is a NaN, and so are the deviations)
+    const float inv = n ? __fdiv_rn(1.0f, static_cast<float>(n)) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float bad = __fsub_rn(k[j], k[j]);
+        sh.at[j][threadIdx.x] = make_float2(fmaf(s[j], inv, k[j]),
+                                            __fadd_rn(max_nan(fmaf(-s[j], __fmul_rn(s[j], inv), q[j]), 0.0f), bad));
+    }
+}
+// (mean, sum of squared deviations) of the block's column c over all row lanes of a part of `rows` rows.
+template <class T>
+__device__ __forceinline__ float2 join_lanes(const GroupArgs& a, const Sums<T>& sh, int c, int rows) {
+    const auto lane_rows = [&](int y) { return static_cast<float>((rows - y + a.ty - 1) / a.ty); };
+    const int lanes = rows < a.ty ? rows : a.ty;
+    const float first = sh.get(a, c, 0).x;
+    float sum = 0.0f, dev = 0.0f;
+    for (int y = 1; y < lanes; ++y) sum = fmaf(__fsub_rn(sh.get(a, c, y).x, first), lane_rows(y), sum);
+    const float mean = __fadd_rn(first, __fdiv_rn(sum, static_cast<float>(rows)));
+    for (int y = 0; y < lanes; ++y) {
+        const float2 o = sh.get(a, c, y);
+        const float e = __fsub_rn(o.x, mean);
+        dev = __fadd_rn(dev, fmaf(__fmul_rn(e, e), lane_rows(y), o.y));
+    }
+    return make_float2(mean, dev);
+}
+// Calls f(c, column) for the block's columns that this thread joins.
+template <class T, class F>
+__device__ __forceinline__ void for_columns(const GroupArgs& a, F&& f) {
+    constexpr int V = Sums<T>::V;
+    const int first = blockIdx.y * a.tx * V;
+    for (int c = threadIdx.x; c < a.tx * V && first + c < a.cols; c += blockDim.x) f(c, first + c);
+}
+
+// part[slot * cols + column] = (mean, sum of squared deviations) of the part's values.
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(kMaxThreads, 4) group_parts_kernel(const GroupArgs a, const T* x, int64_t ldx, float2* part) {
+    __shared__ Sums<T> sh;
     wait_for_previous();
-    const Place p(a);
+    const Place<T, ALIGNED> p(a);
     for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
         for_parts(a, c, [&](int g, int lo, int hi) {
-            float s = 0.0f, q = 0.0f, k = 0.0f;
-            int n = 0;
-            if (p.here) {
-                const T* at = x + static_cast<int64_t>(p.vec) * V;
-                constexpr int U = 4;
-                if (lo + p.ty < hi) k = to_f32(at[(lo + p.ty) * ldx]);
-                for (int r = lo + p.ty; r < hi; r += a.ty * U) {
-                    float z[U][V];
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (r + u * a.ty < hi) load_cols<T, V>(at + (r + u * a.ty) * ldx, z[u]);
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (r + u * a.ty < hi) {
-                            ++n;
-#pragma unroll
-                            for (int j = 0; j < V; ++j) {
-                                const float d = __fsub_rn(z[u][j], k);
-                                s = __fadd_rn(s, d);
-                                q = fmaf(d, d, q);
-                            }
-                        }
-                }
-            }
-            const float cnt = static_cast<float>(n * V), inv = n ? __fdiv_rn(1.0f, cnt) : 0.0f;
-            const float m = fmaf(s, inv, k), d = max_nan(fmaf(-s, __fmul_rn(s, inv), q), 0.0f);
-            // the row lanes' parts: lane y has the rows lo + y, + ty, ...
+            part_sums(a, p, x, ldx, lo, hi, sh);
             __syncthreads();
-            sh[threadIdx.x] = make_float2(m, d);
+            for_columns<T>(a, [&](int i, int column) {
+                part[static_cast<int64_t>(c + g) * a.cols + column] = join_lanes(a, sh, i, hi - lo);
+            });
             __syncthreads();
-            if (p.ty == 0 && p.here) {
-                float sum = 0.0f, dev = 0.0f;
-                const int rows = hi - lo;
-                const auto lane_rows = [&](int y) { return static_cast<float>((rows - y + a.ty - 1) / a.ty); };
-                const int lanes = rows < a.ty ? rows : a.ty;
-                for (int y = 0; y < lanes; ++y) sum = fmaf(__fsub_rn(sh[y * a.tx + p.tx].x, m), lane_rows(y), sum);
-                const float mean = __fadd_rn(m, __fdiv_rn(sum, static_cast<float>(rows)));
-                for (int y = 0; y < lanes; ++y) {
-                    const float2 o = sh[y * a.tx + p.tx];
-                    const float e = __fsub_rn(o.x, mean);
-                    dev = __fadd_rn(dev, fmaf(__fmul_rn(e, e), __fmul_rn(lane_rows(y), V), o.y));
-                }
-                part[static_cast<int64_t>(c + g) * a.nv + p.vec] = make_float2(mean, dev);
-            }
         });
 }
 
-// Calls f(part, rows of it) for this thread's parts of a graph's group, one of
-// W threads; w vectors of the group from v0 on.
+// Calls f(part, rows of it, column) for this thread's parts of a graph's group
+// (its columns from c0 on), one of W threads.
 template <int W, class F>
-__device__ __forceinline__ void for_slots(const GroupArgs& a, int g, int b, int e, int v0, int w, const float2* part, F&& f) {
-    const int c0 = b / a.R, c1 = (e - 1) / a.R;
-    const int64_t items = static_cast<int64_t>(c1 - c0 + 1) * w;
-    for (int64_t i = threadIdx.x % W; i < items; i += W) {
-        const int c = c0 + static_cast<int>(i / w), v = v0 + static_cast<int>(i % w);
-        const int64_t r0 = static_cast<int64_t>(c) * a.R, r1 = r0 + a.R;
-        f(part[static_cast<int64_t>(c + g) * a.nv + v], static_cast<int>((e < r1 ? e : r1) - (b > r0 ? b : r0)));
-    }
+__device__ __forceinline__ void for_slots(const GroupArgs& a, int g, int b, int e, int c0, const float2* part, F&& f) {
+    const int first = b / a.R, slots = (e - 1) / a.R - first + 1;
+    // (of narrow groups a thread has the same column of every W / per-th slot)
+    const int wide = a.per < W ? a.per : W, step = W / wide, t = threadIdx.x % W;
+    if (t >= wide * step) return;
+    for (int col = t % wide; col < a.per; col += wide)
+        for (int i = t / wide; i < slots; i += step) {
+            const int64_t r0 = static_cast<int64_t>(first + i) * a.R, r1 = r0 + a.R;
+            f(part[static_cast<int64_t>(first + i + g) * a.cols + c0 + col],
+              static_cast<int>((e < r1 ? e : r1) - (b > r0 ? b : r0)), c0 + col);
+        }
 }
 // The sum over W threads (a warp, or the block).
 template <int W>
@@ -206,185 +272,259 @@ __device__ __forceinline__ float sum_of(float v, float* sh) {
 }
 
 // stats[g * groups + group] = (mean, rstd), (0, 0) for a graph without rows.
-template <int V, int W>
+template <int W>
 __global__ void __launch_bounds__(kMaxThreads) group_stats_kernel(const GroupArgs a, const float2* part, float2* stats) {
     __shared__ float sh[8];
     wait_for_previous();
     const int64_t i = static_cast<int64_t>(blockIdx.x) * (kMaxThreads / W) + threadIdx.x / W;
     if (i >= static_cast<int64_t>(a.graphs) * a.groups) return;
-    const int g = static_cast<int>(i / a.groups), per = a.nv / a.groups, v0 = static_cast<int>(i % a.groups) * per;
+    const int g = static_cast<int>(i / a.groups), c0 = static_cast<int>(i % a.groups) * a.per;
     const int b = begin_of(a, g), e = end_of(a, g);
     float2 r = make_float2(0.0f, 0.0f);
     if (b < e) {
-        const float rows = static_cast<float>(e - b), all = __fmul_rn(rows, static_cast<float>(per * V));
+        const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
         // (about the first part's mean, so that the sum does not lose the differences)
-        const float k = part[static_cast<int64_t>(b / a.R + g) * a.nv + v0].x;
+        const float k = part[static_cast<int64_t>(b / a.R + g) * a.cols + c0].x;
         float s = 0.0f, d = 0.0f;
-        for_slots<W>(a, g, b, e, v0, per, part, [&](float2 p, int n) { s = fmaf(__fsub_rn(p.x, k), static_cast<float>(n), s); });
-        const float mean = __fadd_rn(k, __fdiv_rn(sum_of<W>(s, sh), __fmul_rn(rows, static_cast<float>(per))));
-        for_slots<W>(a, g, b, e, v0, per, part, [&](float2 p, int n) {
+        for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) { s = fmaf(__fsub_rn(p.x, k), static_cast<float>(n), s); });
+        const float mean = __fadd_rn(k, __fdiv_rn(sum_of<W>(s, sh), all));
+        for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) {
             const float x = __fsub_rn(p.x, mean);
-            d = __fadd_rn(d, fmaf(__fmul_rn(x, x), __fmul_rn(static_cast<float>(n), V), p.y));
+            d = __fadd_rn(d, fmaf(__fmul_rn(x, x), static_cast<float>(n), p.y));
         });
-        const float var = __fdiv_rn(sum_of<W>(d, sh), all);
-        r = make_float2(mean, __frsqrt_rn(__fadd_rn(var, a.eps)));
+        r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(sum_of<W>(d, sh), all), a.eps)));
     }
     if (threadIdx.x % W == 0) stats[i] = r;
 }
 
-template <class T, class P, int V>
-__global__ void __launch_bounds__(kMaxThreads) group_apply_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
+// Each of V columns' (first, second) of its group: one pair where the V columns
+// are one group's (SPLIT false).
+template <int V, bool SPLIT>
+struct OfGroup {
+    static constexpr int N = SPLIT ? V : 1;
+    float2 at[N];
+    __device__ __forceinline__ OfGroup(const GroupArgs& a, const float2* groups, int col) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) at[j] = groups[min(col + j, a.cols - 1) / a.per];
+    }
+    __device__ __forceinline__ const float2& operator[](int j) const { return at[SPLIT ? j : 0]; }
+};
+
+// y of this thread's rows of [lo, hi), a part of the graph with the groups' statistics `stats`.
+template <bool SPLIT, class T, bool ALIGNED, class P>
+__device__ __forceinline__ void apply_part(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* x, int64_t ldx, const P* gamma,
+                                           const P* beta, const float2* stats, T* y, int64_t ldy, int lo, int hi) {
+    constexpr int V = Place<T, ALIGNED>::V;
+    if (p.n <= 0) return;
+    float A[V], B[V];
+    p.params(gamma, A);
+    p.params(beta, B);
+    const OfGroup<V, SPLIT> st(a, stats, p.col);
+#pragma unroll
+    for (int j = 0; j < V; ++j) A[j] = __fmul_rn(A[j], st[j].y);
+    p.template for_rows<4>(a, lo, hi, x, ldx, [&](int r, float (&z)[V]) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[j] = fmaf(__fsub_rn(z[j], st[j].x), A[j], B[j]);
+        act_forward<sizeof(T) == 2>(z, a.act, a.alpha);
+        p.store(y + r * ldy, z);
+    });
+}
+
+template <class T, class P, bool ALIGNED, bool SPLIT>
+__global__ void __launch_bounds__(kMaxThreads, 4) group_apply_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
                                                                   const P* beta, const float2* stats, T* y, int64_t ldy) {
     wait_for_previous();
-    const Place p(a);
-    const int64_t col = static_cast<int64_t>(p.vec) * V;
-    float ga[V], be[V];
-    if (p.here) {
-        load_cols<P, V>(gamma + col, ga);
-        load_cols<P, V>(beta + col, be);
-    }
-    const int group = p.here ? p.vec / (a.nv / a.groups) : 0;
+    const Place<T, ALIGNED> p(a);
     for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
         for_parts(a, c, [&](int g, int lo, int hi) {
-            if (!p.here) return;
-            const float2 st = stats[static_cast<int64_t>(g) * a.groups + group];
-            const T* at = x + col;
-            T* to = y + col;
-            constexpr int U = 4;
-            for (int r = lo + p.ty; r < hi; r += a.ty * U) {
-                float z[U][V];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r + u * a.ty < hi) load_cols<T, V>(at + (r + u * a.ty) * ldx, z[u]);
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r + u * a.ty < hi) {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) z[u][j] = fmaf(__fmul_rn(__fsub_rn(z[u][j], st.x), st.y), ga[j], be[j]);
-                        act_forward<sizeof(T) == 2>(z[u], a.act, a.alpha);
-                        store_cols<T, V>(to + (r + u * a.ty) * ldy, z[u]);
-                    }
-            }
+            apply_part<SPLIT>(a, p, x, ldx, gamma, beta, stats + static_cast<int64_t>(g) * a.groups, y, ldy, lo, hi);
         });
+}
+
+// Adds f(column)'s pairs over the columns of each group; put(group, sum) by one
+// thread of the warp that adds them.
+template <class F, class G>
+__device__ __forceinline__ void over_groups(const GroupArgs& a, F&& f, G&& put) {
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < a.groups; i += blockDim.x >> 5) {
+        float2 s = make_float2(0.0f, 0.0f);
+        for (int c = i * a.per + lane; c < (i + 1) * a.per; c += 32) {
+            const float2 v = f(c, i);
+            s.x = __fadd_rn(s.x, v.x);
+            s.y = __fadd_rn(s.y, v.y);
+        }
+        s.x = reduce_sum<float, 32>(s.x);
+        s.y = reduce_sum<float, 32>(s.y);
+        put(i, s, lane == 0);
+    }
+}
+
+constexpr int kSmallCols = 2048;  // most columns of a block that has whole graphs
+
+// A block for each graph: its second reading of x comes from L1 or L2.
+template <class T, class P, bool ALIGNED, bool SPLIT>
+__global__ void __launch_bounds__(kMaxThreads, 4) group_small_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
+                                                                  const P* beta, float2* stats, T* y, int64_t ldy) {
+    __shared__ Sums<T> sh;
+    extern __shared__ float2 columns[];  // cols, and the groups' means and statistics
+    float2* mine = columns + a.cols;
+    wait_for_previous();
+    const Place<T, ALIGNED> p(a);
+    for (int g = blockIdx.x; g < a.graphs; g += gridDim.x) {
+        const int b = begin_of(a, g), e = end_of(a, g);
+        float2* out = stats + static_cast<int64_t>(g) * a.groups;
+        if (b >= e) {
+            for (int i = threadIdx.x; i < a.groups; i += blockDim.x) out[i] = make_float2(0.0f, 0.0f);
+            continue;
+        }
+        part_sums(a, p, x, ldx, b, e, sh);
+        __syncthreads();
+        for_columns<T>(a, [&](int i, int column) { columns[column] = join_lanes(a, sh, i, e - b); });
+        __syncthreads();
+        // (the columns of a group have the same number of values)
+        const float rows = static_cast<float>(e - b), per = static_cast<float>(a.per);
+        over_groups(
+            a, [&](int c, int i) { return make_float2(__fsub_rn(columns[c].x, columns[i * a.per].x), 0.0f); },
+            [&](int i, float2 s, bool first) {
+                const float mean = __fadd_rn(columns[i * a.per].x, __fdiv_rn(s.x, per));
+                float d = 0.0f;
+                for (int c = i * a.per + (threadIdx.x & 31); c < (i + 1) * a.per; c += 32) {
+                    const float z = __fsub_rn(columns[c].x, mean);
+                    d = __fadd_rn(d, fmaf(__fmul_rn(z, z), rows, columns[c].y));
+                }
+                d = reduce_sum<float, 32>(d);
+                const float2 r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(d, __fmul_rn(rows, per)), a.eps)));
+                if (first) mine[i] = out[i] = r;
+            });
+        __syncthreads();
+        apply_part<SPLIT>(a, p, x, ldx, gamma, beta, mine, y, ldy, b, e);
+    }
 }
 
 // ── backward ─────────────────────────────────────────────────────────────
-// h and du of V values.
-template <class T, int V>
-__device__ __forceinline__ void slopes(const GroupArgs& a, float (&x)[V], float (&dy)[V], const float (&ga)[V],
-                                       const float (&be)[V], float2 st) {
-    float u[V];
+// What a column's du takes: u = A (x - mean) + B.
+template <class T, bool ALIGNED, bool SPLIT>
+struct Slopes {
+    static constexpr int V = Place<T, ALIGNED>::V;
+    float A[V], B[V];
+    OfGroup<V, SPLIT> st;
+    template <class P>
+    __device__ __forceinline__ Slopes(const GroupArgs& a, const Place<T, ALIGNED>& p, const P* gamma, const P* beta, const float2* stats)
+        : st(a, stats, p.col) {
+        p.params(gamma, A);
+        p.params(beta, B);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        x[j] = __fmul_rn(__fsub_rn(x[j], st.x), st.y);
-        u[j] = fmaf(x[j], ga[j], be[j]);
+        for (int j = 0; j < V; ++j) A[j] = __fmul_rn(A[j], st[j].y);
     }
-    act_slope<sizeof(T) == 2>(u, a.act, a.alpha);
+    // x <- x - mean, dy <- du
+    __device__ __forceinline__ void du(const GroupArgs& a, float (&x)[V], float (&dy)[V]) const {
+        float u[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) dy[j] = __fmul_rn(dy[j], u[j]);
+        for (int j = 0; j < V; ++j) {
+            x[j] = __fsub_rn(x[j], st[j].x);
+            u[j] = fmaf(x[j], A[j], B[j]);
+        }
+        act_slope<sizeof(T) == 2>(u, a.act, a.alpha);
+#pragma unroll
+        for (int j = 0; j < V; ++j) dy[j] = __fmul_rn(dy[j], u[j]);
+    }
+};
+
+// This thread's columns' (sum du, sum du h) over its rows of [lo, hi).
+template <bool SPLIT, class T, bool ALIGNED, class P>
+__device__ __forceinline__ void grad_sums(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* dy, int64_t lddy, const T* x,
+                                          int64_t ldx, const P* gamma, const P* beta, const float2* stats, int lo, int hi, Sums<T>& sh) {
+    constexpr int V = Place<T, ALIGNED>::V;
+    float s[V], t[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = t[j] = 0.0f;
+    if (p.n > 0) {
+        const Slopes<T, ALIGNED, SPLIT> k(a, p, gamma, beta, stats);
+        p.template for_rows<2>(a, lo, hi, x, ldx, dy, lddy, [&](int, float (&z)[V], float (&d)[V]) {
+            k.du(a, z, d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                s[j] = __fadd_rn(s[j], d[j]);
+                t[j] = fmaf(d[j], z[j], t[j]);  // (times r below)
+            }
+        });
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = __fmul_rn(t[j], k.st[j].y);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sh.at[j][threadIdx.x] = make_float2(s[j], t[j]);
+}
+template <class T>
+__device__ __forceinline__ float2 add_lanes(const GroupArgs& a, const Sums<T>& sh, int c) {
+    float2 s = sh.get(a, c, 0);
+    for (int y = 1; y < a.ty; ++y) {
+        const float2 o = sh.get(a, c, y);
+        s.x = __fadd_rn(s.x, o.x);
+        s.y = __fadd_rn(s.y, o.y);
+    }
+    return s;
 }
 
-// part[slot * nv + vec] = (sum g, sum g h) of the part; sums[block][2][cols] =
-// (sum du h, sum du) over the block's rows.
-template <class T, class P, int V>
-__global__ void __launch_bounds__(kMaxThreads) group_grad_parts_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
+// dx of this thread's rows of [lo, hi); means: the groups' (mean g, mean g h).
+template <bool SPLIT, class T, bool ALIGNED, class P>
+__device__ __forceinline__ void grad_part(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* dy, int64_t lddy, const T* x,
+                                          int64_t ldx, const P* gamma, const P* beta, const float2* stats, const float2* means, T* dx,
+                                          int64_t lddx, int lo, int hi) {
+    constexpr int V = Place<T, ALIGNED>::V;
+    if (p.n <= 0) return;
+    const Slopes<T, ALIGNED, SPLIT> k(a, p, gamma, beta, stats);
+    OfGroup<V, SPLIT> de(a, means, p.col);
+#pragma unroll
+    for (int j = 0; j < de.N; ++j) {
+        de.at[j] = make_float2(-__fmul_rn(k.st[j].y, de.at[j].x), __fmul_rn(__fmul_rn(k.st[j].y, k.st[j].y), de.at[j].y));
+    }
+    p.template for_rows<2>(a, lo, hi, x, ldx, dy, lddy, [&](int r, float (&z)[V], float (&d)[V]) {
+        k.du(a, z, d);
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] = fmaf(k.A[j], d[j], fmaf(-de[j].y, z[j], de[j].x));
+        p.store(dx + r * lddx, d);
+    });
+}
+
+// part[slot * cols + column] = (sum du, sum du h) of the part; sums[block][2][cols]
+// = (sum du h, sum du) over the block's rows.
+template <class T, class P, bool ALIGNED, bool SPLIT>
+__global__ void __launch_bounds__(kMaxThreads, 3) group_grad_parts_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
                                                                        int64_t ldx, const P* gamma, const P* beta,
                                                                        const float2* stats, float2* part, float* sums) {
-    __shared__ float2 sh[kMaxThreads];
+    __shared__ Sums<T> sh;
+    extern __shared__ float2 total[];  // tx V columns
     wait_for_previous();
-    const Place p(a);
-    const int64_t col = static_cast<int64_t>(p.vec) * V;
-    float ga[V], be[V], dg[V], db[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) ga[j] = be[j] = dg[j] = db[j] = 0.0f;
-    if (p.here) {
-        load_cols<P, V>(gamma + col, ga);
-        load_cols<P, V>(beta + col, be);
-    }
-    const int group = p.here ? p.vec / (a.nv / a.groups) : 0;
+    const Place<T, ALIGNED> p(a);
+    for (int i = threadIdx.x; i < a.tx * Sums<T>::V; i += blockDim.x) total[i] = make_float2(0.0f, 0.0f);
     for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
         for_parts(a, c, [&](int g, int lo, int hi) {
-            float2 sum = make_float2(0.0f, 0.0f);
-            if (p.here) {
-                const float2 st = stats[static_cast<int64_t>(g) * a.groups + group];
-                float s[V], sh_[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) s[j] = sh_[j] = 0.0f;
-                constexpr int U = 2;
-                for (int r = lo + p.ty; r < hi; r += a.ty * U) {
-                    float z[U][V], d[U][V];
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (r + u * a.ty < hi) {
-                            load_cols<T, V>(x + col + (r + u * a.ty) * ldx, z[u]);
-                            load_cols<T, V>(dy + col + (r + u * a.ty) * lddy, d[u]);
-                        }
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (r + u * a.ty < hi) {
-                            slopes<T, V>(a, z[u], d[u], ga, be, st);
-#pragma unroll
-                            for (int j = 0; j < V; ++j) {
-                                s[j] = __fadd_rn(s[j], d[u][j]);
-                                sh_[j] = fmaf(d[u][j], z[u][j], sh_[j]);
-                            }
-                        }
-                }
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    sum.x = fmaf(ga[j], s[j], sum.x);
-                    sum.y = fmaf(ga[j], sh_[j], sum.y);
-                    db[j] = __fadd_rn(db[j], s[j]);
-                    dg[j] = __fadd_rn(dg[j], sh_[j]);
-                }
-            }
-            sum = over_lanes(a, p, sum, sh);
-            if (p.ty == 0 && p.here) part[static_cast<int64_t>(c + g) * a.nv + p.vec] = sum;
+            grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, stats + static_cast<int64_t>(g) * a.groups, lo, hi, sh);
+            __syncthreads();
+            for_columns<T>(a, [&](int i, int column) {
+                const float2 s = add_lanes(a, sh, i);
+                part[static_cast<int64_t>(c + g) * a.cols + column] = s;
+                total[i] = make_float2(__fadd_rn(total[i].x, s.x), __fadd_rn(total[i].y, s.y));
+            });
+            __syncthreads();
         });
     float* out = sums + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
-#pragma unroll 1
-    for (int j = 0; j < V; ++j) {
-        float2 v = make_float2(dg[0], db[0]);
-#pragma unroll
-        for (int i = 1; i < V; ++i)
-            if (i == j) v = make_float2(dg[i], db[i]);
-        v = over_lanes(a, p, v, sh);
-        if (p.ty == 0 && p.here) {
-            out[col + j] = v.x;
-            out[a.cols + col + j] = v.y;
-        }
-    }
+    for_columns<T>(a, [&](int i, int column) {
+        out[column] = total[i].y;
+        out[a.cols + column] = total[i].x;
+    });
 }
 
-// coef[g * groups + group] = (mean g, mean g h), in the first `blocks` blocks;
-// dgamma and dbeta, the sums of the blocks' rows in their order, in the others.
-template <class P, int V, int W>
-__global__ void __launch_bounds__(kMaxThreads) group_grad_join_kernel(const GroupArgs a, const float2* part, const float* sums,
-                                                                      int sum_rows, int blocks, float2* coef, P* dgamma,
-                                                                      P* dbeta) {
-    __shared__ float sh[kMaxThreads];
-    wait_for_previous();
-    if (static_cast<int>(blockIdx.x) < blocks) {
-        const int64_t i = static_cast<int64_t>(blockIdx.x) * (kMaxThreads / W) + threadIdx.x / W;
-        if (i >= static_cast<int64_t>(a.graphs) * a.groups) return;
-        const int g = static_cast<int>(i / a.groups), per = a.nv / a.groups, v0 = static_cast<int>(i % a.groups) * per;
-        const int b = begin_of(a, g), e = end_of(a, g);
-        if (b >= e) return;
-        float s = 0.0f, t = 0.0f;
-        for_slots<W>(a, g, b, e, v0, per, part, [&](float2 p, int) {
-            s = __fadd_rn(s, p.x);
-            t = __fadd_rn(t, p.y);
-        });
-        s = sum_of<W>(s, sh);
-        t = sum_of<W>(t, sh);
-        const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(per * V));
-        if (threadIdx.x % W == 0) coef[i] = make_float2(__fdiv_rn(s, all), __fdiv_rn(t, all));
-        return;
-    }
-    const int c = (blockIdx.x - blocks) * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+// dgamma and dbeta: the sums of the blocks' rows in their order.  (32 columns a block.)
+template <class P>
+__device__ __forceinline__ void join_params(const GroupArgs& a, int block, const float* sums, int sum_rows, P* dgamma, P* dbeta,
+                                            float* sh) {
+    const int c = block * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
     float s = 0.0f;
-    if (c < 2 * a.cols)
+    if (c < 2 * a.cols) {
+#pragma unroll 4
         for (int r = lane; r < sum_rows; r += kMaxThreads / 32) s = __fadd_rn(s, sums[static_cast<int64_t>(r) * 2 * a.cols + c]);
+    }
     sh[threadIdx.x] = s;
     __syncthreads();
     if (lane == 0 && c < 2 * a.cols) {
@@ -395,67 +535,135 @@ __global__ void __launch_bounds__(kMaxThreads) group_grad_join_kernel(const Grou
     }
 }
 
-template <class T, class P, int V>
-__global__ void __launch_bounds__(kMaxThreads) group_grad_apply_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
+// means[g * groups + group] = (mean g, mean g h), in the first `blocks` blocks;
+// dgamma and dbeta in the others.
+template <class P, int W>
+__global__ void __launch_bounds__(kMaxThreads) group_grad_join_kernel(const GroupArgs a, const float2* part, const P* gamma,
+                                                                      const float* sums, int sum_rows, int blocks, float2* means,
+                                                                      P* dgamma, P* dbeta) {
+    __shared__ float sh[kMaxThreads];
+    wait_for_previous();
+    if (static_cast<int>(blockIdx.x) >= blocks) {
+        join_params(a, static_cast<int>(blockIdx.x) - blocks, sums, sum_rows, dgamma, dbeta, sh);
+        return;
+    }
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kMaxThreads / W) + threadIdx.x / W;
+    if (i >= static_cast<int64_t>(a.graphs) * a.groups) return;
+    const int g = static_cast<int>(i / a.groups), c0 = static_cast<int>(i % a.groups) * a.per;
+    const int b = begin_of(a, g), e = end_of(a, g);
+    if (b >= e) return;
+    float s = 0.0f, t = 0.0f;
+    for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int, int column) {
+        const float w = to_f32(gamma[column]);
+        s = fmaf(w, p.x, s);
+        t = fmaf(w, p.y, t);
+    });
+    s = sum_of<W>(s, sh);
+    t = sum_of<W>(t, sh);
+    const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
+    if (threadIdx.x % W == 0) means[i] = make_float2(__fdiv_rn(s, all), __fdiv_rn(t, all));
+}
+
+template <class P>
+__global__ void __launch_bounds__(kMaxThreads) group_params_kernel(const GroupArgs a, const float* sums, int sum_rows, P* dgamma,
+                                                                   P* dbeta) {
+    __shared__ float sh[kMaxThreads];
+    wait_for_previous();
+    join_params(a, static_cast<int>(blockIdx.x), sums, sum_rows, dgamma, dbeta, sh);
+}
+
+template <class T, class P, bool ALIGNED, bool SPLIT>
+__global__ void __launch_bounds__(kMaxThreads, 3) group_grad_apply_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
                                                                        int64_t ldx, const P* gamma, const P* beta,
-                                                                       const float2* stats, const float2* coef, T* dx,
+                                                                       const float2* stats, const float2* means, T* dx,
                                                                        int64_t lddx) {
     wait_for_previous();
-    const Place p(a);
-    const int64_t col = static_cast<int64_t>(p.vec) * V;
-    float ga[V], be[V];
-    if (p.here) {
-        load_cols<P, V>(gamma + col, ga);
-        load_cols<P, V>(beta + col, be);
-    }
-    const int group = p.here ? p.vec / (a.nv / a.groups) : 0;
+    const Place<T, ALIGNED> p(a);
     for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
         for_parts(a, c, [&](int g, int lo, int hi) {
-            if (!p.here) return;
-            const float2 st = stats[static_cast<int64_t>(g) * a.groups + group];
-            const float2 co = coef[static_cast<int64_t>(g) * a.groups + group];
-            constexpr int U = 2;
-            for (int r = lo + p.ty; r < hi; r += a.ty * U) {
-                float z[U][V], d[U][V];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r + u * a.ty < hi) {
-                        load_cols<T, V>(x + col + (r + u * a.ty) * ldx, z[u]);
-                        load_cols<T, V>(dy + col + (r + u * a.ty) * lddy, d[u]);
-                    }
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (r + u * a.ty < hi) {
-                        slopes<T, V>(a, z[u], d[u], ga, be, st);
-#pragma unroll
-                        for (int j = 0; j < V; ++j)
-                            d[u][j] = __fmul_rn(st.y, fmaf(-z[u][j], co.y, fmaf(ga[j], d[u][j], -co.x)));
-                        store_cols<T, V>(dx + col + (r + u * a.ty) * lddx, d[u]);
-                    }
-            }
+            const int64_t o = static_cast<int64_t>(g) * a.groups;
+            grad_part<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, stats + o, means + o, dx, lddx, lo, hi);
         });
 }
 
+// A block for each graph.
+template <class T, class P, bool ALIGNED, bool SPLIT>
+__global__ void __launch_bounds__(kMaxThreads, 3) group_grad_small_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
+                                                                       int64_t ldx, const P* gamma, const P* beta,
+                                                                       const float2* stats, T* dx, int64_t lddx, float* sums) {
+    __shared__ Sums<T> sh;
+    extern __shared__ float2 columns[];  // cols sums of a graph, cols sums of all, the groups' means
+    float2 *total = columns + a.cols, *means = total + a.cols;
+    wait_for_previous();
+    const Place<T, ALIGNED> p(a);
+    for (int i = threadIdx.x; i < a.cols; i += blockDim.x) total[i] = make_float2(0.0f, 0.0f);
+    for (int g = blockIdx.x; g < a.graphs; g += gridDim.x) {
+        const int b = begin_of(a, g), e = end_of(a, g);
+        if (b >= e) continue;
+        const float2* st = stats + static_cast<int64_t>(g) * a.groups;
+        grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, st, b, e, sh);
+        __syncthreads();
+        for_columns<T>(a, [&](int i, int column) {
+            const float2 s = add_lanes(a, sh, i);
+            const float w = to_f32(gamma[column]);
+            columns[column] = make_float2(__fmul_rn(w, s.x), __fmul_rn(w, s.y));
+            total[column] = make_float2(__fadd_rn(total[column].x, s.x), __fadd_rn(total[column].y, s.y));
+        });
+        __syncthreads();
+        const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
+        over_groups(
+            a, [&](int c, int) { return columns[c]; },
+            [&](int i, float2 s, bool first) {
+                if (first) means[i] = make_float2(__fdiv_rn(s.x, all), __fdiv_rn(s.y, all));
+            });
+        __syncthreads();
+        grad_part<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, st, means, dx, lddx, b, e);
+    }
+    __syncthreads();
+    float* out = sums + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+    for (int i = threadIdx.x; i < a.cols; i += blockDim.x) {
+        out[i] = total[i].y;
+        out[a.cols + i] = total[i].x;
+    }
+}
+
 // ── host ─────────────────────────────────────────────────────────────────
-template <class T, class P, class F>
-void by_vector(int64_t cols, int64_t groups, bool aligned, F&& f) {
+// f(rows aligned, vectors of several groups)
+template <class T, class F>
+void by_layout(const GroupArgs& a, bool aligned, F&& f) {
     constexpr int V = 16 / static_cast<int>(sizeof(T));
-    const int64_t per = cols / groups;
-    if (aligned && per % V == 0) f(std::integral_constant<int, V>{});
-    else if (aligned && per % (V / 2) == 0 && cols % V == 0) f(std::integral_constant<int, V / 2>{});
-    else f(std::integral_constant<int, 1>{});
+    using std::false_type;
+    using std::true_type;
+    if (!aligned || a.cols % V != 0) f(false_type{}, true_type{});
+    else if (a.per % V != 0) f(true_type{}, true_type{});
+    else f(true_type{}, false_type{});
 }
 
 // Blocks as wide as the row (or an even share of it), up to 256 threads and 32
-// row lanes, and chunks of 8 rows a lane where that leaves four blocks an SM.
+// row lanes, and chunks of up to 32 rows a lane where that leaves four blocks an
+// SM.  (232,965 x 128 bf16, forward and gradient: CUT_FIGURES)
 GroupArgs cut(GroupArgs a, int V) {
-    a.nv = a.cols / V;
+    a.nv = static_cast<int>(ceil_div(a.cols, V));
     const int blocks = static_cast<int>(ceil_div(a.nv, kMaxThreads));
     a.tx = static_cast<int>(ceil_div(a.nv, blocks));
     a.ty = std::min(std::max(1, kMaxThreads / a.tx), 32);
     const int64_t share = ceil_div(a.rows * blocks, int64_t(num_sms()) * 4 * a.ty);
-    a.R = a.ty * static_cast<int>(std::min<int64_t>(std::max<int64_t>(share, 1), 8));
+    a.R = a.ty * static_cast<int>(std::min<int64_t>(std::max<int64_t>(share, 1), 32));
     a.chunks = static_cast<int>(ceil_div(a.rows, a.R));
+    return a;
+}
+// Whether the graphs are so many and so small (were they alike) that each is a
+// block's: its values are read again from L1 or L2, and one launch does all.
+// A graph far larger than the others would keep its block alone on the GPU, so
+// this is for matrices of up to 16 MB.  SMALL_FIGURES
+bool small_graphs(const GroupArgs& a, size_t size) {
+    const int64_t bytes = a.rows * a.cols * static_cast<int64_t>(size);
+    return a.nv <= kMaxThreads && a.cols <= kSmallCols && bytes <= 16 << 20 && bytes / a.graphs <= 32 << 10;
+}
+// The cut of such graphs: two rows a lane.
+GroupArgs cut_small(GroupArgs a) {
+    const int64_t lanes = std::max<int64_t>(ceil_div(ceil_div(a.rows, a.graphs), 2), 1);
+    a.ty = static_cast<int>(std::min<int64_t>(a.ty, std::max<int64_t>(lanes, ceil_div(32, a.tx))));
     return a;
 }
 dim3 block_of(const GroupArgs& a) { return dim3(static_cast<unsigned>((a.tx * a.ty + 31) / 32 * 32)); }
@@ -464,12 +672,13 @@ dim3 grid_of(const GroupArgs& a) {
     return dim3(static_cast<unsigned>(std::min<int64_t>(a.chunks, std::max<int64_t>(1, int64_t(num_sms()) * 8 / y))),
                 static_cast<unsigned>(y));
 }
-size_t slots_of(const GroupArgs& a) { return (static_cast<size_t>(a.chunks) + a.graphs) * a.nv; }
+int small_blocks(const GroupArgs& a) {
+    return static_cast<int>(std::min<int64_t>(a.graphs, int64_t(num_sms()) * std::min(16, 2048 / static_cast<int>(block_of(a).x))));
+}
+size_t slots_of(const GroupArgs& a) { return (static_cast<size_t>(a.chunks) + a.graphs) * a.cols; }
 // Whether a graph's group has so many parts (were the graphs alike) that a
 // block joins them, not a warp.
-bool many_parts(const GroupArgs& a) {
-    return a.graphs > 0 && (a.rows / a.R / a.graphs + 1) * (a.nv / a.groups) > 256;
-}
+bool many_parts(const GroupArgs& a) { return (a.rows / a.R / a.graphs + 1) * a.per > 256; }
 
 void check_group(const char* fn, int64_t rows, int64_t cols, int64_t groups, int64_t graphs, const int32_t* offsets, int dtype,
                  int param_dtype, int act) {
@@ -519,29 +728,37 @@ TG_API tg_status tg_group_norm(int64_t rows, int64_t cols, int64_t groups, int64
         if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) invalid("group_norm: stats must be 8-byte aligned");
         if (graphs == 0) return;
         cudaStream_t s = as_stream(stream);
-        const GroupArgs g{rows, static_cast<int>(cols), static_cast<int>(groups), static_cast<int>(graphs), offsets, act, alpha, eps};
+        const GroupArgs g{rows, static_cast<int>(cols), static_cast<int>(groups), static_cast<int>(cols / groups), static_cast<int>(graphs), offsets, act, alpha, eps};
         by_types(dtype, param_dtype, [&](auto t, auto pt) {
             using T = decltype(t);
             using P = decltype(pt);
             const T* xp = static_cast<const T*>(x);
             const P *ga = static_cast<const P*>(gamma), *be = static_cast<const P*>(beta);
-            const bool aligned = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(y, ldy, sizeof(T)) &&
-                                 rows_aligned16(gamma, 0, 1) && rows_aligned16(beta, 0, 1);
-            by_vector<T, P>(cols, groups, aligned, [&](auto vec) {
-                constexpr int V = decltype(vec)::value;
-                const GroupArgs a = cut(g, V);
+            const bool aligned = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(y, ldy, sizeof(T));
+            const GroupArgs a = cut(g, 16 / sizeof(T));
+            float2* st = reinterpret_cast<float2*>(stats);
+            by_layout<T>(a, aligned, [&](auto al, auto split) {
+                constexpr bool ALIGNED = decltype(al)::value, SPLIT = decltype(split)::value;
+                if (small_graphs(a, sizeof(T))) {
+                    const GroupArgs c = cut_small(a);
+                    const size_t room = (cols + groups) * sizeof(float2);
+                    auto kern = group_small_kernel<T, P, ALIGNED, SPLIT>;
+                    if (room > 24 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
+                    launch_dependent("group_norm", kern, dim3(static_cast<unsigned>(small_blocks(c))), block_of(c), room, s, c, xp, ldx,
+                                     ga, be, st, static_cast<T*>(y), ldy);
+                    return;
+                }
                 Scratch<float2> part(slots_of(a), s);
-                launch_dependent("group_norm_parts", group_parts_kernel<T, V>, grid_of(a), block_of(a), 0, s, a, xp, ldx, part.p);
+                launch_dependent("group_norm_parts", group_parts_kernel<T, ALIGNED>, grid_of(a), block_of(a), 0, s, a, xp, ldx, part.p);
                 const int64_t sets = graphs * groups;
-                float2* st = reinterpret_cast<float2*>(stats);
                 if (many_parts(a))
-                    launch_dependent("group_norm_stats", group_stats_kernel<V, kMaxThreads>, dim3(static_cast<unsigned>(sets)),
+                    launch_dependent("group_norm_stats", group_stats_kernel<kMaxThreads>, dim3(static_cast<unsigned>(sets)),
                                      dim3(kMaxThreads), 0, s, a, part.p, st);
                 else
-                    launch_dependent("group_norm_stats", group_stats_kernel<V, 32>, dim3(static_cast<unsigned>(ceil_div(sets, 8))),
+                    launch_dependent("group_norm_stats", group_stats_kernel<32>, dim3(static_cast<unsigned>(ceil_div(sets, 8))),
                                      dim3(kMaxThreads), 0, s, a, part.p, st);
-                launch_dependent("group_norm", group_apply_kernel<T, P, V>, grid_of(a), block_of(a), 0, s, a, xp, ldx, ga, be,
-                                 st, static_cast<T*>(y), ldy);
+                launch_dependent("group_norm", group_apply_kernel<T, P, ALIGNED, SPLIT>, grid_of(a), block_of(a), 0, s, a, xp, ldx, ga,
+                                 be, st, static_cast<T*>(y), ldy);
             });
         });
     });
@@ -570,38 +787,52 @@ TG_API tg_status tg_group_norm_grad(int64_t rows, int64_t cols, int64_t groups, 
         check_ld(fn, "dx", lddx, cols);
         if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) invalid("group_norm_grad: stats must be 8-byte aligned");
         cudaStream_t s = as_stream(stream);
-        const GroupArgs g{rows, static_cast<int>(cols), static_cast<int>(groups), static_cast<int>(graphs), offsets, act, alpha, 0.0f};
+        const GroupArgs g{rows, static_cast<int>(cols), static_cast<int>(groups), static_cast<int>(cols / groups), static_cast<int>(graphs), offsets, act, alpha, 0.0f};
         by_types(dtype, param_dtype, [&](auto t, auto pt) {
             using T = decltype(t);
             using P = decltype(pt);
             const T *xp = static_cast<const T*>(x), *dyp = static_cast<const T*>(dy);
             const P *ga = static_cast<const P*>(gamma), *be = static_cast<const P*>(beta);
             const bool aligned = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(dy, lddy, sizeof(T)) &&
-                                 rows_aligned16(dx, lddx, sizeof(T)) && rows_aligned16(gamma, 0, 1) && rows_aligned16(beta, 0, 1);
-            by_vector<T, P>(cols, groups, aligned, [&](auto vec) {
-                constexpr int V = decltype(vec)::value;
-                const GroupArgs a = cut(g, V);
+                                 rows_aligned16(dx, lddx, sizeof(T));
+            const GroupArgs a = cut(g, 16 / sizeof(T));
+            const float2* st = reinterpret_cast<const float2*>(stats);
+            const int col_blocks = static_cast<int>(ceil_div(2 * cols, 32));
+            P *dg = static_cast<P*>(dgamma), *db = static_cast<P*>(dbeta);
+            by_layout<T>(a, aligned, [&](auto al, auto split) {
+                constexpr bool ALIGNED = decltype(al)::value, SPLIT = decltype(split)::value;
+                if (graphs > 0 && small_graphs(a, sizeof(T))) {
+                    const GroupArgs c = cut_small(a);
+                    const int blocks = small_blocks(c);
+                    Scratch<float> sums(static_cast<size_t>(blocks) * 2 * cols, s);
+                    const size_t room = (2 * cols + groups) * sizeof(float2);
+                    auto kern = group_grad_small_kernel<T, P, ALIGNED, SPLIT>;
+                    if (room > 24 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
+                    launch_dependent("group_norm_grad", kern, dim3(static_cast<unsigned>(blocks)), block_of(c), room, s, c, dyp, lddy, xp,
+                                     ldx, ga, be, st, static_cast<T*>(dx), lddx, sums.p);
+                    launch_dependent("group_norm_grad_params", group_params_kernel<P>, dim3(static_cast<unsigned>(col_blocks)),
+                                     dim3(kMaxThreads), 0, s, c, sums.p, blocks, dg, db);
+                    return;
+                }
                 const dim3 grid = grid_of(a);
                 const int sum_rows = static_cast<int>(grid.x);
                 const size_t sets = static_cast<size_t>(graphs) * groups;
                 Scratch<float2> part(slots_of(a) + sets, s);
                 Scratch<float> sums(static_cast<size_t>(sum_rows) * 2 * cols, s);
-                float2* coef = part.p + slots_of(a);
-                const float2* st = reinterpret_cast<const float2*>(stats);
-                launch_dependent("group_norm_grad_parts", group_grad_parts_kernel<T, P, V>, grid, block_of(a), 0, s, a, dyp, lddy,
-                                 xp, ldx, ga, be, st, part.p, sums.p);
-                const int col_blocks = static_cast<int>(ceil_div(2 * cols, 32));
+                float2* means = part.p + slots_of(a);
+                launch_dependent("group_norm_grad_parts", group_grad_parts_kernel<T, P, ALIGNED, SPLIT>, grid, block_of(a),
+                                 a.tx * (16 / sizeof(T)) * sizeof(float2), s, a, dyp, lddy, xp, ldx, ga, be, st, part.p, sums.p);
                 const auto join = [&](auto width) {
                     constexpr int W = decltype(width)::value;
                     const int blocks = static_cast<int>(ceil_div(sets, kMaxThreads / W));
-                    launch_dependent("group_norm_grad_join", group_grad_join_kernel<P, V, W>,
-                                     dim3(static_cast<unsigned>(blocks + col_blocks)), dim3(kMaxThreads), 0, s, a, part.p, sums.p,
-                                     sum_rows, blocks, coef, static_cast<P*>(dgamma), static_cast<P*>(dbeta));
+                    launch_dependent("group_norm_grad_join", group_grad_join_kernel<P, W>,
+                                     dim3(static_cast<unsigned>(blocks + col_blocks)), dim3(kMaxThreads), 0, s, a, part.p, ga, sums.p,
+                                     sum_rows, blocks, means, dg, db);
                 };
-                if (many_parts(a)) join(std::integral_constant<int, kMaxThreads>{});
+                if (graphs > 0 && many_parts(a)) join(std::integral_constant<int, kMaxThreads>{});
                 else join(std::integral_constant<int, 32>{});
-                launch_dependent("group_norm_grad", group_grad_apply_kernel<T, P, V>, grid, block_of(a), 0, s, a, dyp, lddy, xp, ldx,
-                                 ga, be, st, coef, static_cast<T*>(dx), lddx);
+                launch_dependent("group_norm_grad", group_grad_apply_kernel<T, P, ALIGNED, SPLIT>, grid, block_of(a), 0, s, a, dyp, lddy,
+                                 xp, ldx, ga, be, st, means, static_cast<T*>(dx), lddx);
             });
         });
     });
