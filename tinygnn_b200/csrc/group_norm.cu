@@ -86,6 +86,13 @@ __device__ __forceinline__ void for_parts(const GroupArgs& a, int c, F&& f) {
 }
 
 constexpr int kMaxThreads = 256;
+// Blocks of an SM of the kernels that walk chunks.
+constexpr int kParts = 4, kGrad = 2;
+template <bool SPLIT>
+constexpr int kApply = SPLIT ? 2 : 3;
+constexpr int kJoinThreads = 1024;  // that join a graph's group of many parts
+template <int W>
+constexpr int kJoinBlock = W == 32 ? 256 : W;
 
 // A thread's place: V columns from `col` on, of which `n` are there (ALIGNED: all
 // or none), in the rows ty, ty + a.ty, ... of a part.
@@ -116,81 +123,109 @@ struct Place {
 #pragma unroll
         for (int j = 0; j < V; ++j) x[j] = j < n ? to_f32(p[col + j]) : 0.0f;
     }
-    // Calls f(row, values) for this thread's rows of [lo, hi); U rows are asked
-    // for before the first is looked at.
+    // This thread's rows of [lo, hi).
+    __device__ __forceinline__ int rows_of(const GroupArgs& a, int lo, int hi) const {
+        return n > 0 && lo + ty < hi ? (hi - lo - ty + a.ty - 1) / a.ty : 0;
+    }
+    // Calls f(values, the row of `out`, u) for this thread's rows of [lo, hi); U
+    // rows are asked for before the first (u = 0) is looked at.
     template <int U, class F>
-    __device__ __forceinline__ void for_rows(const GroupArgs& a, int lo, int hi, const T* x, int64_t ldx, F&& f) const {
-        if (n <= 0) return;
-        for (int r = lo + ty; r < hi; r += a.ty * U) {
+    __device__ __forceinline__ void for_rows(const GroupArgs& a, int lo, int hi, const T* x, int64_t ldx, T* out, int64_t ldo,
+                                             F&& f) const {
+        const int64_t step = a.ty * ldx, step_out = a.ty * ldo;
+        const T* row = x + static_cast<int64_t>(lo + ty) * ldx;
+        T* to = out + static_cast<int64_t>(lo + ty) * ldo;
+        for (int left = rows_of(a, lo, hi); left > 0; left -= U) {
             Values v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + u * a.ty < hi) fetch(v[u], x + (r + u * a.ty) * ldx);
+                if (u < left) fetch(v[u], row + u * step);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (r + u * a.ty < hi) {
-                    float z[V];
-                    values(v[u], x + (r + u * a.ty) * ldx, z);
-                    f(r + u * a.ty, z);
-                }
+            for (int u = 0; u < U; ++u) {
+                if (u >= left) break;
+                float z[V];
+                values(v[u], row + u * step, z);
+                f(z, to, u);
+                to += step_out;
+            }
+            row += U * step;
         }
     }
     // The same for two matrices.
     template <int U, class F>
     __device__ __forceinline__ void for_rows(const GroupArgs& a, int lo, int hi, const T* x, int64_t ldx, const T* y, int64_t ldy,
-                                             F&& f) const {
-        if (n <= 0) return;
-        for (int r = lo + ty; r < hi; r += a.ty * U) {
+                                             T* out, int64_t ldo, F&& f) const {
+        const int64_t step = a.ty * ldx, step_y = a.ty * ldy, step_out = a.ty * ldo;
+        const T *row = x + static_cast<int64_t>(lo + ty) * ldx, *row_y = y + static_cast<int64_t>(lo + ty) * ldy;
+        T* to = out + static_cast<int64_t>(lo + ty) * ldo;
+        for (int left = rows_of(a, lo, hi); left > 0; left -= U) {
             Values v[U], w[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (r + u * a.ty < hi) {
-                    fetch(v[u], x + (r + u * a.ty) * ldx);
-                    fetch(w[u], y + (r + u * a.ty) * ldy);
+                if (u < left) {
+                    fetch(v[u], row + u * step);
+                    fetch(w[u], row_y + u * step_y);
                 }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (r + u * a.ty < hi) {
-                    float z[V], d[V];
-                    values(v[u], x + (r + u * a.ty) * ldx, z);
-                    values(w[u], y + (r + u * a.ty) * ldy, d);
-                    f(r + u * a.ty, z, d);
-                }
+            for (int u = 0; u < U; ++u) {
+                if (u >= left) break;
+                float z[V], d[V];
+                values(v[u], row + u * step, z);
+                values(w[u], row_y + u * step_y, d);
+                f(z, d, to);
+                to += step_out;
+            }
+            row += U * step;
+            row_y += U * step_y;
         }
     }
 };
 
+// x <- f(x) for the pairs of V values.
+template <int V, class F>
+__device__ __forceinline__ void pairs(float (&x)[V], F&& f) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) f(j, Pair(x[j], x[j + 1])).get(x[j], x[j + 1]);
+}
+
 // Two sums of every column of a block's threads, before they are joined over
-// the row lanes.  (One pair more a plane: neighbouring columns lie in other banks.)
+// the row lanes, in shared memory.  (One pair more a plane: neighbouring columns
+// lie in other banks.)
 template <class T>
 struct Sums {
     static constexpr int V = 16 / static_cast<int>(sizeof(T));
-    float2 at[V][kMaxThreads + 1];
+    float2* at;
+    static __host__ __device__ constexpr int pairs(int threads) { return V * (threads + 1); }
+    __device__ __forceinline__ void set(int j, float2 v) const { at[j * (blockDim.x + 1) + threadIdx.x] = v; }
     // Column c of the block's in row lane y.
-    __device__ __forceinline__ float2 get(const GroupArgs& a, int c, int y) const { return at[c % V][y * a.tx + c / V]; }
+    __device__ __forceinline__ float2 get(const GroupArgs& a, int c, int y) const {
+        return at[(c % V) * (blockDim.x + 1) + y * a.tx + c / V];
+    }
 };
 
 // ── forward ──────────────────────────────────────────────────────────────
-// This thread's columns' means and sums of squared deviations over its rows of [lo, hi).
-template <class T, bool ALIGNED>
+// This thread's columns' means and sums of squared deviations over its rows of
+// [lo, hi), U of them at a time.
+template <int U, class T, bool ALIGNED>
 __device__ __forceinline__ void part_sums(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* x, int64_t ldx, int lo, int hi,
-                                          Sums<T>& sh) {
+                                          const Sums<T>& sh) {
     constexpr int V = Place<T, ALIGNED>::V;
     float k[V], s[V], q[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) k[j] = s[j] = q[j] = 0.0f;
-    int n = 0;
-    p.template for_rows<4>(a, lo, hi, x, ldx, [&](int, const float (&z)[V]) {
-        if (n++ == 0) {
+    const int n = p.rows_of(a, lo, hi);
+    bool first = true;
+    p.template for_rows<U>(a, lo, hi, x, ldx, static_cast<T*>(nullptr), 0, [&](float (&z)[V], T*, int u) {
+        if (u == 0 && first) {
 #pragma unroll
             for (int j = 0; j < V; ++j) k[j] = z[j];
-        } else {
+            first = false;
+        }
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = __fsub_rn(z[j], k[j]);
-                s[j] = __fadd_rn(s[j], d);
-                q[j] = fmaf(d, d, q[j]);
-            }
+        for (int j = 0; j < V; j += 2) {
+            const Pair d = add2(Pair(z[j], z[j + 1]), Pair(-k[j], -k[j + 1]));
+            add2(Pair(s[j], s[j + 1]), d).get(s[j], s[j + 1]);
+            fma2(d, d, Pair(q[j], q[j + 1])).get(q[j], q[j + 1]);
         }
     });
     // (a value that is not finite: x - x is a NaN, and so are the deviations)
@@ -198,8 +233,7 @@ __device__ __forceinline__ void part_sums(const GroupArgs& a, const Place<T, ALI
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const float bad = __fsub_rn(k[j], k[j]);
-        sh.at[j][threadIdx.x] = make_float2(fmaf(s[j], inv, k[j]),
-                                            __fadd_rn(max_nan(fmaf(-s[j], __fmul_rn(s[j], inv), q[j]), 0.0f), bad));
+        sh.set(j, make_float2(fmaf(s[j], inv, k[j]), __fadd_rn(max_nan(fmaf(-s[j], __fmul_rn(s[j], inv), q[j]), 0.0f), bad)));
     }
 }
 // (mean, sum of squared deviations) of the block's column c over all row lanes of a part of `rows` rows.
@@ -228,19 +262,20 @@ __device__ __forceinline__ void for_columns(const GroupArgs& a, F&& f) {
 
 // part[slot * cols + column] = (mean, sum of squared deviations) of the part's values.
 template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(kMaxThreads, 4) group_parts_kernel(const GroupArgs a, const T* x, int64_t ldx, float2* part) {
-    __shared__ Sums<T> sh;
+__global__ void __launch_bounds__(kMaxThreads, kParts) group_parts_kernel(const GroupArgs a, const T* x, int64_t ldx, float2* part) {
+    extern __shared__ float2 room[];
+    const Sums<T> sh{room};
     wait_for_previous();
     const Place<T, ALIGNED> p(a);
-    for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
-        for_parts(a, c, [&](int g, int lo, int hi) {
-            part_sums(a, p, x, ldx, lo, hi, sh);
-            __syncthreads();
-            for_columns<T>(a, [&](int i, int column) {
-                part[static_cast<int64_t>(c + g) * a.cols + column] = join_lanes(a, sh, i, hi - lo);
-            });
-            __syncthreads();
+    const int c = blockIdx.x;
+    for_parts(a, c, [&](int g, int lo, int hi) {
+        part_sums<4>(a, p, x, ldx, lo, hi, sh);
+        __syncthreads();
+        for_columns<T>(a, [&](int i, int column) {
+            part[static_cast<int64_t>(c + g) * a.cols + column] = join_lanes(a, sh, i, hi - lo);
         });
+        __syncthreads();
+    });
 }
 
 // Calls f(part, rows of it, column) for this thread's parts of a graph's group
@@ -252,10 +287,11 @@ __device__ __forceinline__ void for_slots(const GroupArgs& a, int g, int b, int 
     const int wide = a.per < W ? a.per : W, step = W / wide, t = threadIdx.x % W;
     if (t >= wide * step) return;
     for (int col = t % wide; col < a.per; col += wide)
+#pragma unroll 4
         for (int i = t / wide; i < slots; i += step) {
-            const int64_t r0 = static_cast<int64_t>(first + i) * a.R, r1 = r0 + a.R;
-            f(part[static_cast<int64_t>(first + i + g) * a.cols + c0 + col],
-              static_cast<int>((e < r1 ? e : r1) - (b > r0 ? b : r0)), c0 + col);
+            // (a slot's rows; the last chunk's end may pass 2^31)
+            const int r0 = (first + i) * a.R, r1 = e - r0 < a.R ? e : r0 + a.R;
+            f(part[static_cast<int64_t>(first + i + g) * a.cols + c0 + col], r1 - (b > r0 ? b : r0), c0 + col);
         }
 }
 // The sum over W threads (a warp, or the block).
@@ -273,26 +309,30 @@ __device__ __forceinline__ float sum_of(float v, float* sh) {
 
 // stats[g * groups + group] = (mean, rstd), (0, 0) for a graph without rows.
 template <int W>
-__global__ void __launch_bounds__(kMaxThreads) group_stats_kernel(const GroupArgs a, const float2* part, float2* stats) {
-    __shared__ float sh[8];
+__global__ void __launch_bounds__(kJoinBlock<W>) group_stats_kernel(const GroupArgs a, const float2* part, float2* stats) {
+    __shared__ float sh[32];
     wait_for_previous();
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kMaxThreads / W) + threadIdx.x / W;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinBlock<W> / W) + threadIdx.x / W;
     if (i >= static_cast<int64_t>(a.graphs) * a.groups) return;
     const int g = static_cast<int>(i / a.groups), c0 = static_cast<int>(i % a.groups) * a.per;
     const int b = begin_of(a, g), e = end_of(a, g);
     float2 r = make_float2(0.0f, 0.0f);
     if (b < e) {
         const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
-        // (about the first part's mean, so that the sum does not lose the differences)
+        // The parts' means m about the first part's, k: as in a part, the sum of
+        // n (m - k)^2 less that of their mean cannot lose the deviations.
         const float k = part[static_cast<int64_t>(b / a.R + g) * a.cols + c0].x;
         float s = 0.0f, d = 0.0f;
-        for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) { s = fmaf(__fsub_rn(p.x, k), static_cast<float>(n), s); });
-        const float mean = __fadd_rn(k, __fdiv_rn(sum_of<W>(s, sh), all));
         for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) {
-            const float x = __fsub_rn(p.x, mean);
-            d = __fadd_rn(d, fmaf(__fmul_rn(x, x), static_cast<float>(n), p.y));
+            const float z = __fsub_rn(p.x, k), w = __fmul_rn(z, static_cast<float>(n));
+            s = __fadd_rn(s, w);
+            d = __fadd_rn(d, fmaf(z, w, p.y));
         });
-        r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(sum_of<W>(d, sh), all), a.eps)));
+        s = sum_of<W>(s, sh);
+        d = sum_of<W>(d, sh);
+        const float shift = __fdiv_rn(s, all), mean = __fadd_rn(k, shift);
+        d = max_nan(fmaf(-s, shift, d), 0.0f);
+        r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(d, all), a.eps)));
     }
     if (threadIdx.x % W == 0) stats[i] = r;
 }
@@ -310,35 +350,45 @@ struct OfGroup {
     __device__ __forceinline__ const float2& operator[](int j) const { return at[SPLIT ? j : 0]; }
 };
 
+// A thread's gamma and beta.
+template <int V>
+struct Params {
+    float gamma[V], beta[V];
+    template <class T, bool ALIGNED, class P>
+    __device__ __forceinline__ Params(const Place<T, ALIGNED>& p, const P* g, const P* b) {
+        p.params(g, gamma);
+        p.params(b, beta);
+    }
+};
+
 // y of this thread's rows of [lo, hi), a part of the graph with the groups' statistics `stats`.
-template <bool SPLIT, class T, bool ALIGNED, class P>
-__device__ __forceinline__ void apply_part(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* x, int64_t ldx, const P* gamma,
-                                           const P* beta, const float2* stats, T* y, int64_t ldy, int lo, int hi) {
-    constexpr int V = Place<T, ALIGNED>::V;
+template <bool SPLIT, class T, bool ALIGNED, int V>
+__device__ __forceinline__ void apply_part(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* x, int64_t ldx,
+                                           const Params<V>& k, const float2* stats, T* y, int64_t ldy, int lo, int hi) {
     if (p.n <= 0) return;
-    float A[V], B[V];
-    p.params(gamma, A);
-    p.params(beta, B);
     const OfGroup<V, SPLIT> st(a, stats, p.col);
+    float A[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) A[j] = __fmul_rn(A[j], st[j].y);
-    p.template for_rows<4>(a, lo, hi, x, ldx, [&](int r, float (&z)[V]) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) z[j] = fmaf(__fsub_rn(z[j], st[j].x), A[j], B[j]);
+    for (int j = 0; j < V; ++j) A[j] = __fmul_rn(k.gamma[j], st[j].y);
+    p.template for_rows<4>(a, lo, hi, x, ldx, y, ldy, [&](float (&z)[V], T* to, int) {
+        pairs(z, [&](int j, Pair v) {
+            return fma2(add2(v, Pair(-st[j].x, -st[j + 1].x)), Pair(A[j], A[j + 1]), Pair(k.beta[j], k.beta[j + 1]));
+        });
         act_forward<sizeof(T) == 2>(z, a.act, a.alpha);
-        p.store(y + r * ldy, z);
+        p.store(to, z);
     });
 }
 
 template <class T, class P, bool ALIGNED, bool SPLIT>
-__global__ void __launch_bounds__(kMaxThreads, 4) group_apply_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
+__global__ void __launch_bounds__(kMaxThreads, kApply<SPLIT>) group_apply_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
                                                                   const P* beta, const float2* stats, T* y, int64_t ldy) {
     wait_for_previous();
     const Place<T, ALIGNED> p(a);
-    for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
-        for_parts(a, c, [&](int g, int lo, int hi) {
-            apply_part<SPLIT>(a, p, x, ldx, gamma, beta, stats + static_cast<int64_t>(g) * a.groups, y, ldy, lo, hi);
-        });
+    const int c = blockIdx.x;
+    for_parts(a, c, [&](int g, int lo, int hi) {
+        const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
+        apply_part<SPLIT>(a, p, x, ldx, k, stats + static_cast<int64_t>(g) * a.groups, y, ldy, lo, hi);
+    });
 }
 
 // Adds f(column)'s pairs over the columns of each group; put(group, sum) by one
@@ -363,13 +413,14 @@ constexpr int kSmallCols = 2048;  // most columns of a block that has whole grap
 
 // A block for each graph: its second reading of x comes from L1 or L2.
 template <class T, class P, bool ALIGNED, bool SPLIT>
-__global__ void __launch_bounds__(kMaxThreads, 4) group_small_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
+__global__ void __launch_bounds__(kMaxThreads, 2) group_small_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
                                                                   const P* beta, float2* stats, T* y, int64_t ldy) {
-    __shared__ Sums<T> sh;
-    extern __shared__ float2 columns[];  // cols, and the groups' means and statistics
-    float2* mine = columns + a.cols;
+    extern __shared__ float2 room[];
+    const Sums<T> sh{room};
+    float2 *columns = room + Sums<T>::pairs(blockDim.x), *mine = columns + a.cols;  // the columns', the groups' statistics
     wait_for_previous();
     const Place<T, ALIGNED> p(a);
+    const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
     for (int g = blockIdx.x; g < a.graphs; g += gridDim.x) {
         const int b = begin_of(a, g), e = end_of(a, g);
         float2* out = stats + static_cast<int64_t>(g) * a.groups;
@@ -377,7 +428,7 @@ __global__ void __launch_bounds__(kMaxThreads, 4) group_small_kernel(const Group
             for (int i = threadIdx.x; i < a.groups; i += blockDim.x) out[i] = make_float2(0.0f, 0.0f);
             continue;
         }
-        part_sums(a, p, x, ldx, b, e, sh);
+        part_sums<8>(a, p, x, ldx, b, e, sh);
         __syncthreads();
         for_columns<T>(a, [&](int i, int column) { columns[column] = join_lanes(a, sh, i, e - b); });
         __syncthreads();
@@ -397,62 +448,55 @@ __global__ void __launch_bounds__(kMaxThreads, 4) group_small_kernel(const Group
                 if (first) mine[i] = out[i] = r;
             });
         __syncthreads();
-        apply_part<SPLIT>(a, p, x, ldx, gamma, beta, mine, y, ldy, b, e);
+        apply_part<SPLIT>(a, p, x, ldx, k, mine, y, ldy, b, e);
     }
 }
 
 // ── backward ─────────────────────────────────────────────────────────────
-// What a column's du takes: u = A (x - mean) + B.
-template <class T, bool ALIGNED, bool SPLIT>
+// What a column's du takes: u = A (x - mean) + beta.
+template <int V, bool SPLIT>
 struct Slopes {
-    static constexpr int V = Place<T, ALIGNED>::V;
-    float A[V], B[V];
+    float A[V];
+    const Params<V>& k;
     OfGroup<V, SPLIT> st;
-    template <class P>
-    __device__ __forceinline__ Slopes(const GroupArgs& a, const Place<T, ALIGNED>& p, const P* gamma, const P* beta, const float2* stats)
-        : st(a, stats, p.col) {
-        p.params(gamma, A);
-        p.params(beta, B);
+    __device__ __forceinline__ Slopes(const GroupArgs& a, int col, const Params<V>& k_, const float2* stats) : k(k_), st(a, stats, col) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) A[j] = __fmul_rn(A[j], st[j].y);
+        for (int j = 0; j < V; ++j) A[j] = __fmul_rn(k.gamma[j], st[j].y);
     }
     // x <- x - mean, dy <- du
+    template <bool FAST>
     __device__ __forceinline__ void du(const GroupArgs& a, float (&x)[V], float (&dy)[V]) const {
         float u[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            x[j] = __fsub_rn(x[j], st[j].x);
-            u[j] = fmaf(x[j], A[j], B[j]);
+        for (int j = 0; j < V; j += 2) {
+            const Pair z = add2(Pair(x[j], x[j + 1]), Pair(-st[j].x, -st[j + 1].x));
+            z.get(x[j], x[j + 1]);
+            fma2(z, Pair(A[j], A[j + 1]), Pair(k.beta[j], k.beta[j + 1])).get(u[j], u[j + 1]);
         }
-        act_slope<sizeof(T) == 2>(u, a.act, a.alpha);
-#pragma unroll
-        for (int j = 0; j < V; ++j) dy[j] = __fmul_rn(dy[j], u[j]);
+        act_slope<FAST>(u, a.act, a.alpha);
+        pairs(dy, [&](int j, Pair d) { return mul2(d, Pair(u[j], u[j + 1])); });
     }
 };
 
 // This thread's columns' (sum du, sum du h) over its rows of [lo, hi).
-template <bool SPLIT, class T, bool ALIGNED, class P>
+template <bool SPLIT, class T, bool ALIGNED, int V>
 __device__ __forceinline__ void grad_sums(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* dy, int64_t lddy, const T* x,
-                                          int64_t ldx, const P* gamma, const P* beta, const float2* stats, int lo, int hi, Sums<T>& sh) {
-    constexpr int V = Place<T, ALIGNED>::V;
+                                          int64_t ldx, const Params<V>& params, const float2* stats, int lo, int hi, const Sums<T>& sh) {
     float s[V], t[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s[j] = t[j] = 0.0f;
     if (p.n > 0) {
-        const Slopes<T, ALIGNED, SPLIT> k(a, p, gamma, beta, stats);
-        p.template for_rows<2>(a, lo, hi, x, ldx, dy, lddy, [&](int, float (&z)[V], float (&d)[V]) {
-            k.du(a, z, d);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                s[j] = __fadd_rn(s[j], d[j]);
-                t[j] = fmaf(d[j], z[j], t[j]);  // (times r below)
-            }
+        const Slopes<V, SPLIT> k(a, p.col, params, stats);
+        p.template for_rows<SPLIT ? 2 : 4>(a, lo, hi, x, ldx, dy, lddy, static_cast<T*>(nullptr), 0, [&](float (&z)[V], float (&d)[V], T*) {
+            k.template du<sizeof(T) == 2>(a, z, d);
+            pairs(s, [&](int j, Pair v) { return add2(v, Pair(d[j], d[j + 1])); });
+            pairs(t, [&](int j, Pair v) { return fma2(Pair(d[j], d[j + 1]), Pair(z[j], z[j + 1]), v); });  // (times r below)
         });
 #pragma unroll
         for (int j = 0; j < V; ++j) t[j] = __fmul_rn(t[j], k.st[j].y);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) sh.at[j][threadIdx.x] = make_float2(s[j], t[j]);
+    for (int j = 0; j < V; ++j) sh.set(j, make_float2(s[j], t[j]));
 }
 template <class T>
 __device__ __forceinline__ float2 add_lanes(const GroupArgs& a, const Sums<T>& sh, int c) {
@@ -466,48 +510,50 @@ __device__ __forceinline__ float2 add_lanes(const GroupArgs& a, const Sums<T>& s
 }
 
 // dx of this thread's rows of [lo, hi); means: the groups' (mean g, mean g h).
-template <bool SPLIT, class T, bool ALIGNED, class P>
+template <bool SPLIT, class T, bool ALIGNED, int V>
 __device__ __forceinline__ void grad_part(const GroupArgs& a, const Place<T, ALIGNED>& p, const T* dy, int64_t lddy, const T* x,
-                                          int64_t ldx, const P* gamma, const P* beta, const float2* stats, const float2* means, T* dx,
+                                          int64_t ldx, const Params<V>& params, const float2* stats, const float2* means, T* dx,
                                           int64_t lddx, int lo, int hi) {
-    constexpr int V = Place<T, ALIGNED>::V;
     if (p.n <= 0) return;
-    const Slopes<T, ALIGNED, SPLIT> k(a, p, gamma, beta, stats);
+    const Slopes<V, SPLIT> k(a, p.col, params, stats);
     OfGroup<V, SPLIT> de(a, means, p.col);
 #pragma unroll
-    for (int j = 0; j < de.N; ++j) {
-        de.at[j] = make_float2(-__fmul_rn(k.st[j].y, de.at[j].x), __fmul_rn(__fmul_rn(k.st[j].y, k.st[j].y), de.at[j].y));
-    }
-    p.template for_rows<2>(a, lo, hi, x, ldx, dy, lddy, [&](int r, float (&z)[V], float (&d)[V]) {
-        k.du(a, z, d);
-#pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = fmaf(k.A[j], d[j], fmaf(-de[j].y, z[j], de[j].x));
-        p.store(dx + r * lddx, d);
+    for (int j = 0; j < de.N; ++j)
+        de.at[j] = make_float2(-__fmul_rn(k.st[j].y, de.at[j].x), -__fmul_rn(__fmul_rn(k.st[j].y, k.st[j].y), de.at[j].y));
+    p.template for_rows<SPLIT ? 2 : 4>(a, lo, hi, x, ldx, dy, lddy, dx, lddx, [&](float (&z)[V], float (&d)[V], T* to) {
+        k.template du<sizeof(T) == 2>(a, z, d);
+        pairs(d, [&](int j, Pair v) {
+            return fma2(Pair(k.A[j], k.A[j + 1]), v,
+                        fma2(Pair(de[j].y, de[j + 1].y), Pair(z[j], z[j + 1]), Pair(de[j].x, de[j + 1].x)));
+        });
+        p.store(to, d);
     });
 }
 
 // part[slot * cols + column] = (sum du, sum du h) of the part; sums[block][2][cols]
 // = (sum du h, sum du) over the block's rows.
 template <class T, class P, bool ALIGNED, bool SPLIT>
-__global__ void __launch_bounds__(kMaxThreads, 3) group_grad_parts_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
+__global__ void __launch_bounds__(kMaxThreads, kGrad) group_grad_parts_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
                                                                        int64_t ldx, const P* gamma, const P* beta,
                                                                        const float2* stats, float2* part, float* sums) {
-    __shared__ Sums<T> sh;
-    extern __shared__ float2 total[];  // tx V columns
+    extern __shared__ float2 room[];
+    const Sums<T> sh{room};
+    float2* total = room + Sums<T>::pairs(blockDim.x);  // of the block's columns
     wait_for_previous();
     const Place<T, ALIGNED> p(a);
     for (int i = threadIdx.x; i < a.tx * Sums<T>::V; i += blockDim.x) total[i] = make_float2(0.0f, 0.0f);
-    for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
-        for_parts(a, c, [&](int g, int lo, int hi) {
-            grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, stats + static_cast<int64_t>(g) * a.groups, lo, hi, sh);
-            __syncthreads();
-            for_columns<T>(a, [&](int i, int column) {
-                const float2 s = add_lanes(a, sh, i);
-                part[static_cast<int64_t>(c + g) * a.cols + column] = s;
-                total[i] = make_float2(__fadd_rn(total[i].x, s.x), __fadd_rn(total[i].y, s.y));
-            });
-            __syncthreads();
+    const int c = blockIdx.x;
+    for_parts(a, c, [&](int g, int lo, int hi) {
+        const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
+        grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, k, stats + static_cast<int64_t>(g) * a.groups, lo, hi, sh);
+        __syncthreads();
+        for_columns<T>(a, [&](int i, int column) {
+            const float2 s = add_lanes(a, sh, i);
+            part[static_cast<int64_t>(c + g) * a.cols + column] = s;
+            total[i] = make_float2(__fadd_rn(total[i].x, s.x), __fadd_rn(total[i].y, s.y));
         });
+        __syncthreads();
+    });
     float* out = sums + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
     for_columns<T>(a, [&](int i, int column) {
         out[column] = total[i].y;
@@ -515,21 +561,27 @@ __global__ void __launch_bounds__(kMaxThreads, 3) group_grad_parts_kernel(const 
     });
 }
 
-// dgamma and dbeta: the sums of the blocks' rows in their order.  (32 columns a block.)
+// dgamma and dbeta: the sums of the blocks' rows in their order, kJoinColumns
+// columns a block.
+constexpr int kJoinColumns = 8;
 template <class P>
 __device__ __forceinline__ void join_params(const GroupArgs& a, int block, const float* sums, int sum_rows, P* dgamma, P* dbeta,
                                             float* sh) {
-    const int c = block * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+    const int c = block * kJoinColumns + threadIdx.x % kJoinColumns, lane = threadIdx.x / kJoinColumns;
+    const int lanes = blockDim.x / kJoinColumns;
     float s = 0.0f;
     if (c < 2 * a.cols) {
-#pragma unroll 4
-        for (int r = lane; r < sum_rows; r += kMaxThreads / 32) s = __fadd_rn(s, sums[static_cast<int64_t>(r) * 2 * a.cols + c]);
+#pragma unroll 8
+        for (int r = lane; r < sum_rows; r += lanes) s = __fadd_rn(s, sums[static_cast<int64_t>(r) * 2 * a.cols + c]);
     }
-    sh[threadIdx.x] = s;
+    // the lanes of a warp have the same columns four times over
+    s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 8));
+    s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, 16));
+    if (threadIdx.x % 32 < kJoinColumns) sh[threadIdx.x / 32 * kJoinColumns + threadIdx.x % 32] = s;
     __syncthreads();
     if (lane == 0 && c < 2 * a.cols) {
         s = 0.0f;
-        for (int w = 0; w < kMaxThreads / 32; ++w) s = __fadd_rn(s, sh[w * 32 + threadIdx.x]);
+        for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) s = __fadd_rn(s, sh[w * kJoinColumns + threadIdx.x]);
         if (c < a.cols) dgamma[c] = from_f32<P>(s);
         else dbeta[c - a.cols] = from_f32<P>(s);
     }
@@ -538,16 +590,16 @@ __device__ __forceinline__ void join_params(const GroupArgs& a, int block, const
 // means[g * groups + group] = (mean g, mean g h), in the first `blocks` blocks;
 // dgamma and dbeta in the others.
 template <class P, int W>
-__global__ void __launch_bounds__(kMaxThreads) group_grad_join_kernel(const GroupArgs a, const float2* part, const P* gamma,
+__global__ void __launch_bounds__(kJoinBlock<W>) group_grad_join_kernel(const GroupArgs a, const float2* part, const P* gamma,
                                                                       const float* sums, int sum_rows, int blocks, float2* means,
                                                                       P* dgamma, P* dbeta) {
-    __shared__ float sh[kMaxThreads];
+    __shared__ float sh[kJoinBlock<W> / 32 * kJoinColumns];
     wait_for_previous();
     if (static_cast<int>(blockIdx.x) >= blocks) {
         join_params(a, static_cast<int>(blockIdx.x) - blocks, sums, sum_rows, dgamma, dbeta, sh);
         return;
     }
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kMaxThreads / W) + threadIdx.x / W;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinBlock<W> / W) + threadIdx.x / W;
     if (i >= static_cast<int64_t>(a.graphs) * a.groups) return;
     const int g = static_cast<int>(i / a.groups), c0 = static_cast<int>(i % a.groups) * a.per;
     const int b = begin_of(a, g), e = end_of(a, g);
@@ -565,43 +617,46 @@ __global__ void __launch_bounds__(kMaxThreads) group_grad_join_kernel(const Grou
 }
 
 template <class P>
-__global__ void __launch_bounds__(kMaxThreads) group_params_kernel(const GroupArgs a, const float* sums, int sum_rows, P* dgamma,
+__global__ void __launch_bounds__(kJoinThreads) group_params_kernel(const GroupArgs a, const float* sums, int sum_rows, P* dgamma,
                                                                    P* dbeta) {
-    __shared__ float sh[kMaxThreads];
+    __shared__ float sh[kJoinThreads / 32 * kJoinColumns];
     wait_for_previous();
     join_params(a, static_cast<int>(blockIdx.x), sums, sum_rows, dgamma, dbeta, sh);
 }
 
 template <class T, class P, bool ALIGNED, bool SPLIT>
-__global__ void __launch_bounds__(kMaxThreads, 3) group_grad_apply_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
+__global__ void __launch_bounds__(kMaxThreads, kGrad) group_grad_apply_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
                                                                        int64_t ldx, const P* gamma, const P* beta,
                                                                        const float2* stats, const float2* means, T* dx,
                                                                        int64_t lddx) {
     wait_for_previous();
     const Place<T, ALIGNED> p(a);
-    for (int c = blockIdx.x; c < a.chunks; c += gridDim.x)
-        for_parts(a, c, [&](int g, int lo, int hi) {
-            const int64_t o = static_cast<int64_t>(g) * a.groups;
-            grad_part<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, stats + o, means + o, dx, lddx, lo, hi);
-        });
+    const int c = blockIdx.x;
+    for_parts(a, c, [&](int g, int lo, int hi) {
+        const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
+        const int64_t o = static_cast<int64_t>(g) * a.groups;
+        grad_part<SPLIT>(a, p, dy, lddy, x, ldx, k, stats + o, means + o, dx, lddx, lo, hi);
+    });
 }
 
 // A block for each graph.
 template <class T, class P, bool ALIGNED, bool SPLIT>
-__global__ void __launch_bounds__(kMaxThreads, 3) group_grad_small_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
+__global__ void __launch_bounds__(kMaxThreads, 2) group_grad_small_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
                                                                        int64_t ldx, const P* gamma, const P* beta,
                                                                        const float2* stats, T* dx, int64_t lddx, float* sums) {
-    __shared__ Sums<T> sh;
-    extern __shared__ float2 columns[];  // cols sums of a graph, cols sums of all, the groups' means
-    float2 *total = columns + a.cols, *means = total + a.cols;
+    extern __shared__ float2 room[];
+    const Sums<T> sh{room};
+    // the columns' sums in a graph and in all, the groups' means
+    float2 *columns = room + Sums<T>::pairs(blockDim.x), *total = columns + a.cols, *means = total + a.cols;
     wait_for_previous();
     const Place<T, ALIGNED> p(a);
+    const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
     for (int i = threadIdx.x; i < a.cols; i += blockDim.x) total[i] = make_float2(0.0f, 0.0f);
     for (int g = blockIdx.x; g < a.graphs; g += gridDim.x) {
         const int b = begin_of(a, g), e = end_of(a, g);
         if (b >= e) continue;
         const float2* st = stats + static_cast<int64_t>(g) * a.groups;
-        grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, st, b, e, sh);
+        grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, k, st, b, e, sh);
         __syncthreads();
         for_columns<T>(a, [&](int i, int column) {
             const float2 s = add_lanes(a, sh, i);
@@ -617,7 +672,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) group_grad_small_kernel(const 
                 if (first) means[i] = make_float2(__fdiv_rn(s.x, all), __fdiv_rn(s.y, all));
             });
         __syncthreads();
-        grad_part<SPLIT>(a, p, dy, lddy, x, ldx, gamma, beta, st, means, dx, lddx, b, e);
+        grad_part<SPLIT>(a, p, dy, lddy, x, ldx, k, st, means, dx, lddx, b, e);
     }
     __syncthreads();
     float* out = sums + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
@@ -640,15 +695,16 @@ void by_layout(const GroupArgs& a, bool aligned, F&& f) {
 }
 
 // Blocks as wide as the row (or an even share of it), up to 256 threads and 32
-// row lanes, and chunks of up to 32 rows a lane where that leaves four blocks an
-// SM.  (232,965 x 128 bf16, forward and gradient: CUT_FIGURES)
-GroupArgs cut(GroupArgs a, int V) {
+// row lanes, and one chunk for each of the `resident` blocks of an SM: a kernel
+// whose blocks run in one and a third waves takes as long as with two.
+GroupArgs cut(GroupArgs a, int V, int resident) {
     a.nv = static_cast<int>(ceil_div(a.cols, V));
     const int blocks = static_cast<int>(ceil_div(a.nv, kMaxThreads));
     a.tx = static_cast<int>(ceil_div(a.nv, blocks));
     a.ty = std::min(std::max(1, kMaxThreads / a.tx), 32);
-    const int64_t share = ceil_div(a.rows * blocks, int64_t(num_sms()) * 4 * a.ty);
-    a.R = a.ty * static_cast<int>(std::min<int64_t>(std::max<int64_t>(share, 1), 32));
+    const int threads = (a.tx * a.ty + 31) / 32 * 32;
+    const int64_t each = std::max<int64_t>(1, int64_t(num_sms()) * resident * (kMaxThreads / threads) / blocks);
+    a.R = a.ty * static_cast<int>(std::max<int64_t>(1, ceil_div(a.rows, each * a.ty)));
     a.chunks = static_cast<int>(ceil_div(a.rows, a.R));
     return a;
 }
@@ -660,25 +716,29 @@ bool small_graphs(const GroupArgs& a, size_t size) {
     const int64_t bytes = a.rows * a.cols * static_cast<int64_t>(size);
     return a.nv <= kMaxThreads && a.cols <= kSmallCols && bytes <= 16 << 20 && bytes / a.graphs <= 32 << 10;
 }
-// The cut of such graphs: two rows a lane.
+// The cut of such graphs: eight rows a lane.
 GroupArgs cut_small(GroupArgs a) {
-    const int64_t lanes = std::max<int64_t>(ceil_div(ceil_div(a.rows, a.graphs), 2), 1);
+    const int64_t lanes = std::max<int64_t>(ceil_div(ceil_div(a.rows, a.graphs), 8), 1);
     a.ty = static_cast<int>(std::min<int64_t>(a.ty, std::max<int64_t>(lanes, ceil_div(32, a.tx))));
     return a;
 }
 dim3 block_of(const GroupArgs& a) { return dim3(static_cast<unsigned>((a.tx * a.ty + 31) / 32 * 32)); }
-dim3 grid_of(const GroupArgs& a) {
-    const int64_t y = ceil_div(a.nv, a.tx);
-    return dim3(static_cast<unsigned>(std::min<int64_t>(a.chunks, std::max<int64_t>(1, int64_t(num_sms()) * 8 / y))),
-                static_cast<unsigned>(y));
-}
-int small_blocks(const GroupArgs& a) {
-    return static_cast<int>(std::min<int64_t>(a.graphs, int64_t(num_sms()) * std::min(16, 2048 / static_cast<int>(block_of(a).x))));
+dim3 grid_of(const GroupArgs& a) { return dim3(static_cast<unsigned>(a.chunks), static_cast<unsigned>(ceil_div(a.nv, a.tx))); }
+// Blocks with `room` bytes of shared memory that run at a time, at most one a graph (`threads` an SM).
+int small_blocks(const GroupArgs& a, size_t room, int threads) {
+    const int fit = std::min({16, threads / static_cast<int>(block_of(a).x), static_cast<int>(228 * 1024 / (room + 1024))});
+    return static_cast<int>(std::min<int64_t>(a.graphs, int64_t(num_sms()) * std::max(1, fit)));
 }
 size_t slots_of(const GroupArgs& a) { return (static_cast<size_t>(a.chunks) + a.graphs) * a.cols; }
-// Whether a graph's group has so many parts (were the graphs alike) that a
-// block joins them, not a warp.
-bool many_parts(const GroupArgs& a) { return (a.rows / a.R / a.graphs + 1) * a.per > 256; }
+// Calls f with the threads that join a graph's group: by its parts, were the
+// graphs alike.
+template <class F>
+void by_parts(const GroupArgs& a, F&& f) {
+    const int64_t parts = (a.rows / a.R / std::max(a.graphs, 1) + 1) * a.per;
+    if (parts <= 256) f(std::integral_constant<int, 32>{});
+    else if (parts <= 4096) f(std::integral_constant<int, 256>{});
+    else f(std::integral_constant<int, kJoinThreads>{});
+}
 
 void check_group(const char* fn, int64_t rows, int64_t cols, int64_t groups, int64_t graphs, const int32_t* offsets, int dtype,
                  int param_dtype, int act) {
@@ -735,29 +795,31 @@ TG_API tg_status tg_group_norm(int64_t rows, int64_t cols, int64_t groups, int64
             const T* xp = static_cast<const T*>(x);
             const P *ga = static_cast<const P*>(gamma), *be = static_cast<const P*>(beta);
             const bool aligned = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(y, ldy, sizeof(T));
-            const GroupArgs a = cut(g, 16 / sizeof(T));
+            const GroupArgs a = cut(g, 16 / sizeof(T), kParts);
             float2* st = reinterpret_cast<float2*>(stats);
             by_layout<T>(a, aligned, [&](auto al, auto split) {
                 constexpr bool ALIGNED = decltype(al)::value, SPLIT = decltype(split)::value;
                 if (small_graphs(a, sizeof(T))) {
                     const GroupArgs c = cut_small(a);
-                    const size_t room = (cols + groups) * sizeof(float2);
+                    const size_t room = (Sums<T>::pairs(block_of(c).x) + cols + groups) * sizeof(float2);
                     auto kern = group_small_kernel<T, P, ALIGNED, SPLIT>;
-                    if (room > 24 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
-                    launch_dependent("group_norm", kern, dim3(static_cast<unsigned>(small_blocks(c))), block_of(c), room, s, c, xp, ldx,
+                    if (room > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
+                    launch_dependent("group_norm", kern, dim3(static_cast<unsigned>(small_blocks(c, room, 512))), block_of(c), room, s, c, xp, ldx,
                                      ga, be, st, static_cast<T*>(y), ldy);
                     return;
                 }
                 Scratch<float2> part(slots_of(a), s);
-                launch_dependent("group_norm_parts", group_parts_kernel<T, ALIGNED>, grid_of(a), block_of(a), 0, s, a, xp, ldx, part.p);
+                launch_dependent("group_norm_parts", group_parts_kernel<T, ALIGNED>, grid_of(a), block_of(a),
+                                 Sums<T>::pairs(block_of(a).x) * sizeof(float2), s, a, xp, ldx, part.p);
                 const int64_t sets = graphs * groups;
-                if (many_parts(a))
-                    launch_dependent("group_norm_stats", group_stats_kernel<kMaxThreads>, dim3(static_cast<unsigned>(sets)),
-                                     dim3(kMaxThreads), 0, s, a, part.p, st);
-                else
-                    launch_dependent("group_norm_stats", group_stats_kernel<32>, dim3(static_cast<unsigned>(ceil_div(sets, 8))),
-                                     dim3(kMaxThreads), 0, s, a, part.p, st);
-                launch_dependent("group_norm", group_apply_kernel<T, P, ALIGNED, SPLIT>, grid_of(a), block_of(a), 0, s, a, xp, ldx, ga,
+                by_parts(a, [&](auto width) {
+                    constexpr int W = decltype(width)::value;
+                    launch_dependent("group_norm_stats", group_stats_kernel<W>,
+                                     dim3(static_cast<unsigned>(ceil_div(sets, kJoinBlock<W> / W))), dim3(kJoinBlock<W>), 0, s, a, part.p,
+                                     st);
+                });
+                const GroupArgs c = cut(g, 16 / sizeof(T), kApply<SPLIT>);
+                launch_dependent("group_norm", group_apply_kernel<T, P, ALIGNED, SPLIT>, grid_of(c), block_of(c), 0, s, c, xp, ldx, ga,
                                  be, st, static_cast<T*>(y), ldy);
             });
         });
@@ -795,23 +857,23 @@ TG_API tg_status tg_group_norm_grad(int64_t rows, int64_t cols, int64_t groups, 
             const P *ga = static_cast<const P*>(gamma), *be = static_cast<const P*>(beta);
             const bool aligned = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(dy, lddy, sizeof(T)) &&
                                  rows_aligned16(dx, lddx, sizeof(T));
-            const GroupArgs a = cut(g, 16 / sizeof(T));
+            const GroupArgs a = cut(g, 16 / sizeof(T), kGrad);
             const float2* st = reinterpret_cast<const float2*>(stats);
-            const int col_blocks = static_cast<int>(ceil_div(2 * cols, 32));
+            const int col_blocks = static_cast<int>(ceil_div(2 * cols, kJoinColumns));
             P *dg = static_cast<P*>(dgamma), *db = static_cast<P*>(dbeta);
             by_layout<T>(a, aligned, [&](auto al, auto split) {
                 constexpr bool ALIGNED = decltype(al)::value, SPLIT = decltype(split)::value;
                 if (graphs > 0 && small_graphs(a, sizeof(T))) {
                     const GroupArgs c = cut_small(a);
-                    const int blocks = small_blocks(c);
+                    const size_t room = (Sums<T>::pairs(block_of(c).x) + 2 * cols + groups) * sizeof(float2);
+                    const int blocks = small_blocks(c, room, 512);
                     Scratch<float> sums(static_cast<size_t>(blocks) * 2 * cols, s);
-                    const size_t room = (2 * cols + groups) * sizeof(float2);
                     auto kern = group_grad_small_kernel<T, P, ALIGNED, SPLIT>;
-                    if (room > 24 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
+                    if (room > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
                     launch_dependent("group_norm_grad", kern, dim3(static_cast<unsigned>(blocks)), block_of(c), room, s, c, dyp, lddy, xp,
                                      ldx, ga, be, st, static_cast<T*>(dx), lddx, sums.p);
                     launch_dependent("group_norm_grad_params", group_params_kernel<P>, dim3(static_cast<unsigned>(col_blocks)),
-                                     dim3(kMaxThreads), 0, s, c, sums.p, blocks, dg, db);
+                                     dim3(kJoinThreads), 0, s, c, sums.p, blocks, dg, db);
                     return;
                 }
                 const dim3 grid = grid_of(a);
@@ -821,16 +883,14 @@ TG_API tg_status tg_group_norm_grad(int64_t rows, int64_t cols, int64_t groups, 
                 Scratch<float> sums(static_cast<size_t>(sum_rows) * 2 * cols, s);
                 float2* means = part.p + slots_of(a);
                 launch_dependent("group_norm_grad_parts", group_grad_parts_kernel<T, P, ALIGNED, SPLIT>, grid, block_of(a),
-                                 a.tx * (16 / sizeof(T)) * sizeof(float2), s, a, dyp, lddy, xp, ldx, ga, be, st, part.p, sums.p);
-                const auto join = [&](auto width) {
+                                 (Sums<T>::pairs(block_of(a).x) + a.tx * (16 / sizeof(T))) * sizeof(float2), s, a, dyp, lddy, xp, ldx, ga, be, st, part.p, sums.p);
+                by_parts(a, [&](auto width) {
                     constexpr int W = decltype(width)::value;
-                    const int blocks = static_cast<int>(ceil_div(sets, kMaxThreads / W));
+                    const int blocks = static_cast<int>(ceil_div(sets, kJoinBlock<W> / W));
                     launch_dependent("group_norm_grad_join", group_grad_join_kernel<P, W>,
-                                     dim3(static_cast<unsigned>(blocks + col_blocks)), dim3(kMaxThreads), 0, s, a, part.p, ga, sums.p,
+                                     dim3(static_cast<unsigned>(blocks + col_blocks)), dim3(kJoinBlock<W>), 0, s, a, part.p, ga, sums.p,
                                      sum_rows, blocks, means, dg, db);
-                };
-                if (graphs > 0 && many_parts(a)) join(std::integral_constant<int, kMaxThreads>{});
-                else join(std::integral_constant<int, 32>{});
+                });
                 launch_dependent("group_norm_grad", group_grad_apply_kernel<T, P, ALIGNED, SPLIT>, grid, block_of(a), 0, s, a, dyp, lddy,
                                  xp, ldx, ga, be, st, means, static_cast<T*>(dx), lddx);
             });

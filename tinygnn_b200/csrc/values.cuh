@@ -242,6 +242,29 @@ __device__ __forceinline__ void store_some(T* p, const float (&x)[V], int n) {
     }
 }
 
+// Two floats an instruction.
+struct Pair {
+    uint64_t v;
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Pair(uint64_t x) : v(x) {}
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return Pair(r);
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a.v), "l"(b.v));
+    return Pair(r);
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return Pair(r);
+}
+
 // max(a, |b|) that keeps a NaN (fmaxf drops it).
 __device__ __forceinline__ float max_mag(float a, float b) {
     float r;
