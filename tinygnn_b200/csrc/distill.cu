@@ -33,7 +33,7 @@ struct DistillArgs {
     int64_t ldc;
     const void* teacher;  // rows x k
     int64_t ldt;
-    float temperature;
+    float temperature, inverse;  // inverse: 1 / temperature
     const float* weights;  // nullable
     float* loss;
 };
@@ -56,9 +56,9 @@ struct Teacher {
 
 // A lane's entries lane, lane + W, ... of a row as they were read.  They are
 // kept as they lie in memory: an instruction on them would wait for them.
-template <class T, class U, int W>
+template <class T, class U, int N_>
 struct Entries {
-    static constexpr int N = (kMaxTop + W - 1) / W;
+    static constexpr int W = 32, N = N_;
     uint2 c[N];
     U v[N];
     T z[N];  // the student's scores of the classes
@@ -93,7 +93,7 @@ struct Entries {
 // returned.  (A lane reads what it wrote, and t.c of all lanes.)
 template <int W>
 __device__ __forceinline__ float finish_teacher(const DistillArgs& a, int lane, const Teacher& t, float weight) {
-    const float c = __fdiv_rn(1.0f, a.temperature);
+    const float c = a.inverse;
     float most = -INFINITY;
     for (int i = lane; i < a.k; i += W) most = max_nan(most, t.q[i]);
     most = reduce_max<W>(most);
@@ -150,8 +150,8 @@ __device__ __forceinline__ float finish_teacher(const DistillArgs& a, int lane, 
 }
 
 // Fills `t` from a warp's entries; returned as above.
-template <class T, class U>
-__device__ __forceinline__ float read_teacher(const DistillArgs& a, const Entries<T, U, 32>& in, int lane, const Teacher& t) {
+template <class T, class U, int N>
+__device__ __forceinline__ float read_teacher(const DistillArgs& a, const Entries<T, U, N>& in, int lane, const Teacher& t) {
 #pragma unroll
     for (int i = 0; i < in.N; ++i) {
         const int e = lane + i * 32, j = in.class_of(a, i);
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
     wait_for_previous();
     const int lane = threadIdx.x % LPR, place = threadIdx.x / LPR, per = RPB * turns;
     const Teacher t = Teacher::in(reinterpret_cast<float*>(sh + stage) + place * Teacher::floats(a.k), a.k);
-    const float c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
+    const float c = FAST ? __fmul_rn(kLog2e, a.inverse) : a.inverse;
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
         const int rows = a.rows - r0 < per ? static_cast<int>(a.rows - r0) : per;
         T* st = stage_in(sh, x, ldx, r0, rows, a.n);
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
 // ring's slots kAhead are for the next rows.
 constexpr int kTeams = 4;
 
-template <class T, class U, bool GRAD>
+template <class T, class U, int N, bool GRAD>
 __global__ void __launch_bounds__(32 * kTeams, 5) distill_warp_kernel(const DistillArgs a, const T* x, int64_t ldx, T* dx,
                                                                       int64_t lddx, int slots) {
     constexpr bool FAST = sizeof(T) == 2;
@@ -333,12 +333,12 @@ __global__ void __launch_bounds__(32 * kTeams, 5) distill_warp_kernel(const Dist
     wait_for_previous();
     const int lane = threadIdx.x & 31, team = threadIdx.x >> 5;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kTeams, first = static_cast<int64_t>(blockIdx.x) * kTeams + team;
-    const float c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
+    const float c = FAST ? __fmul_rn(kLog2e, a.inverse) : a.inverse;
     Stream<T, 32> in(x, ldx, a.rows, a.n, first, step, 0, 0, room + team * slots * Stream<T, 32>::kSlot, slots, false);
     const Teacher t = Teacher::in(
         reinterpret_cast<float*>(room + kTeams * slots * Stream<T, 32>::kSlot) + team * Teacher::floats(a.k), a.k);
     // (a row's entries are asked for a row ahead, the scores of their classes at its start)
-    Entries<T, U, 32> entries;
+    Entries<T, U, N> entries;
     if (first < a.rows) entries.fetch(a, first, lane);
     for (int64_t row = first; row < a.rows; row += step) {
         const Part<T> p(x + row * ldx, a.n, 0, 0);
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(32 * kTeams, 5) distill_warp_kernel(const Dist
             add_scores<FAST, false>(s, z, c);
         }
         lanes_soft<FAST, false, 32>(s, c);
-        float loss = read_teacher<T, U>(a, entries, lane, t);
+        float loss = read_teacher(a, entries, lane, t);
         if (row + step < a.rows) entries.fetch(a, row + step, lane);
         const RowScale<FAST> r(s, c, *t.scale);
         for (int i = lane; i < a.k; i += 32)
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(NT + 32, 768 / NT) distill_wide_kernel(const D
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks()), log_ranks = __ffs(ranks) - 1;
     const int64_t clusters = gridDim.x / ranks, first = blockIdx.x / ranks;
-    const float c = __fdiv_rn(FAST ? kLog2e : 1.0f, a.temperature);
+    const float c = FAST ? __fmul_rn(kLog2e, a.inverse) : a.inverse;
     const auto meet = [] { asm volatile("bar.sync 2, %0;" ::"n"(NT + 32) : "memory"); };
     const auto all = [&] {  // the CTAs' states are there
         if (ranks > 1) cluster.sync();
@@ -463,12 +463,12 @@ __global__ void __launch_bounds__(NT + 32, 768 / NT) distill_wide_kernel(const D
         const auto entries = [&](int b) { return Teacher{teacher.c[b], teacher.q[b], teacher.z[b], &teacher.scale[b]}; };
         // A row's entries are asked for two rows ahead, the scores of their classes
         // while the row before is read, and put into shared memory after it.
-        Entries<T, U, 32> next;
+        Entries<T, U, kMaxTop / 32> next;
         float own = 0.0f;
         if (first < a.rows) {
             next.fetch(a, first, lane);
             next.fetch_scores(a, x + first * ldx);
-            own = read_teacher<T, U>(a, next, lane, entries(0));
+            own = read_teacher(a, next, lane, entries(0));
         }
         if (first + clusters < a.rows) next.fetch(a, first + clusters, lane);
         for (int64_t row = first; row < a.rows; row += clusters, ++round) {
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(NT + 32, 768 / NT) distill_wide_kernel(const D
                 for (int e = lane; e < a.k; e += 32)
                     if (t.c[e] >= 0 && r.w != 0.0f && p.has(t.c[e])) dx[row * lddx + t.c[e]] = from_f32<T>(entry_grad<FAST>(t, e, r));
             }
-            if (row + clusters < a.rows) own = read_teacher<T, U>(a, next, lane, entries(b ^ 1));
+            if (row + clusters < a.rows) own = read_teacher(a, next, lane, entries(b ^ 1));
             if (row + 2 * clusters < a.rows) next.fetch(a, row + 2 * clusters, lane);
         }
     }
@@ -518,7 +518,8 @@ void distill(const DistillArgs& a, const T* x, int64_t ldx, T* dx, int64_t lddx,
         using In = Stream<T, 32>;
         const int slots = (dx ? static_cast<int>(ceil_div(a.n / kVec<T>, 32 * In::W)) : 0) + kAhead;
         const int bytes = kTeams * (slots * In::kSlot + Teacher::floats(a.k) * 4);
-        auto kern = dx ? distill_warp_kernel<T, U, true> : distill_warp_kernel<T, U, false>;
+        auto kern = a.k <= 32 ? (dx ? distill_warp_kernel<T, U, 1, true> : distill_warp_kernel<T, U, 1, false>)
+                              : (dx ? distill_warp_kernel<T, U, kMaxTop / 32, true> : distill_warp_kernel<T, U, kMaxTop / 32, false>);
         launch_rows("distill_loss", kern, ceil_div(a.rows, kTeams), 1, std::min(5, kSharedSm / (bytes + 1024)), 32 * kTeams, bytes, s, a, x, ldx, dx,
                     lddx, slots);
         return;
@@ -575,10 +576,10 @@ TG_API tg_status tg_distill_loss(int64_t rows, int64_t classes, int32_t dtype, c
         check_ld(fn, "top_classes", ld_classes, k);
         check_ld(fn, "top_logits", ld_logits, k);
         if (dlogits) check_ld(fn, "dlogits", lddz, classes);
-        if (!(temperature > 0.0f && temperature <= 3.0e38f))
-            invalid(std::string(fn) + ": temperature must be positive and finite");
+        if (!(temperature >= 1e-30f && temperature <= 1e30f))
+            invalid(std::string(fn) + ": temperature must be positive and finite (1e-30 to 1e30)");
         const DistillArgs a{rows, static_cast<int>(classes), static_cast<int>(k), top_classes, class_bytes == 8, ld_classes,
-                            top_logits, ld_logits, temperature, weights, loss};
+                            top_logits, ld_logits, temperature, 1.0f / temperature, weights, loss};
         by_dtype(dtype, [&](auto t) {
             using T = decltype(t);
             const T* x = static_cast<const T*>(logits);

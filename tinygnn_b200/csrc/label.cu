@@ -60,16 +60,39 @@ __device__ __forceinline__ void write_row(const LabelArgs& a, int64_t row, bool 
 }
 
 // ── narrow rows ──────────────────────────────────────────────────────────
+template <int LPR>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+    if constexpr (LPR == 32) {
+        return __reduce_max_sync(0xffffffffu, x);
+    } else {
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+        return x;
+    }
+}
+template <int LPR>
+__device__ __forceinline__ int lanes_min(int x) {
+    if constexpr (LPR == 32) {
+        return __reduce_min_sync(0xffffffffu, x);
+    } else {
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) x = min(x, __shfl_xor_sync(0xffffffffu, x, o));
+        return x;
+    }
+}
+
 template <class T, int LPR, int E, bool TOP>
 __global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const LabelArgs a, const T* x, int64_t ldx, int turns) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr float C = FAST ? kLog2e : 1.0f;
     constexpr int RPB = kNarrowThreads / LPR;
     extern __shared__ __align__(16) uint8_t sh[];
+    __shared__ int labels[kNarrowThreads];
     wait_for_previous();
     const int lane = threadIdx.x % LPR, per = RPB * turns;
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
         const int rows = a.rows - r0 < per ? static_cast<int>(a.rows - r0) : per;
+        if (threadIdx.x < rows) labels[threadIdx.x] = class_at(a.labels, r0 + threadIdx.x, a.wide_labels);
         const T* st = stage_in(sh, x, ldx, r0, rows, a.n);
         __syncthreads();
         for (int sub = threadIdx.x / LPR; sub - static_cast<int>(threadIdx.x) / LPR < rows; sub += RPB) {
@@ -85,7 +108,7 @@ __global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const Labe
             const RowResult r = finish_row<FAST>(s);
             const int64_t row = r0 + sub;
             if (lane == 0 && sub < rows) {
-                const int label = class_at(a.labels, row, a.wide_labels);
+                const int label = labels[sub];
                 const bool labelled = label >= 0 && label < a.n;
                 write_row(a, row, labelled, labelled ? to_f32(st[sub * a.n + label]) : 0.0f, r);
             }
@@ -96,34 +119,24 @@ __global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const Labe
                 uint32_t kept = 0;
                 int kept_class = 0;
                 for (int k = 0; k < a.top; ++k) {
+                    // the row's greatest, then the first of its classes
                     uint32_t best = rank[0];
-                    int at = 0;
 #pragma unroll
-                    for (int i = 1; i < E; ++i)
-                        if (rank[i] > best) best = rank[i], at = i;
-                    int j = lane + at * LPR;
-                    if (LPR == 32) {
-                        const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-                        j = __reduce_min_sync(0xffffffffu, best == most ? j : INT_MAX);
-                        best = most;
-                    } else {
+                    for (int i = 1; i < E; ++i) best = max(best, rank[i]);
+                    best = lanes_max<LPR>(best);
+                    int j = INT_MAX;
 #pragma unroll
-                        for (int o = LPR / 2; o > 0; o >>= 1) {
-                            const uint32_t other = __shfl_xor_sync(0xffffffffu, best, o);
-                            const int oj = __shfl_xor_sync(0xffffffffu, j, o);
-                            if (other > best || (other == best && oj < j)) best = other, j = oj;
-                        }
-                    }
-                    if (lane == j % LPR) {
+                    for (int i = E - 1; i >= 0; --i) j = rank[i] == best ? lane + i * LPR : j;
+                    j = lanes_min<LPR>(j);
 #pragma unroll
-                        for (int i = 0; i < E; ++i)
-                            if (i == j / LPR) rank[i] = 0u;
-                    }
+                    for (int i = 0; i < E; ++i) rank[i] = lane + i * LPR == j ? 0u : rank[i];
                     if (lane == k % LPR) kept = best, kept_class = j;
-                    if ((k % LPR == LPR - 1 || k == a.top - 1) && k - k % LPR + lane <= k && sub < rows) {
+                    if (k % LPR == LPR - 1 || k == a.top - 1) {
                         const int64_t o = row * a.top + k - k % LPR + lane;
-                        a.top_log_probs[o] = log_prob(score_of(kept), r);
-                        a.top_classes[o] = kept_class;
+                        if (lane <= k % LPR && sub < rows) {
+                            a.top_log_probs[o] = log_prob(score_of(kept), r);
+                            a.top_classes[o] = kept_class;
+                        }
                     }
                 }
             }
@@ -226,9 +239,13 @@ __device__ __forceinline__ void part_top(TopShared<NT>& sh, const Part<T>& p, ui
             if (mine)
                 for (int v = p.v0 + tid; v < p.v1; v += 32) look_at(v);
         } else {
-            // A warp for each of those threads' vectors.
-            for (int i = warp; i < sh.n_threads; i += NT / 32)
-                for (int v = p.v0 + sh.threads[i] + lane * NT; v < p.v1; v += 32 * NT) look_at(v);
+            // Those threads' vectors, dealt out to all.
+            const int each = (p.v1 - p.v0 + NT - 1) / NT;
+            const int64_t items = static_cast<int64_t>(sh.n_threads) * each;
+            for (int64_t i = tid; i < items; i += NT) {
+                const int t = static_cast<int>(i / each), v = p.v0 + sh.threads[t] + static_cast<int>(i - int64_t(t) * each) * NT;
+                if (v < p.v1) look_at(v);
+            }
         }
         Team::sync();
         above = sh.n_above;
@@ -436,14 +453,16 @@ __global__ void __launch_bounds__(kNarrowThreads) label_grad_narrow_kernel(const
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int RPB = kNarrowThreads / LPR;
     extern __shared__ __align__(16) uint8_t sh[];
+    __shared__ RowGrad grads[kNarrowThreads];
     wait_for_previous();
     const int lane = threadIdx.x % LPR, per = RPB * turns;
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < g.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
         const int rows = g.rows - r0 < per ? static_cast<int>(g.rows - r0) : per;
+        if (threadIdx.x < rows) grads[threadIdx.x] = row_grad<FAST>(g, r0 + threadIdx.x);
         T* st = stage_in(sh, x, ldx, r0, rows, g.n);
         __syncthreads();
         for (int sub = threadIdx.x / LPR; sub < rows; sub += RPB) {
-            const RowGrad r = row_grad<FAST>(g, r0 + sub);
+            const RowGrad r = grads[sub];
             T* p = st + sub * g.n;
 #pragma unroll
             for (int i = 0; i < E; ++i) {

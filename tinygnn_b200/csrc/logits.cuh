@@ -470,14 +470,16 @@ template <class F>
 void by_narrow(int64_t n, F&& f) {
     using std::integral_constant;
     if (n <= 16) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    else if (n <= 48) f(integral_constant<int, 8>{}, integral_constant<int, 6>{});
     else if (n <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
     else if (n <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     else f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
 }
-// How often RPB rows of n classes, taken together, make up about 16 KB.
+// How often RPB rows of n classes, taken together, make up about 16 KB; at most
+// as many rows as threads.
 inline int narrow_turns(int rpb, int64_t n, size_t size, int64_t rows) {
-    const int64_t fit = std::max<int64_t>(1, 16384 / (rpb * n * static_cast<int64_t>(size)));
-    return static_cast<int>(std::max<int64_t>(1, std::min({fit, int64_t(8), ceil_div(rows, int64_t(rpb) * num_sms() * 4)})));
+    const int64_t fit = std::min<int64_t>(16384 / (rpb * n * static_cast<int64_t>(size)), kNarrowThreads / rpb);
+    return static_cast<int>(std::max<int64_t>(1, std::min(fit, ceil_div(rows, int64_t(rpb) * num_sms() * 4))));
 }
 
 // An integer of 4 or 8 bytes; what does not fit an int is none (-1).
