@@ -260,27 +260,35 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
     constexpr int RPB = kNarrowThreads / LPR;
     extern __shared__ __align__(16) uint8_t sh[];
     wait_for_previous();
-    const int lane = threadIdx.x % LPR, place = threadIdx.x / LPR, per = RPB * turns;
-    const Teacher t = Teacher::in(reinterpret_cast<float*>(sh + stage) + place * Teacher::floats(a.k), a.k);
+    const int lane = threadIdx.x % LPR, place = threadIdx.x / LPR, per = RPB * turns, room = Teacher::floats(a.k);
+    float* teachers = reinterpret_cast<float*>(sh + stage);  // of all rows
     const float c = FAST ? __fmul_rn(kLog2e, a.inverse) : a.inverse;
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
         const int rows = a.rows - r0 < per ? static_cast<int>(a.rows - r0) : per;
+        for (int i = threadIdx.x; i < rows * a.k; i += kNarrowThreads) {
+            const int r = i / a.k, e = i - r * a.k;
+            const int j = class_at(a.classes, (r0 + r) * a.ldc + e, a.wide_classes);
+            const float v = to_f32(static_cast<const U*>(a.teacher)[(r0 + r) * a.ldt + e]);
+            const Teacher t = Teacher::in(teachers + r * room, a.k);
+            const bool in = j >= 0 && j < a.n && v != -INFINITY;
+            t.c[e] = in ? j : -1;
+            t.q[e] = in ? v : -INFINITY;
+        }
+        if (threadIdx.x < rows) *Teacher::in(teachers + threadIdx.x * room, a.k).scale = a.weights ? a.weights[r0 + threadIdx.x] : 1.0f;
         T* st = stage_in(sh, x, ldx, r0, rows, a.n);
         __syncthreads();
         for (int first = 0; first < rows; first += RPB) {
-            // (lanes without a row compute the first one's, and write nothing)
+            // (lanes without a row compute the first one's, without a teacher, and write nothing)
             const bool here = first + place < rows;
             const int sub = here ? first + place : first;
             const int64_t row = r0 + sub;
             T* p = st + sub * a.n;
-            for (int i = lane; i < a.k; i += LPR) {
-                const int j = class_at(a.classes, row * a.ldc + i, a.wide_classes);
-                const bool in = j >= 0 && j < a.n;
-                const float v = in ? to_f32(static_cast<const U*>(a.teacher)[row * a.ldt + i]) : -INFINITY;
-                t.z[i] = in ? to_f32(p[j]) : 0.0f;
-                t.c[i] = v == -INFINITY ? -1 : j;
-                t.q[i] = v;
+            const Teacher t = Teacher::in(teachers + (here ? sub : rows + place) * room, a.k);
+            if (!here) {
+                for (int i = lane; i < a.k; i += LPR) t.c[i] = -1, t.q[i] = -INFINITY;
+                if (lane == 0) *t.scale = 0.0f;
             }
+            for (int i = lane; i < a.k; i += LPR) t.z[i] = t.c[i] >= 0 ? to_f32(p[t.c[i]]) : 0.0f;
             float z[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) {
@@ -288,7 +296,7 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
                 z[i] = j < a.n ? to_f32(p[j]) : -INFINITY;
             }
             __syncwarp();  // (before the row's first lanes write over its scores)
-            float loss = finish_teacher<LPR>(a, lane, t, a.weights ? a.weights[row] : 1.0f);
+            float loss = finish_teacher<LPR>(a, lane, t, *t.scale);
             Soft s;
             add_scores<FAST, false>(s, z, c);
             lanes_soft<FAST, false, LPR>(s, c);
@@ -504,9 +512,10 @@ void distill(const DistillArgs& a, const T* x, int64_t ldx, T* dx, int64_t lddx,
         by_narrow(a.n, [&](auto lpr, auto e) {
             constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = kNarrowThreads / LPR;
             auto kern = dx ? distill_narrow_kernel<T, U, LPR, E, true> : distill_narrow_kernel<T, U, LPR, E, false>;
-            const int turns = narrow_turns(RPB, a.n, sizeof(T), a.rows);
+            const int turns = narrow_turns(RPB, a.n + Teacher::floats(a.k) * 4 / static_cast<int>(sizeof(T)), sizeof(T), a.rows);
             const int stage = static_cast<int>((RPB * turns * a.n * sizeof(T) + 32 + 15) / 16 * 16);
-            const size_t bytes = stage + RPB * Teacher::floats(a.k) * sizeof(float);
+            // (and a teacher for each of a turn's lanes that may have no row)
+            const size_t bytes = stage + (RPB * turns + RPB) * Teacher::floats(a.k) * sizeof(float);
             if (bytes > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
             launch_dependent("distill_loss", kern,
                              dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(a.rows, RPB * turns), num_sms() * 8))),

@@ -391,22 +391,30 @@ __global__ void __launch_bounds__(kMaxThreads, kApply<SPLIT>) group_apply_kernel
     });
 }
 
-// Adds f(column)'s pairs over the columns of each group; put(group, sum) by one
-// thread of the warp that adds them.
+// Adds f(column, group)'s pairs over the columns of each group with the lanes
+// that suit a group's width; put(group, sum, lanes, lane) by all of them.
+template <int LANES, class F, class G>
+__device__ __forceinline__ void over_groups_by(const GroupArgs& a, F&& f, G&& put) {
+    const int lane = threadIdx.x % LANES, step = blockDim.x / LANES, first = threadIdx.x / LANES;
+    // (all lanes of a warp go round as often)
+    for (int i = first; i - first < a.groups; i += step) {
+        float2 s = make_float2(0.0f, 0.0f);
+        if (i < a.groups)
+            for (int c = i * a.per + lane; c < (i + 1) * a.per; c += LANES) {
+                const float2 v = f(c, i);
+                s.x = __fadd_rn(s.x, v.x);
+                s.y = __fadd_rn(s.y, v.y);
+            }
+        s.x = reduce_sum<float, LANES>(s.x);
+        s.y = reduce_sum<float, LANES>(s.y);
+        put(i, s, std::integral_constant<int, LANES>{}, lane);
+    }
+}
 template <class F, class G>
 __device__ __forceinline__ void over_groups(const GroupArgs& a, F&& f, G&& put) {
-    const int lane = threadIdx.x & 31;
-    for (int i = threadIdx.x >> 5; i < a.groups; i += blockDim.x >> 5) {
-        float2 s = make_float2(0.0f, 0.0f);
-        for (int c = i * a.per + lane; c < (i + 1) * a.per; c += 32) {
-            const float2 v = f(c, i);
-            s.x = __fadd_rn(s.x, v.x);
-            s.y = __fadd_rn(s.y, v.y);
-        }
-        s.x = reduce_sum<float, 32>(s.x);
-        s.y = reduce_sum<float, 32>(s.y);
-        put(i, s, lane == 0);
-    }
+    if (a.per <= 4) over_groups_by<1>(a, f, put);
+    else if (a.per <= 32) over_groups_by<8>(a, f, put);
+    else over_groups_by<32>(a, f, put);
 }
 
 constexpr int kSmallCols = 2048;  // most columns of a block that has whole graphs
@@ -436,16 +444,19 @@ __global__ void __launch_bounds__(kMaxThreads, 2) group_small_kernel(const Group
         const float rows = static_cast<float>(e - b), per = static_cast<float>(a.per);
         over_groups(
             a, [&](int c, int i) { return make_float2(__fsub_rn(columns[c].x, columns[i * a.per].x), 0.0f); },
-            [&](int i, float2 s, bool first) {
-                const float mean = __fadd_rn(columns[i * a.per].x, __fdiv_rn(s.x, per));
+            [&](int i, float2 s, auto lanes, int lane) {
+                constexpr int LANES = decltype(lanes)::value;
+                const bool here = i < a.groups;
+                const float mean = here ? __fadd_rn(columns[i * a.per].x, __fdiv_rn(s.x, per)) : 0.0f;
                 float d = 0.0f;
-                for (int c = i * a.per + (threadIdx.x & 31); c < (i + 1) * a.per; c += 32) {
-                    const float z = __fsub_rn(columns[c].x, mean);
-                    d = __fadd_rn(d, fmaf(__fmul_rn(z, z), rows, columns[c].y));
-                }
-                d = reduce_sum<float, 32>(d);
+                if (here)
+                    for (int c = i * a.per + lane; c < (i + 1) * a.per; c += LANES) {
+                        const float z = __fsub_rn(columns[c].x, mean);
+                        d = __fadd_rn(d, fmaf(__fmul_rn(z, z), rows, columns[c].y));
+                    }
+                d = reduce_sum<float, LANES>(d);
                 const float2 r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(d, __fmul_rn(rows, per)), a.eps)));
-                if (first) mine[i] = out[i] = r;
+                if (here && lane == 0) mine[i] = out[i] = r;
             });
         __syncthreads();
         apply_part<SPLIT>(a, p, x, ldx, k, mine, y, ldy, b, e);
@@ -668,8 +679,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) group_grad_small_kernel(const 
         const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
         over_groups(
             a, [&](int c, int) { return columns[c]; },
-            [&](int i, float2 s, bool first) {
-                if (first) means[i] = make_float2(__fdiv_rn(s.x, all), __fdiv_rn(s.y, all));
+            [&](int i, float2 s, auto, int lane) {
+                if (i < a.groups && lane == 0) means[i] = make_float2(__fdiv_rn(s.x, all), __fdiv_rn(s.y, all));
             });
         __syncthreads();
         grad_part<SPLIT>(a, p, dy, lddy, x, ldx, k, st, means, dx, lddx, b, e);
@@ -716,8 +727,9 @@ bool small_graphs(const GroupArgs& a, size_t size) {
     const int64_t bytes = a.rows * a.cols * static_cast<int64_t>(size);
     return a.nv <= kMaxThreads && a.cols <= kSmallCols && bytes <= 16 << 20 && bytes / a.graphs <= 32 << 10;
 }
-// The cut of such graphs: eight rows a lane.
+// The cut of such graphs: eight rows a lane, where there are blocks enough.
 GroupArgs cut_small(GroupArgs a) {
+    if (a.graphs < 4 * num_sms()) return a;
     const int64_t lanes = std::max<int64_t>(ceil_div(ceil_div(a.rows, a.graphs), 8), 1);
     a.ty = static_cast<int>(std::min<int64_t>(a.ty, std::max<int64_t>(lanes, ceil_div(32, a.tx))));
     return a;

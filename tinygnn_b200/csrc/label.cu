@@ -59,6 +59,31 @@ __device__ __forceinline__ void write_row(const LabelArgs& a, int64_t row, bool 
     a.stats[row] = make_float2(r.m, r.log_s);
 }
 
+// A score and its class as one number: greater for a greater score, and among
+// equal scores for a lower class.  0: none.
+__device__ __forceinline__ uint64_t entry(uint32_t rank, int column) {
+    return static_cast<uint64_t>(rank) << 32 | (0xffffffffu - static_cast<uint32_t>(column));
+}
+__device__ __forceinline__ uint32_t entry_rank(uint64_t e) { return static_cast<uint32_t>(e >> 32); }
+__device__ __forceinline__ int entry_column(uint64_t e) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(e)); }
+
+// How many of the first n entries are greater than e.
+__device__ __forceinline__ int place_of(const uint64_t* entries, int n, uint64_t e) {
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) place += entries[j] > e;
+    return place;
+}
+
+// The lowest bits that the ranks of a type's scores share: zeros, ones for
+// negative scores.
+template <class T>
+constexpr int kLow = sizeof(T) == 4 ? 0 : (std::is_same<T, __half>::value ? 13 : 16);
+template <class T>
+__device__ __forceinline__ uint32_t with_low_bits(uint32_t bound) {
+    return bound >> 31 == 0 ? bound | ((1u << kLow<T>) - 1) : bound;
+}
+
 // ── narrow rows ──────────────────────────────────────────────────────────
 template <int LPR>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
@@ -81,13 +106,50 @@ __device__ __forceinline__ int lanes_min(int x) {
     }
 }
 
-template <class T, int LPR, int E, bool TOP>
+// The row's k best of a warp's E ranks a lane (0: none), class lane + 32 i, into
+// list: the k-th greatest rank bit by bit, the ranks above it, and of those
+// equal to it the first.
+template <class T, int E>
+__device__ __forceinline__ void warp_top(const uint32_t (&rank)[E], int k, uint64_t* list) {
+    const int lane = threadIdx.x & 31;
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= kLow<T>; --bit) {
+        const uint32_t next = bound | 1u << bit;
+        int reached = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) reached += rank[i] >= next;
+        reached = __reduce_add_sync(0xffffffffu, reached);
+        if (reached >= k) bound = next;
+        if (reached == k) break;
+    }
+    bound = with_low_bits<T>(bound);
+    int taken = 0;
+    const auto take = [&](int i, bool x) {
+        const uint32_t m = __ballot_sync(0xffffffffu, x);
+        const int at = taken + __popc(m & ((1u << lane) - 1));
+        if (x && at < k) list[at] = entry(rank[i], lane + i * 32);
+        taken += __popc(m);
+    };
+#pragma unroll
+    for (int i = 0; i < E; ++i) take(i, rank[i] > bound);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (taken < k) take(i, rank[i] == bound);
+    __syncwarp();
+}
+
+// How a row's best classes are found: one after the other (a few), or by the
+// rank of the last (warp_top).  207,595 x 80 bf16, 20 classes: SELECT_FIGURES
+enum Top { kNone, kRounds, kSelect };
+
+template <class T, int LPR, int E, Top TOP>
 __global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const LabelArgs a, const T* x, int64_t ldx, int turns) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr float C = FAST ? kLog2e : 1.0f;
     constexpr int RPB = kNarrowThreads / LPR;
     extern __shared__ __align__(16) uint8_t sh[];
     __shared__ int labels[kNarrowThreads];
+    __shared__ uint64_t lists[TOP == kSelect ? RPB : 1][TOP == kSelect ? kMaxTop : 1];
     wait_for_previous();
     const int lane = threadIdx.x % LPR, per = RPB * turns;
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * per) {
@@ -112,10 +174,22 @@ __global__ void __launch_bounds__(kNarrowThreads) label_narrow_kernel(const Labe
                 const bool labelled = label >= 0 && label < a.n;
                 write_row(a, row, labelled, labelled ? to_f32(st[sub * a.n + label]) : 0.0f, r);
             }
-            if constexpr (TOP) {
+            if constexpr (TOP != kNone) {
                 uint32_t rank[E];
 #pragma unroll
                 for (int i = 0; i < E; ++i) rank[i] = lane + i * LPR < a.n ? rank_of(z[i]) : 0u;
+                if constexpr (TOP == kSelect) {
+                    uint64_t* list = lists[threadIdx.x / LPR];
+                    warp_top<T>(rank, a.top, list);
+                    for (int i = lane; i < a.top && sub < rows; i += 32) {
+                        const uint64_t e = list[i];
+                        const int64_t o = row * a.top + place_of(list, a.top, e);
+                        a.top_log_probs[o] = log_prob(score_of(entry_rank(e)), r);
+                        a.top_classes[o] = entry_column(e);
+                    }
+                    __syncwarp();
+                    continue;
+                }
                 uint32_t kept = 0;
                 int kept_class = 0;
                 for (int k = 0; k < a.top; ++k) {
@@ -152,14 +226,6 @@ constexpr int kCandidates = NT == 32 ? 256 : 512;
 template <int NT>
 constexpr int kEquals = NT == 32 ? 64 : 256;
 
-// A score and its class as one number: greater for a greater score, and among
-// equal scores for a lower class.  0: none.
-__device__ __forceinline__ uint64_t entry(uint32_t rank, int column) {
-    return static_cast<uint64_t>(rank) << 32 | (0xffffffffu - static_cast<uint32_t>(column));
-}
-__device__ __forceinline__ uint32_t entry_rank(uint64_t e) { return static_cast<uint32_t>(e >> 32); }
-__device__ __forceinline__ int entry_column(uint64_t e) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(e)); }
-
 template <int NT>
 struct TopShared {
     uint64_t best[kMaxTop];  // this CTA's best, in order
@@ -170,14 +236,6 @@ struct TopShared {
     int sums[NT / 32];
     uint32_t bound;
 };
-
-// How many of the first n entries are greater than e.
-__device__ __forceinline__ int place_of(const uint64_t* entries, int n, uint64_t e) {
-    int place = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) place += entries[j] > e;
-    return place;
-}
 
 // The `k` best scores of the part into sh.best, 0 where it has fewer.  `most`:
 // the rank of this thread's greatest score among its vectors (0 without one).
@@ -191,15 +249,13 @@ __device__ __forceinline__ void part_top(TopShared<NT>& sh, const Part<T>& p, ui
     // reach will do).
     uint32_t bound = 0;
     if (Team::count(most != 0) >= k) {
-        // (the lowest bits of a 16-bit type's scores are alike)
-        constexpr int kLow = sizeof(T) == 4 ? 0 : (std::is_same<T, __half>::value ? 13 : 16);
-        for (int bit = 31; bit >= kLow; --bit) {
+        for (int bit = 31; bit >= kLow<T>; --bit) {
             const uint32_t next = bound | 1u << bit;
             const int reached = Team::count(most >= next);
             if (reached >= k) bound = next;
             if (reached >= k && reached <= k + NT / 16) break;
         }
-        if (bound >> 31 == 0) bound |= (1u << kLow) - 1;  // (of negative scores' ranks they are ones)
+        bound = with_low_bits<T>(bound);
     }
     int above;
     for (;;) {
@@ -558,15 +614,28 @@ TG_API tg_status tg_label_log_probs(int64_t rows, int64_t classes, int32_t dtype
         by_dtype(dtype, [&](auto t) {
             using T = decltype(t);
             const T* x = static_cast<const T*>(logits);
+            const auto narrow = [&](auto lpr, auto e, auto top_by) {
+                constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = logits::kNarrowThreads / LPR;
+                const int turns = logits::narrow_turns(RPB, classes, sizeof(T), rows);
+                launch_dependent("label_log_probs", label_narrow_kernel<T, LPR, E, decltype(top_by)::value>,
+                                 dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB * turns), num_sms() * 8))),
+                                 dim3(logits::kNarrowThreads), staged_bytes(RPB * turns, classes, sizeof(T)), s, a, x, ldz, turns);
+            };
+            using std::integral_constant;
+            if (top > 0 && (top > 6 || classes > logits::kNarrow) && classes <= 1024) {
+                const integral_constant<Top, kSelect> select;
+                const integral_constant<int, 32> lanes;
+                if (classes <= 64) narrow(lanes, integral_constant<int, 2>{}, select);
+                else if (classes <= 128) narrow(lanes, integral_constant<int, 4>{}, select);
+                else if (classes <= 256) narrow(lanes, integral_constant<int, 8>{}, select);
+                else if (classes <= 512) narrow(lanes, integral_constant<int, 16>{}, select);
+                else narrow(lanes, integral_constant<int, 32>{}, select);
+                return;
+            }
             if (classes <= logits::kNarrow) {
                 logits::by_narrow(classes, [&](auto lpr, auto e) {
-                    constexpr int LPR = decltype(lpr)::value, E = decltype(e)::value, RPB = logits::kNarrowThreads / LPR;
-                    auto kern = top ? label_narrow_kernel<T, LPR, E, true> : label_narrow_kernel<T, LPR, E, false>;
-                    const int turns = logits::narrow_turns(RPB, classes, sizeof(T), rows);
-                    launch_dependent("label_log_probs", kern,
-                                     dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(rows, RPB * turns), num_sms() * 8))),
-                                     dim3(logits::kNarrowThreads), staged_bytes(RPB * turns, classes, sizeof(T)), s, a, x, ldz,
-                                     turns);
+                    if (top) narrow(lpr, e, integral_constant<Top, kRounds>{});
+                    else narrow(lpr, e, integral_constant<Top, kNone>{});
                 });
                 return;
             }
@@ -580,8 +649,8 @@ TG_API tg_status tg_label_log_probs(int64_t rows, int64_t classes, int32_t dtype
                                     std::min(1024 / (NT * TEAMS), logits::kSharedSm / (room + fixed + 1024)), NT * TEAMS, room, s, a,
                                     x, ldz);
             };
-            using std::integral_constant;
-            if (classes <= logits::kWarp && rows > num_sms()) go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+            // (a warp's 32 maxima bound few best classes well)
+            if (classes <= logits::kWarp && rows > num_sms() && top <= 16) go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
             else if (classes / ranks <= 8192) go(integral_constant<int, 128>{}, integral_constant<int, 1>{});
             else go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
         });
