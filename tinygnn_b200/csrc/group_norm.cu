@@ -16,8 +16,8 @@
 //  it; chunk c's part of graph g is slot c + g, which no other part has, and there
 //  are at most chunks + graphs of them.  A second, small kernel joins a graph's
 //  slots in their order (no atomics, the same bits every run), and a third applies
-//  the statistics.  Many small graphs are a block's each instead, in one kernel
-//  (and one more that joins dgamma and dbeta): see small_graphs below.
+//  the statistics.  Where graphs are small (small_graphs below) each is a block's
+//  instead, in one kernel, and the three have the larger ones alone.
 //
 //  A part's mean and sum of squared deviations come from one pass: each thread
 //  sums x - k and (x - k)^2 with k its first value of the column, which cannot
@@ -45,6 +45,9 @@ struct GroupArgs {
     int act;
     float alpha, eps;
     // the cut
+    int least;               // graphs of at most as many rows are a block's (0: none are)
+    int* large;              // of the `blocks` blocks that have whole graphs: whether one met a larger graph (with least)
+    int blocks;
     int R, chunks;           // rows of a chunk, number of chunks
     int nv, tx, ty;          // vectors of a row, of a block; row lanes of a block
 };
@@ -72,17 +75,40 @@ __device__ __forceinline__ int graph_at(const GroupArgs& a, int r) {
     }
     return lo;
 }
-// Calls f(g, first row, end) for the graphs' parts of chunk c.
+// Whether all graphs are a block's, so that the chunks' kernels have nothing to do.
+__device__ __forceinline__ bool none_large(const GroupArgs& a) {
+    if (a.least == 0) return false;
+    int any = 0;
+    for (int i = threadIdx.x; i < a.blocks; i += blockDim.x) any |= a.large[i];
+    return !__syncthreads_or(any);
+}
+// The first graph from g on that the chunks' kernels have; one that begins at
+// row `end` or later (or a.graphs) where there is none before that row.
+__device__ __forceinline__ int next_graph(const GroupArgs& a, int g, int64_t end) {
+    if (a.least == 0) return g;
+    for (const int lane = threadIdx.x & 31;; g += 32) {
+        const int i = g + lane;
+        const uint32_t m = __ballot_sync(0xffffffffu, i >= a.graphs || begin_of(a, i) >= end || end_of(a, i) - begin_of(a, i) > a.least);
+        if (m) return g + __ffs(m) - 1;
+    }
+}
+// Calls f(g, first row, end, slot) for the graphs' parts of chunk c.  With a.least a
+// chunk has no whole graph (R <= least), so at most two parts: slots 2 c, and
+// 2 c + 1 for the graph that begins in it.
 template <class F>
 __device__ __forceinline__ void for_parts(const GroupArgs& a, int c, F&& f) {
     const int64_t c0 = static_cast<int64_t>(c) * a.R, c1 = c0 + a.R < a.rows ? c0 + a.R : a.rows;
-    for (int g = graph_at(a, static_cast<int>(c0)); g < a.graphs; ++g) {
+    for (int g = next_graph(a, graph_at(a, static_cast<int>(c0)), c1); g < a.graphs; g = next_graph(a, g + 1, c1)) {
         const int b = begin_of(a, g), e = end_of(a, g);
         if (b >= c1) break;
         const int lo = b > c0 ? b : static_cast<int>(c0), hi = e < c1 ? e : static_cast<int>(c1);
-        if (lo < hi) f(g, lo, hi);
+        if (lo < hi) f(g, lo, hi, a.least ? 2 * static_cast<int64_t>(c) + (b >= c0) : static_cast<int64_t>(c) + g);
         if (e >= c1) break;
     }
+}
+// Slot of the i-th part of graph g, whose first is in chunk `first`.
+__device__ __forceinline__ int64_t slot_of(const GroupArgs& a, int g, int first, int i) {
+    return a.least ? 2 * static_cast<int64_t>(first + i) + (i == 0) : static_cast<int64_t>(first + i) + g;
 }
 
 constexpr int kMaxThreads = 256;
@@ -93,6 +119,8 @@ constexpr int kApply = SPLIT ? 2 : 3;
 constexpr int kJoinThreads = 1024;  // that join a graph's group of many parts
 template <int W>
 constexpr int kJoinBlock = W == 32 ? 256 : W;
+// Blocks that share the groups of a large graph among small ones.
+__host__ __device__ constexpr int large_blocks(int groups) { return groups < 4 ? groups : 4; }
 
 // A thread's place: V columns from `col` on, of which `n` are there (ALIGNED: all
 // or none), in the rows ty, ty + a.ty, ... of a part.
@@ -266,13 +294,14 @@ __global__ void __launch_bounds__(kMaxThreads, kParts) group_parts_kernel(const 
     extern __shared__ float2 room[];
     const Sums<T> sh{room};
     wait_for_previous();
+    if (none_large(a)) return;
     const Place<T, ALIGNED> p(a);
     const int c = blockIdx.x;
-    for_parts(a, c, [&](int g, int lo, int hi) {
+    for_parts(a, c, [&](int g, int lo, int hi, int64_t slot) {
         part_sums<4>(a, p, x, ldx, lo, hi, sh);
         __syncthreads();
         for_columns<T>(a, [&](int i, int column) {
-            part[static_cast<int64_t>(c + g) * a.cols + column] = join_lanes(a, sh, i, hi - lo);
+            part[slot * a.cols + column] = join_lanes(a, sh, i, hi - lo);
         });
         __syncthreads();
     });
@@ -291,7 +320,7 @@ __device__ __forceinline__ void for_slots(const GroupArgs& a, int g, int b, int 
         for (int i = t / wide; i < slots; i += step) {
             // (a slot's rows; the last chunk's end may pass 2^31)
             const int r0 = (first + i) * a.R, r1 = e - r0 < a.R ? e : r0 + a.R;
-            f(part[static_cast<int64_t>(first + i + g) * a.cols + c0 + col], r1 - (b > r0 ? b : r0), c0 + col);
+            f(part[slot_of(a, g, first, i) * a.cols + c0 + col], r1 - (b > r0 ? b : r0), c0 + col);
         }
 }
 // The sum over W threads (a warp, or the block).
@@ -307,34 +336,51 @@ __device__ __forceinline__ float sum_of(float v, float* sh) {
     return v;
 }
 
+// Calls f(g, group) for the graphs' groups that W threads join: one, blockIdx.x's
+// W-th part's; of large graphs among small ones those of the graph that begins in
+// chunk blockIdx.x.
+template <int W, class F>
+__device__ __forceinline__ void for_sets(const GroupArgs& a, int block, F&& f) {
+    if (a.least == 0) {
+        const int64_t i = static_cast<int64_t>(block) * (kJoinBlock<W> / W) + threadIdx.x / W;
+        if (i < static_cast<int64_t>(a.graphs) * a.groups) f(static_cast<int>(i / a.groups), static_cast<int>(i % a.groups));
+        return;
+    }
+    const int share = large_blocks(a.groups);
+    for_parts(a, block / share, [&](int g, int, int, int64_t slot) {
+        if (slot % 2)
+            for (int i = block % share; i < a.groups; i += share) f(g, i);
+    });
+}
+
 // stats[g * groups + group] = (mean, rstd), (0, 0) for a graph without rows.
 template <int W>
 __global__ void __launch_bounds__(kJoinBlock<W>) group_stats_kernel(const GroupArgs a, const float2* part, float2* stats) {
     __shared__ float sh[32];
     wait_for_previous();
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinBlock<W> / W) + threadIdx.x / W;
-    if (i >= static_cast<int64_t>(a.graphs) * a.groups) return;
-    const int g = static_cast<int>(i / a.groups), c0 = static_cast<int>(i % a.groups) * a.per;
-    const int b = begin_of(a, g), e = end_of(a, g);
-    float2 r = make_float2(0.0f, 0.0f);
-    if (b < e) {
-        const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
-        // The parts' means m about the first part's, k: as in a part, the sum of
-        // n (m - k)^2 less that of their mean cannot lose the deviations.
-        const float k = part[static_cast<int64_t>(b / a.R + g) * a.cols + c0].x;
-        float s = 0.0f, d = 0.0f;
-        for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) {
-            const float z = __fsub_rn(p.x, k), w = __fmul_rn(z, static_cast<float>(n));
-            s = __fadd_rn(s, w);
-            d = __fadd_rn(d, fmaf(z, w, p.y));
-        });
-        s = sum_of<W>(s, sh);
-        d = sum_of<W>(d, sh);
-        const float shift = __fdiv_rn(s, all), mean = __fadd_rn(k, shift);
-        d = max_nan(fmaf(-s, shift, d), 0.0f);
-        r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(d, all), a.eps)));
-    }
-    if (threadIdx.x % W == 0) stats[i] = r;
+    if (none_large(a)) return;
+    for_sets<W>(a, blockIdx.x, [&](int g, int group) {
+        const int c0 = group * a.per, b = begin_of(a, g), e = end_of(a, g);
+        float2 r = make_float2(0.0f, 0.0f);
+        if (b < e) {
+            const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
+            // The parts' means m about the first part's, k: as in a part, the sum of
+            // n (m - k)^2 less that of their mean cannot lose the deviations.
+            const float k = part[slot_of(a, g, b / a.R, 0) * a.cols + c0].x;
+            float s = 0.0f, d = 0.0f;
+            for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) {
+                const float z = __fsub_rn(p.x, k), w = __fmul_rn(z, static_cast<float>(n));
+                s = __fadd_rn(s, w);
+                d = __fadd_rn(d, fmaf(z, w, p.y));
+            });
+            s = sum_of<W>(s, sh);
+            d = sum_of<W>(d, sh);
+            const float shift = __fdiv_rn(s, all), mean = __fadd_rn(k, shift);
+            d = max_nan(fmaf(-s, shift, d), 0.0f);
+            r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(d, all), a.eps)));
+        }
+        if (threadIdx.x % W == 0) stats[static_cast<int64_t>(g) * a.groups + group] = r;
+    });
 }
 
 // Each of V columns' (first, second) of its group: one pair where the V columns
@@ -383,9 +429,10 @@ template <class T, class P, bool ALIGNED, bool SPLIT>
 __global__ void __launch_bounds__(kMaxThreads, kApply<SPLIT>) group_apply_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
                                                                   const P* beta, const float2* stats, T* y, int64_t ldy) {
     wait_for_previous();
+    if (none_large(a)) return;
     const Place<T, ALIGNED> p(a);
     const int c = blockIdx.x;
-    for_parts(a, c, [&](int g, int lo, int hi) {
+    for_parts(a, c, [&](int g, int lo, int hi, int64_t slot) {
         const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
         apply_part<SPLIT>(a, p, x, ldx, k, stats + static_cast<int64_t>(g) * a.groups, y, ldy, lo, hi);
     });
@@ -419,7 +466,8 @@ __device__ __forceinline__ void over_groups(const GroupArgs& a, F&& f, G&& put) 
 
 constexpr int kSmallCols = 2048;  // most columns of a block that has whole graphs
 
-// A block for each graph: its second reading of x comes from L1 or L2.
+// A block for each graph of at most a.least rows: its second reading of x comes
+// from L1 or L2.
 template <class T, class P, bool ALIGNED, bool SPLIT>
 __global__ void __launch_bounds__(kMaxThreads, 2) group_small_kernel(const GroupArgs a, const T* x, int64_t ldx, const P* gamma,
                                                                   const P* beta, float2* stats, T* y, int64_t ldy) {
@@ -429,8 +477,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) group_small_kernel(const Group
     wait_for_previous();
     const Place<T, ALIGNED> p(a);
     const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
+    int large = 0;
     for (int g = blockIdx.x; g < a.graphs; g += gridDim.x) {
         const int b = begin_of(a, g), e = end_of(a, g);
+        if (e - b > a.least) {
+            large = 1;
+            continue;
+        }
         float2* out = stats + static_cast<int64_t>(g) * a.groups;
         if (b >= e) {
             for (int i = threadIdx.x; i < a.groups; i += blockDim.x) out[i] = make_float2(0.0f, 0.0f);
@@ -461,6 +514,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) group_small_kernel(const Group
         __syncthreads();
         apply_part<SPLIT>(a, p, x, ldx, k, mine, y, ldy, b, e);
     }
+    if (threadIdx.x == 0) a.large[blockIdx.x] = large;
 }
 
 // ── backward ─────────────────────────────────────────────────────────────
@@ -551,16 +605,17 @@ __global__ void __launch_bounds__(kMaxThreads, kGrad) group_grad_parts_kernel(co
     const Sums<T> sh{room};
     float2* total = room + Sums<T>::pairs(blockDim.x);  // of the block's columns
     wait_for_previous();
+    if (none_large(a)) return;  // (nor are this block's sums read)
     const Place<T, ALIGNED> p(a);
     for (int i = threadIdx.x; i < a.tx * Sums<T>::V; i += blockDim.x) total[i] = make_float2(0.0f, 0.0f);
     const int c = blockIdx.x;
-    for_parts(a, c, [&](int g, int lo, int hi) {
+    for_parts(a, c, [&](int g, int lo, int hi, int64_t slot) {
         const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
         grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, k, stats + static_cast<int64_t>(g) * a.groups, lo, hi, sh);
         __syncthreads();
         for_columns<T>(a, [&](int i, int column) {
             const float2 s = add_lanes(a, sh, i);
-            part[static_cast<int64_t>(c + g) * a.cols + column] = s;
+            part[slot * a.cols + column] = s;
             total[i] = make_float2(__fadd_rn(total[i].x, s.x), __fadd_rn(total[i].y, s.y));
         });
         __syncthreads();
@@ -606,25 +661,27 @@ __global__ void __launch_bounds__(kJoinBlock<W>) group_grad_join_kernel(const Gr
                                                                       P* dgamma, P* dbeta) {
     __shared__ float sh[kJoinBlock<W> / 32 * kJoinColumns];
     wait_for_previous();
+    const bool none = none_large(a);
     if (static_cast<int>(blockIdx.x) >= blocks) {
-        join_params(a, static_cast<int>(blockIdx.x) - blocks, sums, sum_rows, dgamma, dbeta, sh);
+        join_params(a, static_cast<int>(blockIdx.x) - blocks, sums, none ? a.blocks : sum_rows, dgamma, dbeta, sh);
         return;
     }
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinBlock<W> / W) + threadIdx.x / W;
-    if (i >= static_cast<int64_t>(a.graphs) * a.groups) return;
-    const int g = static_cast<int>(i / a.groups), c0 = static_cast<int>(i % a.groups) * a.per;
-    const int b = begin_of(a, g), e = end_of(a, g);
-    if (b >= e) return;
-    float s = 0.0f, t = 0.0f;
-    for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int, int column) {
-        const float w = to_f32(gamma[column]);
-        s = fmaf(w, p.x, s);
-        t = fmaf(w, p.y, t);
+    if (none) return;
+    for_sets<W>(a, blockIdx.x, [&](int g, int group) {
+        const int b = begin_of(a, g), e = end_of(a, g);
+        if (b >= e) return;
+        float s = 0.0f, t = 0.0f;
+        for_slots<W>(a, g, b, e, group * a.per, part, [&](float2 p, int, int column) {
+            const float w = to_f32(gamma[column]);
+            s = fmaf(w, p.x, s);
+            t = fmaf(w, p.y, t);
+        });
+        s = sum_of<W>(s, sh);
+        t = sum_of<W>(t, sh);
+        const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
+        if (threadIdx.x % W == 0)
+            means[static_cast<int64_t>(g) * a.groups + group] = make_float2(__fdiv_rn(s, all), __fdiv_rn(t, all));
     });
-    s = sum_of<W>(s, sh);
-    t = sum_of<W>(t, sh);
-    const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
-    if (threadIdx.x % W == 0) means[i] = make_float2(__fdiv_rn(s, all), __fdiv_rn(t, all));
 }
 
 template <class P>
@@ -641,16 +698,17 @@ __global__ void __launch_bounds__(kMaxThreads, kGrad) group_grad_apply_kernel(co
                                                                        const float2* stats, const float2* means, T* dx,
                                                                        int64_t lddx) {
     wait_for_previous();
+    if (none_large(a)) return;
     const Place<T, ALIGNED> p(a);
     const int c = blockIdx.x;
-    for_parts(a, c, [&](int g, int lo, int hi) {
+    for_parts(a, c, [&](int g, int lo, int hi, int64_t slot) {
         const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
         const int64_t o = static_cast<int64_t>(g) * a.groups;
         grad_part<SPLIT>(a, p, dy, lddy, x, ldx, k, stats + o, means + o, dx, lddx, lo, hi);
     });
 }
 
-// A block for each graph.
+// A block for each graph of at most a.least rows.
 template <class T, class P, bool ALIGNED, bool SPLIT>
 __global__ void __launch_bounds__(kMaxThreads, 2) group_grad_small_kernel(const GroupArgs a, const T* dy, int64_t lddy, const T* x,
                                                                        int64_t ldx, const P* gamma, const P* beta,
@@ -663,9 +721,11 @@ __global__ void __launch_bounds__(kMaxThreads, 2) group_grad_small_kernel(const 
     const Place<T, ALIGNED> p(a);
     const Params<Place<T, ALIGNED>::V> k(p, gamma, beta);
     for (int i = threadIdx.x; i < a.cols; i += blockDim.x) total[i] = make_float2(0.0f, 0.0f);
+    int large = 0;
     for (int g = blockIdx.x; g < a.graphs; g += gridDim.x) {
         const int b = begin_of(a, g), e = end_of(a, g);
-        if (b >= e) continue;
+        large |= e - b > a.least;
+        if (b >= e || e - b > a.least) continue;
         const float2* st = stats + static_cast<int64_t>(g) * a.groups;
         grad_sums<SPLIT>(a, p, dy, lddy, x, ldx, k, st, b, e, sh);
         __syncthreads();
@@ -691,6 +751,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) group_grad_small_kernel(const 
         out[i] = total[i].y;
         out[a.cols + i] = total[i].x;
     }
+    if (threadIdx.x == 0) a.large[blockIdx.x] = large;
 }
 
 // ── host ─────────────────────────────────────────────────────────────────
@@ -719,13 +780,17 @@ GroupArgs cut(GroupArgs a, int V, int resident) {
     a.chunks = static_cast<int>(ceil_div(a.rows, a.R));
     return a;
 }
-// Whether the graphs are so many and so small (were they alike) that each is a
-// block's: its values are read again from L1 or L2, and one launch does all.
-// A graph far larger than the others would keep its block alone on the GPU, so
-// this is for matrices of up to 16 MB.  SMALL_FIGURES
-bool small_graphs(const GroupArgs& a, size_t size) {
-    const int64_t bytes = a.rows * a.cols * static_cast<int64_t>(size);
-    return a.nv <= kMaxThreads && a.cols <= kSmallCols && bytes <= 16 << 20 && bytes / a.graphs <= 32 << 10;
+// Most rows of a graph that is a block's: 64 KB, or the rows of a chunk.  0 where
+// graphs are larger than half of that on the average: then all are cut in chunks,
+// since a block has no other graph to go on with.  64 columns fp32, forward and
+// gradient, us with whole graphs / in chunks alone: 2,048 graphs of 25 rows 24 + 25
+// / 33 + 31, 16,384 80 + 105 / 167 + 204, 2,047 of one row and one of 49,153 46 + 37 /
+// 337 + 435.  (About 10 of each are the launches that find no larger graph: without
+// them 11 + 16, and 1,944 + 3,599 where there is one.)
+int small_rows(const GroupArgs& a, size_t size) {
+    const int64_t row = a.cols * static_cast<int64_t>(size);
+    if (a.nv > kMaxThreads || a.cols > kSmallCols || a.graphs == 0 || a.rows / a.graphs * row > 32 << 10) return 0;
+    return static_cast<int>(std::max<int64_t>(std::max<int64_t>((64 << 10) / row, 1), a.R));
 }
 // The cut of such graphs: eight rows a lane, where there are blocks enough.
 GroupArgs cut_small(GroupArgs a) {
@@ -741,11 +806,18 @@ int small_blocks(const GroupArgs& a, size_t room, int threads) {
     const int fit = std::min({16, threads / static_cast<int>(block_of(a).x), static_cast<int>(228 * 1024 / (room + 1024))});
     return static_cast<int>(std::min<int64_t>(a.graphs, int64_t(num_sms()) * std::max(1, fit)));
 }
-size_t slots_of(const GroupArgs& a) { return (static_cast<size_t>(a.chunks) + a.graphs) * a.cols; }
+size_t slots_of(const GroupArgs& a) {
+    return (a.least ? 2 * static_cast<size_t>(a.chunks) : static_cast<size_t>(a.chunks) + a.graphs) * a.cols;
+}
+template <int W>
+unsigned join_blocks(const GroupArgs& a, int64_t sets) {
+    return static_cast<unsigned>(a.least ? int64_t(a.chunks) * large_blocks(a.groups) : ceil_div(sets, kJoinBlock<W> / W));
+}
 // Calls f with the threads that join a graph's group: by its parts, were the
-// graphs alike.
+// graphs alike (256 for the large ones among small ones).
 template <class F>
 void by_parts(const GroupArgs& a, F&& f) {
+    if (a.least) return f(std::integral_constant<int, 256>{});
     const int64_t parts = (a.rows / a.R / std::max(a.graphs, 1) + 1) * a.per;
     if (parts <= 256) f(std::integral_constant<int, 32>{});
     else if (parts <= 4096) f(std::integral_constant<int, 256>{});
@@ -758,6 +830,7 @@ void check_group(const char* fn, int64_t rows, int64_t cols, int64_t groups, int
     if (param_dtype != TG_F32 && param_dtype != dtype)
         invalid(std::string(fn) + ": gamma and beta must be fp32 or of the rows' type");
     check_rows_cols(fn, rows, cols);
+    if (rows > INT32_MAX - 1024) invalid(std::string(fn) + ": more than 2^31 - 1024 rows");  // (row lanes count past the last)
     if (groups < 1 || cols % groups != 0)
         invalid(std::string(fn) + ": " + std::to_string(cols) + " columns cannot be cut into " + std::to_string(groups) + " groups");
     if (graphs < 0 || graphs > (1 << 24)) invalid(std::string(fn) + ": " + std::to_string(graphs) + " graphs are outside [0, 2^24]");
@@ -807,30 +880,38 @@ TG_API tg_status tg_group_norm(int64_t rows, int64_t cols, int64_t groups, int64
             const T* xp = static_cast<const T*>(x);
             const P *ga = static_cast<const P*>(gamma), *be = static_cast<const P*>(beta);
             const bool aligned = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(y, ldy, sizeof(T));
-            const GroupArgs a = cut(g, 16 / sizeof(T), kParts);
+            GroupArgs a = cut(g, 16 / sizeof(T), kParts);
+            a.least = small_rows(a, sizeof(T));
             float2* st = reinterpret_cast<float2*>(stats);
             by_layout<T>(a, aligned, [&](auto al, auto split) {
                 constexpr bool ALIGNED = decltype(al)::value, SPLIT = decltype(split)::value;
-                if (small_graphs(a, sizeof(T))) {
-                    const GroupArgs c = cut_small(a);
-                    const size_t room = (Sums<T>::pairs(block_of(c).x) + cols + groups) * sizeof(float2);
+                const GroupArgs small = cut_small(a);
+                const size_t room = (Sums<T>::pairs(block_of(small).x) + cols + groups) * sizeof(float2);
+                const bool chunks = a.least == 0 || rows > a.least;  // else there is no larger graph
+                a.blocks = a.least ? small_blocks(small, room, 512) : 0;
+                // (one allocation: each takes the host 2 us)
+                Scratch<float2> part((chunks ? slots_of(a) : 0) + (a.blocks + 1) / 2, s);
+                a.large = reinterpret_cast<int*>(part.p + (chunks ? slots_of(a) : 0));
+                if (a.least) {
+                    GroupArgs c = small;
+                    c.blocks = a.blocks;
+                    c.large = a.large;
                     auto kern = group_small_kernel<T, P, ALIGNED, SPLIT>;
                     if (room > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
-                    launch_dependent("group_norm", kern, dim3(static_cast<unsigned>(small_blocks(c, room, 512))), block_of(c), room, s, c, xp, ldx,
+                    launch_dependent("group_norm", kern, dim3(static_cast<unsigned>(c.blocks)), block_of(c), room, s, c, xp, ldx,
                                      ga, be, st, static_cast<T*>(y), ldy);
-                    return;
+                    if (!chunks) return;
                 }
-                Scratch<float2> part(slots_of(a), s);
                 launch_dependent("group_norm_parts", group_parts_kernel<T, ALIGNED>, grid_of(a), block_of(a),
                                  Sums<T>::pairs(block_of(a).x) * sizeof(float2), s, a, xp, ldx, part.p);
                 const int64_t sets = graphs * groups;
                 by_parts(a, [&](auto width) {
                     constexpr int W = decltype(width)::value;
-                    launch_dependent("group_norm_stats", group_stats_kernel<W>,
-                                     dim3(static_cast<unsigned>(ceil_div(sets, kJoinBlock<W> / W))), dim3(kJoinBlock<W>), 0, s, a, part.p,
+                    launch_dependent("group_norm_stats", group_stats_kernel<W>, dim3(join_blocks<W>(a, sets)), dim3(kJoinBlock<W>), 0, s, a, part.p,
                                      st);
                 });
-                const GroupArgs c = cut(g, 16 / sizeof(T), kApply<SPLIT>);
+                GroupArgs c = cut(g, 16 / sizeof(T), kApply<SPLIT>);
+                c.least = a.least, c.large = a.large, c.blocks = a.blocks;
                 launch_dependent("group_norm", group_apply_kernel<T, P, ALIGNED, SPLIT>, grid_of(c), block_of(c), 0, s, c, xp, ldx, ga,
                                  be, st, static_cast<T*>(y), ldy);
             });
@@ -869,38 +950,46 @@ TG_API tg_status tg_group_norm_grad(int64_t rows, int64_t cols, int64_t groups, 
             const P *ga = static_cast<const P*>(gamma), *be = static_cast<const P*>(beta);
             const bool aligned = rows_aligned16(x, ldx, sizeof(T)) && rows_aligned16(dy, lddy, sizeof(T)) &&
                                  rows_aligned16(dx, lddx, sizeof(T));
-            const GroupArgs a = cut(g, 16 / sizeof(T), kGrad);
+            GroupArgs a = cut(g, 16 / sizeof(T), kGrad);
+            a.least = small_rows(a, sizeof(T));
             const float2* st = reinterpret_cast<const float2*>(stats);
             const int col_blocks = static_cast<int>(ceil_div(2 * cols, kJoinColumns));
             P *dg = static_cast<P*>(dgamma), *db = static_cast<P*>(dbeta);
             by_layout<T>(a, aligned, [&](auto al, auto split) {
                 constexpr bool ALIGNED = decltype(al)::value, SPLIT = decltype(split)::value;
-                if (graphs > 0 && small_graphs(a, sizeof(T))) {
-                    const GroupArgs c = cut_small(a);
-                    const size_t room = (Sums<T>::pairs(block_of(c).x) + 2 * cols + groups) * sizeof(float2);
-                    const int blocks = small_blocks(c, room, 512);
-                    Scratch<float> sums(static_cast<size_t>(blocks) * 2 * cols, s);
+                // dgamma's and dbeta's sums of the blocks that have whole graphs, then those of the chunks
+                GroupArgs c = cut_small(a);
+                const size_t room = (Sums<T>::pairs(block_of(c).x) + 2 * cols + groups) * sizeof(float2);
+                const int small = a.least ? small_blocks(c, room, 512) : 0;
+                a.blocks = c.blocks = small;
+                const bool large = a.least == 0 || rows > a.least;
+                const dim3 grid = grid_of(a);
+                const int sum_rows = small + (large ? static_cast<int>(grid.x) : 0);
+                const size_t sets = static_cast<size_t>(graphs) * groups;
+                // the parts, the groups' means, the blocks' sums and whether they met a larger graph
+                Scratch<float2> part((large ? slots_of(a) + sets : 0) + static_cast<size_t>(sum_rows) * cols + (small + 1) / 2, s);
+                float2* means = part.p + slots_of(a);
+                float* sums = reinterpret_cast<float*>(large ? means + sets : part.p);
+                a.large = c.large = reinterpret_cast<int*>(sums + static_cast<size_t>(sum_rows) * 2 * cols);
+                if (a.least) {
                     auto kern = group_grad_small_kernel<T, P, ALIGNED, SPLIT>;
                     if (room > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
-                    launch_dependent("group_norm_grad", kern, dim3(static_cast<unsigned>(blocks)), block_of(c), room, s, c, dyp, lddy, xp,
-                                     ldx, ga, be, st, static_cast<T*>(dx), lddx, sums.p);
-                    launch_dependent("group_norm_grad_params", group_params_kernel<P>, dim3(static_cast<unsigned>(col_blocks)),
-                                     dim3(kJoinThreads), 0, s, c, sums.p, blocks, dg, db);
-                    return;
+                    launch_dependent("group_norm_grad", kern, dim3(static_cast<unsigned>(small)), block_of(c), room, s, c, dyp, lddy, xp,
+                                     ldx, ga, be, st, static_cast<T*>(dx), lddx, sums);
+                    if (!large) {
+                        launch_dependent("group_norm_grad_params", group_params_kernel<P>, dim3(static_cast<unsigned>(col_blocks)),
+                                         dim3(kJoinThreads), 0, s, c, sums, sum_rows, dg, db);
+                        return;
+                    }
                 }
-                const dim3 grid = grid_of(a);
-                const int sum_rows = static_cast<int>(grid.x);
-                const size_t sets = static_cast<size_t>(graphs) * groups;
-                Scratch<float2> part(slots_of(a) + sets, s);
-                Scratch<float> sums(static_cast<size_t>(sum_rows) * 2 * cols, s);
-                float2* means = part.p + slots_of(a);
                 launch_dependent("group_norm_grad_parts", group_grad_parts_kernel<T, P, ALIGNED, SPLIT>, grid, block_of(a),
-                                 (Sums<T>::pairs(block_of(a).x) + a.tx * (16 / sizeof(T))) * sizeof(float2), s, a, dyp, lddy, xp, ldx, ga, be, st, part.p, sums.p);
+                                 (Sums<T>::pairs(block_of(a).x) + a.tx * (16 / sizeof(T))) * sizeof(float2), s, a, dyp, lddy, xp, ldx, ga,
+                                 be, st, part.p, sums + static_cast<size_t>(small) * 2 * cols);
                 by_parts(a, [&](auto width) {
                     constexpr int W = decltype(width)::value;
-                    const int blocks = static_cast<int>(ceil_div(sets, kJoinBlock<W> / W));
+                    const int blocks = static_cast<int>(join_blocks<W>(a, sets));
                     launch_dependent("group_norm_grad_join", group_grad_join_kernel<P, W>,
-                                     dim3(static_cast<unsigned>(blocks + col_blocks)), dim3(kJoinBlock<W>), 0, s, a, part.p, ga, sums.p,
+                                     dim3(static_cast<unsigned>(blocks + col_blocks)), dim3(kJoinBlock<W>), 0, s, a, part.p, ga, sums,
                                      sum_rows, blocks, means, dg, db);
                 });
                 launch_dependent("group_norm_grad", group_grad_apply_kernel<T, P, ALIGNED, SPLIT>, grid, block_of(a), 0, s, a, dyp, lddy,

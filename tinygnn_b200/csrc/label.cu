@@ -138,8 +138,11 @@ __device__ __forceinline__ void warp_top(const uint32_t (&rank)[E], int k, uint6
     __syncwarp();
 }
 
-// How a row's best classes are found: one after the other (a few), or by the
-// rank of the last (warp_top).  207,595 x 80 bf16, 20 classes: SELECT_FIGURES
+// How a row's best classes are found: one after the other, which takes longer
+// for each, or by the rank of the last (warp_top), which gives a row 32 lanes
+// whatever its classes.  us for 8, 12 and 20 classes, rounds / select: 200,000 x 41
+// fp32 53, 69, 100 / 126, 129, 129; x 80 bf16 121, 163, 250 / 154, 159, 168;
+// 80,000 x 168 fp16 85, 113, 168 / 90, 93, 98.
 enum Top { kNone, kRounds, kSelect };
 
 template <class T, int LPR, int E, Top TOP>
@@ -622,7 +625,8 @@ TG_API tg_status tg_label_log_probs(int64_t rows, int64_t classes, int32_t dtype
                                  dim3(logits::kNarrowThreads), staged_bytes(RPB * turns, classes, sizeof(T)), s, a, x, ldz, turns);
             };
             using std::integral_constant;
-            if (top > 0 && (top > 6 || classes > logits::kNarrow) && classes <= 1024) {
+            const int rounds = classes <= 48 ? 24 : (classes <= 128 ? 12 : (classes <= logits::kNarrow ? 8 : 0));
+            if (top > rounds && classes <= 1024) {
                 const integral_constant<Top, kSelect> select;
                 const integral_constant<int, 32> lanes;
                 if (classes <= 64) narrow(lanes, integral_constant<int, 2>{}, select);
@@ -649,8 +653,14 @@ TG_API tg_status tg_label_log_probs(int64_t rows, int64_t classes, int32_t dtype
                                     std::min(1024 / (NT * TEAMS), logits::kSharedSm / (room + fixed + 1024)), NT * TEAMS, room, s, a,
                                     x, ldz);
             };
-            // (a warp's 32 maxima bound few best classes well)
-            if (classes <= logits::kWarp && rows > num_sms() && top <= 16) go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+            // A warp a row where there are rows for all warps, or a block: us by warp
+            // / block, bf16: 16,000 x 1,500 16 / 38, x 4,096 30 / 48; 8,000 x 8,000
+            // 32 / 36, 4,000 x 16,000 30 / 37.  With best classes: of 5, 16,000 x
+            // 4,096 87 / 91, 8,000 x 8,000 82 / 62; of 32, 16,000 x 1,500 359 / 98
+            // (its 32 maxima bound few of them well).
+            const bool many = rows > 16 * num_sms();
+            if (top == 0 ? classes <= (many ? 16384 : logits::kWarp) && rows > num_sms()
+                         : classes <= logits::kWarp && rows > num_sms() && top <= 16) go(integral_constant<int, 32>{}, integral_constant<int, 4>{});
             else if (classes / ranks <= 8192) go(integral_constant<int, 128>{}, integral_constant<int, 1>{});
             else go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
         });
