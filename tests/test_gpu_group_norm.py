@@ -384,7 +384,7 @@ def test_c_abi_refusals(tg):
 
     def bwd(groups=2, graphs=1, off=None, dtype=0, dy=p, lddy=8, lddx=8, act=0, stats=p):
         return lib.tg_group_norm_grad(4, 8, groups, graphs, off, dtype, dy, lddy, p, 8, stats, 0, p, p, act, 0.0, p, lddx, p, p, None)
-    calls = [fwd(rows=-1), fwd(cols=0), fwd(groups=3), fwd(graphs=2), fwd(graphs=-1), fwd(graphs=1 << 25, off=p), fwd(dtype=4),
+    calls = [fwd(rows=-1), fwd(rows=2 ** 31 - 1), fwd(cols=0), fwd(groups=3), fwd(graphs=2), fwd(graphs=-1), fwd(graphs=1 << 25, off=p), fwd(dtype=4),
              fwd(x=None), fwd(ldx=7), fwd(pd=1), fwd(act=9), fwd(ldy=7), fwd(stats=None), fwd(stats=p + 4), bwd(groups=3),
              bwd(graphs=0), bwd(dtype=9), bwd(dy=None), bwd(lddy=7), bwd(lddx=7), bwd(act=-1), bwd(stats=None)]
     assert calls == [_lib.INVALID_ARGUMENT] * len(calls)

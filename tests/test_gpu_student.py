@@ -36,9 +36,9 @@ def step64(p, x, sizes, groups, labels, ids, best, mix=0.7, temperature=2.0, ent
     a = x @ p["w1"][0] + p["b1"][0]
     parts, o = [], 0
     for s in sizes:
-        v = a[o:o + s].view(s, groups, -1)
-        o += s
         if s:
+            v = a[o:o + s].view(s, groups, -1)
+            o += s
             m = v.mean((0, 2), keepdim=True)
             parts.append(((v - m) / (((v - m) ** 2).mean((0, 2), keepdim=True) + 1e-5).sqrt()).reshape(s, -1))
     h = torch.nn.functional.gelu(torch.cat(parts) * p["gamma"] + p["beta"], approximate="tanh")
