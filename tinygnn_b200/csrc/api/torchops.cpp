@@ -1,6 +1,6 @@
 // ============================================================================
 //  torchops.cpp -- the Python module `tinygnn_b200._torch_ops`: the training
-//  operators' entry points on torch tensors (tinygnn_b200/training.py wraps
+//  operators' (norms, typed linear maps, saved activations, losses) entry points on torch tensors (tinygnn_b200/training.py wraps
 //  them).
 //
 //  Each function checks its arguments, allocates its results with torch on

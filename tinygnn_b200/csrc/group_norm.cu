@@ -24,6 +24,12 @@
 //  lose the deviations (k is one of the few values it is subtracted from), and
 //  parts are joined by their means and deviations, not by sums of squares.
 //
+//  232,965 x 128 bf16 in one graph, 8 groups: forward 46 us, gradient 64; x and dy
+//  are read twice, and the second reading of 60 or 120 MB comes from HBM again
+//  (its floor is 9.3 us a matrix).  16 graphs of 4,096 x 320 fp16 in 32 groups,
+//  GELU: 43 and 70, bound by issue slots (50 %) and by 15 warps an SM, since
+//  vectors of columns of two groups keep the factors of each column.
+//
 //  What is applied to a value is linear in its distance from the mean, with
 //  factors of its column (the mean is not folded into the addend: a constant
 //  graph's y is beta):
