@@ -216,6 +216,20 @@ def test_many_graphs_and_repeats(tg):
         assert all(torch.equal(p, q) for p, q in zip(first, again))
 
 
+@pytest.mark.parametrize("cols,groups,dtype", [(64, 1, torch.float32), (48, 16, torch.bfloat16), (37, 37, torch.float16),
+                                               (320, 32, torch.float16), (1000, 8, torch.bfloat16)])
+def test_large_graphs_among_small_ones(tg, cols, groups, dtype):
+    """Several graphs larger than a block's among many of few rows or none, neighbours and apart, first and last; all in
+    one; and all alike, at the block's limit and one past it."""
+    g = torch.Generator().manual_seed(cols)
+    limit = max(65536 // (cols * (4 if dtype == torch.float32 else 2)), 1)
+    small = torch.randint(0, 6, (700,), generator=g).tolist()
+    mixed = [3 * limit] + small[:200] + [limit + 1, 2 * limit + 5, 0, limit, limit - 1] + small[200:] + [5 * limit + 1]
+    for sizes in (mixed, [0] * 50 + [4 * limit + 3] + [1] * 300, [limit] * 3 + [0] * 40, [limit + 1] * 3 + [0] * 40):
+        x, dy, gamma, beta = inputs(sum(sizes), cols, dtype, torch.float32, seed=cols)
+        check(tg, x, dy, gamma, beta, sizes, groups, "gelu", 0.0, what=f"{len(sizes)} graphs")
+
+
 def test_one_large_graph(tg):
     for dtype in (torch.float32, torch.bfloat16):
         x, dy, gamma, beta = inputs(100003, 40, dtype, dtype, seed=2)

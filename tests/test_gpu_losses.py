@@ -164,6 +164,46 @@ def test_label(tg, dtype, classes):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [257, 512, 1000, 1030, 2011, 4096, 4097, 4104])
+def test_label_of_many_rows(tg, dtype, classes):
+    """Rows enough for a warp each, several rows a warp, aligned and not."""
+    for rows, layout in ((1500, None), (163, (3, 1))):
+        z = rand(rows, classes, seed=classes, scale=3.0, dtype=dtype)
+        z[rows // 2] = -INF
+        z[rows // 3] = torch.finfo(dtype).min
+        labels = ints(-1, classes + 1, (rows,), seed=classes)
+        if layout:
+            z = strided(z, *layout)
+        for top in (0, 1, 7, 16, 17, 100):
+            out = check_label(tg, z, labels, top, f"{rows} rows, top {top}")
+        check_label_grad(tg, z, labels, out, seed=classes)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_label_of_many_wide_rows(tg, dtype):
+    """More rows than a wave of warps of more than 4,096 classes, and more than a wave of clusters."""
+    for rows, classes in ((2400, 5001), (2400, 16384), (700, 16385)):
+        z = rand(rows, classes, seed=classes, scale=3.0, dtype=dtype)
+        labels = ints(-1, classes + 1, (rows,), seed=classes)
+        out = check_label(tg, z, labels, 0, f"{rows} x {classes}")
+        check_label_grad(tg, z, labels, out, seed=classes)
+    check_label(tg, z, labels, 30, "30 best")
+
+
+@pytest.mark.parametrize("dtype,classes", [(torch.float32, 140001), (torch.bfloat16, 300007), (torch.float16, 1200000)])
+def test_the_widest_rows(tg, dtype, classes):
+    """Rows that eight CTAs cannot hold: the distillation reads them twice."""
+    for rows in (1, 3, 40):
+        if rows * classes > 2 ** 24:
+            continue
+        z = rand(rows, classes, seed=rows, scale=3.0, dtype=dtype)
+        labels = ints(0, classes, (rows,), seed=1)
+        out = check_label(tg, z, labels, 50, f"{rows} rows")
+        check_label_grad(tg, z, labels, out, seed=1)
+        check_distill(tg, z, ints(-2, classes + 2, (rows, 60), 3), rand(rows, 60, seed=4, dtype=dtype), 1.3, rand(rows, seed=5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("classes", [5, 41, 300, 1024, 5003, 33000])
 def test_label_masks(tg, dtype, classes):
     """Masked classes (-inf and the type's lowest value), rows of them alone, NaN, +inf, constant rows, and k larger
@@ -319,6 +359,21 @@ def test_distill(tg, dtype, classes):
         weights = rand(rows, seed=5) if rows != 5 else None
         check_distill(tg, z, pick(rows, classes, k, classes, kind) if rows > 1 else ints(0, classes, (1, 1), 1, kind), teacher,
                       temperature, weights, f"{rows} rows")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [16, 48, 257, 512, 1001, 2048, 4096, 4099, 9000, 40001])
+def test_distill_of_many_rows(tg, dtype, classes):
+    """Rows enough for a warp each and for several rounds of every block and cluster; few and many entries."""
+    for rows, k, kind, layout in ((1500, 8, torch.int32, None), (1100, 32, torch.int64, (3, 1)), (333, 128, torch.int64, None)):
+        if rows * classes > 2 ** 25:
+            continue
+        z = rand(rows, classes, seed=classes + k, scale=3.0, dtype=dtype)
+        z[rows // 3] = -INF
+        if layout:
+            z = strided(z, *layout)
+        check_distill(tg, z, pick(rows, classes, k, classes, kind), rand(rows, k, seed=2, scale=2.0, dtype=dtype), 1.7,
+                      rand(rows, seed=3), f"{rows} rows, {k} entries")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -335,8 +335,9 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
 }
 
 // ── rows of a warp ───────────────────────────────────────────────────────
-// As the wide rows' kernel below, with a warp in the place of the block: of the
-// ring's slots kAhead are for the next rows.
+// As the wide rows' kernel below, with a warp in the place of the block: the ring
+// has a row and kAhead slots of the next ones; without a gradient no row is held,
+// and it has kAhead slots in all.
 constexpr int kTeams = 4;
 
 template <class T, class U, int N, bool GRAD>
@@ -361,8 +362,9 @@ __global__ void __launch_bounds__(32 * kTeams, 5) distill_warp_kernel(const Dist
         entries.fetch_scores(a, p.row);
         Soft s;
         const int steps = in.steps_of(p), mine_first = in.from, count = p.v1 - p.v0;
-        in.template wait<kAhead>();
+        if (GRAD) in.template wait<kAhead>();  // the row is there
         for (int i = 0, have = count; i < steps; ++i, have -= 32 * in.W) {
+            if (!GRAD) in.template wait<kAhead - 1>();  // its next slot is
             in.template add<false>(s, in.from, have, c);
             in.from = in.next(in.from);
             if (!GRAD) in.ask();
