@@ -70,7 +70,7 @@ def test_step_against_the_whole_formula(tg, example):
     want, z64 = step64(p, x.double(), sizes, 6, labels, ids, best)
     want.backward()
     tol = 8 * 5 * 2.0 ** -23 * (8 + math.sqrt(64))
-    assert abs(float(loss) - float(want)) <= tol * abs(float(want))
+    assert abs(float(loss) - float(want.detach())) <= tol * abs(float(want.detach()))
     for name, got, ref in (("z", z, z64.detach()), *((k, grads[k].view_as(p[k]), p[k].grad) for k in grads)):
         off_by = float((got.double() - ref).norm() / ref.norm())
         assert off_by <= tol, f"{name}: {off_by}"
