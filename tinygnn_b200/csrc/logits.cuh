@@ -55,10 +55,13 @@ struct Soft {
 };
 
 // 16-bit scores whose entropy is not asked for (FUSED): d = z c - M with M = m c
-// rounded once, one instruction a score.  M's rounding shifts all of a row's d
-// alike and falls out of log p = d - log s; only a maximum whose product with c
-// leaves fp32's range (`far`) takes (z - m) c.  (With the entropy, whose log p of
-// a sure label is to be 0, all rows take the latter.)
+// rounded once, one instruction a score.  M's rounding r = m c - M shifts all of
+// a row's d alike and falls out of log p = d - log s; it is at most 2^-15 while
+// |M| <= 1024.  A maximum beyond that (`far`: a mask of a large finite number, a
+// small temperature), where r could leave the exponential's range, takes
+// (z - m) c, which is 0 at the maximum.  A row's state is always that of its own
+// maximum's form; `between` takes r along where the two differ.  (With the entropy,
+// whose log p of a sure label is to be 0, all rows take (z - m) c.)
 template <bool FAST, bool ENTROPY>
 constexpr bool kFused = FAST && !ENTROPY;
 struct Origin {
@@ -66,19 +69,21 @@ struct Origin {
     bool far;
     __device__ __forceinline__ Origin(float most, float c) : m(origin(most)) {
         M = __fmul_rn(m, c);
-        far = !(fabsf(M) <= 1e38f);  // (or NaN)
+        far = !(fabsf(M) <= 1024.0f);  // (or NaN)
     }
     // At least -inf: its exponential is 0.
     __device__ __forceinline__ float d(float z, float c) const {
         return far ? __fmul_rn(__fsub_rn(z, m), c) : fmaf(z, c, -M);
     }
 };
-// d of the maximum `from` as seen from the maximum `to`.
+// d of the maximum `from` as seen from the maximum `to`: what scales a state of
+// the one to the other.
 template <bool FUSED>
 __device__ __forceinline__ float between(float from, float to, float c) {
     if (FUSED && from != -INFINITY) {
         const Origin a(from, c), b(to, c);
-        if (!a.far && !b.far) return __fsub_rn(a.M, b.M);
+        if (!a.far) return b.far ? -fmaf(to, c, -a.M) : __fsub_rn(a.M, b.M);
+        if (!b.far) return fmaf(from, c, -b.M);
     }
     return distance(from, to, c);
 }
