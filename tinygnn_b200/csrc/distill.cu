@@ -5,6 +5,7 @@
 //      q = softmax(t / T) over the teacher's k classes c_i of the row
 //      p = softmax(z / T) over all classes
 //      loss = T^2 sum_i q_i (log q_i - log p_{c_i})
+//           = T (T sum_i q_i log q_i - sum_i q_i ((z_{c_i} - max z) - T log s))
 //      dz_j = w T (p_j - sum over i with c_i = j of q_i)
 //
 //  The gradient needs the row's sum before its first value, and the row's
@@ -95,7 +96,7 @@ struct Entries {
 };
 
 // From a row's classes and logits in t.c and t.q (-inf for none), W lanes set
-// their probabilities and the row's scale; each lane's part of sum q (log q) is
+// their probabilities and the row's scale; each lane's part of T sum q log q is
 // returned.  (A lane reads what it wrote, and t.c of all lanes.)
 template <int W>
 __device__ __forceinline__ float finish_teacher(const DistillArgs& a, int lane, const Teacher& t, float weight) {
@@ -152,7 +153,7 @@ __device__ __forceinline__ float finish_teacher(const DistillArgs& a, int lane, 
     }
     if (lane == 0) *t.scale = most == -INFINITY ? 0.0f : __fmul_rn(a.temperature, weight);
     __syncwarp();
-    return entropy;
+    return __fmul_rn(a.temperature, entropy);
 }
 
 // Fills `t` from a warp's entries; returned as above.
@@ -176,6 +177,7 @@ template <bool FAST>
 struct RowScale {
     Origin o;
     float c, log_s;  // log of the sum, in the exponential's units
+    float shift;     // T log p = (z - max) - shift: T times the sum's log, of the exact origin
     float w;         // w T; 0 for a row without gradient
     // Where fp32 holds them well the origin, the sum and the weight go into one
     // addend: w p = +-2^(z c - K).  (|M| <= 64 and a weight above 2^-64 keep |K|
@@ -184,18 +186,19 @@ struct RowScale {
     bool quick;
     uint32_t sign;  // of two 16-bit results
 
-    __device__ __forceinline__ RowScale(const Soft& s, float c_, float scale) : o(s.m, c_), c(c_) {
-        log_s = __fmul_rn(logf(s.s), FAST ? kLog2e : 1.0f);
+    __device__ __forceinline__ RowScale(const Soft& s, float c_, float temperature, float scale) : o(s.m, c_), c(c_) {
+        const float natural = logf(s.s);
+        log_s = __fmul_rn(natural, FAST ? kLog2e : 1.0f);
+        // (a folded row's sum has the rounding of M)
+        shift = __fmul_rn(temperature, FAST && !o.far ? fmaf(-kLn2, fmaf(o.m, c, -o.M), natural) : natural);
         w = s.m == -INFINITY ? 0.0f : scale;  // (no class is left, no gradient)
         quick = FAST && fabsf(o.M) <= 64.0f && fabsf(w) > 5.421e-20f;
         K = __fsub_rn(__fadd_rn(o.M, log_s), __log2f(fabsf(w)));
         sign = w < 0.0f ? 0x80008000u : 0u;
     }
-    // log p of a score in natural units; NaN in a row without any score above -inf.
-    __device__ __forceinline__ float log_p(float z) const {
-        if (!FAST) return __fsub_rn(__fmul_rn(__fsub_rn(z, o.m), c), log_s);
-        return __fmul_rn(__fsub_rn(o.d(z, c), log_s), kLn2);
-    }
+    // T log p of a score; NaN in a row without any score above -inf.  (Without T
+    // the quotient of a finite difference could pass fp32's range.)
+    __device__ __forceinline__ float t_log_p(float z) const { return __fsub_rn(__fsub_rn(z, o.m), shift); }
     __device__ __forceinline__ float prob(float z) const {
         const float d = FAST ? o.d(z, c) : __fmul_rn(__fsub_rn(z, o.m), c);
         return expo<FAST>(max_nan(__fsub_rn(d, log_s), -200.0f));
@@ -306,11 +309,11 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
             Soft s;
             add_scores<FAST, false>(s, z, c);
             lanes_soft<FAST, false, LPR>(s, c);
-            const RowScale<FAST> r(s, c, *t.scale);
+            const RowScale<FAST> r(s, c, a.temperature, *t.scale);
             for (int i = lane; i < a.k; i += LPR)
-                if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.log_p(t.z[i]), loss);
+                if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.t_log_p(t.z[i]), loss);
             loss = reduce_sum<float, LPR>(loss);
-            if (lane == 0 && here) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
+            if (lane == 0 && here) a.loss[row] = __fmul_rn(a.temperature, loss);
             if constexpr (GRAD) {
                 if (here) {
 #pragma unroll
@@ -376,11 +379,11 @@ __global__ void __launch_bounds__(32 * kTeams, 5) distill_warp_kernel(const Dist
         lanes_soft<FAST, false, 32>(s, c);
         float loss = read_teacher(a, entries, lane, t);
         if (row + step < a.rows) entries.fetch(a, row + step, lane);
-        const RowScale<FAST> r(s, c, *t.scale);
+        const RowScale<FAST> r(s, c, a.temperature, *t.scale);
         for (int i = lane; i < a.k; i += 32)
-            if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.log_p(t.z[i]), loss);
+            if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.t_log_p(t.z[i]), loss);
         loss = reduce_sum<float, 32>(loss);
-        if (lane == 0) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
+        if (lane == 0) a.loss[row] = __fmul_rn(a.temperature, loss);
         if constexpr (GRAD) {
             T* out = dx + row * lddx;
             write_grad<FAST, T, 32>(in, mine_first, steps, count, r, out + p.column(p.v0 + lane),
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(NT + 32, 768 / NT) distill_wide_kernel(const D
             all();
             if constexpr (GRAD) {
                 s = joined(b);
-                const RowScale<FAST> r(s, c, teacher.scale[b]);
+                const RowScale<FAST> r(s, c, a.temperature, teacher.scale[b]);
                 T* out = dx + row * lddx;
                 const int end = write_grad<FAST, T, NT>(in, hold ? mine_first : in.from, steps, count, r,
                                                         out + p.column(p.v0 + threadIdx.x),
@@ -493,13 +496,13 @@ __global__ void __launch_bounds__(NT + 32, 768 / NT) distill_wide_kernel(const D
             if (row + clusters < a.rows) next.fetch_scores(a, x + (row + clusters) * ldx);
             all();
             const Soft s = joined(b);
-            const RowScale<FAST> r(s, c, *t.scale);
+            const RowScale<FAST> r(s, c, a.temperature, *t.scale);
             float loss = own;
             if (rank == 0) {
                 for (int i = lane; i < a.k; i += 32)
-                    if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.log_p(t.z[i]), loss);
+                    if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.t_log_p(t.z[i]), loss);
                 loss = reduce_sum<float, 32>(loss);
-                if (lane == 0) a.loss[row] = __fmul_rn(__fmul_rn(a.temperature, a.temperature), loss);
+                if (lane == 0) a.loss[row] = __fmul_rn(a.temperature, loss);
             }
             meet();
             if constexpr (GRAD) {
