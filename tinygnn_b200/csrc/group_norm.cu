@@ -16,13 +16,14 @@
 //  it; chunk c's part of graph g is slot c + g, which no other part has, and there
 //  are at most chunks + graphs of them.  A second, small kernel joins a graph's
 //  slots in their order (no atomics, the same bits every run), and a third applies
-//  the statistics.  Where graphs are small (small_graphs below) each is a block's
+//  the statistics.  Where graphs are small (small_rows below) each is a block's
 //  instead, in one kernel, and the three have the larger ones alone.
 //
 //  A part's mean and sum of squared deviations come from one pass: each thread
-//  sums x - k and (x - k)^2 with k its first value of the column, which cannot
-//  lose the deviations (k is one of the few values it is subtracted from), and
-//  parts are joined by their means and deviations, not by sums of squares.
+//  sums x - k and (x - k)^2 with k its first value of the column (one of the
+//  values it is subtracted from: where it is far from the others, so is the part's
+//  deviation, and each row costs 2^-24 of it at most), and parts are joined by their
+//  means and deviations, not by sums of squares.
 //
 //  232,965 x 128 bf16 in one graph, 8 groups: forward 46 us, gradient 64; x and dy
 //  are read twice, and the second reading of 60 or 120 MB comes from HBM again
@@ -341,6 +342,20 @@ __device__ __forceinline__ float sum_of(float v, float* sh) {
     for (int w = 0; w < W / 32; ++w) v = __fadd_rn(v, sh[w]);
     return v;
 }
+// Two sums in 64 bits (both at a time: a double's addition takes long to come back).
+template <int W>
+__device__ __forceinline__ void sums_of(double& s, double& d, double2* sh) {
+    s = reduce_sum<double, 32>(s);
+    d = reduce_sum<double, 32>(d);
+    if (W == 32) return;
+    const int lane = threadIdx.x & 31;
+    __syncthreads();
+    if (lane == 0) sh[threadIdx.x >> 5] = make_double2(s, d);
+    __syncthreads();
+    const double2 v = lane < W / 32 ? sh[lane] : make_double2(0.0, 0.0);
+    s = reduce_sum<double, 32>(v.x);
+    d = reduce_sum<double, 32>(v.y);
+}
 
 // Calls f(g, group) for the graphs' groups that W threads join: one, blockIdx.x's
 // W-th part's; of large graphs among small ones those of the graph that begins in
@@ -362,28 +377,31 @@ __device__ __forceinline__ void for_sets(const GroupArgs& a, int block, F&& f) {
 // stats[g * groups + group] = (mean, rstd), (0, 0) for a graph without rows.
 template <int W>
 __global__ void __launch_bounds__(kJoinBlock<W>) group_stats_kernel(const GroupArgs a, const float2* part, float2* stats) {
-    __shared__ float sh[32];
+    __shared__ double2 sh[32];
     wait_for_previous();
     if (none_large(a)) return;
     for_sets<W>(a, blockIdx.x, [&](int g, int group) {
         const int c0 = group * a.per, b = begin_of(a, g), e = end_of(a, g);
         float2 r = make_float2(0.0f, 0.0f);
         if (b < e) {
-            const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
-            // The parts' means m about the first part's, k: as in a part, the sum of
-            // n (m - k)^2 less that of their mean cannot lose the deviations.
-            const float k = part[slot_of(a, g, b / a.R, 0) * a.cols + c0].x;
-            float s = 0.0f, d = 0.0f;
+            const double inv = 1.0 / (static_cast<double>(e - b) * a.per);
+            // The parts' means m about the first part's, k, in 64 bits: k is one mean
+            // of a hundred thousand, and where its column or its rows stand apart from
+            // the rest the sum of n (m - k)^2 is that many times what is left of it
+            // less that of their mean.  (In 32 bits, 4,096 x 1,024 with a first column
+            // 1,000 deviations off: rstd off by 5e-5.  64 bits cost 1.5 us of the 111 of
+            // 232,965 x 128 in one graph, by the latency of their additions.)
+            const double k = part[slot_of(a, g, b / a.R, 0) * a.cols + c0].x;
+            double s = 0.0, d = 0.0;
             for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) {
-                const float z = __fsub_rn(p.x, k), w = __fmul_rn(z, static_cast<float>(n));
-                s = __fadd_rn(s, w);
-                d = __fadd_rn(d, fmaf(z, w, p.y));
+                const double z = p.x - k, w = z * n;
+                s += w;
+                d += fma(z, w, static_cast<double>(p.y));
             });
-            s = sum_of<W>(s, sh);
-            d = sum_of<W>(d, sh);
-            const float shift = __fdiv_rn(s, all), mean = __fadd_rn(k, shift);
-            d = max_nan(fmaf(-s, shift, d), 0.0f);
-            r = make_float2(mean, __frsqrt_rn(__fadd_rn(__fdiv_rn(d, all), a.eps)));
+            sums_of<W>(s, d, sh);
+            const double shift = s * inv;
+            const float var = max_nan(static_cast<float>(fma(-s, shift, d) * inv), 0.0f);
+            r = make_float2(static_cast<float>(k + shift), __frsqrt_rn(__fadd_rn(var, a.eps)));
         }
         if (threadIdx.x % W == 0) stats[static_cast<int64_t>(g) * a.groups + group] = r;
     });
