@@ -527,7 +527,7 @@ void distill(const DistillArgs& a, const T* x, int64_t ldx, T* dx, int64_t lddx,
             const int stage = static_cast<int>((RPB * turns * a.n * sizeof(T) + 32 + 15) / 16 * 16);
             // (and a teacher for each of a turn's lanes that may have no row)
             const size_t bytes = stage + (RPB * turns + RPB) * Teacher::floats(a.k) * sizeof(float);
-            if (bytes > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+            if (bytes > 48 * 1024) allow_shared(kern, kMaxShared);
             launch_dependent("distill_loss", kern,
                              dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(a.rows, RPB * turns), num_sms() * 8))),
                              dim3(kNarrowThreads), bytes, s, a, x, ldx, dx, lddx, turns, stage);

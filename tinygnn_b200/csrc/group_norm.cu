@@ -921,7 +921,7 @@ TG_API tg_status tg_group_norm(int64_t rows, int64_t cols, int64_t groups, int64
                     c.blocks = a.blocks;
                     c.large = a.large;
                     auto kern = group_small_kernel<T, P, ALIGNED, SPLIT>;
-                    if (room > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
+                    if (room > 48 * 1024) allow_shared(kern, kMaxShared);
                     launch_dependent("group_norm", kern, dim3(static_cast<unsigned>(c.blocks)), block_of(c), room, s, c, xp, ldx,
                                      ga, be, st, static_cast<T*>(y), ldy);
                     if (!chunks) return;
@@ -997,7 +997,7 @@ TG_API tg_status tg_group_norm_grad(int64_t rows, int64_t cols, int64_t groups, 
                 a.large = c.large = reinterpret_cast<int*>(sums + static_cast<size_t>(sum_rows) * 2 * cols);
                 if (a.least) {
                     auto kern = group_grad_small_kernel<T, P, ALIGNED, SPLIT>;
-                    if (room > 48 * 1024) TG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
+                    if (room > 48 * 1024) allow_shared(kern, kMaxShared);
                     launch_dependent("group_norm_grad", kern, dim3(static_cast<unsigned>(small)), block_of(c), room, s, c, dyp, lddy, xp,
                                      ldx, ga, be, st, static_cast<T*>(dx), lddx, sums);
                     if (!large) {

@@ -10,6 +10,15 @@ namespace tg {
 void count_launch(const char* name);  // one per kernel launch (tg_kernel_launch_count, tg_last_kernel_name)
 void require_device();   // throws TG_ERR_NO_DEVICE without a GPU
 
+// Lets `kernel` be launched with up to `most` bytes of dynamic shared memory: the
+// most that any call of it needs, since a limit that followed each call's own need
+// could be lowered by another host thread between this thread's setting and launch.
+template <class K>
+inline void allow_shared(K kernel, int most) {
+    TG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+}
+constexpr int kMaxShared = 227 * 1024;  // of a block, its static shared memory included
+
 // Launch `kernel<<<grid, block, smem, stream>>>(args...)`, count it and check
 // the launch.  Empty grids launch nothing.
 template <class K, class... A>

@@ -494,6 +494,8 @@ __device__ __forceinline__ int class_at(const void* p, int64_t i, bool wide) {
     return v < 0 || v > INT32_MAX ? -1 : static_cast<int>(v);
 }
 
+constexpr int kFixed = 5 * 1024;  // more than the static shared memory of a kernel that takes over 32 KB beside it
+
 // Launches clusters of `ranks` blocks for `rows` rows, at most as many as run at
 // a time (`resident` blocks an SM: each cluster walks rows, and one that had to
 // wait for another to end would come last), dependent on the previous kernel
@@ -502,7 +504,7 @@ template <class K, class... A>
 void launch_rows(const char* name, K kernel, int64_t rows, int ranks, int resident, int block, size_t smem, cudaStream_t s,
                  A... args) {
     if (rows == 0) return;
-    if (smem > 32 * 1024) TG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    if (smem > 32 * 1024) allow_shared(kernel, kMaxShared - kFixed);
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(static_cast<unsigned>(block));
     cfg.dynamicSmemBytes = smem;

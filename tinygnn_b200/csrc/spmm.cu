@@ -330,7 +330,7 @@ void csr_degree_order(int64_t M, const int32_t* rp, int32_t* out, cudaStream_t s
     constexpr int64_t kScanSmemMax = 200 * 1024;  // counts staged through shared memory up to this size
     if (n * 4 <= kScanSmemMax) {
         const int smem = static_cast<int>(n * 4);
-        TG_CUDA(cudaFuncSetAttribute(order_scan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        allow_shared(order_scan_kernel<true>, static_cast<int>(kScanSmemMax));
         launch("order_scan", order_scan_kernel<true>, dim3(1), dim3(1024), static_cast<size_t>(smem), s, counts.p, n);
     } else {
         launch("order_scan", order_scan_kernel<false>, dim3(1), dim3(1024), 0, s, counts.p, n);
