@@ -270,6 +270,7 @@ __device__ __forceinline__ void part_top(TopShared<NT>& sh, const Part<T>& p, ui
     int above;
     for (;;) {
         if (tid == 0) sh.n_above = sh.n_equal = sh.n_threads = 0;
+        if (NT == 32) __syncwarp();  // (a block's count is a barrier, a warp's ballot orders no memory)
         // Where many threads reach the bound its score is a common one: then
         // only those above it are looked at, and the equal ones found below.
         const bool common = Team::count(most != 0 && most >= bound) > (NT == 32 ? NT : 2 * k + 32);

@@ -196,7 +196,7 @@ struct Team {
         if (NT == 32) __syncwarp();
         else asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
     }
-    // How many of them; and a sync.
+    // How many of them; and a block's sync (a warp's ballot orders no memory).
     static __device__ __forceinline__ int count(bool x) {
         if (NT == 32) return __popc(__ballot_sync(0xffffffffu, x));
         int n;
