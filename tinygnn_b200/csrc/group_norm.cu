@@ -314,22 +314,27 @@ __global__ void __launch_bounds__(kMaxThreads, kParts) group_parts_kernel(const 
     });
 }
 
-// Calls f(part, rows of it, column) for this thread's parts of a graph's group
-// (its columns from c0 on), one of W threads.
-template <int W, class F>
-__device__ __forceinline__ void for_slots(const GroupArgs& a, int g, int b, int e, int c0, const float2* part, F&& f) {
-    const int first = b / a.R, slots = (e - 1) / a.R - first + 1;
-    // (of narrow groups a thread has the same column of every W / per-th slot)
-    const int wide = a.per < W ? a.per : W, step = W / wide, t = threadIdx.x % W;
-    if (t >= wide * step) return;
-    for (int col = t % wide; col < a.per; col += wide)
-#pragma unroll 4
-        for (int i = t / wide; i < slots; i += step) {
-            // (a slot's rows; the last chunk's end may pass 2^31)
-            const int r0 = (first + i) * a.R, r1 = e - r0 < a.R ? e : r0 + a.R;
-            f(part[slot_of(a, g, first, i) * a.cols + c0 + col], r1 - (b > r0 ? b : r0), c0 + col);
-        }
-}
+// This thread's parts of a graph's group, one of W threads: those of its columns
+// c0 + col for col = first_col, + wide, ... < per, of each the slots first_slot,
+// + step, ...
+template <int W>
+struct Share {
+    int first, slots, wide, step, first_col, first_slot;
+    __device__ __forceinline__ Share(const GroupArgs& a, int b, int e) : first(b / a.R), slots((e - 1) / a.R - first + 1) {
+        // (of narrow groups a thread has the same column of every W / per-th slot)
+        wide = a.per < W ? a.per : W;
+        step = W / wide;
+        const int t = threadIdx.x % W;
+        first_col = t < wide * step ? t % wide : a.per;
+        first_slot = t / wide;
+    }
+    // Rows of a graph's (b .. e) part in slot i.
+    __device__ __forceinline__ int rows(const GroupArgs& a, int b, int e, int i) const {
+        // (the last chunk's end may pass 2^31)
+        const int r0 = (first + i) * a.R, r1 = e - r0 < a.R ? e : r0 + a.R;
+        return r1 - (b > r0 ? b : r0);
+    }
+};
 // The sum over W threads (a warp, or the block).
 template <int W>
 __device__ __forceinline__ float sum_of(float v, float* sh) {
@@ -384,23 +389,50 @@ __global__ void __launch_bounds__(kJoinBlock<W>) group_stats_kernel(const GroupA
         const int c0 = group * a.per, b = begin_of(a, g), e = end_of(a, g);
         float2 r = make_float2(0.0f, 0.0f);
         if (b < e) {
-            const double inv = 1.0 / (static_cast<double>(e - b) * a.per);
-            // The parts' means m about the first part's, k, in 64 bits: k is one mean
-            // of a hundred thousand, and where its column or its rows stand apart from
-            // the rest the sum of n (m - k)^2 is that many times what is left of it
-            // less that of their mean.  (In 32 bits, 4,096 x 1,024 with a first column
-            // 1,000 deviations off: rstd off by 5e-5.  64 bits cost 1.5 us of the 111 of
-            // 232,965 x 128 in one graph, by the latency of their additions.)
+            const double all = static_cast<double>(e - b) * a.per;
+            const float inv = __frcp_rn(static_cast<float>(all));
+            // The parts' means m about the first part's, k: k is one mean of a hundred
+            // thousand, and where its column or its rows stand apart from the rest the
+            // sum of n (m - k)^2 is that many times what is left of it less that of
+            // their mean.  So U parts at a time are summed about the first of them in
+            // 32 bits, and those sums about k in 64: with z = m_0 - k,
+            //     sum n (m - k)^2 = sum n (m - m_0)^2 + 2 z sum n (m - m_0) + z^2 sum n.
+            // (4,096 x 1,024 with a first column 1,000 deviations off: rstd within 1.1e-4
+            // in 32 bits alone, 1e-7 so.  An SM converts 16 numbers a clock to 64 bits:
+            // each part by itself took 9 us longer of 80,000 parts.)
+            constexpr int U = 8;
             const double k = part[slot_of(a, g, b / a.R, 0) * a.cols + c0].x;
             double s = 0.0, d = 0.0;
-            for_slots<W>(a, g, b, e, c0, part, [&](float2 p, int n, int) {
-                const double z = p.x - k, w = z * n;
-                s += w;
-                d += fma(z, w, static_cast<double>(p.y));
-            });
+            const Share<W> mine(a, b, e);
+            for (int col = mine.first_col; col < a.per; col += mine.wide)
+                for (int i = mine.first_slot; i < mine.slots; i += U * mine.step) {
+                    float2 p[U];
+                    int n[U], rows = 0;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        // (one that is not there: the last, without rows)
+                        const int slot = min(i + u * mine.step, mine.slots - 1);
+                        p[u] = part[slot_of(a, g, mine.first, slot) * a.cols + c0 + col];
+                        n[u] = i + u * mine.step < mine.slots ? mine.rows(a, b, e, slot) : 0;
+                        rows += n[u];
+                    }
+                    float t = 0.0f, q = p[0].y;
+#pragma unroll
+                    for (int u = 1; u < U; ++u) {
+                        const float x = __fsub_rn(p[u].x, p[0].x), w = __fmul_rn(x, static_cast<float>(n[u]));
+                        t = __fadd_rn(t, w);
+                        q = __fadd_rn(q, fmaf(x, w, n[u] ? p[u].y : 0.0f));
+                    }
+                    const double z = p[0].x - k, all_t = t, w = z * rows;
+                    s += w + all_t;
+                    d += fma(z, fma(2.0, all_t, w), static_cast<double>(q));
+                }
             sums_of<W>(s, d, sh);
-            const double shift = s * inv;
-            const float var = max_nan(static_cast<float>(fma(-s, shift, d) * inv), 0.0f);
+            // (s / all by its quotient in 32 bits and that of the remainder: a division in
+            // 64 bits takes 2 us)
+            const double near = __fmul_rn(static_cast<float>(s), inv);
+            const double shift = near + __fmul_rn(static_cast<float>(fma(-near, all, s)), inv);
+            const float var = max_nan(__fmul_rn(static_cast<float>(fma(-s, shift, d)), inv), 0.0f);
             r = make_float2(static_cast<float>(k + shift), __frsqrt_rn(__fadd_rn(var, a.eps)));
         }
         if (threadIdx.x % W == 0) stats[static_cast<int64_t>(g) * a.groups + group] = r;
@@ -695,11 +727,16 @@ __global__ void __launch_bounds__(kJoinBlock<W>) group_grad_join_kernel(const Gr
         const int b = begin_of(a, g), e = end_of(a, g);
         if (b >= e) return;
         float s = 0.0f, t = 0.0f;
-        for_slots<W>(a, g, b, e, group * a.per, part, [&](float2 p, int, int column) {
-            const float w = to_f32(gamma[column]);
-            s = fmaf(w, p.x, s);
-            t = fmaf(w, p.y, t);
-        });
+        const Share<W> mine(a, b, e);
+        for (int col = mine.first_col; col < a.per; col += mine.wide)
+#pragma unroll 4
+            for (int i = mine.first_slot; i < mine.slots; i += mine.step) {
+                const int column = group * a.per + col;
+                const float2 p = part[slot_of(a, g, mine.first, i) * a.cols + column];
+                const float w = to_f32(gamma[column]);
+                s = fmaf(w, p.x, s);
+                t = fmaf(w, p.y, t);
+            }
         s = sum_of<W>(s, sh);
         t = sum_of<W>(t, sh);
         const float all = __fmul_rn(static_cast<float>(e - b), static_cast<float>(a.per));
