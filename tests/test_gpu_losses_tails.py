@@ -38,3 +38,17 @@ def test_best_classes_beside_the_vectors(tg, dtype, classes, rows):
             assert torch.equal(first[4], want), f"offset {offset}, top {top}"
             for _ in range(20):
                 assert all(torch.equal(a, b) for a, b in zip(tg.label_log_probs(into, labels, top), first))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [5, 16, 41, 64, 100, 256])
+def test_last_rows_of_a_block(tg, dtype, classes):
+    """Narrow rows whose block has lanes without a row beside theirs: the same bits as among more rows."""
+    z = rand(300, classes, seed=classes, scale=3.0, dtype=dtype)
+    ids = torch.arange(300 * 6, device="cuda").view(300, 6) * 7 % classes
+    teacher, w = rand(300, 6, seed=1), rand(300, seed=2)
+    loss, dz = tg.distill_loss(z, ids, teacher, 2.0, w)
+    for rows in (1, 2, 3, 7, 8, 9, 31, 33, 63, 65, 100, 127, 257):
+        part = tg.distill_loss(z[:rows], ids[:rows], teacher[:rows], 2.0, w[:rows])
+        assert torch.equal(part[0], loss[:rows]) and torch.equal(part[1], dz[:rows]), f"{rows} rows"
+        assert torch.equal(tg.distill_loss(z[:rows], ids[:rows], teacher[:rows], 2.0, grad=False), loss[:rows])

@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
         T* st = stage_in(sh, x, ldx, r0, rows, a.n);
         __syncthreads();
         for (int first = 0; first < rows; first += RPB) {
-            // (lanes without a row compute the first one's, without a teacher, and write nothing)
+            // (lanes without a row have masked scores and no teacher, and write nothing: any
+            // row's scores may be written over by its own lanes)
             const bool here = first + place < rows;
             const int sub = here ? first + place : first;
             const int64_t row = r0 + sub;
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const int j = lane + i * LPR;
-                z[i] = j < a.n ? to_f32(p[j]) : -INFINITY;
+                z[i] = here && j < a.n ? to_f32(p[j]) : -INFINITY;
             }
             __syncwarp();  // (before the row's first lanes write over its scores)
             float loss = finish_teacher<LPR>(a, lane, t, *t.scale);
