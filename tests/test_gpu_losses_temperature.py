@@ -73,3 +73,19 @@ def test_both_factors_of_the_temperature(tg, dtype):
     # 2^-24 of a few numbers up to log 300 and the differences of the scores (within 10)
     for t in (0.5, 4.0):
         assert (at[t] - at[1.0]).abs().max() <= 2.0 ** -24 * 2 * 40
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", CLASSES)
+def test_teacher_of_masked_classes_alone(tg, dtype, classes):
+    """All of the teacher's probability at the type's lowest score: the sum over its entries is the largest there is,
+    and the loss T times that."""
+    rows, k = 160, min(classes - 2, 46)
+    low = torch.finfo(dtype).min
+    z = rand(rows, classes, seed=classes, scale=2.0, dtype=dtype)
+    z[:, :k] = low
+    ids = torch.arange(k, device="cuda").expand(rows, k)
+    teacher = rand(rows, k, seed=2, dtype=torch.float32)
+    for t in (0.1, 0.5, 0.9):
+        loss, _ = check_distill(tg, z, ids, teacher, t, None, f"T {t}")
+        assert loss.isfinite().all()

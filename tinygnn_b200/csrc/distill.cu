@@ -8,6 +8,9 @@
 //           = T (T sum_i q_i log q_i - sum_i q_i ((z_{c_i} - max z) - T log s))
 //      dz_j = w T (p_j - sum over i with c_i = j of q_i)
 //
+//  (A factor T < 1 goes into the loss's terms: of scores at the type's lowest value
+//  the sum may pass fp32's range where the loss does not.)
+//
 //  The gradient needs the row's sum before its first value, and the row's
 //  scores twice: the second time they come from shared memory, so HBM sees them
 //  once (269 MB read of 1,024 x 131,072 bf16; 386 when the second reading went to
@@ -96,8 +99,8 @@ struct Entries {
 };
 
 // From a row's classes and logits in t.c and t.q (-inf for none), W lanes set
-// their probabilities and the row's scale; each lane's part of T sum q log q is
-// returned.  (A lane reads what it wrote, and t.c of all lanes.)
+// their probabilities and the row's scale; each lane's part of T sum q log q, times
+// min(T, 1), is returned.  (A lane reads what it wrote, and t.c of all lanes.)
 template <int W>
 __device__ __forceinline__ float finish_teacher(const DistillArgs& a, int lane, const Teacher& t, float weight) {
     const float c = a.inverse;
@@ -153,7 +156,7 @@ __device__ __forceinline__ float finish_teacher(const DistillArgs& a, int lane, 
     }
     if (lane == 0) *t.scale = most == -INFINITY ? 0.0f : __fmul_rn(a.temperature, weight);
     __syncwarp();
-    return __fmul_rn(a.temperature, entropy);
+    return __fmul_rn(__fmul_rn(a.temperature, fminf(a.temperature, 1.0f)), entropy);
 }
 
 // Fills `t` from a warp's entries; returned as above.
@@ -178,6 +181,7 @@ struct RowScale {
     Origin o;
     float c, log_s;  // log of the sum, in the exponential's units
     float shift;     // T log p = (z - max) - shift: T times the sum's log, of the exact origin
+    float inner;     // min(T, 1)
     float w;         // w T; 0 for a row without gradient
     // Where fp32 holds them well the origin, the sum and the weight go into one
     // addend: w p = +-2^(z c - K).  (|M| <= 64 and a weight above 2^-64 keep |K|
@@ -190,15 +194,16 @@ struct RowScale {
         const float natural = logf(s.s);
         log_s = __fmul_rn(natural, FAST ? kLog2e : 1.0f);
         // (a folded row's sum has the rounding of M)
+        inner = fminf(temperature, 1.0f);
         shift = __fmul_rn(temperature, FAST && !o.far ? fmaf(-kLn2, fmaf(o.m, c, -o.M), natural) : natural);
         w = s.m == -INFINITY ? 0.0f : scale;  // (no class is left, no gradient)
         quick = FAST && fabsf(o.M) <= 64.0f && fabsf(w) > 5.421e-20f;
         K = __fsub_rn(__fadd_rn(o.M, log_s), __log2f(fabsf(w)));
         sign = w < 0.0f ? 0x80008000u : 0u;
     }
-    // T log p of a score; NaN in a row without any score above -inf.  (Without T
-    // the quotient of a finite difference could pass fp32's range.)
-    __device__ __forceinline__ float t_log_p(float z) const { return __fsub_rn(__fsub_rn(z, o.m), shift); }
+    // T log p min(T, 1) of a score; NaN in a row without any score above -inf.
+    // (Without T the quotient of a finite difference could pass fp32's range.)
+    __device__ __forceinline__ float t_log_p(float z) const { return __fmul_rn(inner, __fsub_rn(__fsub_rn(z, o.m), shift)); }
     __device__ __forceinline__ float prob(float z) const {
         const float d = FAST ? o.d(z, c) : __fmul_rn(__fsub_rn(z, o.m), c);
         return expo<FAST>(max_nan(__fsub_rn(d, log_s), -200.0f));
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(kNarrowThreads) distill_narrow_kernel(const Di
             for (int i = lane; i < a.k; i += LPR)
                 if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.t_log_p(t.z[i]), loss);
             loss = reduce_sum<float, LPR>(loss);
-            if (lane == 0 && here) a.loss[row] = __fmul_rn(a.temperature, loss);
+            if (lane == 0 && here) a.loss[row] = __fmul_rn(fmaxf(a.temperature, 1.0f), loss);
             if constexpr (GRAD) {
                 if (here) {
 #pragma unroll
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(32 * kTeams, 5) distill_warp_kernel(const Dist
         for (int i = lane; i < a.k; i += 32)
             if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.t_log_p(t.z[i]), loss);
         loss = reduce_sum<float, 32>(loss);
-        if (lane == 0) a.loss[row] = __fmul_rn(a.temperature, loss);
+        if (lane == 0) a.loss[row] = __fmul_rn(fmaxf(a.temperature, 1.0f), loss);
         if constexpr (GRAD) {
             T* out = dx + row * lddx;
             write_grad<FAST, T, 32>(in, mine_first, steps, count, r, out + p.column(p.v0 + lane),
@@ -503,7 +508,7 @@ __global__ void __launch_bounds__(NT + 32, 768 / NT) distill_wide_kernel(const D
                 for (int i = lane; i < a.k; i += 32)
                     if (t.q[i] != 0.0f) loss = fmaf(-t.q[i], r.t_log_p(t.z[i]), loss);
                 loss = reduce_sum<float, 32>(loss);
-                if (lane == 0) a.loss[row] = __fmul_rn(a.temperature, loss);
+                if (lane == 0) a.loss[row] = __fmul_rn(fmaxf(a.temperature, 1.0f), loss);
             }
             meet();
             if constexpr (GRAD) {
