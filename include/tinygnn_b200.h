@@ -325,7 +325,8 @@ TG_API tg_status tg_label_log_probs_grad(int64_t rows, int64_t classes, int32_t 
  * alone) = weights[i] (nullable: 1) times its gradient.  A class outside
  * [0, classes), and one whose logit is -inf, is none; a row without any has
  * loss and gradient 0.  A class named twice has both its probabilities.  A row
- * of masked scores alone has a NaN for its loss and no gradient. */
+ * of masked scores alone has a NaN for its loss and no gradient.  temperature is
+ * between 1e-30 and 1e30. */
 TG_API tg_status tg_distill_loss(int64_t rows, int64_t classes, int32_t dtype, const void* logits,
                                  int64_t ldz, int64_t k, const void* top_classes, int32_t class_bytes,
                                  int64_t ld_classes, int32_t teacher_dtype, const void* top_logits,

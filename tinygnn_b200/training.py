@@ -231,5 +231,6 @@ def distill_loss(logits: torch.Tensor, top_classes: torch.Tensor, top_logits: to
     ``top`` gives both: log probabilities will do).  A class outside the logits'
     classes, or one with a logit of -inf, is none; a row without any has loss and
     gradient 0; a class that occurs twice has both its probabilities.  A row of
-    masked logits (-inf) alone has a NaN for its loss and no gradient."""
+    masked logits (-inf) alone has a NaN for its loss and no gradient.
+    ``temperature`` is between 1e-30 and 1e30."""
     return _ops.distill_loss(logits, top_classes, top_logits, temperature, weights, grad)
